@@ -218,7 +218,7 @@ def _plan(st):
     head = st["head"].long()
     status = torch.where((need > 0) & (head + end > free.numel()), 2, status)
     ok = status == 0
-    taken = torch.where(ok, end, 0).amax()
+    taken = torch.where(ok & (need > 0), end, 0).amax()
     col = torch.arange(table.shape[1], device=dev)[None, :]
     src = (head + (end - need)[:, None] + col - have[:, None]).clamp(0, free.numel() - 1)
     fresh = ok[:, None] & (col >= have[:, None]) & (col < want[:, None])
