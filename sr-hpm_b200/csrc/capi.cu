@@ -141,6 +141,61 @@ int check_logits(const srhpm_tensor * lg, int min_rows) {
     return SRHPM_OK;
 }
 
+// a paged cache: k / v of one type, [D, page, Hkv, pages], rows contiguous; `mult` divides every stride in bytes
+int check_paged(const srhpm_tensor * k, const srhpm_tensor * v, size_t mult, PagedCache * c) {
+    if (!k || !v) return SRHPM_ERR_INVALID;
+    if (k->type != v->type || (k->type != SRHPM_TYPE_F16 && k->type != SRHPM_TYPE_Q8_0)) return SRHPM_UNSUPPORTED;
+    for (int i = 0; i < 4; i++) {
+        if (k->ne[i] != v->ne[i] || k->ne[i] < 1 || k->ne[i] > INT32_MAX) return SRHPM_ERR_INVALID;
+    }
+    const int64_t D = k->ne[0];
+    if (D != 64 && D != 128 && D != 256) return SRHPM_UNSUPPORTED;
+    if (k->ne[1] * k->ne[3] > INT64_C(1) << 40 || k->ne[2] > 65536) return SRHPM_ERR_INVALID;
+    const size_t rowb = srhpm_row_size(k->type, D);
+    for (const srhpm_tensor * t : { k, v }) {
+        if (!t->data || t->nb[0] != srhpm_type_size(t->type)) return SRHPM_ERR_INVALID;
+        if (!aligned(t->data, mult)) return SRHPM_ERR_ALIGN;
+        for (int i = 1; i < 4; i++) {
+            if (t->ne[i] > 1 && t->nb[i] < rowb) return SRHPM_ERR_INVALID;
+            if (t->nb[i] % mult) return SRHPM_ERR_ALIGN;
+        }
+    }
+    c->type    = k->type;
+    c->D       = (int) D;
+    c->page    = (int) k->ne[1];
+    c->Hkv     = (int) k->ne[2];
+    c->n_pages = k->ne[3];
+    c->k       = (const uint8_t *) k->data;
+    c->knb1    = (int64_t) k->nb[1];
+    c->knb2    = (int64_t) k->nb[2];
+    c->knb3    = (int64_t) k->nb[3];
+    c->v       = (const uint8_t *) v->data;
+    c->vnb1    = (int64_t) v->nb[1];
+    c->vnb2    = (int64_t) v->nb[2];
+    c->vnb3    = (int64_t) v->nb[3];
+    return SRHPM_OK;
+}
+
+// block table i32 [entries, n_seqs], entries contiguous
+int check_table(const srhpm_tensor * t) {
+    if (!t || t->type != SRHPM_TYPE_I32 || !t->data || t->nb[0] != 4) return SRHPM_ERR_INVALID;
+    if (t->ne[0] < 1 || t->ne[0] > INT32_MAX || t->ne[1] < 1 || t->ne[1] > INT32_MAX || t->ne[2] != 1 || t->ne[3] != 1) {
+        return SRHPM_ERR_INVALID;
+    }
+    if (t->nb[1] % 4 || !aligned(t->data, 4)) return SRHPM_ERR_ALIGN;
+    if (t->ne[1] > 1 && t->nb[1] < 4 * (size_t) t->ne[0]) return SRHPM_ERR_INVALID;
+    return SRHPM_OK;
+}
+
+// token rows of heads: f32 or f16 [D, ., .], 16-byte aligned, strides multiples of 16
+int check_rows16(const srhpm_tensor * q, int64_t D) {
+    if (!q || !q->data || q->ne[0] != D || q->ne[3] != 1) return SRHPM_ERR_INVALID;
+    if (q->type != SRHPM_TYPE_F32 && q->type != SRHPM_TYPE_F16) return SRHPM_UNSUPPORTED;
+    if (q->nb[0] != srhpm_type_size(q->type)) return SRHPM_ERR_INVALID;
+    if (q->nb[1] % 16 || q->nb[2] % 16 || !aligned(q->data, 16)) return SRHPM_ERR_ALIGN;
+    return SRHPM_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -600,6 +655,147 @@ int srhpm_swiglu(srhpm_ctx * ctx, const float * gate, const float * up, int64_t 
         return SRHPM_ERR_INVALID;
     }
     return swiglu_run(ctx, gate, up, ld_in, out, ld_out, n, n_ff, (cudaStream_t) stream);
+}
+
+int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_new, int n_seqs, int page_size,
+                    const srhpm_tensor * block_table, const int32_t * free_pages, int n_free, const int32_t * free_head,
+                    int n_rows, int32_t * q_start, int32_t * kv_len, int32_t * pos, int64_t * slots, int32_t * status,
+                    int32_t * n_taken, void * stream) {
+    if (!ctx || !n_past || !n_new || !q_start || !kv_len || !status || !n_taken) return SRHPM_ERR_INVALID;
+    if (n_seqs < 1 || page_size < 1 || n_free < 0 || n_rows < 0) return SRHPM_ERR_INVALID;
+    if ((n_free > 0 && !free_pages) || (n_rows > 0 && (!pos || !slots))) return SRHPM_ERR_INVALID;
+    const int st = check_table(block_table);
+    if (st != SRHPM_OK) return st;
+    if (block_table->ne[1] != n_seqs) return SRHPM_ERR_INVALID;
+    if (!aligned(slots, 8)) return SRHPM_ERR_ALIGN;
+    return page_plan_run(ctx, n_past, n_new, n_seqs, page_size, block_table->data, (int64_t) block_table->nb[1],
+                         (int) block_table->ne[0], free_pages, n_free, free_head, n_rows, q_start, kv_len, pos, slots,
+                         status, n_taken, (cudaStream_t) stream);
+}
+
+int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, int n_head_kv, const int32_t * pos,
+                        const int64_t * slots, float theta_base, const srhpm_tensor * q_out,
+                        const srhpm_tensor * k_cache, const srhpm_tensor * v_cache, void * stream) {
+    if (!ctx || !qkv || !pos || !slots || !q_out || !k_cache || !v_cache) return SRHPM_ERR_INVALID;
+    if (n_head < 1 || n_head > 65536 || n_head_kv < 1 || !(theta_base > 0.0f)) return SRHPM_ERR_INVALID;
+    PagedCache c;
+    int        st = check_paged(k_cache, v_cache, k_cache->type == SRHPM_TYPE_Q8_0 ? 2 : 16, &c);
+    if (st != SRHPM_OK) return st;
+    if (c.Hkv != n_head_kv) return SRHPM_ERR_INVALID;
+    if (qkv->type != SRHPM_TYPE_F32) return SRHPM_UNSUPPORTED;
+    if (!qkv->data || qkv->nb[0] != 4 || qkv->ne[2] != 1 || qkv->ne[3] != 1) return SRHPM_ERR_INVALID;
+    const int64_t width = (int64_t) (n_head + 2 * n_head_kv) * c.D, n = qkv->ne[1];
+    if (qkv->ne[0] != width || n < 1 || n > INT32_MAX || (n > 1 && qkv->nb[1] < (size_t) width * 4)) {
+        return SRHPM_ERR_INVALID;
+    }
+    if (!aligned(qkv->data, 16) || qkv->nb[1] % 16 || !aligned(slots, 8)) return SRHPM_ERR_ALIGN;
+    st = check_rows16(q_out, c.D);
+    if (st != SRHPM_OK) return st;
+    if (q_out->ne[1] != n || q_out->ne[2] != n_head) return SRHPM_ERR_INVALID;
+    return rope_kv_paged_run(ctx, (const uint8_t *) qkv->data, (int64_t) qkv->nb[1], (int) n, n_head, n_head_kv, c.D,
+                             pos, slots, theta_base, q_out, c, (cudaStream_t) stream);
+}
+
+// the shapes that size the work buffer
+static int check_fa_paged(const srhpm_tensor * q, const srhpm_tensor * k, const srhpm_tensor * v, PagedCache * c) {
+    int st = check_paged(k, v, 16, c);
+    if (st != SRHPM_OK) return st;
+    if (c->page % 16 || (c->type == SRHPM_TYPE_Q8_0 && c->D != 256)) return SRHPM_UNSUPPORTED;
+    st = check_rows16(q, c->D);
+    if (st != SRHPM_OK) return st;
+    const int64_t T = q->ne[1], H = q->ne[2];
+    if (T < 1 || T > (1 << 24) || H < 1 || H > 65536 || H % c->Hkv) return SRHPM_ERR_INVALID;
+    return SRHPM_OK;
+}
+
+int srhpm_flash_attn_paged_work_size(const srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_tensor * k_cache,
+                                     int n_seqs, size_t * size) {
+    if (!ctx || !size || !q || n_seqs < 1) return SRHPM_ERR_INVALID;
+    PagedCache c;
+    const int  st = check_fa_paged(q, k_cache, k_cache, &c);
+    if (st != SRHPM_OK) return st;
+    *size = fa_paged_work_size(ctx, (int) q->ne[1], (int) q->ne[2], c.Hkv, c.D, n_seqs);
+    return SRHPM_OK;
+}
+
+int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_tensor * k_cache,
+                           const srhpm_tensor * v_cache, const srhpm_tensor * block_table, const int32_t * q_start,
+                           const int32_t * kv_len, const srhpm_tensor * sinks, float scale, float softcap, int window,
+                           srhpm_tensor * dst, void * wdata, size_t wsize, void * stream) {
+    if (!ctx || !q || !q_start || !kv_len || !dst || window < 0) return SRHPM_ERR_INVALID;
+    if (!(scale > 0.0f) || !(softcap >= 0.0f)) return SRHPM_ERR_INVALID;
+    FaPagedView v;
+    int         st = check_fa_paged(q, k_cache, v_cache, &v.c);
+    if (st != SRHPM_OK) return st;
+    st = check_table(block_table);
+    if (st != SRHPM_OK) return st;
+    st = check_rows16(dst, v.c.D);
+    if (st != SRHPM_OK) return st;
+    if (dst->type != q->type || dst->ne[1] != q->ne[2] || dst->ne[2] != q->ne[1]) return SRHPM_ERR_INVALID;
+    if (sinks && (sinks->type != SRHPM_TYPE_F32 || sinks->ne[0] != q->ne[2] || sinks->nb[0] != 4 || !sinks->data)) {
+        return SRHPM_ERR_INVALID;
+    }
+    v.q       = (const uint8_t *) q->data;
+    v.qnb1    = (int64_t) q->nb[1];
+    v.qnb2    = (int64_t) q->nb[2];
+    v.f32     = q->type == SRHPM_TYPE_F32;
+    v.T       = (int) q->ne[1];
+    v.H       = (int) q->ne[2];
+    v.S       = (int) block_table->ne[1];
+    v.table   = (const uint8_t *) block_table->data;
+    v.tstride = (int64_t) block_table->nb[1];
+    v.cols    = (int) block_table->ne[0];
+    v.q_start = q_start;
+    v.kv_len  = kv_len;
+    v.sinks   = sinks ? (const float *) sinks->data : nullptr;
+    v.scale   = scale;
+    v.softcap = softcap;
+    v.window  = window;
+    v.dst     = (uint8_t *) dst->data;
+    v.dnb1    = (int64_t) dst->nb[1];
+    v.dnb2    = (int64_t) dst->nb[2];
+    return fa_paged_run(ctx, v, wdata, wsize, (cudaStream_t) stream);
+}
+
+int srhpm_verify_sample_work_size(const srhpm_ctx * ctx, const srhpm_tensor * logits, int n_seqs, size_t * size) {
+    if (!ctx || !size || n_seqs < 1) return SRHPM_ERR_INVALID;
+    const int st = check_logits(logits, 1);
+    if (st != SRHPM_OK) return st;
+    if (logits->ne[1] > (1 << 24)) return SRHPM_ERR_INVALID;
+    *size = verify_sample_work_size(ctx, (int) logits->ne[0], (int) logits->ne[1], n_seqs);
+    return SRHPM_OK;
+}
+
+int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start,
+                        int n_seqs, const srhpm_tensor * draft_probs, const float * temperature,
+                        const float * u_accept, const float * u_sample, int32_t * out_ids, int32_t * out_n,
+                        float * p_draft, void * wdata, size_t wsize, void * stream) {
+    if (!ctx || !ids || !q_start || !u_accept || !u_sample || !out_ids || !out_n || n_seqs < 1) return SRHPM_ERR_INVALID;
+    int st = check_logits(logits, 1);
+    if (st != SRHPM_OK) return st;
+    if (logits->ne[1] > (1 << 24)) return SRHPM_ERR_INVALID;
+    if (draft_probs) {
+        st = check_logits(draft_probs, (int) logits->ne[1]);
+        if (st != SRHPM_OK) return st;
+        if (draft_probs->ne[0] != logits->ne[0]) return SRHPM_ERR_INVALID;
+    }
+    SampleView v;
+    v.logits  = (const uint8_t *) logits->data;
+    v.ldb     = (int64_t) logits->nb[1];
+    v.V       = (int) logits->ne[0];
+    v.T       = (int) logits->ne[1];
+    v.S       = n_seqs;
+    v.ids     = ids;
+    v.q_start = q_start;
+    v.dprobs  = draft_probs ? (const uint8_t *) draft_probs->data : nullptr;
+    v.dldb    = draft_probs ? (int64_t) draft_probs->nb[1] : 0;
+    v.temp    = temperature;
+    v.u       = u_accept;
+    v.us      = u_sample;
+    v.out_ids = out_ids;
+    v.out_n   = out_n;
+    v.p_draft = p_draft;
+    return verify_sample_run(ctx, v, wdata, wsize, (cudaStream_t) stream);
 }
 
 }  // extern "C"

@@ -134,4 +134,63 @@ int rope_kv_run(srhpm_ctx * ctx, float * qkv, int64_t ld, int n, int H, int Hkv,
 int swiglu_run(srhpm_ctx * ctx, const float * gate, const float * up, int64_t ld_in, float * out, int64_t ld_out,
                int rows, int64_t cols, cudaStream_t stream);
 
+// a paged KV cache: pages of `page` token slots, byte strides of a token, a KV head and a page
+struct PagedCache {
+    int             type, D, page, Hkv;
+    int64_t         n_pages;
+    const uint8_t * k;
+    int64_t         knb1, knb2, knb3;
+    const uint8_t * v;
+    int64_t         vnb1, vnb2, vnb3;
+};
+
+// paged_ops.cu: the page plan of a step, RoPE with the store into pages
+int page_plan_run(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_new, int S, int page, void * table,
+                  int64_t tstride, int cols, const int32_t * free_pages, int n_free, const int32_t * free_head,
+                  int n_rows, int32_t * q_start, int32_t * kv_len, int32_t * pos, int64_t * slots, int32_t * status,
+                  int32_t * n_taken, cudaStream_t stream);
+int rope_kv_paged_run(srhpm_ctx * ctx, const uint8_t * qkv, int64_t ldb, int n, int H, int Hkv, int D,
+                      const int32_t * pos, const int64_t * slots, float theta_base, const srhpm_tensor * q_out,
+                      const PagedCache & c, cudaStream_t stream);
+
+// fa_paged.cu: attention of the new tokens of a batch over the paged cache
+struct FaPagedView {
+    const uint8_t * q;
+    int64_t         qnb1, qnb2;  // token, head
+    int             f32;         // rows and output f32 (else f16)
+    int             T, H, S;
+    PagedCache      c;
+    const uint8_t * table;
+    int64_t         tstride;
+    int             cols;
+    const int32_t * q_start;
+    const int32_t * kv_len;
+    const float *   sinks;
+    float           scale, softcap;
+    int             window;
+    uint8_t *       dst;
+    int64_t         dnb1, dnb2;  // head, token
+};
+size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S);
+int    fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t wsize, cudaStream_t stream);
+
+// verify_sample.cu: acceptance of drafted tokens by sampling
+struct SampleView {
+    const uint8_t * logits;
+    int64_t         ldb;
+    int             V, T, S;
+    const int32_t * ids;
+    const int32_t * q_start;
+    const uint8_t * dprobs;  // or null
+    int64_t         dldb;
+    const float *   temp;    // or null
+    const float *   u;
+    const float *   us;
+    int32_t *       out_ids;
+    int32_t *       out_n;
+    float *         p_draft;
+};
+size_t verify_sample_work_size(const srhpm_ctx * ctx, int V, int T, int S);
+int    verify_sample_run(srhpm_ctx * ctx, const SampleView & v, void * wdata, size_t wsize, cudaStream_t stream);
+
 }  // namespace srhpm

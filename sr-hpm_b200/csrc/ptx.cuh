@@ -25,6 +25,7 @@ enum : int32_t {
     kErrPeerWait    = 4,
     kErrClusterWait = 5,
     kErrGridWait    = 6,
+    kErrPage        = 7,  // a block table entry that is not a page of the cache
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void * p) {

@@ -10,10 +10,14 @@
                                    patch/srhpm.patch:779-823, with devices as the chunks)
     Context.sample_and_accept_n()  greedy longest-prefix acceptance (reference: common_sampler_sample_and_accept_n,
                                    patch/srhpm.patch:1-37)
+    Context.page_plan / rope_kv_paged / flash_attn_paged / verify_sample
+                                   a batch of sequences over a paged KV cache: the step's tables and slots, the store
+                                   into pages, attention over them, acceptance by sampling (no reference counterpart)
 
 Tensors are torch tensors in device memory; torch only provides allocation and streams. Every compute call goes to
 libsrhpm_b200.so through its C ABI; a missing library raises.
 """
+import collections
 import ctypes
 import warnings
 
@@ -44,6 +48,53 @@ def f32_rows_view(x):
 def _stream_ptr(stream):
     s = stream if stream is not None else torch.cuda.current_stream()
     return ctypes.c_void_p(s.cuda_stream)
+
+
+_I64x4, _SZx4 = ctypes.c_int64 * 4, ctypes.c_size_t * 4
+
+PagePlan = collections.namedtuple("PagePlan", "q_start kv_len pos slots status n_taken")
+
+
+def _view(t, type_, ne, nb):
+    """A ggml view with all four dimensions given."""
+    return ctypes.byref(L.SrhpmTensor(type_, _I64x4(*ne), _SZx4(*nb), t.data_ptr()))
+
+
+def _rows_2d(x, type_, size):
+    """View of a 2-D tensor [rows, cols] with contiguous rows: ne = [cols, rows]."""
+    r, c = x.shape
+    nb = x.stride(0) * size
+    return _view(x, type_, (c, r, 1, 1), (size, nb, nb * r, nb * r))
+
+
+def _head_rows(x, heads_first):
+    """View of token rows [T, H, D] (f32 or f16, any strides of the first two): ne = [D, T, H], or [D, H, T]."""
+    if x.dtype not in (torch.float16, torch.float32) or x.dim() != 3 or x.stride(2) != 1:
+        raise ValueError("rows must be f16 or f32 [T, H, D] with contiguous heads")
+    T, H, D = x.shape
+    e = x.element_size()
+    a, b = x.stride(0) * e, x.stride(1) * e
+    if heads_first:
+        return _view(x, L.F16 if e == 2 else L.F32, (D, H, T, 1), (e, b, a, a * T))
+    return _view(x, L.F16 if e == 2 else L.F32, (D, T, H, 1), (e, a, b, a * T))
+
+
+def _paged(c, kv_type):
+    """View of a paged cache uint8 [pages, page_size, Hkv, row bytes]: ne = [D, page_size, Hkv, pages]."""
+    if c.dtype != torch.uint8 or c.dim() != 4 or c.stride(3) != 1:
+        raise ValueError("a paged cache is uint8 [pages, page_size, Hkv, row bytes] with contiguous rows")
+    n, P, Hkv, rowb = c.shape
+    size, blk = (34, 32) if kv_type == L.Q8_0 else (2, 1)
+    if rowb % size:
+        raise ValueError("row bytes do not hold whole blocks of the cache type")
+    return _view(c, kv_type, (rowb // size * blk, P, Hkv, n), (size, c.stride(1), c.stride(2), c.stride(0)))
+
+
+def _ints(t, dtype, n, what):
+    """Address of a contiguous integer or f32 vector of at least n values."""
+    if t.dtype != dtype or t.dim() != 1 or t.numel() < n or (t.stride(0) != 1 and n > 1):
+        raise ValueError(f"{what} must be a contiguous {dtype} vector of at least {n} values")
+    return t.data_ptr()
 
 
 def quantize_chunk(w, qtype):
@@ -411,6 +462,131 @@ class Context:
                                             ctypes.c_void_p(ids.data_ptr()), ctypes.c_void_p(n.data_ptr()),
                                             _stream_ptr(stream)), "srhpm_accept_merge")
         return ids, n
+
+    # ---- a batch of sequences over a paged KV cache --------------------------------------------------------------
+    # Scratch and new outputs of these calls come from torch's allocator on the call's stream, call by call: calls on
+    # several streams never share a buffer, and a captured graph keeps its own.
+    def _on_device(self, *tensors):
+        for t in tensors:
+            if t is not None and t.device != self.device and t.device != torch.device("cuda", self.device.index or 0):
+                raise ValueError(f"a tensor on {t.device} given to a context of {self.device}")
+
+    def _new(self, shape, dtype, stream):
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=self.device)
+
+    def _call(self, fn, what, *args, stream=None):
+        """One C-ABI call on `stream` (the context's device's current stream by default)."""
+        s = stream if stream is not None else torch.cuda.current_stream(self.device)
+        if torch.cuda.current_device() == (self.device.index or 0):
+            st = fn(self.handle, *args, s.cuda_stream)
+        else:
+            with torch.cuda.device(self.device):
+                st = fn(self.handle, *args, s.cuda_stream)
+        if st != L.OK:
+            raise L.SrhpmError(st, what, self.lib)
+
+    def page_plan(self, n_past, n_new, block_table, free_pages, page_size, n_rows, free_head=None, out=None,
+                  stream=None):
+        """Tables and slots of a step (srhpm_page_plan): n_past, n_new int32 [S]; block_table int32 [S, entries] (new
+        entries are written into it); free_pages int32 [F], taken from free_head (int32 [1], 0 if None). Returns a
+        PagePlan: q_start int32 [S + 1], kv_len int32 [S], pos int32 [n_rows], slots int64 [n_rows], status int32 [S],
+        n_taken int32 [1] (`out`: one to write into)."""
+        S = n_past.numel()
+        self._on_device(n_past, n_new, block_table, free_pages, free_head)
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+            raise ValueError("block_table must be int32 [S, entries] with contiguous rows")
+        if out is None:
+            i32 = self._new(3 * S + 2 + n_rows, torch.int32, stream)
+            out = PagePlan(i32[:S + 1], i32[S + 1:2 * S + 1], i32[3 * S + 2:], self._new(n_rows, torch.int64, stream),
+                           i32[2 * S + 1:3 * S + 1], i32[3 * S + 1:3 * S + 2])
+        else:
+            self._on_device(*out)
+        i32 = torch.int32
+        self._call(self.lib.srhpm_page_plan, "srhpm_page_plan", _ints(n_past, i32, S, "n_past"),
+                   _ints(n_new, i32, S, "n_new"), S, page_size, _rows_2d(block_table, L.I32, 4),
+                   _ints(free_pages, i32, 0, "free_pages"), free_pages.numel(),
+                   None if free_head is None else _ints(free_head, i32, 1, "free_head"), n_rows,
+                   _ints(out.q_start, i32, S + 1, "q_start"), _ints(out.kv_len, i32, S, "kv_len"),
+                   _ints(out.pos, i32, n_rows, "pos"), _ints(out.slots, torch.int64, n_rows, "slots"),
+                   _ints(out.status, i32, S, "status"), _ints(out.n_taken, i32, 1, "n_taken"), stream=stream)
+        return out
+
+    def rope_kv_paged(self, qkv, pos, slots, k_cache, v_cache, kv_type, q_out, theta_base=1e6, stream=None):
+        """RoPE of fused rows qkv f32 [n, (H + 2 Hkv) D] (only read) at pos int32 [n]: turned queries into q_out [n, H,
+        D] (f16 or f32), turned keys and values into the cache rows of slots int64 [n] (srhpm_rope_kv_paged). Caches:
+        uint8 [pages, page_size, Hkv, row bytes]. Returns q_out."""
+        n = qkv.shape[0]
+        self._on_device(qkv, pos, slots, k_cache, v_cache, q_out)
+        if qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
+            raise ValueError("qkv must be f32 [n, width] with contiguous rows")
+        self._call(self.lib.srhpm_rope_kv_paged, "srhpm_rope_kv_paged", _rows_2d(qkv, L.F32, 4), q_out.shape[1],
+                   k_cache.shape[2], _ints(pos, torch.int32, n, "pos"), _ints(slots, torch.int64, n, "slots"),
+                   theta_base, _head_rows(q_out, False), _paged(k_cache, kv_type), _paged(v_cache, kv_type),
+                   stream=stream)
+        return q_out
+
+    def flash_attn_paged(self, q, k_cache, v_cache, kv_type, block_table, q_start, kv_len, scale=1.0, softcap=0.0,
+                         window=0, sinks=None, out=None, stream=None, work=None):
+        """Causal attention of the new rows q [T, H, D] (f16 or f32) of S sequences over their pages
+        (srhpm_flash_attn_paged): block_table int32 [S, entries], q_start int32 [S + 1], kv_len int32 [S] as page_plan
+        gives them; window > 0: only the last `window` positions. Returns out [T, H, D] of q's type (padding rows as
+        they were; of a new tensor: anything)."""
+        S = block_table.shape[0]
+        if out is None:
+            out = self._new(q.shape, q.dtype, stream)
+        self._on_device(q, k_cache, v_cache, block_table, q_start, kv_len, sinks, out, work)
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
+            raise ValueError("block_table must be int32 [S, entries] with contiguous rows")
+        qv, kv = _head_rows(q, False), _paged(k_cache, kv_type)
+        sz = ctypes.c_size_t()
+        L.check(self.lib.srhpm_flash_attn_paged_work_size(self.handle, qv, kv, S, ctypes.byref(sz)),
+                "srhpm_flash_attn_paged_work_size")
+        buf = work if work is not None else self._new(max(sz.value, 16), torch.uint8, stream)
+        sv = None
+        if sinks is not None:
+            _ints(sinks, torch.float32, q.shape[1], "sinks")
+            sv = _view(sinks, L.F32, (sinks.shape[0], 1, 1, 1), (4, 4, 4, 4))
+        self._call(self.lib.srhpm_flash_attn_paged, "srhpm_flash_attn_paged", qv, kv, _paged(v_cache, kv_type),
+                   _rows_2d(block_table, L.I32, 4), _ints(q_start, torch.int32, S + 1, "q_start"),
+                   _ints(kv_len, torch.int32, S, "kv_len"), sv, scale, softcap, window, _head_rows(out, True),
+                   buf.data_ptr(), buf.numel(), stream=stream)
+        return out
+
+    def verify_sample(self, logits, ids, q_start, u_accept, u_sample, draft_probs=None, temperature=None, out=None,
+                      stream=None, work=None):
+        """Acceptance of drafted tokens by sampling (srhpm_verify_sample): logits f32 [T, V] of the step's rows, ids
+        int32 [T] its input tokens (the drafted token of row r is ids[r + 1]), q_start int32 [S + 1], u_accept f32 [T],
+        u_sample f32 [S], draft_probs f32 [T, V] or None (a drafter without distributions), temperature f32 [S] or
+        None. Returns (out_ids int32 [T], out_n int32 [S], p_draft f32 [T]); sequence s emitted
+        out_ids[q_start[s] : q_start[s] + out_n[s]]."""
+        T, S = logits.shape[0], q_start.numel() - 1
+        self._on_device(logits, ids, q_start, u_accept, u_sample, draft_probs, temperature, work)
+        for x in (logits, draft_probs):
+            if x is not None and (x.dtype != torch.float32 or x.dim() != 2 or x.stride(1) != 1):
+                raise ValueError("logits and draft_probs must be f32 [T, V] with contiguous rows")
+        if out is None:
+            out = (self._new(T, torch.int32, stream), self._new(S, torch.int32, stream),
+                   self._new(T, torch.float32, stream))
+        else:
+            self._on_device(*out)
+        i32, f32 = torch.int32, torch.float32
+        lv = _rows_2d(logits, L.F32, 4)
+        sz = ctypes.c_size_t()
+        L.check(self.lib.srhpm_verify_sample_work_size(self.handle, lv, S, ctypes.byref(sz)),
+                "srhpm_verify_sample_work_size")
+        buf = work if work is not None else self._new(max(sz.value, 16), torch.uint8, stream)
+        self._call(self.lib.srhpm_verify_sample, "srhpm_verify_sample", lv, _ints(ids, i32, T, "ids"),
+                   _ints(q_start, i32, S + 1, "q_start"), S,
+                   None if draft_probs is None else _rows_2d(draft_probs, L.F32, 4),
+                   None if temperature is None else _ints(temperature, f32, S, "temperature"),
+                   _ints(u_accept, f32, T, "u_accept"), _ints(u_sample, f32, S, "u_sample"),
+                   _ints(out[0], i32, T, "out_ids"), _ints(out[1], i32, S, "out_n"),
+                   None if out[2] is None else _ints(out[2], f32, T, "p_draft"), buf.data_ptr(), buf.numel(),
+                   stream=stream)
+        return out
 
     def quantize_rows_q8_K(self, X, stream=None):
         X = X.contiguous()
