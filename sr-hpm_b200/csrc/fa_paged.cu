@@ -1,98 +1,1136 @@
-// Attention of a batch's new tokens over a paged KV cache: one CTA per (row, head), a warp per cached token.
+// Attention of a batch's new tokens over a paged KV cache (srhpm_flash_attn_paged), on the 5th-generation tensor cores.
+//
+// The R = G * n rows (G query heads per KV head, n new tokens) that a sequence has for one KV head are packed token by
+// token into tiles of 128: a decode step's few rows and a prompt's thousands take the same path, and K/V is read once
+// for all heads of a group. Per tile of 128 rows and 128 cached tokens:
+//   S = Q K^T      M = 128 rows, N = 128 tokens, f32 in tensor memory (both operands from shared memory)
+//   softmax        one pass with the running maximum m and sum l of each row in registers; the maximum is raised only
+//                  when a tile exceeds it by more than 2^8 (then O is rescaled in place), p = 2^(s - m + 7) <= 2^15 as
+//                  f16 back into S's place in tensor memory: the 2^7 keeps probabilities down to 2^-21 of the row's
+//                  largest out of f16's subnormals
+//   O += P V       A = P from tensor memory, B = V as it lies in shared memory (N = head_dim)
+// f32 rows (PREC): Q and P as sums of two f16 parts (2^-22), two products each. f16 rows: one product each, P rounded to
+// f16 (2^-11 of each probability; the sums l stay f32).
+//
+// Work: an item is (sequence, KV head, row tile); its units are the 128-token tiles that the rows see. All items' units
+// stand in one line that is cut into equal parts, one per CTA (one CTA per SM: any mix of lengths keeps every SM busy to
+// the end, and one long row is spread over the whole GPU). An item cut between CTAs leaves (m, l, O) records, which
+// fa_paged_merge_kernel joins in the order of the cuts (same bits every run). The plan is taken from the lengths on the
+// device by every CTA itself, in its prologue: no planning launch.
+//
+// Roles: 8 softmax warps, 1 MMA warp, 1 producer warp (TMA boxes of at most 64 tokens x 64 dims, each within a page, into
+// a ring of 128-byte-swizzled chunks), and for a q8_0 cache 4 converter warps (raw rows by TMA into a second ring, d * q
+// rounded to f16 into the chunks). NT = 1: the 8 softmax warps halve the columns of one row tile and S has two buffers;
+// NT = 2 (head_dim <= 128): two row tiles share K/V, each with its own 4 softmax warps and buffer.
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "internal.h"
 #include "launch.cuh"
 #include "ptx.cuh"
+#include "tc.cuh"
 
 namespace srhpm {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e   = 1.4426950408889634f;
+constexpr float kLazy    = 8.0f;   // raise the running maximum only beyond 2^8
+constexpr float kShift   = 7.0f;   // p is kept times 2^7
+constexpr int   kBM      = 128;    // rows of a tile
+constexpr int   kBN      = 128;    // tokens of a tile
+constexpr int   kSmWarps = 8;      // softmax warps
+constexpr int   kMaxSeqs = 8192;
+constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s (a probe sleeps up to 4 us)
+constexpr int   kRawTok  = 32;     // tokens of a raw q8_0 slot
+constexpr int   kRawB    = kRawTok * 272;
 
-__device__ __forceinline__ float cache_value(const uint8_t * row, int d, int q8) {
-    if (!q8) return __half2float(reinterpret_cast<const __half *>(row)[d]);
-    const uint8_t * b = row + (d >> 5) * 34;
-    const float     s = __half2float(*reinterpret_cast<const __half *>(b));
-    return __half2float(__float2half_rn(s * (float) (int8_t) b[2 + (d & 31)]));
+struct PArgs {
+    const uint8_t * q;
+    int64_t         qnb1, qnb2;
+    uint8_t *       dst;
+    int64_t         dnb1, dnb2;
+    const uint8_t * table;
+    int64_t         tstride;
+    int             cols, page, n_pages, box;  // box: tokens of a TMA box (divides the page)
+    const int32_t * q_start;
+    const int32_t * kv_len;
+    int             S, T, H, Hkv, G, window;
+    float           qscale;      // scale * log2e, or scale / softcap
+    float           softcap_l2;  // softcap * log2e, 0 = none
+    const float *   sinks;
+    float *         part_acc;    // [2 n_cta][prow][D]
+    float2 *        part_ms;     // [2 n_cta][prow] (max in log2 units, sum * 2^kShift)
+    int4 *          desc;        // [n_cta][2]: parts of the item that a CTA opens and leaves unfinished, and its rows
+    int             prow;        // rows of a record
+    int32_t *       status;
+};
+
+// ---- work items --------------------------------------------------------------------------------------------------
+struct Span {
+    int kt0, nkv;  // first tile, tiles (0: nothing visible)
+    int lo, hi;    // visible tokens of any row
+    int units;     // max(nkv, 1)
+};
+
+// q_start, clamped into the row buffer
+__device__ __forceinline__ int row_at(const PArgs & a, int s) { return min(max(a.q_start[s], 0), a.T); }
+
+template <int BMN> __device__ __forceinline__ Span span_of(const PArgs & a, int n, int kv, int rt) {
+    const int64_t r0 = (int64_t) rt * BMN, r1 = min((int64_t) n * a.G, r0 + BMN);
+    const int     t0 = (int) (r0 / a.G), t1 = (int) ((r1 - 1) / a.G);
+    const int64_t base = (int64_t) kv - n;
+    const int64_t cap  = (int64_t) a.cols * a.page;
+    Span          p;
+    p.hi = (int) max((int64_t) 0, min(base + t1 + 1, min(cap, (int64_t) INT32_MAX - kBN)));
+    p.lo = a.window > 0 ? (int) max((int64_t) 0, base + t0 - a.window + 1) : 0;
+    if (p.hi <= p.lo) {
+        p.kt0 = p.nkv = 0;
+        p.lo = p.hi = 0;
+    } else {
+        p.kt0 = p.lo / kBN;
+        p.nkv = (p.hi + kBN - 1) / kBN - p.kt0;
+    }
+    p.units = max(p.nkv, 1);
+    return p;
+}
+template <int BMN> __device__ __forceinline__ int tiles_of(const PArgs & a, int n) {
+    return (int) (((int64_t) n * a.G + BMN - 1) / BMN);
 }
 
-__global__ void __launch_bounds__(128) fa_paged_kernel(const FaPagedView a, int32_t * status) {
-    const int t = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// a CTA's walk over its part of the line; every role keeps its own
+struct Walk {
+    int     s, h, rt;   // item
+    int     off;        // first unit of the item in this CTA
+    int64_t rem;        // units left in this CTA
+    int     r0, n, kv;  // the sequence's first row, rows and cache length
+    Span    sp;
+    int     take;       // units of the item done here
+};
+
+template <int BMN> __device__ __forceinline__ void walk_load(const PArgs & a, Walk & w) {
+    w.r0 = row_at(a, w.s);
+    w.n  = row_at(a, w.s + 1) - w.r0;
+    w.kv = a.kv_len[w.s];
+}
+template <int BMN> __device__ __forceinline__ void walk_item(const PArgs & a, Walk & w) {
+    w.sp   = span_of<BMN>(a, w.n, w.kv, w.rt);
+    w.take = (int) min((int64_t) (w.sp.units - w.off), w.rem);
+}
+// to the next item; false at the end of the part
+template <int BMN> __device__ __forceinline__ bool walk_next(const PArgs & a, Walk & w) {
+    w.rem -= w.take;
+    if (w.rem <= 0) return false;
+    w.off = 0;
+    if (++w.rt >= tiles_of<BMN>(a, w.n)) {
+        w.rt = 0;
+        if (++w.h >= a.Hkv) {
+            w.h = 0;
+            do {
+                if (++w.s >= a.S) return false;
+                walk_load<BMN>(a, w);
+            } while (w.n <= 0);
+        }
+    }
+    walk_item<BMN>(a, w);
+    return true;
+}
+
+// ring order of the K and V tiles: the order in which the products take them
+// NT = 1: K0 K1 V0 K2 V1 ... V(n-1);  NT = 2: K0 V0 K1 V1 ...
+template <int NT> __device__ __forceinline__ int v_pos(int i, int n) {
+    return NT == 2 ? 2 * i + 1 : (i == n - 1 ? 2 * n - 1 : 2 * i + 2);
+}
+template <int NT> __device__ __forceinline__ int k_pos(int i) { return NT == 2 ? 2 * i : (i == 0 ? 0 : 2 * i - 1); }
+template <int NT> __device__ __forceinline__ void at_pos(int pos, int n, bool & isk, int & i) {
+    if (NT == 2) {
+        isk = (pos & 1) == 0;
+        i   = pos >> 1;
+    } else if (pos == 2 * n - 1) {
+        isk = false;
+        i   = n - 1;
+    } else if (pos == 0 || (pos & 1)) {
+        isk = true;
+        i   = (pos + 1) >> 1;
+    } else {
+        isk = false;
+        i   = (pos >> 1) - 1;
+    }
+}
+
+// ---- shared memory -----------------------------------------------------------------------------------------------
+template <int D, int NT, bool PREC, bool Q8> struct Lay {
+    static constexpr int CH     = D == 256 ? 2 : 1;            // chunks of a K or V tile
+    static constexpr int chunk  = kBN * D * 2 / CH;            // bytes: K 128 tokens x (D / CH) dims, V (128 / CH) tokens x D
+    static constexpr int vtok   = kBN / CH;                    // tokens of a V chunk
+    static constexpr int qtile  = kBM * D * 2;                 // one part (hi or lo) of one row tile
+    static constexpr int qparts = PREC ? 2 : 1;
+    static constexpr int q      = 0;                           // [NT][qparts][qtile]
+    static constexpr int ring   = NT * qparts * qtile;
+    static constexpr int NS     = Q8 ? (PREC ? 2 : 3) : D == 256 ? (PREC ? 3 : 5) : D == 128 ? (PREC && NT == 2 ? 3 : 5) : 6;
+    static constexpr int raw    = ring + NS * chunk;
+    static constexpr int NR     = Q8 ? (PREC ? 3 : 7) : 0;     // raw slots
+    static constexpr int red    = raw + NR * kRawB;            // f32 [2][2][128]
+    static constexpr int bar    = red + 2 * 2 * kBM * 4;
+    static constexpr int nbar   = 2 * NS + 2 * NR + 2 + 2 + 2 + 1;
+    static constexpr int misc   = bar + nbar * 8;
+    static constexpr int total  = misc + 64;
+    static constexpr int alloc  = total;  // dynamic shared memory starts on 1024 bytes (checked by the kernel)
+    static constexpr int threads = (kSmWarps + 2 + (Q8 ? 4 : 0)) * 32;
+    static_assert(alloc <= 232448, "shared memory");
+    static_assert(NS * chunk >= kMaxSeqs * 8, "the plan's sums fit the ring");
+};
+
+__device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap * m, int x, int y, int z, int w, uint64_t * bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// A from tensor memory (K-major f16 pairs, lane = row)
+__device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u)
+        : "memory");
+}
+
+__device__ __forceinline__ void ld32(uint32_t t, uint32_t * r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(t));
+}
+__device__ __forceinline__ void st32(uint32_t t, const uint32_t * r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// a wait that ran out marks the kernel's status; the thread then waits for nothing more (its results are void, its
+// accesses stay in bounds) so that every role comes to its end
+__device__ __forceinline__ void wait_bar(uint64_t * bar, uint32_t parity, int32_t * status, bool & bad) {
+    if (bad) return;
+    for (uint32_t i = 0; i < kProbes; i++) {
+        if (mbar_try_wait(bar, parity)) return;
+    }
+    bad = true;
+    atomicExch(status, kErrWaitFull);
+}
+
+// 64 q8_0 values (two blocks, 68 bytes from byte 68 qr of a row) to f16 = round(d * q): 8 words of 16 bytes, chunk c of
+// the token's 128-byte row at the swizzled place
+__device__ __forceinline__ void convert_q8(const uint8_t * row, int qr, uint8_t * dst_row, int t, bool zero) {
+    uint32_t w[20];
+    const uint4 * src = reinterpret_cast<const uint4 *>(row + 64 * qr);
+#pragma unroll
+    for (int c = 0; c < 5; c++) {
+        const uint4 u = src[c];
+        w[4 * c] = u.x; w[4 * c + 1] = u.y; w[4 * c + 2] = u.z; w[4 * c + 3] = u.w;
+    }
+    // the quarter starts qr words into the 80 bytes
+    uint32_t v[17];
+#pragma unroll
+    for (int i = 0; i < 17; i++) {
+        v[i] = qr == 0 ? w[i] : qr == 1 ? w[i + 1] : qr == 2 ? w[i + 2] : w[i + 3];
+    }
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480u), __ushort_as_half(0x6480u));  // 1024 + 128
+#pragma unroll
+    for (int bb = 0; bb < 2; bb++) {
+        const int      od    = 34 * bb;
+        const uint32_t dbits = (v[od >> 2] >> (8 * (od & 3))) & 0xffffu;
+        const __half2  dd    = __halves2half2(__ushort_as_half((unsigned short) dbits), __ushort_as_half((unsigned short) dbits));
+        uint32_t       f[16];
+#pragma unroll
+        for (int m = 0; m < 16; m++) {
+            const int      o  = od + 2 + 2 * m;  // even: the pair sits in one word
+            const uint32_t wx = v[o >> 2] ^ 0x80808080u;
+            uint32_t       mg;
+            asm("prmt.b32 %0, %1, %2, %3;" : "=r"(mg) : "r"(wx), "r"(0x64u), "r"(((o >> 1) & 1) ? 0x4342u : 0x4140u));
+            __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&mg), bias);  // exact: |q| <= 128
+            h         = __hmul2(h, dd);
+            f[m]      = zero ? 0u : *reinterpret_cast<const uint32_t *>(&h);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            *reinterpret_cast<uint4 *>(dst_row + (((4 * bb + c) ^ (t & 7)) << 4)) =
+                make_uint4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
+        }
+    }
+}
+
+template <int D, int NT, bool PREC, bool Q8>
+__global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
+    fa_paged_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                    const __grid_constant__ PArgs a) {
+    using Ly           = Lay<D, NT, PREC, Q8>;
+    constexpr int BMN  = kBM * NT;
+    constexpr int CH   = Ly::CH;
+    constexpr int NS   = Ly::NS;
+    constexpr int NC   = NT == 2 ? 128 : 64;  // score columns per softmax thread
+    constexpr int OC   = NT == 2 ? D : D / 2; // output columns per softmax thread
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint64_t * kvfull  = reinterpret_cast<uint64_t *>(sm + Ly::bar);
+    uint64_t * kvempty = kvfull + NS;
+    uint64_t * rfull   = kvempty + NS;
+    uint64_t * rempty  = rfull + Ly::NR;
+    uint64_t * s_full  = rempty + Ly::NR;  // [2]
+    uint64_t * p_rdy   = s_full + 2;       // [2]
+    uint64_t * pv_done = p_rdy + 2;        // [2] per row tile (NT = 2) or in turn
+    uint64_t * q_full  = pv_done + 2;
+    uint32_t * tptr    = reinterpret_cast<uint32_t *>(sm + Ly::misc);
+    int *      first   = reinterpret_cast<int *>(sm + Ly::misc + 8);       // s, h, rt, off of the part's first unit
+    int64_t *  range   = reinterpret_cast<int64_t *>(sm + Ly::misc + 24);  // part start, end, units in all, parts
+    float *    red     = reinterpret_cast<float *>(sm + Ly::red);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    bool      bad = false;
+    if (smem_u32(sm) & 1023u) {  // the swizzled operands need it; the linker places the only shared array so
+        if (tid == 0) atomicExch(a.status, kErrWaitFull);
+        pdl_wait();
+        return;
+    }
+
+    if (tid == 0) {
+        for (int i = 0; i < NS; i++) {
+            mbar_init(&kvfull[i], Q8 ? 4 : 1);
+            mbar_init(&kvempty[i], 1);
+        }
+        for (int i = 0; i < Ly::NR; i++) {
+            mbar_init(&rfull[i], 1);
+            mbar_init(&rempty[i], 4);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_rdy[i], NT == 2 ? 4 : 8);
+            mbar_init(&pv_done[i], 1);
+        }
+        mbar_init(q_full, kSmWarps);
+        fence_mbar_init();
+        first[0] = -1;
+    }
+    if (warp == kSmWarps) tc::tmem_alloc(tptr, 512);
+    if (warp == kSmWarps + 1 && lane == 0) {
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+    }
     pdl_launch_dependents();
     pdl_wait();
-    if (t >= a.q_start[a.S]) return;
-    int lo = 0, hi = a.S;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.q_start[mid] <= t) {
-            lo = mid;
-        } else {
-            hi = mid;
+
+    // ---------------- plan: this CTA's part of the line of units ----------------
+    {
+        int * tot = reinterpret_cast<int *>(sm + Ly::ring);  // units per KV head of each sequence
+        int * big = tot + a.S;                               // sequences whose tiles a warp sums up
+        int * nbg = reinterpret_cast<int *>(sm + Ly::red);
+        if (tid == 0) *nbg = 0;
+        __syncthreads();
+        for (int s = tid; s < a.S; s += blockDim.x) {
+            const int r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = n > 0 ? tiles_of<BMN>(a, n) : 0;
+            int       u = 0;
+            if (nt <= 2) {
+                const int kv = nt ? a.kv_len[s] : 0;
+                for (int rt = 0; rt < nt; rt++) u += span_of<BMN>(a, n, kv, rt).units;
+            } else {
+                big[atomicAdd(nbg, 1)] = s;  // any order: each entry is worked out by itself
+            }
+            tot[s] = u;
+        }
+        __syncthreads();
+        for (int b = warp; b < *nbg; b += blockDim.x / 32) {
+            const int s = big[b], r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = a.kv_len[s];
+            int       u = 0;
+            for (int rt = lane; rt < nt; rt += 32) u += span_of<BMN>(a, n, kv, rt).units;
+            u = __reduce_add_sync(0xffffffffu, u);
+            if (lane == 0) tot[s] = u;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int64_t sum = 0;
+            for (int s = lane; s < a.S; s += 32) sum += tot[s];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            // fewer units than CTAs: one each for the first W, so that an item's parts stand in neighbouring CTAs
+            const int64_t W = sum * a.Hkv, np = max((int64_t) 1, min((int64_t) gridDim.x, W)), c = min((int64_t) blockIdx.x, np);
+            const int64_t b0 = W * c / np, b1 = W * min(c + 1, np) / np;
+            if (lane == 0) {
+                range[0] = b0;
+                range[1] = b1;
+                range[2] = W;
+                range[3] = np;
+            }
+            if (b1 > b0) {
+                int64_t before = 0;
+                for (int s0 = 0; s0 < a.S; s0 += 32) {
+                    const int64_t v   = s0 + lane < a.S ? (int64_t) tot[s0 + lane] * a.Hkv : 0;
+                    int64_t       inc = v;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+                        if (lane >= o) inc += x;
+                    }
+                    const int64_t  end = before + inc, beg = end - v;
+                    const uint32_t hit = __ballot_sync(0xffffffffu, b0 >= beg && b0 < end);
+                    if (hit) {
+                        const int     src = __ffs(hit) - 1, s = s0 + src;
+                        const int64_t in  = b0 - __shfl_sync(0xffffffffu, beg, src);
+                        const int     per = tot[s];
+                        const int     h   = (int) (in / per);
+                        int           off = (int) (in - (int64_t) h * per);
+                        const int     r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = a.kv_len[s];
+                        for (int t0 = 0; t0 < nt; t0 += 32) {
+                            const int u  = t0 + lane < nt ? span_of<BMN>(a, n, kv, t0 + lane).units : 0;
+                            int       ic = u;
+#pragma unroll
+                            for (int o = 1; o < 32; o <<= 1) {
+                                const int x = __shfl_up_sync(0xffffffffu, ic, o);
+                                if (lane >= o) ic += x;
+                            }
+                            const uint32_t ht = __ballot_sync(0xffffffffu, off >= ic - u && off < ic);
+                            if (ht) {
+                                const int l = __ffs(ht) - 1;
+                                off -= __shfl_sync(0xffffffffu, ic - u, l);
+                                if (lane == 0) {
+                                    first[0] = s;
+                                    first[1] = h;
+                                    first[2] = t0 + l;
+                                    first[3] = off;
+                                }
+                                break;
+                            }
+                            off -= __shfl_sync(0xffffffffu, ic, 31);
+                        }
+                        break;
+                    }
+                    before = __shfl_sync(0xffffffffu, end, 31);
+                }
+            }
         }
     }
-    const int D = a.c.D, e = D / 32, q8 = a.c.type == SRHPM_TYPE_Q8_0, g = h / (a.H / a.c.Hkv);
-    const int n = a.q_start[lo + 1] - a.q_start[lo], p = a.kv_len[lo] - n + t - a.q_start[lo];
-    float     q[8];
-    for (int i = 0; i < e; i++) {
-        const uint8_t * src = a.q + (int64_t) t * a.qnb1 + (int64_t) h * a.qnb2;
-        q[i] = a.f32 ? reinterpret_cast<const float *>(src)[i * 32 + lane]
-                     : __half2float(reinterpret_cast<const __half *>(src)[i * 32 + lane]);
-    }
-    float     m = -INFINITY, l = 0.0f, acc[8] = {};
-    const int first = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    const int end   = (int) min((int64_t) p + 1, (int64_t) a.cols * a.c.page);
-    for (int j = first + warp; j < end; j += 4) {
-        const int page = reinterpret_cast<const int32_t *>(a.table + (int64_t) lo * a.tstride)[j / a.c.page];
-        const bool ok  = page >= 0 && page < a.c.n_pages;
-        if (!ok && lane == 0) atomicExch(status, kErrPage);
-        const uint8_t * kr = a.c.k + (int64_t) page * a.c.knb3 + (int64_t) (j % a.c.page) * a.c.knb1 + (int64_t) g * a.c.knb2;
-        const uint8_t * vr = a.c.v + (int64_t) page * a.c.vnb3 + (int64_t) (j % a.c.page) * a.c.vnb1 + (int64_t) g * a.c.vnb2;
-        float           s  = 0.0f;
-        for (int i = 0; i < e; i++) s = fmaf(q[i], ok ? cache_value(kr, i * 32 + lane, q8) : 0.0f, s);
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s *= a.scale;
-        if (a.softcap != 0.0f) s = a.softcap * tanhf(s / a.softcap);
-        const float mn = fmaxf(m, s), al = expf(m - mn), w = expf(s - mn);
-        l = l * al + w;
-        for (int i = 0; i < e; i++) acc[i] = acc[i] * al + w * (ok ? cache_value(vr, i * 32 + lane, q8) : 0.0f);
-        m = mn;
-    }
-    __shared__ float sm[4], sl[4], sa[4][256];
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
-    }
-    for (int i = 0; i < e; i++) sa[warp][i * 32 + lane] = acc[i];
+    tc::fence_before();
     __syncthreads();
-    const float sink = a.sinks ? a.sinks[h] : -INFINITY;
-    const float M    = fmaxf(fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), sink);
-    float       L    = M > -INFINITY ? expf(sink - M) : 0.0f;
-    for (int w = 0; w < 4; w++) L += sl[w] > 0.0f ? sl[w] * expf(sm[w] - M) : 0.0f;
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float o = 0.0f;
-        for (int w = 0; w < 4; w++) o += sl[w] > 0.0f ? sa[w][d] * expf(sm[w] - M) : 0.0f;
-        o             = L > 0.0f ? o / L : 0.0f;
-        uint8_t * dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) t * a.dnb2;
-        if (a.f32) {
-            reinterpret_cast<float *>(dst)[d] = o;
-        } else {
-            reinterpret_cast<__half *>(dst)[d] = __float2half_rn(o);
+    tc::fence_after();
+    const uint32_t tbase = *tptr;
+    const uint32_t tO    = tbase;        // row tile q: columns q * D
+    const uint32_t tS    = tbase + 256;  // buffer b: columns 256 + 128 b
+    if (tid == 0) a.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+
+    Walk w;
+    w.s         = first[0];
+    bool active = w.s >= 0;
+    if (active) {
+        w.h   = first[1];
+        w.rt  = first[2];
+        w.off = first[3];
+        w.rem = range[1] - range[0];
+        walk_load<BMN>(a, w);
+        walk_item<BMN>(a, w);
+    }
+
+    if (warp == kSmWarps + 1) {
+        // ---------------- producer ----------------
+        uint32_t  rc = 0;                 // chunks (q8_0: raw slots) so far
+        const int box = a.box;            // q8_0: at most kRawTok
+        const int nsub = kBN / box;       // boxes per 128 tokens: 2, 4 or 8
+        for (; active; active = walk_next<BMN>(a, w)) {
+            const int n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
+            const int32_t * row = reinterpret_cast<const int32_t *>(a.table + (int64_t) w.s * a.tstride);
+            // lane j: page and place of the tile's j-th box, -1 when no row sees it
+            auto entry = [&](int pos, int & in) -> int {
+                bool isk;
+                int  i;
+                at_pos<NT>(pos, n, isk, i);
+                const int tok = (kt + i) * kBN + lane * box;
+                in            = tok % a.page;
+                if (lane >= nsub || tok >= w.sp.hi || tok + box <= w.sp.lo) return -1;
+                const int pg = row[tok / a.page];
+                return pg < 0 || pg >= a.n_pages ? a.n_pages : pg;  // no page: outside the map, reads as zeros
+            };
+            int in_next = 0, e_next = n ? entry(0, in_next) : -1;
+            for (int pos = 0; pos < 2 * n; pos++) {
+                bool isk;
+                int  i;
+                at_pos<NT>(pos, n, isk, i);
+                const int e = e_next, in = in_next;
+                if (pos + 1 < 2 * n) e_next = entry(pos + 1, in_next);  // in flight during this tile's waits
+                if (e == a.n_pages) atomicExch(a.status, kErrPage);
+                const CUtensorMap * m = isk ? &mk : &mv;
+                if constexpr (Q8) {
+                    constexpr int NRAW = kBN / kRawTok;
+                    const int     per  = kRawTok / box;  // boxes per raw slot: 1 or 2
+#pragma unroll 1
+                    for (int r = 0; r < NRAW; r++, rc++) {
+                        const int slot = rc % Ly::NR;
+                        if (rc >= Ly::NR) wait_bar(&rempty[slot], (rc / Ly::NR - 1) & 1, a.status, bad);
+                        if (bad) break;
+                        const int      sub  = r * per + lane;
+                        const int      ee   = __shfl_sync(0xffffffffu, e, sub & 31);
+                        const int      ii   = __shfl_sync(0xffffffffu, in, sub & 31);
+                        const bool     go   = lane < per && ee >= 0;
+                        const uint32_t many = __popc(__ballot_sync(0xffffffffu, go));
+                        if (lane == 0) mbar_arrive_expect_tx(&rfull[slot], many * box * 272);
+                        __syncwarp();
+                        if (go) {
+                            tma4(smem_u32(sm + Ly::raw + slot * kRawB) + lane * box * 272, m, 0, ii, w.h, ee, &rfull[slot]);
+                        }
+                    }
+                } else {
+#pragma unroll 1
+                    for (int ch = 0; ch < CH; ch++, rc++) {
+                        const int slot = rc % NS;
+                        if (rc >= NS) wait_bar(&kvempty[slot], (rc / NS - 1) & 1, a.status, bad);
+                        if (bad) break;
+                        // boxes of the chunk: K all tokens and D / CH dims, V tokens 128 / CH and all dims
+                        const int  planes = isk ? D / 64 / CH : D / 64;
+                        const int  ns     = isk ? nsub : nsub / CH;
+                        const int  sub0   = isk ? 0 : ch * ns;
+                        const int  p0     = isk ? ch * planes : 0;
+                        const int  rows   = isk ? kBN : Ly::vtok;
+                        const int  sub = lane % ns, pl = lane / ns;  // at most 4 planes x 8 boxes
+                        const int  ee  = __shfl_sync(0xffffffffu, e, sub0 + sub);
+                        const int  ii  = __shfl_sync(0xffffffffu, in, sub0 + sub);
+                        const bool go  = pl < planes && ee >= 0;
+                        const uint32_t many = __popc(__ballot_sync(0xffffffffu, go));
+                        if (lane == 0) mbar_arrive_expect_tx(&kvfull[slot], many * box * 128);
+                        __syncwarp();
+                        if (go) {
+                            tma4(smem_u32(sm + Ly::ring + slot * Ly::chunk) + pl * rows * 128 + sub * box * 128, m,
+                                 (p0 + pl) * 64, ii, w.h, ee, &kvfull[slot]);
+                        }
+                    }
+                }
+            }
+        }
+        if (bad) {  // the loads in flight land before this CTA's shared memory goes
+            constexpr int ND = Q8 ? Ly::NR : NS;
+            for (uint32_t c = rc > ND ? rc - ND : 0; c < rc; c++) mbar_wait(&(Q8 ? rfull : kvfull)[c % ND], (c / ND) & 1);
+        }
+    } else if (warp == kSmWarps) {
+        // ---------------- MMA ----------------
+        if (lane == 0) {
+            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, kBN, kBM);
+            constexpr uint32_t idpv = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kMNMajor, D, kBM);
+            constexpr uint64_t sw   = 2ull << 61;
+            const uint32_t     qs   = smem_u32(sm + Ly::q), rs = smem_u32(sm + Ly::ring);
+            uint32_t           rc0 = 0, items = 0, pc[2] = { 0, 0 }, pvn = 0;
+            for (; active; active = walk_next<BMN>(a, w)) {
+                const int n = w.sp.nkv ? w.take : 0;
+                if (n == 0) continue;
+                const int  nq  = NT == 2 && (int64_t) w.n * a.G - (int64_t) w.rt * BMN > kBM ? 2 : 1;
+                wait_bar(q_full, items & 1, a.status, bad);
+                items++;
+                tc::fence_after();
+                auto qk = [&](int i, int q, bool last) {  // last: the tile's last product with this K
+                    const int      b = NT == 2 ? q : (i & 1);
+                    const uint32_t d = tS + 128 * b;
+#pragma unroll
+                    for (int ch = 0; ch < CH; ch++) {
+                        const uint32_t c = rc0 + k_pos<NT>(i) * CH + ch, slot = c % NS;
+                        wait_bar(&kvfull[slot], (c / NS) & 1, a.status, bad);
+                        tc::fence_after();
+                        const uint32_t kb = rs + slot * Ly::chunk;
+#pragma unroll
+                        for (int j = 0; j < D / CH / 16; j++) {
+                            const int      jj = ch * (D / CH / 16) + j;  // k-step over all dims
+                            const uint64_t bd = tc::sdesc(kb + (j >> 2) * (kBN * 128) + (j & 3) * 32, 16, 1024) | sw;
+#pragma unroll
+                            for (int part = 0; part < Ly::qparts; part++) {
+                                const uint32_t qa = qs + (q * Ly::qparts + part) * Ly::qtile + (jj >> 2) * (kBM * 128) + (jj & 3) * 32;
+                                tc::mma_f16(d, tc::sdesc(qa, 16, 1024) | sw, bd, idqk, (uint32_t) (jj > 0 || part > 0));
+                            }
+                        }
+                        if (last) tc::commit(&kvempty[slot]);
+                    }
+                    tc::commit(&s_full[b]);
+                };
+                auto pv = [&](int i, int q, bool last) {
+                    const int      b = NT == 2 ? q : (i & 1);
+                    const uint32_t p = tS + 128 * b, d = tO + q * D;
+                    wait_bar(&p_rdy[b], pc[b] & 1, a.status, bad);
+                    pc[b]++;
+#pragma unroll
+                    for (int ch = 0; ch < CH; ch++) {
+                        const uint32_t c = rc0 + v_pos<NT>(i, n) * CH + ch, slot = c % NS;
+                        wait_bar(&kvfull[slot], (c / NS) & 1, a.status, bad);
+                        tc::fence_after();
+                        const uint32_t vb = rs + slot * Ly::chunk;
+#pragma unroll
+                        for (int j = 0; j < Ly::vtok / 16; j++) {
+                            const int      jj = ch * (Ly::vtok / 16) + j;
+                            const uint64_t bd = tc::sdesc(vb + j * 2048, Ly::vtok * 128, 1024) | sw;
+#pragma unroll
+                            for (int part = 0; part < Ly::qparts; part++) {
+                                mma_f16_ta(d, p + part * 64 + jj * 8, bd, idpv, (uint32_t) (i > 0 || jj > 0 || part > 0));
+                            }
+                        }
+                        if (last) tc::commit(&kvempty[slot]);
+                    }
+                    tc::commit(&pv_done[NT == 2 ? q : (pvn++ & 1)]);
+                };
+                if constexpr (NT == 1) {
+                    qk(0, 0, true);
+                    for (int i = 0; i < n; i++) {
+                        if (i + 1 < n) qk(i + 1, 0, true);
+                        pv(i, 0, true);
+                    }
+                } else {
+                    for (int q = 0; q < nq; q++) qk(0, q, q == nq - 1);
+                    for (int i = 0; i < n; i++) {
+                        for (int q = 0; q < nq; q++) {
+                            pv(i, q, q == nq - 1);
+                            if (i + 1 < n) qk(i + 1, q, q == nq - 1);
+                        }
+                    }
+                }
+                rc0 += 2 * n * CH;
+            }
+        }
+        __syncwarp();
+    } else if (warp < kSmWarps) {
+        // ---------------- softmax ----------------
+        const int wg = warp >> 2, wq = warp & 3, row = 32 * wq + lane;  // row of the tile (tensor-memory lane)
+        const int q    = NT == 2 ? wg : 0;                              // row tile
+        const int c0   = NT == 2 ? 0 : 64 * wg;                         // first score column of this thread
+        uint32_t  rc0 = 0, sc[2] = { 0, 0 }, pvc = 0, pvw = 0, turn = 0, items = 0;
+        for (; active; active = walk_next<BMN>(a, w)) {
+            const int     n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
+            const int64_t R  = (int64_t) w.n * a.G;
+            const int64_t rb = (int64_t) w.rt * BMN + q * kBM;      // first row of this tile
+            const int     rows = (int) max((int64_t) 0, min((int64_t) kBM, R - rb));
+            const bool    mine = row < rows;                        // this thread's row exists
+            const bool    some = 32 * wq < rows;                    // the warp has a row
+            // Q rows to shared memory: 16-byte chunks of 8 dims, 128-byte swizzle
+            if (n > 0) {
+                constexpr int per = D / 8;
+                const int     u0 = NT == 2 ? (tid & 127) : tid;
+#pragma unroll 4
+                for (int u = u0; u < kBM * per; u += NT == 2 ? 128 : 256) {
+                    const int r = u / per, c = u % per;
+                    uint4     hi = make_uint4(0, 0, 0, 0), lo = hi;
+                    if (r < rows) {
+                        const int64_t   rr  = rb + r;
+                        const int64_t   t   = w.r0 + rr / a.G;
+                        const int       h   = w.h * a.G + (int) (rr % a.G);
+                        const uint8_t * src = a.q + t * a.qnb1 + (int64_t) h * a.qnb2;
+                        if constexpr (PREC) {
+                            const float4 x0 = __ldg(reinterpret_cast<const float4 *>(src) + 2 * c);
+                            const float4 x1 = __ldg(reinterpret_cast<const float4 *>(src) + 2 * c + 1);
+                            const float  x[8] = { x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w };
+                            uint32_t     hw[4], lw[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const __half2 h2 = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+                                const __half2 l2 = __floats2half2_rn(x[2 * e] - __low2float(h2), x[2 * e + 1] - __high2float(h2));
+                                hw[e] = *reinterpret_cast<const uint32_t *>(&h2);
+                                lw[e] = *reinterpret_cast<const uint32_t *>(&l2);
+                            }
+                            hi = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                            lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                        } else {
+                            hi = __ldg(reinterpret_cast<const uint4 *>(src) + c);
+                        }
+                    }
+                    uint8_t * d = sm + Ly::q + q * Ly::qparts * Ly::qtile + (c >> 3) * (kBM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(d) = hi;
+                    if constexpr (PREC) *reinterpret_cast<uint4 *>(d + Ly::qtile) = lo;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
+            }
+            // the row's visible tokens
+            const int pos = (int) ((int64_t) w.kv - w.n + (mine ? (rb + row) / a.G : 0));
+            const int vhi = mine ? min(pos + 1, w.sp.hi) : 0;
+            const int vlo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+            // tokens that every row of the tile sees: no masking there
+            const int pmin = (int) ((int64_t) w.kv - w.n + rb / a.G);
+            const int pmax = (int) ((int64_t) w.kv - w.n + (rb + max(rows, 1) - 1) / a.G);
+            const int ahi = min(pmin + 1, w.sp.hi), alo = a.window > 0 ? max(0, pmax - a.window + 1) : 0;
+            float     m = -INFINITY, l = 0.0f;
+            const bool run = NT == 1 || q == 0 || rows > 0;  // this warp group has units
+            // waits until this row tile's first `upto` products P V are done, phase by phase: a parity wait must neither
+            // skip a phase nor come after the next one. NT = 1 asks late (two products may end before a slow warp
+            // looks), so its products take two barriers in turn, each of which waits for this warp's next P
+            auto pv_wait = [&](uint32_t upto) {
+                for (; pvw < upto; pvw++) {
+                    if constexpr (NT == 2) {
+                        wait_bar(&pv_done[q], pvw & 1, a.status, bad);
+                    } else {
+                        wait_bar(&pv_done[pvw & 1], (pvw >> 1) & 1, a.status, bad);
+                    }
+                }
+            };
+            if (n > 0) {
+                // a group without units must not arrive for a later item before the other has arrived for this one
+                if (!run) wait_bar(q_full, items & 1, a.status, bad);
+                items++;
+            }
+            for (int i = 0; run && i < n; i++) {
+                const int b = NT == 2 ? q : (i & 1), t0 = (kt + i) * kBN;
+                wait_bar(&s_full[b], sc[b] & 1, a.status, bad);
+                sc[b]++;
+                // done: these products were issued before this tile's scores
+                if constexpr (NT == 2) {
+                    pv_wait(pvc);
+                } else if (pvc > 0) {
+                    pv_wait(pvc - 1);
+                }
+                tc::fence_after();
+                const uint32_t tb = tc::taddr(tS + 128 * b, wq, 0);
+                float          s[NC];
+                float          mt = -INFINITY;
+                if (some) {
+#pragma unroll
+                    for (int c = 0; c < NC; c += 32) ld32(tb + c0 + c, reinterpret_cast<uint32_t *>(s) + c);
+                    tc::wait_ld();
+                    if (a.softcap_l2 != 0.0f) {
+#pragma unroll
+                        for (int c = 0; c < NC; c++) s[c] = a.softcap_l2 * tanhf(s[c] * a.qscale);
+                    }
+                    if (t0 < alo || t0 + kBN > ahi) {
+                        const int l0 = vlo - t0 - c0, h0 = vhi - t0 - c0;
+#pragma unroll
+                        for (int c = 0; c < NC; c++) s[c] = c >= l0 && c < h0 ? s[c] : -INFINITY;
+                    }
+                    float mx[4] = { s[0], s[1], s[2], s[3] };
+#pragma unroll
+                    for (int c = 4; c < NC; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+                    mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                }
+                if constexpr (NT == 1) {  // the other half of the row; both halves have read S before either writes P
+                    float * rd = red + (turn & 1) * 2 * kBM;
+                    turn++;
+                    rd[wg * kBM + row] = mt;
+                    named_bar_sync(1 + wq, 64);
+                    mt = fmaxf(mt, rd[(wg ^ 1) * kBM + row]);
+                }
+                if (some) {
+                    const float qs = a.softcap_l2 != 0.0f ? 1.0f : a.qscale;
+                    mt *= qs;  // log2 units (qs > 0)
+                    const bool up = mt > m + kLazy;
+                    if (__any_sync(0xffffffffu, up)) {
+                        const float mn = up ? mt : m, f = up ? ex2(m - mn) : 1.0f;
+                        if (i > 0) {
+                            l *= f;
+                            pv_wait(pvc);
+                            tc::fence_after();
+                            const uint32_t to = tc::taddr(tO + q * D, wq, NT == 2 ? 0 : OC * wg);
+#pragma unroll 1
+                            for (int c = 0; c < OC; c += 32) {
+                                uint32_t o[32];
+                                ld32(to + c, o);
+                                tc::wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                st32(to + c, o);
+                            }
+                        }
+                        m = mn;
+                    }
+                    const float off = (m == -INFINITY ? 0.0f : m) - kShift;
+                    const f2    q2 = f2_pack(qs, qs), o2 = f2_pack(-off, -off);
+                    f2          l2[2] = { 0ull, 0ull };
+#pragma unroll
+                    for (int c = 0; c < NC; c += 64) {
+                        uint32_t hi[32], lo[32];
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            float x0, x1;
+                            f2_unpack(f2_fma(f2_pack(s[c + 2 * e], s[c + 2 * e + 1]), q2, o2), x0, x1);
+                            x0 = ex2(x0);
+                            x1 = ex2(x1);
+                            l2[e & 1] = f2_add(l2[e & 1], f2_pack(x0, x1));
+                            const __half2 h2 = __floats2half2_rn(x0, x1);
+                            hi[e]            = *reinterpret_cast<const uint32_t *>(&h2);
+                            if constexpr (PREC) {
+                                const __half2 r2 = __floats2half2_rn(x0 - __low2float(h2), x1 - __high2float(h2));
+                                lo[e]            = *reinterpret_cast<const uint32_t *>(&r2);
+                            }
+                        }
+                        st32(tb + (c0 + c) / 2, hi);
+                        if constexpr (PREC) st32(tb + 64 + (c0 + c) / 2, lo);
+                    }
+                    float y0, y1;
+                    f2_unpack(f2_add(l2[0], l2[1]), y0, y1);
+                    l += y0 + y1;
+                    tc::wait_st();
+                }
+                pvc++;
+                if constexpr (!Q8) {
+                    // V rows that no row of the item sees hold anything; 0 * NaN is NaN, so they become zeros
+                    if ((NT == 1 || q == 0) && (t0 < w.sp.lo || t0 + kBN > w.sp.hi)) {
+                        const int z0 = max(0, w.sp.lo - t0), z1 = min(kBN, w.sp.hi - t0);  // kept rows
+#pragma unroll
+                        for (int ch = 0; ch < CH; ch++) {
+                            const uint32_t c = rc0 + v_pos<NT>(i, n) * CH + ch, slot = c % NS;
+                            wait_bar(&kvfull[slot], (c / NS) & 1, a.status, bad);
+                            uint8_t * vb = sm + Ly::ring + slot * Ly::chunk;
+                            for (int u = NT == 2 ? (tid & 127) : tid; u < Ly::chunk / 16; u += NT == 2 ? 128 : 256) {
+                                const int r = ch * Ly::vtok + (u >> 3) % Ly::vtok;
+                                if (r < z0 || r >= z1) *reinterpret_cast<uint4 *>(vb + u * 16) = make_uint4(0, 0, 0, 0);
+                            }
+                        }
+                        fence_proxy_async_smem();
+                    }
+                }
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_rdy[b]);
+            }
+            // ---------------- the item's end ----------------
+            if (run && n > 0) {
+                pv_wait(pvc);
+                tc::fence_after();
+            }
+            const bool whole = w.off == 0 && w.take == w.sp.units;
+            if constexpr (NT == 1) {
+                float * rd = red + (turn & 1) * 2 * kBM;
+                turn++;
+                rd[wg * kBM + row] = l;
+                named_bar_sync(1 + wq, 64);
+                l += rd[(wg ^ 1) * kBM + row];
+            }
+            const int     o0 = NT == 2 ? 0 : OC * wg;
+            const int64_t rr = rb + row;
+            const int     slot = 2 * blockIdx.x + (w.off == 0 ? 1 : 0);
+            float         f    = 1.0f;
+            if (whole) {
+                float L = l;
+                if (a.sinks && mine) {
+                    const float sk = a.sinks[w.h * a.G + (int) (rr % a.G)] * kLog2e;
+                    // relative to the larger of the two maxima
+                    if (sk > m) {
+                        const float d = m == -INFINITY ? 0.0f : ex2(m - sk);
+                        L             = l * d + exp2f(kShift);
+                        f             = d;
+                    } else {
+                        L += ex2(sk - m + kShift);
+                    }
+                }
+                f = L > 0.0f ? f / L : 0.0f;
+            } else if (mine && (NT == 2 || wg == 0)) {
+                a.part_ms[(int64_t) slot * a.prow + q * kBM + row] = make_float2(m, l);
+            }
+            if (some && run) {
+                uint8_t * dst = a.dst;
+                float *   acc = a.part_acc;
+                if (mine) {
+                    dst += (int64_t) (w.h * a.G + (int) (rr % a.G)) * a.dnb1 + (w.r0 + rr / a.G) * a.dnb2;
+                    acc += ((int64_t) slot * a.prow + q * kBM + row) * D;
+                }
+#pragma unroll 1
+                for (int c = 0; c < OC; c += 32) {
+                    uint32_t o[32];
+                    if (n > 0) {
+                        ld32(tc::taddr(tO + q * D, wq, o0 + c), o);
+                        tc::wait_ld();
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = 0;
+                    }
+                    if (!mine) continue;
+                    if (!whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            __stcg(reinterpret_cast<uint4 *>(acc + o0 + c + e), make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(f != 0.0f ? __uint_as_float(o[e]) * f : 0.0f);
+                        if constexpr (PREC) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) {
+                                *reinterpret_cast<uint4 *>(dst + 4 * (o0 + c + e)) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) {
+                                uint32_t h[4];
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    const __half2 h2 = __floats2half2_rn(__uint_as_float(o[e + 2 * k]), __uint_as_float(o[e + 2 * k + 1]));
+                                    h[k]             = *reinterpret_cast<const uint32_t *>(&h2);
+                                }
+                                *reinterpret_cast<uint4 *>(dst + 2 * (o0 + c + e)) = make_uint4(h[0], h[1], h[2], h[3]);
+                            }
+                        }
+                    }
+                }
+            }
+            tc::fence_before();  // O is read: the next item's products may write it
+            if (tid == 0 && !whole && w.off == 0) {
+                // this CTA opens an item that others go on with: parts of it, for the merge
+                const int64_t end = range[0] + (range[1] - range[0] - w.rem) + w.sp.units;
+                int           e   = blockIdx.x;
+                while (range[2] * (e + 1) / range[3] < end) e++;
+                a.desc[2 * blockIdx.x + 1] = make_int4((int) ((int64_t) w.rt * BMN), (int) min((int64_t) BMN, R - (int64_t) w.rt * BMN), 0, 0);
+                a.desc[2 * blockIdx.x]     = make_int4(e - (int) blockIdx.x + 1, w.h, w.r0, 0);
+            }
+            rc0 += 2 * n * CH;
+        }
+    } else if constexpr (Q8) {
+        // ---------------- converters (q8_0): raw rows -> f16 chunks ----------------
+        const int qr = warp - kSmWarps - 2;  // quarter of the row: dims 64 qr .. 64 qr + 63, one swizzled plane
+        uint32_t  rc = 0, rr = 0;            // chunks, raw slots so far
+        for (; active; active = walk_next<BMN>(a, w)) {
+            const int n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
+            for (int pos = 0; pos < 2 * n; pos++) {
+                bool isk;
+                int  i;
+                at_pos<NT>(pos, n, isk, i);
+                const int t0 = (kt + i) * kBN;
+#pragma unroll 1
+                for (int r = 0; r < kBN / kRawTok; r++, rr++) {
+                    // K: both chunks at the first raw slot; V: chunk r / 2 at its first
+                    if (isk ? r == 0 : (r & 1) == 0) {
+                        for (int c = isk ? 0 : r >> 1; c < (isk ? 2 : (r >> 1) + 1); c++) {
+                            const uint32_t k = rc + c;
+                            if (k >= NS) wait_bar(&kvempty[k % NS], (k / NS - 1) & 1, a.status, bad);
+                        }
+                    }
+                    const int slot = rr % Ly::NR;
+                    wait_bar(&rfull[slot], (rr / Ly::NR) & 1, a.status, bad);
+                    const int  t    = kRawTok * r + lane;  // token of the tile
+                    const int  tk   = t0 + t;
+                    const bool zero = !isk && (tk < w.sp.lo || tk >= w.sp.hi);
+                    uint8_t *  dst  = isk ? sm + Ly::ring + ((rc + (qr >> 1)) % NS) * Ly::chunk + (qr & 1) * (kBN * 128) + t * 128
+                                          : sm + Ly::ring + ((rc + (r >> 1)) % NS) * Ly::chunk + qr * (64 * 128) + (t & 63) * 128;
+                    convert_q8(sm + Ly::raw + slot * kRawB + lane * 272, qr, dst, t, zero);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&rempty[slot]);
+                        if (isk && r == 3) {
+                            mbar_arrive(&kvfull[rc % NS]);
+                            mbar_arrive(&kvfull[(rc + 1) % NS]);
+                        } else if (!isk && (r & 1)) {
+                            mbar_arrive(&kvfull[(rc + (r >> 1)) % NS]);
+                        }
+                    }
+                }
+                rc += 2;
+            }
+        }
+    }
+    __syncwarp();
+    tc::fence_before();
+    __syncthreads();
+    if (warp == kSmWarps) tc::tmem_free(tbase, 512);
+}
+
+// The records of an item cut between CTAs, joined in the order of the cuts; one warp per row. CTA c opens the item
+// (record 2c + 1), CTAs c + 1 .. c + parts - 1 go on with it (records 2(c + 1), 2(c + 2), ...).
+template <int D, bool F32> __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const __grid_constant__ PArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int  c  = blockIdx.x;
+    const int4 d0 = a.desc[2 * c];
+    if (d0.x == 0) return;
+    const int4 d1 = a.desc[2 * c + 1];
+    const int  lane = threadIdx.x & 31;
+    for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < d1.y; row += gridDim.y * 8) {
+        const int rr = d1.x + row, h = d0.y * a.G + rr % a.G;
+        auto      rec = [&](int p) { return (int64_t) (2 * (c + p) + (p == 0 ? 1 : 0)) * a.prow + row; };
+        float     M   = -INFINITY;
+        for (int p = lane; p < d0.x; p += 32) {
+            const float2 v = __ldcg(a.part_ms + rec(p));
+            if (v.y > 0.0f) M = fmaxf(M, v.x);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        float sk = -INFINITY;
+        if (a.sinks) {
+            sk = a.sinks[h] * kLog2e;
+            M  = fmaxf(M, sk);
+        }
+        float L = sk > -INFINITY ? ex2(sk - M + kShift) : 0.0f;
+        float acc[D / 32];
+#pragma unroll
+        for (int e = 0; e < D / 32; e++) acc[e] = 0.0f;
+#pragma unroll 4
+        for (int p = 0; p < d0.x; p++) {
+            const float2 v = __ldcg(a.part_ms + rec(p));
+            const float  w = v.y > 0.0f ? ex2(v.x - M) : 0.0f;
+            L              = fmaf(w, v.y, L);
+            const float * src = a.part_acc + rec(p) * D;
+            if constexpr (D >= 128) {
+#pragma unroll
+                for (int e = 0; e < D / 128; e++) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(src) + 32 * e + lane);
+                    acc[4 * e]     = w > 0.0f ? fmaf(w, x.x, acc[4 * e]) : acc[4 * e];
+                    acc[4 * e + 1] = w > 0.0f ? fmaf(w, x.y, acc[4 * e + 1]) : acc[4 * e + 1];
+                    acc[4 * e + 2] = w > 0.0f ? fmaf(w, x.z, acc[4 * e + 2]) : acc[4 * e + 2];
+                    acc[4 * e + 3] = w > 0.0f ? fmaf(w, x.w, acc[4 * e + 3]) : acc[4 * e + 3];
+                }
+            } else {
+                const float2 x = __ldcg(reinterpret_cast<const float2 *>(src) + lane);
+                acc[0]         = w > 0.0f ? fmaf(w, x.x, acc[0]) : acc[0];
+                acc[1]         = w > 0.0f ? fmaf(w, x.y, acc[1]) : acc[1];
+            }
+        }
+        const float f   = L > 0.0f ? 1.0f / L : 0.0f;
+        uint8_t *   dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) (d0.z + rr / a.G) * a.dnb2;
+        constexpr int V = D >= 128 ? 4 : 2;  // values a lane holds side by side
+#pragma unroll
+        for (int e = 0; e < D / 32; e += V) {
+            const int at = (e / V) * 32 * V + lane * V;
+#pragma unroll
+            for (int k = 0; k < V; k += 2) {
+                if constexpr (F32) {
+                    *reinterpret_cast<float2 *>(dst + 4 * (at + k)) = make_float2(acc[e + k] * f, acc[e + k + 1] * f);
+                } else {
+                    *reinterpret_cast<__half2 *>(dst + 2 * (at + k)) = __floats2half2_rn(acc[e + k] * f, acc[e + k + 1] * f);
+                }
+            }
         }
     }
 }
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_fn() {
+    static EncodeTiled fn = [] {
+        void *                          p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess) {
+            p = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// row tiles per CTA: two share K/V (head_dim <= 128) where the sequences' rows fill more than one on average; with fewer
+// rows the second would be empty and one tile with two score buffers keeps the products and the softmax apart
+int row_tiles(int T, int S, int G, int D) { return D <= 128 && (int64_t) T * G > (int64_t) S * kBM ? 2 : 1; }
+
+template <int D, int NT, bool PREC, bool Q8>
+int launch_paged(srhpm_ctx * ctx, const PArgs & a, const CUtensorMap & mk, const CUtensorMap & mv, cudaStream_t stream) {
+    using Ly = Lay<D, NT, PREC, Q8>;
+    static std::atomic<unsigned> done{ 0 };
+    const unsigned               bit = 1u << (ctx->device & 31);
+    if (!(done.load() & bit)) {
+        const int st = cuda_status(cudaFuncSetAttribute(fa_paged_kernel<D, NT, PREC, Q8>,
+                                                        cudaFuncAttributeMaxDynamicSharedMemorySize, Ly::alloc));
+        if (st != SRHPM_OK) return st;
+        done.fetch_or(bit);
+    }
+    int st = cuda_status(launch_k_pdl(fa_paged_kernel<D, NT, PREC, Q8>, dim3(ctx->num_sms), dim3(Ly::threads), Ly::alloc,
+                                      stream, mk, mv, a));
+    ctx->launches.fetch_add(1);
+    if (st != SRHPM_OK) return st;
+    st = cuda_status(launch_k_pdl(fa_paged_merge_kernel<D, PREC>, dim3(ctx->num_sms, std::min(16, (a.prow + 7) / 8)),
+                                  dim3(256), 0, stream, a));
+    ctx->launches.fetch_add(1);
+    return st;
+}
+
+int record_rows(int T, int G, int NT) { return (int) std::min<int64_t>((int64_t) kBM * NT, (int64_t) T * G); }
+
+size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
 }  // namespace
 
-size_t fa_paged_work_size(const srhpm_ctx *, int, int, int, int, int) { return 0; }
+size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S) {
+    const int    NT   = row_tiles(T, S, H / Hkv, D);
+    const size_t recs = (size_t) 2 * ctx->num_sms * record_rows(T, H / Hkv, NT);
+    return recs * D * sizeof(float) + align16(recs * sizeof(float2)) + 2 * (size_t) ctx->num_sms * sizeof(int4) + 16;
+}
 
-int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void *, size_t, cudaStream_t stream) {
-    const int st = cuda_status(launch_k_pdl(fa_paged_kernel, dim3(v.T, v.H), dim3(128), 0, stream, v, ctx->d_status));
-    ctx->launches.fetch_add(1);
-    return st;
+int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t wsize, cudaStream_t stream) {
+    const int D = v.c.D, G = v.H / v.c.Hkv;
+    if (v.S > kMaxSeqs) return SRHPM_UNSUPPORTED;
+    if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.c.Hkv, D, v.S)) return SRHPM_ERR_WORKSPACE;
+    const int NT = row_tiles(v.T, v.S, G, D);
+    PArgs     a;
+    a.q       = v.q;
+    a.qnb1    = v.qnb1;
+    a.qnb2    = v.qnb2;
+    a.dst     = v.dst;
+    a.dnb1    = v.dnb1;
+    a.dnb2    = v.dnb2;
+    a.table   = v.table;
+    a.tstride = v.tstride;
+    a.cols    = v.cols;
+    a.page    = v.c.page;
+    a.n_pages = (int) v.c.n_pages;
+    a.q_start = v.q_start;
+    a.kv_len  = v.kv_len;
+    a.S       = v.S;
+    a.T       = v.T;
+    a.H       = v.H;
+    a.Hkv     = v.c.Hkv;
+    a.G       = G;
+    a.window  = v.window;
+    a.qscale     = v.softcap != 0.0f ? v.scale / v.softcap : v.scale * kLog2e;
+    a.softcap_l2 = v.softcap * kLog2e;
+    a.sinks      = v.sinks;
+    a.prow       = record_rows(v.T, G, NT);
+    const size_t recs = (size_t) 2 * ctx->num_sms * a.prow;
+    uint8_t *    wb   = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(wdata) + 15) & ~(uintptr_t) 15);
+    a.part_acc = reinterpret_cast<float *>(wb);
+    a.part_ms  = reinterpret_cast<float2 *>(wb + recs * D * sizeof(float));
+    a.desc     = reinterpret_cast<int4 *>(wb + recs * D * sizeof(float) + align16(recs * sizeof(float2)));
+    a.status   = ctx->d_status;
+
+    const bool q8 = v.c.type == SRHPM_TYPE_Q8_0;
+    a.box = q8 ? kRawTok : 64;
+    while (a.page % a.box) a.box >>= 1;  // the page is a multiple of 16
+
+    EncodeTiled enc = encode_fn();
+    if (!enc) return SRHPM_ERR_CUDA;
+    CUtensorMap mk, mv;
+    for (int i = 0; i < 2; i++) {
+        const cuuint64_t row = q8 ? 272 : (cuuint64_t) D * 2;
+        // a dimension of one element never steps: any valid stride
+        auto str = [&](int64_t nb, int64_t ne) { return ne > 1 ? (cuuint64_t) nb : row; };
+        const cuuint64_t dims[4] = { q8 ? 68 : (cuuint64_t) D, (cuuint64_t) v.c.page, (cuuint64_t) v.c.Hkv, (cuuint64_t) v.c.n_pages };
+        const cuuint64_t st[3]   = { str(i ? v.c.vnb1 : v.c.knb1, v.c.page), str(i ? v.c.vnb2 : v.c.knb2, v.c.Hkv),
+                                     str(i ? v.c.vnb3 : v.c.knb3, v.c.n_pages) };
+        const cuuint32_t box[4]  = { q8 ? 68u : 64u, (cuuint32_t) a.box, 1, 1 }, es[4] = { 1, 1, 1, 1 };
+        const CUresult   r = enc(i ? &mv : &mk, q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4,
+                                 const_cast<uint8_t *>(i ? v.c.v : v.c.k), dims, st, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                 q8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return SRHPM_ERR_INVALID;
+    }
+    if (q8) return v.f32 ? launch_paged<256, 1, true, true>(ctx, a, mk, mv, stream) : launch_paged<256, 1, false, true>(ctx, a, mk, mv, stream);
+    switch (D * 4 + NT * 2 - 2 + (v.f32 ? 1 : 0)) {
+        case 64 * 4: return launch_paged<64, 1, false, false>(ctx, a, mk, mv, stream);
+        case 64 * 4 + 1: return launch_paged<64, 1, true, false>(ctx, a, mk, mv, stream);
+        case 64 * 4 + 2: return launch_paged<64, 2, false, false>(ctx, a, mk, mv, stream);
+        case 64 * 4 + 3: return launch_paged<64, 2, true, false>(ctx, a, mk, mv, stream);
+        case 128 * 4: return launch_paged<128, 1, false, false>(ctx, a, mk, mv, stream);
+        case 128 * 4 + 1: return launch_paged<128, 1, true, false>(ctx, a, mk, mv, stream);
+        case 128 * 4 + 2: return launch_paged<128, 2, false, false>(ctx, a, mk, mv, stream);
+        case 128 * 4 + 3: return launch_paged<128, 2, true, false>(ctx, a, mk, mv, stream);
+        case 256 * 4: return launch_paged<256, 1, false, false>(ctx, a, mk, mv, stream);
+        default: return launch_paged<256, 1, true, false>(ctx, a, mk, mv, stream);
+    }
 }
 
 }  // namespace srhpm

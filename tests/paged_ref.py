@@ -93,6 +93,29 @@ def attention(q, kc, vc, table, q_start, kv_len, scale, softcap=0.0, window=0, s
     return out, mag, big
 
 
+def attention_dense(q, k, v, q_start, kv_len, scale, window=0):
+    """The same for long inputs, on the inputs' device (torch): k, v [S][L, Hkv, D] values of each sequence. Returns
+    (out, |v| average, largest sum |q k| scale) in 64 bits."""
+    import torch
+    T, H, D = q.shape
+    out, mag = (torch.zeros((T, H, D), dtype=torch.float64, device=q.device) for _ in range(2))
+    big = torch.zeros((T, H, 1), dtype=torch.float64, device=q.device)
+    for s in range(len(kv_len)):
+        r0, r1 = int(q_start[s]), int(q_start[s + 1])
+        L, G = int(kv_len[s]), H // k[s].shape[1]
+        p = torch.arange(L - (r1 - r0), L, device=q.device)[:, None]
+        j = torch.arange(L, device=q.device)
+        hide = (j > p) | ((j <= p - window) if window > 0 else (j < 0))
+        for h in range(H):
+            kk, vv = k[s][:, h // G].double(), v[s][:, h // G].double()
+            qq = q[r0:r1, h].double()
+            sc = (qq @ kk.T * scale).masked_fill(hide, -math.inf)
+            w = torch.softmax(sc, 1)
+            out[r0:r1, h], mag[r0:r1, h] = w @ vv, w @ vv.abs()
+            big[r0:r1, h] = (qq.abs() @ kk.abs().T).masked_fill(hide, 0).amax(1, keepdim=True) * scale
+    return out.cpu().numpy(), mag.cpu().numpy(), big.cpu().numpy()
+
+
 def sample(logits, ids, q_start, u, us, dp=None, temp=None):
     """(out_ids with -1 for what is not emitted and None behind the last sequence, out_n, p_draft)."""
     T, V = logits.shape

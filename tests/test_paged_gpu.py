@@ -205,10 +205,14 @@ def attn_case(rng, past, new, H, Hkv, D, P, kv, qt, poison=True, pad_rows=0, spr
 
 
 def attn_check(got, q, vals, table, q_start, kv_len, scale, **kw):
+    attn_bound(got, q, R.attention(q.astype(np.float64), np.nan_to_num(vals[0].astype(np.float64), posinf=0, neginf=0),
+                                   np.nan_to_num(vals[1].astype(np.float64), posinf=0, neginf=0), table, q_start,
+                                   kv_len, scale, **kw), q_start, kv_len)
+
+
+def attn_bound(got, q, ref, q_start, kv_len):
+    want, A, B = ref
     used = int(q_start[-1])
-    want, A, B = R.attention(q.astype(np.float64), np.nan_to_num(vals[0].astype(np.float64), posinf=0, neginf=0),
-                             np.nan_to_num(vals[1].astype(np.float64), posinf=0, neginf=0), table, q_start, kv_len,
-                             scale, **kw)
     D, n = q.shape[2], int(max(kv_len.max(), 1))
     e = (D / 8 + 2) * 2.0 ** -23 * B
     if q.dtype == np.float16:
@@ -341,6 +345,35 @@ def test_attention_layouts(ctx, kv, D):
     attn_check(out[:, :H].cpu().numpy(), q, vals, table, q_start, kv_len, D ** -0.5)
     assert (out[:, H] == 7.0).all()
     ctx.check()
+
+
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+@pytest.mark.parametrize("kv,D,H,Hkv,P,past,new,window", [
+    (L.F16, 128, 32, 8, 48, [1326, 2666, 2194, 237, 153, 0, 1738], [13, 441, 297, 7, 229, 565, 1], 1024),
+    (L.F16, 64, 8, 8, 16, [0, 3000, 10, 900] * 5, [700, 40, 1, 129] * 5, 0),
+    (L.F16, 256, 24, 4, 64, [700, 5, 3000, 129], [300, 9, 1, 128], 0),
+    (L.Q8_0, 256, 12, 4, 32, [700, 5, 3000, 129], [300, 9, 1, 128], 200),
+    (L.F16, 128, 16, 8, 16, [0, 1, 2, 6000, 5000, 4000, 3000, 20] * 4, [1, 2, 3, 4, 1, 1, 9, 20] * 4, 0)])
+def test_attention_many_tiles_per_cta(ctx, qt, kv, D, H, Hkv, P, past, new, window):
+    """Far more tiles than SMs: every CTA takes several items of several tiles each, whole ones and cut ones, one row tile
+    and two; ten times over, since what a slow warp meets depends on its timing."""
+    rng = np.random.default_rng(D + P)
+    q, caches, vals, table, q_start, kv_len = attn_case(rng, past, new, H, Hkv, D, P, kv, qt)
+    d = [cu(x) for x in (q, caches[0], caches[1], table, q_start, kv_len)]
+    runs = [ctx.flash_attn_paged(d[0], d[1], d[2], kv, d[3], d[4], d[5], scale=D ** -0.5, window=window)
+            for _ in range(10)]
+    torch.cuda.synchronize()
+    ctx.check()
+    seqs = [[], []]
+    for c, v in zip(seqs, vals):
+        vt = cu(v)
+        for s, L_ in enumerate(kv_len):
+            pages = cu(table[s, :-(-int(L_) // P)].astype(np.int64))
+            c.append(vt[pages].flatten(0, 1)[:int(L_)])
+    ref = R.attention_dense(d[0], seqs[0], seqs[1], q_start, kv_len, D ** -0.5, window)
+    attn_bound(runs[0].cpu().numpy(), q, ref, q_start, kv_len)
+    for r in runs[1:]:
+        assert torch.equal(r, runs[0])
 
 
 def test_attention_far_pages(ctx):
