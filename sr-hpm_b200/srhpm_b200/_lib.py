@@ -90,14 +90,15 @@ _SIGNATURES = {
                                      ctypes.c_float, _T, _T, _P]),
     "srhpm_swiglu": (ctypes.c_int, [_P, _P, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_int64,
                                     _P]),
-    "srhpm_page_plan": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, ctypes.c_int, _T, _P, ctypes.c_int, _P, ctypes.c_int,
+    # the views of these are passed as the bytes of the structure (ops._pack)
+    "srhpm_page_plan": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, ctypes.c_int, _P, _P, ctypes.c_int, _P, ctypes.c_int,
                                        _P, _P, _P, _P, _P, _P, _P]),
-    "srhpm_rope_kv_paged": (ctypes.c_int, [_P, _T, ctypes.c_int, ctypes.c_int, _P, _P, ctypes.c_float, _T, _T, _T, _P]),
-    "srhpm_flash_attn_paged_work_size": (ctypes.c_int, [_P, _T, _T, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
-    "srhpm_flash_attn_paged": (ctypes.c_int, [_P, _T, _T, _T, _T, _P, _P, _T, ctypes.c_float, ctypes.c_float,
-                                              ctypes.c_int, _T, _P, ctypes.c_size_t, _P]),
-    "srhpm_verify_sample_work_size": (ctypes.c_int, [_P, _T, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
-    "srhpm_verify_sample": (ctypes.c_int, [_P, _T, _P, _P, ctypes.c_int, _T, _P, _P, _P, _P, _P, _P, _P,
+    "srhpm_rope_kv_paged": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_int, _P, _P, ctypes.c_float, _P, _P, _P, _P]),
+    "srhpm_flash_attn_paged_work_size": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "srhpm_flash_attn_paged": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_float, ctypes.c_float,
+                                              ctypes.c_int, _P, _P, ctypes.c_size_t, _P]),
+    "srhpm_verify_sample_work_size": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "srhpm_verify_sample": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, _P,
                                            ctypes.c_size_t, _P]),
     "srhpm_quantize_chunk": (ctypes.c_size_t, [ctypes.c_int, _P, _P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                                 _P]),

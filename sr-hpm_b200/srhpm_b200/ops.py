@@ -19,6 +19,7 @@ libsrhpm_b200.so through its C ABI; a missing library raises.
 """
 import collections
 import ctypes
+import struct
 import warnings
 
 import numpy as np
@@ -50,49 +51,57 @@ def _stream_ptr(stream):
     return ctypes.c_void_p(s.cuda_stream)
 
 
-_I64x4, _SZx4 = ctypes.c_int64 * 4, ctypes.c_size_t * 4
+# cudaStream_t of a device's current stream (torch's own shortcut where it has one: the public way takes 2 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 PagePlan = collections.namedtuple("PagePlan", "q_start kv_len pos slots status n_taken")
 
+# The calls of a serving step are short on the GPU, so their host side is kept short too: a view is the bytes of an
+# srhpm_tensor (type, ne[4], nb[4], data), packed in one go.
+_pack = struct.Struct("@iqqqqNNNNP").pack
+assert struct.calcsize("@iqqqqNNNNP") == ctypes.sizeof(L.SrhpmTensor)
 
-def _view(t, type_, ne, nb):
-    """A ggml view with all four dimensions given."""
-    return ctypes.byref(L.SrhpmTensor(type_, _I64x4(*ne), _SZx4(*nb), t.data_ptr()))
 
-
-def _rows_2d(x, type_, size):
-    """View of a 2-D tensor [rows, cols] with contiguous rows: ne = [cols, rows]."""
+def _rows_2d(x, dtype, type_, what):
+    """View of a 2-D tensor [rows, cols] of 4-byte values with contiguous rows: ne = [cols, rows]."""
+    if x.dtype is not dtype or x.dim() != 2 or (x.stride(1) != 1 and x.shape[1] > 1):
+        raise ValueError(f"{what} must be {dtype} [rows, cols] with contiguous rows")
     r, c = x.shape
-    nb = x.stride(0) * size
-    return _view(x, type_, (c, r, 1, 1), (size, nb, nb * r, nb * r))
+    nb = x.stride(0) * 4
+    return _pack(type_, c, r, 1, 1, 4, nb, nb * r, nb * r, x.data_ptr())
 
 
 def _head_rows(x, heads_first):
     """View of token rows [T, H, D] (f32 or f16, any strides of the first two): ne = [D, T, H], or [D, H, T]."""
-    if x.dtype not in (torch.float16, torch.float32) or x.dim() != 3 or x.stride(2) != 1:
+    e = 2 if x.dtype is torch.float16 else 4 if x.dtype is torch.float32 else 0
+    if e == 0 or x.dim() != 3 or x.stride(2) != 1:
         raise ValueError("rows must be f16 or f32 [T, H, D] with contiguous heads")
     T, H, D = x.shape
-    e = x.element_size()
-    a, b = x.stride(0) * e, x.stride(1) * e
+    a, b, _ = x.stride()
+    a *= e
+    b *= e
+    t = L.F16 if e == 2 else L.F32
     if heads_first:
-        return _view(x, L.F16 if e == 2 else L.F32, (D, H, T, 1), (e, b, a, a * T))
-    return _view(x, L.F16 if e == 2 else L.F32, (D, T, H, 1), (e, a, b, a * T))
+        return _pack(t, D, H, T, 1, e, b, a, a * T, x.data_ptr())
+    return _pack(t, D, T, H, 1, e, a, b, a * T, x.data_ptr())
 
 
 def _paged(c, kv_type):
     """View of a paged cache uint8 [pages, page_size, Hkv, row bytes]: ne = [D, page_size, Hkv, pages]."""
-    if c.dtype != torch.uint8 or c.dim() != 4 or c.stride(3) != 1:
+    if c.dtype is not torch.uint8 or c.dim() != 4 or c.stride(3) != 1:
         raise ValueError("a paged cache is uint8 [pages, page_size, Hkv, row bytes] with contiguous rows")
     n, P, Hkv, rowb = c.shape
+    n3, n1, n2, _ = c.stride()
     size, blk = (34, 32) if kv_type == L.Q8_0 else (2, 1)
     if rowb % size:
         raise ValueError("row bytes do not hold whole blocks of the cache type")
-    return _view(c, kv_type, (rowb // size * blk, P, Hkv, n), (size, c.stride(1), c.stride(2), c.stride(0)))
+    return _pack(kv_type, rowb // size * blk, P, Hkv, n, size, n1, n2, n3, c.data_ptr())
 
 
 def _ints(t, dtype, n, what):
     """Address of a contiguous integer or f32 vector of at least n values."""
-    if t.dtype != dtype or t.dim() != 1 or t.numel() < n or (t.stride(0) != 1 and n > 1):
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{what} must be a contiguous {dtype} vector of at least {n} values")
     return t.data_ptr()
 
@@ -178,6 +187,8 @@ class Context:
         L.check(self.lib.srhpm_ctx_create(self.device.index or 0, ctypes.byref(h)), "srhpm_ctx_create")
         self.handle = h
         self._work = None
+        self._index = self.device.index or 0
+        self._sizes = {}
 
     def close(self):
         if self.handle:
@@ -468,8 +479,8 @@ class Context:
     # several streams never share a buffer, and a captured graph keeps its own.
     def _on_device(self, *tensors):
         for t in tensors:
-            if t is not None and t.device != self.device and t.device != torch.device("cuda", self.device.index or 0):
-                raise ValueError(f"a tensor on {t.device} given to a context of {self.device}")
+            if t is not None and t.get_device() != self._index:
+                raise ValueError(f"a tensor on {t.device} given to a context of cuda:{self._index}")
 
     def _new(self, shape, dtype, stream):
         if stream is None:
@@ -477,16 +488,25 @@ class Context:
         with torch.cuda.stream(stream):
             return torch.empty(shape, dtype=dtype, device=self.device)
 
-    def _call(self, fn, what, *args, stream=None):
-        """One C-ABI call on `stream` (the context's device's current stream by default)."""
-        s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        if torch.cuda.current_device() == (self.device.index or 0):
-            st = fn(self.handle, *args, s.cuda_stream)
+    def _call(self, fn, what, stream, *args):
+        """One C-ABI call on `stream` (the current stream of the context's device if None)."""
+        s = _raw_stream(self._index) if stream is None else stream.cuda_stream
+        if torch.cuda.current_device() == self._index:
+            st = fn(self.handle, *args, s)
         else:
             with torch.cuda.device(self.device):
-                st = fn(self.handle, *args, s.cuda_stream)
+                st = fn(self.handle, *args, s)
         if st != L.OK:
             raise L.SrhpmError(st, what, self.lib)
+
+    def _scratch(self, fn, what, key, stream, *args):
+        """Work buffer of a call; its size goes by the shapes in `key` alone and is asked for once for each."""
+        n = self._sizes.get(key)
+        if n is None:
+            sz = ctypes.c_size_t()
+            L.check(fn(self.handle, *args, ctypes.byref(sz)), what)
+            n = self._sizes[key] = max(sz.value, 16)
+        return self._new(n, torch.uint8, stream)
 
     def page_plan(self, n_past, n_new, block_table, free_pages, page_size, n_rows, free_head=None, out=None,
                   stream=None):
@@ -496,22 +516,23 @@ class Context:
         n_taken int32 [1] (`out`: one to write into)."""
         S = n_past.numel()
         self._on_device(n_past, n_new, block_table, free_pages, free_head)
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
-            raise ValueError("block_table must be int32 [S, entries] with contiguous rows")
+        i32 = torch.int32
         if out is None:
-            i32 = self._new(3 * S + 2 + n_rows, torch.int32, stream)
-            out = PagePlan(i32[:S + 1], i32[S + 1:2 * S + 1], i32[3 * S + 2:], self._new(n_rows, torch.int64, stream),
-                           i32[2 * S + 1:3 * S + 1], i32[3 * S + 1:3 * S + 2])
+            at = self._new(3 * S + 2 + n_rows, i32, stream)
+            q, k, st, nt, pos = at.split_with_sizes((S + 1, S, S, 1, n_rows))
+            out = PagePlan(q, k, pos, self._new(n_rows, torch.int64, stream), st, nt)
+            p = at.data_ptr()
+            ptrs = (p, p + 4 * (S + 1), p + 4 * (3 * S + 2), out.slots.data_ptr(), p + 4 * (2 * S + 1),
+                    p + 4 * (3 * S + 1))
         else:
             self._on_device(*out)
-        i32 = torch.int32
-        self._call(self.lib.srhpm_page_plan, "srhpm_page_plan", _ints(n_past, i32, S, "n_past"),
-                   _ints(n_new, i32, S, "n_new"), S, page_size, _rows_2d(block_table, L.I32, 4),
+            ptrs = (_ints(out.q_start, i32, S + 1, "q_start"), _ints(out.kv_len, i32, S, "kv_len"),
+                    _ints(out.pos, i32, n_rows, "pos"), _ints(out.slots, torch.int64, n_rows, "slots"),
+                    _ints(out.status, i32, S, "status"), _ints(out.n_taken, i32, 1, "n_taken"))
+        self._call(self.lib.srhpm_page_plan, "srhpm_page_plan", stream, _ints(n_past, i32, S, "n_past"),
+                   _ints(n_new, i32, S, "n_new"), S, page_size, _rows_2d(block_table, i32, L.I32, "block_table"),
                    _ints(free_pages, i32, 0, "free_pages"), free_pages.numel(),
-                   None if free_head is None else _ints(free_head, i32, 1, "free_head"), n_rows,
-                   _ints(out.q_start, i32, S + 1, "q_start"), _ints(out.kv_len, i32, S, "kv_len"),
-                   _ints(out.pos, i32, n_rows, "pos"), _ints(out.slots, torch.int64, n_rows, "slots"),
-                   _ints(out.status, i32, S, "status"), _ints(out.n_taken, i32, 1, "n_taken"), stream=stream)
+                   None if free_head is None else _ints(free_head, i32, 1, "free_head"), n_rows, *ptrs)
         return out
 
     def rope_kv_paged(self, qkv, pos, slots, k_cache, v_cache, kv_type, q_out, theta_base=1e6, stream=None):
@@ -520,12 +541,10 @@ class Context:
         uint8 [pages, page_size, Hkv, row bytes]. Returns q_out."""
         n = qkv.shape[0]
         self._on_device(qkv, pos, slots, k_cache, v_cache, q_out)
-        if qkv.dtype != torch.float32 or qkv.dim() != 2 or qkv.stride(1) != 1:
-            raise ValueError("qkv must be f32 [n, width] with contiguous rows")
-        self._call(self.lib.srhpm_rope_kv_paged, "srhpm_rope_kv_paged", _rows_2d(qkv, L.F32, 4), q_out.shape[1],
-                   k_cache.shape[2], _ints(pos, torch.int32, n, "pos"), _ints(slots, torch.int64, n, "slots"),
-                   theta_base, _head_rows(q_out, False), _paged(k_cache, kv_type), _paged(v_cache, kv_type),
-                   stream=stream)
+        self._call(self.lib.srhpm_rope_kv_paged, "srhpm_rope_kv_paged", stream,
+                   _rows_2d(qkv, torch.float32, L.F32, "qkv"), q_out.shape[1], k_cache.shape[2],
+                   _ints(pos, torch.int32, n, "pos"), _ints(slots, torch.int64, n, "slots"), theta_base,
+                   _head_rows(q_out, False), _paged(k_cache, kv_type), _paged(v_cache, kv_type))
         return q_out
 
     def flash_attn_paged(self, q, k_cache, v_cache, kv_type, block_table, q_start, kv_len, scale=1.0, softcap=0.0,
@@ -538,21 +557,18 @@ class Context:
         if out is None:
             out = self._new(q.shape, q.dtype, stream)
         self._on_device(q, k_cache, v_cache, block_table, q_start, kv_len, sinks, out, work)
-        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1:
-            raise ValueError("block_table must be int32 [S, entries] with contiguous rows")
         qv, kv = _head_rows(q, False), _paged(k_cache, kv_type)
-        sz = ctypes.c_size_t()
-        L.check(self.lib.srhpm_flash_attn_paged_work_size(self.handle, qv, kv, S, ctypes.byref(sz)),
-                "srhpm_flash_attn_paged_work_size")
-        buf = work if work is not None else self._new(max(sz.value, 16), torch.uint8, stream)
+        if work is None:
+            work = self._scratch(self.lib.srhpm_flash_attn_paged_work_size, "srhpm_flash_attn_paged_work_size",
+                                 ("fa", q.shape, k_cache.shape, kv_type, S), stream, qv, kv, S)
         sv = None
         if sinks is not None:
-            _ints(sinks, torch.float32, q.shape[1], "sinks")
-            sv = _view(sinks, L.F32, (sinks.shape[0], 1, 1, 1), (4, 4, 4, 4))
-        self._call(self.lib.srhpm_flash_attn_paged, "srhpm_flash_attn_paged", qv, kv, _paged(v_cache, kv_type),
-                   _rows_2d(block_table, L.I32, 4), _ints(q_start, torch.int32, S + 1, "q_start"),
+            at = _ints(sinks, torch.float32, q.shape[1], "sinks")
+            sv = _pack(L.F32, sinks.shape[0], 1, 1, 1, 4, 4, 4, 4, at)
+        self._call(self.lib.srhpm_flash_attn_paged, "srhpm_flash_attn_paged", stream, qv, kv, _paged(v_cache, kv_type),
+                   _rows_2d(block_table, torch.int32, L.I32, "block_table"), _ints(q_start, torch.int32, S + 1, "q_start"),
                    _ints(kv_len, torch.int32, S, "kv_len"), sv, scale, softcap, window, _head_rows(out, True),
-                   buf.data_ptr(), buf.numel(), stream=stream)
+                   work.data_ptr(), work.numel())
         return out
 
     def verify_sample(self, logits, ids, q_start, u_accept, u_sample, draft_probs=None, temperature=None, out=None,
@@ -564,28 +580,22 @@ class Context:
         out_ids[q_start[s] : q_start[s] + out_n[s]]."""
         T, S = logits.shape[0], q_start.numel() - 1
         self._on_device(logits, ids, q_start, u_accept, u_sample, draft_probs, temperature, work)
-        for x in (logits, draft_probs):
-            if x is not None and (x.dtype != torch.float32 or x.dim() != 2 or x.stride(1) != 1):
-                raise ValueError("logits and draft_probs must be f32 [T, V] with contiguous rows")
+        i32, f32 = torch.int32, torch.float32
         if out is None:
-            out = (self._new(T, torch.int32, stream), self._new(S, torch.int32, stream),
-                   self._new(T, torch.float32, stream))
+            out = (self._new(T, i32, stream), self._new(S, i32, stream), self._new(T, f32, stream))
         else:
             self._on_device(*out)
-        i32, f32 = torch.int32, torch.float32
-        lv = _rows_2d(logits, L.F32, 4)
-        sz = ctypes.c_size_t()
-        L.check(self.lib.srhpm_verify_sample_work_size(self.handle, lv, S, ctypes.byref(sz)),
-                "srhpm_verify_sample_work_size")
-        buf = work if work is not None else self._new(max(sz.value, 16), torch.uint8, stream)
-        self._call(self.lib.srhpm_verify_sample, "srhpm_verify_sample", lv, _ints(ids, i32, T, "ids"),
+        lv = _rows_2d(logits, f32, L.F32, "logits")
+        if work is None:
+            work = self._scratch(self.lib.srhpm_verify_sample_work_size, "srhpm_verify_sample_work_size",
+                                 ("vs", logits.shape, S), stream, lv, S)
+        self._call(self.lib.srhpm_verify_sample, "srhpm_verify_sample", stream, lv, _ints(ids, i32, T, "ids"),
                    _ints(q_start, i32, S + 1, "q_start"), S,
-                   None if draft_probs is None else _rows_2d(draft_probs, L.F32, 4),
+                   None if draft_probs is None else _rows_2d(draft_probs, f32, L.F32, "draft_probs"),
                    None if temperature is None else _ints(temperature, f32, S, "temperature"),
                    _ints(u_accept, f32, T, "u_accept"), _ints(u_sample, f32, S, "u_sample"),
                    _ints(out[0], i32, T, "out_ids"), _ints(out[1], i32, S, "out_n"),
-                   None if out[2] is None else _ints(out[2], f32, T, "p_draft"), buf.data_ptr(), buf.numel(),
-                   stream=stream)
+                   None if out[2] is None else _ints(out[2], f32, T, "p_draft"), work.data_ptr(), work.numel())
         return out
 
     def quantize_rows_q8_K(self, X, stream=None):
