@@ -18,7 +18,7 @@
 // fa_paged_merge_kernel joins in the order of the cuts (same bits every run). The plan is taken from the lengths on the
 // device by every CTA itself, in its prologue: no planning launch.
 //
-// Roles: 8 softmax warps, 1 MMA warp, 1 producer warp (TMA boxes of at most 64 tokens x 64 dims, each within a page, into
+// Roles: 8 softmax warps, 1 MMA warp, 3 producer warps (TMA boxes of at most 64 tokens x 64 dims, each within a page, into
 // a ring of 128-byte-swizzled chunks), and for a q8_0 cache 4 converter warps (raw rows by TMA into a second ring, d * q
 // rounded to f16 into the chunks). NT = 1: the 8 softmax warps halve the columns of one row tile and S has two buffers;
 // NT = 2 (head_dim <= 128): two row tiles share K/V, each with its own 4 softmax warps and buffer.
@@ -44,10 +44,25 @@ constexpr float kShift   = 7.0f;   // p is kept times 2^7
 constexpr int   kBM      = 128;    // rows of a tile
 constexpr int   kBN      = 128;    // tokens of a tile
 constexpr int   kSmWarps = 8;      // softmax warps
+constexpr int   kProd    = 3;      // producer warps (f16 cache)
 constexpr int   kMaxSeqs = 8192;
 constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s (a probe sleeps up to 4 us)
 constexpr int   kRawTok  = 32;     // tokens of a raw q8_0 slot
 constexpr int   kRawB    = kRawTok * 272;
+
+// n / d for 0 <= n < 2^31, d >= 1: one high product (d a power of two or not; the rounded-up reciprocal's error stays
+// under 1 / d for every n < 2^31)
+struct FastDiv {
+    uint32_t mul, shr, d;
+    static FastDiv of(uint32_t d) {
+        FastDiv f{ 0, 0, d };
+        while ((1ull << f.shr) < d) f.shr++;
+        // 2^(31 + shr) / d rounded up: below 2^32, since 2^shr < 2 d
+        f.mul = (uint32_t) (((1ull << (31 + f.shr)) + d - 1) / d);
+        return f;
+    }
+    __device__ __forceinline__ int div(int n) const { return (int) (((uint64_t) (uint32_t) n * mul) >> (31 + shr)); }
+};
 
 struct PArgs {
     const uint8_t * q;
@@ -60,6 +75,7 @@ struct PArgs {
     const int32_t * q_start;
     const int32_t * kv_len;
     int             S, T, H, Hkv, G, window;
+    FastDiv         byG, byPage;
     float           qscale;      // scale * log2e, or scale / softcap
     float           softcap_l2;  // softcap * log2e, 0 = none
     const float *   sinks;
@@ -81,13 +97,13 @@ struct Span {
 __device__ __forceinline__ int row_at(const PArgs & a, int s) { return min(max(a.q_start[s], 0), a.T); }
 
 template <int BMN> __device__ __forceinline__ Span span_of(const PArgs & a, int n, int kv, int rt) {
-    const int64_t r0 = (int64_t) rt * BMN, r1 = min((int64_t) n * a.G, r0 + BMN);
-    const int     t0 = (int) (r0 / a.G), t1 = (int) ((r1 - 1) / a.G);
-    const int64_t base = (int64_t) kv - n;
-    const int64_t cap  = (int64_t) a.cols * a.page;
+    const int     r0 = rt * BMN, r1 = min(n * a.G, r0 + BMN);  // T * G < 2^31 (checked)
+    const int     t0 = a.byG.div(r0), t1 = a.byG.div(r1 - 1);
+    const int     base = kv - n;
+    const int64_t cap  = min((int64_t) a.cols * a.page, (int64_t) INT32_MAX - kBN);
     Span          p;
-    p.hi = (int) max((int64_t) 0, min(base + t1 + 1, min(cap, (int64_t) INT32_MAX - kBN)));
-    p.lo = a.window > 0 ? (int) max((int64_t) 0, base + t0 - a.window + 1) : 0;
+    p.hi = (int) max((int64_t) 0, min((int64_t) base + t1 + 1, cap));
+    p.lo = a.window > 0 ? (int) max((int64_t) 0, (int64_t) base + t0 - a.window + 1) : 0;
     if (p.hi <= p.lo) {
         p.kt0 = p.nkv = 0;
         p.lo = p.hi = 0;
@@ -98,9 +114,7 @@ template <int BMN> __device__ __forceinline__ Span span_of(const PArgs & a, int 
     p.units = max(p.nkv, 1);
     return p;
 }
-template <int BMN> __device__ __forceinline__ int tiles_of(const PArgs & a, int n) {
-    return (int) (((int64_t) n * a.G + BMN - 1) / BMN);
-}
+template <int BMN> __device__ __forceinline__ int tiles_of(const PArgs & a, int n) { return (n * a.G + BMN - 1) / BMN; }
 
 // a CTA's walk over its part of the line; every role keeps its own
 struct Walk {
@@ -115,7 +129,7 @@ struct Walk {
 template <int BMN> __device__ __forceinline__ void walk_load(const PArgs & a, Walk & w) {
     w.r0 = row_at(a, w.s);
     w.n  = row_at(a, w.s + 1) - w.r0;
-    w.kv = a.kv_len[w.s];
+    w.kv = max(a.kv_len[w.s], 0);
 }
 template <int BMN> __device__ __forceinline__ void walk_item(const PArgs & a, Walk & w) {
     w.sp   = span_of<BMN>(a, w.n, w.kv, w.rt);
@@ -180,7 +194,7 @@ template <int D, int NT, bool PREC, bool Q8> struct Lay {
     static constexpr int misc   = bar + nbar * 8;
     static constexpr int total  = misc + 64;
     static constexpr int alloc  = total;  // dynamic shared memory starts on 1024 bytes (checked by the kernel)
-    static constexpr int threads = (kSmWarps + 2 + (Q8 ? 4 : 0)) * 32;
+    static constexpr int threads = (kSmWarps + 4 + (Q8 ? 4 : 0)) * 32;  // MMA and producers: the third warpgroup
     static_assert(alloc <= 232448, "shared memory");
     static_assert(NS * chunk >= kMaxSeqs * 8, "the plan's sums fit the ring");
 };
@@ -191,6 +205,15 @@ __device__ __forceinline__ void tma4(uint32_t dst, const CUtensorMap * m, int x,
         "[%6];" ::"r"(dst),
         "l"(m), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
         : "memory");
+}
+
+// One lane of a converged warp. Tensor-core and TMA instructions take their operands from uniform registers: issued
+// under elect in warp-uniform code they cost a few cycles each, under `lane == 0` the compiler has to loop over lanes
+// that might differ (measured: 190 cycles per product).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
 
 // A from tensor memory (K-major f16 pairs, lane = row)
@@ -315,7 +338,7 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
 
     if (tid == 0) {
         for (int i = 0; i < NS; i++) {
-            mbar_init(&kvfull[i], Q8 ? 4 : 1);
+            mbar_init(&kvfull[i], Q8 ? 4 : kProd);
             mbar_init(&kvempty[i], 1);
         }
         for (int i = 0; i < Ly::NR; i++) {
@@ -350,7 +373,7 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
             const int r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = n > 0 ? tiles_of<BMN>(a, n) : 0;
             int       u = 0;
             if (nt <= 2) {
-                const int kv = nt ? a.kv_len[s] : 0;
+                const int kv = nt ? max(a.kv_len[s], 0) : 0;
                 for (int rt = 0; rt < nt; rt++) u += span_of<BMN>(a, n, kv, rt).units;
             } else {
                 big[atomicAdd(nbg, 1)] = s;  // any order: each entry is worked out by itself
@@ -359,7 +382,7 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
         }
         __syncthreads();
         for (int b = warp; b < *nbg; b += blockDim.x / 32) {
-            const int s = big[b], r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = a.kv_len[s];
+            const int s = big[b], r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = max(a.kv_len[s], 0);
             int       u = 0;
             for (int rt = lane; rt < nt; rt += 32) u += span_of<BMN>(a, n, kv, rt).units;
             u = __reduce_add_sync(0xffffffffu, u);
@@ -398,7 +421,7 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                         const int     per = tot[s];
                         const int     h   = (int) (in / per);
                         int           off = (int) (in - (int64_t) h * per);
-                        const int     r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = a.kv_len[s];
+                        const int     r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = max(a.kv_len[s], 0);
                         for (int t0 = 0; t0 < nt; t0 += 32) {
                             const int u  = t0 + lane < nt ? span_of<BMN>(a, n, kv, t0 + lane).units : 0;
                             int       ic = u;
@@ -448,166 +471,9 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
         walk_item<BMN>(a, w);
     }
 
-    if (warp == kSmWarps + 1) {
-        // ---------------- producer ----------------
-        uint32_t  rc = 0;                 // chunks (q8_0: raw slots) so far
-        const int box = a.box;            // q8_0: at most kRawTok
-        const int nsub = kBN / box;       // boxes per 128 tokens: 2, 4 or 8
-        for (; active; active = walk_next<BMN>(a, w)) {
-            const int n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
-            const int32_t * row = reinterpret_cast<const int32_t *>(a.table + (int64_t) w.s * a.tstride);
-            // lane j: page and place of the tile's j-th box, -1 when no row sees it
-            auto entry = [&](int pos, int & in) -> int {
-                bool isk;
-                int  i;
-                at_pos<NT>(pos, n, isk, i);
-                const int tok = (kt + i) * kBN + lane * box;
-                in            = tok % a.page;
-                if (lane >= nsub || tok >= w.sp.hi || tok + box <= w.sp.lo) return -1;
-                const int pg = row[tok / a.page];
-                return pg < 0 || pg >= a.n_pages ? a.n_pages : pg;  // no page: outside the map, reads as zeros
-            };
-            int in_next = 0, e_next = n ? entry(0, in_next) : -1;
-            for (int pos = 0; pos < 2 * n; pos++) {
-                bool isk;
-                int  i;
-                at_pos<NT>(pos, n, isk, i);
-                const int e = e_next, in = in_next;
-                if (pos + 1 < 2 * n) e_next = entry(pos + 1, in_next);  // in flight during this tile's waits
-                if (e == a.n_pages) atomicExch(a.status, kErrPage);
-                const CUtensorMap * m = isk ? &mk : &mv;
-                if constexpr (Q8) {
-                    constexpr int NRAW = kBN / kRawTok;
-                    const int     per  = kRawTok / box;  // boxes per raw slot: 1 or 2
-#pragma unroll 1
-                    for (int r = 0; r < NRAW; r++, rc++) {
-                        const int slot = rc % Ly::NR;
-                        if (rc >= Ly::NR) wait_bar(&rempty[slot], (rc / Ly::NR - 1) & 1, a.status, bad);
-                        if (bad) break;
-                        const int      sub  = r * per + lane;
-                        const int      ee   = __shfl_sync(0xffffffffu, e, sub & 31);
-                        const int      ii   = __shfl_sync(0xffffffffu, in, sub & 31);
-                        const bool     go   = lane < per && ee >= 0;
-                        const uint32_t many = __popc(__ballot_sync(0xffffffffu, go));
-                        if (lane == 0) mbar_arrive_expect_tx(&rfull[slot], many * box * 272);
-                        __syncwarp();
-                        if (go) {
-                            tma4(smem_u32(sm + Ly::raw + slot * kRawB) + lane * box * 272, m, 0, ii, w.h, ee, &rfull[slot]);
-                        }
-                    }
-                } else {
-#pragma unroll 1
-                    for (int ch = 0; ch < CH; ch++, rc++) {
-                        const int slot = rc % NS;
-                        if (rc >= NS) wait_bar(&kvempty[slot], (rc / NS - 1) & 1, a.status, bad);
-                        if (bad) break;
-                        // boxes of the chunk: K all tokens and D / CH dims, V tokens 128 / CH and all dims
-                        const int  planes = isk ? D / 64 / CH : D / 64;
-                        const int  ns     = isk ? nsub : nsub / CH;
-                        const int  sub0   = isk ? 0 : ch * ns;
-                        const int  p0     = isk ? ch * planes : 0;
-                        const int  rows   = isk ? kBN : Ly::vtok;
-                        const int  sub = lane % ns, pl = lane / ns;  // at most 4 planes x 8 boxes
-                        const int  ee  = __shfl_sync(0xffffffffu, e, sub0 + sub);
-                        const int  ii  = __shfl_sync(0xffffffffu, in, sub0 + sub);
-                        const bool go  = pl < planes && ee >= 0;
-                        const uint32_t many = __popc(__ballot_sync(0xffffffffu, go));
-                        if (lane == 0) mbar_arrive_expect_tx(&kvfull[slot], many * box * 128);
-                        __syncwarp();
-                        if (go) {
-                            tma4(smem_u32(sm + Ly::ring + slot * Ly::chunk) + pl * rows * 128 + sub * box * 128, m,
-                                 (p0 + pl) * 64, ii, w.h, ee, &kvfull[slot]);
-                        }
-                    }
-                }
-            }
-        }
-        if (bad) {  // the loads in flight land before this CTA's shared memory goes
-            constexpr int ND = Q8 ? Ly::NR : NS;
-            for (uint32_t c = rc > ND ? rc - ND : 0; c < rc; c++) mbar_wait(&(Q8 ? rfull : kvfull)[c % ND], (c / ND) & 1);
-        }
-    } else if (warp == kSmWarps) {
-        // ---------------- MMA ----------------
-        if (lane == 0) {
-            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, kBN, kBM);
-            constexpr uint32_t idpv = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kMNMajor, D, kBM);
-            constexpr uint64_t sw   = 2ull << 61;
-            const uint32_t     qs   = smem_u32(sm + Ly::q), rs = smem_u32(sm + Ly::ring);
-            uint32_t           rc0 = 0, items = 0, pc[2] = { 0, 0 }, pvn = 0;
-            for (; active; active = walk_next<BMN>(a, w)) {
-                const int n = w.sp.nkv ? w.take : 0;
-                if (n == 0) continue;
-                const int  nq  = NT == 2 && (int64_t) w.n * a.G - (int64_t) w.rt * BMN > kBM ? 2 : 1;
-                wait_bar(q_full, items & 1, a.status, bad);
-                items++;
-                tc::fence_after();
-                auto qk = [&](int i, int q, bool last) {  // last: the tile's last product with this K
-                    const int      b = NT == 2 ? q : (i & 1);
-                    const uint32_t d = tS + 128 * b;
-#pragma unroll
-                    for (int ch = 0; ch < CH; ch++) {
-                        const uint32_t c = rc0 + k_pos<NT>(i) * CH + ch, slot = c % NS;
-                        wait_bar(&kvfull[slot], (c / NS) & 1, a.status, bad);
-                        tc::fence_after();
-                        const uint32_t kb = rs + slot * Ly::chunk;
-#pragma unroll
-                        for (int j = 0; j < D / CH / 16; j++) {
-                            const int      jj = ch * (D / CH / 16) + j;  // k-step over all dims
-                            const uint64_t bd = tc::sdesc(kb + (j >> 2) * (kBN * 128) + (j & 3) * 32, 16, 1024) | sw;
-#pragma unroll
-                            for (int part = 0; part < Ly::qparts; part++) {
-                                const uint32_t qa = qs + (q * Ly::qparts + part) * Ly::qtile + (jj >> 2) * (kBM * 128) + (jj & 3) * 32;
-                                tc::mma_f16(d, tc::sdesc(qa, 16, 1024) | sw, bd, idqk, (uint32_t) (jj > 0 || part > 0));
-                            }
-                        }
-                        if (last) tc::commit(&kvempty[slot]);
-                    }
-                    tc::commit(&s_full[b]);
-                };
-                auto pv = [&](int i, int q, bool last) {
-                    const int      b = NT == 2 ? q : (i & 1);
-                    const uint32_t p = tS + 128 * b, d = tO + q * D;
-                    wait_bar(&p_rdy[b], pc[b] & 1, a.status, bad);
-                    pc[b]++;
-#pragma unroll
-                    for (int ch = 0; ch < CH; ch++) {
-                        const uint32_t c = rc0 + v_pos<NT>(i, n) * CH + ch, slot = c % NS;
-                        wait_bar(&kvfull[slot], (c / NS) & 1, a.status, bad);
-                        tc::fence_after();
-                        const uint32_t vb = rs + slot * Ly::chunk;
-#pragma unroll
-                        for (int j = 0; j < Ly::vtok / 16; j++) {
-                            const int      jj = ch * (Ly::vtok / 16) + j;
-                            const uint64_t bd = tc::sdesc(vb + j * 2048, Ly::vtok * 128, 1024) | sw;
-#pragma unroll
-                            for (int part = 0; part < Ly::qparts; part++) {
-                                mma_f16_ta(d, p + part * 64 + jj * 8, bd, idpv, (uint32_t) (i > 0 || jj > 0 || part > 0));
-                            }
-                        }
-                        if (last) tc::commit(&kvempty[slot]);
-                    }
-                    tc::commit(&pv_done[NT == 2 ? q : (pvn++ & 1)]);
-                };
-                if constexpr (NT == 1) {
-                    qk(0, 0, true);
-                    for (int i = 0; i < n; i++) {
-                        if (i + 1 < n) qk(i + 1, 0, true);
-                        pv(i, 0, true);
-                    }
-                } else {
-                    for (int q = 0; q < nq; q++) qk(0, q, q == nq - 1);
-                    for (int i = 0; i < n; i++) {
-                        for (int q = 0; q < nq; q++) {
-                            pv(i, q, q == nq - 1);
-                            if (i + 1 < n) qk(i + 1, q, q == nq - 1);
-                        }
-                    }
-                }
-                rc0 += 2 * n * CH;
-            }
-        }
-        __syncwarp();
-    } else if (warp < kSmWarps) {
+    // registers go to the softmax warps (a row of scores each): the launch's 168 (q8_0: 128) per thread, shared out anew
+    if (warp < kSmWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q8 ? 160 : 200));
         // ---------------- softmax ----------------
         const int wg = warp >> 2, wq = warp & 3, row = 32 * wq + lane;  // row of the tile (tensor-memory lane)
         const int q    = NT == 2 ? wg : 0;                              // row tile
@@ -615,58 +481,73 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
         uint32_t  rc0 = 0, sc[2] = { 0, 0 }, pvc = 0, pvw = 0, turn = 0, items = 0;
         for (; active; active = walk_next<BMN>(a, w)) {
             const int     n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
-            const int64_t R  = (int64_t) w.n * a.G;
-            const int64_t rb = (int64_t) w.rt * BMN + q * kBM;      // first row of this tile
-            const int     rows = (int) max((int64_t) 0, min((int64_t) kBM, R - rb));
+            const int     R    = w.n * a.G;
+            const int     rb   = w.rt * BMN + q * kBM;              // first row of this tile
+            const int     rows = max(0, min(kBM, R - rb));
             const bool    mine = row < rows;                        // this thread's row exists
             const bool    some = 32 * wq < rows;                    // the warp has a row
             // Q rows to shared memory: 16-byte chunks of 8 dims, 128-byte swizzle
             if (n > 0) {
-                constexpr int per = D / 8;
-                const int     u0 = NT == 2 ? (tid & 127) : tid;
-#pragma unroll 4
-                for (int u = u0; u < kBM * per; u += NT == 2 ? 128 : 256) {
-                    const int r = u / per, c = u % per;
-                    uint4     hi = make_uint4(0, 0, 0, 0), lo = hi;
-                    if (r < rows) {
-                        const int64_t   rr  = rb + r;
-                        const int64_t   t   = w.r0 + rr / a.G;
-                        const int       h   = w.h * a.G + (int) (rr % a.G);
-                        const uint8_t * src = a.q + t * a.qnb1 + (int64_t) h * a.qnb2;
-                        if constexpr (PREC) {
-                            const float4 x0 = __ldg(reinterpret_cast<const float4 *>(src) + 2 * c);
-                            const float4 x1 = __ldg(reinterpret_cast<const float4 *>(src) + 2 * c + 1);
-                            const float  x[8] = { x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w };
-                            uint32_t     hw[4], lw[4];
+                constexpr int per = D / 8, step = (NT == 2 ? 128 : 256) / per;  // rows apart of a thread's chunks
+                const int     u0 = NT == 2 ? (tid & 127) : tid, c = u0 % per;
+                uint8_t *     d0 = sm + Ly::q + q * Ly::qparts * Ly::qtile + (c >> 3) * (kBM * 128);
+                // rows behind the last one repeat it: their scores and outputs go nowhere
+                auto source = [&](int r) {
+                    const int rr = rb + min(r, rows - 1), t = a.byG.div(rr), h = w.h * a.G + (rr - t * a.G);
+                    return a.q + (int64_t) (w.r0 + t) * a.qnb1 + (int64_t) h * a.qnb2;
+                };
+                auto dest = [&](int r) { return d0 + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
+                if (rows == 0) {
+                } else if constexpr (!PREC) {
+#pragma unroll
+                    for (int k = 0; k < kBM / step; k++) {
+                        const int r = u0 / per + k * step;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dest(r))), "l"(source(r) + 16 * c) : "memory");
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                } else {
+                    constexpr int UN = 4;  // rows in flight
+                    static_assert(kBM % (UN * step) == 0, "whole turns");
+#pragma unroll 1
+                    for (int k0 = 0; k0 < kBM / step; k0 += UN) {
+                        float4 x[UN][2];
+#pragma unroll
+                        for (int k = 0; k < UN; k++) {
+                            const float4 * src = reinterpret_cast<const float4 *>(source(u0 / per + (k0 + k) * step)) + 2 * c;
+                            x[k][0] = __ldg(src);
+                            x[k][1] = __ldg(src + 1);
+                        }
+#pragma unroll
+                        for (int k = 0; k < UN; k++) {
+                            const float f[8] = { x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w,
+                                                 x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w };
+                            uint32_t    hw[4], lw[4];
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const __half2 h2 = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-                                const __half2 l2 = __floats2half2_rn(x[2 * e] - __low2float(h2), x[2 * e + 1] - __high2float(h2));
+                                const __half2 h2 = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+                                const __half2 l2 = __floats2half2_rn(f[2 * e] - __low2float(h2), f[2 * e + 1] - __high2float(h2));
                                 hw[e] = *reinterpret_cast<const uint32_t *>(&h2);
                                 lw[e] = *reinterpret_cast<const uint32_t *>(&l2);
                             }
-                            hi = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                            lo = make_uint4(lw[0], lw[1], lw[2], lw[3]);
-                        } else {
-                            hi = __ldg(reinterpret_cast<const uint4 *>(src) + c);
+                            uint8_t * d = dest(u0 / per + (k0 + k) * step);
+                            *reinterpret_cast<uint4 *>(d)             = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                            *reinterpret_cast<uint4 *>(d + Ly::qtile) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
                         }
                     }
-                    uint8_t * d = sm + Ly::q + q * Ly::qparts * Ly::qtile + (c >> 3) * (kBM * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                    *reinterpret_cast<uint4 *>(d) = hi;
-                    if constexpr (PREC) *reinterpret_cast<uint4 *>(d + Ly::qtile) = lo;
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
             }
             // the row's visible tokens
-            const int pos = (int) ((int64_t) w.kv - w.n + (mine ? (rb + row) / a.G : 0));
+            const int tok = mine ? a.byG.div(rb + row) : 0;  // of the sequence's new ones
+            const int pos = w.kv - w.n + tok;
             const int vhi = mine ? min(pos + 1, w.sp.hi) : 0;
-            const int vlo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+            const int vlo = a.window > 0 ? max(w.sp.lo, (int) max((int64_t) INT32_MIN, (int64_t) pos - a.window + 1)) : 0;
             // tokens that every row of the tile sees: no masking there
-            const int pmin = (int) ((int64_t) w.kv - w.n + rb / a.G);
-            const int pmax = (int) ((int64_t) w.kv - w.n + (rb + max(rows, 1) - 1) / a.G);
-            const int ahi = min(pmin + 1, w.sp.hi), alo = a.window > 0 ? max(0, pmax - a.window + 1) : 0;
+            const int pmin = w.kv - w.n + a.byG.div(rb), pmax = w.kv - w.n + a.byG.div(rb + max(rows, 1) - 1);
+            const int ahi = min(pmin + 1, w.sp.hi);
+            const int alo = a.window > 0 ? (int) max((int64_t) 0, (int64_t) pmax - a.window + 1) : 0;
             float     m = -INFINITY, l = 0.0f;
             const bool run = NT == 1 || q == 0 || rows > 0;  // this warp group has units
             // waits until this row tile's first `upto` products P V are done, phase by phase: a parity wait must neither
@@ -812,13 +693,13 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                 l += rd[(wg ^ 1) * kBM + row];
             }
             const int     o0 = NT == 2 ? 0 : OC * wg;
-            const int64_t rr = rb + row;
+            const int     head = w.h * a.G + (rb + row - tok * a.G);
             const int     slot = 2 * blockIdx.x + (w.off == 0 ? 1 : 0);
             float         f    = 1.0f;
             if (whole) {
                 float L = l;
                 if (a.sinks && mine) {
-                    const float sk = a.sinks[w.h * a.G + (int) (rr % a.G)] * kLog2e;
+                    const float sk = a.sinks[head] * kLog2e;
                     // relative to the larger of the two maxima
                     if (sk > m) {
                         const float d = m == -INFINITY ? 0.0f : ex2(m - sk);
@@ -836,7 +717,7 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                 uint8_t * dst = a.dst;
                 float *   acc = a.part_acc;
                 if (mine) {
-                    dst += (int64_t) (w.h * a.G + (int) (rr % a.G)) * a.dnb1 + (w.r0 + rr / a.G) * a.dnb2;
+                    dst += (int64_t) head * a.dnb1 + (int64_t) (w.r0 + tok) * a.dnb2;
                     acc += ((int64_t) slot * a.prow + q * kBM + row) * D;
                 }
 #pragma unroll 1
@@ -884,14 +765,196 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                 const int64_t end = range[0] + (range[1] - range[0] - w.rem) + w.sp.units;
                 int           e   = blockIdx.x;
                 while (range[2] * (e + 1) / range[3] < end) e++;
-                a.desc[2 * blockIdx.x + 1] = make_int4((int) ((int64_t) w.rt * BMN), (int) min((int64_t) BMN, R - (int64_t) w.rt * BMN), 0, 0);
+                a.desc[2 * blockIdx.x + 1] = make_int4(w.rt * BMN, min(BMN, R - w.rt * BMN), 0, 0);
                 a.desc[2 * blockIdx.x]     = make_int4(e - (int) blockIdx.x + 1, w.h, w.r0, 0);
             }
             rc0 += 2 * n * CH;
         }
+    } else if (!Q8 || warp < kSmWarps + 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q8 ? 80 : 104));
+        if (Q8 ? warp == kSmWarps + 1 : warp > kSmWarps) {
+            // ---------------- producers ----------------
+            // f16: the boxes of a chunk are dealt over the lanes of three warps (a page of 16 tokens makes 16 boxes of
+            // 2 KB per chunk, and a warp issues one in some 150 cycles); each announces its own bytes
+            const int pw = warp - kSmWarps - 1;
+            uint32_t  rc = 0;                 // chunks (q8_0: raw slots) so far
+            const int box = a.box;            // q8_0: at most kRawTok
+            const int nsub = kBN / box;       // boxes per 128 tokens: 2, 4 or 8
+            for (; active; active = walk_next<BMN>(a, w)) {
+                const int n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
+                const int32_t * row = reinterpret_cast<const int32_t *>(a.table + (int64_t) w.s * a.tstride);
+                // lane j: page and place of the tile's j-th box, -1 when no row sees it
+                auto entry = [&](int pos, int & in) -> int {
+                    bool isk;
+                    int  i;
+                    at_pos<NT>(pos, n, isk, i);
+                    const int tok = (kt + i) * kBN + lane * box;
+                    if (lane >= nsub || tok >= w.sp.hi || tok + box <= w.sp.lo) return -1;
+                    const int pi = a.byPage.div(tok);
+                    in           = tok - pi * a.page;
+                    const int pg = row[pi];
+                    return pg < 0 || pg >= a.n_pages ? a.n_pages : pg;  // no page: outside the map, reads as zeros
+                };
+                int in_next = 0, e_next = n ? entry(0, in_next) : -1;
+                for (int pos = 0; pos < 2 * n; pos++) {
+                    bool isk;
+                    int  i;
+                    at_pos<NT>(pos, n, isk, i);
+                    const int e = e_next, in = in_next;
+                    if (pos + 1 < 2 * n) e_next = entry(pos + 1, in_next);  // in flight during this tile's waits
+                    if (e == a.n_pages) atomicExch(a.status, kErrPage);
+                    const CUtensorMap * m = isk ? &mk : &mv;
+                    if constexpr (Q8) {
+                        constexpr int NRAW = kBN / kRawTok;
+                        const int     per  = kRawTok / box;  // boxes per raw slot: 1 or 2
+#pragma unroll 1
+                        for (int r = 0; r < NRAW; r++, rc++) {
+                            const int slot = rc % (Ly::NR + !Q8);
+                            if (rc >= Ly::NR) wait_bar(&rempty[slot], (rc / Ly::NR - 1) & 1, a.status, bad);
+                            if (bad) break;
+                            const uint32_t seen = __ballot_sync(0xffffffffu, e >= 0) >> (r * per) & ((1u << per) - 1);
+                            if (elect_one()) mbar_arrive_expect_tx(&rfull[slot], __popc(seen) * box * 272);
+                            __syncwarp();
+                            for (int j = 0; j < per; j++) {
+                                const int ee = __shfl_sync(0xffffffffu, e, r * per + j);
+                                const int ii = __shfl_sync(0xffffffffu, in, r * per + j);
+                                if (ee >= 0 && elect_one()) {
+                                    tma4(smem_u32(sm + Ly::raw + slot * kRawB) + j * box * 272, m, 0, ii, w.h, ee, &rfull[slot]);
+                                }
+                                __syncwarp();
+                            }
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int ch = 0; ch < CH; ch++, rc++) {
+                            const int slot = rc % NS;
+                            if (rc >= NS) wait_bar(&kvempty[slot], (rc / NS - 1) & 1, a.status, bad);
+                            if (bad) break;
+                            // boxes of the chunk: K all tokens and D / CH dims, V tokens 128 / CH and all dims
+                            const int  planes = isk ? D / 64 / CH : D / 64;
+                            const int  ns     = isk ? nsub : nsub / CH;
+                            const int  sub0   = isk ? 0 : ch * ns;
+                            const int  p0     = isk ? ch * planes : 0;
+                            const int  rows   = isk ? kBN : Ly::vtok;
+                            const int      box0 = lane * kProd + pw;  // box and plane of this lane: at most 16 in all
+                            const int      j = box0 % ns, pl = box0 / ns;
+                            const int      ee = __shfl_sync(0xffffffffu, e, (sub0 + j) & 31);
+                            const int      ii = __shfl_sync(0xffffffffu, in, (sub0 + j) & 31);
+                            const bool     go = pl < planes && ee >= 0;
+                            const uint32_t many = __popc(__ballot_sync(0xffffffffu, go));
+                            if (lane == 0) mbar_arrive_expect_tx(&kvfull[slot], many * box * 128);
+                            __syncwarp();
+                            if (go) {
+                                tma4(smem_u32(sm + Ly::ring + slot * Ly::chunk) + pl * rows * 128 + j * box * 128, m,
+                                     (p0 + pl) * 64, ii, w.h, ee, &kvfull[slot]);
+                            }
+                            __syncwarp();
+                        }
+                    }
+                }
+            }
+            if (bad) {  // the loads in flight land before this CTA's shared memory goes
+                constexpr int ND = Q8 ? Ly::NR : NS;
+                for (uint32_t c = rc > ND ? rc - ND : 0; c < rc; c++) mbar_wait(&(Q8 ? rfull : kvfull)[c % ND], (c / ND) & 1);
+            }
+        } else if (warp == kSmWarps) {
+            // ---------------- MMA ----------------
+            // the warp walks together, one elected lane issues
+            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, kBN, kBM);
+            constexpr uint32_t idpv = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kMNMajor, D, kBM);
+            constexpr uint64_t sw   = 2ull << 61;
+            const uint64_t     qd0  = tc::sdesc(smem_u32(sm + Ly::q), 16, 1024) | sw;  // addresses step by bytes / 16
+            const uint64_t     kd0  = tc::sdesc(smem_u32(sm + Ly::ring), 16, 1024) | sw;
+            const uint64_t     vd0  = tc::sdesc(smem_u32(sm + Ly::ring), Ly::vtok * 128, 1024) | sw;
+            uint32_t           rc0 = 0, items = 0, pc0 = 0, pc1 = 0, pvn = 0;
+            for (; active; active = walk_next<BMN>(a, w)) {
+                const int n = __shfl_sync(0xffffffffu, w.sp.nkv ? w.take : 0, 0);
+                if (n == 0) continue;
+                const int nq = __shfl_sync(0xffffffffu, NT == 2 && w.n * a.G - w.rt * BMN > kBM ? 2 : 1, 0);
+                wait_bar(q_full, items & 1, a.status, bad);
+                items++;
+                tc::fence_after();
+                auto qk = [&](int i, int q, bool last) {  // last: the tile's last product with this K
+                    const int      b = NT == 2 ? q : (i & 1);
+                    const uint32_t d = tS + 128 * b;
+#pragma unroll
+                    for (int ch = 0; ch < CH; ch++) {
+                        const uint32_t c = rc0 + k_pos<NT>(i) * CH + ch, slot = c % NS;
+                        wait_bar(&kvfull[slot], (c / NS) & 1, a.status, bad);
+                        tc::fence_after();
+                        __syncwarp();
+                        if (elect_one()) {
+                            const uint64_t kd = kd0 + slot * (Ly::chunk / 16), qd = qd0 + q * (Ly::qparts * Ly::qtile / 16);
+#pragma unroll
+                            for (int j = 0; j < D / CH / 16; j++) {
+                                const int      jj = ch * (D / CH / 16) + j;  // k-step over all dims
+                                const uint64_t bd = kd + ((j >> 2) * (kBN * 128) + (j & 3) * 32) / 16;
+#pragma unroll
+                                for (int part = 0; part < Ly::qparts; part++) {
+                                    tc::mma_f16(d, qd + (part * Ly::qtile + (jj >> 2) * (kBM * 128) + (jj & 3) * 32) / 16, bd, idqk,
+                                                (uint32_t) (jj > 0 || part > 0));
+                                }
+                            }
+                            if (last) tc::commit(&kvempty[slot]);
+                            if (ch == CH - 1) tc::commit(&s_full[b]);
+                        }
+                        __syncwarp();
+                    }
+                };
+                auto pv = [&](int i, int q, bool last) {
+                    const int      b = NT == 2 ? q : (i & 1);
+                    const uint32_t p = tS + 128 * b, d = tO + q * D;
+                    uint32_t &     pc = b ? pc1 : pc0;
+                    wait_bar(&p_rdy[b], pc & 1, a.status, bad);
+                    pc++;
+#pragma unroll
+                    for (int ch = 0; ch < CH; ch++) {
+                        const uint32_t c = rc0 + v_pos<NT>(i, n) * CH + ch, slot = c % NS;
+                        wait_bar(&kvfull[slot], (c / NS) & 1, a.status, bad);
+                        tc::fence_after();
+                        __syncwarp();
+                        if (elect_one()) {
+                            const uint64_t vd = vd0 + slot * (Ly::chunk / 16);
+#pragma unroll
+                            for (int j = 0; j < Ly::vtok / 16; j++) {
+                                const int jj = ch * (Ly::vtok / 16) + j;
+#pragma unroll
+                                for (int part = 0; part < Ly::qparts; part++) {
+                                    mma_f16_ta(d, p + part * 64 + jj * 8, vd + j * 2048 / 16, idpv, (uint32_t) (i > 0 || jj > 0 || part > 0));
+                                }
+                            }
+                            if (last) tc::commit(&kvempty[slot]);
+                            if (ch == CH - 1) tc::commit(&pv_done[NT == 2 ? q : (pvn & 1)]);
+                        }
+                        __syncwarp();
+                    }
+                    pvn++;
+                };
+                if constexpr (NT == 1) {
+                    qk(0, 0, true);
+                    for (int i = 0; i < n; i++) {
+                        if (i + 1 < n) qk(i + 1, 0, true);
+                        pv(i, 0, true);
+                    }
+                } else {
+                    qk(0, 0, nq == 1);
+                    if (nq == 2) qk(0, 1, true);
+                    for (int i = 0; i < n; i++) {
+                        pv(i, 0, nq == 1);
+                        if (i + 1 < n) qk(i + 1, 0, nq == 1);
+                        if (nq == 2) {
+                            pv(i, 1, true);
+                            if (i + 1 < n) qk(i + 1, 1, true);
+                        }
+                    }
+                }
+                rc0 += 2 * n * CH;
+            }
+        }
     } else if constexpr (Q8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(104));
         // ---------------- converters (q8_0): raw rows -> f16 chunks ----------------
-        const int qr = warp - kSmWarps - 2;  // quarter of the row: dims 64 qr .. 64 qr + 63, one swizzled plane
+        const int qr = warp - kSmWarps - 4;  // quarter of the row: dims 64 qr .. 64 qr + 63, one swizzled plane
         uint32_t  rc = 0, rr = 0;            // chunks, raw slots so far
         for (; active; active = walk_next<BMN>(a, w)) {
             const int n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
@@ -939,9 +1002,13 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
     if (warp == kSmWarps) tc::tmem_free(tbase, 512);
 }
 
-// The records of an item cut between CTAs, joined in the order of the cuts; one warp per row. CTA c opens the item
-// (record 2c + 1), CTAs c + 1 .. c + parts - 1 go on with it (records 2(c + 1), 2(c + 2), ...).
+// The records of an item cut between CTAs, joined in the order of the cuts. CTA c opens the item (record 2c + 1), CTAs
+// c + 1 .. c + parts - 1 go on with it (records 2(c + 1), 2(c + 2), ...). A warp per row and 128 values of it, 16 records
+// in flight: the join is a few round trips to L2, whatever the number of parts.
 template <int D, bool F32> __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const __grid_constant__ PArgs a) {
+    constexpr int W  = D >= 128 ? 4 : 2;   // values per lane
+    constexpr int PP = D > 128 ? D / 128 : 1;  // pieces of a row
+    constexpr int MO = 16;                 // records in flight
     pdl_launch_dependents();
     pdl_wait();
     const int  c  = blockIdx.x;
@@ -949,8 +1016,9 @@ template <int D, bool F32> __global__ void __launch_bounds__(256) fa_paged_merge
     if (d0.x == 0) return;
     const int4 d1 = a.desc[2 * c + 1];
     const int  lane = threadIdx.x & 31;
-    for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < d1.y; row += gridDim.y * 8) {
-        const int rr = d1.x + row, h = d0.y * a.G + rr % a.G;
+    for (int job = blockIdx.y * 8 + (threadIdx.x >> 5); job < d1.y * PP; job += gridDim.y * 8) {
+        const int row = job / PP, piece = job % PP;
+        const int tok = a.byG.div(d1.x + row), h = d0.y * a.G + (d1.x + row - tok * a.G);
         auto      rec = [&](int p) { return (int64_t) (2 * (c + p) + (p == 0 ? 1 : 0)) * a.prow + row; };
         float     M   = -INFINITY;
         for (int p = lane; p < d0.x; p += 32) {
@@ -965,43 +1033,45 @@ template <int D, bool F32> __global__ void __launch_bounds__(256) fa_paged_merge
             M  = fmaxf(M, sk);
         }
         float L = sk > -INFINITY ? ex2(sk - M + kShift) : 0.0f;
-        float acc[D / 32];
+        float acc[W];
 #pragma unroll
-        for (int e = 0; e < D / 32; e++) acc[e] = 0.0f;
-#pragma unroll 4
-        for (int p = 0; p < d0.x; p++) {
-            const float2 v = __ldcg(a.part_ms + rec(p));
-            const float  w = v.y > 0.0f ? ex2(v.x - M) : 0.0f;
-            L              = fmaf(w, v.y, L);
-            const float * src = a.part_acc + rec(p) * D;
-            if constexpr (D >= 128) {
+        for (int e = 0; e < W; e++) acc[e] = 0.0f;
+        for (int p0 = 0; p0 < d0.x; p0 += MO) {
+            float x[MO][W];
 #pragma unroll
-                for (int e = 0; e < D / 128; e++) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(src) + 32 * e + lane);
-                    acc[4 * e]     = w > 0.0f ? fmaf(w, x.x, acc[4 * e]) : acc[4 * e];
-                    acc[4 * e + 1] = w > 0.0f ? fmaf(w, x.y, acc[4 * e + 1]) : acc[4 * e + 1];
-                    acc[4 * e + 2] = w > 0.0f ? fmaf(w, x.z, acc[4 * e + 2]) : acc[4 * e + 2];
-                    acc[4 * e + 3] = w > 0.0f ? fmaf(w, x.w, acc[4 * e + 3]) : acc[4 * e + 3];
+            for (int k = 0; k < MO; k++) {
+                if (p0 + k < d0.x) {
+                    const float * src = a.part_acc + rec(p0 + k) * D + piece * 128 + lane * W;
+                    if constexpr (W == 4) {
+                        const float4 f = __ldcg(reinterpret_cast<const float4 *>(src));
+                        x[k][0] = f.x; x[k][1] = f.y; x[k][2] = f.z; x[k][3] = f.w;
+                    } else {
+                        const float2 f = __ldcg(reinterpret_cast<const float2 *>(src));
+                        x[k][0] = f.x; x[k][1] = f.y;
+                    }
                 }
-            } else {
-                const float2 x = __ldcg(reinterpret_cast<const float2 *>(src) + lane);
-                acc[0]         = w > 0.0f ? fmaf(w, x.x, acc[0]) : acc[0];
-                acc[1]         = w > 0.0f ? fmaf(w, x.y, acc[1]) : acc[1];
+            }
+            const float2 v = lane < MO && p0 + lane < d0.x ? __ldcg(a.part_ms + rec(p0 + lane)) : make_float2(0.0f, 0.0f);
+            const float  w = v.y > 0.0f ? ex2(v.x - M) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < MO; k++) {
+                const float wk = __shfl_sync(0xffffffffu, w, k), lk = __shfl_sync(0xffffffffu, v.y, k);
+                if (wk > 0.0f) {  // a record without weight may hold anything
+                    L = fmaf(wk, lk, L);
+#pragma unroll
+                    for (int e = 0; e < W; e++) acc[e] = fmaf(wk, x[k][e], acc[e]);
+                }
             }
         }
         const float f   = L > 0.0f ? 1.0f / L : 0.0f;
-        uint8_t *   dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) (d0.z + rr / a.G) * a.dnb2;
-        constexpr int V = D >= 128 ? 4 : 2;  // values a lane holds side by side
+        uint8_t *   dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) (d0.z + tok) * a.dnb2;
+        const int   at  = piece * 128 + lane * W;
 #pragma unroll
-        for (int e = 0; e < D / 32; e += V) {
-            const int at = (e / V) * 32 * V + lane * V;
-#pragma unroll
-            for (int k = 0; k < V; k += 2) {
-                if constexpr (F32) {
-                    *reinterpret_cast<float2 *>(dst + 4 * (at + k)) = make_float2(acc[e + k] * f, acc[e + k + 1] * f);
-                } else {
-                    *reinterpret_cast<__half2 *>(dst + 2 * (at + k)) = __floats2half2_rn(acc[e + k] * f, acc[e + k + 1] * f);
-                }
+        for (int k = 0; k < W; k += 2) {
+            if constexpr (F32) {
+                *reinterpret_cast<float2 *>(dst + 4 * (at + k)) = make_float2(acc[k] * f, acc[k + 1] * f);
+            } else {
+                *reinterpret_cast<__half2 *>(dst + 2 * (at + k)) = __floats2half2_rn(acc[k] * f, acc[k + 1] * f);
             }
         }
     }
@@ -1043,7 +1113,7 @@ int launch_paged(srhpm_ctx * ctx, const PArgs & a, const CUtensorMap & mk, const
                                       stream, mk, mv, a));
     ctx->launches.fetch_add(1);
     if (st != SRHPM_OK) return st;
-    st = cuda_status(launch_k_pdl(fa_paged_merge_kernel<D, PREC>, dim3(ctx->num_sms, std::min(16, (a.prow + 7) / 8)),
+    st = cuda_status(launch_k_pdl(fa_paged_merge_kernel<D, PREC>, dim3(ctx->num_sms, std::min(16, (a.prow * (D > 128 ? 2 : 1) + 7) / 8)),
                                   dim3(256), 0, stream, a));
     ctx->launches.fetch_add(1);
     return st;
@@ -1063,7 +1133,7 @@ size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, i
 
 int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t wsize, cudaStream_t stream) {
     const int D = v.c.D, G = v.H / v.c.Hkv;
-    if (v.S > kMaxSeqs) return SRHPM_UNSUPPORTED;
+    if (v.S > kMaxSeqs || (int64_t) v.T * G + 2 * kBM > INT32_MAX) return SRHPM_UNSUPPORTED;
     if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.c.Hkv, D, v.S)) return SRHPM_ERR_WORKSPACE;
     const int NT = row_tiles(v.T, v.S, G, D);
     PArgs     a;
@@ -1086,6 +1156,8 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     a.Hkv     = v.c.Hkv;
     a.G       = G;
     a.window  = v.window;
+    a.byG     = FastDiv::of((uint32_t) G);
+    a.byPage  = FastDiv::of((uint32_t) v.c.page);
     a.qscale     = v.softcap != 0.0f ? v.scale / v.softcap : v.scale * kLog2e;
     a.softcap_l2 = v.softcap * kLog2e;
     a.sinks      = v.sinks;
