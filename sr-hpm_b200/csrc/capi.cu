@@ -714,7 +714,8 @@ int srhpm_flash_attn_paged_work_size(const srhpm_ctx * ctx, const srhpm_tensor *
     PagedCache c;
     const int  st = check_fa_paged(q, k_cache, k_cache, &c);
     if (st != SRHPM_OK) return st;
-    *size = fa_paged_work_size(ctx, (int) q->ne[1], (int) q->ne[2], c.Hkv, c.D, n_seqs);
+    *size = fa_paged_work_size(ctx, (int) q->ne[1], (int) q->ne[2], c.Hkv, c.D, n_seqs,
+                               c.type == SRHPM_TYPE_Q8_0 && q->type == SRHPM_TYPE_F32);
     return SRHPM_OK;
 }
 

@@ -19,7 +19,7 @@
 // device by every CTA itself, in its prologue: no planning launch.
 //
 // Roles: 8 softmax warps, 1 MMA warp, 3 producer warps (TMA boxes of at most 64 tokens x 64 dims, each within a page, into
-// a ring of 128-byte-swizzled chunks), and for a q8_0 cache 4 converter warps (raw rows by TMA into a second ring, d * q
+// a ring of 128-byte-swizzled chunks), and for a q8_0 cache 16 converter warps (raw rows by TMA into a second ring, d * q
 // rounded to f16 into the chunks). NT = 1: the 8 softmax warps halve the columns of one row tile and S has two buffers;
 // NT = 2 (head_dim <= 128): two row tiles share K/V, each with its own 4 softmax warps and buffer.
 #include <cuda.h>
@@ -45,6 +45,8 @@ constexpr int   kBM      = 128;    // rows of a tile
 constexpr int   kBN      = 128;    // tokens of a tile
 constexpr int   kSmWarps = 8;      // softmax warps
 constexpr int   kProd    = 3;      // producer warps (f16 cache)
+constexpr int   kConv    = 16;     // converter warps (q8_0 cache): K's two groups of four, then V's
+constexpr int   kFew     = 56;     // rows of a tile where sequences bring few (below)
 constexpr int   kMaxSeqs = 8192;
 constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s (a probe sleeps up to 4 us)
 constexpr int   kRawTok  = 32;     // tokens of a raw q8_0 slot
@@ -177,24 +179,28 @@ template <int NT> __device__ __forceinline__ void at_pos(int pos, int n, bool & 
 }
 
 // ---- shared memory -----------------------------------------------------------------------------------------------
-template <int D, int NT, bool PREC, bool Q8> struct Lay {
+template <int D, int NT, int BR, bool PREC, bool Q8> struct Lay {
     static constexpr int CH     = D == 256 ? 2 : 1;            // chunks of a K or V tile
     static constexpr int chunk  = kBN * D * 2 / CH;            // bytes: K 128 tokens x (D / CH) dims, V (128 / CH) tokens x D
     static constexpr int vtok   = kBN / CH;                    // tokens of a V chunk
-    static constexpr int qtile  = kBM * D * 2;                 // one part (hi or lo) of one row tile
+    static constexpr int qtile  = BR * D * 2;                  // one part (hi or lo) of one row tile
     static constexpr int qparts = PREC ? 2 : 1;
     static constexpr int q      = 0;                           // [NT][qparts][qtile]
     static constexpr int ring   = NT * qparts * qtile;
-    static constexpr int NS     = Q8 ? (PREC ? 2 : 3) : D == 256 ? (PREC ? 3 : 5) : D == 128 ? (PREC && NT == 2 ? 3 : 5) : 6;
+    // chunks in flight: what shared memory holds beside Q (at most 8); q8_0 gives the rest to the raw rows
+    static constexpr int room   = 232448 - 2400 - ring;
+    // q8_0: K has a ring of one tile (2 chunks), V one of 1 or 2 chunks, the raw rows the rest
+    static constexpr int NS     = !Q8 ? (room / chunk < 8 ? room / chunk : 8) : BR < 128 && !PREC ? 4 : 3;
     static constexpr int raw    = ring + NS * chunk;
-    static constexpr int NR     = Q8 ? (PREC ? 3 : 7) : 0;     // raw slots
+    static constexpr int NG     = !Q8 ? 0 : (room - NS * chunk) / (4 * kRawB) < 3 ? (room - NS * chunk) / (4 * kRawB) : 3;
+    static constexpr int NR     = 4 * NG;                      // raw slots: a ring of NG for each converter group
     static constexpr int red    = raw + NR * kRawB;            // f32 [2][2][128]
     static constexpr int bar    = red + 2 * 2 * kBM * 4;
     static constexpr int nbar   = 2 * NS + 2 * NR + 2 + 2 + 2 + 1;
     static constexpr int misc   = bar + nbar * 8;
     static constexpr int total  = misc + 64;
     static constexpr int alloc  = total;  // dynamic shared memory starts on 1024 bytes (checked by the kernel)
-    static constexpr int threads = (kSmWarps + 4 + (Q8 ? 4 : 0)) * 32;  // MMA and producers: the third warpgroup
+    static constexpr int threads = (kSmWarps + 4 + (Q8 ? kConv : 0)) * 32;  // MMA and producers: the third warpgroup
     static_assert(alloc <= 232448, "shared memory");
     static_assert(NS * chunk >= kMaxSeqs * 8, "the plan's sums fit the ring");
 };
@@ -263,38 +269,34 @@ __device__ __forceinline__ void wait_bar(uint64_t * bar, uint32_t parity, int32_
     atomicExch(status, kErrWaitFull);
 }
 
-// 64 q8_0 values (two blocks, 68 bytes from byte 68 qr of a row) to f16 = round(d * q): 8 words of 16 bytes, chunk c of
-// the token's 128-byte row at the swizzled place
-__device__ __forceinline__ void convert_q8(const uint8_t * row, int qr, uint8_t * dst_row, int t, bool zero) {
-    uint32_t w[20];
-    const uint4 * src = reinterpret_cast<const uint4 *>(row + 64 * qr);
+// 64 q8_0 values (two blocks, 68 bytes from byte 68 QR of a row) to f16 = round(d * q): the 128-byte row of a swizzled
+// plane, 16-byte chunk c at place c ^ (t & 7). The 80 bytes from 64 QR are read in 16-byte loads (rows of 272 bytes: no
+// bank conflicts across tokens); the quarter starts QR words into them.
+template <int QR> __device__ __forceinline__ void convert_q8(const uint8_t * row, uint8_t * dst_row, int t) {
+    uint32_t      w[20];
+    const uint4 * src = reinterpret_cast<const uint4 *>(row + 64 * QR);
 #pragma unroll
     for (int c = 0; c < 5; c++) {
         const uint4 u = src[c];
         w[4 * c] = u.x; w[4 * c + 1] = u.y; w[4 * c + 2] = u.z; w[4 * c + 3] = u.w;
     }
-    // the quarter starts qr words into the 80 bytes
-    uint32_t v[17];
-#pragma unroll
-    for (int i = 0; i < 17; i++) {
-        v[i] = qr == 0 ? w[i] : qr == 1 ? w[i + 1] : qr == 2 ? w[i + 2] : w[i + 3];
-    }
     const __half2 bias = __halves2half2(__ushort_as_half(0x6480u), __ushort_as_half(0x6480u));  // 1024 + 128
 #pragma unroll
     for (int bb = 0; bb < 2; bb++) {
-        const int      od    = 34 * bb;
-        const uint32_t dbits = (v[od >> 2] >> (8 * (od & 3))) & 0xffffu;
-        const __half2  dd    = __halves2half2(__ushort_as_half((unsigned short) dbits), __ushort_as_half((unsigned short) dbits));
-        uint32_t       f[16];
+        const int od = 4 * QR + 34 * bb;
+        uint32_t  dw;  // d twice
+        asm("prmt.b32 %0, %1, %1, %2;" : "=r"(dw) : "r"(w[od >> 2]), "r"((od & 3) ? 0x3232u : 0x1010u));
+        const __half2 dd = *reinterpret_cast<const __half2 *>(&dw);
+        uint32_t      f[16];
 #pragma unroll
         for (int m = 0; m < 16; m++) {
             const int      o  = od + 2 + 2 * m;  // even: the pair sits in one word
-            const uint32_t wx = v[o >> 2] ^ 0x80808080u;
+            const uint32_t wx = w[o >> 2] ^ 0x80808080u;
             uint32_t       mg;
             asm("prmt.b32 %0, %1, %2, %3;" : "=r"(mg) : "r"(wx), "r"(0x64u), "r"(((o >> 1) & 1) ? 0x4342u : 0x4140u));
             __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&mg), bias);  // exact: |q| <= 128
             h         = __hmul2(h, dd);
-            f[m]      = zero ? 0u : *reinterpret_cast<const uint32_t *>(&h);
+            f[m]      = *reinterpret_cast<const uint32_t *>(&h);
         }
 #pragma unroll
         for (int c = 0; c < 4; c++) {
@@ -304,12 +306,12 @@ __device__ __forceinline__ void convert_q8(const uint8_t * row, int qr, uint8_t 
     }
 }
 
-template <int D, int NT, bool PREC, bool Q8>
-__global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
+template <int D, int NT, int BR, bool PREC, bool Q8>
+__global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     fa_paged_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                     const __grid_constant__ PArgs a) {
-    using Ly           = Lay<D, NT, PREC, Q8>;
-    constexpr int BMN  = kBM * NT;
+    using Ly           = Lay<D, NT, BR, PREC, Q8>;
+    constexpr int BMN  = BR * NT;
     constexpr int CH   = Ly::CH;
     constexpr int NS   = Ly::NS;
     constexpr int NC   = NT == 2 ? 128 : 64;  // score columns per softmax thread
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
 
     if (tid == 0) {
         for (int i = 0; i < NS; i++) {
-            mbar_init(&kvfull[i], Q8 ? 4 : kProd);
+            mbar_init(&kvfull[i], Q8 ? kConv / 2 : kProd);
             mbar_init(&kvempty[i], 1);
         }
         for (int i = 0; i < Ly::NR; i++) {
@@ -471,9 +473,9 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
         walk_item<BMN>(a, w);
     }
 
-    // registers go to the softmax warps (a row of scores each): the launch's 168 (q8_0: 128) per thread, shared out anew
+    // registers go to the softmax warps (a row of scores each): the launch's 168 (q8_0: 72) per thread, shared out anew
     if (warp < kSmWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q8 ? 160 : 200));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q8 ? 128 : 200));
         // ---------------- softmax ----------------
         const int wg = warp >> 2, wq = warp & 3, row = 32 * wq + lane;  // row of the tile (tensor-memory lane)
         const int q    = NT == 2 ? wg : 0;                              // row tile
@@ -482,15 +484,15 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
         for (; active; active = walk_next<BMN>(a, w)) {
             const int     n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
             const int     R    = w.n * a.G;
-            const int     rb   = w.rt * BMN + q * kBM;              // first row of this tile
-            const int     rows = max(0, min(kBM, R - rb));
+            const int     rb   = w.rt * BMN + q * BR;               // first row of this tile
+            const int     rows = max(0, min(BR, R - rb));
             const bool    mine = row < rows;                        // this thread's row exists
             const bool    some = 32 * wq < rows;                    // the warp has a row
             // Q rows to shared memory: 16-byte chunks of 8 dims, 128-byte swizzle
             if (n > 0) {
                 constexpr int per = D / 8, step = (NT == 2 ? 128 : 256) / per;  // rows apart of a thread's chunks
                 const int     u0 = NT == 2 ? (tid & 127) : tid, c = u0 % per;
-                uint8_t *     d0 = sm + Ly::q + q * Ly::qparts * Ly::qtile + (c >> 3) * (kBM * 128);
+                uint8_t *     d0 = sm + Ly::q + q * Ly::qparts * Ly::qtile + (c >> 3) * (BR * 128);
                 // rows behind the last one repeat it: their scores and outputs go nowhere
                 auto source = [&](int r) {
                     const int rr = rb + min(r, rows - 1), t = a.byG.div(rr), h = w.h * a.G + (rr - t * a.G);
@@ -500,16 +502,16 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                 if (rows == 0) {
                 } else if constexpr (!PREC) {
 #pragma unroll
-                    for (int k = 0; k < kBM / step; k++) {
+                    for (int k = 0; k < (BR + step - 1) / step; k++) {
                         const int r = u0 / per + k * step;
+                        if (BR % step && r >= BR) break;
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dest(r))), "l"(source(r) + 16 * c) : "memory");
                     }
                     asm volatile("cp.async.wait_all;" ::: "memory");
                 } else {
-                    constexpr int UN = 4;  // rows in flight
-                    static_assert(kBM % (UN * step) == 0, "whole turns");
+                    constexpr int NK = (BR + step - 1) / step, UN = NK < 4 ? NK : 4;  // rows of a thread, in flight
 #pragma unroll 1
-                    for (int k0 = 0; k0 < kBM / step; k0 += UN) {
+                    for (int k0 = 0; k0 < NK; k0 += UN) {
                         float4 x[UN][2];
 #pragma unroll
                         for (int k = 0; k < UN; k++) {
@@ -529,7 +531,9 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                                 hw[e] = *reinterpret_cast<const uint32_t *>(&h2);
                                 lw[e] = *reinterpret_cast<const uint32_t *>(&l2);
                             }
-                            uint8_t * d = dest(u0 / per + (k0 + k) * step);
+                            const int r = u0 / per + (k0 + k) * step;
+                            if ((BR % (UN * step)) && r >= BR) break;
+                            uint8_t * d = dest(r);
                             *reinterpret_cast<uint4 *>(d)             = make_uint4(hw[0], hw[1], hw[2], hw[3]);
                             *reinterpret_cast<uint4 *>(d + Ly::qtile) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
                         }
@@ -711,14 +715,14 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                 }
                 f = L > 0.0f ? f / L : 0.0f;
             } else if (mine && (NT == 2 || wg == 0)) {
-                a.part_ms[(int64_t) slot * a.prow + q * kBM + row] = make_float2(m, l);
+                a.part_ms[(int64_t) slot * a.prow + q * BR + row] = make_float2(m, l);
             }
             if (some && run) {
                 uint8_t * dst = a.dst;
                 float *   acc = a.part_acc;
                 if (mine) {
                     dst += (int64_t) head * a.dnb1 + (int64_t) (w.r0 + tok) * a.dnb2;
-                    acc += ((int64_t) slot * a.prow + q * kBM + row) * D;
+                    acc += ((int64_t) slot * a.prow + q * BR + row) * D;
                 }
 #pragma unroll 1
                 for (int c = 0; c < OC; c += 32) {
@@ -771,11 +775,12 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
             rc0 += 2 * n * CH;
         }
     } else if (!Q8 || warp < kSmWarps + 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q8 ? 80 : 104));
-        if (Q8 ? warp == kSmWarps + 1 : warp > kSmWarps) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q8 ? 56 : 104));
+        if (warp > kSmWarps && (!Q8 || warp < kSmWarps + 3)) {
             // ---------------- producers ----------------
             // f16: the boxes of a chunk are dealt over the lanes of three warps (a page of 16 tokens makes 16 boxes of
             // 2 KB per chunk, and a warp issues one in some 150 cycles); each announces its own bytes
+            // q8_0: one warp brings K's raw rows, one V's
             const int pw = warp - kSmWarps - 1;
             uint32_t  rc = 0;                 // chunks (q8_0: raw slots) so far
             const int box = a.box;            // q8_0: at most kRawTok
@@ -787,7 +792,11 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                 auto entry = [&](int pos, int & in) -> int {
                     bool isk;
                     int  i;
-                    at_pos<NT>(pos, n, isk, i);
+                    if (Q8) {
+                        i = pos;
+                    } else {
+                        at_pos<NT>(pos, n, isk, i);
+                    }
                     const int tok = (kt + i) * kBN + lane * box;
                     if (lane >= nsub || tok >= w.sp.hi || tok + box <= w.sp.lo) return -1;
                     const int pi = a.byPage.div(tok);
@@ -795,22 +804,26 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                     const int pg = row[pi];
                     return pg < 0 || pg >= a.n_pages ? a.n_pages : pg;  // no page: outside the map, reads as zeros
                 };
-                int in_next = 0, e_next = n ? entry(0, in_next) : -1;
-                for (int pos = 0; pos < 2 * n; pos++) {
-                    bool isk;
+                int       in_next = 0, e_next = n ? entry(0, in_next) : -1;
+                const int npos = Q8 ? n : 2 * n;
+                for (int pos = 0; pos < npos; pos++) {
+                    bool isk = pw == 0;
                     int  i;
-                    at_pos<NT>(pos, n, isk, i);
+                    if constexpr (!Q8) at_pos<NT>(pos, n, isk, i);
                     const int e = e_next, in = in_next;
-                    if (pos + 1 < 2 * n) e_next = entry(pos + 1, in_next);  // in flight during this tile's waits
+                    if (pos + 1 < npos) e_next = entry(pos + 1, in_next);  // in flight during this tile's waits
                     if (e == a.n_pages) atomicExch(a.status, kErrPage);
                     const CUtensorMap * m = isk ? &mk : &mv;
                     if constexpr (Q8) {
-                        constexpr int NRAW = kBN / kRawTok;
+                        constexpr uint32_t NG   = Ly::NG;
+                        constexpr int      NRAW = kBN / kRawTok;
                         const int     per  = kRawTok / box;  // boxes per raw slot: 1 or 2
 #pragma unroll 1
                         for (int r = 0; r < NRAW; r++, rc++) {
-                            const int slot = rc % (Ly::NR + !Q8);
-                            if (rc >= Ly::NR) wait_bar(&rempty[slot], (rc / Ly::NR - 1) & 1, a.status, bad);
+                            // tokens 32 r ..: group r % 2 of K's or V's two
+                            const uint32_t own  = (rc >> 2) * 2 + (r >> 1);
+                            const int      slot = (pw * 2 + (r & 1)) * NG + own % NG;
+                            if (own >= NG) wait_bar(&rempty[slot], (own / NG - 1) & 1, a.status, bad);
                             if (bad) break;
                             const uint32_t seen = __ballot_sync(0xffffffffu, e >= 0) >> (r * per) & ((1u << per) - 1);
                             if (elect_one()) mbar_arrive_expect_tx(&rfull[slot], __popc(seen) * box * 272);
@@ -854,8 +867,14 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                 }
             }
             if (bad) {  // the loads in flight land before this CTA's shared memory goes
-                constexpr int ND = Q8 ? Ly::NR : NS;
-                for (uint32_t c = rc > ND ? rc - ND : 0; c < rc; c++) mbar_wait(&(Q8 ? rfull : kvfull)[c % ND], (c / ND) & 1);
+                if constexpr (Q8) {
+                    for (uint32_t c = rc > 2 * Ly::NG ? rc - 2 * Ly::NG : 0; c < rc; c++) {
+                        const uint32_t own = (c >> 2) * 2 + ((c & 3) >> 1);
+                        mbar_wait(&rfull[(pw * 2 + (c & 1)) * Ly::NG + own % Ly::NG], (own / Ly::NG) & 1);
+                    }
+                } else {
+                    for (uint32_t c = rc > NS ? rc - NS : 0; c < rc; c++) mbar_wait(&kvfull[c % NS], (c / NS) & 1);
+                }
             }
         } else if (warp == kSmWarps) {
             // ---------------- MMA ----------------
@@ -867,10 +886,24 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
             const uint64_t     kd0  = tc::sdesc(smem_u32(sm + Ly::ring), 16, 1024) | sw;
             const uint64_t     vd0  = tc::sdesc(smem_u32(sm + Ly::ring), Ly::vtok * 128, 1024) | sw;
             uint32_t           rc0 = 0, items = 0, pc0 = 0, pc1 = 0, pvn = 0;
+            // slot and use of a tile's chunk in the ring (rc0: chunks before the item; q8_0: tiles)
+            auto chunk_at = [&](bool isk, int i, int n, int ch, uint32_t & use) -> uint32_t {
+                uint32_t c;
+                if constexpr (Q8) {
+                    c = 2 * (rc0 + i) + ch;
+                    constexpr uint32_t nv = NS - 2;
+                    use = isk ? c / 2 : c / nv;
+                    return isk ? (uint32_t) ch : 2 + c % nv;
+                } else {
+                    c   = rc0 + (isk ? k_pos<NT>(i) : v_pos<NT>(i, n)) * CH + ch;
+                    use = c / NS;
+                    return c % NS;
+                }
+            };
             for (; active; active = walk_next<BMN>(a, w)) {
                 const int n = __shfl_sync(0xffffffffu, w.sp.nkv ? w.take : 0, 0);
                 if (n == 0) continue;
-                const int nq = __shfl_sync(0xffffffffu, NT == 2 && w.n * a.G - w.rt * BMN > kBM ? 2 : 1, 0);
+                const int nq = __shfl_sync(0xffffffffu, NT == 2 && w.n * a.G - w.rt * BMN > BR ? 2 : 1, 0);
                 wait_bar(q_full, items & 1, a.status, bad);
                 items++;
                 tc::fence_after();
@@ -879,8 +912,9 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                     const uint32_t d = tS + 128 * b;
 #pragma unroll
                     for (int ch = 0; ch < CH; ch++) {
-                        const uint32_t c = rc0 + k_pos<NT>(i) * CH + ch, slot = c % NS;
-                        wait_bar(&kvfull[slot], (c / NS) & 1, a.status, bad);
+                        uint32_t       use;
+                        const uint32_t slot = chunk_at(true, i, n, ch, use);
+                        wait_bar(&kvfull[slot], use & 1, a.status, bad);
                         tc::fence_after();
                         __syncwarp();
                         if (elect_one()) {
@@ -891,7 +925,7 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                                 const uint64_t bd = kd + ((j >> 2) * (kBN * 128) + (j & 3) * 32) / 16;
 #pragma unroll
                                 for (int part = 0; part < Ly::qparts; part++) {
-                                    tc::mma_f16(d, qd + (part * Ly::qtile + (jj >> 2) * (kBM * 128) + (jj & 3) * 32) / 16, bd, idqk,
+                                    tc::mma_f16(d, qd + (part * Ly::qtile + (jj >> 2) * (BR * 128) + (jj & 3) * 32) / 16, bd, idqk,
                                                 (uint32_t) (jj > 0 || part > 0));
                                 }
                             }
@@ -909,8 +943,9 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                     pc++;
 #pragma unroll
                     for (int ch = 0; ch < CH; ch++) {
-                        const uint32_t c = rc0 + v_pos<NT>(i, n) * CH + ch, slot = c % NS;
-                        wait_bar(&kvfull[slot], (c / NS) & 1, a.status, bad);
+                        uint32_t       use;
+                        const uint32_t slot = chunk_at(false, i, n, ch, use);
+                        wait_bar(&kvfull[slot], use & 1, a.status, bad);
                         tc::fence_after();
                         __syncwarp();
                         if (elect_one()) {
@@ -948,51 +983,65 @@ __global__ void __launch_bounds__(Lay<D, NT, PREC, Q8>::threads, 1)
                         }
                     }
                 }
-                rc0 += 2 * n * CH;
+                rc0 += Q8 ? n : 2 * n * CH;
             }
         }
     } else if constexpr (Q8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(104));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(48));
         // ---------------- converters (q8_0): raw rows -> f16 chunks ----------------
-        const int qr = warp - kSmWarps - 4;  // quarter of the row: dims 64 qr .. 64 qr + 63, one swizzled plane
-        uint32_t  rc = 0, rr = 0;            // chunks, raw slots so far
+        // warp = (K or V; group: every other 32 tokens; quarter of the row: dims 64 qr .. 64 qr + 63, one swizzled plane).
+        // A job is 32 tokens: wait, load, unpack, store and fence take 0.7 us for 250 instructions, so 16 warps work at
+        // once; K and V have chunks, raw rows and warps of their own, so that the next K does not queue behind a V that
+        // waits for its place (in one queue: 4.2 us per K and V tile). A group takes every use of its raw slots, and of
+        // the chunks that it fills, in order: a wait by parity must not skip one.
+        const int  qr = warp & 3, grp = ((warp - kSmWarps - 4) >> 2) & 1;
+        const bool isk = warp < kSmWarps + 4 + kConv / 2;
+        uint32_t   tile = 0;  // tiles so far
+        constexpr uint32_t NV = NS - 2;
         for (; active; active = walk_next<BMN>(a, w)) {
             const int n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
-            for (int pos = 0; pos < 2 * n; pos++) {
-                bool isk;
-                int  i;
-                at_pos<NT>(pos, n, isk, i);
-                const int t0 = (kt + i) * kBN;
+            for (int i = 0; i < n; i++, tile++) {
 #pragma unroll 1
-                for (int r = 0; r < kBN / kRawTok; r++, rr++) {
-                    // K: both chunks at the first raw slot; V: chunk r / 2 at its first
-                    if (isk ? r == 0 : (r & 1) == 0) {
-                        for (int c = isk ? 0 : r >> 1; c < (isk ? 2 : (r >> 1) + 1); c++) {
-                            const uint32_t k = rc + c;
-                            if (k >= NS) wait_bar(&kvempty[k % NS], (k / NS - 1) & 1, a.status, bad);
+                for (int r = 0; r < 2; r++) {  // the tile's tokens 32 (2 r + grp) ..
+                    const uint32_t own = 2 * tile + r;
+                    const int      slot = ((isk ? 0 : 2) + grp) * Ly::NG + own % Ly::NG;
+                    uint8_t *      dst;
+                    if (isk) {
+                        if (r == 0 && tile > 0) {
+                            wait_bar(&kvempty[0], (tile - 1) & 1, a.status, bad);
+                            wait_bar(&kvempty[1], (tile - 1) & 1, a.status, bad);
                         }
+                        dst = sm + Ly::ring + (qr >> 1) * Ly::chunk + (qr & 1) * (kBN * 128) + (32 * (2 * r + grp) + lane) * 128;
+                    } else {
+                        if (own >= NV) wait_bar(&kvempty[2 + own % NV], (own / NV - 1) & 1, a.status, bad);
+                        dst = sm + Ly::ring + (2 + own % NV) * Ly::chunk + qr * (64 * 128) + (32 * grp + lane) * 128;
                     }
-                    const int slot = rr % Ly::NR;
-                    wait_bar(&rfull[slot], (rr / Ly::NR) & 1, a.status, bad);
-                    const int  t    = kRawTok * r + lane;  // token of the tile
-                    const int  tk   = t0 + t;
-                    const bool zero = !isk && (tk < w.sp.lo || tk >= w.sp.hi);
-                    uint8_t *  dst  = isk ? sm + Ly::ring + ((rc + (qr >> 1)) % NS) * Ly::chunk + (qr & 1) * (kBN * 128) + t * 128
-                                          : sm + Ly::ring + ((rc + (r >> 1)) % NS) * Ly::chunk + qr * (64 * 128) + (t & 63) * 128;
-                    convert_q8(sm + Ly::raw + slot * kRawB + lane * 272, qr, dst, t, zero);
+                    wait_bar(&rfull[slot], (own / Ly::NG) & 1, a.status, bad);
+                    const uint8_t * src = sm + Ly::raw + slot * kRawB + lane * 272;
+                    switch (qr) {
+                        case 0: convert_q8<0>(src, dst, lane); break;
+                        case 1: convert_q8<1>(src, dst, lane); break;
+                        case 2: convert_q8<2>(src, dst, lane); break;
+                        default: convert_q8<3>(src, dst, lane); break;
+                    }
+                    // V rows that no row of the item sees hold anything; 0 * NaN is NaN, so they become zeros
+                    const int tok = (kt + i) * kBN + 32 * (2 * r + grp) + lane;
+                    if (!isk && (tok < w.sp.lo || tok >= w.sp.hi)) {
+#pragma unroll
+                        for (int c = 0; c < 8; c++) *reinterpret_cast<uint4 *>(dst + 16 * c) = make_uint4(0, 0, 0, 0);
+                    }
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(&rempty[slot]);
-                        if (isk && r == 3) {
-                            mbar_arrive(&kvfull[rc % NS]);
-                            mbar_arrive(&kvfull[(rc + 1) % NS]);
-                        } else if (!isk && (r & 1)) {
-                            mbar_arrive(&kvfull[(rc + (r >> 1)) % NS]);
+                        if (!isk) {
+                            mbar_arrive(&kvfull[2 + own % NV]);
+                        } else if (r == 1) {
+                            mbar_arrive(&kvfull[0]);
+                            mbar_arrive(&kvfull[1]);
                         }
                     }
                 }
-                rc += 2;
             }
         }
     }
@@ -1094,49 +1143,63 @@ EncodeTiled encode_fn() {
     return fn;
 }
 
-// row tiles per CTA: two share K/V (head_dim <= 128) where the sequences' rows fill more than one on average; with fewer
-// rows the second would be empty and one tile with two score buffers keeps the products and the softmax apart
-int row_tiles(int T, int S, int G, int D) { return D <= 128 && (int64_t) T * G > (int64_t) S * kBM ? 2 : 1; }
+// Rows of a CTA's tile by the sequences' average: at most kFew (decoding, verifying): one tile of kFew rows, whose Q takes
+// less than half the shared memory of 128 and leaves it to the K/V ring. The products still have M = 128: their upper rows
+// read what lies behind Q and go nowhere. kFew: what lets a q8_0 cache's rings (4 chunks, 8 raw slots) stand beside Q; it
+// holds 9 tokens of 6 heads. More: 128 rows, and with head_dim <= 128 two such tiles that share K/V. f32 rows over a q8_0
+// cache: always kFew (Q's two parts of 128 rows do not fit beside the rings).
+struct Tile {
+    int nt, br;
+};
+Tile tile_of(int T, int S, int G, int D, bool q8f32) {
+    if (q8f32 || (int64_t) T * G <= (int64_t) S * kFew) return { 1, kFew };
+    return { D <= 128 ? 2 : 1, 128 };
+}
 
-template <int D, int NT, bool PREC, bool Q8>
+template <int D, int NT, int BR, bool PREC, bool Q8>
 int launch_paged(srhpm_ctx * ctx, const PArgs & a, const CUtensorMap & mk, const CUtensorMap & mv, cudaStream_t stream) {
-    using Ly = Lay<D, NT, PREC, Q8>;
+    using Ly = Lay<D, NT, BR, PREC, Q8>;
+    auto                         kern = fa_paged_kernel<D, NT, BR, PREC, Q8>;
     static std::atomic<unsigned> done{ 0 };
     const unsigned               bit = 1u << (ctx->device & 31);
     if (!(done.load() & bit)) {
-        const int st = cuda_status(cudaFuncSetAttribute(fa_paged_kernel<D, NT, PREC, Q8>,
-                                                        cudaFuncAttributeMaxDynamicSharedMemorySize, Ly::alloc));
+        const int st = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Ly::alloc));
         if (st != SRHPM_OK) return st;
         done.fetch_or(bit);
     }
-    int st = cuda_status(launch_k_pdl(fa_paged_kernel<D, NT, PREC, Q8>, dim3(ctx->num_sms), dim3(Ly::threads), Ly::alloc,
-                                      stream, mk, mv, a));
+    int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms), dim3(Ly::threads), Ly::alloc, stream, mk, mv, a));
     ctx->launches.fetch_add(1);
     if (st != SRHPM_OK) return st;
-    st = cuda_status(launch_k_pdl(fa_paged_merge_kernel<D, PREC>, dim3(ctx->num_sms, std::min(16, (a.prow * (D > 128 ? 2 : 1) + 7) / 8)),
-                                  dim3(256), 0, stream, a));
+    st = cuda_status(launch_k_pdl(fa_paged_merge_kernel<D, PREC>,
+                                  dim3(ctx->num_sms, std::min(16, (a.prow * (D > 128 ? 2 : 1) + 7) / 8)), dim3(256), 0, stream, a));
     ctx->launches.fetch_add(1);
     return st;
 }
 
-int record_rows(int T, int G, int NT) { return (int) std::min<int64_t>((int64_t) kBM * NT, (int64_t) T * G); }
+template <int D, bool PREC, bool Q8>
+int launch_tile(srhpm_ctx * ctx, Tile t, const PArgs & a, const CUtensorMap & mk, const CUtensorMap & mv, cudaStream_t stream) {
+    if (t.br == kFew) return launch_paged<D, 1, kFew, PREC, Q8>(ctx, a, mk, mv, stream);
+    if constexpr (PREC && Q8) return SRHPM_ERR_INVALID;  // tile_of gives it kFew rows
+    else return launch_paged<D, D <= 128 ? 2 : 1, 128, PREC, Q8>(ctx, a, mk, mv, stream);
+}
+
+int record_rows(int T, int G, Tile t) { return (int) std::min<int64_t>((int64_t) t.br * t.nt, (int64_t) T * G); }
 
 size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
 }  // namespace
 
-size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S) {
-    const int    NT   = row_tiles(T, S, H / Hkv, D);
-    const size_t recs = (size_t) 2 * ctx->num_sms * record_rows(T, H / Hkv, NT);
+size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S, bool q8f32) {
+    const size_t recs = (size_t) 2 * ctx->num_sms * record_rows(T, H / Hkv, tile_of(T, S, H / Hkv, D, q8f32));
     return recs * D * sizeof(float) + align16(recs * sizeof(float2)) + 2 * (size_t) ctx->num_sms * sizeof(int4) + 16;
 }
 
 int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t wsize, cudaStream_t stream) {
     const int D = v.c.D, G = v.H / v.c.Hkv;
     if (v.S > kMaxSeqs || (int64_t) v.T * G + 2 * kBM > INT32_MAX) return SRHPM_UNSUPPORTED;
-    if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.c.Hkv, D, v.S)) return SRHPM_ERR_WORKSPACE;
-    const int NT = row_tiles(v.T, v.S, G, D);
-    PArgs     a;
+    if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.c.Hkv, D, v.S, v.f32 && v.c.type == SRHPM_TYPE_Q8_0)) return SRHPM_ERR_WORKSPACE;
+    const Tile tl = tile_of(v.T, v.S, G, D, v.f32 && v.c.type == SRHPM_TYPE_Q8_0);
+    PArgs      a;
     a.q       = v.q;
     a.qnb1    = v.qnb1;
     a.qnb2    = v.qnb2;
@@ -1161,7 +1224,7 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     a.qscale     = v.softcap != 0.0f ? v.scale / v.softcap : v.scale * kLog2e;
     a.softcap_l2 = v.softcap * kLog2e;
     a.sinks      = v.sinks;
-    a.prow       = record_rows(v.T, G, NT);
+    a.prow       = record_rows(v.T, G, tl);
     const size_t recs = (size_t) 2 * ctx->num_sms * a.prow;
     uint8_t *    wb   = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(wdata) + 15) & ~(uintptr_t) 15);
     a.part_acc = reinterpret_cast<float *>(wb);
@@ -1190,19 +1253,10 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
         if (r != CUDA_SUCCESS) return SRHPM_ERR_INVALID;
     }
-    if (q8) return v.f32 ? launch_paged<256, 1, true, true>(ctx, a, mk, mv, stream) : launch_paged<256, 1, false, true>(ctx, a, mk, mv, stream);
-    switch (D * 4 + NT * 2 - 2 + (v.f32 ? 1 : 0)) {
-        case 64 * 4: return launch_paged<64, 1, false, false>(ctx, a, mk, mv, stream);
-        case 64 * 4 + 1: return launch_paged<64, 1, true, false>(ctx, a, mk, mv, stream);
-        case 64 * 4 + 2: return launch_paged<64, 2, false, false>(ctx, a, mk, mv, stream);
-        case 64 * 4 + 3: return launch_paged<64, 2, true, false>(ctx, a, mk, mv, stream);
-        case 128 * 4: return launch_paged<128, 1, false, false>(ctx, a, mk, mv, stream);
-        case 128 * 4 + 1: return launch_paged<128, 1, true, false>(ctx, a, mk, mv, stream);
-        case 128 * 4 + 2: return launch_paged<128, 2, false, false>(ctx, a, mk, mv, stream);
-        case 128 * 4 + 3: return launch_paged<128, 2, true, false>(ctx, a, mk, mv, stream);
-        case 256 * 4: return launch_paged<256, 1, false, false>(ctx, a, mk, mv, stream);
-        default: return launch_paged<256, 1, true, false>(ctx, a, mk, mv, stream);
-    }
+    if (q8) return v.f32 ? launch_tile<256, true, true>(ctx, tl, a, mk, mv, stream) : launch_tile<256, false, true>(ctx, tl, a, mk, mv, stream);
+    if (D == 64) return v.f32 ? launch_tile<64, true, false>(ctx, tl, a, mk, mv, stream) : launch_tile<64, false, false>(ctx, tl, a, mk, mv, stream);
+    if (D == 128) return v.f32 ? launch_tile<128, true, false>(ctx, tl, a, mk, mv, stream) : launch_tile<128, false, false>(ctx, tl, a, mk, mv, stream);
+    return v.f32 ? launch_tile<256, true, false>(ctx, tl, a, mk, mv, stream) : launch_tile<256, false, false>(ctx, tl, a, mk, mv, stream);
 }
 
 }  // namespace srhpm

@@ -171,7 +171,7 @@ struct FaPagedView {
     uint8_t *       dst;
     int64_t         dnb1, dnb2;  // head, token
 };
-size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S);
+size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S, bool q8f32);
 int    fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t wsize, cudaStream_t stream);
 
 // verify_sample.cu: acceptance of drafted tokens by sampling

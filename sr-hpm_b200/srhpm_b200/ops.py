@@ -560,7 +560,7 @@ class Context:
         qv, kv = _head_rows(q, False), _paged(k_cache, kv_type)
         if work is None:
             work = self._scratch(self.lib.srhpm_flash_attn_paged_work_size, "srhpm_flash_attn_paged_work_size",
-                                 ("fa", q.shape, k_cache.shape, kv_type, S), stream, qv, kv, S)
+                                 ("fa", q.shape, q.dtype, k_cache.shape, kv_type, S), stream, qv, kv, S)
         sv = None
         if sinks is not None:
             at = _ints(sinks, torch.float32, q.shape[1], "sinks")
