@@ -360,7 +360,8 @@ int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_
  * rows, -1 in the rest of them; out_n i32 [n_seqs]: their count (accepted + 1; 0 for a sequence without rows); p_draft
  * f32 [T] or NULL: p_r(x) of each row with a drafted token, 0 for a last row. Padding rows of out_ids and p_draft stay
  * as they are. u_accept f32 [T], u_sample f32 [n_seqs], in [0, 1). The weights of a drawn token and their sums are
- * kept in 64 bits, so the token does not hang on the order of summation. n_vocab <= 2^29. wdata: srhpm_verify_sample_work_size bytes. */
+ * kept in 64 bits, so the token does not hang on the order of summation (a weight below 2^-990 of the row's largest
+ * counts as 0). n_vocab <= 2^29. wdata: srhpm_verify_sample_work_size bytes. */
 int srhpm_verify_sample_work_size(const srhpm_ctx * ctx, const srhpm_tensor * logits, int n_seqs, size_t * size);
 int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start,
                         int n_seqs, const srhpm_tensor * draft_probs, const float * temperature,

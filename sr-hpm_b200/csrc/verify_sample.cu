@@ -12,12 +12,14 @@
 //                        that emits. An accepted token is a comparison of two numbers, f32 exponentials (2^-22) do; a drawn
 //                        token is a place in a sum over the whole vocabulary: with V tokens and sums off by d, the place
 //                        moves in 2 V d of all draws, so 10^5 tokens want d well below 2^-30. Weights of that row and
-//                        their sums are taken in 64 bits. The row is split over the cluster in blocks of 128 tokens or
+//                        their sums are taken in 64 bits. The row is split over the cluster in blocks of 512 tokens or
 //                        more, in order; block sums, CTA sums and the sums inside one block find the place.
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "internal.h"
 #include "launch.cuh"
@@ -27,11 +29,10 @@ namespace srhpm {
 namespace {
 
 constexpr int   kPartThreads = 256;
-constexpr int   kPartVec     = 8;                              // 16-byte loads per thread
+constexpr int   kPartVec     = 4;                              // 16-byte loads per thread
 constexpr int   kSeg         = kPartThreads * kPartVec * 4;    // tokens per record
 constexpr int   kPickThreads = 512;
 constexpr int   kPickWarps   = kPickThreads / 32;
-constexpr int   kCluster     = 8;
 constexpr int   kMaxBlocks   = 1024;                           // blocks of a CTA's share
 constexpr float kLog2e       = 1.4426950408889634f;
 
@@ -140,35 +141,50 @@ __global__ void __launch_bounds__(kPartThreads) sample_part_kernel(const SampleA
     }
 }
 
-// exp((x - m) / t) in 64 bits, x <= m: 2^(k/32) from a table of 32 values times a polynomial of degree 6 in
-// |r| <= ln 2 / 64 (its rest: r^7 / 7! < 2^-57). Far cheaper than the full-range function and good to a few 2^-53.
+// exp((x - m) / t) in 64 bits, x <= m, as 2^y, y = x (log2 e / t) - m (log2 e / t) = k + f with |f| <= 1/2: 2^f by the series
+// of exp(f ln 2) up to the 11th power (its rest: (ln 2 / 2)^12 / 12! < 2^-45), k added to the exponent. 16 instructions of
+// 64 bits, no table and no branches: these are what a drawn token costs. Weights below e^-690 of the row's largest are 0.
 struct Exp64 {
-    double         m, inv_t;  // inv_t 0: all weight on `top`
-    float          mf;
-    int            top;
-    const double * tab;
-    __device__ __forceinline__ double operator()(float x, int j) const {
-        if (inv_t == 0.0) return j == top ? 1.0 : 0.0;
-        if (x == mf) return 1.0;
-        const double d = ((double) x - m) * inv_t;
-        if (!(d > -745.0)) return 0.0;  // below the smallest number (and -inf)
-        const double kk = rint(d * 46.16624130844683);  // 32 / ln 2
-        const int    k  = (int) kk;
-        // ln 2 / 32 in two parts, the first of 36 bits: |kk| < 2^16 times it is exact
-        double r = fma(kk, -0.021660849392446835, d);
-        r        = fma(kk, -5.145609244655338e-14, r);
-        double p = 1.0 / 720.0;
-        p = fma(p, r, 1.0 / 120.0);
-        p = fma(p, r, 1.0 / 24.0);
-        p = fma(p, r, 1.0 / 6.0);
-        p = fma(p, r, 0.5);
-        p = fma(p, r, 1.0);
-        p = fma(p, r, 1.0);
-        const int    e = k >> 5;  // power of two, down to -1075
-        const double s = tab[k & 31] * p;
-        // in two steps below the normal range
-        return e > -1022 ? s * __hiloint2double((1023 + e) << 20, 0)
-                         : s * __hiloint2double((1023 + e + 600) << 20, 0) * __hiloint2double((1023 - 600) << 20, 0);
+    double a, b;   // y = a x + b
+    float  least;  // x below it: 0
+    float  mf;
+    int    top, mode;  // 0: as above; 1: the maximum is +inf, all weight on those; 2: all weight on `top`
+    __device__ __forceinline__ void set(float m, int t, float temp) {
+        mf   = m;
+        top  = t;
+        mode = !(temp > 0.0f) ? 2 : m == INFINITY ? 1 : 0;
+        a    = mode == 0 ? 1.4426950408889634 / (double) temp : 0.0;
+        b    = mode == 0 && m > -INFINITY ? -(double) m * a : 0.0;
+        least = mode == 0 ? m - 690.0f * temp : 0.0f;
+    }
+    template <bool ZERO> __device__ __forceinline__ double of(float x) const {
+        const double y = fma((double) fmaxf(x, least), a, b);
+        const double t = y + 6755399441055744.0;  // rounds to a whole number
+        const double f = y - (t - 6755399441055744.0);
+        double       p = fma(f, 4.4455382718708116e-10, 7.054911620801123e-09);
+        p        = fma(p, f, 1.01780860092397e-07);
+        p        = fma(p, f, 1.321548679014431e-06);
+        p        = fma(p, f, 1.5252733804059841e-05);
+        p        = fma(p, f, 0.0001540353039338161);
+        p        = fma(p, f, 0.0013333558146428443);
+        p        = fma(p, f, 0.009618129107628477);
+        p        = fma(p, f, 0.05550410866482158);
+        p        = fma(p, f, 0.24022650695910072);
+        p        = fma(p, f, 0.6931471805599453);
+        p        = fma(p, f, 1.0);
+        p = __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+        return !ZERO || x >= least ? p : 0.0;
+    }
+    // weights of tokens j .. j + 3; mode is the same for the whole row. Without ZERO e^-690 stands for smaller ones: nothing
+    // to a sum of weights up to 1, but a token that is drawn must have one
+    template <bool ZERO> __device__ __forceinline__ void four(const float (&x)[4], int j, double (&w)[4]) const {
+        if (mode == 0) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = of<ZERO>(x[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = (mode == 1 ? x[e] == mf : j + e == top) ? 1.0 : 0.0;
+        }
     }
 };
 
@@ -184,13 +200,13 @@ __device__ __forceinline__ double ld_dsmem_f64(uint32_t addr) {
     return v;
 }
 
-__global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(const SampleArgs a) {
+template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sample_pick_kernel(const SampleArgs a) {
     const SampleView & v = a.v;
-    __shared__ double  tab[32], bsum[kMaxBlocks], share[2], wred[kPickWarps];
+    __shared__ double  bsum[kMaxBlocks], qsum[kMaxBlocks], share[3], wred[kPickWarps];
     __shared__ float   row_m[kPickWarps];
+    __shared__ double  row_z[kPickWarps];
     __shared__ int     row_top[kPickWarps], row_ok[kPickWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = blockIdx.x % kCluster, s = blockIdx.x / kCluster;
-    if (threadIdx.x < 32) tab[threadIdx.x] = exp2((double) threadIdx.x / 32.0);
     pdl_launch_dependents();
     pdl_wait();
     __syncthreads();
@@ -200,16 +216,14 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(const SampleA
         return;
     }
     const float  tf    = v.temp ? v.temp[s] : 1.0f;
-    const double inv_t = tf > 0.0f ? 1.0 / (double) tf : 0.0;
     const float  c     = tf > 0.0f ? kLog2e / tf : 0.0f;
 
     // ---- acceptance: a warp per row, kPickWarps rows at a time; every CTA of the cluster decides for itself
     Exp64 ex;
-    ex.tab   = tab;
-    ex.inv_t = inv_t;
     int    pick = -1;  // the row that emits
     float  pm = 0.0f;
     int    ptop = 0;
+    double pz = 0.0;  // its sum from the f32 records
     for (int b = r0; b < r1; b += kPickWarps) {
         const int r = b + warp;
         if (r < r1) {
@@ -238,22 +252,26 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(const SampleA
                 const float pm_ = __int_as_float(p.x);
                 if (pm_ > -INFINITY) z += (pm_ == m ? 1.0 : (double) exp2f((pm_ - m) * c)) * (double) __int_as_float(p.y);
             }
-            z = warp_sum(z);
+            z = tf > 0.0f ? warp_sum(z) : 1.0;
             if (m == -INFINITY) top = 0;
-            ex.m   = (double) m;
-            ex.mf  = m;
-            ex.top = top;
+            ex.set(m, top, tf);
             const bool last = r == r1 - 1;
             const int  x    = last ? -1 : v.ids[r + 1];
             double     p = 0.0, q = 0.0;
             if (x >= 0 && x < v.V) {
                 const float l = clean(reinterpret_cast<const float *>(v.logits + (int64_t) r * v.ldb)[x]);
-                if (m > -INFINITY) p = inv_t == 0.0 ? (x == top ? 1.0 : 0.0) : ex(l, x) / z;
+                if (m > -INFINITY) {
+                    const float l4[4] = { l, l, l, l };
+                    double      w4[4];
+                    ex.four<true>(l4, x, w4);
+                    p = w4[0] / z;
+                }
                 q = v.dprobs ? (double) reinterpret_cast<const float *>(v.dprobs + (int64_t) r * v.dldb)[x] : 1.0;
             }
             if (lane == 0) {
                 row_m[warp]   = m;
                 row_top[warp] = top;
+                row_z[warp]   = z;
                 row_ok[warp]  = !last && (double) v.u[r] * q < p;
                 if (rank == 0 && v.p_draft) v.p_draft[r] = (float) p;
             }
@@ -265,6 +283,7 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(const SampleA
                     pick = b + w;
                     pm   = row_m[w];
                     ptop = row_top[w];
+                    pz   = row_z[w];
                     break;
                 }
             }
@@ -284,22 +303,26 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(const SampleA
     const float * row  = reinterpret_cast<const float *>(v.logits + (int64_t) pick * v.ldb);
     const float * qr   = !last && v.dprobs ? reinterpret_cast<const float *>(v.dprobs + (int64_t) pick * v.dldb) : nullptr;
     const bool    vec  = (reinterpret_cast<uintptr_t>(row) & 15) == 0, qvec = (reinterpret_cast<uintptr_t>(qr) & 15) == 0;
-    const int     len  = 128 * (int) (((int64_t) v.V + (int64_t) kCluster * kMaxBlocks * 128 - 1) / ((int64_t) kCluster * kMaxBlocks * 128));
+    // blocks of 512 tokens, 16 per lane, pay for the sums across the lanes and the loop; of 128 where a warp would have
+    // no more than two of those; longer ones where kMaxBlocks would not do
+    const int     few = (int64_t) v.V <= (int64_t) kCluster * kPickWarps * 1024 ? 128 : 512;
+    const int     len = few == 128 ? 128 : 512 * (int) (((int64_t) v.V + (int64_t) kCluster * kMaxBlocks * 512 - 1) / ((int64_t) kCluster * kMaxBlocks * 512));
     const int     nblk = (int) (((int64_t) v.V + len - 1) / len), per = (nblk + kCluster - 1) / kCluster;
     const int     g0 = min(nblk, rank * per), g1 = min(nblk, g0 + per);
     const bool    none = pm == -INFINITY;
-    ex.m   = (double) pm;
-    ex.mf  = pm;
-    ex.top = ptop;
+    ex.set(pm, ptop, tf);
     double inv_z = 1.0;
-    auto weights = [&](int j, double (&w)[4]) {  // tokens j .. j + 3
-        float l[4];
-        load4(row, vec, j, v.V, -INFINITY, l);
-        float q[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+    auto logits4 = [&](int j, float (&l)[4]) { load4(row, vec, j, v.V, -INFINITY, l); };
+    auto drafts4 = [&](int j, float (&q)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[e] = 0.0f;
         if (qr) load4(qr, qvec, j, v.V, 0.0f, q);
+    };
+    auto weights = [&](int j, const float (&l)[4], const float (&q)[4], double (&w)[4]) {  // tokens j .. j + 3
+        ex.four<true>(l, j, w);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            w[e] = none || j + e >= v.V ? 0.0 : ex(l[e], j + e);
+            if (none || j + e >= v.V) w[e] = 0.0;
             if (qr) {
                 w[e] = fmax(w[e] * inv_z - (double) q[e], 0.0);
             } else if (j + e == x) {
@@ -308,45 +331,100 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(const SampleA
         }
     };
     auto cluster_get = [&](int i, int r) { return ld_dsmem_f64(mapa_shared(smem_u32(&share[i]), r)); };
-    if (qr) {  // the row's sum in 64 bits: weights are differences of probabilities
-        double z = 0.0;
-        for (int g = g0 + warp; g < g1; g += kPickWarps) {
-            for (int k = lane * 4; k < len; k += 128) {
-                const int j = g * len + k;
-                float     l[4];
-                load4(row, vec, j, v.V, -INFINITY, l);
+    // One pass over the share gives the row's sum Z, and per block the sums of e and of q over the tokens with e / Z > q,
+    // told apart by the f32 records' Z: a token on the wrong side has |e / Z - q| below 2^-20 of either, and few are that
+    // near, so the block's weight (sum e) / Z - sum q is as good as its terms.
+    {
+        const float pzf = (float) pz;
+        double      sz = 0.0;
+        auto block = [&](auto pieces, int at, double & se, double & sq) {  // `pieces` times 128 tokens from `at`
+            constexpr int P = decltype(pieces)::value;
+            float         l[P][4], q[P][4];
+            const int     j0 = at + lane * 4;
+            if (vec && qvec && at + P * 128 <= v.V) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) z += none || j + e >= v.V ? 0.0 : ex(l[e], j + e);
+                for (int k = 0; k < P; k++) {
+                    const float4 f = __ldcs(reinterpret_cast<const float4 *>(row + j0) + 32 * k);
+                    l[k][0] = f.x; l[k][1] = f.y; l[k][2] = f.z; l[k][3] = f.w;
+                }
+#pragma unroll
+                for (int k = 0; k < P; k++) {
+                    const float4 f = qr ? __ldcs(reinterpret_cast<const float4 *>(qr + j0) + 32 * k) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    q[k][0] = f.x; q[k][1] = f.y; q[k][2] = f.z; q[k][3] = f.w;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < P; k++) {
+                    logits4(j0 + 128 * k, l[k]);
+                    drafts4(j0 + 128 * k, q[k]);
+                }
+            }
+            if (lane < 4 * P) {  // the warp's next block on its way to L2
+                const int64_t next = min((int64_t) at + (int64_t) kPickWarps * len + 32 * lane, (int64_t) v.V - 1);
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(row + next));
+                if (qr) asm volatile("prefetch.global.L2 [%0];" ::"l"(qr + next));
+            }
+            const bool ragged = none || at + P * 128 > v.V;
+#pragma unroll
+            for (int k = 0; k < P; k++) {
+                const int j = j0 + 128 * k;
+                double    w[4];
+                ex.four<false>(l[k], j, w);
+                if (ragged) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w[e] = none || j + e >= v.V ? 0.0 : w[e];
+                }
+                if (qr) {
+                    sz += (w[0] + w[1]) + (w[2] + w[3]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool over = ex.mode == 0 ? fast_ex2((l[k][e] - pm) * c) > q[k][e] * pzf : w[e] > (double) q[k][e] * pz;
+                        se += over ? w[e] : 0.0;
+                        sq += (double) (over ? q[k][e] : 0.0f);
+                    }
+                } else {
+                    if (x >= j && x < j + 4) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[e] = j + e == x ? 0.0 : w[e];
+                    }
+                    se += (w[0] + w[1]) + (w[2] + w[3]);
+                }
+            }
+        };
+        for (int g = g0 + warp; g < g1; g += kPickWarps) {
+            double se = 0.0, sq = 0.0;
+            if (len == 128) {
+                block(std::integral_constant<int, 1>{}, g * 128, se, sq);
+            } else {
+                for (int k = 0; k < len; k += 512) block(std::integral_constant<int, 4>{}, g * len + k, se, sq);
+            }
+            se = warp_sum(se);
+            if (qr) sq = warp_sum(sq);
+            if (lane == 0) {
+                bsum[g - g0] = se;
+                qsum[g - g0] = sq;
             }
         }
-        z = warp_sum(z);
-        if (lane == 0) wred[warp] = z;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            double t = 0.0;
-            for (int w = 0; w < kPickWarps; w++) t += wred[w];
-            share[0] = t;
+        if (qr) {
+            sz = warp_sum(sz);
+            if (lane == 0) wred[warp] = sz;
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                double t = 0.0;
+                for (int w = 0; w < kPickWarps; w++) t += wred[w];
+                share[0] = t;
+            }
+            cluster_sync_all();
+            sz = 0.0;
+            for (int r = 0; r < kCluster; r++) sz += cluster_get(0, r);
+            inv_z = sz > 0.0 ? 1.0 / sz : 0.0;
         }
-        cluster_sync_all();
-        z = 0.0;
-        for (int r = 0; r < kCluster; r++) z += cluster_get(0, r);
-        inv_z = z > 0.0 ? 1.0 / z : 0.0;
-    }
-    for (int g = g0 + warp; g < g1; g += kPickWarps) {
-        double t = 0.0;
-        for (int k = lane * 4; k < len; k += 128) {
-            double w[4];
-            weights(g * len + k, w);
-            t += (w[0] + w[1]) + (w[2] + w[3]);
-        }
-        t = warp_sum(t);
-        if (lane == 0) bsum[g - g0] = t;
     }
     __syncthreads();
     if (warp == 0) {  // inclusive sums of the blocks
         double before = 0.0;
         for (int b = 0; b < g1 - g0; b += 32) {
-            double t = b + lane < g1 - g0 ? bsum[b + lane] : 0.0;
+            double t = b + lane < g1 - g0 ? (qr ? fmax(bsum[b + lane] * inv_z - qsum[b + lane], 0.0) : bsum[b + lane]) : 0.0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const double u = __shfl_up_sync(0xffffffffu, t, o);
@@ -403,8 +481,11 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(const SampleA
             int    at = -1, lastw = -1;
             for (int k = 0; k < len && at < 0; k += 128) {
                 const int j = (g0 + blk) * len + k + lane * 4;
+                float     l[4], q[4];
                 double    w[4];
-                weights(j, w);
+                logits4(j, l);
+                drafts4(j, q);
+                weights(j, l, q, w);
                 double t4 = (w[0] + w[1]) + (w[2] + w[3]), inc = t4;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -426,10 +507,38 @@ __global__ void __launch_bounds__(kPickThreads) sample_pick_kernel(const SampleA
                 if (mine != INT32_MAX) at = mine;
                 start += __shfl_sync(0xffffffffu, inc, 31);
             }
-            if (lane == 0) v.out_ids[pick] = at >= 0 ? at : lastw;
+            if (lane == 0) v.out_ids[pick] = at >= 0 ? at : lastw >= 0 ? lastw : ptop;
         }
     }
     cluster_sync_all();  // no CTA leaves while another reads its sums
+}
+
+template <int CL> int launch_pick(srhpm_ctx * ctx, const SampleArgs & a, cudaStream_t stream) {
+    if (CL > 8) {
+        static std::atomic<unsigned> done{ 0 };
+        const unsigned               bit = 1u << (ctx->device & 31);
+        if (!(done.load() & bit)) {
+            const int st = cuda_status(cudaFuncSetAttribute(sample_pick_kernel<CL>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            if (st != SRHPM_OK) return st;
+            done.fetch_or(bit);
+        }
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim            = dim3((unsigned) a.v.S * CL);
+    cfg.blockDim           = dim3(kPickThreads);
+    cfg.stream             = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id                                         = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x                           = CL;
+    attr[1].val.clusterDim.y                           = 1;
+    attr[1].val.clusterDim.z                           = 1;
+    cfg.attrs                                          = attr;
+    cfg.numAttrs                                       = 2;
+    const int st = cuda_status(cudaLaunchKernelEx(&cfg, sample_pick_kernel<CL>, a));
+    ctx->launches.fetch_add(1);
+    return st;
 }
 
 }  // namespace
@@ -448,22 +557,12 @@ int verify_sample_run(srhpm_ctx * ctx, const SampleView & v, void * wdata, size_
     int st = cuda_status(launch_k_pdl(sample_part_kernel, dim3(v.T, a.nseg), dim3(kPartThreads), 0, stream, a));
     ctx->launches.fetch_add(1);
     if (st != SRHPM_OK) return st;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim            = dim3((unsigned) v.S * kCluster);
-    cfg.blockDim           = dim3(kPickThreads);
-    cfg.stream             = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id                                         = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x                           = kCluster;
-    attr[1].val.clusterDim.y                           = 1;
-    attr[1].val.clusterDim.z                           = 1;
-    cfg.attrs                                          = attr;
-    cfg.numAttrs                                       = 2;
-    st = cuda_status(cudaLaunchKernelEx(&cfg, sample_pick_kernel, a));
-    ctx->launches.fetch_add(1);
-    return st;
+    // as many CTAs per sequence as one wave of two per SM holds: a wave and a bit would take twice as long
+    const int64_t slots = 2 * (int64_t) ctx->num_sms;
+    if (v.S * 16 <= slots) return launch_pick<16>(ctx, a, stream);
+    if (v.S * 8 <= slots) return launch_pick<8>(ctx, a, stream);
+    if (v.S * 4 <= slots) return launch_pick<4>(ctx, a, stream);
+    return launch_pick<2>(ctx, a, stream);
 }
 
 }  // namespace srhpm
