@@ -6,8 +6,8 @@
 // e_j (the last row).
 //
 // Two launches:
-//   sample_part_kernel   every row's logits once (bandwidth bound): per 8192 tokens the maximum, its first place and the
-//                        sum of exponentials in f32. A CTA holds its 32 KB in registers between the maximum and the sum.
+//   sample_part_kernel   every row's logits once (bandwidth bound): per 512 to 4096 tokens the maximum, its first place
+//                        and the sum of exponentials in f32.
 //   sample_pick_kernel   a cluster of CTAs per sequence: joins the rows' records, accepts, and draws from the one row
 //                        that emits. An accepted token is a comparison of two numbers, f32 exponentials (2^-22) do; a drawn
 //                        token is a place in a sum over the whole vocabulary: with V tokens and sums off by d, the place
@@ -29,8 +29,9 @@ namespace srhpm {
 namespace {
 
 constexpr int   kPartThreads = 256;
-constexpr int   kPartVec     = 4;                              // 16-byte loads per thread
-constexpr int   kSeg         = kPartThreads * kPartVec * 4;    // tokens per record
+constexpr int   kPartVec     = 4;                // 16-byte loads of a lane in flight
+constexpr int   kTurn        = kPartVec * 128;   // tokens of a warp's turn
+constexpr int   kMaxTurns    = 8;                // of a record
 constexpr int   kPickThreads = 512;
 constexpr int   kPickWarps   = kPickThreads / 32;
 constexpr int   kMaxBlocks   = 1024;                           // blocks of a CTA's share
@@ -38,7 +39,7 @@ constexpr float kLog2e       = 1.4426950408889634f;
 
 struct SampleArgs {
     SampleView v;
-    int        nseg;
+    int        seg, nseg;  // tokens of a record, records of a row
     int4 *     part;  // [T][nseg]: maximum, sum (bits), first place of the maximum
 };
 
@@ -82,62 +83,116 @@ __device__ __forceinline__ int seq_of_row(const SampleView & v, int t) {
     return lo;
 }
 
-__global__ void __launch_bounds__(kPartThreads) sample_part_kernel(const SampleArgs a) {
+// A warp takes whole records of 1 to 8 turns, 512 tokens a turn, the next turn's loads in flight (over the border of a record too); every
+// lane keeps its own maximum, sum and place, joined across the lanes at a record's end: no barrier, 148 SMs x 32 warps each
+// with 2 KB on the way.
+__global__ void __launch_bounds__(kPartThreads, 4) sample_part_kernel(const SampleArgs a) {
     const SampleView & v = a.v;
-    __shared__ float   sm[kPartThreads / 32], ss[kPartThreads / 32];
-    __shared__ int     si[kPartThreads / 32];
     pdl_launch_dependents();
     pdl_wait();
-    const int     t = blockIdx.x, seg = blockIdx.y, j0 = seg * kSeg, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float * row = reinterpret_cast<const float *>(v.logits + (int64_t) t * v.ldb);
-    const bool    vec = (reinterpret_cast<uintptr_t>(row) & 15) == 0;
-    float         x[kPartVec][4];
+    const int     lane = threadIdx.x & 31;
+    const int64_t jobs = (int64_t) v.T * a.nseg, step = (int64_t) gridDim.x * (kPartThreads / 32);
+    int64_t       job = (int64_t) blockIdx.x * (kPartThreads / 32) + (threadIdx.x >> 5);
+    if (job >= jobs) return;
+    int   t = (int) (job / a.nseg), at = (int) (job % a.nseg) * a.seg;  // row, first token of the turn
+    int   end = min(v.V, at + a.seg);
+    float nx[kPartVec][4];
+    auto  fetch = [&](int row_t, int from, int to) {
+        const float * row = reinterpret_cast<const float *>(v.logits + (int64_t) row_t * v.ldb);
+        const int     j   = from + lane * 4;
+        if ((reinterpret_cast<uintptr_t>(row) & 15) == 0 && from + kTurn <= to) {
 #pragma unroll
-    for (int k = 0; k < kPartVec; k++) load4(row, vec, j0 + (k * kPartThreads + (int) threadIdx.x) * 4, v.V, -INFINITY, x[k]);
-    float c = kLog2e;
-    if (v.temp) {
-        const int s = seq_of_row(v, t);  // while the loads are in flight
-        if (s >= 0) c = kLog2e / v.temp[s];
-    }
-    float m = -INFINITY;
+            for (int k = 0; k < kPartVec; k++) {
+                const float4 f = __ldcs(reinterpret_cast<const float4 *>(row + j) + 32 * k);
+                nx[k][0] = f.x; nx[k][1] = f.y; nx[k][2] = f.z; nx[k][3] = f.w;
+            }
+        } else {
 #pragma unroll
-    for (int k = 0; k < kPartVec; k++) m = fmaxf(m, fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3])));
+            for (int k = 0; k < kPartVec; k++) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) sm[warp] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kPartThreads / 32; w++) m = fmaxf(m, sm[w]);
-    // differences first: a rounded product m * c would count into every term
-    float sum = 0.0f;
-    int   top = INT32_MAX;
-#pragma unroll
-    for (int k = kPartVec - 1; k >= 0; k--) {
-        float p[4];
-#pragma unroll
-        for (int e = 3; e >= 0; e--) {
-            const bool is = x[k][e] == m;
-            p[e]          = is ? 1.0f : fast_ex2((x[k][e] - m) * c);
-            if (is) top = j0 + (k * kPartThreads + (int) threadIdx.x) * 4 + e;
+                for (int e = 0; e < 4; e++) nx[k][e] = j + 128 * k + e < to ? __ldcs(row + j + 128 * k + e) : -INFINITY;
+            }
         }
-        sum += (p[0] + p[1]) + (p[2] + p[3]);
-    }
-    if (m == -INFINITY) sum = 0.0f;
-    top = __reduce_min_sync(0xffffffffu, top);
+    };
+    fetch(t, at, end);
+    float c = kLog2e, m = -INFINITY, sum = 0.0f;
+    int   top = INT32_MAX, known = -1;
+    for (;;) {
+        float x[kPartVec][4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) {
-        ss[warp] = sum;
-        si[warp] = top;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
+        for (int k = 0; k < kPartVec; k++) {
 #pragma unroll
-        for (int w = 1; w < kPartThreads / 32; w++) {
-            sum += ss[w];
-            top = min(top, si[w]);
+            for (int e = 0; e < 4; e++) x[k][e] = nx[k][e];
         }
-        a.part[(int64_t) t * a.nseg + seg] = make_int4(__float_as_int(m), __float_as_int(sum), top, 0);
+        // the next turn
+        const bool    last = at + kTurn >= end;
+        const int64_t nj   = last ? job + step : job;
+        int           nt = t, na = at + kTurn, ne = end;
+        if (last && nj < jobs) {
+            nt = (int) (nj / a.nseg);
+            na = (int) (nj - (int64_t) nt * a.nseg) * a.seg;
+            ne = min(v.V, na + a.seg);
+        }
+        if (nj < jobs) fetch(nt, na, ne);
+        if (v.temp && t != known) {  // with the loads in flight
+            const int s = seq_of_row(v, t);
+            c           = s >= 0 ? kLog2e / v.temp[s] : kLog2e;
+            known       = t;
+        }
+        float mt = m;
+#pragma unroll
+        for (int k = 0; k < kPartVec; k++) mt = fmaxf(mt, fmaxf(fmaxf(x[k][0], x[k][1]), fmaxf(x[k][2], x[k][3])));  // NaN: left out
+        if (mt > m) {  // its first place; seldom after the first turns
+            sum *= m == -INFINITY ? 0.0f : fast_ex2((m - mt) * c);
+            m = mt;
+#pragma unroll
+            for (int k = kPartVec - 1; k >= 0; k--) {
+#pragma unroll
+                for (int e = 3; e >= 0; e--) {
+                    if (x[k][e] == m) top = at + lane * 4 + 128 * k + e;
+                }
+            }
+        }
+        // differences first: a rounded product m * c would count into every term. fmaxf: a NaN becomes nothing (2^-200)
+#pragma unroll
+        for (int k = 0; k < kPartVec; k++) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) p[e] = fast_ex2(fmaxf((x[k][e] - m) * c, -200.0f));
+            sum += (p[0] + p[1]) + (p[2] + p[3]);
+        }
+        if (m == INFINITY) {  // the weight stands on the infinities alone
+#pragma unroll
+            for (int k = 0; k < kPartVec; k++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum += x[k][e] == m ? 1.0f : 0.0f;
+            }
+        }
+        if (last) {
+            if (m == -INFINITY) {
+                sum = 0.0f;
+                top = INT32_MAX;
+            }
+            float mw = m;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, o));
+            sum = m == mw ? sum : m == -INFINITY ? 0.0f : sum * fast_ex2((m - mw) * c);
+            if (m != mw) top = INT32_MAX;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            top = __reduce_min_sync(0xffffffffu, top);
+            if (lane == 0) {
+                a.part[(int64_t) t * a.nseg + at / a.seg] = make_int4(__float_as_int(mw), __float_as_int(sum), top, 0);
+            }
+            m   = -INFINITY;
+            sum = 0.0f;
+            top = INT32_MAX;
+            if (nj >= jobs) break;
+        }
+        job = nj;
+        t   = nt;
+        at  = na;
+        end = ne;
     }
 }
 
@@ -227,30 +282,41 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
     for (int b = r0; b < r1; b += kPickWarps) {
         const int r = b + warp;
         if (r < r1) {
-            float m = -INFINITY;
-            int   top = INT32_MAX;
-            for (int g = lane; g < a.nseg; g += 32) {
-                const int4 p = __ldcg(a.part + (int64_t) r * a.nseg + g);
-                const float pm_ = __int_as_float(p.x);
-                if (pm_ > m) {
-                    m   = pm_;
-                    top = p.z;
-                }
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const float om = __shfl_xor_sync(0xffffffffu, m, o);
-                const int   ot = __shfl_xor_sync(0xffffffffu, top, o);
-                if (om > m || (om == m && ot < top)) {
-                    m   = om;
-                    top = ot;
-                }
-            }
+            float  m = -INFINITY;
+            int    top = INT32_MAX;
             double z = 0.0;
-            for (int g = lane; g < a.nseg; g += 32) {
-                const int4  p   = __ldcg(a.part + (int64_t) r * a.nseg + g);
-                const float pm_ = __int_as_float(p.x);
-                if (pm_ > -INFINITY) z += (pm_ == m ? 1.0 : (double) exp2f((pm_ - m) * c)) * (double) __int_as_float(p.y);
+            for (int g0_ = 0; g0_ < a.nseg; g0_ += 128) {  // four records per lane in flight
+                int4 p[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int g = g0_ + 32 * k + lane;
+                    p[k] = g < a.nseg ? __ldcg(a.part + (int64_t) r * a.nseg + g) : make_int4(__float_as_int(-INFINITY), 0, INT32_MAX, 0);
+                }
+                float mn = m;
+#pragma unroll
+                for (int k = 0; k < 4; k++) mn = fmaxf(mn, __int_as_float(p[k].x));
+                if (mn > m) {
+                    z  = m == -INFINITY ? 0.0 : z * (double) exp2f((m - mn) * c);
+                    m  = mn;
+                    top = INT32_MAX;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float pm_ = __int_as_float(p[k].x);
+                    if (pm_ == m) top = min(top, p[k].z);
+                    if (pm_ > -INFINITY) z += (pm_ == m ? 1.0 : (double) exp2f((pm_ - m) * c)) * (double) __int_as_float(p[k].y);
+                }
+            }
+            {
+                float mw = m;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) mw = fmaxf(mw, __shfl_xor_sync(0xffffffffu, mw, o));
+                if (m != mw) {
+                    z   = m == -INFINITY ? 0.0 : z * (double) exp2f((m - mw) * c);
+                    top = INT32_MAX;
+                }
+                m   = mw;
+                top = __reduce_min_sync(0xffffffffu, top);
             }
             z = tf > 0.0f ? warp_sum(z) : 1.0;
             if (m == -INFINITY) top = 0;
@@ -543,18 +609,30 @@ template <int CL> int launch_pick(srhpm_ctx * ctx, const SampleArgs & a, cudaStr
 
 }  // namespace
 
-size_t verify_sample_work_size(const srhpm_ctx *, int V, int T, int) {
-    return (size_t) T * ((V + (int64_t) kSeg - 1) / kSeg) * sizeof(int4) + 16;
+// tokens of a record: as many turns as leave every warp of the GPU a record (32 warps per SM), 8 at most
+static int seg_tokens(const srhpm_ctx * ctx, int V, int T) {
+    const int64_t turns = (int64_t) T * ((V + (int64_t) kTurn - 1) / kTurn), warps = 32 * (int64_t) ctx->num_sms;
+    int           k = 2;  // one turn leaves too many records to join: 17.5 us instead of 16.4 for 9 rows of 151936
+    while (k < kMaxTurns && turns >= 2 * k * warps) k *= 2;
+    return k * kTurn;
+}
+
+size_t verify_sample_work_size(const srhpm_ctx * ctx, int V, int T, int) {
+    const int seg = seg_tokens(ctx, V, T);
+    return (size_t) T * ((V + (int64_t) seg - 1) / seg) * sizeof(int4) + 16;
 }
 
 int verify_sample_run(srhpm_ctx * ctx, const SampleView & v, void * wdata, size_t wsize, cudaStream_t stream) {
     if (wdata == nullptr || wsize < verify_sample_work_size(ctx, v.V, v.T, v.S)) return SRHPM_ERR_WORKSPACE;
     SampleArgs a;
     a.v    = v;
-    a.nseg = (int) ((v.V + (int64_t) kSeg - 1) / kSeg);
+    a.seg  = seg_tokens(ctx, v.V, v.T);
+    a.nseg = (int) ((v.V + (int64_t) a.seg - 1) / a.seg);
     a.part = reinterpret_cast<int4 *>((reinterpret_cast<uintptr_t>(wdata) + 15) & ~(uintptr_t) 15);
-    if (a.nseg > 65535) return SRHPM_UNSUPPORTED;
-    int st = cuda_status(launch_k_pdl(sample_part_kernel, dim3(v.T, a.nseg), dim3(kPartThreads), 0, stream, a));
+    if (v.V > 1 << 29) return SRHPM_UNSUPPORTED;
+    const int64_t want = ((int64_t) v.T * a.nseg + kPartThreads / 32 - 1) / (kPartThreads / 32);
+    const int     grid = (int) std::min<int64_t>(4 * (int64_t) ctx->num_sms, want);
+    int st = cuda_status(launch_k_pdl(sample_part_kernel, dim3(grid), dim3(kPartThreads), 0, stream, a));
     ctx->launches.fetch_add(1);
     if (st != SRHPM_OK) return st;
     // as many CTAs per sequence as one wave of two per SM holds: a wave and a bit would take twice as long
