@@ -258,6 +258,12 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // a wait that ran out marks the kernel's status; the thread then waits for nothing more (its results are void, its
 // accesses stay in bounds) so that every role comes to its end
 __device__ __forceinline__ void wait_bar(uint64_t * bar, uint32_t parity, int32_t * status, bool & bad) {
@@ -481,7 +487,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         const int q    = NT == 2 ? wg : 0;                              // row tile
         const int c0   = NT == 2 ? 0 : 64 * wg;                         // first score column of this thread
         uint32_t  rc0 = 0, sc[2] = { 0, 0 }, pvc = 0, pvw = 0, turn = 0, items = 0;
-        for (; active; active = walk_next<BMN>(a, w)) {
+        while (active) {
             const int     n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
             const int     R    = w.n * a.G;
             const int     rb   = w.rt * BMN + q * BR;               // first row of this tile
@@ -543,11 +549,24 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
             }
+            // the next item, and its rows on their way to L2: from memory they take 2.4 us
+            Walk       nw   = w;
+            const bool more = walk_next<BMN>(a, nw);
+            if (more && nw.sp.nkv) {
+                constexpr int per = D * (PREC ? 4 : 2) / 128;  // lines of a row
+                const int     nr  = min(BMN, nw.n * a.G - nw.rt * BMN);
+                for (int u = tid; u < nr * per; u += kSmWarps * 32) {
+                    const int rr = nw.rt * BMN + u / per, t = a.byG.div(rr), h = nw.h * a.G + (rr - t * a.G);
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.q + (int64_t) (nw.r0 + t) * a.qnb1 + (int64_t) h * a.qnb2 + u % per * 128));
+                }
+            }
             // the row's visible tokens
             const int tok = mine ? a.byG.div(rb + row) : 0;  // of the sequence's new ones
             const int pos = w.kv - w.n + tok;
             const int vhi = mine ? min(pos + 1, w.sp.hi) : 0;
             const int vlo = a.window > 0 ? max(w.sp.lo, (int) max((int64_t) INT32_MIN, (int64_t) pos - a.window + 1)) : 0;
+            // what every row of the warp sees
+            const int wlo = __reduce_max_sync(0xffffffffu, mine ? vlo : 0), whi = __reduce_min_sync(0xffffffffu, mine ? vhi : INT32_MAX);
             // tokens that every row of the tile sees: no masking there
             const int pmin = w.kv - w.n + a.byG.div(rb), pmax = w.kv - w.n + a.byG.div(rb + max(rows, 1) - 1);
             const int ahi = min(pmin + 1, w.sp.hi);
@@ -593,15 +612,21 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
 #pragma unroll
                         for (int c = 0; c < NC; c++) s[c] = a.softcap_l2 * tanhf(s[c] * a.qscale);
                     }
+                    // per 32 columns: all rows of the warp see them, none does, or lane by lane
                     if (t0 < alo || t0 + kBN > ahi) {
-                        const int l0 = vlo - t0 - c0, h0 = vhi - t0 - c0;
 #pragma unroll
-                        for (int c = 0; c < NC; c++) s[c] = c >= l0 && c < h0 ? s[c] : -INFINITY;
+                        for (int c = 0; c < NC; c += 32) {
+                            const int u0 = t0 + c0 + c;
+                            if (u0 >= wlo && u0 + 32 <= whi) continue;
+                            const int l0 = vlo - u0, h0 = vhi - u0;
+#pragma unroll
+                            for (int e = 0; e < 32; e++) s[c + e] = e >= l0 && e < h0 ? s[c + e] : -INFINITY;
+                        }
                     }
                     float mx[4] = { s[0], s[1], s[2], s[3] };
 #pragma unroll
-                    for (int c = 4; c < NC; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-                    mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    for (int c = 4; c < NC; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], s[c], s[c + 1]);
+                    mt = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
                 }
                 if constexpr (NT == 1) {  // the other half of the row; both halves have read S before either writes P
                     float * rd = red + (turn & 1) * 2 * kBM;
@@ -773,6 +798,8 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 a.desc[2 * blockIdx.x]     = make_int4(e - (int) blockIdx.x + 1, w.h, w.r0, 0);
             }
             rc0 += 2 * n * CH;
+            w      = nw;
+            active = more;
         }
     } else if (!Q8 || warp < kSmWarps + 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q8 ? 56 : 104));
@@ -907,79 +934,122 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 wait_bar(q_full, items & 1, a.status, bad);
                 items++;
                 tc::fence_after();
-                auto qk = [&](int i, int q, bool last) {  // last: the tile's last product with this K
-                    const int      b = NT == 2 ? q : (i & 1);
-                    const uint32_t d = tS + 128 * b;
+                // products of one chunk (the elected lane)
+                auto qk_chunk = [&](uint32_t slot, int b, int q, int ch) {
+                    const uint64_t kd = kd0 + slot * (Ly::chunk / 16), qd = qd0 + q * (Ly::qparts * Ly::qtile / 16);
 #pragma unroll
-                    for (int ch = 0; ch < CH; ch++) {
-                        uint32_t       use;
-                        const uint32_t slot = chunk_at(true, i, n, ch, use);
-                        wait_bar(&kvfull[slot], use & 1, a.status, bad);
-                        tc::fence_after();
-                        __syncwarp();
-                        if (elect_one()) {
-                            const uint64_t kd = kd0 + slot * (Ly::chunk / 16), qd = qd0 + q * (Ly::qparts * Ly::qtile / 16);
+                    for (int j = 0; j < D / CH / 16; j++) {
+                        const int      jj = ch * (D / CH / 16) + j;  // k-step over all dims
+                        const uint64_t bd = kd + ((j >> 2) * (kBN * 128) + (j & 3) * 32) / 16;
 #pragma unroll
-                            for (int j = 0; j < D / CH / 16; j++) {
-                                const int      jj = ch * (D / CH / 16) + j;  // k-step over all dims
-                                const uint64_t bd = kd + ((j >> 2) * (kBN * 128) + (j & 3) * 32) / 16;
-#pragma unroll
-                                for (int part = 0; part < Ly::qparts; part++) {
-                                    tc::mma_f16(d, qd + (part * Ly::qtile + (jj >> 2) * (BR * 128) + (jj & 3) * 32) / 16, bd, idqk,
-                                                (uint32_t) (jj > 0 || part > 0));
-                                }
-                            }
-                            if (last) tc::commit(&kvempty[slot]);
-                            if (ch == CH - 1) tc::commit(&s_full[b]);
+                        for (int part = 0; part < Ly::qparts; part++) {
+                            tc::mma_f16(tS + 128 * b, qd + (part * Ly::qtile + (jj >> 2) * (BR * 128) + (jj & 3) * 32) / 16, bd, idqk,
+                                        (uint32_t) (jj > 0 || part > 0));
                         }
-                        __syncwarp();
                     }
                 };
-                auto pv = [&](int i, int q, bool last) {
-                    const int      b = NT == 2 ? q : (i & 1);
-                    const uint32_t p = tS + 128 * b, d = tO + q * D;
-                    uint32_t &     pc = b ? pc1 : pc0;
-                    wait_bar(&p_rdy[b], pc & 1, a.status, bad);
-                    pc++;
+                auto pv_chunk = [&](uint32_t slot, int b, int q, int ch, bool first) {
+                    const uint64_t vd = vd0 + slot * (Ly::chunk / 16);
 #pragma unroll
-                    for (int ch = 0; ch < CH; ch++) {
-                        uint32_t       use;
-                        const uint32_t slot = chunk_at(false, i, n, ch, use);
-                        wait_bar(&kvfull[slot], use & 1, a.status, bad);
-                        tc::fence_after();
-                        __syncwarp();
-                        if (elect_one()) {
-                            const uint64_t vd = vd0 + slot * (Ly::chunk / 16);
+                    for (int j = 0; j < Ly::vtok / 16; j++) {
+                        const int jj = ch * (Ly::vtok / 16) + j;
 #pragma unroll
-                            for (int j = 0; j < Ly::vtok / 16; j++) {
-                                const int jj = ch * (Ly::vtok / 16) + j;
-#pragma unroll
-                                for (int part = 0; part < Ly::qparts; part++) {
-                                    mma_f16_ta(d, p + part * 64 + jj * 8, vd + j * 2048 / 16, idpv, (uint32_t) (i > 0 || jj > 0 || part > 0));
-                                }
-                            }
-                            if (last) tc::commit(&kvempty[slot]);
-                            if (ch == CH - 1) tc::commit(&pv_done[NT == 2 ? q : (pvn & 1)]);
+                        for (int part = 0; part < Ly::qparts; part++) {
+                            mma_f16_ta(tO + q * D, tS + 128 * b + part * 64 + jj * 8, vd + j * 2048 / 16, idpv,
+                                       (uint32_t) (!first || jj > 0 || part > 0));
                         }
-                        __syncwarp();
                     }
-                    pvn++;
                 };
+                uint32_t use;
                 if constexpr (NT == 1) {
-                    qk(0, 0, true);
-                    for (int i = 0; i < n; i++) {
-                        if (i + 1 < n) qk(i + 1, 0, true);
-                        pv(i, 0, true);
+                    auto qk = [&](int i) {
+#pragma unroll
+                        for (int ch = 0; ch < CH; ch++) {
+                            const uint32_t slot = chunk_at(true, i, n, ch, use);
+                            wait_bar(&kvfull[slot], use & 1, a.status, bad);
+                            tc::fence_after();
+                            __syncwarp();
+                            if (elect_one()) {
+                                qk_chunk(slot, i & 1, 0, ch);
+                                tc::commit(&kvempty[slot]);
+                                if (ch == CH - 1) tc::commit(&s_full[i & 1]);
+                            }
+                            __syncwarp();
+                        }
+                    };
+                    qk(0);
+                    for (int i = 0; i < n; i++, pvn++) {
+                        if (i + 1 < n) qk(i + 1);
+                        // V first: it is there before P in most turns, and P's arrival is what the products wait for
+                        uint32_t sl[CH];
+#pragma unroll
+                        for (int ch = 0; ch < CH; ch++) {
+                            sl[ch] = chunk_at(false, i, n, ch, use);
+                            if (!Q8 || ch == 0) wait_bar(&kvfull[sl[ch]], use & 1, a.status, bad);
+                        }
+                        uint32_t & pc = (i & 1) ? pc1 : pc0;
+                        wait_bar(&p_rdy[i & 1], pc & 1, a.status, bad);
+                        pc++;
+                        tc::fence_after();
+                        __syncwarp();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int ch = 0; ch < (Q8 ? 1 : CH); ch++) {
+                                pv_chunk(sl[ch], i & 1, 0, ch, i == 0);
+                                tc::commit(&kvempty[sl[ch]]);
+                            }
+                            if (!Q8 || CH == 1) tc::commit(&pv_done[pvn & 1]);
+                        }
+                        __syncwarp();
+                        if constexpr (Q8) {  // its V ring may hold one chunk
+                            wait_bar(&kvfull[sl[1]], use & 1, a.status, bad);
+                            tc::fence_after();
+                            __syncwarp();
+                            if (elect_one()) {
+                                pv_chunk(sl[1], i & 1, 0, 1, false);
+                                tc::commit(&kvempty[sl[1]]);
+                                tc::commit(&pv_done[pvn & 1]);
+                            }
+                            __syncwarp();
+                        }
                     }
-                } else {
-                    qk(0, 0, nq == 1);
-                    if (nq == 2) qk(0, 1, true);
+                } else {  // one chunk per tile; K and V are waited for once, before the first row tile's P
+                    uint32_t ks = chunk_at(true, 0, n, 0, use), vs = 0;
+                    wait_bar(&kvfull[ks], use & 1, a.status, bad);
+                    tc::fence_after();
+                    __syncwarp();
+                    if (elect_one()) {
+                        for (int q = 0; q < nq; q++) {
+                            qk_chunk(ks, q, q, 0);
+                            if (q == nq - 1) tc::commit(&kvempty[ks]);
+                            tc::commit(&s_full[q]);
+                        }
+                    }
+                    __syncwarp();
                     for (int i = 0; i < n; i++) {
-                        pv(i, 0, nq == 1);
-                        if (i + 1 < n) qk(i + 1, 0, nq == 1);
-                        if (nq == 2) {
-                            pv(i, 1, true);
-                            if (i + 1 < n) qk(i + 1, 1, true);
+                        vs = chunk_at(false, i, n, 0, use);
+                        wait_bar(&kvfull[vs], use & 1, a.status, bad);
+                        if (i + 1 < n) {
+                            ks = chunk_at(true, i + 1, n, 0, use);
+                            wait_bar(&kvfull[ks], use & 1, a.status, bad);
+                        }
+                        for (int q = 0; q < nq; q++) {
+                            uint32_t & pc = q ? pc1 : pc0;
+                            wait_bar(&p_rdy[q], pc & 1, a.status, bad);
+                            pc++;
+                            tc::fence_after();
+                            __syncwarp();
+                            if (elect_one()) {
+                                pv_chunk(vs, q, q, 0, i == 0);
+                                if (q == nq - 1) tc::commit(&kvempty[vs]);
+                                tc::commit(&pv_done[q]);
+                                if (i + 1 < n) {
+                                    qk_chunk(ks, q, q, 0);
+                                    if (q == nq - 1) tc::commit(&kvempty[ks]);
+                                    tc::commit(&s_full[q]);
+                                }
+                            }
+                            __syncwarp();
                         }
                     }
                 }
