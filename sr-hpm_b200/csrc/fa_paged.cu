@@ -71,6 +71,7 @@ struct PArgs {
     int64_t         qnb1, qnb2;
     uint8_t *       dst;
     int64_t         dnb1, dnb2;
+    int             wide;  // dst and its strides are multiples of 32 bytes
     const uint8_t * table;
     int64_t         tstride;
     int             cols, page, n_pages, box;  // box: tokens of a TMA box (divides the page)
@@ -256,6 +257,13 @@ __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
+}
+
+// 32 bytes at a time: a row per lane makes every store of a warp 32 separate sectors, whole ones this way
+__device__ __forceinline__ void st_row8(void * p, const uint32_t * r) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -487,15 +495,13 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         const int q    = NT == 2 ? wg : 0;                              // row tile
         const int c0   = NT == 2 ? 0 : 64 * wg;                         // first score column of this thread
         uint32_t  rc0 = 0, sc[2] = { 0, 0 }, pvc = 0, pvw = 0, turn = 0, items = 0;
-        while (active) {
-            const int     n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
-            const int     R    = w.n * a.G;
-            const int     rb   = w.rt * BMN + q * BR;               // first row of this tile
-            const int     rows = max(0, min(BR, R - rb));
-            const bool    mine = row < rows;                        // this thread's row exists
-            const bool    some = 32 * wq < rows;                    // the warp has a row
-            // Q rows to shared memory: 16-byte chunks of 8 dims, 128-byte swizzle
-            if (n > 0) {
+        // Q rows of an item to shared memory: 16-byte chunks of 8 dims, 128-byte swizzle. q_issue starts the copies (f32 rows:
+        // does nothing yet), q_finish ends with the rows there and the MMA warp told. For the next item q_issue runs as
+        // soon as the last scores of the one before are there (its Q is read no more) and q_finish behind its last P: the
+        // next scores are then on their way during the epilogue.
+        auto q_rows = [&](const Walk & w, bool finish) {
+            const int rb = w.rt * BMN + q * BR, rows = max(0, min(BR, w.n * a.G - rb));
+            if (PREC == finish && rows > 0) {
                 constexpr int per = D / 8, step = (NT == 2 ? 128 : 256) / per;  // rows apart of a thread's chunks
                 const int     u0 = NT == 2 ? (tid & 127) : tid, c = u0 % per;
                 uint8_t *     d0 = sm + Ly::q + q * Ly::qparts * Ly::qtile + (c >> 3) * (BR * 128);
@@ -505,15 +511,13 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     return a.q + (int64_t) (w.r0 + t) * a.qnb1 + (int64_t) h * a.qnb2;
                 };
                 auto dest = [&](int r) { return d0 + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
-                if (rows == 0) {
-                } else if constexpr (!PREC) {
+                if constexpr (!PREC) {
 #pragma unroll
                     for (int k = 0; k < (BR + step - 1) / step; k++) {
                         const int r = u0 / per + k * step;
                         if (BR % step && r >= BR) break;
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dest(r))), "l"(source(r) + 16 * c) : "memory");
                     }
-                    asm volatile("cp.async.wait_all;" ::: "memory");
                 } else {
                     constexpr int NK = (BR + step - 1) / step, UN = NK < 4 ? NK : 4;  // rows of a thread, in flight
 #pragma unroll 1
@@ -545,14 +549,27 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         }
                     }
                 }
+            }
+            if (finish) {
+                if constexpr (!PREC) asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full);
             }
+        };
+        auto q_issue  = [&](const Walk & w) { q_rows(w, false); };
+        auto q_finish = [&](const Walk & w) { q_rows(w, true); };
+        for (bool boot = true; active; boot = false) {  // first a turn without an item, which brings the first one's rows
+            const int     n = w.sp.nkv && !boot ? w.take : 0, kt = w.sp.kt0 + w.off;
+            const int     R    = w.n * a.G;
+            const int     rb   = w.rt * BMN + q * BR;               // first row of this tile
+            const int     rows = max(0, min(BR, R - rb));
+            const bool    mine = row < rows;                        // this thread's row exists
+            const bool    some = 32 * wq < rows;                    // the warp has a row
             // the next item, and its rows on their way to L2: from memory they take 2.4 us
             Walk       nw   = w;
-            const bool more = walk_next<BMN>(a, nw);
-            if (more && nw.sp.nkv) {
+            const bool more = boot || walk_next<BMN>(a, nw);
+            if (more && nw.sp.nkv && !boot) {
                 constexpr int per = D * (PREC ? 4 : 2) / 128;  // lines of a row
                 const int     nr  = min(BMN, nw.n * a.G - nw.rt * BMN);
                 for (int u = tid; u < nr * per; u += kSmWarps * 32) {
@@ -590,6 +607,12 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 if (!run) wait_bar(q_full, items & 1, a.status, bad);
                 items++;
             }
+            const bool ahead = more && nw.sp.nkv;  // the next item has rows to bring
+            if (ahead && (n == 0 || !run)) {
+                q_issue(nw);
+                q_finish(nw);
+            }
+            if (boot) continue;
             for (int i = 0; run && i < n; i++) {
                 const int b = NT == 2 ? q : (i & 1), t0 = (kt + i) * kBN;
                 wait_bar(&s_full[b], sc[b] & 1, a.status, bad);
@@ -601,6 +624,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     pv_wait(pvc - 1);
                 }
                 tc::fence_after();
+                if (ahead && i == n - 1) q_issue(nw);
                 const uint32_t tb = tc::taddr(tS + 128 * b, wq, 0);
                 float          s[NC];
                 float          mt = -INFINITY;
@@ -707,13 +731,14 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_rdy[b]);
+                if (ahead && i == n - 1) q_finish(nw);
             }
             // ---------------- the item's end ----------------
             if (run && n > 0) {
                 pv_wait(pvc);
                 tc::fence_after();
             }
-            const bool whole = w.off == 0 && w.take == w.sp.units;
+            const bool whole = w.off == 0 && w.take == w.sp.units, wide = a.wide != 0;
             if constexpr (NT == 1) {
                 float * rd = red + (turn & 1) * 2 * kBM;
                 turn++;
@@ -762,27 +787,33 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     if (!mine) continue;
                     if (!whole) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            __stcg(reinterpret_cast<uint4 *>(acc + o0 + c + e), make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
-                        }
+                        for (int e = 0; e < 32; e += 8) st_row8(acc + o0 + c + e, o + e);
                     } else {
 #pragma unroll
                         for (int e = 0; e < 32; e++) o[e] = __float_as_uint(f != 0.0f ? __uint_as_float(o[e]) * f : 0.0f);
                         if constexpr (PREC) {
 #pragma unroll
                             for (int e = 0; e < 32; e += 4) {
-                                *reinterpret_cast<uint4 *>(dst + 4 * (o0 + c + e)) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                                if (wide) {
+                                    if ((e & 7) == 0) st_row8(dst + 4 * (o0 + c + e), o + e);
+                                } else {
+                                    *reinterpret_cast<uint4 *>(dst + 4 * (o0 + c + e)) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                                }
                             }
                         } else {
+                            uint32_t h[16];
 #pragma unroll
-                            for (int e = 0; e < 32; e += 8) {
-                                uint32_t h[4];
+                            for (int k = 0; k < 16; k++) {
+                                const __half2 h2 = __floats2half2_rn(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1]));
+                                h[k]             = *reinterpret_cast<const uint32_t *>(&h2);
+                            }
 #pragma unroll
-                                for (int k = 0; k < 4; k++) {
-                                    const __half2 h2 = __floats2half2_rn(__uint_as_float(o[e + 2 * k]), __uint_as_float(o[e + 2 * k + 1]));
-                                    h[k]             = *reinterpret_cast<const uint32_t *>(&h2);
+                            for (int k = 0; k < 16; k += 4) {
+                                if (wide) {
+                                    if ((k & 7) == 0) st_row8(dst + 2 * (o0 + c) + 4 * k, h + k);
+                                } else {
+                                    *reinterpret_cast<uint4 *>(dst + 2 * (o0 + c) + 4 * k) = make_uint4(h[k], h[k + 1], h[k + 2], h[k + 3]);
                                 }
-                                *reinterpret_cast<uint4 *>(dst + 2 * (o0 + c + e)) = make_uint4(h[0], h[1], h[2], h[3]);
                             }
                         }
                     }
@@ -927,10 +958,13 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     return c % NS;
                 }
             };
-            for (; active; active = walk_next<BMN>(a, w)) {
-                const int n = __shfl_sync(0xffffffffu, w.sp.nkv ? w.take : 0, 0);
+            for (Walk nw; active; w = nw) {
+                const int n  = __shfl_sync(0xffffffffu, w.sp.nkv ? w.take : 0, 0);
+                const int nr = w.n * a.G - w.rt * BMN;
+                nw           = w;  // looked up now: behind the last product it would wait among the epilogue's stores
+                active       = walk_next<BMN>(a, nw);
                 if (n == 0) continue;
-                const int nq = __shfl_sync(0xffffffffu, NT == 2 && w.n * a.G - w.rt * BMN > BR ? 2 : 1, 0);
+                const int nq = __shfl_sync(0xffffffffu, NT == 2 && nr > BR ? 2 : 1, 0);
                 wait_bar(q_full, items & 1, a.status, bad);
                 items++;
                 tc::fence_after();
@@ -1261,7 +1295,7 @@ size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 
 size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S, bool q8f32) {
     const size_t recs = (size_t) 2 * ctx->num_sms * record_rows(T, H / Hkv, tile_of(T, S, H / Hkv, D, q8f32));
-    return recs * D * sizeof(float) + align16(recs * sizeof(float2)) + 2 * (size_t) ctx->num_sms * sizeof(int4) + 16;
+    return recs * D * sizeof(float) + align16(recs * sizeof(float2)) + 2 * (size_t) ctx->num_sms * sizeof(int4) + 32;
 }
 
 int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t wsize, cudaStream_t stream) {
@@ -1276,6 +1310,7 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     a.dst     = v.dst;
     a.dnb1    = v.dnb1;
     a.dnb2    = v.dnb2;
+    a.wide    = ((reinterpret_cast<uintptr_t>(v.dst) | v.dnb1 | v.dnb2) & 31) == 0;
     a.table   = v.table;
     a.tstride = v.tstride;
     a.cols    = v.cols;
@@ -1296,7 +1331,7 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     a.sinks      = v.sinks;
     a.prow       = record_rows(v.T, G, tl);
     const size_t recs = (size_t) 2 * ctx->num_sms * a.prow;
-    uint8_t *    wb   = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(wdata) + 15) & ~(uintptr_t) 15);
+    uint8_t *    wb   = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(wdata) + 31) & ~(uintptr_t) 31);
     a.part_acc = reinterpret_cast<float *>(wb);
     a.part_ms  = reinterpret_cast<float2 *>(wb + recs * D * sizeof(float));
     a.desc     = reinterpret_cast<int4 *>(wb + recs * D * sizeof(float) + align16(recs * sizeof(float2)));
