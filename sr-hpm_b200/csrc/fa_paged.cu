@@ -1156,25 +1156,29 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
 }
 
 // The records of an item cut between CTAs, joined in the order of the cuts. CTA c opens the item (record 2c + 1), CTAs
-// c + 1 .. c + parts - 1 go on with it (records 2(c + 1), 2(c + 2), ...). A warp per row and 128 values of it, 16 records
-// in flight: the join is a few round trips to L2, whatever the number of parts.
-template <int D, bool F32> __global__ void __launch_bounds__(256) fa_paged_merge_kernel(const __grid_constant__ PArgs a) {
-    constexpr int W  = D >= 128 ? 4 : 2;   // values per lane
-    constexpr int PP = D > 128 ? D / 128 : 1;  // pieces of a row
-    constexpr int MO = 16;                 // records in flight
+// c + 1 .. c + parts - 1 go on with it (records 2(c + 1), 2(c + 2), ...). Few parts (prompts: two or three, hundreds of
+// rows): a warp per row. Many (long caches, few rows): the CTA's 8 warps share out a row's parts, every eighth each, and join
+// in shared memory. Four records of a lane in flight: 16 took so many registers that the cut items of 18 prompts of 64
+// tokens were joined in 41 us instead of 17.
+template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_merge_kernel(const __grid_constant__ PArgs a) {
+    constexpr int V  = D / 32;  // values per lane, in pairs or fours side by side
+    constexpr int VW = V >= 4 ? 4 : 2;
+    constexpr int MO = 4;
+    __shared__ float part_s[8][D];
+    __shared__ float l_s[8];
     pdl_launch_dependents();
     pdl_wait();
     const int  c  = blockIdx.x;
     const int4 d0 = a.desc[2 * c];
     if (d0.x == 0) return;
     const int4 d1 = a.desc[2 * c + 1];
-    const int  lane = threadIdx.x & 31;
-    for (int job = blockIdx.y * 8 + (threadIdx.x >> 5); job < d1.y * PP; job += gridDim.y * 8) {
-        const int row = job / PP, piece = job % PP;
+    const int  lane = threadIdx.x & 31, warp = threadIdx.x >> 5, parts = d0.x;
+    const bool many = parts > 6 && d1.y <= 64;
+    for (int row = many ? blockIdx.y : blockIdx.y * 8 + warp; row < d1.y; row += many ? gridDim.y : gridDim.y * 8) {
         const int tok = a.byG.div(d1.x + row), h = d0.y * a.G + (d1.x + row - tok * a.G);
         auto      rec = [&](int p) { return (int64_t) (2 * (c + p) + (p == 0 ? 1 : 0)) * a.prow + row; };
         float     M   = -INFINITY;
-        for (int p = lane; p < d0.x; p += 32) {
+        for (int p = lane; p < parts; p += 32) {
             const float2 v = __ldcg(a.part_ms + rec(p));
             if (v.y > 0.0f) M = fmaxf(M, v.x);
         }
@@ -1185,47 +1189,82 @@ template <int D, bool F32> __global__ void __launch_bounds__(256) fa_paged_merge
             sk = a.sinks[h] * kLog2e;
             M  = fmaxf(M, sk);
         }
-        float L = sk > -INFINITY ? ex2(sk - M + kShift) : 0.0f;
-        float acc[W];
+        float L = 0.0f, acc[V];
 #pragma unroll
-        for (int e = 0; e < W; e++) acc[e] = 0.0f;
-        for (int p0 = 0; p0 < d0.x; p0 += MO) {
-            float x[MO][W];
+        for (int e = 0; e < V; e++) acc[e] = 0.0f;
+        const int first = many ? warp : 0, step = many ? 8 : 1;
+        for (int p0 = first; p0 < parts; p0 += MO * step) {
+            float  x[MO][V];
+            float2 ms[MO];
 #pragma unroll
             for (int k = 0; k < MO; k++) {
-                if (p0 + k < d0.x) {
-                    const float * src = a.part_acc + rec(p0 + k) * D + piece * 128 + lane * W;
-                    if constexpr (W == 4) {
-                        const float4 f = __ldcg(reinterpret_cast<const float4 *>(src));
-                        x[k][0] = f.x; x[k][1] = f.y; x[k][2] = f.z; x[k][3] = f.w;
-                    } else {
-                        const float2 f = __ldcg(reinterpret_cast<const float2 *>(src));
-                        x[k][0] = f.x; x[k][1] = f.y;
+                const int p = p0 + k * step;
+                ms[k]       = make_float2(0.0f, 0.0f);
+                if (p < parts) {
+                    ms[k]             = __ldcg(a.part_ms + rec(p));
+                    const float * src = a.part_acc + rec(p) * D + lane * VW;
+#pragma unroll
+                    for (int e = 0; e < V; e += VW) {
+                        if constexpr (VW == 4) {
+                            const float4 f = __ldcg(reinterpret_cast<const float4 *>(src + 32 * e));
+                            x[k][e] = f.x; x[k][e + 1] = f.y; x[k][e + 2] = f.z; x[k][e + 3] = f.w;
+                        } else {
+                            const float2 f = __ldcg(reinterpret_cast<const float2 *>(src + 32 * e));
+                            x[k][e] = f.x; x[k][e + 1] = f.y;
+                        }
                     }
                 }
             }
-            const float2 v = lane < MO && p0 + lane < d0.x ? __ldcg(a.part_ms + rec(p0 + lane)) : make_float2(0.0f, 0.0f);
-            const float  w = v.y > 0.0f ? ex2(v.x - M) : 0.0f;
 #pragma unroll
             for (int k = 0; k < MO; k++) {
-                const float wk = __shfl_sync(0xffffffffu, w, k), lk = __shfl_sync(0xffffffffu, v.y, k);
-                if (wk > 0.0f) {  // a record without weight may hold anything
-                    L = fmaf(wk, lk, L);
+                if (ms[k].y > 0.0f) {  // a record without weight may hold anything
+                    const float w = ex2(ms[k].x - M);
+                    L             = fmaf(w, ms[k].y, L);
 #pragma unroll
-                    for (int e = 0; e < W; e++) acc[e] = fmaf(wk, x[k][e], acc[e]);
+                    for (int e = 0; e < V; e++) acc[e] = fmaf(w, x[k][e], acc[e]);
                 }
             }
         }
-        const float f   = L > 0.0f ? 1.0f / L : 0.0f;
-        uint8_t *   dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) (d0.z + tok) * a.dnb2;
-        const int   at  = piece * 128 + lane * W;
+        const float sink = sk > -INFINITY ? ex2(sk - M + kShift) : 0.0f;
+        uint8_t *   dst  = a.dst + (int64_t) h * a.dnb1 + (int64_t) (d0.z + tok) * a.dnb2;
+        if (!many) {
+            L += sink;
+            const float f = L > 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
-        for (int k = 0; k < W; k += 2) {
-            if constexpr (F32) {
-                *reinterpret_cast<float2 *>(dst + 4 * (at + k)) = make_float2(acc[k] * f, acc[k + 1] * f);
-            } else {
-                *reinterpret_cast<__half2 *>(dst + 2 * (at + k)) = __floats2half2_rn(acc[k] * f, acc[k + 1] * f);
+            for (int e = 0; e < V; e += VW) {
+#pragma unroll
+                for (int k = 0; k < VW; k += 2) {
+                    const int at = 32 * e + lane * VW + k;
+                    if constexpr (F32) {
+                        *reinterpret_cast<float2 *>(dst + 4 * at) = make_float2(acc[e + k] * f, acc[e + k + 1] * f);
+                    } else {
+                        *reinterpret_cast<__half2 *>(dst + 2 * at) = __floats2half2_rn(acc[e + k] * f, acc[e + k + 1] * f);
+                    }
+                }
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e += VW) {
+#pragma unroll
+                for (int k = 0; k < VW; k++) part_s[warp][32 * e + lane * VW + k] = acc[e + k];
+            }
+            if (lane == 0) l_s[warp] = L;
+            __syncthreads();
+            L = sink;
+#pragma unroll
+            for (int w = 0; w < 8; w++) L += l_s[w];
+            const float f = L > 0.0f ? 1.0f / L : 0.0f;
+            for (int at = threadIdx.x; at < D; at += 256) {
+                float o = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 8; w++) o += part_s[w][at];
+                if constexpr (F32) {
+                    reinterpret_cast<float *>(dst)[at] = o * f;
+                } else {
+                    reinterpret_cast<__half *>(dst)[at] = __float2half_rn(o * f);
+                }
+            }
+            __syncthreads();
         }
     }
 }
@@ -1275,7 +1314,7 @@ int launch_paged(srhpm_ctx * ctx, const PArgs & a, const CUtensorMap & mk, const
     ctx->launches.fetch_add(1);
     if (st != SRHPM_OK) return st;
     st = cuda_status(launch_k_pdl(fa_paged_merge_kernel<D, PREC>,
-                                  dim3(ctx->num_sms, std::min(16, (a.prow * (D > 128 ? 2 : 1) + 7) / 8)), dim3(256), 0, stream, a));
+                                  dim3(ctx->num_sms, BR == kFew ? std::min(32, a.prow) : 16), dim3(256), 0, stream, a));
     ctx->launches.fetch_add(1);
     return st;
 }
