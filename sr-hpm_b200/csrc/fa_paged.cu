@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     constexpr int BMN  = BR * NT;
     constexpr int CH   = Ly::CH;
     constexpr int NS   = Ly::NS;
+    constexpr int MM   = BR <= 64 ? 64 : 128; // rows of a product
     constexpr int NC   = NT == 2 ? 128 : 64;  // score columns per softmax thread
     constexpr int OC   = NT == 2 ? D : D / 2; // output columns per softmax thread
     extern __shared__ __align__(1024) uint8_t sm[];
@@ -491,7 +492,9 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     if (warp < kSmWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Q8 ? 128 : 200));
         // ---------------- softmax ----------------
-        const int wg = warp >> 2, wq = warp & 3, row = 32 * wq + lane;  // row of the tile (tensor-memory lane)
+        const int wg = warp >> 2, wq = warp & 3;
+        // row of the tile: its tensor-memory lane, or with M = 64 16 rows in the lower lanes of each quarter
+        const int row = MM == 64 ? 16 * wq + (lane & 15) : 32 * wq + lane, tl = 32 * wq + lane;
         const int q    = NT == 2 ? wg : 0;                              // row tile
         const int c0   = NT == 2 ? 0 : 64 * wg;                         // first score column of this thread
         uint32_t  rc0 = 0, sc[2] = { 0, 0 }, pvc = 0, pvw = 0, turn = 0, items = 0;
@@ -505,7 +508,8 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 constexpr int per = D / 8, step = (NT == 2 ? 128 : 256) / per;  // rows apart of a thread's chunks
                 const int     u0 = NT == 2 ? (tid & 127) : tid, c = u0 % per;
                 uint8_t *     d0 = sm + Ly::q + q * Ly::qparts * Ly::qtile + (c >> 3) * (BR * 128);
-                // rows behind the last one repeat it: their scores and outputs go nowhere
+                // rows behind the last one are zeros: what they give goes nowhere, but random rows heat the products (a
+                // 1000 W card lowers its clock for it)
                 auto source = [&](int r) {
                     const int rr = rb + min(r, rows - 1), t = a.byG.div(rr), h = w.h * a.G + (rr - t * a.G);
                     return a.q + (int64_t) (w.r0 + t) * a.qnb1 + (int64_t) h * a.qnb2;
@@ -516,7 +520,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     for (int k = 0; k < (BR + step - 1) / step; k++) {
                         const int r = u0 / per + k * step;
                         if (BR % step && r >= BR) break;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dest(r))), "l"(source(r) + 16 * c) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dest(r))), "l"(source(r) + 16 * c), "r"(r < rows ? 16 : 0) : "memory");
                     }
                 } else {
                     constexpr int NK = (BR + step - 1) / step, UN = NK < 4 ? NK : 4;  // rows of a thread, in flight
@@ -531,6 +535,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         }
 #pragma unroll
                         for (int k = 0; k < UN; k++) {
+                            if (u0 / per + (k0 + k) * step >= rows) x[k][0] = x[k][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             const float f[8] = { x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w,
                                                  x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w };
                             uint32_t    hw[4], lw[4];
@@ -564,8 +569,8 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             const int     R    = w.n * a.G;
             const int     rb   = w.rt * BMN + q * BR;               // first row of this tile
             const int     rows = max(0, min(BR, R - rb));
-            const bool    mine = row < rows;                        // this thread's row exists
-            const bool    some = 32 * wq < rows;                    // the warp has a row
+            const bool    mine = (MM == 128 || lane < 16) && row < rows;  // this thread's row exists
+            const bool    some = MM / 4 * wq < rows;                      // the warp has a row
             // the next item, and its rows on their way to L2: from memory they take 2.4 us
             Walk       nw   = w;
             const bool more = boot || walk_next<BMN>(a, nw);
@@ -655,9 +660,9 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 if constexpr (NT == 1) {  // the other half of the row; both halves have read S before either writes P
                     float * rd = red + (turn & 1) * 2 * kBM;
                     turn++;
-                    rd[wg * kBM + row] = mt;
+                    rd[wg * kBM + tl] = mt;
                     named_bar_sync(1 + wq, 64);
-                    mt = fmaxf(mt, rd[(wg ^ 1) * kBM + row]);
+                    mt = fmaxf(mt, rd[(wg ^ 1) * kBM + tl]);
                 }
                 if (some) {
                     const float qs = a.softcap_l2 != 0.0f ? 1.0f : a.qscale;
@@ -682,7 +687,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         }
                         m = mn;
                     }
-                    const float off = (m == -INFINITY ? 0.0f : m) - kShift;
+                    const float off = !mine ? INFINITY : (m == -INFINITY ? 0.0f : m) - kShift;  // rows that are none: P = 0
                     const f2    q2 = f2_pack(qs, qs), o2 = f2_pack(-off, -off);
                     f2          l2[2] = { 0ull, 0ull };
 #pragma unroll
@@ -742,9 +747,9 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             if constexpr (NT == 1) {
                 float * rd = red + (turn & 1) * 2 * kBM;
                 turn++;
-                rd[wg * kBM + row] = l;
+                rd[wg * kBM + tl] = l;
                 named_bar_sync(1 + wq, 64);
-                l += rd[(wg ^ 1) * kBM + row];
+                l += rd[(wg ^ 1) * kBM + tl];
             }
             const int     o0 = NT == 2 ? 0 : OC * wg;
             const int     head = w.h * a.G + (rb + row - tok * a.G);
@@ -937,8 +942,8 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         } else if (warp == kSmWarps) {
             // ---------------- MMA ----------------
             // the warp walks together, one elected lane issues
-            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, kBN, kBM);
-            constexpr uint32_t idpv = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kMNMajor, D, kBM);
+            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, kBN, MM);
+            constexpr uint32_t idpv = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kMNMajor, D, MM);
             constexpr uint64_t sw   = 2ull << 61;
             const uint64_t     qd0  = tc::sdesc(smem_u32(sm + Ly::q), 16, 1024) | sw;  // addresses step by bytes / 16
             const uint64_t     kd0  = tc::sdesc(smem_u32(sm + Ly::ring), 16, 1024) | sw;
