@@ -30,6 +30,7 @@
 #include <atomic>
 #include <cmath>
 
+#include "fastdiv.cuh"
 #include "internal.h"
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -51,20 +52,6 @@ constexpr int   kMaxSeqs = 8192;
 constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s (a probe sleeps up to 4 us)
 constexpr int   kRawTok  = 32;     // tokens of a raw q8_0 slot
 constexpr int   kRawB    = kRawTok * 272;
-
-// n / d for 0 <= n < 2^31, d >= 1: one high product (d a power of two or not; the rounded-up reciprocal's error stays
-// under 1 / d for every n < 2^31)
-struct FastDiv {
-    uint32_t mul, shr, d;
-    static FastDiv of(uint32_t d) {
-        FastDiv f{ 0, 0, d };
-        while ((1ull << f.shr) < d) f.shr++;
-        // 2^(31 + shr) / d rounded up: below 2^32, since 2^shr < 2 d
-        f.mul = (uint32_t) (((1ull << (31 + f.shr)) + d - 1) / d);
-        return f;
-    }
-    __device__ __forceinline__ int div(int n) const { return (int) (((uint64_t) (uint32_t) n * mul) >> (31 + shr)); }
-};
 
 struct PArgs {
     const uint8_t * q;

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "fastdiv.cuh"
 #include "internal.h"
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -182,6 +183,7 @@ struct StoreArgs {
     const uint8_t * qkv;
     int64_t         ldb;
     int             n, H, Hkv, D;
+    FastDiv         by_units;
     const int32_t * pos;
     const int64_t * slots;
     uint8_t *       q;  // token stride qnb1, head stride qnb2
@@ -233,60 +235,77 @@ __device__ __forceinline__ void put4_q8(uint8_t * dst, int j, float4 v, int mode
 
 template <bool QF16, bool Q8>
 __global__ void __launch_bounds__(kStoreThreads) rope_kv_paged_kernel(const __grid_constant__ StoreArgs a) {
-    __shared__ __align__(16) float cs[kMaxHalf], sn[kMaxHalf];
+    __shared__ __align__(16) float cs[2][kMaxHalf], sn[2][kMaxHalf];
+    constexpr int NU = 3;  // units of a thread in flight: 48 heads of 128 or 32 of 256 in one turn
     pdl_launch_dependents();
     pdl_wait();
     const int half = a.D >> 1, units = half >> 2;  // 4-pair units per head
     const int total = (a.H + 2 * a.Hkv) * units;
-    for (int t = blockIdx.x; t < a.n; t += gridDim.x) {
+    int       par = 0;
+    for (int t = blockIdx.x; t < a.n; t += gridDim.x, par ^= 1) {
         const uint8_t * row  = a.qkv + (int64_t) t * a.ldb;
         const int64_t   slot = a.slots[t];
         const bool      keep = slot >= 0 && slot < a.n_slots;
+        float4          lo[NU], hi[NU];
+        // units is a multiple of 8, so 8 consecutive lanes hold 32 consecutive values of one head (a q8_0 block)
+        auto load = [&](int u0) {
+#pragma unroll
+            for (int k = 0; k < NU; k++) {
+                const int u = u0 + k * kStoreThreads;
+                if (u < total) {
+                    const int     hh = a.by_units.div(u), j = (u - hh * units) * 4;
+                    const float * x  = reinterpret_cast<const float *>(row) + hh * a.D;
+                    lo[k] = __ldcs(reinterpret_cast<const float4 *>(x + j));
+                    hi[k] = __ldcs(reinterpret_cast<const float4 *>(x + half + j));
+                }
+            }
+        };
+        load(threadIdx.x);
         if (threadIdx.x < half) {
             double turns = (double) a.pos[t] * a.freq[threadIdx.x];
             turns -= rint(turns);
             float s, c;
             sincospif((float) (2.0 * turns), &s, &c);
-            cs[threadIdx.x] = c;
-            sn[threadIdx.x] = s;
+            cs[par][threadIdx.x] = c;
+            sn[par][threadIdx.x] = s;
         }
-        const int64_t pg = keep ? slot / a.page : 0, off = keep ? slot % a.page : 0;
+        const int64_t pg = keep ? slot / a.page : 0, off = keep ? slot - pg * a.page : 0;
         uint8_t *     kd = a.kc + pg * a.knb3 + off * a.knb1;
         uint8_t *     vd = a.vc + pg * a.vnb3 + off * a.vnb1;
-        __syncthreads();
-        // units is a multiple of 8, so 8 consecutive lanes hold 32 consecutive values of one head (a q8_0 block)
-        for (int u = threadIdx.x; u < total; u += kStoreThreads) {
-            const int      hh = u / units, j = (u - hh * units) * 4;
-            const float *  x  = reinterpret_cast<const float *>(row) + (int64_t) hh * a.D;
-            float4         lo = __ldcs(reinterpret_cast<const float4 *>(x + j));
-            float4         hi = __ldcs(reinterpret_cast<const float4 *>(x + half + j));
-            if (hh < a.H + a.Hkv) {
-                const float4 c = *reinterpret_cast<const float4 *>(cs + j), s = *reinterpret_cast<const float4 *>(sn + j);
-                const float4 l = lo;
-                lo = make_float4(l.x * c.x - hi.x * s.x, l.y * c.y - hi.y * s.y, l.z * c.z - hi.z * s.z,
-                                 l.w * c.w - hi.w * s.w);
-                hi = make_float4(l.x * s.x + hi.x * c.x, l.y * s.y + hi.y * c.y, l.z * s.z + hi.z * c.z,
-                                 l.w * s.w + hi.w * c.w);
-            }
-            if (hh < a.H) {
-                uint8_t * d = a.q + (int64_t) t * a.qnb1 + (int64_t) hh * a.qnb2;
-                put4<QF16>(d, j, lo);
-                put4<QF16>(d, half + j, hi);
-            } else if (keep) {
-                const bool isk = hh < a.H + a.Hkv;
-                const int  g   = hh - a.H - (isk ? 0 : a.Hkv);
-                uint8_t *  d   = isk ? kd + (int64_t) g * a.knb2 : vd + (int64_t) g * a.vnb2;
-                if constexpr (Q8) {
-                    const uint32_t oct = 0xffu << (threadIdx.x & 24);
-                    put4_q8(d, j, lo, a.q8mode, oct);
-                    put4_q8(d, half + j, hi, a.q8mode, oct);
-                } else {
-                    put4<true>(d, j, lo);
-                    put4<true>(d, half + j, hi);
+        uint8_t *     qd = a.q + (int64_t) t * a.qnb1;
+        __syncthreads();  // one per token: the next one writes the other half of the angles
+        for (int u0 = threadIdx.x; u0 < total; u0 += NU * kStoreThreads) {
+            if (u0 != threadIdx.x) load(u0);
+#pragma unroll
+            for (int k = 0; k < NU; k++) {
+                const int u = u0 + k * kStoreThreads;
+                if (u >= total) break;
+                const int hh = a.by_units.div(u), j = (u - hh * units) * 4;
+                if (hh < a.H + a.Hkv) {
+                    const float4 c = *reinterpret_cast<const float4 *>(cs[par] + j), s = *reinterpret_cast<const float4 *>(sn[par] + j);
+                    const float4 l = lo[k], h = hi[k];
+                    lo[k] = make_float4(l.x * c.x - h.x * s.x, l.y * c.y - h.y * s.y, l.z * c.z - h.z * s.z, l.w * c.w - h.w * s.w);
+                    hi[k] = make_float4(l.x * s.x + h.x * c.x, l.y * s.y + h.y * c.y, l.z * s.z + h.z * c.z, l.w * s.w + h.w * c.w);
+                }
+                if (hh < a.H) {
+                    uint8_t * d = qd + (int64_t) hh * a.qnb2;
+                    put4<QF16>(d, j, lo[k]);
+                    put4<QF16>(d, half + j, hi[k]);
+                } else if (keep) {
+                    const bool isk = hh < a.H + a.Hkv;
+                    const int  g   = hh - a.H - (isk ? 0 : a.Hkv);
+                    uint8_t *  d   = isk ? kd + (int64_t) g * a.knb2 : vd + (int64_t) g * a.vnb2;
+                    if constexpr (Q8) {
+                        const uint32_t oct = 0xffu << (threadIdx.x & 24);
+                        put4_q8(d, j, lo[k], a.q8mode, oct);
+                        put4_q8(d, half + j, hi[k], a.q8mode, oct);
+                    } else {
+                        put4<true>(d, j, lo[k]);
+                        put4<true>(d, half + j, hi[k]);
+                    }
                 }
             }
         }
-        __syncthreads();
     }
 }
 
@@ -338,6 +357,7 @@ int rope_kv_paged_run(srhpm_ctx * ctx, const uint8_t * qkv, int64_t ldb, int n, 
     a.H       = H;
     a.Hkv     = Hkv;
     a.D       = D;
+    a.by_units = FastDiv::of((uint32_t) (D / 8));
     a.pos     = pos;
     a.slots   = slots;
     a.q       = reinterpret_cast<uint8_t *>(q_out->data);
@@ -354,8 +374,14 @@ int rope_kv_paged_run(srhpm_ctx * ctx, const uint8_t * qkv, int64_t ldb, int n, 
     a.page    = c.page;
     a.n_slots = c.n_pages * c.page;
     a.q8mode  = ctx->q8_0_act_mode;
-    const double two_pi = 6.283185307179586476925286766559;
-    for (int j = 0; j < D / 2; j++) a.freq[j] = pow((double) theta_base, -2.0 * j / D) / two_pi;
+    // the frequencies of a model stay the same from call to call: 128 powers took the host 5 us of a 9-row step
+    if (ctx->rope_base != theta_base || ctx->rope_dim != D) {
+        const double two_pi = 6.283185307179586476925286766559;
+        for (int j = 0; j < D / 2; j++) ctx->rope_freq[j] = pow((double) theta_base, -2.0 * j / D) / two_pi;
+        ctx->rope_base = theta_base;
+        ctx->rope_dim  = D;
+    }
+    std::copy(ctx->rope_freq, ctx->rope_freq + D / 2, a.freq);
     const int         grid = std::min(n, 8 * ctx->num_sms);
     const bool        qf = q_out->type == SRHPM_TYPE_F16, q8 = c.type == SRHPM_TYPE_Q8_0;
     const cudaError_t e = qf ? (q8 ? launch_k_pdl(rope_kv_paged_kernel<true, true>, dim3(grid), dim3(kStoreThreads), 0, stream, a)

@@ -101,7 +101,7 @@ def _paged(c, kv_type):
 
 def _ints(t, dtype, n, what):
     """Address of a contiguous integer or f32 vector of at least n values."""
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] < n or (n > 1 and t.stride(0) != 1):
+    if t.dtype is not dtype or not t.is_contiguous() or t.numel() < n:
         raise ValueError(f"{what} must be a contiguous {dtype} vector of at least {n} values")
     return t.data_ptr()
 
