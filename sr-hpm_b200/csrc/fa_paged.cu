@@ -43,7 +43,6 @@ constexpr float kLog2e   = 1.4426950408889634f;
 constexpr float kLazy    = 8.0f;   // raise the running maximum only beyond 2^8
 constexpr float kShift   = 7.0f;   // p is kept times 2^7
 constexpr int   kBM      = 128;    // rows of a tile
-constexpr int   kBN      = 128;    // tokens of a tile
 constexpr int   kSmWarps = 8;      // softmax warps
 constexpr int   kProd    = 3;      // producer warps (f16 cache)
 constexpr int   kConv    = 16;     // converter warps (q8_0 cache): K's two groups of four, then V's
@@ -86,11 +85,11 @@ struct Span {
 // q_start, clamped into the row buffer
 __device__ __forceinline__ int row_at(const PArgs & a, int s) { return min(max(a.q_start[s], 0), a.T); }
 
-template <int BMN> __device__ __forceinline__ Span span_of(const PArgs & a, int n, int kv, int rt) {
+template <int BMN, int BN> __device__ __forceinline__ Span span_of(const PArgs & a, int n, int kv, int rt) {
     const int     r0 = rt * BMN, r1 = min(n * a.G, r0 + BMN);  // T * G < 2^31 (checked)
     const int     t0 = a.byG.div(r0), t1 = a.byG.div(r1 - 1);
     const int     base = kv - n;
-    const int64_t cap  = min((int64_t) a.cols * a.page, (int64_t) INT32_MAX - kBN);
+    const int64_t cap  = min((int64_t) a.cols * a.page, (int64_t) INT32_MAX - BN);
     Span          p;
     p.hi = (int) max((int64_t) 0, min((int64_t) base + t1 + 1, cap));
     p.lo = a.window > 0 ? (int) max((int64_t) 0, (int64_t) base + t0 - a.window + 1) : 0;
@@ -98,8 +97,8 @@ template <int BMN> __device__ __forceinline__ Span span_of(const PArgs & a, int 
         p.kt0 = p.nkv = 0;
         p.lo = p.hi = 0;
     } else {
-        p.kt0 = p.lo / kBN;
-        p.nkv = (p.hi + kBN - 1) / kBN - p.kt0;
+        p.kt0 = p.lo / BN;
+        p.nkv = (p.hi + BN - 1) / BN - p.kt0;
     }
     p.units = max(p.nkv, 1);
     return p;
@@ -121,12 +120,12 @@ template <int BMN> __device__ __forceinline__ void walk_load(const PArgs & a, Wa
     w.n  = row_at(a, w.s + 1) - w.r0;
     w.kv = max(a.kv_len[w.s], 0);
 }
-template <int BMN> __device__ __forceinline__ void walk_item(const PArgs & a, Walk & w) {
-    w.sp   = span_of<BMN>(a, w.n, w.kv, w.rt);
+template <int BMN, int BN> __device__ __forceinline__ void walk_item(const PArgs & a, Walk & w) {
+    w.sp   = span_of<BMN, BN>(a, w.n, w.kv, w.rt);
     w.take = (int) min((int64_t) (w.sp.units - w.off), w.rem);
 }
 // to the next item; false at the end of the part
-template <int BMN> __device__ __forceinline__ bool walk_next(const PArgs & a, Walk & w) {
+template <int BMN, int BN> __device__ __forceinline__ bool walk_next(const PArgs & a, Walk & w) {
     w.rem -= w.take;
     if (w.rem <= 0) return false;
     w.off = 0;
@@ -140,7 +139,7 @@ template <int BMN> __device__ __forceinline__ bool walk_next(const PArgs & a, Wa
             } while (w.n <= 0);
         }
     }
-    walk_item<BMN>(a, w);
+    walk_item<BMN, BN>(a, w);
     return true;
 }
 
@@ -168,16 +167,19 @@ template <int NT> __device__ __forceinline__ void at_pos(int pos, int n, bool & 
 
 // ---- shared memory -----------------------------------------------------------------------------------------------
 template <int D, int NT, int BR, bool PREC, bool Q8> struct Lay {
-    static constexpr int CH     = D == 256 ? 2 : 1;            // chunks of a K or V tile
-    static constexpr int chunk  = kBN * D * 2 / CH;            // bytes: K 128 tokens x (D / CH) dims, V (128 / CH) tokens x D
-    static constexpr int vtok   = kBN / CH;                    // tokens of a V chunk
+    // q8_0: tiles of 64 tokens, one chunk each, so that K and V have two tiles each in half the f16 rings' memory: the next
+    // tile is converted while one is multiplied
+    static constexpr int BN     = Q8 ? 64 : 128;               // tokens of a tile
+    static constexpr int CH     = D == 256 && !Q8 ? 2 : 1;     // chunks of a K or V tile
+    static constexpr int chunk  = BN * D * 2 / CH;             // bytes: K BN tokens x (D / CH) dims, V (BN / CH) tokens x D
+    static constexpr int vtok   = BN / CH;                     // tokens of a V chunk
     static constexpr int qtile  = BR * D * 2;                  // one part (hi or lo) of one row tile
     static constexpr int qparts = PREC ? 2 : 1;
     static constexpr int q      = 0;                           // [NT][qparts][qtile]
     static constexpr int ring   = NT * qparts * qtile;
     // chunks in flight: what shared memory holds beside Q (at most 8); q8_0 gives the rest to the raw rows
     static constexpr int room   = 232448 - 2400 - ring;
-    // q8_0: K has a ring of one tile (2 chunks), V one of 1 or 2 chunks, the raw rows the rest
+    // q8_0: K has a ring of two chunks, V one of one or two, the raw rows the rest
     static constexpr int NS     = !Q8 ? (room / chunk < 8 ? room / chunk : 8) : BR < 128 && !PREC ? 4 : 3;
     static constexpr int raw    = ring + NS * chunk;
     static constexpr int NG     = !Q8 ? 0 : (room - NS * chunk) / (4 * kRawB) < 3 ? (room - NS * chunk) / (4 * kRawB) : 3;
@@ -314,9 +316,10 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     using Ly           = Lay<D, NT, BR, PREC, Q8>;
     constexpr int BMN  = BR * NT;
     constexpr int CH   = Ly::CH;
+    constexpr int BN   = Ly::BN;
     constexpr int NS   = Ly::NS;
     constexpr int MM   = BR <= 64 ? 64 : 128; // rows of a product
-    constexpr int NC   = NT == 2 ? 128 : 64;  // score columns per softmax thread
+    constexpr int NC   = NT == 2 ? 128 : BN / 2;  // score columns per softmax thread
     constexpr int OC   = NT == 2 ? D : D / 2; // output columns per softmax thread
     extern __shared__ __align__(1024) uint8_t sm[];
     uint64_t * kvfull  = reinterpret_cast<uint64_t *>(sm + Ly::bar);
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             int       u = 0;
             if (nt <= 2) {
                 const int kv = nt ? max(a.kv_len[s], 0) : 0;
-                for (int rt = 0; rt < nt; rt++) u += span_of<BMN>(a, n, kv, rt).units;
+                for (int rt = 0; rt < nt; rt++) u += span_of<BMN, BN>(a, n, kv, rt).units;
             } else {
                 big[atomicAdd(nbg, 1)] = s;  // any order: each entry is worked out by itself
             }
@@ -388,7 +391,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         for (int b = warp; b < *nbg; b += blockDim.x / 32) {
             const int s = big[b], r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = max(a.kv_len[s], 0);
             int       u = 0;
-            for (int rt = lane; rt < nt; rt += 32) u += span_of<BMN>(a, n, kv, rt).units;
+            for (int rt = lane; rt < nt; rt += 32) u += span_of<BMN, BN>(a, n, kv, rt).units;
             u = __reduce_add_sync(0xffffffffu, u);
             if (lane == 0) tot[s] = u;
         }
@@ -427,7 +430,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         int           off = (int) (in - (int64_t) h * per);
                         const int     r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = max(a.kv_len[s], 0);
                         for (int t0 = 0; t0 < nt; t0 += 32) {
-                            const int u  = t0 + lane < nt ? span_of<BMN>(a, n, kv, t0 + lane).units : 0;
+                            const int u  = t0 + lane < nt ? span_of<BMN, BN>(a, n, kv, t0 + lane).units : 0;
                             int       ic = u;
 #pragma unroll
                             for (int o = 1; o < 32; o <<= 1) {
@@ -472,7 +475,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         w.off = first[3];
         w.rem = range[1] - range[0];
         walk_load<BMN>(a, w);
-        walk_item<BMN>(a, w);
+        walk_item<BMN, BN>(a, w);
     }
 
     // registers go to the softmax warps (a row of scores each): the launch's 168 (q8_0: 72) per thread, shared out anew
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         // row of the tile: its tensor-memory lane, or with M = 64 16 rows in the lower lanes of each quarter
         const int row = MM == 64 ? 16 * wq + (lane & 15) : 32 * wq + lane, tl = 32 * wq + lane;
         const int q    = NT == 2 ? wg : 0;                              // row tile
-        const int c0   = NT == 2 ? 0 : 64 * wg;                         // first score column of this thread
+        const int c0   = NT == 2 ? 0 : NC * wg;                         // first score column of this thread
         uint32_t  rc0 = 0, sc[2] = { 0, 0 }, pvc = 0, pvw = 0, turn = 0, items = 0;
         // Q rows of an item to shared memory: 16-byte chunks of 8 dims, 128-byte swizzle. q_issue starts the copies (f32 rows:
         // does nothing yet), q_finish ends with the rows there and the MMA warp told. For the next item q_issue runs as
@@ -560,7 +563,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             const bool    some = MM / 4 * wq < rows;                      // the warp has a row
             // the next item, and its rows on their way to L2: from memory they take 2.4 us
             Walk       nw   = w;
-            const bool more = boot || walk_next<BMN>(a, nw);
+            const bool more = boot || walk_next<BMN, BN>(a, nw);
             if (more && nw.sp.nkv && !boot) {
                 constexpr int per = D * (PREC ? 4 : 2) / 128;  // lines of a row
                 const int     nr  = min(BMN, nw.n * a.G - nw.rt * BMN);
@@ -606,7 +609,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             }
             if (boot) continue;
             for (int i = 0; run && i < n; i++) {
-                const int b = NT == 2 ? q : (i & 1), t0 = (kt + i) * kBN;
+                const int b = NT == 2 ? q : (i & 1), t0 = (kt + i) * BN;
                 wait_bar(&s_full[b], sc[b] & 1, a.status, bad);
                 sc[b]++;
                 // done: these products were issued before this tile's scores
@@ -629,7 +632,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         for (int c = 0; c < NC; c++) s[c] = a.softcap_l2 * tanhf(s[c] * a.qscale);
                     }
                     // per 32 columns: all rows of the warp see them, none does, or lane by lane
-                    if (t0 < alo || t0 + kBN > ahi) {
+                    if (t0 < alo || t0 + BN > ahi) {
 #pragma unroll
                         for (int c = 0; c < NC; c += 32) {
                             const int u0 = t0 + c0 + c;
@@ -677,11 +680,12 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     const float off = !mine ? INFINITY : (m == -INFINITY ? 0.0f : m) - kShift;  // rows that are none: P = 0
                     const f2    q2 = f2_pack(qs, qs), o2 = f2_pack(-off, -off);
                     f2          l2[2] = { 0ull, 0ull };
+                    constexpr int CW = NC < 64 ? NC : 64;  // columns of a store
 #pragma unroll
-                    for (int c = 0; c < NC; c += 64) {
-                        uint32_t hi[32], lo[32];
+                    for (int c = 0; c < NC; c += CW) {
+                        uint32_t hi[CW / 2], lo[CW / 2];
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
+                        for (int e = 0; e < CW / 2; e++) {
                             float x0, x1;
                             f2_unpack(f2_fma(f2_pack(s[c + 2 * e], s[c + 2 * e + 1]), q2, o2), x0, x1);
                             x0 = ex2(x0);
@@ -694,8 +698,13 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                                 lo[e]            = *reinterpret_cast<const uint32_t *>(&r2);
                             }
                         }
-                        st32(tb + (c0 + c) / 2, hi);
-                        if constexpr (PREC) st32(tb + 64 + (c0 + c) / 2, lo);
+                        if constexpr (CW == 64) {
+                            st32(tb + (c0 + c) / 2, hi);
+                            if constexpr (PREC) st32(tb + BN / 2 + (c0 + c) / 2, lo);
+                        } else {
+                            tc::st16(tb + (c0 + c) / 2, hi);
+                            if constexpr (PREC) tc::st16(tb + BN / 2 + (c0 + c) / 2, lo);
+                        }
                     }
                     float y0, y1;
                     f2_unpack(f2_add(l2[0], l2[1]), y0, y1);
@@ -705,8 +714,8 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 pvc++;
                 if constexpr (!Q8) {
                     // V rows that no row of the item sees hold anything; 0 * NaN is NaN, so they become zeros
-                    if ((NT == 1 || q == 0) && (t0 < w.sp.lo || t0 + kBN > w.sp.hi)) {
-                        const int z0 = max(0, w.sp.lo - t0), z1 = min(kBN, w.sp.hi - t0);  // kept rows
+                    if ((NT == 1 || q == 0) && (t0 < w.sp.lo || t0 + BN > w.sp.hi)) {
+                        const int z0 = max(0, w.sp.lo - t0), z1 = min(BN, w.sp.hi - t0);  // kept rows
 #pragma unroll
                         for (int ch = 0; ch < CH; ch++) {
                             const uint32_t c = rc0 + v_pos<NT>(i, n) * CH + ch, slot = c % NS;
@@ -834,8 +843,8 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             const int pw = warp - kSmWarps - 1;
             uint32_t  rc = 0;                 // chunks (q8_0: raw slots) so far
             const int box = a.box;            // q8_0: at most kRawTok
-            const int nsub = kBN / box;       // boxes per 128 tokens: 2, 4 or 8
-            for (; active; active = walk_next<BMN>(a, w)) {
+            const int nsub = BN / box;       // boxes per 128 tokens: 2, 4 or 8
+            for (; active; active = walk_next<BMN, BN>(a, w)) {
                 const int n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
                 const int32_t * row = reinterpret_cast<const int32_t *>(a.table + (int64_t) w.s * a.tstride);
                 // lane j: page and place of the tile's j-th box, -1 when no row sees it
@@ -847,7 +856,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     } else {
                         at_pos<NT>(pos, n, isk, i);
                     }
-                    const int tok = (kt + i) * kBN + lane * box;
+                    const int tok = (kt + i) * BN + lane * box;
                     if (lane >= nsub || tok >= w.sp.hi || tok + box <= w.sp.lo) return -1;
                     const int pi = a.byPage.div(tok);
                     in           = tok - pi * a.page;
@@ -866,13 +875,12 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     const CUtensorMap * m = isk ? &mk : &mv;
                     if constexpr (Q8) {
                         constexpr uint32_t NG   = Ly::NG;
-                        constexpr int      NRAW = kBN / kRawTok;
+                        constexpr int      NRAW = BN / kRawTok;
                         const int     per  = kRawTok / box;  // boxes per raw slot: 1 or 2
 #pragma unroll 1
                         for (int r = 0; r < NRAW; r++, rc++) {
-                            // tokens 32 r ..: group r % 2 of K's or V's two
-                            const uint32_t own  = (rc >> 2) * 2 + (r >> 1);
-                            const int      slot = (pw * 2 + (r & 1)) * NG + own % NG;
+                            const uint32_t own  = rc >> 1;  // tokens 32 r .. are for group r of K's or V's two
+                            const int      slot = (pw * 2 + r) * NG + own % NG;
                             if (own >= NG) wait_bar(&rempty[slot], (own / NG - 1) & 1, a.status, bad);
                             if (bad) break;
                             const uint32_t seen = __ballot_sync(0xffffffffu, e >= 0) >> (r * per) & ((1u << per) - 1);
@@ -898,7 +906,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                             const int  ns     = isk ? nsub : nsub / CH;
                             const int  sub0   = isk ? 0 : ch * ns;
                             const int  p0     = isk ? ch * planes : 0;
-                            const int  rows   = isk ? kBN : Ly::vtok;
+                            const int  rows   = isk ? BN : Ly::vtok;
                             const int      box0 = lane * kProd + pw;  // box and plane of this lane: at most 16 in all
                             const int      j = box0 % ns, pl = box0 / ns;
                             const int      ee = __shfl_sync(0xffffffffu, e, (sub0 + j) & 31);
@@ -919,7 +927,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             if (bad) {  // the loads in flight land before this CTA's shared memory goes
                 if constexpr (Q8) {
                     for (uint32_t c = rc > 2 * Ly::NG ? rc - 2 * Ly::NG : 0; c < rc; c++) {
-                        const uint32_t own = (c >> 2) * 2 + ((c & 3) >> 1);
+                        const uint32_t own = c >> 1;
                         mbar_wait(&rfull[(pw * 2 + (c & 1)) * Ly::NG + own % Ly::NG], (own / Ly::NG) & 1);
                     }
                 } else {
@@ -929,7 +937,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         } else if (warp == kSmWarps) {
             // ---------------- MMA ----------------
             // the warp walks together, one elected lane issues
-            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, kBN, MM);
+            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, BN, MM);
             constexpr uint32_t idpv = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kMNMajor, D, MM);
             constexpr uint64_t sw   = 2ull << 61;
             const uint64_t     qd0  = tc::sdesc(smem_u32(sm + Ly::q), 16, 1024) | sw;  // addresses step by bytes / 16
@@ -940,10 +948,10 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             auto chunk_at = [&](bool isk, int i, int n, int ch, uint32_t & use) -> uint32_t {
                 uint32_t c;
                 if constexpr (Q8) {
-                    c = 2 * (rc0 + i) + ch;
+                    c = rc0 + i;
                     constexpr uint32_t nv = NS - 2;
                     use = isk ? c / 2 : c / nv;
-                    return isk ? (uint32_t) ch : 2 + c % nv;
+                    return isk ? c % 2 : 2 + c % nv;
                 } else {
                     c   = rc0 + (isk ? k_pos<NT>(i) : v_pos<NT>(i, n)) * CH + ch;
                     use = c / NS;
@@ -954,7 +962,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 const int n  = __shfl_sync(0xffffffffu, w.sp.nkv ? w.take : 0, 0);
                 const int nr = w.n * a.G - w.rt * BMN;
                 nw           = w;  // looked up now: behind the last product it would wait among the epilogue's stores
-                active       = walk_next<BMN>(a, nw);
+                active       = walk_next<BMN, BN>(a, nw);
                 if (n == 0) continue;
                 const int nq = __shfl_sync(0xffffffffu, NT == 2 && nr > BR ? 2 : 1, 0);
                 wait_bar(q_full, items & 1, a.status, bad);
@@ -966,7 +974,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
 #pragma unroll
                     for (int j = 0; j < D / CH / 16; j++) {
                         const int      jj = ch * (D / CH / 16) + j;  // k-step over all dims
-                        const uint64_t bd = kd + ((j >> 2) * (kBN * 128) + (j & 3) * 32) / 16;
+                        const uint64_t bd = kd + ((j >> 2) * (BN * 128) + (j & 3) * 32) / 16;
 #pragma unroll
                         for (int part = 0; part < Ly::qparts; part++) {
                             tc::mma_f16(tS + 128 * b, qd + (part * Ly::qtile + (jj >> 2) * (BR * 128) + (jj & 3) * 32) / 16, bd, idqk,
@@ -981,7 +989,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         const int jj = ch * (Ly::vtok / 16) + j;
 #pragma unroll
                         for (int part = 0; part < Ly::qparts; part++) {
-                            mma_f16_ta(tO + q * D, tS + 128 * b + part * 64 + jj * 8, vd + j * 2048 / 16, idpv,
+                            mma_f16_ta(tO + q * D, tS + 128 * b + part * (BN / 2) + jj * 8, vd + j * 2048 / 16, idpv,
                                        (uint32_t) (!first || jj > 0 || part > 0));
                         }
                     }
@@ -1011,7 +1019,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
 #pragma unroll
                         for (int ch = 0; ch < CH; ch++) {
                             sl[ch] = chunk_at(false, i, n, ch, use);
-                            if (!Q8 || ch == 0) wait_bar(&kvfull[sl[ch]], use & 1, a.status, bad);
+                            wait_bar(&kvfull[sl[ch]], use & 1, a.status, bad);
                         }
                         uint32_t & pc = (i & 1) ? pc1 : pc0;
                         wait_bar(&p_rdy[i & 1], pc & 1, a.status, bad);
@@ -1020,24 +1028,13 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         __syncwarp();
                         if (elect_one()) {
 #pragma unroll
-                            for (int ch = 0; ch < (Q8 ? 1 : CH); ch++) {
+                            for (int ch = 0; ch < CH; ch++) {
                                 pv_chunk(sl[ch], i & 1, 0, ch, i == 0);
                                 tc::commit(&kvempty[sl[ch]]);
                             }
-                            if (!Q8 || CH == 1) tc::commit(&pv_done[pvn & 1]);
+                            tc::commit(&pv_done[pvn & 1]);
                         }
                         __syncwarp();
-                        if constexpr (Q8) {  // its V ring may hold one chunk
-                            wait_bar(&kvfull[sl[1]], use & 1, a.status, bad);
-                            tc::fence_after();
-                            __syncwarp();
-                            if (elect_one()) {
-                                pv_chunk(sl[1], i & 1, 0, 1, false);
-                                tc::commit(&kvempty[sl[1]]);
-                                tc::commit(&pv_done[pvn & 1]);
-                            }
-                            __syncwarp();
-                        }
                     }
                 } else {  // one chunk per tile; K and V are waited for once, before the first row tile's P
                     uint32_t ks = chunk_at(true, 0, n, 0, use), vs = 0;
@@ -1085,58 +1082,40 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     } else if constexpr (Q8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(48));
         // ---------------- converters (q8_0): raw rows -> f16 chunks ----------------
-        // warp = (K or V; group: every other 32 tokens; quarter of the row: dims 64 qr .. 64 qr + 63, one swizzled plane).
+        // warp = (K or V; group: 32 of a tile's tokens; quarter of the row: dims 64 qr .. 64 qr + 63, one swizzled plane).
         // A job is 32 tokens: wait, load, unpack, store and fence take 0.7 us for 250 instructions, so 16 warps work at
         // once; K and V have chunks, raw rows and warps of their own, so that the next K does not queue behind a V that
-        // waits for its place (in one queue: 4.2 us per K and V tile). A group takes every use of its raw slots, and of
-        // the chunks that it fills, in order: a wait by parity must not skip one.
+        // waits for its place. A group takes every use of its raw slots, and of the chunks that it fills, in order: a wait
+        // by parity must not skip one.
         const int  qr = warp & 3, grp = ((warp - kSmWarps - 4) >> 2) & 1;
         const bool isk = warp < kSmWarps + 4 + kConv / 2;
         uint32_t   tile = 0;  // tiles so far
-        constexpr uint32_t NV = NS - 2;
-        for (; active; active = walk_next<BMN>(a, w)) {
+        for (; active; active = walk_next<BMN, BN>(a, w)) {
             const int n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
             for (int i = 0; i < n; i++, tile++) {
-#pragma unroll 1
-                for (int r = 0; r < 2; r++) {  // the tile's tokens 32 (2 r + grp) ..
-                    const uint32_t own = 2 * tile + r;
-                    const int      slot = ((isk ? 0 : 2) + grp) * Ly::NG + own % Ly::NG;
-                    uint8_t *      dst;
-                    if (isk) {
-                        if (r == 0 && tile > 0) {
-                            wait_bar(&kvempty[0], (tile - 1) & 1, a.status, bad);
-                            wait_bar(&kvempty[1], (tile - 1) & 1, a.status, bad);
-                        }
-                        dst = sm + Ly::ring + (qr >> 1) * Ly::chunk + (qr & 1) * (kBN * 128) + (32 * (2 * r + grp) + lane) * 128;
-                    } else {
-                        if (own >= NV) wait_bar(&kvempty[2 + own % NV], (own / NV - 1) & 1, a.status, bad);
-                        dst = sm + Ly::ring + (2 + own % NV) * Ly::chunk + qr * (64 * 128) + (32 * grp + lane) * 128;
-                    }
-                    wait_bar(&rfull[slot], (own / Ly::NG) & 1, a.status, bad);
-                    const uint8_t * src = sm + Ly::raw + slot * kRawB + lane * 272;
-                    switch (qr) {
-                        case 0: convert_q8<0>(src, dst, lane); break;
-                        case 1: convert_q8<1>(src, dst, lane); break;
-                        case 2: convert_q8<2>(src, dst, lane); break;
-                        default: convert_q8<3>(src, dst, lane); break;
-                    }
-                    // V rows that no row of the item sees hold anything; 0 * NaN is NaN, so they become zeros
-                    const int tok = (kt + i) * kBN + 32 * (2 * r + grp) + lane;
-                    if (!isk && (tok < w.sp.lo || tok >= w.sp.hi)) {
+                const uint32_t ring = isk ? 2 : NS - 2, at = (isk ? 0 : 2) + tile % ring;
+                const int      slot = ((isk ? 0 : 2) + grp) * Ly::NG + tile % Ly::NG;
+                if (tile >= ring) wait_bar(&kvempty[at], (tile / ring - 1) & 1, a.status, bad);
+                wait_bar(&rfull[slot], (tile / Ly::NG) & 1, a.status, bad);
+                uint8_t *       dst = sm + Ly::ring + at * Ly::chunk + qr * (64 * 128) + (32 * grp + lane) * 128;
+                const uint8_t * src = sm + Ly::raw + slot * kRawB + lane * 272;
+                switch (qr) {
+                    case 0: convert_q8<0>(src, dst, lane); break;
+                    case 1: convert_q8<1>(src, dst, lane); break;
+                    case 2: convert_q8<2>(src, dst, lane); break;
+                    default: convert_q8<3>(src, dst, lane); break;
+                }
+                // V rows that no row of the item sees hold anything; 0 * NaN is NaN, so they become zeros
+                const int tok = (kt + i) * BN + 32 * grp + lane;
+                if (!isk && (tok < w.sp.lo || tok >= w.sp.hi)) {
 #pragma unroll
-                        for (int c = 0; c < 8; c++) *reinterpret_cast<uint4 *>(dst + 16 * c) = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(&rempty[slot]);
-                        if (!isk) {
-                            mbar_arrive(&kvfull[2 + own % NV]);
-                        } else if (r == 1) {
-                            mbar_arrive(&kvfull[0]);
-                            mbar_arrive(&kvfull[1]);
-                        }
-                    }
+                    for (int c = 0; c < 8; c++) *reinterpret_cast<uint4 *>(dst + 16 * c) = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&rempty[slot]);
+                    mbar_arrive(&kvfull[at]);
                 }
             }
         }
