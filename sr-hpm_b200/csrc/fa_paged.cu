@@ -167,12 +167,16 @@ template <int NT> __device__ __forceinline__ void at_pos(int pos, int n, bool & 
 
 // ---- shared memory -----------------------------------------------------------------------------------------------
 template <int D, int NT, int BR, bool PREC, bool Q8> struct Lay {
-    // q8_0: tiles of 64 tokens, one chunk each, so that K and V have two tiles each in half the f16 rings' memory: the next
-    // tile is converted while one is multiplied
-    static constexpr int BN     = Q8 ? 64 : 128;               // tokens of a tile
-    static constexpr int CH     = D == 256 && !Q8 ? 2 : 1;     // chunks of a K or V tile
-    static constexpr int chunk  = BN * D * 2 / CH;             // bytes: K BN tokens x (D / CH) dims, V (BN / CH) tokens x D
+    // Tokens of a tile. f32 rows over q8_0: 64, since their V ring has one chunk, which then is a whole tile (131072 tokens:
+    // 141 us, with 128 162); f16 rows over q8_0: 128 (110 us, with 64 119: the softmax of 64 is mostly waiting).
+    static constexpr int BN     = Q8 && PREC ? 64 : 128;
+    static constexpr int CH     = BN * D > 128 * 128 ? BN * D / (128 * 128) : 1;  // chunks of a K or V tile, 32 KB at most
     static constexpr int vtok   = BN / CH;                     // tokens of a V chunk
+    // tokens of a K chunk: all, with D / CH dims each; q8_0: 64 with all dims, as its V, so that the next tile's first half
+    // is converted while the second half is multiplied
+    static constexpr int ktok   = Q8 ? 64 : BN;
+    static constexpr int kdim   = Q8 ? D : D / CH;
+    static constexpr int chunk  = BN * D * 2 / CH;             // bytes of either
     static constexpr int qtile  = BR * D * 2;                  // one part (hi or lo) of one row tile
     static constexpr int qparts = PREC ? 2 : 1;
     static constexpr int q      = 0;                           // [NT][qparts][qtile]
@@ -879,8 +883,8 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         const int     per  = kRawTok / box;  // boxes per raw slot: 1 or 2
 #pragma unroll 1
                         for (int r = 0; r < NRAW; r++, rc++) {
-                            const uint32_t own  = rc >> 1;  // tokens 32 r .. are for group r of K's or V's two
-                            const int      slot = (pw * 2 + r) * NG + own % NG;
+                            const uint32_t own  = rc >> 1;  // tokens 32 r .. are for group r % 2 of K's or V's two
+                            const int      slot = (pw * 2 + (r & 1)) * NG + own % NG;
                             if (own >= NG) wait_bar(&rempty[slot], (own / NG - 1) & 1, a.status, bad);
                             if (bad) break;
                             const uint32_t seen = __ballot_sync(0xffffffffu, e >= 0) >> (r * per) & ((1u << per) - 1);
@@ -937,7 +941,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         } else if (warp == kSmWarps) {
             // ---------------- MMA ----------------
             // the warp walks together, one elected lane issues
-            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, BN, MM);
+            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, Ly::ktok, MM);
             constexpr uint32_t idpv = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kMNMajor, D, MM);
             constexpr uint64_t sw   = 2ull << 61;
             const uint64_t     qd0  = tc::sdesc(smem_u32(sm + Ly::q), 16, 1024) | sw;  // addresses step by bytes / 16
@@ -948,7 +952,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             auto chunk_at = [&](bool isk, int i, int n, int ch, uint32_t & use) -> uint32_t {
                 uint32_t c;
                 if constexpr (Q8) {
-                    c = rc0 + i;
+                    c = CH * (rc0 + i) + ch;
                     constexpr uint32_t nv = NS - 2;
                     use = isk ? c / 2 : c / nv;
                     return isk ? c % 2 : 2 + c % nv;
@@ -971,13 +975,14 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 // products of one chunk (the elected lane)
                 auto qk_chunk = [&](uint32_t slot, int b, int q, int ch) {
                     const uint64_t kd = kd0 + slot * (Ly::chunk / 16), qd = qd0 + q * (Ly::qparts * Ly::qtile / 16);
+                    const uint32_t d  = tS + 128 * b + (Q8 ? ch * Ly::ktok : 0);
 #pragma unroll
-                    for (int j = 0; j < D / CH / 16; j++) {
-                        const int      jj = ch * (D / CH / 16) + j;  // k-step over all dims
-                        const uint64_t bd = kd + ((j >> 2) * (BN * 128) + (j & 3) * 32) / 16;
+                    for (int j = 0; j < Ly::kdim / 16; j++) {
+                        const int      jj = Q8 ? j : ch * (Ly::kdim / 16) + j;  // k-step over all dims
+                        const uint64_t bd = kd + ((j >> 2) * (Ly::ktok * 128) + (j & 3) * 32) / 16;
 #pragma unroll
                         for (int part = 0; part < Ly::qparts; part++) {
-                            tc::mma_f16(tS + 128 * b, qd + (part * Ly::qtile + (jj >> 2) * (BR * 128) + (jj & 3) * 32) / 16, bd, idqk,
+                            tc::mma_f16(d, qd + (part * Ly::qtile + (jj >> 2) * (BR * 128) + (jj & 3) * 32) / 16, bd, idqk,
                                         (uint32_t) (jj > 0 || part > 0));
                         }
                     }
@@ -1015,26 +1020,32 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     for (int i = 0; i < n; i++, pvn++) {
                         if (i + 1 < n) qk(i + 1);
                         // V first: it is there before P in most turns, and P's arrival is what the products wait for
-                        uint32_t sl[CH];
+                        // (a V ring of one chunk: its second half comes after the first half's products)
+                        constexpr int FIRST = Q8 && NS == 3 && CH == 2 ? 1 : CH;
+                        uint32_t      sl[CH];
 #pragma unroll
                         for (int ch = 0; ch < CH; ch++) {
                             sl[ch] = chunk_at(false, i, n, ch, use);
-                            wait_bar(&kvfull[sl[ch]], use & 1, a.status, bad);
+                            if (ch < FIRST) wait_bar(&kvfull[sl[ch]], use & 1, a.status, bad);
                         }
                         uint32_t & pc = (i & 1) ? pc1 : pc0;
                         wait_bar(&p_rdy[i & 1], pc & 1, a.status, bad);
                         pc++;
-                        tc::fence_after();
-                        __syncwarp();
-                        if (elect_one()) {
 #pragma unroll
-                            for (int ch = 0; ch < CH; ch++) {
-                                pv_chunk(sl[ch], i & 1, 0, ch, i == 0);
-                                tc::commit(&kvempty[sl[ch]]);
+                        for (int c0 = 0; c0 < CH; c0 += FIRST) {
+                            if (c0 > 0) wait_bar(&kvfull[sl[c0]], use & 1, a.status, bad);
+                            tc::fence_after();
+                            __syncwarp();
+                            if (elect_one()) {
+#pragma unroll
+                                for (int ch = c0; ch < c0 + FIRST; ch++) {
+                                    pv_chunk(sl[ch], i & 1, 0, ch, i == 0);
+                                    tc::commit(&kvempty[sl[ch]]);
+                                }
+                                if (c0 + FIRST == CH) tc::commit(&pv_done[pvn & 1]);
                             }
-                            tc::commit(&pv_done[pvn & 1]);
+                            __syncwarp();
                         }
-                        __syncwarp();
                     }
                 } else {  // one chunk per tile; K and V are waited for once, before the first row tile's P
                     uint32_t ks = chunk_at(true, 0, n, 0, use), vs = 0;
@@ -1082,21 +1093,21 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     } else if constexpr (Q8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(48));
         // ---------------- converters (q8_0): raw rows -> f16 chunks ----------------
-        // warp = (K or V; group: 32 of a tile's tokens; quarter of the row: dims 64 qr .. 64 qr + 63, one swizzled plane).
+        // warp = (K or V; group: 32 of a chunk's 64 tokens; quarter of the row: dims 64 qr .. 64 qr + 63, one swizzled plane).
         // A job is 32 tokens: wait, load, unpack, store and fence take 0.7 us for 250 instructions, so 16 warps work at
         // once; K and V have chunks, raw rows and warps of their own, so that the next K does not queue behind a V that
         // waits for its place. A group takes every use of its raw slots, and of the chunks that it fills, in order: a wait
         // by parity must not skip one.
         const int  qr = warp & 3, grp = ((warp - kSmWarps - 4) >> 2) & 1;
         const bool isk = warp < kSmWarps + 4 + kConv / 2;
-        uint32_t   tile = 0;  // tiles so far
+        uint32_t   own = 0;  // chunks so far
         for (; active; active = walk_next<BMN, BN>(a, w)) {
             const int n = w.sp.nkv ? w.take : 0, kt = w.sp.kt0 + w.off;
-            for (int i = 0; i < n; i++, tile++) {
-                const uint32_t ring = isk ? 2 : NS - 2, at = (isk ? 0 : 2) + tile % ring;
-                const int      slot = ((isk ? 0 : 2) + grp) * Ly::NG + tile % Ly::NG;
-                if (tile >= ring) wait_bar(&kvempty[at], (tile / ring - 1) & 1, a.status, bad);
-                wait_bar(&rfull[slot], (tile / Ly::NG) & 1, a.status, bad);
+            for (int i = 0; i < CH * n; i++, own++) {
+                const uint32_t ring = isk ? 2 : NS - 2, at = (isk ? 0 : 2) + own % ring;
+                const int      slot = ((isk ? 0 : 2) + grp) * Ly::NG + own % Ly::NG;
+                if (own >= ring) wait_bar(&kvempty[at], (own / ring - 1) & 1, a.status, bad);
+                wait_bar(&rfull[slot], (own / Ly::NG) & 1, a.status, bad);
                 uint8_t *       dst = sm + Ly::ring + at * Ly::chunk + qr * (64 * 128) + (32 * grp + lane) * 128;
                 const uint8_t * src = sm + Ly::raw + slot * kRawB + lane * 272;
                 switch (qr) {
@@ -1106,7 +1117,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     default: convert_q8<3>(src, dst, lane); break;
                 }
                 // V rows that no row of the item sees hold anything; 0 * NaN is NaN, so they become zeros
-                const int tok = (kt + i) * BN + 32 * grp + lane;
+                const int tok = kt * BN + 64 * i + 32 * grp + lane;
                 if (!isk && (tok < w.sp.lo || tok >= w.sp.hi)) {
 #pragma unroll
                     for (int c = 0; c < 8; c++) *reinterpret_cast<uint4 *>(dst + 16 * c) = make_uint4(0, 0, 0, 0);
