@@ -1147,7 +1147,7 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
     constexpr int VW = V >= 4 ? 4 : 2;
     constexpr int MO = 4;
     __shared__ float part_s[8][D];
-    __shared__ float l_s[8];
+    __shared__ float l_s[8], m_s[8];
     pdl_launch_dependents();
     pdl_wait();
     const int  c  = blockIdx.x;
@@ -1159,19 +1159,7 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
     for (int row = many ? blockIdx.y : blockIdx.y * 8 + warp; row < d1.y; row += many ? gridDim.y : gridDim.y * 8) {
         const int tok = a.byG.div(d1.x + row), h = d0.y * a.G + (d1.x + row - tok * a.G);
         auto      rec = [&](int p) { return (int64_t) (2 * (c + p) + (p == 0 ? 1 : 0)) * a.prow + row; };
-        float     M   = -INFINITY;
-        for (int p = lane; p < parts; p += 32) {
-            const float2 v = __ldcg(a.part_ms + rec(p));
-            if (v.y > 0.0f) M = fmaxf(M, v.x);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        float sk = -INFINITY;
-        if (a.sinks) {
-            sk = a.sinks[h] * kLog2e;
-            M  = fmaxf(M, sk);
-        }
-        float L = 0.0f, acc[V];
+        float     M = -INFINITY, L = 0.0f, acc[V];  // of this warp's parts
 #pragma unroll
         for (int e = 0; e < V; e++) acc[e] = 0.0f;
         const int first = many ? warp : 0, step = many ? 8 : 1;
@@ -1197,6 +1185,16 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
                     }
                 }
             }
+            float mn = M;
+#pragma unroll
+            for (int k = 0; k < MO; k++) mn = ms[k].y > 0.0f ? fmaxf(mn, ms[k].x) : mn;
+            if (mn > M) {
+                const float f = ex2(M - mn);  // 0 the first time
+                L *= f;
+#pragma unroll
+                for (int e = 0; e < V; e++) acc[e] *= f;
+                M = mn;
+            }
 #pragma unroll
             for (int k = 0; k < MO; k++) {
                 if (ms[k].y > 0.0f) {  // a record without weight may hold anything
@@ -1207,11 +1205,19 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
                 }
             }
         }
-        const float sink = sk > -INFINITY ? ex2(sk - M + kShift) : 0.0f;
+        const float sk = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
+        // weights relative to the larger of the maximum and the sink: of the sums so far, of the sink
+        auto with_sink = [&](float m, float & ws) {
+            const float top = fmaxf(m, sk);
+            ws              = sk > -INFINITY ? ex2(sk - top + kShift) : 0.0f;
+            return m > -INFINITY ? ex2(m - top) : 0.0f;
+        };
         uint8_t *   dst  = a.dst + (int64_t) h * a.dnb1 + (int64_t) (d0.z + tok) * a.dnb2;
         if (!many) {
-            L += sink;
-            const float f = L > 0.0f ? 1.0f / L : 0.0f;
+            float       ws;
+            const float wm = with_sink(M, ws);
+            L              = L * wm + ws;
+            const float f  = L > 0.0f ? wm / L : 0.0f;
 #pragma unroll
             for (int e = 0; e < V; e += VW) {
 #pragma unroll
@@ -1230,16 +1236,26 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
 #pragma unroll
                 for (int k = 0; k < VW; k++) part_s[warp][32 * e + lane * VW + k] = acc[e + k];
             }
-            if (lane == 0) l_s[warp] = L;
+            if (lane == 0) {
+                l_s[warp] = L;
+                m_s[warp] = M;
+            }
             __syncthreads();
-            L = sink;
+            float m = -INFINITY, wt[8], ws;
 #pragma unroll
-            for (int w = 0; w < 8; w++) L += l_s[w];
+            for (int w = 0; w < 8; w++) m = fmaxf(m, m_s[w]);
+            const float wm = with_sink(m, ws);
+            L              = ws;
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                wt[w] = m_s[w] > -INFINITY ? ex2(m_s[w] - m) * wm : 0.0f;
+                L     = fmaf(wt[w], l_s[w], L);
+            }
             const float f = L > 0.0f ? 1.0f / L : 0.0f;
             for (int at = threadIdx.x; at < D; at += 256) {
                 float o = 0.0f;
 #pragma unroll
-                for (int w = 0; w < 8; w++) o += part_s[w][at];
+                for (int w = 0; w < 8; w++) o = fmaf(wt[w], part_s[w][at], o);
                 if constexpr (F32) {
                     reinterpret_cast<float *>(dst)[at] = o * f;
                 } else {
