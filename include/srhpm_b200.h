@@ -341,7 +341,11 @@ int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, i
  * (q8_0: 256); page_size a multiple of 16; cache data 16-byte aligned, its strides multiples of 16; q and dst 16-byte
  * aligned with strides multiples of 16. Cache slots behind a sequence's kv_len and before its window may hold anything,
  * and pages wholly before the window may be given away (their entries are not read). A table entry that is not a page
- * of the cache reads as zeros and raises the context's device status. wdata: srhpm_flash_attn_paged_work_size bytes. */
+ * of the cache reads as zeros and raises the context's device status; positions behind the table's entries are not seen.
+ * Where the scores of a row hold a NaN, its result is NaN; a value of the cache that is infinite or NaN reaches every
+ * row of its sequence if one of them sees it. f32 q: finite in f16's range. dst overlaps neither q nor the caches.
+ * n_seqs <= 8192, and (T * n_head / n_head_kv / 56 + 1) * (entries * page_size / 64 + 1) < 2^31 (else
+ * SRHPM_UNSUPPORTED). wdata: srhpm_flash_attn_paged_work_size bytes, of the call alone until it is done. */
 int srhpm_flash_attn_paged_work_size(const srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_tensor * k_cache,
                                      int n_seqs, size_t * size);
 int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_tensor * k_cache,
@@ -361,7 +365,8 @@ int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_
  * f32 [T] or NULL: p_r(x) of each row with a drafted token, 0 for a last row. Padding rows of out_ids and p_draft stay
  * as they are. u_accept f32 [T], u_sample f32 [n_seqs], in [0, 1). The weights of a drawn token and their sums are
  * kept in 64 bits, so the token does not hang on the order of summation (a weight below 2^-990 of the row's largest
- * counts as 0). n_vocab <= 2^29. wdata: srhpm_verify_sample_work_size bytes. */
+ * counts as 0). n_vocab <= 2^29; T and n_seqs <= 2^24. wdata: srhpm_verify_sample_work_size bytes, of the call alone until
+ * it is done. */
 int srhpm_verify_sample_work_size(const srhpm_ctx * ctx, const srhpm_tensor * logits, int n_seqs, size_t * size);
 int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start,
                         int n_seqs, const srhpm_tensor * draft_probs, const float * temperature,

@@ -759,7 +759,7 @@ int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_
 }
 
 int srhpm_verify_sample_work_size(const srhpm_ctx * ctx, const srhpm_tensor * logits, int n_seqs, size_t * size) {
-    if (!ctx || !size || n_seqs < 1) return SRHPM_ERR_INVALID;
+    if (!ctx || !size || n_seqs < 1 || n_seqs > (1 << 24)) return SRHPM_ERR_INVALID;
     const int st = check_logits(logits, 1);
     if (st != SRHPM_OK) return st;
     if (logits->ne[1] > (1 << 24)) return SRHPM_ERR_INVALID;
@@ -771,7 +771,8 @@ int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int3
                         int n_seqs, const srhpm_tensor * draft_probs, const float * temperature,
                         const float * u_accept, const float * u_sample, int32_t * out_ids, int32_t * out_n,
                         float * p_draft, void * wdata, size_t wsize, void * stream) {
-    if (!ctx || !ids || !q_start || !u_accept || !u_sample || !out_ids || !out_n || n_seqs < 1) return SRHPM_ERR_INVALID;
+    if (!ctx || !ids || !q_start || !u_accept || !u_sample || !out_ids || !out_n) return SRHPM_ERR_INVALID;
+    if (n_seqs < 1 || n_seqs > (1 << 24)) return SRHPM_ERR_INVALID;
     int st = check_logits(logits, 1);
     if (st != SRHPM_OK) return st;
     if (logits->ne[1] > (1 << 24)) return SRHPM_ERR_INVALID;

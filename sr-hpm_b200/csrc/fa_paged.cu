@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         L += ex2(sk - m + kShift);
                     }
                 }
-                f = L > 0.0f ? f / L : 0.0f;
+                f = L == 0.0f ? 0.0f : f / L;  // a NaN stays one
             } else if (mine && (NT == 2 || wg == 0)) {
                 a.part_ms[(int64_t) slot * a.prow + q * BR + row] = make_float2(m, l);
             }
@@ -1198,7 +1198,7 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
             }
             float mn = M;
 #pragma unroll
-            for (int k = 0; k < MO; k++) mn = ms[k].y > 0.0f ? fmaxf(mn, ms[k].x) : mn;
+            for (int k = 0; k < MO; k++) mn = ms[k].y == 0.0f ? mn : fmaxf(mn, ms[k].x);
             if (mn > M) {
                 const float f = ex2(M - mn);  // 0 the first time
                 L *= f;
@@ -1208,7 +1208,7 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
             }
 #pragma unroll
             for (int k = 0; k < MO; k++) {
-                if (ms[k].y > 0.0f) {  // a record without weight may hold anything
+                if (!(ms[k].y == 0.0f)) {  // a record without weight may hold anything; a NaN stays one
                     const float w = ex2(ms[k].x - M);
                     L             = fmaf(w, ms[k].y, L);
 #pragma unroll
@@ -1228,7 +1228,7 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
             float       ws;
             const float wm = with_sink(M, ws);
             L              = L * wm + ws;
-            const float f  = L > 0.0f ? wm / L : 0.0f;
+            const float f  = L == 0.0f ? 0.0f : wm / L;
 #pragma unroll
             for (int e = 0; e < V; e += VW) {
 #pragma unroll
@@ -1262,7 +1262,7 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
                 wt[w] = m_s[w] > -INFINITY ? ex2(m_s[w] - m) * wm : 0.0f;
                 L     = fmaf(wt[w], l_s[w], L);
             }
-            const float f = L > 0.0f ? 1.0f / L : 0.0f;
+            const float f = L == 0.0f ? 0.0f : 1.0f / L;
             for (int at = threadIdx.x; at < D; at += 256) {
                 float o = 0.0f;
 #pragma unroll
@@ -1349,6 +1349,9 @@ size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, i
 int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t wsize, cudaStream_t stream) {
     const int D = v.c.D, G = v.H / v.c.Hkv;
     if (v.S > kMaxSeqs || (int64_t) v.T * G + 2 * kBM > INT32_MAX) return SRHPM_UNSUPPORTED;
+    // a sequence's units per KV head are counted in 32 bits: tiles of 56 rows or more times tiles of 64 tokens or more
+    const int64_t seen = std::min<int64_t>((int64_t) v.cols * v.c.page, INT32_MAX);
+    if (((int64_t) v.T * G / kFew + 1) * (seen / 64 + 1) > INT32_MAX) return SRHPM_UNSUPPORTED;
     if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.c.Hkv, D, v.S, v.f32 && v.c.type == SRHPM_TYPE_Q8_0)) return SRHPM_ERR_WORKSPACE;
     const Tile tl = tile_of(v.T, v.S, G, D, v.f32 && v.c.type == SRHPM_TYPE_Q8_0);
     PArgs      a;

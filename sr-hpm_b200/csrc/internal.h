@@ -22,6 +22,7 @@ struct srhpm_ctx {
     std::unordered_map<uintptr_t, int>    sync_slots;  // work buffer (aligned base) -> counter index
     int                                   sync_next = 0;
     // RoPE frequencies (turns per position) of the last base and head size that rope_kv_paged was called with
+    std::mutex rope_mu;
     float  rope_base = 0.0f;
     int    rope_dim  = 0;
     double rope_freq[128];

@@ -76,7 +76,7 @@ __device__ __forceinline__ int64_t cta_incl(int64_t v, int64_t * sp, int64_t * t
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs a) {
     extern __shared__ int32_t sh[];
     int32_t *          start = sh;              // [S + 1] first row of each sequence (saturated)
-    int32_t *          first = sh + a.S + 1;    // [S] index of its first new page in the free list, -1: refused
+    int32_t *          first = sh + a.S + 1;    // [S] index of its first new page in the free list (0: needs none), -1: refused
     __shared__ int64_t sp[32];
     pdl_launch_dependents();
     pdl_wait();
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
         // pages handed out: the end of the last sequence that got its own (ends rise, so it is their maximum)
         if (in) {
             start[s] = (int32_t) min(row_end - max(nw, (int64_t) 0), (int64_t) INT32_MAX);
-            first[s] = st == SRHPM_PAGES_OK ? (int32_t) (head + end - need) : -1;
+            first[s] = st != SRHPM_PAGES_OK ? -1 : need > 0 ? (int32_t) (head + end - need) : 0;
             if (blockIdx.x == 0) {
                 a.q_start[s] = start[s];
                 a.kv_len[s]  = st == SRHPM_PAGES_OK ? (int32_t) (pa + nw) : 0;
@@ -375,13 +375,16 @@ int rope_kv_paged_run(srhpm_ctx * ctx, const uint8_t * qkv, int64_t ldb, int n, 
     a.n_slots = c.n_pages * c.page;
     a.q8mode  = ctx->q8_0_act_mode;
     // the frequencies of a model stay the same from call to call: 128 powers took the host 5 us of a 9-row step
-    if (ctx->rope_base != theta_base || ctx->rope_dim != D) {
-        const double two_pi = 6.283185307179586476925286766559;
-        for (int j = 0; j < D / 2; j++) ctx->rope_freq[j] = pow((double) theta_base, -2.0 * j / D) / two_pi;
-        ctx->rope_base = theta_base;
-        ctx->rope_dim  = D;
+    {
+        std::lock_guard<std::mutex> lk(ctx->rope_mu);  // threads that share the context
+        if (ctx->rope_base != theta_base || ctx->rope_dim != D) {
+            const double two_pi = 6.283185307179586476925286766559;
+            for (int j = 0; j < D / 2; j++) ctx->rope_freq[j] = pow((double) theta_base, -2.0 * j / D) / two_pi;
+            ctx->rope_base = theta_base;
+            ctx->rope_dim  = D;
+        }
+        std::copy(ctx->rope_freq, ctx->rope_freq + D / 2, a.freq);
     }
-    std::copy(ctx->rope_freq, ctx->rope_freq + D / 2, a.freq);
     const int         grid = std::min(n, 8 * ctx->num_sms);
     const bool        qf = q_out->type == SRHPM_TYPE_F16, q8 = c.type == SRHPM_TYPE_Q8_0;
     const cudaError_t e = qf ? (q8 ? launch_k_pdl(rope_kv_paged_kernel<true, true>, dim3(grid), dim3(kStoreThreads), 0, stream, a)

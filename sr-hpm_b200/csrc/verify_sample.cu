@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(kPartThreads, 4) sample_part_kernel(const Samp
         if (nj < jobs) fetch(nt, na, ne);
         if (v.temp && t != known) {  // with the loads in flight
             const int s = seq_of_row(v, t);
-            c           = s >= 0 ? kLog2e / v.temp[s] : kLog2e;
+            c           = s >= 0 ? fminf(kLog2e / v.temp[s], FLT_MAX) : kLog2e;  // finite: 0 c is 0
             known       = t;
         }
         float mt = m;
@@ -203,14 +204,18 @@ struct Exp64 {
     double a, b;   // y = a x + b
     float  least;  // x below it: 0
     float  mf;
-    int    top, mode;  // 0: as above; 1: the maximum is +inf, all weight on those; 2: all weight on `top`
+    // 0: as above; 1: all weight on the places of the maximum (+inf, or a temperature so low that the next smaller f32 has
+    // none: y would be the rounding of m (log2 e / t) there); 2: all weight on `top`
+    int    top, mode;
     __device__ __forceinline__ void set(float m, int t, float temp) {
         mf   = m;
         top  = t;
-        mode = !(temp > 0.0f) ? 2 : m == INFINITY ? 1 : 0;
+        // low temperatures: a step of an f32 is many times t; beyond 708 t the exponent would leave the doubles' range
+        least = fmaxf(m - 690.0f * temp, -FLT_MAX);
+        if (m - least > 700.0f * temp) least = nextafterf(least, INFINITY);
+        mode = !(temp > 0.0f) ? 2 : m == INFINITY || (m > -INFINITY && least == m) ? 1 : 0;
         a    = mode == 0 ? 1.4426950408889634 / (double) temp : 0.0;
         b    = mode == 0 && m > -INFINITY ? -(double) m * a : 0.0;
-        least = mode == 0 ? m - 690.0f * temp : 0.0f;
     }
     template <bool ZERO> __device__ __forceinline__ double of(float x) const {
         const double y = fma((double) fmaxf(x, least), a, b);
@@ -271,7 +276,7 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
         return;
     }
     const float  tf    = v.temp ? v.temp[s] : 1.0f;
-    const float  c     = tf > 0.0f ? kLog2e / tf : 0.0f;
+    const float  c     = tf > 0.0f ? fminf(kLog2e / tf, FLT_MAX) : 0.0f;
 
     // ---- acceptance: a warp per row, kPickWarps rows at a time; every CTA of the cluster decides for itself
     Exp64 ex;
@@ -636,10 +641,10 @@ int verify_sample_run(srhpm_ctx * ctx, const SampleView & v, void * wdata, size_
     ctx->launches.fetch_add(1);
     if (st != SRHPM_OK) return st;
     // as many CTAs per sequence as one wave of two per SM holds: a wave and a bit would take twice as long
-    const int64_t slots = 2 * (int64_t) ctx->num_sms;
-    if (v.S * 16 <= slots) return launch_pick<16>(ctx, a, stream);
-    if (v.S * 8 <= slots) return launch_pick<8>(ctx, a, stream);
-    if (v.S * 4 <= slots) return launch_pick<4>(ctx, a, stream);
+    const int64_t slots = 2 * (int64_t) ctx->num_sms, S = v.S;
+    if (S * 16 <= slots) return launch_pick<16>(ctx, a, stream);
+    if (S * 8 <= slots) return launch_pick<8>(ctx, a, stream);
+    if (S * 4 <= slots) return launch_pick<4>(ctx, a, stream);
     return launch_pick<2>(ctx, a, stream);
 }
 

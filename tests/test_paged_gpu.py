@@ -99,6 +99,15 @@ def test_plan_strided_table_and_largest_lengths(ctx):
 
 
 # ---- RoPE and the paged store ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("head", [-1, -2 ** 31, 2 ** 31 - 1])
+def test_plan_heads_outside_the_list(ctx, head):
+    """A sequence that needs no page keeps its rows; one that needs a page is refused."""
+    table = np.array([[4, -1, -1], [9, 2, -1], [7, -1, -1]], np.int32)
+    past, new = np.array([3, 17, 16], np.int32), np.array([5, 2, 1], np.int32)
+    r = check_plan(ctx, past, new, table, np.arange(5, dtype=np.int32), 16, 9, head)
+    assert r.status.cpu().tolist() == [0, 0, 2]
+
+
 @pytest.mark.parametrize("kv,D,H,Hkv,P,n,qt", [
     (L.F16, 256, 24, 4, 64, 9, torch.float32), (L.F16, 128, 7, 7, 48, 33, torch.float16),
     (L.F16, 64, 5, 1, 16, 1, torch.float32), (L.Q8_0, 256, 6, 2, 32, 70, torch.float16),
@@ -164,6 +173,37 @@ def test_store_modes_and_head_major_pages(ctx):
         for c, w in ((kc, rows[:, H:H + Hkv]), (vc, rows[:, H + Hkv:])):  # position 0: keys are not turned
             got = c.cpu().numpy().reshape(2 * P, Hkv, 272)[14:20]
             assert np.array_equal(got, O.cache_rows(L.Q8_0, np.ascontiguousarray(w), mode))
+
+
+def test_store_threads_with_bases_of_their_own(ctx):
+    """Two host threads on one context, two streams, two bases: each gets its own angles every time."""
+    import threading
+    n, H, Hkv, D, P = 5, 2, 1, 64, 16
+    x = torch.randn((n, (H + 2 * Hkv) * D), device="cuda")
+    pos, slots = (torch.arange(n, device="cuda", dtype=t) for t in (torch.int32, torch.int64))
+    kc, vc = (torch.zeros((4, P, Hkv, D * 2), dtype=torch.uint8, device="cuda") for _ in range(2))
+    bases = (1e4, 1e6)
+    outs = [[torch.zeros((n, H, D), device="cuda") for _ in range(100)] for _ in bases]
+    want = [ctx.rope_kv_paged(x, pos + 40000, slots, kc, vc, L.F16, torch.zeros((n, H, D), device="cuda"), theta_base=b)
+            for b in bases]
+    at = pos + 40000
+    streams = [torch.cuda.Stream() for _ in bases]
+    torch.cuda.synchronize()
+
+    def run(i):
+        for o in outs[i]:
+            ctx.rope_kv_paged(x, at, slots, kc, vc, L.F16, o, theta_base=bases[i], stream=streams[i])
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    ctx.check()
+    for w, os_ in zip(want, outs):
+        for o in os_:
+            assert torch.equal(o, w)
 
 
 # ---- attention over pages --------------------------------------------------------------------------------------------
@@ -458,6 +498,27 @@ def test_attention_same_twice(ctx):
         assert torch.equal(one, two)
 
 
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+@pytest.mark.parametrize("kv,D", [(L.F16, 64), (L.F16, 128), (L.F16, 256), (L.Q8_0, 256)])
+@pytest.mark.parametrize("past,new,at", [([300], [3], 301), ([9000, 40], [2, 1], 100), ([0], [500], 130), ([20000], [40], 7)])
+def test_attention_nan_keys(ctx, qt, kv, D, past, new, at):
+    """A NaN among the keys of KV head 0: the rows of its heads that see it are NaN, whole and cut items alike, all others
+    keep their bits."""
+    rng = np.random.default_rng(14)
+    P, H, Hkv = 32, 4, 2
+    q, caches, vals, table, q_start, kv_len = attn_case(rng, past, new, H, Hkv, D, P, kv, qt)
+    d = [cu(x) for x in (q, caches[0], caches[1], table, q_start, kv_len)]
+    clean = ctx.flash_attn_paged(d[0], d[1], d[2], kv, d[3], d[4], d[5], scale=0.1).cpu().numpy()
+    d[1][int(table[0, at // P]), at % P, 0, :2] = 0x7e  # f16 0x7e7e: a value or a block's step
+    got = ctx.flash_attn_paged(d[0], d[1], d[2], kv, d[3], d[4], d[5], scale=0.1).cpu().numpy()
+    ctx.check()
+    sees = np.zeros((q.shape[0], H, 1), bool)
+    sees[max(0, at - past[0]):new[0], :H // Hkv] = True
+    assert np.isnan(got[np.broadcast_to(sees, got.shape)]).all()
+    keep = ~np.broadcast_to(sees, got.shape)
+    assert np.array_equal(got[keep], clean[keep]) and np.isfinite(clean).all()
+
+
 # ---- acceptance by sampling ------------------------------------------------------------------------------------------
 def sample_case(rng, ks, V, draft=True, agree=True):
     T = int(sum(ks)) + len(ks)
@@ -576,6 +637,18 @@ def test_sample_frequencies(ctx):
     p = np.exp(lg1.astype(np.float64))
     p /= p.sum()
     assert (np.abs(got - n * p) <= 5 * np.sqrt(n * p * (1 - p))).all()
+
+
+def test_sample_temperatures(ctx):
+    """From all weight on the maxima (two equal ones) to uniform. The bound of p holds at 1e-9 too: m / t log2 e there is
+    rounded to 2^-20, which is the error of a weight's exponent."""
+    rng = np.random.default_rng(4)
+    temp = np.array([1e-3, 1e-5, 1e-7, 1e-9, 1e-20, 1e-37, 1e3, 1e20, 1e36, np.inf], np.float32)
+    for draft in (True, False):
+        lg, ids, q_start, u, us, dp = sample_case(rng, [3] * len(temp), 1500, draft)
+        lg[:, 700] = lg[:, 90] = lg.max(1) + 0.5
+        ids[1::2] = 700
+        sample_check(ctx, lg, ids, q_start, u, us, dp, temp)
 
 
 # ---- together --------------------------------------------------------------------------------------------------------

@@ -104,6 +104,15 @@ def test_flash_attn_paged(o, st):
     assert attn(**o) == st
 
 
+@pytest.mark.parametrize("o", [
+    dict(tb=table(S=8193)),  # sequences
+    dict(q=rows(T=1 << 24, H=512, nb1=256 * 1024), dst=rows(T=1 << 24, H=512, head_first=True)),  # rows of a KV head
+    dict(q=rows(T=1 << 24), dst=rows(T=1 << 24, head_first=True), tb=table(cols=1200)),  # tiles: 1797560 x 1201
+    dict(q=rows(T=1 << 16), dst=rows(T=1 << 16, head_first=True), tb=table(cols=1 << 30))])  # 7022 x 2^25 (2^31 tokens)
+def test_flash_attn_paged_too_large(o):
+    assert attn(**o) == L.UNSUPPORTED
+
+
 def sample(lg=None, ids=A, qs=A, S=2, dp=None, u=A, us=A, oi=A, on=A, w=A, ws=1 << 30):
     lg = lg or view(L.F32, [1000, 5], [4, 4000])
     return lib.srhpm_verify_sample(CTX, ctypes.byref(lg), ids, qs, S, ctypes.byref(dp) if dp else None, None, u, us, oi,
@@ -117,6 +126,13 @@ def sample(lg=None, ids=A, qs=A, S=2, dp=None, u=A, us=A, oi=A, on=A, w=A, ws=1 
     (dict(dp=view(L.F32, [1000, 4], [4, 4000])), L.ERR_INVALID), (dict(dp=view(L.F32, [999, 5], [4, 4000])), L.ERR_INVALID)])
 def test_verify_sample(o, st):
     assert sample(**o) == st
+
+
+def test_verify_sample_too_many_sequences():
+    assert sample(S=(1 << 24) + 1) == L.ERR_INVALID
+    size = ctypes.c_size_t()
+    lg = view(L.F32, [1000, 5], [4, 4000])
+    assert lib.srhpm_verify_sample_work_size(CTX, ctypes.byref(lg), (1 << 24) + 1, ctypes.byref(size)) == L.ERR_INVALID
 
 
 def test_python_layer():
