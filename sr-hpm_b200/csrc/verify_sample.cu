@@ -197,9 +197,12 @@ __global__ void __launch_bounds__(kPartThreads, 4) sample_part_kernel(const Samp
     }
 }
 
-// exp((x - m) / t) in 64 bits, x <= m, as 2^y, y = x (log2 e / t) - m (log2 e / t) = k + f with |f| <= 1/2: 2^f by the series
-// of exp(f ln 2) up to the 11th power (its rest: (ln 2 / 2)^12 / 12! < 2^-45), k added to the exponent. 16 instructions of
-// 64 bits, no table and no branches: these are what a drawn token costs. Weights below e^-690 of the row's largest are 0.
+// exp((x - m) / t) in 64 bits, x <= m, as 2^y, y = x (log2 e / t) - m (log2 e / t) = k + f with |f| <= 1/2: 2^f by the
+// polynomial that meets it in the 9 Chebyshev points of [-1/2, 1/2] (off by 2^-39.8 at most; the series of exp needs
+// two powers more for the same), k added to the exponent. 13 instructions of 64
+// bits, no table and no branches: these are what a drawn token costs. Weights below e^-690 of the row's largest are 0.
+__constant__ double kPow2[8] = { 0.6931471805459335,    0.2402265069581299,     0.05550410941205933,    0.009618129159402558,
+                                 0.0013333450568000645, 0.00015403455852453838, 1.5310079402249296e-05, 1.3255224878668817e-06 };
 struct Exp64 {
     double a, b;   // y = a x + b
     float  least;  // x below it: 0
@@ -221,17 +224,10 @@ struct Exp64 {
         const double y = fma((double) fmaxf(x, least), a, b);
         const double t = y + 6755399441055744.0;  // rounds to a whole number
         const double f = y - (t - 6755399441055744.0);
-        double       p = fma(f, 4.4455382718708116e-10, 7.054911620801123e-09);
-        p        = fma(p, f, 1.01780860092397e-07);
-        p        = fma(p, f, 1.321548679014431e-06);
-        p        = fma(p, f, 1.5252733804059841e-05);
-        p        = fma(p, f, 0.0001540353039338161);
-        p        = fma(p, f, 0.0013333558146428443);
-        p        = fma(p, f, 0.009618129107628477);
-        p        = fma(p, f, 0.05550410866482158);
-        p        = fma(p, f, 0.24022650695910072);
-        p        = fma(p, f, 0.6931471805599453);
-        p        = fma(p, f, 1.0);
+        double       p = kPow2[7];
+#pragma unroll
+        for (int i = 6; i >= 0; i--) p = fma(p, f, kPow2[i]);
+        p = fma(p, f, 1.0);
         p = __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
         return !ZERO || x >= least ? p : 0.0;
     }
@@ -406,7 +402,6 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
     // told apart by the f32 records' Z: a token on the wrong side has |e / Z - q| below 2^-20 of either, and few are that
     // near, so the block's weight (sum e) / Z - sum q is as good as its terms.
     {
-        const float pzf = (float) pz;
         double      sz = 0.0;
         auto block = [&](auto pieces, int at, double & se, double & sq) {  // `pieces` times 128 tokens from `at`
             constexpr int P = decltype(pieces)::value;
@@ -449,9 +444,10 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
                     sz += (w[0] + w[1]) + (w[2] + w[3]);
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const bool over = ex.mode == 0 ? fast_ex2((l[k][e] - pm) * c) > q[k][e] * pzf : w[e] > (double) q[k][e] * pz;
-                        se += over ? w[e] : 0.0;
-                        sq += (double) (over ? q[k][e] : 0.0f);
+                        const double qe = q[k][e];
+                        asm("{\n\t.reg .pred p;\n\tsetp.gt.f64 p, %2, %3;\n\t@p add.f64 %0, %0, %2;\n\t@p add.f64 %1, %1, %4;\n\t}"
+                            : "+d"(se), "+d"(sq)
+                            : "d"(w[e]), "d"(qe * pz), "d"(qe));
                     }
                 } else {
                     if (x >= j && x < j + 4) {
@@ -550,14 +546,22 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
             if (blk < 0) blk = g1 - g0 - 1;
             double start = before + (blk > 0 ? bsum[blk - 1] : 0.0);
             int    at = -1, lastw = -1;
-            for (int k = 0; k < len && at < 0; k += 128) {
-                const int j = (g0 + blk) * len + k + lane * 4;
-                float     l[4], q[4];
-                double    w[4];
-                logits4(j, l);
-                drafts4(j, q);
-                weights(j, l, q, w);
-                double t4 = (w[0] + w[1]) + (w[2] + w[3]), inc = t4;
+            auto place = [&](auto pieces, int from) {  // 4 `pieces` tokens in a row per lane: one sum across the lanes
+                constexpr int P = decltype(pieces)::value;
+                float         l[P][4], q[P][4];
+                double        w[P][4], t4 = 0.0;
+                const int     j0 = from + lane * 4 * P;
+#pragma unroll
+                for (int i = 0; i < P; i++) {
+                    logits4(j0 + 4 * i, l[i]);
+                    drafts4(j0 + 4 * i, q[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < P; i++) {
+                    weights(j0 + 4 * i, l[i], q[i], w[i]);
+                    t4 += (w[i][0] + w[i][1]) + (w[i][2] + w[i][3]);
+                }
+                double inc = t4;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const double u = __shfl_up_sync(0xffffffffu, inc, o);
@@ -566,17 +570,26 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
                 double run4 = start + (inc - t4);
                 int    mine = INT32_MAX, ml = -1;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    run4 += w[e];
-                    if (w[e] > 0.0) {
-                        ml = j + e;
-                        if (!past && run4 > goal && mine == INT32_MAX) mine = j + e;
+                for (int i = 0; i < P; i++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        run4 += w[i][e];
+                        if (w[i][e] > 0.0) {
+                            ml = j0 + 4 * i + e;
+                            if (!past && run4 > goal && mine == INT32_MAX) mine = ml;
+                        }
                     }
                 }
                 mine  = __reduce_min_sync(0xffffffffu, mine);
                 lastw = max(lastw, __reduce_max_sync(0xffffffffu, ml));
                 if (mine != INT32_MAX) at = mine;
                 start += __shfl_sync(0xffffffffu, inc, 31);
+            };
+            const int from = (g0 + blk) * len;
+            if (len == 128) {
+                place(std::integral_constant<int, 1>{}, from);
+            } else {
+                for (int k = 0; k < len && at < 0; k += 512) place(std::integral_constant<int, 4>{}, from + k);
             }
             if (lane == 0) v.out_ids[pick] = at >= 0 ? at : lastw >= 0 ? lastw : ptop;
         }
