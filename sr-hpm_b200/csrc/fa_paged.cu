@@ -29,6 +29,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "fastdiv.cuh"
 #include "internal.h"
@@ -193,20 +194,24 @@ template <int D, int NT, int BR, bool PREC, bool Q8> struct Lay {
     static constexpr int q      = 0;                           // [NT][qparts][qtile]
     static constexpr int ring   = NT * qparts * qtile;
     // chunks in flight: what shared memory holds beside Q (at most 8); q8_0 gives the rest to the raw rows
-    static constexpr int room   = 232448 - 2400 - ring;
+    static constexpr bool copies = NT == 1 && BR <= 64 && !Q8;  // items of at most 8 rows: a copy in each quarter (below)
+    static constexpr int  sumb   = copies ? 2 * 4 * 8 * 16 * 4 : 0;
+    static constexpr int room   = 232448 - 2400 - sumb - ring;
     // q8_0: K has a ring of two chunks, V one of one or two, the raw rows the rest
     static constexpr int NS     = !Q8 ? (room / chunk < 8 ? room / chunk : 8) : BR < 128 && !PREC ? 4 : 3;
     static constexpr int raw    = ring + NS * chunk;
     static constexpr int NG     = !Q8 ? 0 : (room - NS * chunk) / (4 * kRawB) < 3 ? (room - NS * chunk) / (4 * kRawB) : 3;
     static constexpr int NR     = 4 * NG;                      // raw slots: a ring of NG for each converter group
     static constexpr int red    = raw + NR * kRawB;            // f32 [2][2][128]
-    static constexpr int bar    = red + 2 * 2 * kBM * 4;
+    static constexpr int sum    = red + 2 * 2 * kBM * 4;       // f32 [2][4][8][16]
+    static constexpr int bar    = sum + sumb;
     static constexpr int nbar   = 2 * NS + 2 * NR + 2 + 2 + 2 + 1;
     static constexpr int misc   = bar + nbar * 8;
     static constexpr int total  = misc + 64;
     static constexpr int alloc  = total;  // dynamic shared memory starts on 1024 bytes (checked by the kernel)
     static constexpr int threads = (kSmWarps + 4 + (Q8 ? kConv : 0)) * 32;  // MMA and producers: the third warpgroup
     static_assert(alloc <= 232448, "shared memory");
+    static_assert(Q8 || NS >= 3, "the producers' waits");
     static_assert(NS * chunk >= kMaxSeqs * 8, "the plan's sums fit the ring");
 };
 
@@ -336,6 +341,11 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     constexpr int MM   = BR <= 64 ? 64 : 128; // rows of a product
     constexpr int NC   = NT == 2 ? 128 : BN / 2;  // score columns per softmax thread
     constexpr int OC   = NT == 2 ? D : D / 2; // output columns per softmax thread
+    // An item of at most 8 rows (decoding) would leave all its softmax to the two warps of tensor memory's first quarter:
+    // 64 columns of a row in each thread took 1.3 us a tile, now 0.8 (the loads of one of head_dim 128 take 1.45, of 64
+    // 0.7). So its rows stand in each quarter's 16 rows once more, and every quarter takes 16 of a half's 64 columns (P is
+    // 0 in the others): four partial rows with maxima and sums of their own, added up at the item's end.
+    constexpr bool COPIES = Ly::copies;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint64_t * kvfull  = reinterpret_cast<uint64_t *>(sm + Ly::bar);
     uint64_t * kvempty = kvfull + NS;
@@ -360,7 +370,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
 
     if (tid == 0) {
         for (int i = 0; i < NS; i++) {
-            mbar_init(&kvfull[i], Q8 ? kConv / 2 : kProd);
+            mbar_init(&kvfull[i], Q8 ? kConv / 2 : 1);
             mbar_init(&kvempty[i], 1);
         }
         for (int i = 0; i < Ly::NR; i++) {
@@ -499,7 +509,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         // ---------------- softmax ----------------
         const int wg = warp >> 2, wq = warp & 3;
         // row of the tile: its tensor-memory lane, or with M = 64 16 rows in the lower lanes of each quarter
-        const int row = MM == 64 ? 16 * wq + (lane & 15) : 32 * wq + lane, tl = 32 * wq + lane;
+        const int row0 = MM == 64 ? 16 * wq + (lane & 15) : 32 * wq + lane, tl = 32 * wq + lane;
         const int q    = NT == 2 ? wg : 0;                              // row tile
         const int c0   = NT == 2 ? 0 : NC * wg;                         // first score column of this thread
         uint32_t  rc0 = 0, sc[2] = { 0, 0 }, pvc = 0, pvw = 0, turn = 0, items = 0;
@@ -515,8 +525,9 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 uint8_t *     d0 = sm + Ly::q + q * Ly::qparts * Ly::qtile + (c >> 3) * (BR * 128);
                 // rows behind the last one are zeros: what they give goes nowhere, but random rows heat the products (a
                 // 1000 W card lowers its clock for it)
-                auto source = [&](int r) {
-                    const int rr = rb + min(r, rows - 1), t = a.byG.div(rr), h = w.h * a.G + (rr - t * a.G);
+                const int cut = COPIES && rows <= 8 ? 15 : 255;  // row r of the tile holds row r & cut
+                auto      source = [&](int r) {
+                    const int rr = rb + min(r & cut, rows - 1), t = a.byG.div(rr), h = w.h * a.G + (rr - t * a.G);
                     return a.q + (int64_t) (w.r0 + t) * a.qnb1 + (int64_t) h * a.qnb2;
                 };
                 auto dest = [&](int r) { return d0 + r * 128 + (((c & 7) ^ (r & 7)) << 4); };
@@ -525,7 +536,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     for (int k = 0; k < (BR + step - 1) / step; k++) {
                         const int r = u0 / per + k * step;
                         if (BR % step && r >= BR) break;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dest(r))), "l"(source(r) + 16 * c), "r"(r < rows ? 16 : 0) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dest(r))), "l"(source(r) + 16 * c), "r"((r & cut) < rows ? 16 : 0) : "memory");
                     }
                 } else {
                     constexpr int NK = (BR + step - 1) / step, UN = NK < 4 ? NK : 4;  // rows of a thread, in flight
@@ -540,7 +551,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         }
 #pragma unroll
                         for (int k = 0; k < UN; k++) {
-                            if (u0 / per + (k0 + k) * step >= rows) x[k][0] = x[k][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (((u0 / per + (k0 + k) * step) & cut) >= rows) x[k][0] = x[k][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             const float f[8] = { x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w,
                                                  x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w };
                             uint32_t    hw[4], lw[4];
@@ -574,8 +585,10 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             const int     R    = w.n * a.G;
             const int     rb   = w.rt * BMN + q * BR;               // first row of this tile
             const int     rows = max(0, min(BR, R - rb));
+            const bool    cop  = COPIES && rows <= 8;
+            const int     row  = cop ? row0 & 15 : row0;
             const bool    mine = (MM == 128 || lane < 16) && row < rows;  // this thread's row exists
-            const bool    some = MM / 4 * wq < rows;                      // the warp has a row
+            const bool    some = cop || MM / 4 * wq < rows;               // the warp has a row
             // the next item, and its rows on their way to L2: from memory they take 2.4 us
             Walk       nw   = w;
             const bool more = boot || walk_next<BMN, BN>(a, nw);
@@ -623,43 +636,39 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 q_finish(nw);
             }
             if (boot) continue;
-            for (int i = 0; run && i < n; i++) {
-                const int b = NT == 2 ? q : (i & 1), t0 = w.tile(i) * BN;
-                wait_bar(&s_full[b], sc[b] & 1, a.status, bad);
-                sc[b]++;
-                // done: these products were issued before this tile's scores
-                if constexpr (NT == 2) {
-                    pv_wait(pvc);
-                } else if (pvc > 0) {
-                    pv_wait(pvc - 1);
-                }
-                tc::fence_after();
-                if (ahead && i == n - 1) q_issue(nw);
-                const uint32_t tb = tc::taddr(tS + 128 * b, wq, 0);
-                float          s[NC];
-                float          mt = -INFINITY;
+            // one tile of scores, W columns of a row in each thread of this warp: maximum, exponentials, P
+            auto tile = [&](auto width, int i, int t0, uint32_t tb) {
+                constexpr int W  = decltype(width)::value;
+                const int     cw = W < NC ? c0 + W * wq : c0;
+                float         s[W];
+                float         mt = -INFINITY;
                 if (some) {
+                    if constexpr (W >= 32) {
 #pragma unroll
-                    for (int c = 0; c < NC; c += 32) ld32(tb + c0 + c, reinterpret_cast<uint32_t *>(s) + c);
+                        for (int c = 0; c < W; c += 32) ld32(tb + cw + c, reinterpret_cast<uint32_t *>(s) + c);
+                    } else {
+                        tc::ld_cols<W>(tb + cw, reinterpret_cast<uint32_t *>(s));
+                    }
                     tc::wait_ld();
                     if (a.softcap_l2 != 0.0f) {
 #pragma unroll
-                        for (int c = 0; c < NC; c++) s[c] = a.softcap_l2 * tanhf(s[c] * a.qscale);
+                        for (int c = 0; c < W; c++) s[c] = a.softcap_l2 * tanhf(s[c] * a.qscale);
                     }
+                    constexpr int MW = W < 32 ? W : 32;
                     // per 32 columns: all rows of the warp see them, none does, or lane by lane
                     if (t0 < alo || t0 + BN > ahi) {
 #pragma unroll
-                        for (int c = 0; c < NC; c += 32) {
-                            const int u0 = t0 + c0 + c;
-                            if (u0 >= wlo && u0 + 32 <= whi) continue;
+                        for (int c = 0; c < W; c += MW) {
+                            const int u0 = t0 + cw + c;
+                            if (u0 >= wlo && u0 + MW <= whi) continue;
                             const int l0 = vlo - u0, h0 = vhi - u0;
 #pragma unroll
-                            for (int e = 0; e < 32; e++) s[c + e] = e >= l0 && e < h0 ? s[c + e] : -INFINITY;
+                            for (int e = 0; e < MW; e++) s[c + e] = e >= l0 && e < h0 ? s[c + e] : -INFINITY;
                         }
                     }
                     float mx[4] = { s[0], s[1], s[2], s[3] };
 #pragma unroll
-                    for (int c = 4; c < NC; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], s[c], s[c + 1]);
+                    for (int c = 4; c < W; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], s[c], s[c + 1]);
                     mt = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
                 }
                 if constexpr (NT == 1) {  // the other half of the row; both halves have read S before either writes P
@@ -695,10 +704,11 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     const float off = !mine ? INFINITY : (m == -INFINITY ? 0.0f : m) - kShift;  // rows that are none: P = 0
                     const f2    q2 = f2_pack(qs, qs), o2 = f2_pack(-off, -off);
                     f2          l2[2] = { 0ull, 0ull };
-                    constexpr int CW = NC < 64 ? NC : 64;  // columns of a store
+                    constexpr int CW = W < 64 ? W : 64;  // columns of a store
 #pragma unroll
-                    for (int c = 0; c < NC; c += CW) {
-                        uint32_t hi[CW / 2], lo[CW / 2];
+                    for (int c = 0; c < W; c += CW) {
+                        uint32_t hi[CW / 2];
+                        [[maybe_unused]] uint32_t lo[CW / 2];
 #pragma unroll
                         for (int e = 0; e < CW / 2; e++) {
                             float x0, x1;
@@ -713,7 +723,20 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                                 lo[e]            = *reinterpret_cast<const uint32_t *>(&r2);
                             }
                         }
-                        if constexpr (CW == 64) {
+                        if constexpr (W < NC) {  // this quarter's columns, zeros in the others'
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                uint32_t x[W / 2];
+#pragma unroll
+                                for (int e = 0; e < W / 2; e++) x[e] = k == wq ? hi[e] : 0;
+                                tc::st_cols<W / 2>(tb + (c0 + W * k) / 2, x);
+                                if constexpr (PREC) {
+#pragma unroll
+                                    for (int e = 0; e < W / 2; e++) x[e] = k == wq ? lo[e] : 0;
+                                    tc::st_cols<W / 2>(tb + BN / 2 + (c0 + W * k) / 2, x);
+                                }
+                            }
+                        } else if constexpr (CW == 64) {
                             st32(tb + (c0 + c) / 2, hi);
                             if constexpr (PREC) st32(tb + BN / 2 + (c0 + c) / 2, lo);
                         } else {
@@ -725,6 +748,29 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     f2_unpack(f2_add(l2[0], l2[1]), y0, y1);
                     l += y0 + y1;
                     tc::wait_st();
+                }
+            };
+            for (int i = 0; run && i < n; i++) {
+                const int b = NT == 2 ? q : (i & 1), t0 = w.tile(i) * BN;
+                wait_bar(&s_full[b], sc[b] & 1, a.status, bad);
+                sc[b]++;
+                // done: these products were issued before this tile's scores
+                if constexpr (NT == 2) {
+                    pv_wait(pvc);
+                } else if (pvc > 0) {
+                    pv_wait(pvc - 1);
+                }
+                tc::fence_after();
+                if (ahead && i == n - 1) q_issue(nw);
+                const uint32_t tb = tc::taddr(tS + 128 * b, wq, 0);
+                if constexpr (COPIES) {
+                    if (cop) {
+                        tile(std::integral_constant<int, NC / 4>{}, i, t0, tb);
+                    } else {
+                        tile(std::integral_constant<int, NC>{}, i, t0, tb);
+                    }
+                } else {
+                    tile(std::integral_constant<int, NC>{}, i, t0, tb);
                 }
                 pvc++;
                 if constexpr (!Q8) {
@@ -755,12 +801,29 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 tc::fence_after();
             }
             const bool whole = w.off == 0 && w.take == w.sp.units, wide = a.wide != 0;
+            float share = 1.0f;  // of a copy's sums in the row's
             if constexpr (NT == 1) {
                 float * rd = red + (turn & 1) * 2 * kBM;
                 turn++;
-                rd[wg * kBM + tl] = l;
-                named_bar_sync(1 + wq, 64);
-                l += rd[(wg ^ 1) * kBM + tl];
+                if (!cop || lane < 16) rd[wg * kBM + tl] = l;
+                if (COPIES && cop) {
+                    if (wg == 0 && lane < 16) rd[kBM + tl + 16] = m;  // lanes that hold no row
+                    named_bar_sync(5, kSmWarps * 32);
+                    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) M = fmaxf(M, rd[kBM + 32 * k + 16 + (lane & 15)]);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float mk = rd[kBM + 32 * k + 16 + (lane & 15)];
+                        L += (mk == -INFINITY && M > mk ? 0.0f : ex2(M == -INFINITY ? 0.0f : mk - M)) * (rd[32 * k + (lane & 15)] + rd[kBM + 32 * k + (lane & 15)]);
+                    }
+                    share = m == -INFINITY ? 0.0f : ex2(m - M);
+                    m     = M;
+                    l     = L;
+                } else {
+                    named_bar_sync(1 + wq, 64);
+                    l += rd[(wg ^ 1) * kBM + tl];
+                }
             }
             const int     o0 = NT == 2 ? 0 : OC * wg;
             const int     head = w.h * a.G + (rb + row - tok * a.G);
@@ -780,10 +843,59 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     }
                 }
                 f = L == 0.0f ? 0.0f : f / L;  // a NaN stays one
-            } else if (mine && (NT == 2 || wg == 0)) {
+            } else if (mine && (NT == 2 || wg == 0) && !(cop && wq > 0)) {
                 a.part_ms[(int64_t) slot * a.prow + q * BR + row] = make_float2(m, l);
             }
-            if (some && run) {
+            if (COPIES && cop) {
+                // 16 columns at a time: the four copies' share of 8 rows, added up by 64 threads of this half
+                float *   sm_sum = reinterpret_cast<float *>(sm + Ly::sum) + wg * (4 * 8 * 16);
+                const int u = tid & 127, orow = u >> 3, ocol = (u & 7) * 2;  // of the sums
+                const int otok = a.byG.div(rb + min(orow, rows - 1)), ohead = w.h * a.G + (rb + min(orow, rows - 1) - otok * a.G);
+                const float of = whole ? __shfl_sync(0xffffffffu, f, orow & 7) : 1.0f;
+                uint8_t *   od = a.dst + (int64_t) ohead * a.dnb1 + (int64_t) (w.r0 + otok) * a.dnb2;
+                float *     oa = a.part_acc + ((int64_t) slot * a.prow + min(orow, rows - 1)) * D;
+#pragma unroll 1
+                for (int c = 0; c < OC; c += 16) {
+                    uint32_t o[16];
+                    if (n > 0) {
+                        tc::ld16(tc::taddr(tO, wq, o0 + c), o);
+                        tc::wait_ld();
+                        if (lane < 8) {
+                            float * to = sm_sum + (wq * 8 + lane) * 16;
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4) {
+                                *reinterpret_cast<float4 *>(to + e) =
+                                    make_float4(__uint_as_float(o[e]) * share, __uint_as_float(o[e + 1]) * share,
+                                                __uint_as_float(o[e + 2]) * share, __uint_as_float(o[e + 3]) * share);
+                            }
+                        }
+                    }
+                    named_bar_sync(6 + wg, 128);
+                    if (orow < rows) {
+                        float2 x = make_float2(0.0f, 0.0f);
+                        if (n > 0) {
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const float2 y = *reinterpret_cast<const float2 *>(sm_sum + (k * 8 + orow) * 16 + ocol);
+                                x.x += y.x;
+                                x.y += y.y;
+                            }
+                        }
+                        if (!whole) {
+                            *reinterpret_cast<float2 *>(oa + o0 + c + ocol) = x;
+                        } else {
+                            x.x = of != 0.0f ? x.x * of : 0.0f;
+                            x.y = of != 0.0f ? x.y * of : 0.0f;
+                            if constexpr (PREC) {
+                                *reinterpret_cast<float2 *>(od + 4 * (o0 + c + ocol)) = x;
+                            } else {
+                                *reinterpret_cast<__half2 *>(od + 2 * (o0 + c + ocol)) = __floats2half2_rn(x.x, x.y);
+                            }
+                        }
+                    }
+                    named_bar_sync(6 + wg, 128);
+                }
+            } else if (some && run) {
                 uint8_t * dst = a.dst;
                 float *   acc = a.part_acc;
                 if (mine) {
@@ -852,11 +964,14 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Q8 ? 56 : 104));
         if (warp > kSmWarps && (!Q8 || warp < kSmWarps + 3)) {
             // ---------------- producers ----------------
-            // f16: the boxes of a chunk are dealt over the lanes of three warps (a page of 16 tokens makes 16 boxes of
-            // 2 KB per chunk, and a warp issues one in some 150 cycles); each announces its own bytes
+            // f16: the warps take the chunks in turn. What a warp does once per chunk (entries, waits) took some 1200 cycles
+            // when all three shared every chunk's boxes, more than the chunk's loads themselves (32 sequences decoding 127 us,
+            // in turn 118; 2048 rows over 32768 tokens 1.58 and 1.40 ms; seven sequences of 4000 135 and 139 us). A wait by
+            // parity for the release of slot use c / NS - 1 is safe though a warp has not seen the uses between: its wait for
+            // chunk c - 3 means that all chunks up to c - 3 - NS are read, so c - 2 NS is (NS >= 3).
             // q8_0: one warp brings K's raw rows, one V's
             const int pw = warp - kSmWarps - 1;
-            uint32_t  rc = 0;                 // chunks (q8_0: raw slots) so far
+            uint32_t  rc = 0, issued = 0;     // chunks before the item (q8_0: raw slots so far); end of those brought by this warp
             const int box = a.box;            // q8_0: at most kRawTok
             const int nsub = BN / box;       // boxes per 128 tokens: 2, 4 or 8
             for (; active; active = walk_next<BMN, BN>(a, w)) {
@@ -878,17 +993,13 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                     const int pg = row[pi];
                     return pg < 0 || pg >= a.n_pages ? a.n_pages : pg;  // no page: outside the map, reads as zeros
                 };
-                int       in_next = 0, e_next = n ? entry(0, in_next) : -1;
-                const int npos = Q8 ? n : 2 * n;
-                for (int pos = 0; pos < npos; pos++) {
-                    bool isk = pw == 0;
-                    int  i;
-                    if constexpr (!Q8) at_pos<NT>(pos, n, isk, i);
-                    const int e = e_next, in = in_next;
-                    if (pos + 1 < npos) e_next = entry(pos + 1, in_next);  // in flight during this tile's waits
-                    if (e == a.n_pages) atomicExch(a.status, kErrPage);
-                    const CUtensorMap * m = isk ? &mk : &mv;
-                    if constexpr (Q8) {
+                if constexpr (Q8) {
+                    int in_next = 0, e_next = n ? entry(0, in_next) : -1;
+                    for (int pos = 0; pos < n; pos++) {
+                        const int e = e_next, in = in_next;
+                        if (pos + 1 < n) e_next = entry(pos + 1, in_next);  // in flight during this tile's waits
+                        if (e == a.n_pages) atomicExch(a.status, kErrPage);
+                        const CUtensorMap * m = pw == 0 ? &mk : &mv;
                         constexpr uint32_t NG   = Ly::NG;
                         constexpr int      NRAW = BN / kRawTok;
                         const int     per  = kRawTok / box;  // boxes per raw slot: 1 or 2
@@ -910,34 +1021,47 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                                 __syncwarp();
                             }
                         }
-                    } else {
-#pragma unroll 1
-                        for (int ch = 0; ch < CH; ch++, rc++) {
-                            const int slot = rc % NS;
-                            if (rc >= NS) wait_bar(&kvempty[slot], (rc / NS - 1) & 1, a.status, bad);
-                            if (bad) break;
-                            // boxes of the chunk: K all tokens and D / CH dims, V tokens 128 / CH and all dims
-                            const int  planes = isk ? D / 64 / CH : D / 64;
-                            const int  ns     = isk ? nsub : nsub / CH;
-                            const int  sub0   = isk ? 0 : ch * ns;
-                            const int  p0     = isk ? ch * planes : 0;
-                            const int  rows   = isk ? BN : Ly::vtok;
-                            const int      box0 = lane * kProd + pw;  // box and plane of this lane: at most 16 in all
-                            const int      j = box0 % ns, pl = box0 / ns;
-                            const int      ee = __shfl_sync(0xffffffffu, e, (sub0 + j) & 31);
-                            const int      ii = __shfl_sync(0xffffffffu, in, (sub0 + j) & 31);
-                            const bool     go = pl < planes && ee >= 0;
-                            const uint32_t many = __popc(__ballot_sync(0xffffffffu, go));
-                            if (lane == 0) mbar_arrive_expect_tx(&kvfull[slot], many * box * 128);
-                            __syncwarp();
-                            if (go) {
-                                tma4(smem_u32(sm + Ly::ring + slot * Ly::chunk) + pl * rows * 128 + j * box * 128, m,
-                                     (p0 + pl) * 64, ii, w.h, ee, &kvfull[slot]);
+                    }
+                } else {
+                    const uint32_t nc  = 2 * n * CH;  // chunks of the item
+                    uint32_t       cl  = (kProd + pw - rc % kProd) % kProd;
+                    int            in = 0, e = cl < nc ? entry(cl / CH, in) : -1;
+                    for (; cl < nc; cl += kProd) {
+                        const int      ch = cl % CH;
+                        const uint32_t c = rc + cl, slot = c % NS;
+                        if (e == a.n_pages) atomicExch(a.status, kErrPage);
+                        bool isk;
+                        int  i;
+                        at_pos<NT>(cl / CH, n, isk, i);
+                        if (c >= NS) wait_bar(&kvempty[slot], (c / NS - 1) & 1, a.status, bad);
+                        if (bad) break;
+                        issued = c + 1;
+                        // boxes of the chunk: K all tokens and D / CH dims, V tokens 128 / CH and all dims
+                        const int      planes = isk ? D / 64 / CH : D / 64;
+                        const int      ns = isk ? nsub : nsub / CH;
+                        const int      sub0 = isk ? 0 : ch * ns, p0 = isk ? ch * planes : 0, rows = isk ? BN : Ly::vtok;
+                        const uint32_t seen = __ballot_sync(0xffffffffu, e >= 0) >> sub0 & ((1u << ns) - 1);
+                        const uint32_t at   = smem_u32(sm + Ly::ring + slot * Ly::chunk);
+                        const CUtensorMap * m = isk ? &mk : &mv;
+                        if (elect_one()) mbar_arrive_expect_tx(&kvfull[slot], __popc(seen) * planes * box * 128);
+                        __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {  // at most 8 boxes along the tokens
+                            if (!(seen >> j & 1)) continue;
+                            const int ee = __shfl_sync(0xffffffffu, e, sub0 + j), ii = __shfl_sync(0xffffffffu, in, sub0 + j);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int pl = 0; pl < D / 64; pl++) {
+                                    if (pl < planes) tma4(at + (pl * rows + j * box) * 128, m, (p0 + pl) * 64, ii, w.h, ee, &kvfull[slot]);
+                                }
                             }
                             __syncwarp();
                         }
+                        if (cl + kProd < nc) e = entry((cl + kProd) / CH, in);  // its wait overlaps the next slot's
                     }
+                    rc += nc;
                 }
+                if (bad) break;
             }
             if (bad) {  // the loads in flight land before this CTA's shared memory goes
                 if constexpr (Q8) {
@@ -946,7 +1070,9 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         mbar_wait(&rfull[(pw * 2 + (c & 1)) * Ly::NG + own % Ly::NG], (own / Ly::NG) & 1);
                     }
                 } else {
-                    for (uint32_t c = rc > NS ? rc - NS : 0; c < rc; c++) mbar_wait(&kvfull[c % NS], (c / NS) & 1);
+                    for (uint32_t c = issued > NS ? issued - NS : 0; c < issued; c++) {
+                        if (c % kProd == (uint32_t) pw) mbar_wait(&kvfull[c % NS], (c / NS) & 1);
+                    }
                 }
             }
         } else if (warp == kSmWarps) {
