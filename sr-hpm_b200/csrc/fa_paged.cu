@@ -194,7 +194,7 @@ template <int D, int NT, int BR, bool PREC, bool Q8> struct Lay {
     static constexpr int q      = 0;                           // [NT][qparts][qtile]
     static constexpr int ring   = NT * qparts * qtile;
     // chunks in flight: what shared memory holds beside Q (at most 8); q8_0 gives the rest to the raw rows
-    static constexpr bool copies = NT == 1 && BR <= 64 && !Q8;  // items of at most 8 rows: a copy in each quarter (below)
+    static constexpr bool copies = NT == 1 && BR <= 64 && D <= 128 && !Q8;  // of rows in each quarter (below)
     static constexpr int  sumb   = copies ? 2 * 4 * 8 * 16 * 4 : 0;
     static constexpr int room   = 232448 - 2400 - sumb - ring;
     // q8_0: K has a ring of two chunks, V one of one or two, the raw rows the rest
@@ -342,9 +342,10 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     constexpr int NC   = NT == 2 ? 128 : BN / 2;  // score columns per softmax thread
     constexpr int OC   = NT == 2 ? D : D / 2; // output columns per softmax thread
     // An item of at most 8 rows (decoding) would leave all its softmax to the two warps of tensor memory's first quarter:
-    // 64 columns of a row in each thread took 1.3 us a tile, now 0.8 (the loads of one of head_dim 128 take 1.45, of 64
-    // 0.7). So its rows stand in each quarter's 16 rows once more, and every quarter takes 16 of a half's 64 columns (P is
-    // 0 in the others): four partial rows with maxima and sums of their own, added up at the item's end.
+    // 64 columns of a row in each thread take 1.3 us a tile, the loads of one of head_dim 64 take 0.7. So its rows stand in
+    // each quarter's 16 rows once more, and every quarter takes 16 of a half's 64 columns (P is 0 in the others), 0.8 us:
+    // four partial rows with maxima and sums of their own, added up at the item's end. 32 sequences decoding: head_dim 128
+    // 118 us, without copies 127; 64 185 and 224; 256 117 and 114 (its tiles load for 2.9 us), so not there.
     constexpr bool COPIES = Ly::copies;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint64_t * kvfull  = reinterpret_cast<uint64_t *>(sm + Ly::bar);
