@@ -4,6 +4,8 @@
  *   - small-batch quantized matmul (ggml_mul_mat with ne[1] = 1..16 on Q4_K / Q5_K / Q6_K / Q3_K / IQ4_XS / Q8_0)
  *   - multi-query attention over an f16 or q8_0 KV cache (ggml_flash_attn_ext with 1..16 query rows)
  *   - greedy longest-prefix acceptance over the target logits
+ * and, for a batch of sequences over a paged KV cache, plans the pages of a step, stores into them, attends over them and
+ * accepts drafted tokens by sampling.
  *
  * Conventions (all entry points):
  *   - tensors are ggml-shaped views (srhpm_tensor: type, ne[4] in elements, nb[4] in bytes, data) of DEVICE memory,
@@ -299,7 +301,9 @@ int srhpm_swiglu(srhpm_ctx * ctx, const float * gate, const float * up, int64_t 
 
 /* srhpm_page_plan: the step's block table entries, row starts, cache lengths, positions and slots, from the sequences'
  * lengths: n_past[s] tokens in the cache (its first ceil(n_past / page_size) table entries name their pages) and
- * n_new[s] >= 0 new ones (i32 [n_seqs] both). A sequence that needs pages takes them, in order of sequences, from
+ * n_new[s] >= 0 new ones (i32 [n_seqs] both). n_held i32 [n_seqs] or NULL: table entries that name a sequence's pages
+ * already, where they are more than its cache fills (after rejected tokens: max(n_held, ceil(kv_len / page_size)) of the
+ * step before; without n_held those pages are taken anew). A sequence that needs pages takes them, in order of sequences, from
  * free_pages[*free_head ..] (free_head NULL: 0; n_free entries in all), written behind its entries; n_taken i32 [1]
  * receives how many were taken (the next step's head is *free_head + *n_taken). Outputs: q_start i32 [n_seqs + 1];
  * kv_len i32 [n_seqs] = n_past + n_new; per row pos i32 [n_rows] and slots i64 [n_rows] (padding rows: 0 and -1); status
@@ -314,8 +318,8 @@ enum srhpm_page_status {
     SRHPM_PAGES_BAD_LENGTH = 3, /* a negative length */
     SRHPM_PAGES_NO_ROWS    = 4, /* its rows end behind n_rows */
 };
-int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_new, int n_seqs, int page_size,
-                    const srhpm_tensor * block_table, const int32_t * free_pages, int n_free, const int32_t * free_head,
+int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_new, const int32_t * n_held, int n_seqs,
+                    int page_size, const srhpm_tensor * block_table, const int32_t * free_pages, int n_free, const int32_t * free_head,
                     int n_rows, int32_t * q_start, int32_t * kv_len, int32_t * pos, int64_t * slots, int32_t * status,
                     int32_t * n_taken, void * stream);
 

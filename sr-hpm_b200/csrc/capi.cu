@@ -657,8 +657,8 @@ int srhpm_swiglu(srhpm_ctx * ctx, const float * gate, const float * up, int64_t 
     return swiglu_run(ctx, gate, up, ld_in, out, ld_out, n, n_ff, (cudaStream_t) stream);
 }
 
-int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_new, int n_seqs, int page_size,
-                    const srhpm_tensor * block_table, const int32_t * free_pages, int n_free, const int32_t * free_head,
+int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_new, const int32_t * n_held, int n_seqs,
+                    int page_size, const srhpm_tensor * block_table, const int32_t * free_pages, int n_free, const int32_t * free_head,
                     int n_rows, int32_t * q_start, int32_t * kv_len, int32_t * pos, int64_t * slots, int32_t * status,
                     int32_t * n_taken, void * stream) {
     if (!ctx || !n_past || !n_new || !q_start || !kv_len || !status || !n_taken) return SRHPM_ERR_INVALID;
@@ -668,7 +668,7 @@ int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_n
     if (st != SRHPM_OK) return st;
     if (block_table->ne[1] != n_seqs) return SRHPM_ERR_INVALID;
     if (!aligned(slots, 8)) return SRHPM_ERR_ALIGN;
-    return page_plan_run(ctx, n_past, n_new, n_seqs, page_size, block_table->data, (int64_t) block_table->nb[1],
+    return page_plan_run(ctx, n_past, n_new, n_held, n_seqs, page_size, block_table->data, (int64_t) block_table->nb[1],
                          (int) block_table->ne[0], free_pages, n_free, free_head, n_rows, q_start, kv_len, pos, slots,
                          status, n_taken, (cudaStream_t) stream);
 }

@@ -91,8 +91,8 @@ _SIGNATURES = {
     "srhpm_swiglu": (ctypes.c_int, [_P, _P, _P, ctypes.c_int64, _P, ctypes.c_int64, ctypes.c_int, ctypes.c_int64,
                                     _P]),
     # the views of these are passed as the bytes of the structure (ops._pack)
-    "srhpm_page_plan": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, ctypes.c_int, _P, _P, ctypes.c_int, _P, ctypes.c_int,
-                                       _P, _P, _P, _P, _P, _P, _P]),
+    "srhpm_page_plan": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, ctypes.c_int, _P, _P, ctypes.c_int, _P,
+                                       ctypes.c_int, _P, _P, _P, _P, _P, _P, _P]),
     "srhpm_rope_kv_paged": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.c_int, _P, _P, ctypes.c_float, _P, _P, _P, _P]),
     "srhpm_flash_attn_paged_work_size": (ctypes.c_int, [_P, _P, _P, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "srhpm_flash_attn_paged": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_float, ctypes.c_float,

@@ -509,13 +509,15 @@ class Context:
         return self._new(n, torch.uint8, stream)
 
     def page_plan(self, n_past, n_new, block_table, free_pages, page_size, n_rows, free_head=None, out=None,
-                  stream=None):
+                  stream=None, n_held=None):
         """Tables and slots of a step (srhpm_page_plan): n_past, n_new int32 [S]; block_table int32 [S, entries] (new
-        entries are written into it); free_pages int32 [F], taken from free_head (int32 [1], 0 if None). Returns a
+        entries are written into it); free_pages int32 [F], taken from free_head (int32 [1], 0 if None); n_held int32 [S]:
+        pages that a row names already, if more than n_past fills (after rejected tokens, torch.maximum(n_held,
+        (kv_len + page_size - 1) // page_size) of the step before). Returns a
         PagePlan: q_start int32 [S + 1], kv_len int32 [S], pos int32 [n_rows], slots int64 [n_rows], status int32 [S],
         n_taken int32 [1] (`out`: one to write into)."""
         S = n_past.numel()
-        self._on_device(n_past, n_new, block_table, free_pages, free_head)
+        self._on_device(n_past, n_new, block_table, free_pages, free_head, n_held)
         i32 = torch.int32
         if out is None:
             at = self._new(3 * S + 2 + n_rows, i32, stream)
@@ -530,7 +532,8 @@ class Context:
                     _ints(out.pos, i32, n_rows, "pos"), _ints(out.slots, torch.int64, n_rows, "slots"),
                     _ints(out.status, i32, S, "status"), _ints(out.n_taken, i32, 1, "n_taken"))
         self._call(self.lib.srhpm_page_plan, "srhpm_page_plan", stream, _ints(n_past, i32, S, "n_past"),
-                   _ints(n_new, i32, S, "n_new"), S, page_size, _rows_2d(block_table, i32, L.I32, "block_table"),
+                   _ints(n_new, i32, S, "n_new"), None if n_held is None else _ints(n_held, i32, S, "n_held"), S,
+                   page_size, _rows_2d(block_table, i32, L.I32, "block_table"),
                    _ints(free_pages, i32, 0, "free_pages"), free_pages.numel(),
                    None if free_head is None else _ints(free_head, i32, 1, "free_head"), n_rows, *ptrs)
         return out

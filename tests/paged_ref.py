@@ -4,7 +4,7 @@ import math
 import numpy as np
 
 
-def plan(past, new, table, free, P, n_rows, head=0):
+def plan(past, new, table, free, P, n_rows, head=0, held=None):
     """(table, q_start, kv_len, pos, slots, status, n_taken) of srhpm_page_plan, sequence by sequence."""
     table = table.copy()
     S, cols = table.shape
@@ -14,7 +14,7 @@ def plan(past, new, table, free, P, n_rows, head=0):
     for s in range(S):
         a, n = int(past[s]), int(new[s])
         q_start.append(q_start[-1] + max(n, 0))
-        have, want = -(-a // P), -(-(a + n) // P)
+        have, want = max(-(-a // P), int(held[s]) if held is not None else 0), -(-(a + n) // P)
         if a < 0 or n < 0:
             st = 3
         elif q_start[-1] > n_rows:
@@ -23,7 +23,7 @@ def plan(past, new, table, free, P, n_rows, head=0):
             st = 1
         else:
             st = 0
-            need = want - have
+            need = max(want - have, 0)
             at += need
             if need and (head < 0 or at > len(free)):
                 st = 2

@@ -99,6 +99,33 @@ def test_plan_strided_table_and_largest_lengths(ctx):
 
 
 # ---- RoPE and the paged store ----------------------------------------------------------------------------------------
+@pytest.mark.parametrize("S,P", [(1, 16), (5, 1), (40, 16), (1500, 64)])
+def test_plan_pages_held_behind_the_cache(ctx, S, P):
+    """Pages of rejected tokens stay the sequence's: its next tokens go into them before it takes new ones."""
+    rng = np.random.default_rng(S)
+    past, drafted, new = (rng.integers(0, 6 * P, S), rng.integers(0, 3 * P + 2, S), rng.integers(0, 4 * P, S))
+    past, new = past.astype(np.int32), new.astype(np.int32)
+    held = (-(-(past + drafted) // P)).astype(np.int32)
+    held[::7] = rng.integers(-3, 1, len(held[::7]))  # fewer than the cache fills: the cache's count stands
+    named = np.maximum(held, -(-past // P))
+    cols = int(np.maximum(named, -(-(past + new) // P)).max()) + 1
+    pool = rng.permutation(S * cols).astype(np.int32)
+    table, at = np.full((S, cols), -7, np.int32), 0
+    for s in range(S):
+        table[s, :named[s]] = pool[at:at + named[s]]
+        at += int(named[s])
+    free, rows = pool[at:], int(new.sum()) + 2
+    tb = cu(table)
+    r = ctx.page_plan(cu(past), cu(new), tb, cu(free), P, rows, n_held=cu(held))
+    torch.cuda.synchronize()
+    want = R.plan(past, new, table, free, P, rows, held=held)
+    for g, w in zip((tb, r.q_start, r.kv_len, r.pos, r.slots, r.status, r.n_taken), want):
+        assert np.array_equal(g.cpu().numpy().reshape(-1), np.asarray(w).reshape(-1))
+    used = tb.cpu().numpy()  # no page twice
+    used = used[used >= 0]
+    assert len(np.unique(used)) == len(used)
+
+
 @pytest.mark.parametrize("head", [-1, -2 ** 31, 2 ** 31 - 1])
 def test_plan_heads_outside_the_list(ctx, head):
     """A sequence that needs no page keeps its rows; one that needs a page is refused."""

@@ -43,7 +43,7 @@ def table(cols=8, S=2, type_=L.I32, data=A, nb1=None):
 def plan(**o):
     a = dict(past=A, new=A, S=2, P=16, table=table(), free=A, n_free=5, n_rows=7, q=A, kv=A, pos=A, slots=A, st=A, nt=A)
     a.update(o)
-    return lib.srhpm_page_plan(CTX, a["past"], a["new"], a["S"], a["P"], ctypes.byref(a["table"]), a["free"], a["n_free"],
+    return lib.srhpm_page_plan(CTX, a["past"], a["new"], None, a["S"], a["P"], ctypes.byref(a["table"]), a["free"], a["n_free"],
                                None, a["n_rows"], a["q"], a["kv"], a["pos"], a["slots"], a["st"], a["nt"], None)
 
 
