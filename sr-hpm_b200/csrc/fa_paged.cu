@@ -1,9 +1,9 @@
 // Attention of a batch's new tokens over a paged KV cache (srhpm_flash_attn_paged), on the 5th-generation tensor cores.
 //
 // The R = G * n rows (G query heads per KV head, n new tokens) that a sequence has for one KV head are packed token by
-// token into tiles of 128: a decode step's few rows and a prompt's thousands take the same path, and K/V is read once
-// for all heads of a group. Per tile of 128 rows and 128 cached tokens:
-//   S = Q K^T      M = 128 rows, N = 128 tokens, f32 in tensor memory (both operands from shared memory)
+// token into tiles of BR rows: a decode step's few rows and a prompt's thousands take the same path, and K/V is read once
+// for all heads of a group. Per row tile and tile of BN cached tokens (128; f32 rows over q8_0: 64):
+//   S = Q K^T      M = 128 rows (BR = 56: 64), N = BN tokens, f32 in tensor memory (both operands from shared memory)
 //   softmax        one pass with the running maximum m and sum l of each row in registers; the maximum is raised only
 //                  when a tile exceeds it by more than 2^8 (then O is rescaled in place), p = 2^(s - m + 7) <= 2^15 as
 //                  f16 back into S's place in tensor memory: the 2^7 keeps probabilities down to 2^-21 of the row's
@@ -12,16 +12,28 @@
 // f32 rows (PREC): Q and P as sums of two f16 parts (2^-22), two products each. f16 rows: one product each, P rounded to
 // f16 (2^-11 of each probability; the sums l stay f32).
 //
-// Work: an item is (sequence, KV head, row tile); its units are the 128-token tiles that the rows see. All items' units
+// Work: an item is (sequence, KV head, row tile); its units are the BN-token tiles that the rows see. All items' units
 // stand in one line that is cut into equal parts, one per CTA (one CTA per SM: any mix of lengths keeps every SM busy to
 // the end, and one long row is spread over the whole GPU). An item cut between CTAs leaves (m, l, O) records, which
 // fa_paged_merge_kernel joins in the order of the cuts (same bits every run). The plan is taken from the lengths on the
-// device by every CTA itself, in its prologue: no planning launch.
+// device by every CTA itself, in its prologue (2.5 us): no planning launch. Cuts moved to the items' borders where one was
+// near gained nothing (0 to 7 % slower).
 //
 // Roles: 8 softmax warps, 1 MMA warp, 3 producer warps (TMA boxes of at most 64 tokens x 64 dims, each within a page, into
 // a ring of 128-byte-swizzled chunks), and for a q8_0 cache 16 converter warps (raw rows by TMA into a second ring, d * q
 // rounded to f16 into the chunks). NT = 1: the 8 softmax warps halve the columns of one row tile and S has two buffers;
 // NT = 2 (head_dim <= 128): two row tiles share K/V, each with its own 4 softmax warps and buffer.
+//
+// Measured (6.55 TB/s copy, 1632 TFLOP/s burst and 1321 sustained of a library product), both launches:
+//   32 sequences of 500 to 8192 tokens decoding, 32 / 8 heads of 128, pages of 16: 118 us, 5.4 TB/s; four times as long 6.5:
+//   some 25 us go to the plan, the first loads (their rows 2 to 5 us), items' ends and the join, the rest to memory.
+//   9 rows of f32 over 131072 tokens, 24 / 4 heads of 256: 111 us; back to back 130, the card at 1000 W and 1.6 GHz.
+//   4 sequences of 2048 to 16384 tokens over q8_0, 2 to 9 f16 rows, same heads: 74 us, a quarter of memory's rate: the
+//   conversion (a job of 32 tokens takes a warp 0.7 us) and 12 us until the first scores.
+//   2048 rows over 32768 tokens, 24 / 4 heads of 256: 1.40 ms, 1140 TFLOP/s; 1.57 back to back at 1.45 GHz (of sustained
+//   0.77). Shared memory's reads: QK takes 128 bytes a cycle for M = N = 128, PV 64, the tiles' arrival 64.
+//   seven sequences, prompts to 2000 rows and decoding, window 1024, 32 / 8 heads of 128: 138 us, of which 14 are the join and
+//   3 to 5 each item's end (a row per lane: its stores go at a sector per cycle).
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -1423,8 +1435,8 @@ EncodeTiled encode_fn() {
 }
 
 // Rows of a CTA's tile by the sequences' average: at most kFew (decoding, verifying): one tile of kFew rows, whose Q takes
-// less than half the shared memory of 128 and leaves it to the K/V ring. The products still have M = 128: their upper rows
-// read what lies behind Q and go nowhere. kFew: what lets a q8_0 cache's rings (4 chunks, 8 raw slots) stand beside Q; it
+// less than half the shared memory of 128 and leaves it to the K/V ring. The products have M = 64 there (decode 146 us with
+// 128, 130 with 64): their last 8 rows read what lies behind Q and go nowhere. kFew: what lets a q8_0 cache's rings (4 chunks, 8 raw slots) stand beside Q; it
 // holds 9 tokens of 6 heads. More: 128 rows, and with head_dim <= 128 two such tiles that share K/V. f32 rows over a q8_0
 // cache: always kFew (Q's two parts of 128 rows do not fit beside the rings).
 struct Tile {
