@@ -338,7 +338,7 @@ int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, i
  * positions j <= p, and j > p - window where window > 0:
  * dst = softmax(scale * q k [softcap * tanh(. / softcap)] [+ sink]) v. q: ne = [head_dim, T, n_head], f32 or f16 (token
  * stride nb[1], head stride nb[2]); dst of the same type, ne = [head_dim, n_head, T] (head stride nb[1], token stride
- * nb[2], as in srhpm_flash_attn_ext); head h reads KV head h / (n_head / n_head_kv); sinks f32 [n_head] or NULL. A
+ * nb[2], as in srhpm_flash_attn_ext); head h reads KV head h / (n_head / n_head_kv); sinks f32 [n_head], finite or -inf, or NULL. A
  * row that sees nothing is 0; padding rows of dst stay as they are. f16 rows: probabilities are rounded to f16 for the
  * product with v, sums are kept in f32. f32 rows: q and the probabilities are taken as sums of two f16 parts, so the
  * result is exact to f32's order of magnitude. A q8_0 cache is read as d * q rounded to f16. head_dim 64, 128 or 256

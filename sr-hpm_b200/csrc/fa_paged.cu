@@ -851,7 +851,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                         const float d = m == -INFINITY ? 0.0f : ex2(m - sk);
                         L             = l * d + exp2f(kShift);
                         f             = d;
-                    } else {
+                    } else if (sk > -INFINITY) {
                         L += ex2(sk - m + kShift);
                     }
                 }

@@ -346,6 +346,26 @@ def test_attention_long_rows_split(ctx, qt, kv, D, H, Hkv):
     ctx.check()
 
 
+@pytest.mark.parametrize("qt", [torch.float16, torch.float32])
+@pytest.mark.parametrize("D,H,Hkv", [(64, 8, 2), (128, 8, 1), (128, 3, 3), (256, 12, 2), (64, 18, 2)])
+@pytest.mark.parametrize("window,softcap,sink", [(0, 0.0, False), (1, 0.0, True), (100, 20.0, True), (5000, 0.0, True)])
+def test_attention_few_rows(ctx, qt, D, H, Hkv, window, softcap, sink):
+    """Decoding and short drafts: items of 3 to 18 rows side by side, empty caches, whole and cut items, with every mask."""
+    rng = np.random.default_rng(D + H + window)
+    case = attn_case(rng, [0, 5, 130, 0, 3000, 12000, 127], [1, 2, 1, 0, 2, 1, 1], H, Hkv, D, 16, L.F16, qt, pad_rows=2)
+    kw = dict(window=window, softcap=softcap)
+    if sink:
+        kw["sinks"] = (rng.standard_normal(H) * 2).astype(np.float32)
+        kw["sinks"][0] = -np.inf
+    attn_run(ctx, case, L.F16, D ** -0.5, **kw)
+    q, caches, vals, table, q_start, kv_len = case
+    kv_len[1], kv_len[2] = 1, 0  # a row before position 0, a row that sees nothing
+    caches = [np.nan_to_num(c.view(np.float16)).view(np.uint8) for c in caches]
+    vals = [np.nan_to_num(v) for v in vals]
+    attn_run(ctx, (q, caches, vals, table, q_start, kv_len), L.F16, D ** -0.5, **kw)
+    ctx.check()
+
+
 def test_attention_released_pages_before_the_window(ctx):
     """Pages wholly before the window are given away: their entries are no pages, and nothing of them is read."""
     rng = np.random.default_rng(5)
