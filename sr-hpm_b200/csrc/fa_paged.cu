@@ -223,7 +223,7 @@ template <int D, int NT, int BR, bool PREC, bool Q8> struct Lay {
     static constexpr int alloc  = total;  // dynamic shared memory starts on 1024 bytes (checked by the kernel)
     static constexpr int threads = (kSmWarps + 4 + (Q8 ? kConv : 0)) * 32;  // MMA and producers: the third warpgroup
     static_assert(alloc <= 232448, "shared memory");
-    static_assert(Q8 || NS >= 3, "the producers' waits");
+    static_assert(Q8 || (NS >= 3 && NS >= CH), "the producers' waits; the wait for V rows that become zeros");
     static_assert(NS * chunk >= kMaxSeqs * 8, "the plan's sums fit the ring");
 };
 
@@ -789,6 +789,19 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
                 if constexpr (!Q8) {
                     // V rows that no row of the item sees hold anything; 0 * NaN is NaN, so they become zeros
                     if ((NT == 1 || q == 0) && (t0 < w.sp.lo || t0 + BN > w.sp.hi)) {
+                        // A wait by parity for this use of a slot passes at once while the use before it is still on its
+                        // way, so all chunks up to NS before V's have to be there first. This tile's scores mean that
+                        // those up to K of tile i are, whose last one stands 3 CH chunks before V's last: enough for
+                        // NS >= 3 CH. Otherwise the next scores mean that K of tile i + 1 is there, the last before V
+                        // (and V of tile i - 1: its products were issued before them); in the last tile that V is the
+                        // last, and its products' end says so. Neither waits for this tile's P.
+                        if constexpr (NT == 1 && NS < 3 * CH) {
+                            if (i + 1 < n) {
+                                wait_bar(&s_full[b ^ 1], sc[b ^ 1] & 1, a.status, bad);
+                            } else {
+                                pv_wait(pvc - 1);
+                            }
+                        }
                         const int z0 = max(0, w.sp.lo - t0), z1 = min(BN, w.sp.hi - t0);  // kept rows
 #pragma unroll
                         for (int ch = 0; ch < CH; ch++) {

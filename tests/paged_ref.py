@@ -168,3 +168,38 @@ def sample(logits, ids, q_start, u, us, dp=None, temp=None):
                 out[r] = int(over[0]) if len(over) else int(np.nonzero(w > 0)[0][-1])
         cnt.append(n)
     return out, cnt, pd
+
+
+def turned_items(q_start, kv_len, n_head, n_head_kv, head_dim, q8, f32, window, n_cta):
+    """(items, turned, inside): work items of srhpm_flash_attn_paged, those that one CTA takes whole but not from their first
+    tile on, and those among them with a tile that holds slots no row sees (behind the cache or before the window) and
+    does not come last. Units of all items in one line, cut into n_cta equal parts (every item here has a unit or more)."""
+    S, G, T = len(kv_len), n_head // n_head_kv, int(q_start[-1])
+    few = (q8 and f32) or T * G <= S * 56
+    rows = 56 if few else 256 if head_dim <= 128 else 128
+    bn = 64 if q8 and f32 else 128
+    items = []
+    for s in range(S):
+        n, kv = int(q_start[s + 1] - q_start[s]), int(kv_len[s])
+        for _ in range(n_head_kv):
+            for r in range(0, n * G, rows):
+                hi = kv - n + (min(n * G, r + rows) - 1) // G + 1
+                lo = max(0, kv - n + r // G - window + 1) if window > 0 else 0
+                items.append((lo // bn, -(-hi // bn), bool(lo % bn), bool(hi % bn)))
+    W = sum(b - a for a, b, _, _ in items)
+    parts, at = min(n_cta, W), 0
+    turned = inside = 0
+    for a, b, first, last in items:
+        n = b - a
+        c = ((at + 1) * parts - 1) // W  # the part that holds unit `at`
+        while W * (c + 1) // parts <= at:
+            c += 1
+        start = W * c // parts
+        if n >= 64 and at + n <= W * (c + 1) // parts:
+            turn = (at - start) % n
+            if turn:
+                turned += 1
+                # the order: turn .. n - 1, 0 .. turn - 1
+                inside += last or (first and turn != 1)
+        at += n
+    return len(items), turned, inside

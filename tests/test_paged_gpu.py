@@ -463,6 +463,49 @@ def test_attention_many_tiles_per_cta(ctx, qt, kv, D, H, Hkv, P, past, new, wind
         assert torch.equal(r, runs[0])
 
 
+@pytest.mark.parametrize("kv,qt,D,H,Hkv,past,new,window,shared", [
+    (L.F16, torch.float32, 256, 24, 4, [16001], [1500], 0, 0), (L.F16, torch.float16, 256, 24, 4, [16001], [1500], 0, 0),
+    (L.F16, torch.float32, 256, 24, 4, [16001], [1500], 9001, 0), (L.F16, torch.float16, 256, 24, 4, [16001], [1500], 9001, 0),
+    (L.F16, torch.float16, 128, 32, 8, [15000, 3], [1501, 700], 0, 0), (L.F16, torch.float32, 128, 32, 8, [16001], [1500], 8999, 0),
+    (L.F16, torch.float16, 64, 32, 16, [12345], [3000], 0, 0),
+    (L.Q8_0, torch.float16, 256, 24, 4, [16001], [1500], 0, 0), (L.Q8_0, torch.float32, 256, 24, 4, [11000], [700], 9001, 0),
+    (L.F16, torch.float32, 256, 24, 4, [8960 + 7 * i % 150 for i in range(90)], [1 + i % 3 for i in range(90)], 0, 8960),
+    (L.F16, torch.float16, 256, 24, 4, [8960 + 7 * i % 150 for i in range(90)], [1 + i % 3 for i in range(90)], 0, 8960),
+    (L.F16, torch.float16, 128, 32, 8, [8960 + 7 * i % 150 for i in range(60)], [1 + i % 2 for i in range(60)], 8300, 8960)])
+def test_attention_turned_order(ctx, kv, qt, D, H, Hkv, past, new, window, shared):
+    """Whole items of 64 tiles and more, whose tiles come in a turned order: the tile at the cache's end (or at the window's
+    beginning), with NaN in the slots that no row sees, stands in the middle. Ten runs with the same bits. `shared`: the
+    sequences' first tokens stand in the same pages."""
+    rng = np.random.default_rng(D + H + window)
+    P = 64
+    sh = shared // P
+    q, caches, vals, table, q_start, kv_len = attn_case(rng, [p - shared for p in past], new, H, Hkv, D, P, kv, qt)
+    if sh:  # pages of the common beginning, in front of each sequence's own
+        kv_len = kv_len + np.int32(shared)
+        table = np.concatenate([np.tile(np.arange(sh, dtype=np.int32) + caches[0].shape[0], (len(past), 1)), table], 1)
+        for i in range(2):
+            v = rng.standard_normal((sh, P, Hkv, D)).astype(np.float16)
+            caches[i], vals[i] = np.concatenate([caches[i], v.view(np.uint8)]), np.concatenate([vals[i], v])
+    n_sm = torch.cuda.get_device_properties(0).multi_processor_count
+    _, turned, inside = R.turned_items(q_start, kv_len, H, Hkv, D, kv == L.Q8_0, qt == torch.float32, window, n_sm)
+    assert turned >= 20 and inside >= 20, (turned, inside)
+    d = [cu(x) for x in (q, caches[0], caches[1], table, q_start, kv_len)]
+    runs = [ctx.flash_attn_paged(d[0], d[1], d[2], kv, d[3], d[4], d[5], scale=D ** -0.5, window=window)
+            for _ in range(10)]
+    torch.cuda.synchronize()
+    ctx.check()
+    seqs = [[], []]
+    for c, v in zip(seqs, vals):
+        vt = cu(v)
+        for s, L_ in enumerate(kv_len):
+            pages = cu(table[s, :-(-int(L_) // P)].astype(np.int64))
+            c.append(vt[pages].flatten(0, 1)[:int(L_)])
+    ref = R.attention_dense(d[0], seqs[0], seqs[1], q_start, kv_len, D ** -0.5, window)
+    attn_bound(runs[0].cpu().numpy(), q, ref, q_start, kv_len)
+    for r in runs[1:]:
+        assert torch.equal(r, runs[0])
+
+
 def test_attention_far_pages(ctx):
     """Pages behind 2^32 bytes of a pool."""
     P, Hkv, D, H = 64, 8, 128, 8
