@@ -624,7 +624,7 @@ def sample_case(rng, ks, V, draft=True, agree=True):
     return lg, ids, q_start, u, us, dp if draft else None
 
 
-def sample_check(ctx, lg, ids, q_start, u, us, dp=None, temp=None):
+def sample_check(ctx, lg, ids, q_start, u, us, dp=None, temp=None, ref_temp=None):
     T = lg.shape[0]
     out = (torch.full((T,), -9, dtype=torch.int32, device="cuda"), torch.full((len(q_start) - 1,), -9,
            dtype=torch.int32, device="cuda"), torch.full((T,), -9.0, device="cuda"))
@@ -632,7 +632,7 @@ def sample_check(ctx, lg, ids, q_start, u, us, dp=None, temp=None):
                       temperature=None if temp is None else cu(temp), out=out)
     torch.cuda.synchronize()
     ctx.check()
-    wi, wn, wp = R.sample(lg, ids, q_start, u, us, dp, temp)
+    wi, wn, wp = R.sample(lg, ids, q_start, u, us, dp, temp if ref_temp is None else ref_temp)
     assert out[1].cpu().tolist() == wn
     assert out[0].cpu().tolist() == [-9 if i is None else i for i in wi]
     p = out[2].cpu().numpy()
@@ -739,6 +739,47 @@ def test_sample_temperatures(ctx):
         lg[:, 700] = lg[:, 90] = lg.max(1) + 0.5
         ids[1::2] = 700
         sample_check(ctx, lg, ids, q_start, u, us, dp, temp)
+
+
+@pytest.mark.parametrize("V,ks,draft", [(151936, [2, 0, 3, 1, 2, 0], True), (151936, [2, 0, 3, 1, 2, 0], False),
+                                        (5003, [3, 0, 4, 2, 1, 0] * 8, True), (5003, [3, 0, 4, 2, 1, 0] * 8, False),
+                                        (1200007, [0] * 75, False)])
+def test_sample_tokens_without_weight(ctx, V, ks, draft):
+    """u_sample of 0 and rows that begin with tokens of weight 0 (masked, NaN, at the type's lowest value, far below the
+    maximum at a low temperature): the first token that has a weight, never one of them."""
+    rng = np.random.default_rng(V)
+    T, S_ = sum(ks) + len(ks), len(ks)
+    q_start = np.concatenate([[0], np.cumsum(np.array(ks) + 1)]).astype(np.int32)
+    lg = rng.standard_normal((T, V), dtype=np.float32) * 2
+    temp = np.array([1.0, 0.7, 0.01, 1.3, 2e-4, 1.0] * S_, np.float32)[:S_]
+    lead = V * 2 // 3
+    for s in range(S_):
+        rows = slice(q_start[s], q_start[s + 1])
+        # 200 below: 20000 t and more at the low temperatures. Elsewhere -inf, NaN, the lowest value
+        lg[rows, :lead] = np.float32([-np.inf, np.nan, -200.0, np.finfo(np.float32).min, -200.0, -np.inf][s % 6])
+        lg[rows, lead + 5 + s % 3] = 30.0  # weight of the low temperatures' rows
+    ids = rng.integers(0, V, T).astype(np.int32)
+    u = np.full(T, 0.5, np.float32)
+    dp = None
+    if draft:
+        e = np.exp(np.nan_to_num(rng.standard_normal((T, V), dtype=np.float32)))
+        dp = (e / e.sum(1, keepdims=True)).astype(np.float32)
+    for us in (0.0, 2.0 ** -24, 0.5):
+        sample_check(ctx, lg, ids, q_start, u, np.full(S_, us, np.float32), dp, temp)
+
+
+@pytest.mark.parametrize("draft", [True, False])
+def test_sample_high_temperatures_beside_masked_tokens(ctx, draft):
+    """Temperatures up to infinity leave a masked token its weight of 0: (l - m) / t of -inf is -inf, and for an infinite
+    t (a limit, taken at the largest f32: exp of 1e-36 at most is 1 in 64 bits) the others weigh the same."""
+    rng = np.random.default_rng(21)
+    temp = np.array([1e30, 1e35, 1e36, 1e37, 3e38, np.inf] * 2, np.float32)
+    lg, ids, q_start, u, us, dp = sample_case(rng, [2] * 12, 30011, draft)
+    lg[:, rng.permutation(30011)[:20000]] = -np.inf
+    lg[:, :4000] = -np.inf
+    lg[15:18, [5000, 20000]] = np.inf  # the weight stands on these alone, at t = inf too
+    us[::3] = 0.0
+    sample_check(ctx, lg, ids, q_start, u, us, dp, temp, np.minimum(temp, np.finfo(np.float32).max))
 
 
 # ---- together --------------------------------------------------------------------------------------------------------
