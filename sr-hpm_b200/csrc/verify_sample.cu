@@ -16,7 +16,7 @@
 //                        more, in order; block sums, CTA sums and the sums inside one block find the place.
 //
 // Measured with 151936 tokens: 9 rows of one sequence 16.4 us (latencies: 6 the parts, 3.5 acceptance, 4 the weights, 2 the
-// place); 64 sequences of 3 to 9 rows with the drafter's distributions 72: 35 the parts at the copy rate, 37 the pick, whose
+// place); 64 sequences of 3 to 9 rows with the drafter's distributions 75: 35 the parts at the copy rate, 40 the pick, whose
 // 64-bit instructions and conversions take 67 cycles per 32 tokens and scheduler (two CTAs on 108 SMs, one on the others).
 #include <cuda_runtime.h>
 
@@ -403,11 +403,14 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
     };
     auto cluster_get = [&](int i, int r) { return ld_dsmem_f64(mapa_shared(smem_u32(&share[i]), r)); };
     // One pass over the share gives the row's sum Z, and per block the sums of e and of q over the tokens with e / Z > q,
-    // told apart by the f32 records' Z: a token on the wrong side has |e / Z - q| below 2^-20 of either, and few are that
-    // near, so the block's weight (sum e) / Z - sum q is as good as its terms.
+    // told apart by the f32 records' Z: the block's weight is then (sum e) / Z - sum q. A block with a token whose e / Z is
+    // nearer to q than 2^-19 (to 2^-18: 4 steps of the doubles' upper words) is done again with Z in 64 bits, and so are all
+    // blocks where the records' Z turns out to be off by more than 2^-20 (it is mostly near 2^-22): every other token is on
+    // its side. One token in 10^5 is that near where the drafter is 0.5 off in the logits, all are where it equals the
+    // target. 64 sequences: 75 us; without 72, with a margin of 2^-16, which bounds the records' Z beforehand, 78.
     {
         double      sz = 0.0;
-        auto block = [&](auto pieces, int at, double & se, double & sq) {  // `pieces` times 128 tokens from `at`
+        auto block = [&](auto pieces, int at, double & se, double & sq, bool & near) {  // `pieces` times 128 tokens from `at`
             constexpr int P = decltype(pieces)::value;
             float         l[P][4], q[P][4];
             const int     j0 = at + lane * 4;
@@ -446,6 +449,7 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const double qe = q[k][e];
+                        near |= (uint32_t) (__double2hiint(w[e]) - __double2hiint(qe * pz) + 4) <= 8u;
                         asm("{\n\t.reg .pred p, has;\n\tsetp.ge.f32 has, %6, %7;\n\tsetp.gt.and.f64 p, %3, %4, has;\n\t"
                             "@has add.f64 %2, %2, %3;\n\t@p add.f64 %0, %0, %3;\n\t@p add.f64 %1, %1, %5;\n\t}"
                             : "+d"(se), "+d"(sq), "+d"(sz)
@@ -467,16 +471,18 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
         };
         for (int g = g0 + warp; g < g1; g += kPickWarps) {
             double se = 0.0, sq = 0.0;
+            bool   near = false;
             if (len == 128) {
-                block(std::integral_constant<int, 1>{}, g * 128, se, sq);
+                block(std::integral_constant<int, 1>{}, g * 128, se, sq, near);
             } else {
-                for (int k = 0; k < len; k += 512) block(std::integral_constant<int, 4>{}, g * len + k, se, sq);
+                for (int k = 0; k < len; k += 512) block(std::integral_constant<int, 4>{}, g * len + k, se, sq, near);
             }
             se = warp_sum(se);
             if (qr) sq = warp_sum(sq);
+            near = __any_sync(0xffffffffu, near && ex.mode == 0);  // the other modes' sums are whole numbers
             if (lane == 0) {
                 bsum[g - g0] = se;
-                qsum[g - g0] = sq;
+                qsum[g - g0] = near ? -1.0 : sq;
             }
         }
         if (qr) {
@@ -492,6 +498,38 @@ template <int kCluster> __global__ void __launch_bounds__(kPickThreads, 2) sampl
             sz = 0.0;
             for (int r = 0; r < kCluster; r++) sz += cluster_get(0, r);
             inv_z = sz > 0.0 ? 1.0 / sz : 0.0;
+            const bool all = fabs(sz - pz) > sz * 0x1p-20;
+            __syncwarp();
+            for (int g = g0 + warp; g < g1; g += kPickWarps) {  // of this warp's blocks
+                if (!all && qsum[g - g0] >= 0.0) continue;
+                double sw = 0.0;
+                auto   again = [&](auto pieces, int j0) {  // a piece's loads go out together
+                    constexpr int P = decltype(pieces)::value;
+                    float         l[P][4], q[P][4];
+#pragma unroll
+                    for (int k = 0; k < P; k++) {
+                        logits4(j0 + 128 * k, l[k]);
+                        drafts4(j0 + 128 * k, q[k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < P; k++) {
+                        double w[4];
+                        weights(j0 + 128 * k, l[k], q[k], w);
+                        sw += (w[0] + w[1]) + (w[2] + w[3]);
+                    }
+                };
+                if (len == 128) {
+                    again(std::integral_constant<int, 1>{}, g * 128 + lane * 4);
+                } else {
+                    for (int k = 0; k < len; k += 512) again(std::integral_constant<int, 4>{}, g * len + k + lane * 4);
+                }
+                sw = warp_sum(sw);
+                __syncwarp();
+                if (lane == 0) {
+                    bsum[g - g0] = sw * sz;  // the scan below takes it times 1 / Z
+                    qsum[g - g0] = 0.0;
+                }
+            }
         }
     }
     __syncthreads();

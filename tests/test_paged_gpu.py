@@ -782,6 +782,49 @@ def test_sample_high_temperatures_beside_masked_tokens(ctx, draft):
     sample_check(ctx, lg, ids, q_start, u, us, dp, temp, np.minimum(temp, np.finfo(np.float32).max))
 
 
+@pytest.mark.parametrize("V,rows,flat", [(20011, 48, False), (151936, 8, False), (700, 48, False), (151936, 6, True)])
+def test_sample_drafter_equal_to_the_target(ctx, V, rows, flat):
+    """The drafter's distribution is the target's but for the last places of its f32 values: two steps below p at one token,
+    above p (by one step at least, 2^-24 of it) at all others. The replacement of the rejected token (its q is 2 p) can only be that token, whatever
+    the random number: weights are told from 0 with the 64-bit sum, not with the f32 one of the acceptance. `flat`: all
+    tokens but one at one distance from the maximum, at temperatures where that distance in f32 log2 units is off by
+    more than 2^-19.7, and the f32 sum with it."""
+    rng = np.random.default_rng(V)
+    T = 2 * rows
+    lg = rng.standard_normal((T, V)).astype(np.float32) * 3
+    temp = rng.uniform(0.3, 1.5, rows).astype(np.float32)
+    q_start = np.arange(0, T + 1, 2).astype(np.int32)
+    ids, dp = np.zeros(T, np.int32), np.zeros((T, V), np.float32)
+    only = rng.integers(0, V, rows)
+    if flat:
+        t = rng.uniform(0.9, 1.1, 20000).astype(np.float32)
+        y = np.float32(-10.5) * (np.float32(1.4426950408889634) / t)
+        off = np.log(2) * (y - -10.5 * 1.4426950408889634 / t.astype(np.float64))
+        temp = t[np.argsort(-np.abs(off))[:rows]]
+        assert np.sort(np.abs(off))[-rows] > 2.0 ** -19.7
+        lg[:] = -3.0
+        lg[:, 77777] = 7.5
+    for s in range(rows):
+        l = lg[2 * s].astype(np.float64)
+        e = np.exp((l - l.max()) / float(temp[s]))
+        p = e / e.sum()
+        q = p.astype(np.float32)
+        q = np.where(q < p, np.nextafter(q, np.float32(2)), q)  # p or above
+        down = np.nextafter(np.nextafter(np.nextafter(q, np.float32(0)), np.float32(0)), np.float32(0))
+        q = np.nextafter(q, np.float32(2))
+        q[only[s]] = down[only[s]]
+        x = int(l.argmax())
+        if x == only[s]:
+            x = (x + 1) % V
+        q[x] *= 2
+        ids[2 * s + 1], dp[2 * s] = x, q
+    u, us = np.full(T, 0.9, np.float32), rng.random(rows).astype(np.float32)
+    us[::4] = 0.0
+    out = ctx.verify_sample(cu(lg), cu(ids), cu(q_start), cu(u), cu(us), draft_probs=cu(dp), temperature=cu(temp))
+    assert out[1].cpu().tolist() == [1] * rows
+    assert out[0].cpu().tolist()[::2] == only.tolist()
+
+
 # ---- together --------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kv,D", [(L.F16, 128), (L.Q8_0, 256)])
 def test_steps_of_a_batch(ctx, kv, D):
