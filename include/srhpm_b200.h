@@ -310,7 +310,8 @@ int srhpm_swiglu(srhpm_ctx * ctx, const float * gate, const float * up, int64_t 
  * i32 [n_seqs], one of srhpm_page_status. A refused sequence takes no page, its rows are padding and its kv_len is 0;
  * one that finds no free page refuses every later one that needs a page too. A negative table entry of a page in the
  * cache gives slot -1. Nothing else of the table is written. 1 <= n_seqs <= 8192; page_size >= 1; free_pages, pos and
- * slots may be NULL where n_free or n_rows is 0. */
+ * slots may be NULL where n_free or n_rows is 0. No output may share memory with an input (kv_len with the next step's
+ * n_past, say: SRHPM_ERR_INVALID); the table with neither. */
 enum srhpm_page_status {
     SRHPM_PAGES_OK         = 0,
     SRHPM_PAGES_TABLE_FULL = 1, /* more pages than the table row has entries */
@@ -328,7 +329,7 @@ int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_n
  * turned queries written to q_out (f32 or f16, ne = [head_dim, n, n_head], the query view of srhpm_flash_attn_paged),
  * the turned keys and the values into the cache rows of slots[t] (i64; a slot outside the cache, -1 of a padding row
  * among them, stores nothing; two rows with one slot leave either's values there). f16 values round to nearest, q8_0
- * uses the context's q8_0 mode. head_dim 64, 128 or 256; qkv and q_out 16-byte aligned with row strides multiples of
+ * uses the context's q8_0 mode. q_out shares no memory with qkv or the caches. head_dim 64, 128 or 256; qkv and q_out 16-byte aligned with row strides multiples of
  * 16; cache strides multiples of 16 (f16) or 2 (q8_0). */
 int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, int n_head_kv, const int32_t * pos,
                         const int64_t * slots, float theta_base, const srhpm_tensor * q_out,
@@ -370,9 +371,9 @@ int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_
  * as they are. u_accept f32 [T], u_sample f32 [n_seqs], in [0, 1). p_r(x) of the acceptance and of p_draft has its sum in 32
  * bits: it is off by less than 2^-16 of itself (2^-22 mostly). The weights of a drawn token and their sums are kept in 64
  * bits, each exponential to 2^-39 of itself, so the token does not hang on the order of summation and one whose weight is
- * 0 is never drawn (an exponential below 2^-990 of the row's largest counts as 0). n_vocab <= 2^29; T and n_seqs <= 2^24.
- * wdata: srhpm_verify_sample_work_size bytes, of the call alone until
- * it is done. */
+ * 0 is never drawn (an exponential below 2^-990 of the row's largest counts as 0). out_ids, out_n and p_draft share no
+ * memory with the other vectors (SRHPM_ERR_INVALID). n_vocab <= 2^29; T and n_seqs <= 2^24. wdata:
+ * srhpm_verify_sample_work_size bytes, of the call alone until it is done. */
 int srhpm_verify_sample_work_size(const srhpm_ctx * ctx, const srhpm_tensor * logits, int n_seqs, size_t * size);
 int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start,
                         int n_seqs, const srhpm_tensor * draft_probs, const float * temperature,

@@ -187,6 +187,21 @@ int check_table(const srhpm_tensor * t) {
     return SRHPM_OK;
 }
 
+// An output vector that shares bytes with an input vector: CTAs write their outputs while others still read.
+struct Bytes {
+    const void * p;  // or null
+    size_t       n;
+};
+bool overlap(std::initializer_list<Bytes> out, std::initializer_list<Bytes> in) {
+    for (const Bytes & o : out) {
+        for (const Bytes & i : in) {
+            const uintptr_t a = (uintptr_t) o.p, b = (uintptr_t) i.p;
+            if (o.p && i.p && a < b + i.n && b < a + o.n) return true;
+        }
+    }
+    return false;
+}
+
 // token rows of heads: f32 or f16 [D, ., .], 16-byte aligned, strides multiples of 16
 int check_rows16(const srhpm_tensor * q, int64_t D) {
     if (!q || !q->data || q->ne[0] != D || q->ne[3] != 1) return SRHPM_ERR_INVALID;
@@ -668,6 +683,12 @@ int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_n
     if (st != SRHPM_OK) return st;
     if (block_table->ne[1] != n_seqs) return SRHPM_ERR_INVALID;
     if (!aligned(slots, 8)) return SRHPM_ERR_ALIGN;
+    if (n_seqs > kPlanMaxSeqs) return SRHPM_UNSUPPORTED;
+    const size_t per_seq = 4 * (size_t) n_seqs, rows = (size_t) n_rows;
+    if (overlap({ { q_start, per_seq + 4 }, { kv_len, per_seq }, { status, per_seq }, { n_taken, 4 }, { pos, 4 * rows }, { slots, 8 * rows } },
+                { { n_past, per_seq }, { n_new, per_seq }, { n_held, per_seq }, { free_pages, 4 * (size_t) n_free }, { free_head, 4 } })) {
+        return SRHPM_ERR_INVALID;
+    }
     return page_plan_run(ctx, n_past, n_new, n_held, n_seqs, page_size, block_table->data, (int64_t) block_table->nb[1],
                          (int) block_table->ne[0], free_pages, n_free, free_head, n_rows, q_start, kv_len, pos, slots,
                          status, n_taken, (cudaStream_t) stream);
@@ -780,6 +801,11 @@ int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int3
         st = check_logits(draft_probs, (int) logits->ne[1]);
         if (st != SRHPM_OK) return st;
         if (draft_probs->ne[0] != logits->ne[0]) return SRHPM_ERR_INVALID;
+    }
+    const size_t per_row = 4 * (size_t) logits->ne[1], per_seq = 4 * (size_t) n_seqs;
+    if (overlap({ { out_ids, per_row }, { out_n, per_seq }, { p_draft, per_row } },
+                { { ids, per_row }, { q_start, per_seq + 4 }, { temperature, per_seq }, { u_accept, per_row }, { u_sample, per_seq } })) {
+        return SRHPM_ERR_INVALID;
     }
     SampleView v;
     v.logits  = (const uint8_t *) logits->data;

@@ -149,7 +149,9 @@ struct PagedCache {
     int64_t         vnb1, vnb2, vnb3;
 };
 
-// paged_ops.cu: the page plan of a step, RoPE with the store into pages
+// paged_ops.cu: the page plan of a step (the lengths of at most kPlanMaxSeqs sequences stand in shared memory), RoPE with the
+// store into pages
+constexpr int kPlanMaxSeqs = 8192;
 int page_plan_run(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_new, const int32_t * n_held, int S, int page, void * table,
                   int64_t tstride, int cols, const int32_t * free_pages, int n_free, const int32_t * free_head,
                   int n_rows, int32_t * q_start, int32_t * kv_len, int32_t * pos, int64_t * slots, int32_t * status,

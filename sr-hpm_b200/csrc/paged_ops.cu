@@ -25,7 +25,6 @@ namespace {
 // itself (S <= 8192 lengths from L2, kept in shared memory) and then fills its share of rows and table entries, instead
 // of a scan kernel with a fill kernel behind it. 8 sequences 6.2 us on the GPU, 1024 with 249886 rows 16.4.
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanMaxSeqs = 8192;
 
 struct PlanArgs {
     const int32_t * past;
@@ -327,7 +326,6 @@ int page_plan_run(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_new
                   int64_t tstride, int cols, const int32_t * free_pages, int n_free, const int32_t * free_head,
                   int n_rows, int32_t * q_start, int32_t * kv_len, int32_t * pos, int64_t * slots, int32_t * status,
                   int32_t * n_taken, cudaStream_t stream) {
-    if (S > kPlanMaxSeqs) return SRHPM_UNSUPPORTED;
     PlanArgs a;
     a.past       = n_past;
     a.fresh      = n_new;

@@ -515,7 +515,8 @@ class Context:
         pages that a row names already, if more than n_past fills (after rejected tokens, torch.maximum(n_held,
         (kv_len + page_size - 1) // page_size) of the step before). Returns a
         PagePlan: q_start int32 [S + 1], kv_len int32 [S], pos int32 [n_rows], slots int64 [n_rows], status int32 [S],
-        n_taken int32 [1] (`out`: one to write into)."""
+        n_taken int32 [1] (`out`: one to write into, which shares no memory with the inputs: not the plan whose kv_len is
+        this step's n_past)."""
         S = n_past.numel()
         self._on_device(n_past, n_new, block_table, free_pages, free_head, n_held)
         i32 = torch.int32
@@ -580,7 +581,7 @@ class Context:
         int32 [T] its input tokens (the drafted token of row r is ids[r + 1]), q_start int32 [S + 1], u_accept f32 [T],
         u_sample f32 [S], draft_probs f32 [T, V] or None (a drafter without distributions), temperature f32 [S] or
         None. Returns (out_ids int32 [T], out_n int32 [S], p_draft f32 [T]); sequence s emitted
-        out_ids[q_start[s] : q_start[s] + out_n[s]]."""
+        out_ids[q_start[s] : q_start[s] + out_n[s]]. `out`: three to write into, which share no memory with the inputs."""
         T, S = logits.shape[0], q_start.numel() - 1
         self._on_device(logits, ids, q_start, u_accept, u_sample, draft_probs, temperature, work)
         i32, f32 = torch.int32, torch.float32

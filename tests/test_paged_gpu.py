@@ -135,6 +135,34 @@ def test_plan_heads_outside_the_list(ctx, head):
     assert r.status.cpu().tolist() == [0, 0, 2]
 
 
+def test_plan_steps_that_take_turns(ctx):
+    """Inputs and outputs side by side in one buffer, and each step's lengths from the step before, whose kv_len stays as it
+    is: two plans in turn. The plan that holds this step's lengths is refused as its output."""
+    rng = np.random.default_rng(17)
+    S_, P, T, cols = 5, 16, 64, 30
+    buf = torch.zeros(S_ + 2 * (3 * S_ + 2 + T), dtype=torch.int32, device="cuda")
+    new, *parts = buf.split([S_, S_ + 1, S_, T, S_, 1, S_ + 1, S_, T, S_, 1])
+    slots = torch.zeros(2, T, dtype=torch.int64, device="cuda")
+    plans = [S.PagePlan(*parts[:3], slots[0], *parts[3:5]), S.PagePlan(*parts[5:8], slots[1], *parts[8:])]
+    table = torch.full((S_, cols), -1, dtype=torch.int32, device="cuda")
+    free, head = cu(rng.permutation(S_ * cols).astype(np.int32)), torch.zeros(1, dtype=torch.int32, device="cuda")
+    ref, past, at = table.cpu().numpy(), np.zeros(S_, np.int64), 0
+    for i in range(6):
+        n = rng.integers(0, 13, S_).astype(np.int32)
+        new.copy_(cu(n))
+        before, pl = plans[(i + 1) % 2], plans[i % 2]
+        ctx.page_plan(before.kv_len, new, table, free, P, T, free_head=head, out=pl)
+        with pytest.raises(S.SrhpmError) as e:
+            ctx.page_plan(pl.kv_len, new, table, free, P, T, free_head=head, out=pl)
+        assert e.value.status == L.ERR_INVALID
+        torch.cuda.synchronize()
+        w = R.plan(past, n, ref, free.cpu().numpy(), P, T, at)
+        for g, x in zip((table, pl.q_start, pl.kv_len, pl.pos, pl.slots, pl.status, pl.n_taken), w):
+            assert np.array_equal(g.cpu().numpy().reshape(-1), np.asarray(x).reshape(-1))
+        ref, past, at = w[0], w[2], at + w[6]
+        head += pl.n_taken
+
+
 @pytest.mark.parametrize("kv,D,H,Hkv,P,n,qt", [
     (L.F16, 256, 24, 4, 64, 9, torch.float32), (L.F16, 128, 7, 7, 48, 33, torch.float16),
     (L.F16, 64, 5, 1, 16, 1, torch.float32), (L.Q8_0, 256, 6, 2, 32, 70, torch.float16),

@@ -150,3 +150,40 @@ def test_python_layer():
         _ints(torch.zeros(3, dtype=torch.int32), torch.int32, 4, "ids")
     with pytest.raises(ValueError):
         _ints(torch.zeros(8, dtype=torch.int32)[::2], torch.int32, 4, "ids")
+
+
+# vectors a page apart; n_seqs 2, n_rows 7, n_free 5
+PLAN_IN = {"n_past": 8, "n_new": 8, "n_held": 8, "free": 20, "free_head": 4}
+PLAN_OUT = {"q_start": 12, "kv_len": 8, "pos": 28, "slots": 56, "status": 8, "n_taken": 4}
+
+
+@pytest.mark.parametrize("i", PLAN_IN)
+@pytest.mark.parametrize("o", PLAN_OUT)
+@pytest.mark.parametrize("where", ["same", "first byte", "last byte"])
+def test_page_plan_outputs_that_share_memory_with_inputs(i, o, where):
+    """kv_len as the next step's n_past, above all: other CTAs read lengths that this one has written over."""
+    at = {n: A + 4096 * k for k, n in enumerate([*PLAN_IN, *PLAN_OUT])}
+    if o == "slots":  # stays aligned: the input moves instead
+        at[i] = at[o] + {"same": 0, "first byte": 4 - PLAN_IN[i], "last byte": PLAN_OUT[o] - 4}[where]
+    else:
+        at[o] = at[i] + {"same": 0, "first byte": 4 - PLAN_OUT[o], "last byte": PLAN_IN[i] - 4}[where]
+    st = lib.srhpm_page_plan(CTX, at["n_past"], at["n_new"], at["n_held"], 2, 16, ctypes.byref(table(data=A + (1 << 18))), at["free"], 5,
+                             at["free_head"], 7, at["q_start"], at["kv_len"], at["pos"], at["slots"], at["status"],
+                             at["n_taken"], None)
+    assert st == L.ERR_INVALID
+
+
+SAMPLE_IN = {"ids": 20, "q_start": 12, "temperature": 8, "u": 20, "us": 8}
+SAMPLE_OUT = {"out_ids": 20, "out_n": 8, "p_draft": 20}
+
+
+@pytest.mark.parametrize("i", SAMPLE_IN)
+@pytest.mark.parametrize("o", SAMPLE_OUT)
+@pytest.mark.parametrize("where", ["same", "first byte", "last byte"])
+def test_verify_sample_outputs_that_share_memory_with_inputs(i, o, where):
+    at = {n: A + 4096 * k for k, n in enumerate([*SAMPLE_IN, *SAMPLE_OUT])}
+    at[o] = at[i] + {"same": 0, "first byte": 4 - SAMPLE_OUT[o], "last byte": SAMPLE_IN[i] - 4}[where]
+    st = lib.srhpm_verify_sample(CTX, ctypes.byref(view(L.F32, [1000, 5], [4, 4000])), at["ids"], at["q_start"], 2, None,
+                                 at["temperature"], at["u"], at["us"], at["out_ids"], at["out_n"], at["p_draft"], A,
+                                 1 << 30, None)
+    assert st == L.ERR_INVALID
