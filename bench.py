@@ -209,6 +209,19 @@ def cpu_sample(host_w, host_x, ops, target_s):
     return b / t / 1e9, t, passes, nth, kind, (O.ref_variant() or "none")
 
 
+def cpu_baseline(host_w, host_x, ops, target_s):
+    """The line's CPU baseline. Without the reference's kernels (their sources were not here) the line goes without it; any
+    other failure is one."""
+    sys.path.insert(0, os.path.join(ROOT, "oracle"))
+    import oracle as O
+    if O.load_ref() is None and any(op[1] != TYPE_IDS["q8_0"] for op in ops):
+        return {"unavailable": "the reference kernels (oracle/_ref) are not built"}
+    gbs, secs, passes, nth, kind, variant = cpu_sample(host_w, host_x, ops, target_s)
+    return {"value": round(gbs, 3), "unit": "GB/s", "cores": nth, "kind": kind,
+            "sample": f"{passes} full passes of the workload ({secs:.1f} s of CPU time); reference srv kernels build "
+                      f"{variant}; Q8_0 (no srv kernel) through the restated stock path"}
+
+
 # ------------------------------------------------------------------------------------------------------------------
 
 def dist_setup():
@@ -691,13 +704,7 @@ def run_gpu(args):
                                                                    n_past=131072, reps=5)
         cpu = None
         if world == 1 and not args.no_cpu:
-            try:
-                gbs, secs, passes, nth, kind, variant = cpu_sample(host_w, host_x, base_ops, args.cpu_seconds)
-                cpu = {"value": round(gbs, 3), "unit": "GB/s", "cores": nth, "kind": kind,
-                       "sample": f"{passes} full passes of the workload ({secs:.1f} s of CPU time); reference srv "
-                                 f"kernels build {variant}; Q8_0 (no srv kernel) through the restated stock path"}
-            except RuntimeError as e:  # without the reference's sources: the line without its baseline
-                cpu = {"unavailable": str(e)}
+            cpu = cpu_baseline(host_w, host_x, base_ops, args.cpu_seconds)
             # the baseline's own outputs against the device's outputs of the timed step, every row of every product
             try:
                 meas["sweep_parity_vs_reference_kernels"] = cpu_parity(host_w, host_x, ops, y_dev, yoff)
