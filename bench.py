@@ -248,7 +248,7 @@ def run_reference(args):
     ref = O.load_ref()
     if ref is None:
         print(json.dumps({"impl": "reference", "unavailable": "the reference kernels (oracle/_ref) are not built: its "
-                                                              "sources are not here"}))
+                                                              "sources are not here"}), file=JSON_OUT, flush=True)
         return 0
     ops = sweep_ops(args.only)
     host_w = make_host_weights(ops, oracle_quantizer())

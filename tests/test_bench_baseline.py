@@ -1,5 +1,7 @@
 """The CPU baseline of the bench line: left out only where the reference's kernels are not built."""
+import json
 import os
+import subprocess
 import sys
 
 import numpy as np
@@ -37,3 +39,13 @@ def test_q8_0_needs_no_reference_kernels(monkeypatch):
     r = bench.cpu_baseline({(Q80, 64, 256): w}, {(4, 256): np.ones((4, 256), np.float32)},
                            [(4, Q80, 64, 256)], 0.01)
     assert r["kind"] == "port" and r["value"] > 0
+
+
+@pytest.mark.skipif(O.load_ref() is not None, reason="the reference's kernels are built: its arm runs")
+def test_the_reference_arm_without_its_kernels():
+    """One JSON line on the standard output, as every run of the bench prints it."""
+    r = subprocess.run([sys.executable, bench.__file__, "--impl", "reference", "--steps", "1", "--warmup", "0"],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0
+    line = json.loads(r.stdout)
+    assert line["impl"] == "reference" and line["unavailable"]
