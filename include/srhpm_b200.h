@@ -290,28 +290,31 @@ int srhpm_swiglu(srhpm_ctx * ctx, const float * gate, const float * up, int64_t 
 
 /* ---- a batch of sequences over a paged KV cache ----------------------------------------------------------------
  * One step of a batch: the new token rows of n_seqs sequences stand one sequence after another in row buffers of T
- * rows; sequence s has rows q_start[s] .. q_start[s + 1] - 1 (any number, 0 too), and rows behind the last sequence are
- * padding. The caches are pools of pages: k / v views with ne = [head_dim, page_size, n_head_kv, n_pages] and strides
- * nb[1] (token), nb[2] (KV head), nb[3] (page), type f16 or q8_0. A sequence's position p sits in slot p % page_size of
- * the page that entry p / page_size of its block table row names (block_table: i32, ne = [entries, n_seqs], row stride
- * nb[1]); a slot number is page * page_size + p % page_size. All lengths, tables and slots are read on the device, so a
- * step can be captured once and replayed with new ones. A verify step calls, in this order: srhpm_page_plan, then per
- * layer srhpm_rope_kv_paged and srhpm_flash_attn_paged, and srhpm_verify_sample on the logits of the rows. No
- * counterpart in the reference (one sequence, a contiguous cache, greedy acceptance). */
+ * rows; sequence s has rows q_start[s] .. q_start[s + 1] - 1 (any number, 0 too), and rows behind the last sequence
+ * are padding. The caches are pools of pages: k / v views with ne = [head_dim, page_size, n_head_kv, n_pages] and
+ * strides nb[1] (token), nb[2] (KV head), nb[3] (page), type f16 or q8_0. A sequence's position p sits in slot p %
+ * page_size of the page that entry p / page_size of its block table row names (block_table: i32, ne = [entries,
+ * n_seqs], row stride nb[1]); a slot number is page * page_size + p % page_size. All lengths, tables and slots are
+ * read on the device, so a step can be captured once and replayed with new ones. A verify step calls, in this
+ * order: srhpm_page_plan, then per layer srhpm_rope_kv_paged and srhpm_flash_attn_paged, and srhpm_verify_sample on
+ * the logits of the rows to be scored (all of a draft, the last one of a prompt, none of a refused sequence), with
+ * starts of their own. No counterpart in the reference (one sequence, a contiguous cache, greedy acceptance). */
 
-/* srhpm_page_plan: the step's block table entries, row starts, cache lengths, positions and slots, from the sequences'
- * lengths: n_past[s] tokens in the cache (its first ceil(n_past / page_size) table entries name their pages) and
- * n_new[s] >= 0 new ones (i32 [n_seqs] both). n_held i32 [n_seqs] or NULL: table entries that name a sequence's pages
- * already, where they are more than its cache fills (after rejected tokens: max(n_held, ceil(kv_len / page_size)) of the
- * step before; without n_held those pages are taken anew). A sequence that needs pages takes them, in order of sequences, from
- * free_pages[*free_head ..] (free_head NULL: 0; n_free entries in all), written behind its entries; n_taken i32 [1]
- * receives how many were taken (the next step's head is *free_head + *n_taken). Outputs: q_start i32 [n_seqs + 1];
- * kv_len i32 [n_seqs] = n_past + n_new; per row pos i32 [n_rows] and slots i64 [n_rows] (padding rows: 0 and -1); status
- * i32 [n_seqs], one of srhpm_page_status. A refused sequence takes no page, its rows are padding and its kv_len is 0;
- * one that finds no free page refuses every later one that needs a page too. A negative table entry of a page in the
- * cache gives slot -1. Nothing else of the table is written. 1 <= n_seqs <= 8192; page_size >= 1; free_pages, pos and
- * slots may be NULL where n_free or n_rows is 0. No output may share memory with an input (kv_len with the next step's
- * n_past, say: SRHPM_ERR_INVALID); the table with neither. */
+/* srhpm_page_plan: the step's block table entries, row starts, cache lengths, positions and slots, from the
+ * sequences' lengths: n_past[s] tokens in the cache (its first ceil(n_past / page_size) table entries name their
+ * pages) and n_new[s] >= 0 new ones (i32 [n_seqs] both). n_held i32 [n_seqs] or NULL: table entries that name a
+ * sequence's pages already, where they are more than its cache fills (after rejected tokens: max(n_held, ceil(kv_len
+ * / page_size)) of the step before; without n_held those pages are taken anew). A sequence that needs pages takes
+ * them, in order of sequences, from free_pages[*free_head ..] (free_head NULL: 0; n_free entries in all), written
+ * behind its entries; n_taken i32 [1] receives how many were taken (the next step's head is *free_head + *n_taken).
+ * Outputs: q_start i32 [n_seqs + 1]; kv_len i32 [n_seqs] = n_past + n_new; per row pos i32 [n_rows] and slots i64
+ * [n_rows] (padding rows: 0 and -1); status i32 [n_seqs], one of srhpm_page_status. A refused sequence takes no page
+ * and its kv_len is 0; its rows keep their place in q_start, with the pos and slots of padding (they store nothing
+ * and attend to nothing, but srhpm_verify_sample would score them); one that finds no free page refuses every later
+ * one that needs a page too. A negative table entry of a page in the cache gives slot -1. Nothing else of the table
+ * is written. 1 <= n_seqs <= 8192; page_size >= 1; free_pages, pos and slots may be NULL where n_free or n_rows is 0.
+ * No output may share memory with an input (kv_len with the next step's n_past, say: SRHPM_ERR_INVALID); the table
+ * with neither. */
 enum srhpm_page_status {
     SRHPM_PAGES_OK         = 0,
     SRHPM_PAGES_TABLE_FULL = 1, /* more pages than the table row has entries */
@@ -324,13 +327,14 @@ int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_n
                     int n_rows, int32_t * q_start, int32_t * kv_len, int32_t * pos, int64_t * slots, int32_t * status,
                     int32_t * n_taken, void * stream);
 
-/* srhpm_rope_kv_paged: qkv f32 rows, ne = [(n_head + 2 n_head_kv) * head_dim, n] (query heads | key heads | value heads;
- * only read): NeoX rotary embedding of the query and key heads at pos[t] (as srhpm_rope_kv, the angles in 64 bits), the
- * turned queries written to q_out (f32 or f16, ne = [head_dim, n, n_head], the query view of srhpm_flash_attn_paged),
- * the turned keys and the values into the cache rows of slots[t] (i64; a slot outside the cache, -1 of a padding row
- * among them, stores nothing; two rows with one slot leave either's values there). f16 values round to nearest, q8_0
- * uses the context's q8_0 mode. q_out shares no memory with qkv or the caches. head_dim 64, 128 or 256; qkv and q_out 16-byte aligned with row strides multiples of
- * 16; cache strides multiples of 16 (f16) or 2 (q8_0). */
+/* srhpm_rope_kv_paged: qkv f32 rows, ne = [(n_head + 2 n_head_kv) * head_dim, n] (query heads | key heads | value
+ * heads; only read): NeoX rotary embedding of the query and key heads at pos[t] (as srhpm_rope_kv, the angles in 64
+ * bits), the turned queries written to q_out (f32 or f16, ne = [head_dim, n, n_head], the query view of
+ * srhpm_flash_attn_paged), the turned keys and the values into the cache rows of slots[t] (i64; a slot outside the
+ * cache, -1 of a padding row among them, stores nothing; two rows with one slot leave either's values there). f16
+ * values round to nearest, q8_0 uses the context's q8_0 mode. q_out shares no memory with qkv or the caches. head_dim
+ * 64, 128 or 256; qkv and q_out 16-byte aligned with row strides multiples of 16; cache strides multiples of 16 (f16)
+ * or 2 (q8_0). */
 int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, int n_head_kv, const int32_t * pos,
                         const int64_t * slots, float theta_base, const srhpm_tensor * q_out,
                         const srhpm_tensor * k_cache, const srhpm_tensor * v_cache, void * stream);
@@ -359,21 +363,23 @@ int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_
                            srhpm_tensor * dst, void * wdata, size_t wsize, void * stream);
 
 /* srhpm_verify_sample: acceptance of drafted tokens that keeps the target's distribution, from given random numbers.
- * logits f32 [n_vocab, T]; ids i32 [T] are the step's input tokens: row r of a sequence scores the token behind ids[r],
- * so its drafted token is x = ids[r + 1] (none for the sequence's last row). p_r = softmax(logits_r / temperature[s])
- * (temperature NULL: 1; <= 0: all on the row's first maximum); q_r the drafter's distribution (draft_probs f32
- * [n_vocab, >= T], >= 0; NULL: all on x). Rows are scanned in order: x is accepted when u_accept[r] * q_r(x) < p_r(x);
- * the first row whose x is not accepted emits a token drawn from max(p_r - q_r, 0), and when all are accepted the last
- * row emits one drawn from p_r: the first j whose inclusive sum of weights is above u_sample[s] times their total (a
- * total of 0: the row's first maximum). NaN logits count as -inf. out_ids i32 [T]: the emitted ids in the sequence's
- * rows, -1 in the rest of them; out_n i32 [n_seqs]: their count (accepted + 1; 0 for a sequence without rows); p_draft
- * f32 [T] or NULL: p_r(x) of each row with a drafted token, 0 for a last row. Padding rows of out_ids and p_draft stay
- * as they are. u_accept f32 [T], u_sample f32 [n_seqs], in [0, 1). p_r(x) of the acceptance and of p_draft has its sum in 32
- * bits: it is off by less than 2^-16 of itself (2^-22 mostly). The weights of a drawn token and their sums are kept in 64
- * bits, each exponential to 2^-39 of itself, so the token does not hang on the order of summation and one whose weight is
- * 0 is never drawn (an exponential below 2^-990 of the row's largest counts as 0). out_ids, out_n and p_draft share no
- * memory with the other vectors (SRHPM_ERR_INVALID). n_vocab <= 2^29; T and n_seqs <= 2^24. wdata:
- * srhpm_verify_sample_work_size bytes, of the call alone until it is done. */
+ * logits f32 [n_vocab, T]; ids i32 [T] are the rows' input tokens: row r of a sequence scores the token behind
+ * ids[r], so its drafted token is x = ids[r + 1] (none for the sequence's last row). Every row but the last is taken
+ * for a draft's: of a prompt, whose tokens are given, only the last row belongs here, and no row of a sequence that
+ * srhpm_page_plan refused; q_start i32 [n_seqs + 1] are the starts of these rows. p_r = softmax(logits_r /
+ * temperature[s]) (temperature NULL: 1; <= 0: all on the row's first maximum); q_r the drafter's distribution
+ * (draft_probs f32 [n_vocab, >= T], >= 0; NULL: all on x). Rows are scanned in order: x is accepted when u_accept[r]
+ * * q_r(x) < p_r(x); the first row whose x is not accepted emits a token drawn from max(p_r - q_r, 0), and when all
+ * are accepted the last row emits one drawn from p_r: the first j whose inclusive sum of weights is above u_sample[s]
+ * times their total (a total of 0: the row's first maximum). NaN logits count as -inf. out_ids i32 [T]: the emitted
+ * ids in the sequence's rows, -1 in the rest of them; out_n i32 [n_seqs]: their count (accepted + 1; 0 for a sequence
+ * without rows); p_draft f32 [T] or NULL: p_r(x) of each row with a drafted token, 0 for a last row. Padding rows of
+ * out_ids and p_draft stay as they are. u_accept f32 [T], u_sample f32 [n_seqs], in [0, 1). p_r(x) of the acceptance
+ * and of p_draft has its sum in 32 bits: it is off by less than 2^-16 of itself (2^-22 mostly). The weights of a
+ * drawn token and their sums are kept in 64 bits, each exponential to 2^-39 of itself, so the token does not hang on
+ * the order of summation and one whose weight is 0 is never drawn (an exponential below 2^-990 of the row's largest
+ * counts as 0). out_ids, out_n and p_draft share no memory with the other vectors (SRHPM_ERR_INVALID). n_vocab <=
+ * 2^29; T and n_seqs <= 2^24. wdata: srhpm_verify_sample_work_size bytes, of the call alone until it is done. */
 int srhpm_verify_sample_work_size(const srhpm_ctx * ctx, const srhpm_tensor * logits, int n_seqs, size_t * size);
 int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start,
                         int n_seqs, const srhpm_tensor * draft_probs, const float * temperature,

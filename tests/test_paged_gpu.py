@@ -926,3 +926,83 @@ def test_steps_of_a_batch(ctx, kv, D):
         assert res[0].cpu().tolist()[:n] == si[:n] and res[1].cpu().tolist() == sn
         lens += np.array(sn)
     ctx.check()
+
+
+@pytest.mark.parametrize("kv,D", [(L.F16, 128), (L.Q8_0, 256)])
+def test_steps_with_prompts_refusals_and_held_pages(ctx, kv, D):
+    """The loop as the documents show it, captured once: prompts (only their last row is scored) beside drafts, a sequence that
+    finds no rows and comes again, one that finds no page, pages of rejected tokens that stay with their sequence. Lengths
+    and held pages are kept on the device and held to the host's."""
+    rng = np.random.default_rng(19)
+    S_, H, Hkv, P, cols, T, R_, V, pages = 4, 4, 2, 16, 12, 64, 24, 211, 11
+    i32 = dict(dtype=torch.int32, device="cuda")
+    n_past, n_new, held, head = (torch.zeros(n, **i32) for n in (S_, S_, S_, 1))
+    prompt = torch.zeros(S_, dtype=torch.bool, device="cuda")
+    table = torch.full((S_, cols), -1, **i32)
+    free = cu(rng.permutation(pages).astype(np.int32))
+    row = 2 * D if kv == L.F16 else D // 32 * 34
+    kc, vc = (torch.full((pages, P, Hkv, row), 0x7f, dtype=torch.uint8, device="cuda") for _ in range(2))
+    qkv, ids = torch.zeros((T, (H + 2 * Hkv) * D), device="cuda"), torch.zeros(T, **i32)
+    q = torch.zeros((T, H, D), device="cuda")
+    att = torch.zeros_like(q)
+    Wv = cu((rng.standard_normal((H * D, V)) * 0.5).astype(np.float32))
+    u, us = torch.zeros(R_, device="cuda"), torch.zeros(S_, device="cuda")
+    r = torch.arange(R_, device="cuda")
+
+    def step():
+        pl = ctx.page_plan(n_past, n_new, table, free, P, T, free_head=head, n_held=held)
+        ctx.rope_kv_paged(qkv, pl.pos, pl.slots, kc, vc, kv, q)
+        ctx.flash_attn_paged(q, kc, vc, kv, table, pl.q_start, pl.kv_len, scale=D ** -0.5, out=att)
+        ok = pl.status == 0
+        n_score = torch.where(ok, torch.where(prompt, n_new.clamp(max=1), n_new), 0)
+        v_start = torch.nn.functional.pad(n_score.cumsum(0), (1, 0)).int()
+        s = (torch.searchsorted(v_start, r, right=True) - 1).clamp(max=S_ - 1)
+        rows = (pl.q_start[s + 1] - v_start[s + 1] + r).clamp(0, T - 1)
+        logits = att.view(T, H * D)[rows] @ Wv
+        out = ctx.verify_sample(logits, ids[rows], v_start, u, us)
+        n_past.add_(torch.where(ok, n_new - n_score + out[1], 0))
+        torch.maximum(held, (pl.kv_len + P - 1) // P, out=held)
+        head.add_(pl.n_taken)
+        return pl, out, logits, v_start, rows
+
+    step()
+    for t, v in ((n_past, 0), (held, 0), (head, 0), (table, -1), (kc, 0x7f), (vc, 0x7f)):
+        t.fill_(v)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        pl, out, logits, v_start, rows = step()
+    for t, v in ((n_past, 0), (held, 0), (head, 0), (table, -1), (kc, 0x7f), (vc, 0x7f)):
+        t.fill_(v)
+    lens, hold, ref_table, at, seen = np.zeros(S_, np.int64), np.zeros(S_, np.int64), np.full((S_, cols), -1, np.int32), 0, []
+    for new, pr in (([30, 20, 17, 0], [1, 1, 1, 0]), ([14, 1, 17, 9], [0, 0, 1, 1]), ([5, 3, 6, 9], [0] * 4),
+                    ([6, 5, 5, 5], [0] * 4), ([2, 40, 3, 1], [0, 1, 0, 0]), ([3, 4, 5, 9], [0] * 4)):
+        x = rng.standard_normal((T, (H + 2 * Hkv) * D)).astype(np.float32)
+        ids_n, u_n, us_n = rng.integers(0, V, T).astype(np.int32), rng.random(R_).astype(np.float32), rng.random(S_).astype(np.float32)
+        u_n[:6] = 0.0  # some drafts are accepted
+        for t, v in ((n_new, np.array(new, np.int32)), (prompt, np.array(pr, bool)), (qkv, x), (ids, ids_n), (u, u_n), (us, us_n)):
+            t.copy_(cu(v))
+        g.replay()
+        torch.cuda.synchronize()
+        w = R.plan(lens, new, ref_table, free.cpu().numpy(), P, T, at, hold)
+        ref_table, q_start, kv_len, pos, slots, status = w[:6]
+        at += w[6]
+        seen += status.tolist()
+        for a, b in ((table, ref_table), (pl.q_start, q_start), (pl.kv_len, kv_len), (pl.slots, slots), (pl.status, status)):
+            assert np.array_equal(a.cpu().numpy(), b)
+        raw = [c.cpu().numpy() for c in (kc, vc)]
+        vals = [c.view(np.float16) if kv == L.F16 else R.q8_values(c) for c in raw]
+        attn_check(att.cpu().numpy(), q.cpu().numpy(), vals, ref_table, np.minimum(q_start, T), kv_len, D ** -0.5)
+        score = np.where(status == 0, np.where(np.array(pr, bool), np.minimum(new, 1), new), 0)
+        starts = np.concatenate([[0], np.cumsum(score)])
+        at_rows = np.concatenate([np.arange(q_start[s + 1] - score[s], q_start[s + 1]) for s in range(S_)])
+        n = len(at_rows)
+        assert np.array_equal(v_start.cpu().numpy(), starts) and np.array_equal(rows.cpu().numpy()[:n], at_rows)
+        si, sn, _ = R.sample(logits.cpu().numpy()[:n], ids_n[at_rows], starts, u_n, us_n)
+        assert out[0].cpu().tolist()[:n] == si and out[1].cpu().tolist() == sn
+        lens += np.where(status == 0, np.array(new) - score + np.array(sn), 0)
+        hold = np.maximum(hold, -(-kv_len // P))
+        assert np.array_equal(n_past.cpu().numpy(), lens) and np.array_equal(held.cpu().numpy(), hold)
+        # every page that was taken is some sequence's, and no page is two sequences'
+        assert int(head) == at == int(hold.sum()) == int((ref_table >= 0).sum()) == len(np.unique(ref_table[ref_table >= 0]))
+    assert {0, 2, 4} <= set(seen)
+    ctx.check()
