@@ -1303,7 +1303,10 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
 // The records of an item cut between CTAs, joined in the order of the cuts. CTA c opens the item (record 2c + 1), CTAs
 // c + 1 .. c + parts - 1 go on with it (records 2(c + 1), 2(c + 2), ...). Few parts (prompts: two or three, hundreds of
 // rows): a warp per row. Many (long caches, few rows): the CTA's 8 warps share out a row's parts, every eighth each, and join
-// in shared memory. Four records of a lane in flight: 16 took so many registers that the cut items of 18 prompts of 64
+// in shared memory. The border by whole calls over 8000 tokens (a warp per row / shared out, us), where both meet at some 1.5
+// rows per part: 6 rows in 37 parts 23.1 / 18.3, 54 in 37 25.4 / 23.8, 24 in 18 25.5 / 25.5, 54 in 18 27.7 / 28.7, 54 in 12
+// 36.4 / 38.5 (24 / 4 heads of 256); 4 rows in 9 parts 22.6 / 22.0, 64 in 9 36.5 / 40.9 (32 / 8 heads of 128). Tiles of more
+// rows have 16 CTAs per item: 126 rows in 148 parts 58 / 66. Four records of a lane in flight: 16 took so many registers that the cut items of 18 prompts of 64
 // tokens were joined in 41 us instead of 17.
 template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_merge_kernel(const __grid_constant__ PArgs a) {
     constexpr int V  = D / 32;  // values per lane, in pairs or fours side by side
@@ -1318,7 +1321,7 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
     if (d0.x == 0) return;
     const int4 d1 = a.desc[2 * c + 1];
     const int  lane = threadIdx.x & 31, warp = threadIdx.x >> 5, parts = d0.x;
-    const bool many = parts > 6 && d1.y <= 64;
+    const bool many = 2 * d1.y <= 3 * parts && d1.y <= 64;
     for (int row = many ? blockIdx.y : blockIdx.y * 8 + warp; row < d1.y; row += many ? gridDim.y : gridDim.y * 8) {
         const int tok = a.byG.div(d1.x + row), h = d0.y * a.G + (d1.x + row - tok * a.G);
         auto      rec = [&](int p) { return (int64_t) (2 * (c + p) + (p == 0 ? 1 : 0)) * a.prow + row; };
@@ -1447,11 +1450,20 @@ EncodeTiled encode_fn() {
     return fn;
 }
 
-// Rows of a CTA's tile by the sequences' average: at most kFew (decoding, verifying): one tile of kFew rows, whose Q takes
-// less than half the shared memory of 128 and leaves it to the K/V ring. The products have M = 64 there (decode 146 us with
-// 128, 130 with 64): their last 8 rows read what lies behind Q and go nowhere. kFew: what lets a q8_0 cache's rings (4 chunks, 8 raw slots) stand beside Q; it
-// holds 9 tokens of 6 heads. More: 128 rows, and with head_dim <= 128 two such tiles that share K/V. f32 rows over a q8_0
-// cache: always kFew (Q's two parts of 128 rows do not fit beside the rings).
+// Rows of a CTA's tile by the sequences' average (of the row buffer, padding included: the host knows no more): at most kFew
+// (decoding, verifying): one tile of kFew rows, whose Q takes less than half the shared memory of 128 and leaves it to the
+// K/V ring. The products have M = 64 there (decode 146 us with 128, 130 with 64): their last 8 rows read what lies behind Q
+// and go nowhere. kFew: what lets a q8_0 cache's rings (4 chunks, 8 raw slots) stand beside Q; it holds 9 tokens of 6 heads.
+// More: 128 rows, and with head_dim <= 128 two such tiles that share K/V. f32 rows over a q8_0 cache: always kFew (Q's two
+// parts of 128 rows do not fit beside the rings). 24 sequences of 500 to 8192 tokens, kFew / full tiles, us by rows of a
+// sequence and KV head:
+//   32 / 8 heads of 128, f16 rows: 4: 91 / 144, 48: 114 / 160, 64: 205 / 169, 128: 303 / 164; f32: 56: 136 / 221, 64: 187 / 173
+//   28 / 4 heads of 128: 28: 64 / 83, 63: 89 / 82, 140: 135 / 91
+//   24 / 4 heads of 256, f16: 6: 87 / 84, 54: 83 / 79, 72: 135 / 88; f32: 6: 95 / 98, 54: 122 / 128, 72: 209 / 130
+//   the same over q8_0, f16: 6: 149 / 142, 24: 113 / 115, 54: 130 / 140, 72: 217 / 134
+// Mixtures, for which the average says little: 64 single tokens beside a prompt of 500 rows 343 / 494 (takes kFew), 8 beside it
+// 92 / 105 (takes full tiles), 64 beside 2000 rows 479 / 508 (full). Padding: 32 single tokens in a buffer of 512 rows take
+// full tiles, 184 us instead of 111.
 struct Tile {
     int nt, br;
 };
