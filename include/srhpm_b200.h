@@ -14,7 +14,8 @@
  *   - calls are asynchronous and ordered on `stream` (a cudaStream_t; NULL = the legacy default stream).
  *   - errors are returned as srhpm_status codes, never by aborting. SRHPM_UNSUPPORTED means "not handled here, run
  *     the stock path", as the reference's compute_forward returning false does.
- *   - one srhpm_ctx per device; a context may be used from several host threads only with external serialisation.
+ *   - one srhpm_ctx per device; a context may be used from several host threads only with external serialisation, but for
+ *     the calls of a batch over a paged KV cache (srhpm_page_plan to srhpm_verify_sample), which may come at once.
  */
 #ifndef SRHPM_B200_H
 #define SRHPM_B200_H
@@ -341,20 +342,21 @@ int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, i
 
 /* srhpm_flash_attn_paged: row i of sequence s, at position p = kv_len[s] - (rows of s) + i, attends to the cached
  * positions j <= p, and j > p - window where window > 0: dst = softmax(scale * q k [softcap * tanh(. / softcap)] [+
- * sink]) v. q: ne = [head_dim, T, n_head], f32 or f16 (token stride nb[1], head stride nb[2]); dst of the same type, ne
- * = [head_dim, n_head, T] (head stride nb[1], token stride nb[2], as in srhpm_flash_attn_ext); head h reads KV head h /
- * (n_head / n_head_kv); sinks f32 [n_head], finite or -inf, or NULL. A row that sees nothing is 0; padding rows of dst
- * stay as they are. f16 rows: probabilities are rounded to f16 for the product with v, sums are kept in f32. f32 rows:
- * q and the probabilities are taken as sums of two f16 parts, so the result is exact to f32's order of magnitude. A
- * q8_0 cache is read as d * q rounded to f16. head_dim 64, 128 or 256 (q8_0: 256); page_size a multiple of 16; cache
- * data 16-byte aligned, its strides multiples of 16; q and dst 16-byte aligned with strides multiples of 16. Cache
- * slots behind a sequence's kv_len and before its window may hold anything, and pages wholly before the window may be
- * given away (their entries are not read). A table entry that is not a page of the cache reads as zeros and raises the
- * context's device status; positions behind the table's entries are not seen. Where the scores of a row hold a NaN, its
- * result is NaN; a value of the cache that is infinite or NaN reaches every row of its sequence if one of them sees it.
- * f32 q: finite in f16's range. dst overlaps neither q nor the caches. n_seqs <= 8192, and (T * n_head / n_head_kv / 56
- * + 1) * (entries * page_size / 64 + 1) < 2^31 (else SRHPM_UNSUPPORTED). wdata: srhpm_flash_attn_paged_work_size bytes,
- * of the call alone until it is done. */
+ * sink]) v. q: ne = [head_dim, T, n_head], f32 or f16 (token stride nb[1], head stride nb[2]); dst of the same type,
+ * ne = [head_dim, n_head, T] (head stride nb[1], token stride nb[2], as in srhpm_flash_attn_ext); head h reads KV
+ * head h / (n_head / n_head_kv); sinks f32 [n_head], finite or -inf, or NULL. A row that sees nothing is 0; padding
+ * rows of dst stay as they are. f16 rows: probabilities are rounded to f16 for the product with v, sums are kept in
+ * f32. f32 rows: q and the probabilities are taken as sums of two f16 parts: off by at most 2^-22 of themselves, or
+ * 2^-25 (q) and 2^-32 of the row's largest (probabilities) where that is more, beside f32 sums. A q8_0 cache is read
+ * as d * q rounded to f16 (2^-11 of each value), with f32 rows too. head_dim 64, 128 or 256 (q8_0: 256); page_size a
+ * multiple of 16; cache data 16-byte aligned, its strides multiples of 16; q and dst 16-byte aligned with strides
+ * multiples of 16. Cache slots behind a sequence's kv_len and before its window may hold anything, and pages wholly
+ * before the window may be given away (their entries are not read). A table entry that is not a page of the cache
+ * reads as zeros and raises the context's device status; positions behind the table's entries are not seen. Where the
+ * scores of a row hold a NaN, its result is NaN; a value of the cache that is infinite or NaN reaches every row of
+ * its sequence if one of them sees it. f32 q: finite in f16's range. dst overlaps neither q nor the caches. n_seqs <=
+ * 8192, and (T * n_head / n_head_kv / 56 + 1) * (entries * page_size / 64 + 1) < 2^31 (else SRHPM_UNSUPPORTED).
+ * wdata: srhpm_flash_attn_paged_work_size bytes, of the call alone until it is done. */
 int srhpm_flash_attn_paged_work_size(const srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_tensor * k_cache,
                                      int n_seqs, size_t * size);
 int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_tensor * k_cache,

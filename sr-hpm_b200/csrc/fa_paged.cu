@@ -25,15 +25,16 @@
 // NT = 2 (head_dim <= 128): two row tiles share K/V, each with its own 4 softmax warps and buffer.
 //
 // Measured (6.55 TB/s copy, 1632 TFLOP/s burst and 1321 sustained of a library product), both launches:
-//   32 sequences of 500 to 8192 tokens decoding, 32 / 8 heads of 128, pages of 16: 118 us, 5.4 TB/s; four times as long 6.5:
-//   some 25 us go to the plan, the first loads (their rows 2 to 5 us), items' ends and the join, the rest to memory.
-//   9 rows of f32 over 131072 tokens, 24 / 4 heads of 256: 111 us; back to back 130, the card at 1000 W and 1.6 GHz.
-//   4 sequences of 2048 to 16384 tokens over q8_0, 2 to 9 f16 rows, same heads: 74 us, a quarter of memory's rate: the
-//   conversion (a job of 32 tokens takes a warp 0.7 us) and 12 us until the first scores.
-//   2048 rows over 32768 tokens, 24 / 4 heads of 256: 1.40 ms, 1140 TFLOP/s; 1.57 back to back at 1.45 GHz (of sustained
-//   0.77). Shared memory's reads: QK takes 128 bytes a cycle for M = N = 128, PV 64, the tiles' arrival 64.
-//   seven sequences, prompts to 2000 rows and decoding, window 1024, 32 / 8 heads of 128: 138 us, of which 14 are the join and
-//   3 to 5 each item's end (a row per lane: its stores go at a sector per cycle).
+//   32 sequences of 500 to 8192 tokens decoding, 32 / 8 heads of 128, pages of 16: 119 us, 5.3 TB/s, back to back 125; four
+//   times as long 6.5 TB/s: 8 us go to the plan and the first loads, 11 to the spread of the CTAs' ends, 7 to the join.
+//   9 rows of f32 over 131072 tokens, 24 / 4 heads of 256: 109 us; back to back 129, the card at 1000 W and 1.6 GHz.
+//   4 sequences of 2048 to 16384 tokens over q8_0, 2 to 9 f16 rows, same heads: 71 us, a quarter of memory's rate: 3.3 us per
+//   tile and CTA (the conversion, a job of 32 tokens in 0.7 us, is under half of it) and 12 us until the first scores.
+//   2048 rows over 32768 tokens, 24 / 4 heads of 256: 1.38 ms, 1155 TFLOP/s; 1.63 back to back at 1.45 GHz (of sustained
+//   0.74). Shared memory's reads: QK takes 128 bytes a cycle for M = N = 128, PV 64, the tiles' arrival 64.
+//   seven sequences, prompts to 1000 rows and decoding, window 1024, 32 / 8 heads of 128: 137 us: 22 tiles per CTA at 3.4 us, 3
+//   to 4 for each item's end (a row per lane: its stores go at a sector per cycle; 2 to 11 items per CTA, so that the slowest
+//   is 28 us behind the mean), 12 the join.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
