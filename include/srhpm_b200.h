@@ -379,9 +379,10 @@ int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_
  * out_ids and p_draft stay as they are. u_accept f32 [T], u_sample f32 [n_seqs], in [0, 1). p_r(x) of the acceptance
  * and of p_draft has its sum in 32 bits: it is off by less than 2^-16 of itself (2^-22 mostly). The weights of a
  * drawn token and their sums are kept in 64 bits, each exponential to 2^-39 of itself, so the token does not hang on
- * the order of summation and one whose weight is 0 is never drawn (an exponential below 2^-990 of the row's largest
- * counts as 0). out_ids, out_n and p_draft share no memory with the other vectors (SRHPM_ERR_INVALID). n_vocab <=
- * 2^29; T and n_seqs <= 2^24. wdata: srhpm_verify_sample_work_size bytes, of the call alone until it is done. */
+ * the order of summation and one whose weight is 0 is never drawn (an exponential below e^-690 of the row's largest,
+ * a border taken in f32, counts as 0). out_ids, out_n and p_draft share no memory with the other vectors
+ * (SRHPM_ERR_INVALID). n_vocab <= 2^29; T and n_seqs <= 2^24. wdata: srhpm_verify_sample_work_size bytes, of the call
+ * alone until it is done. */
 int srhpm_verify_sample_work_size(const srhpm_ctx * ctx, const srhpm_tensor * logits, int n_seqs, size_t * size);
 int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start,
                         int n_seqs, const srhpm_tensor * draft_probs, const float * temperature,
