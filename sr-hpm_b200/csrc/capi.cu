@@ -196,7 +196,7 @@ bool overlap(std::initializer_list<Bytes> out, std::initializer_list<Bytes> in) 
     for (const Bytes & o : out) {
         for (const Bytes & i : in) {
             const uintptr_t a = (uintptr_t) o.p, b = (uintptr_t) i.p;
-            if (o.p && i.p && a < b + i.n && b < a + o.n) return true;
+            if (o.p && i.p && o.n && i.n && a < b + i.n && b < a + o.n) return true;
         }
     }
     return false;
