@@ -4,8 +4,9 @@
  *   - small-batch quantized matmul (ggml_mul_mat with ne[1] = 1..16 on Q4_K / Q5_K / Q6_K / Q3_K / IQ4_XS / Q8_0)
  *   - multi-query attention over an f16 or q8_0 KV cache (ggml_flash_attn_ext with 1..16 query rows)
  *   - greedy longest-prefix acceptance over the target logits
- * and, for a batch of sequences over a paged KV cache, plans the pages of a step, stores into them, attends over them and
- * accepts drafted tokens by sampling.
+ * and, for a batch of sequences over a paged KV cache (f16, q8_0 or q4_0), plans the pages of a step, stores into them,
+ * attends over them, applies penalties, biases and token masks to the logits and accepts drafted tokens by sampling; between
+ * steps it forks sequences, gives pages back and moves them together.
  *
  * Conventions (all entry points):
  *   - tensors are ggml-shaped views (srhpm_tensor: type, ne[4] in elements, nb[4] in bytes, data) of DEVICE memory,
@@ -15,7 +16,7 @@
  *   - errors are returned as srhpm_status codes, never by aborting. SRHPM_UNSUPPORTED means "not handled here, run
  *     the stock path", as the reference's compute_forward returning false does.
  *   - one srhpm_ctx per device; a context may be used from several host threads only with external serialisation, but for
- *     the calls of a batch over a paged KV cache (srhpm_page_plan to srhpm_verify_sample), which may come at once.
+ *     the calls of a batch over a paged KV cache (srhpm_page_plan to srhpm_adjust_logits), which may come at once.
  */
 #ifndef SRHPM_B200_H
 #define SRHPM_B200_H
@@ -31,6 +32,7 @@ extern "C" {
 enum srhpm_type {
     SRHPM_TYPE_F32    = 0,
     SRHPM_TYPE_F16    = 1,
+    SRHPM_TYPE_Q4_0   = 2,  /* of paged caches only */
     SRHPM_TYPE_Q8_0   = 8,
     SRHPM_TYPE_Q3_K   = 11,
     SRHPM_TYPE_Q4_K   = 12,
@@ -293,7 +295,8 @@ int srhpm_swiglu(srhpm_ctx * ctx, const float * gate, const float * up, int64_t 
  * One step of a batch: the new token rows of n_seqs sequences stand one sequence after another in row buffers of T
  * rows; sequence s has rows q_start[s] .. q_start[s + 1] - 1 (any number, 0 too), and rows behind the last sequence
  * are padding. The caches are pools of pages: k / v views with ne = [head_dim, page_size, n_head_kv, n_pages] and
- * strides nb[1] (token), nb[2] (KV head), nb[3] (page), type f16 or q8_0. A sequence's position p sits in slot p %
+ * strides nb[1] (token), nb[2] (KV head), nb[3] (page), type f16, q8_0 or q4_0 (ggml's blocks of 32 values: the step d as
+ * f16, then 16 bytes of which byte j holds number j in its low and number j + 16 in its high half; value d * (number - 8)). A sequence's position p sits in slot p %
  * page_size of the page that entry p / page_size of its block table row names (block_table: i32, ne = [entries,
  * n_seqs], row stride nb[1]); a slot number is page * page_size + p % page_size. All lengths, tables and slots are
  * read on the device, so a step can be captured once and replayed with new ones. A verify step calls, in this
@@ -333,9 +336,11 @@ int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_n
  * bits), the turned queries written to q_out (f32 or f16, ne = [head_dim, n, n_head], the query view of
  * srhpm_flash_attn_paged), the turned keys and the values into the cache rows of slots[t] (i64; a slot outside the
  * cache, -1 of a padding row among them, stores nothing; two rows with one slot leave either's values there). f16
- * values round to nearest, q8_0 uses the context's q8_0 mode. q_out shares no memory with qkv or the caches. head_dim
+ * values round to nearest, q8_0 uses the context's q8_0 mode, q4_0 ggml's reference rounding (d = -m / 8 for the value m of
+ * largest size, the first of equals; number = min(15, trunc(x * (1 / d) + 8.5)) in f32; a turned key next to the border of
+ * two numbers is turned in 64 bits). q_out shares no memory with qkv or the caches. head_dim
  * 64, 128 or 256; qkv and q_out 16-byte aligned with row strides multiples of 16; cache strides multiples of 16 (f16)
- * or 2 (q8_0). */
+ * or 2 (q8_0, q4_0). */
 int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, int n_head_kv, const int32_t * pos,
                         const int64_t * slots, float theta_base, const srhpm_tensor * q_out,
                         const srhpm_tensor * k_cache, const srhpm_tensor * v_cache, void * stream);
@@ -347,9 +352,10 @@ int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, i
  * head h / (n_head / n_head_kv); sinks f32 [n_head], finite or -inf, or NULL. A row that sees nothing is 0; padding
  * rows of dst stay as they are. f16 rows: probabilities are rounded to f16 for the product with v, sums are kept in
  * f32. f32 rows: q and the probabilities are taken as sums of two f16 parts: off by at most 2^-22 of themselves, or
- * 2^-25 (q) and 2^-32 of the row's largest (probabilities) where that is more, beside f32 sums. A q8_0 cache is read
- * as d * q rounded to f16 (2^-11 of each value), with f32 rows too. head_dim 64, 128 or 256 (q8_0: 256); page_size a
- * multiple of 16; cache data 16-byte aligned, its strides multiples of 16; q and dst 16-byte aligned with strides
+ * 2^-25 (q) and 2^-32 of the row's largest (probabilities) where that is more, beside f32 sums. A q8_0 or q4_0
+ * cache is read as d * q or d * (q - 8) rounded to f16 (2^-11 of each value), with f32 rows too. head_dim 64, 128 or 256
+ * (q8_0: 256); page_size a multiple of 16; cache data aligned to 16 bytes and its strides multiples of 16 (q4_0: of head_dim
+ * / 16 bytes); q and dst 16-byte aligned with strides
  * multiples of 16. Cache slots behind a sequence's kv_len and before its window may hold anything, and pages wholly
  * before the window may be given away (their entries are not read). A table entry that is not a page of the cache
  * reads as zeros and raises the context's device status; positions behind the table's entries are not seen. Where the
@@ -388,6 +394,70 @@ int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int3
                         int n_seqs, const srhpm_tensor * draft_probs, const float * temperature,
                         const float * u_accept, const float * u_sample, int32_t * out_ids, int32_t * out_n,
                         float * p_draft, void * wdata, size_t wsize, void * stream);
+
+/* srhpm_page_fork: n_forks new sequences that begin with the first n_keep[i] >= 0 tokens of others: block table row child[i]
+ * gets the first ceil(n_keep / page_size) entries of row parent[i]. Whole pages are shared: page_refs i32 [n_pages] (zeros at
+ * the start, kept by these calls) counts a page's holders beyond the first. A partly filled last page is replaced by one
+ * taken from free_pages, in order of forks, as srhpm_page_plan takes them (free_head, n_taken), and its copy is left to
+ * srhpm_page_copy: src[i], dst[i] (i32 [n_forks]; -1 and -1 where there is nothing to copy). The child's n_past is n_keep[i]. status i32
+ * [n_forks], of srhpm_page_status: a refused fork writes no entry and takes nothing; SRHPM_PAGES_BAD_LENGTH also for a row
+ * that the table lacks and for parent = child. An entry that is no page is handed on uncounted; if it is the partly filled
+ * one's, a page is taken and nothing copied. No two forks have one child, and no child is a parent of the same call (the rows
+ * then hold either's entries). Nothing else of the table is written. n_forks <= 8192. No output shares memory with an input
+ * or another output (SRHPM_ERR_INVALID). Not before n_keep[i] tokens of the parent are stored: calls are ordered on the
+ * stream. */
+int srhpm_page_fork(srhpm_ctx * ctx, const int32_t * parent, const int32_t * child, const int32_t * n_keep, int n_forks,
+                    int page_size, const srhpm_tensor * block_table, int32_t * page_refs, int n_pages,
+                    const int32_t * free_pages, int n_free, const int32_t * free_head, int32_t * src, int32_t * dst,
+                    int32_t * status, int32_t * n_taken, void * stream);
+
+/* srhpm_page_copy: page src[i] copied to page dst[i], i < n (i32 [n]; where either is not a page, nothing), in each of
+ * n_caches pools (an array of views in HOST memory: K and V of every layer, say), in one launch per 256 of them. The pools
+ * have one type (f16, q8_0 or q4_0), shape and strides (any multiples of 2). n_moves i32 [1] or NULL: only the first *n_moves. No dst stands
+ * twice or is a src of the same call (its page then holds either's bytes). */
+int srhpm_page_copy(srhpm_ctx * ctx, const srhpm_tensor * caches, int n_caches, const int32_t * src, const int32_t * dst, int n,
+                    const int32_t * n_moves, void * stream);
+
+/* srhpm_page_free: entries begin[i] .. end[i] - 1 (i32 [n]; begin NULL: 0) of block table rows rows[i] are given up: they
+ * become -1, each page's count of holders goes down, and the pages without one are written in front of *free_head into
+ * free_pages (i32 [n_free]), in the order of their numbers; n_freed i32 [1] receives how many (the next step's head is
+ * *free_head - *n_freed). For sequences that are done (0, entries held), and for pages behind a cache or before a window. An
+ * entry given up twice counts once; rows that the table lacks and entries that are no page are passed over. Pages that find
+ * no room in front of the head (more than were taken from the list) are lost, and the context's device status is raised.
+ * n_pages <= 2^22. No output shares memory with an input or another output (SRHPM_ERR_INVALID). */
+int srhpm_page_free(srhpm_ctx * ctx, const int32_t * rows, const int32_t * begin, const int32_t * end, int n,
+                    const srhpm_tensor * block_table, int32_t * page_refs, int n_pages, int32_t * free_pages, int n_free,
+                    const int32_t * free_head, int32_t * n_freed, void * stream);
+
+/* srhpm_page_compact: the pages in use (named by the first n_held[s] entries of the block table's rows; i32 [n_seqs]) get the
+ * lowest numbers, so that the pool's end can be given away: with n_used of them, the k-th page in use from n_used on goes to
+ * the k-th number below n_used that is not. The table's entries and page_refs follow, free_pages (i32 [n_pages]) becomes the
+ * number i at place i for n_used <= i < n_pages (its head is n_used from here on; the places before it stay), and src, dst (i32 [n_pages / 2]),
+ * n_moves, n_used (i32 [1]) say what srhpm_page_copy has to move; entries behind n_moves stay as they are. n_pages <= 2^22.
+ * No output shares memory with an input or another output (SRHPM_ERR_INVALID). */
+int srhpm_page_compact(srhpm_ctx * ctx, const srhpm_tensor * block_table, const int32_t * n_held, int32_t * page_refs, int n_pages,
+                       int32_t * free_pages, int32_t * src, int32_t * dst, int32_t * n_moves, int32_t * n_used, void * stream);
+
+/* srhpm_adjust_logits: rules on the logits f32 [n_vocab, T] of the rows that a step scores, before srhpm_verify_sample (ids
+ * and q_start as there). For the tokens x of row r of sequence s, in this order:
+ *   bias        l += bias[j] where bias_ids[j] = x for a j in bias_start[s] .. bias_start[s + 1] - 1 (the last such j; i32
+ *               [n_seqs + 1], i32 and f32 [n_bias]; n_bias 0: none)
+ *   penalties   where x stands c > 0 times in the row's window: l = l / repeat[s] if l > 0, else l * repeat[s]; then l -= c *
+ *               frequency[s] + presence[s] (f32 [n_seqs] each, repeat > 0; NULL: 1, 0 and 0). The window is the last
+ *               last_n[s] (i32 [n_seqs]; negative, or NULL: all) tokens of the sequence's history (i32, ne = [capacity,
+ *               n_seqs], n_history[s] of them: those before its first row here; or NULL) followed by ids[q_start[s]] ..
+ *               ids[r], so a drafted token counts in the rows behind it
+ *   mask        l = -inf where bit x % 32 of word x / 32 is 0 in the row's mask (mask i32, ne = [>= ceil(n_vocab / 32),
+ *               masks], or NULL): mask_row[r] (i32 [T]; outside the masks: none), or r where mask_row is NULL
+ * each step rounded to f32. out f32 [n_vocab, T]: the logits themselves, of which then only what changes is written, or
+ * memory that shares nothing with them; padding rows of out stay as they are. Tokens outside the vocabulary are passed
+ * over. A row whose mask leaves nothing is all -inf (srhpm_verify_sample then emits token 0). T and n_seqs <= 2^24, n_vocab <= 2^29, T *
+ * ceil(n_vocab / 8192) < 2^31 (else SRHPM_UNSUPPORTED). */
+int srhpm_adjust_logits(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start, int n_seqs,
+                        const srhpm_tensor * history, const int32_t * n_history, const int32_t * last_n, const float * repeat,
+                        const float * frequency, const float * presence, const int32_t * bias_start, const int32_t * bias_ids,
+                        const float * bias, int n_bias, const srhpm_tensor * mask, const int32_t * mask_row,
+                        const srhpm_tensor * out, void * stream);
 
 /* ---- host-side weight quantizer (CPU) -------------------------------------------------------------------------
  * f32 rows -> GGUF blocks of `type` (Q4_K, Q5_K, Q6_K, Q3_K, IQ4_XS, Q8_0, F16). Host pointers. Returns the bytes

@@ -144,7 +144,9 @@ int check_logits(const srhpm_tensor * lg, int min_rows) {
 // a paged cache: k / v of one type, [D, page, Hkv, pages], rows contiguous; `mult` divides every stride in bytes
 int check_paged(const srhpm_tensor * k, const srhpm_tensor * v, size_t mult, PagedCache * c) {
     if (!k || !v) return SRHPM_ERR_INVALID;
-    if (k->type != v->type || (k->type != SRHPM_TYPE_F16 && k->type != SRHPM_TYPE_Q8_0)) return SRHPM_UNSUPPORTED;
+    if (k->type != v->type || (k->type != SRHPM_TYPE_F16 && k->type != SRHPM_TYPE_Q8_0 && k->type != SRHPM_TYPE_Q4_0)) {
+        return SRHPM_UNSUPPORTED;
+    }
     for (int i = 0; i < 4; i++) {
         if (k->ne[i] != v->ne[i] || k->ne[i] < 1 || k->ne[i] > INT32_MAX) return SRHPM_ERR_INVALID;
     }
@@ -200,6 +202,16 @@ bool overlap(std::initializer_list<Bytes> out, std::initializer_list<Bytes> in) 
         }
     }
     return false;
+}
+
+// outputs that share bytes with each other or with an input
+bool clash(std::initializer_list<Bytes> out, std::initializer_list<Bytes> in) {
+    for (const Bytes * o = out.begin(); o != out.end(); o++) {
+        for (const Bytes * p = o + 1; p != out.end(); p++) {
+            if (overlap({ *o }, { *p })) return true;
+        }
+    }
+    return overlap(out, in);
 }
 
 // token rows of heads: f32 or f16 [D, ., .], 16-byte aligned, strides multiples of 16
@@ -297,6 +309,7 @@ int srhpm_blck_size(int type) {
         case SRHPM_TYPE_F32:
         case SRHPM_TYPE_F16:
         case SRHPM_TYPE_I32: return 1;
+        case SRHPM_TYPE_Q4_0:
         case SRHPM_TYPE_Q8_0: return 32;
         case SRHPM_TYPE_Q3_K:
         case SRHPM_TYPE_Q4_K:
@@ -313,6 +326,7 @@ size_t srhpm_type_size(int type) {
         case SRHPM_TYPE_F32: return 4;
         case SRHPM_TYPE_F16: return 2;
         case SRHPM_TYPE_I32: return 4;
+        case SRHPM_TYPE_Q4_0: return 18;
         case SRHPM_TYPE_Q8_0: return 34;
         case SRHPM_TYPE_Q3_K: return 110;
         case SRHPM_TYPE_Q4_K: return 144;
@@ -700,7 +714,7 @@ int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, i
     if (!ctx || !qkv || !pos || !slots || !q_out || !k_cache || !v_cache) return SRHPM_ERR_INVALID;
     if (n_head < 1 || n_head > 65536 || n_head_kv < 1 || !(theta_base > 0.0f)) return SRHPM_ERR_INVALID;
     PagedCache c;
-    int        st = check_paged(k_cache, v_cache, k_cache->type == SRHPM_TYPE_Q8_0 ? 2 : 16, &c);
+    int        st = check_paged(k_cache, v_cache, k_cache->type == SRHPM_TYPE_F16 ? 16 : 2, &c);
     if (st != SRHPM_OK) return st;
     if (c.Hkv != n_head_kv) return SRHPM_ERR_INVALID;
     if (qkv->type != SRHPM_TYPE_F32) return SRHPM_UNSUPPORTED;
@@ -719,7 +733,10 @@ int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, i
 
 // the shapes that size the work buffer
 static int check_fa_paged(const srhpm_tensor * q, const srhpm_tensor * k, const srhpm_tensor * v, PagedCache * c) {
-    int st = check_paged(k, v, 16, c);
+    if (!k) return SRHPM_ERR_INVALID;
+    // a q4_0 row of D values comes in 9 copies of D / 16 bytes
+    const size_t mult = k->type == SRHPM_TYPE_Q4_0 && k->ne[0] >= 64 && k->ne[0] <= 256 ? (size_t) k->ne[0] / 16 : 16;
+    int st = check_paged(k, v, mult, c);
     if (st != SRHPM_OK) return st;
     if (c->page % 16 || (c->type == SRHPM_TYPE_Q8_0 && c->D != 256)) return SRHPM_UNSUPPORTED;
     st = check_rows16(q, c->D);
@@ -735,8 +752,7 @@ int srhpm_flash_attn_paged_work_size(const srhpm_ctx * ctx, const srhpm_tensor *
     PagedCache c;
     const int  st = check_fa_paged(q, k_cache, k_cache, &c);
     if (st != SRHPM_OK) return st;
-    *size = fa_paged_work_size(ctx, (int) q->ne[1], (int) q->ne[2], c.Hkv, c.D, n_seqs,
-                               c.type == SRHPM_TYPE_Q8_0 && q->type == SRHPM_TYPE_F32);
+    *size = fa_paged_work_size(ctx, (int) q->ne[1], (int) q->ne[2], c.Hkv, c.D, n_seqs, c.type, q->type == SRHPM_TYPE_F32);
     return SRHPM_OK;
 }
 
@@ -824,6 +840,153 @@ int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int3
     v.out_n   = out_n;
     v.p_draft = p_draft;
     return verify_sample_run(ctx, v, wdata, wsize, (cudaStream_t) stream);
+}
+
+static PageTable table_of(const srhpm_tensor * t) {
+    return { (uint8_t *) t->data, (int64_t) t->nb[1], (int) t->ne[0], (int) t->ne[1] };
+}
+static Bytes bytes_of(const srhpm_tensor * t) { return { t->data, (size_t) (t->ne[1] - 1) * t->nb[1] + 4 * (size_t) t->ne[0] }; }
+
+int srhpm_page_fork(srhpm_ctx * ctx, const int32_t * parent, const int32_t * child, const int32_t * n_keep, int n_forks,
+                    int page_size, const srhpm_tensor * block_table, int32_t * page_refs, int n_pages,
+                    const int32_t * free_pages, int n_free, const int32_t * free_head, int32_t * src, int32_t * dst,
+                    int32_t * status, int32_t * n_taken, void * stream) {
+    if (!ctx || !parent || !child || !n_keep || !page_refs || !src || !dst || !status || !n_taken) return SRHPM_ERR_INVALID;
+    if (n_forks < 1 || page_size < 1 || n_pages < 1 || n_free < 0 || (n_free > 0 && !free_pages)) return SRHPM_ERR_INVALID;
+    const int st = check_table(block_table);
+    if (st != SRHPM_OK) return st;
+    if (n_forks > kPlanMaxSeqs) return SRHPM_UNSUPPORTED;
+    const size_t n = 4 * (size_t) n_forks, pages = 4 * (size_t) n_pages;
+    const Bytes  table = bytes_of(block_table);
+    if (clash({ { src, n }, { dst, n }, { status, n }, { n_taken, 4 }, { page_refs, pages }, table },
+              { { parent, n }, { child, n }, { n_keep, n }, { free_pages, 4 * (size_t) n_free }, { free_head, 4 } })) {
+        return SRHPM_ERR_INVALID;
+    }
+    return page_fork_run(ctx, table_of(block_table), parent, child, n_keep, n_forks, page_size, page_refs, n_pages, free_pages, n_free,
+                         free_head, src, dst, status, n_taken, (cudaStream_t) stream);
+}
+
+int srhpm_page_copy(srhpm_ctx * ctx, const srhpm_tensor * caches, int n_caches, const int32_t * src, const int32_t * dst, int n,
+                    const int32_t * n_moves, void * stream) {
+    if (!ctx || !caches || n_caches < 1 || n < 0 || (n > 0 && (!src || !dst))) return SRHPM_ERR_INVALID;
+    const srhpm_tensor & c    = caches[0];
+    const size_t         rowb = srhpm_row_size(c.type, c.ne[0]);
+    if (c.type != SRHPM_TYPE_F16 && c.type != SRHPM_TYPE_Q8_0 && c.type != SRHPM_TYPE_Q4_0) return SRHPM_UNSUPPORTED;
+    if (c.ne[0] < 1 || rowb == 0 || c.nb[0] != srhpm_type_size(c.type)) return SRHPM_ERR_INVALID;
+    for (int i = 1; i < 4; i++) {
+        if (c.ne[i] < 1 || c.ne[i] > INT32_MAX) return SRHPM_ERR_INVALID;
+        if (c.ne[i] > 1 && c.nb[i] < rowb) return SRHPM_ERR_INVALID;
+        if (c.nb[i] % 2) return SRHPM_ERR_ALIGN;
+    }
+    if (c.ne[1] * c.ne[2] > INT32_MAX) return SRHPM_UNSUPPORTED;
+    for (int k = 0; k < n_caches; k++) {
+        const srhpm_tensor & t = caches[k];
+        if (!t.data || t.type != c.type) return SRHPM_ERR_INVALID;
+        if (!aligned(t.data, 2)) return SRHPM_ERR_ALIGN;
+        for (int i = 0; i < 4; i++) {
+            if (t.ne[i] != c.ne[i] || (t.ne[i] > 1 && t.nb[i] != c.nb[i])) return SRHPM_ERR_INVALID;
+        }
+    }
+    if (n == 0) return SRHPM_OK;
+    return page_copy_run(ctx, caches, n_caches, src, dst, n, n_moves, (cudaStream_t) stream);
+}
+
+int srhpm_page_free(srhpm_ctx * ctx, const int32_t * rows, const int32_t * begin, const int32_t * end, int n,
+                    const srhpm_tensor * block_table, int32_t * page_refs, int n_pages, int32_t * free_pages, int n_free,
+                    const int32_t * free_head, int32_t * n_freed, void * stream) {
+    if (!ctx || !page_refs || !free_head || !n_freed || n < 0 || n_pages < 1 || n_free < 0) return SRHPM_ERR_INVALID;
+    if ((n > 0 && (!rows || !end)) || (n_free > 0 && !free_pages)) return SRHPM_ERR_INVALID;
+    const int st = check_table(block_table);
+    if (st != SRHPM_OK) return st;
+    if (n_pages > kMaxPages) return SRHPM_UNSUPPORTED;
+    const size_t per = 4 * (size_t) n, pages = 4 * (size_t) n_pages, list = 4 * (size_t) n_free;
+    const Bytes  table = bytes_of(block_table);
+    if (clash({ { n_freed, 4 }, { free_pages, list }, { page_refs, pages }, table },
+              { { rows, per }, { begin, per }, { end, per }, { free_head, 4 } })) {
+        return SRHPM_ERR_INVALID;
+    }
+    return page_free_run(ctx, table_of(block_table), rows, begin, end, n, page_refs, n_pages, free_pages, n_free, free_head, n_freed,
+                         (cudaStream_t) stream);
+}
+
+int srhpm_page_compact(srhpm_ctx * ctx, const srhpm_tensor * block_table, const int32_t * n_held, int32_t * page_refs, int n_pages,
+                       int32_t * free_pages, int32_t * src, int32_t * dst, int32_t * n_moves, int32_t * n_used, void * stream) {
+    if (!ctx || !n_held || !page_refs || !free_pages || !n_moves || !n_used || n_pages < 1) return SRHPM_ERR_INVALID;
+    if (n_pages > 1 && (!src || !dst)) return SRHPM_ERR_INVALID;
+    const int st = check_table(block_table);
+    if (st != SRHPM_OK) return st;
+    if (n_pages > kMaxPages) return SRHPM_UNSUPPORTED;
+    const size_t pages = 4 * (size_t) n_pages, moves = 4 * (size_t) (n_pages / 2), held = 4 * (size_t) block_table->ne[1];
+    const Bytes  table = bytes_of(block_table);
+    if (clash({ { page_refs, pages }, { free_pages, pages }, { src, moves }, { dst, moves }, { n_moves, 4 }, { n_used, 4 }, table },
+              { { n_held, held } })) {
+        return SRHPM_ERR_INVALID;
+    }
+    return page_compact_run(ctx, table_of(block_table), n_held, page_refs, n_pages, free_pages, src, dst, n_moves, n_used,
+                            (cudaStream_t) stream);
+}
+
+int srhpm_adjust_logits(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start, int n_seqs,
+                        const srhpm_tensor * history, const int32_t * n_history, const int32_t * last_n, const float * repeat,
+                        const float * frequency, const float * presence, const int32_t * bias_start, const int32_t * bias_ids,
+                        const float * bias, int n_bias, const srhpm_tensor * mask, const int32_t * mask_row,
+                        const srhpm_tensor * out, void * stream) {
+    if (!ctx || !ids || !q_start || n_seqs < 1 || n_seqs > (1 << 24) || n_bias < 0) return SRHPM_ERR_INVALID;
+    int st = check_logits(logits, 1);
+    if (st != SRHPM_OK) return st;
+    st = check_logits(out, 1);
+    if (st != SRHPM_OK) return st;
+    const int64_t V = logits->ne[0], T = logits->ne[1];
+    if (T > (1 << 24) || V > (1 << 29) || out->ne[0] != V || out->ne[1] != T) return SRHPM_ERR_INVALID;
+    if (history) {
+        st = check_table(history);
+        if (st != SRHPM_OK) return st;
+        if (history->ne[1] != n_seqs || !n_history || history->ne[0] > (1 << 30)) return SRHPM_ERR_INVALID;
+    }
+    if (n_bias > 0 && (!bias_start || !bias_ids || !bias)) return SRHPM_ERR_INVALID;
+    if (mask) {
+        st = check_table(mask);
+        if (st != SRHPM_OK) return st;
+        if (mask->ne[0] < (V + 31) / 32 || (!mask_row && mask->ne[1] < T)) return SRHPM_ERR_INVALID;
+    }
+    auto whole = [](const srhpm_tensor * t) { return Bytes{ t->data, (size_t) (t->ne[1] - 1) * t->nb[1] + 4 * (size_t) t->ne[0] }; };
+    const Bytes to = whole(out);
+    // out is the logits themselves or shares nothing with them
+    const bool same = out->data == logits->data && (T == 1 || out->nb[1] == logits->nb[1]);
+    if (!same && overlap({ to }, { whole(logits) })) return SRHPM_ERR_INVALID;
+    const size_t per = 4 * (size_t) n_seqs, rows = 4 * (size_t) T, nb = 4 * (size_t) n_bias;
+    if (overlap({ to }, { { ids, rows }, { q_start, per + 4 }, { n_history, per }, { last_n, per }, { repeat, per }, { frequency, per },
+                          { presence, per }, { n_bias ? bias_start : nullptr, per + 4 }, { bias_ids, nb }, { bias, nb }, { mask_row, rows } }) ||
+        (history && overlap({ to }, { whole(history) })) || (mask && overlap({ to }, { whole(mask) }))) {
+        return SRHPM_ERR_INVALID;
+    }
+    LogitView v;
+    v.logits     = (const uint8_t *) logits->data;
+    v.ldb        = (int64_t) logits->nb[1];
+    v.V          = (int) V;
+    v.T          = (int) T;
+    v.S          = n_seqs;
+    v.ids        = ids;
+    v.q_start    = q_start;
+    v.history    = history ? (const uint8_t *) history->data : nullptr;
+    v.ldh        = history ? (int64_t) history->nb[1] : 0;
+    v.cap        = history ? (int) history->ne[0] : 0;
+    v.n_history  = n_history;
+    v.last_n     = last_n;
+    v.repeat     = repeat;
+    v.frequency  = frequency;
+    v.presence   = presence;
+    v.bias_start = bias_start;
+    v.bias_ids   = bias_ids;
+    v.bias       = bias;
+    v.n_bias     = n_bias;
+    v.mask       = mask ? (const uint8_t *) mask->data : nullptr;
+    v.ldm        = mask ? (int64_t) mask->nb[1] : 0;
+    v.n_masks    = mask ? (int) mask->ne[1] : 0;
+    v.mask_row   = mask_row;
+    v.out        = (uint8_t *) out->data;
+    v.ldo        = (int64_t) out->nb[1];
+    return adjust_logits_run(ctx, v, (cudaStream_t) stream);
 }
 
 }  // extern "C"

@@ -44,6 +44,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "fa_paged.cuh"
 #include "fastdiv.cuh"
 #include "internal.h"
 #include "launch.cuh"
@@ -51,122 +52,17 @@
 #include "tc.cuh"
 
 namespace srhpm {
+using namespace fap;
 namespace {
 
-constexpr float kLog2e   = 1.4426950408889634f;
-constexpr float kLazy    = 8.0f;   // raise the running maximum only beyond 2^8
-constexpr float kShift   = 7.0f;   // p is kept times 2^7
 constexpr int   kBM      = 128;    // rows of a tile
 constexpr int   kSmWarps = 8;      // softmax warps
 constexpr int   kProd    = 3;      // producer warps (f16 cache)
 constexpr int   kConv    = 16;     // converter warps (q8_0 cache): K's two groups of four, then V's
 constexpr int   kFew     = 56;     // rows of a tile where sequences bring few (below)
-constexpr int   kMaxSeqs = 8192;
 constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s (a probe sleeps up to 4 us)
 constexpr int   kRawTok  = 32;     // tokens of a raw q8_0 slot
 constexpr int   kRawB    = kRawTok * 272;
-
-struct PArgs {
-    const uint8_t * q;
-    int64_t         qnb1, qnb2;
-    uint8_t *       dst;
-    int64_t         dnb1, dnb2;
-    int             wide;  // dst and its strides are multiples of 32 bytes
-    const uint8_t * table;
-    int64_t         tstride;
-    int             cols, page, n_pages, box;  // box: tokens of a TMA box (divides the page)
-    const int32_t * q_start;
-    const int32_t * kv_len;
-    int             S, T, H, Hkv, G, window;
-    FastDiv         byG, byPage;
-    float           qscale;      // scale * log2e, or scale / softcap
-    float           softcap_l2;  // softcap * log2e, 0 = none
-    const float *   sinks;
-    float *         part_acc;    // [2 n_cta][prow][D]
-    float2 *        part_ms;     // [2 n_cta][prow] (max in log2 units, sum * 2^kShift)
-    int4 *          desc;        // [n_cta][2]: parts of the item that a CTA opens and leaves unfinished, and its rows
-    int             prow;        // rows of a record
-    int32_t *       status;
-};
-
-// ---- work items --------------------------------------------------------------------------------------------------
-struct Span {
-    int kt0, nkv;  // first tile, tiles (0: nothing visible)
-    int lo, hi;    // visible tokens of any row
-    int units;     // max(nkv, 1)
-};
-
-// q_start, clamped into the row buffer
-__device__ __forceinline__ int row_at(const PArgs & a, int s) { return min(max(a.q_start[s], 0), a.T); }
-
-template <int BMN, int BN> __device__ __forceinline__ Span span_of(const PArgs & a, int n, int kv, int rt) {
-    const int     r0 = rt * BMN, r1 = min(n * a.G, r0 + BMN);  // T * G < 2^31 (checked)
-    const int     t0 = a.byG.div(r0), t1 = a.byG.div(r1 - 1);
-    const int     base = kv - n;
-    const int64_t cap  = min((int64_t) a.cols * a.page, (int64_t) INT32_MAX - BN);
-    Span          p;
-    p.hi = (int) max((int64_t) 0, min((int64_t) base + t1 + 1, cap));
-    p.lo = a.window > 0 ? (int) max((int64_t) 0, (int64_t) base + t0 - a.window + 1) : 0;
-    if (p.hi <= p.lo) {
-        p.kt0 = p.nkv = 0;
-        p.lo = p.hi = 0;
-    } else {
-        p.kt0 = p.lo / BN;
-        p.nkv = (p.hi + BN - 1) / BN - p.kt0;
-    }
-    p.units = max(p.nkv, 1);
-    return p;
-}
-template <int BMN> __device__ __forceinline__ int tiles_of(const PArgs & a, int n) { return (n * a.G + BMN - 1) / BMN; }
-
-// a CTA's walk over its part of the line; every role keeps its own
-struct Walk {
-    int     s, h, rt;   // item
-    int     off;        // first unit of the item in this CTA
-    int64_t rem;        // units left in this CTA
-    int     r0, n, kv;  // the sequence's first row, rows and cache length
-    Span    sp;
-    int     take;       // units of the item done here
-    int64_t part;       // units of this CTA in all
-    int     tile0, lap; // first tile in this CTA's order; the turn at which the order goes back to the item's first tile
-    __device__ __forceinline__ int tile(int i) const { return tile0 + i - (i >= lap ? sp.nkv : 0); }
-};
-
-template <int BMN> __device__ __forceinline__ void walk_load(const PArgs & a, Walk & w) {
-    w.r0 = row_at(a, w.s);
-    w.n  = row_at(a, w.s + 1) - w.r0;
-    w.kv = max(a.kv_len[w.s], 0);
-}
-template <int BMN, int BN> __device__ __forceinline__ void walk_item(const PArgs & a, Walk & w) {
-    w.sp   = span_of<BMN, BN>(a, w.n, w.kv, w.rt);
-    w.take = (int) min((int64_t) (w.sp.units - w.off), w.rem);
-    // A whole item's tiles may come in any order: a long one begins where CTAs that began together and took a tile per turn
-    // would be by now, so that those of one KV head read the same tiles at the same time and find them in L2 (2048 rows over
-    // 32768 tokens: 1.4 GB from memory instead of 5.2, 1.52 ms instead of 1.69). Short ones find theirs there anyhow (a mixed
-    // batch of up to 4000 tokens took 136 us turned and 133 not).
-    const bool turned = w.off == 0 && w.take == w.sp.nkv && w.sp.nkv >= 64;
-    const int  turn   = turned ? (int) ((uint64_t) (w.part - w.rem) % (uint32_t) w.sp.nkv) : 0;
-    w.tile0 = w.sp.kt0 + w.off + turn;
-    w.lap   = w.sp.nkv - w.off - turn;
-}
-// to the next item; false at the end of the part
-template <int BMN, int BN> __device__ __forceinline__ bool walk_next(const PArgs & a, Walk & w) {
-    w.rem -= w.take;
-    if (w.rem <= 0) return false;
-    w.off = 0;
-    if (++w.rt >= tiles_of<BMN>(a, w.n)) {
-        w.rt = 0;
-        if (++w.h >= a.Hkv) {
-            w.h = 0;
-            do {
-                if (++w.s >= a.S) return false;
-                walk_load<BMN>(a, w);
-            } while (w.n <= 0);
-        }
-    }
-    walk_item<BMN, BN>(a, w);
-    return true;
-}
 
 // ring order of the K and V tiles: the order in which the products take them
 // NT = 1: K0 K1 V0 K2 V1 ... V(n-1);  NT = 2: K0 V0 K1 V1 ...
@@ -409,94 +305,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     pdl_wait();
 
     // ---------------- plan: this CTA's part of the line of units ----------------
-    {
-        int * tot = reinterpret_cast<int *>(sm + Ly::ring);  // units per KV head of each sequence
-        int * big = tot + a.S;                               // sequences whose tiles a warp sums up
-        int * nbg = reinterpret_cast<int *>(sm + Ly::red);
-        if (tid == 0) *nbg = 0;
-        __syncthreads();
-        for (int s = tid; s < a.S; s += blockDim.x) {
-            const int r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = n > 0 ? tiles_of<BMN>(a, n) : 0;
-            int       u = 0;
-            if (nt <= 2) {
-                const int kv = nt ? max(a.kv_len[s], 0) : 0;
-                for (int rt = 0; rt < nt; rt++) u += span_of<BMN, BN>(a, n, kv, rt).units;
-            } else {
-                big[atomicAdd(nbg, 1)] = s;  // any order: each entry is worked out by itself
-            }
-            tot[s] = u;
-        }
-        __syncthreads();
-        for (int b = warp; b < *nbg; b += blockDim.x / 32) {
-            const int s = big[b], r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = max(a.kv_len[s], 0);
-            int       u = 0;
-            for (int rt = lane; rt < nt; rt += 32) u += span_of<BMN, BN>(a, n, kv, rt).units;
-            u = __reduce_add_sync(0xffffffffu, u);
-            if (lane == 0) tot[s] = u;
-        }
-        __syncthreads();
-        if (warp == 0) {
-            int64_t sum = 0;
-            for (int s = lane; s < a.S; s += 32) sum += tot[s];
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            // fewer units than CTAs: one each for the first W, so that an item's parts stand in neighbouring CTAs
-            const int64_t W = sum * a.Hkv, np = max((int64_t) 1, min((int64_t) gridDim.x, W)), c = min((int64_t) blockIdx.x, np);
-            const int64_t b0 = W * c / np, b1 = W * min(c + 1, np) / np;
-            if (lane == 0) {
-                range[0] = b0;
-                range[1] = b1;
-                range[2] = W;
-                range[3] = np;
-            }
-            if (b1 > b0) {
-                int64_t before = 0;
-                for (int s0 = 0; s0 < a.S; s0 += 32) {
-                    const int64_t v   = s0 + lane < a.S ? (int64_t) tot[s0 + lane] * a.Hkv : 0;
-                    int64_t       inc = v;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-                        if (lane >= o) inc += x;
-                    }
-                    const int64_t  end = before + inc, beg = end - v;
-                    const uint32_t hit = __ballot_sync(0xffffffffu, b0 >= beg && b0 < end);
-                    if (hit) {
-                        const int     src = __ffs(hit) - 1, s = s0 + src;
-                        const int64_t in  = b0 - __shfl_sync(0xffffffffu, beg, src);
-                        const int     per = tot[s];
-                        const int     h   = (int) (in / per);
-                        int           off = (int) (in - (int64_t) h * per);
-                        const int     r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = max(a.kv_len[s], 0);
-                        for (int t0 = 0; t0 < nt; t0 += 32) {
-                            const int u  = t0 + lane < nt ? span_of<BMN, BN>(a, n, kv, t0 + lane).units : 0;
-                            int       ic = u;
-#pragma unroll
-                            for (int o = 1; o < 32; o <<= 1) {
-                                const int x = __shfl_up_sync(0xffffffffu, ic, o);
-                                if (lane >= o) ic += x;
-                            }
-                            const uint32_t ht = __ballot_sync(0xffffffffu, off >= ic - u && off < ic);
-                            if (ht) {
-                                const int l = __ffs(ht) - 1;
-                                off -= __shfl_sync(0xffffffffu, ic - u, l);
-                                if (lane == 0) {
-                                    first[0] = s;
-                                    first[1] = h;
-                                    first[2] = t0 + l;
-                                    first[3] = off;
-                                }
-                                break;
-                            }
-                            off -= __shfl_sync(0xffffffffu, ic, 31);
-                        }
-                        break;
-                    }
-                    before = __shfl_sync(0xffffffffu, end, 31);
-                }
-            }
-        }
-    }
+    plan_part<BMN, BN>(a, reinterpret_cast<int *>(sm + Ly::ring), reinterpret_cast<int *>(sm + Ly::red), first, range);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -1468,8 +1277,9 @@ EncodeTiled encode_fn() {
 struct Tile {
     int nt, br;
 };
-Tile tile_of(int T, int S, int G, int D, bool q8f32) {
-    if (q8f32 || (int64_t) T * G <= (int64_t) S * kFew) return { 1, kFew };
+Tile tile_of(int T, int S, int G, int D, int kv_type, bool f32) {
+    if (kv_type == SRHPM_TYPE_Q4_0) return { 1, q4_few_rows(D) };
+    if ((kv_type == SRHPM_TYPE_Q8_0 && f32) || (int64_t) T * G <= (int64_t) S * kFew) return { 1, kFew };
     return { D <= 128 ? 2 : 1, 128 };
 }
 
@@ -1487,10 +1297,7 @@ int launch_paged(srhpm_ctx * ctx, const PArgs & a, const CUtensorMap & mk, const
     int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms), dim3(Ly::threads), Ly::alloc, stream, mk, mv, a));
     ctx->launches.fetch_add(1);
     if (st != SRHPM_OK) return st;
-    st = cuda_status(launch_k_pdl(fa_paged_merge_kernel<D, PREC>,
-                                  dim3(ctx->num_sms, BR == kFew ? std::min(32, a.prow) : 16), dim3(256), 0, stream, a));
-    ctx->launches.fetch_add(1);
-    return st;
+    return merge_launch(ctx, a, D, PREC, BR == kFew ? std::min(32, a.prow) : 16, stream);
 }
 
 template <int D, bool PREC, bool Q8>
@@ -1502,12 +1309,19 @@ int launch_tile(srhpm_ctx * ctx, Tile t, const PArgs & a, const CUtensorMap & mk
 
 int record_rows(int T, int G, Tile t) { return (int) std::min<int64_t>((int64_t) t.br * t.nt, (int64_t) T * G); }
 
-size_t align16(size_t n) { return (n + 15) / 16 * 16; }
-
 }  // namespace
 
-size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S, bool q8f32) {
-    const size_t recs = (size_t) 2 * ctx->num_sms * record_rows(T, H / Hkv, tile_of(T, S, H / Hkv, D, q8f32));
+int fap::merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int rows_y, cudaStream_t stream) {
+    auto kern = D == 64 ? (f32 ? fa_paged_merge_kernel<64, true> : fa_paged_merge_kernel<64, false>)
+                : D == 128 ? (f32 ? fa_paged_merge_kernel<128, true> : fa_paged_merge_kernel<128, false>)
+                           : (f32 ? fa_paged_merge_kernel<256, true> : fa_paged_merge_kernel<256, false>);
+    const int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms, rows_y), dim3(256), 0, stream, a));
+    ctx->launches.fetch_add(1);
+    return st;
+}
+
+size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S, int kv_type, bool f32) {
+    const size_t recs = (size_t) 2 * ctx->num_sms * record_rows(T, H / Hkv, tile_of(T, S, H / Hkv, D, kv_type, f32));
     return recs * D * sizeof(float) + align16(recs * sizeof(float2)) + 2 * (size_t) ctx->num_sms * sizeof(int4) + 32;
 }
 
@@ -1516,9 +1330,10 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     if (v.S > kMaxSeqs || (int64_t) v.T * G + 2 * kBM > INT32_MAX) return SRHPM_UNSUPPORTED;
     // a sequence's units per KV head are counted in 32 bits: tiles of 56 rows or more times tiles of 64 tokens or more
     const int64_t seen = std::min<int64_t>((int64_t) v.cols * v.c.page, INT32_MAX);
-    if (((int64_t) v.T * G / kFew + 1) * (seen / 64 + 1) > INT32_MAX) return SRHPM_UNSUPPORTED;
-    if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.c.Hkv, D, v.S, v.f32 && v.c.type == SRHPM_TYPE_Q8_0)) return SRHPM_ERR_WORKSPACE;
-    const Tile tl = tile_of(v.T, v.S, G, D, v.f32 && v.c.type == SRHPM_TYPE_Q8_0);
+    if (v.c.type != SRHPM_TYPE_Q4_0 && ((int64_t) v.T * G / kFew + 1) * (seen / 64 + 1) > INT32_MAX) return SRHPM_UNSUPPORTED;
+    if (v.c.type == SRHPM_TYPE_Q4_0 && ((int64_t) v.T * G / 8 + 1) * (seen / 128 + 1) > INT32_MAX) return SRHPM_UNSUPPORTED;
+    if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.c.Hkv, D, v.S, v.c.type, v.f32)) return SRHPM_ERR_WORKSPACE;
+    const Tile tl = tile_of(v.T, v.S, G, D, v.c.type, v.f32);
     PArgs      a;
     a.q       = v.q;
     a.qnb1    = v.qnb1;
@@ -1553,6 +1368,7 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     a.desc     = reinterpret_cast<int4 *>(wb + recs * D * sizeof(float) + align16(recs * sizeof(float2)));
     a.status   = ctx->d_status;
 
+    if (v.c.type == SRHPM_TYPE_Q4_0) return q4_few_run(ctx, a, v.c, v.f32, stream);
     const bool q8 = v.c.type == SRHPM_TYPE_Q8_0;
     a.box = q8 ? kRawTok : 64;
     while (a.page % a.box) a.box >>= 1;  // the page is a multiple of 16

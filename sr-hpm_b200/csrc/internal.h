@@ -160,6 +160,52 @@ int rope_kv_paged_run(srhpm_ctx * ctx, const uint8_t * qkv, int64_t ldb, int n, 
                       const int32_t * pos, const int64_t * slots, float theta_base, const srhpm_tensor * q_out,
                       const PagedCache & c, cudaStream_t stream);
 
+// page_share.cu: forks, copies, frees and compaction of pages (sets of pages at most kMaxPages: bits in shared memory)
+constexpr int kMaxPages = 1 << 22;
+struct PageTable {
+    uint8_t * data;
+    int64_t   stride;
+    int       cols, rows;
+};
+int page_fork_run(srhpm_ctx * ctx, const PageTable & t, const int32_t * parent, const int32_t * child, const int32_t * keep, int n,
+                  int page, int32_t * refs, int n_pages, const int32_t * free_pages, int n_free, const int32_t * free_head,
+                  int32_t * src, int32_t * dst, int32_t * status, int32_t * n_taken, cudaStream_t stream);
+int page_free_run(srhpm_ctx * ctx, const PageTable & t, const int32_t * rows, const int32_t * begin, const int32_t * end, int n,
+                  int32_t * refs, int n_pages, int32_t * free_pages, int n_free, const int32_t * free_head, int32_t * n_freed,
+                  cudaStream_t stream);
+int page_compact_run(srhpm_ctx * ctx, const PageTable & t, const int32_t * held, int32_t * refs, int n_pages, int32_t * free_pages,
+                     int32_t * src, int32_t * dst, int32_t * n_moves, int32_t * n_used, cudaStream_t stream);
+int page_copy_run(srhpm_ctx * ctx, const srhpm_tensor * caches, int n_caches, const int32_t * src, const int32_t * dst, int n,
+                  const int32_t * n_moves, cudaStream_t stream);
+
+// logits.cu: biases, penalties and masks
+struct LogitView {
+    const uint8_t * logits;
+    int64_t         ldb;
+    int             V, T, S;
+    const int32_t * ids;
+    const int32_t * q_start;
+    const uint8_t * history;  // i32 [S][cap] or null
+    int64_t         ldh;
+    int             cap;
+    const int32_t * n_history;
+    const int32_t * last_n;  // or null (all)
+    const float *   repeat;
+    const float *   frequency;
+    const float *   presence;  // each or null
+    const int32_t * bias_start;
+    const int32_t * bias_ids;
+    const float *   bias;
+    int             n_bias;  // 0: none
+    const uint8_t * mask;    // or null
+    int64_t         ldm;
+    int             n_masks;
+    const int32_t * mask_row;  // or null (row r has mask r)
+    uint8_t *       out;
+    int64_t         ldo;
+};
+int adjust_logits_run(srhpm_ctx * ctx, const LogitView & v, cudaStream_t stream);
+
 // fa_paged.cu: attention of the new tokens of a batch over the paged cache
 struct FaPagedView {
     const uint8_t * q;
@@ -178,7 +224,7 @@ struct FaPagedView {
     uint8_t *       dst;
     int64_t         dnb1, dnb2;  // head, token
 };
-size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S, bool q8f32);
+size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S, int kv_type, bool f32);
 int    fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t wsize, cudaStream_t stream);
 
 // verify_sample.cu: acceptance of drafted tokens by sampling

@@ -245,7 +245,69 @@ __device__ __forceinline__ void put4_q8(uint8_t * dst, int j, float4 v, int mode
     w[1]         = (uint16_t) ((q[2] & 0xff) | (q[3] & 0xff) << 8);
 }
 
-template <bool QF16, bool Q8>
+// what the 8 lanes of a q4_0 block need: -1/8 of its value of largest size (the first of equals) and the reciprocal
+struct Step4 {
+    float d, id;
+};
+__device__ __forceinline__ Step4 step_q4(int j, float4 v, uint32_t mask) {
+    const float x[4] = { v.x, v.y, v.z, v.w };
+    float       amax = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
+    int at = 64;  // 2 * place + sign
+#pragma unroll
+    for (int e = 3; e >= 0; e--) {
+        if (fabsf(x[e]) == amax) at = 2 * ((j & 31) + e) + (x[e] < 0.0f);
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(mask, at, o));
+    const float d = ((at & 1) ? amax : -amax) * 0.125f;
+    return { d, d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f };
+}
+__device__ __forceinline__ float level_q4(float x, float id) { return __fadd_rn(__fmul_rn(x, id), 8.5f); }
+// a value stands so near to the border of two numbers that the rounding of its rotation may decide
+__device__ __forceinline__ bool near_q4(float4 v, float id) {
+    const float x[4] = { v.x, v.y, v.z, v.w };
+    bool        r = false;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float y = level_q4(x[e], id);
+        r |= fabsf(y - rintf(y)) < 0x1p-15f;
+    }
+    return r;
+}
+// 4 of the 32 values of a q4_0 block: byte j holds number j in its low and number j + 16 in its high half
+__device__ __forceinline__ void put4_q4(uint8_t * dst, int j, float4 v, Step4 s, uint32_t mask) {
+    const float x[4] = { v.x, v.y, v.z, v.w };
+    uint32_t    q = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) q |= (uint32_t) min(max(__float2int_rz(level_q4(x[e], s.id)), 0), 15) << (8 * e);
+    const uint32_t up = __shfl_xor_sync(mask, q, 4);
+    uint8_t *      b  = dst + (j >> 5) * 18;
+    if ((j & 31) == 0) *reinterpret_cast<__half *>(b) = __float2half_rn(s.d);
+    if ((j & 16) == 0) {
+        const uint32_t w = q | up << 4;
+        uint16_t *     p = reinterpret_cast<uint16_t *>(b + 2 + (j & 15));
+        p[0]             = (uint16_t) w;
+        p[1]             = (uint16_t) (w >> 16);
+    }
+}
+
+// 4 pairs turned in 64 bits
+__device__ __noinline__ void turn64(float4 & l, float4 & h, double pos, const double * freq) {
+    float * x = reinterpret_cast<float *>(&l);
+    float * y = reinterpret_cast<float *>(&h);
+    for (int e = 0; e < 4; e++) {
+        double turns = pos * freq[e], s, c;
+        turns -= rint(turns);
+        sincospi(2.0 * turns, &s, &c);
+        const double a = x[e], b = y[e];
+        x[e] = (float) (a * c - b * s);
+        y[e] = (float) (a * s + b * c);
+    }
+}
+
+template <bool QF16, int KV>
 __global__ void __launch_bounds__(kStoreThreads) rope_kv_paged_kernel(const __grid_constant__ StoreArgs a) {
     __shared__ __align__(16) float cs[2][kMaxHalf], sn[2][kMaxHalf];
     constexpr int NU = 3;  // units of a thread in flight: 48 heads of 128 or 32 of 256 in one turn
@@ -293,6 +355,7 @@ __global__ void __launch_bounds__(kStoreThreads) rope_kv_paged_kernel(const __gr
                 const int u = u0 + k * kStoreThreads;
                 if (u >= total) break;
                 const int hh = a.by_units.div(u), j = (u - hh * units) * 4;
+                [[maybe_unused]] const float4 l0 = lo[k], h0 = hi[k];
                 if (hh < a.H + a.Hkv) {
                     const float4 c = *reinterpret_cast<const float4 *>(cs[par] + j), s = *reinterpret_cast<const float4 *>(sn[par] + j);
                     const float4 l = lo[k], h = hi[k];
@@ -307,8 +370,21 @@ __global__ void __launch_bounds__(kStoreThreads) rope_kv_paged_kernel(const __gr
                     const bool isk = hh < a.H + a.Hkv;
                     const int  g   = hh - a.H - (isk ? 0 : a.Hkv);
                     uint8_t *  d   = isk ? kd + (int64_t) g * a.knb2 : vd + (int64_t) g * a.vnb2;
-                    if constexpr (Q8) {
-                        const uint32_t oct = 0xffu << (threadIdx.x & 24);
+                    [[maybe_unused]] const uint32_t oct = 0xffu << (threadIdx.x & 24);
+                    if constexpr (KV == SRHPM_TYPE_Q4_0) {
+                        Step4 sl = step_q4(j, lo[k], oct), sh = step_q4(half + j, hi[k], oct);
+                        // a number hangs on the 32-bit rotation only where a value is next to a border: there the whole
+                        // block's are taken in 64 bits (one block in 500)
+                        if (isk && (__ballot_sync(oct, near_q4(lo[k], sl.id) || near_q4(hi[k], sh.id)) & oct)) {
+                            lo[k] = l0;
+                            hi[k] = h0;
+                            turn64(lo[k], hi[k], (double) a.pos[t], a.freq + j);
+                            sl = step_q4(j, lo[k], oct);
+                            sh = step_q4(half + j, hi[k], oct);
+                        }
+                        put4_q4(d, j, lo[k], sl, oct);
+                        put4_q4(d, half + j, hi[k], sh, oct);
+                    } else if constexpr (KV == SRHPM_TYPE_Q8_0) {
                         put4_q8(d, j, lo[k], a.q8mode, oct);
                         put4_q8(d, half + j, hi[k], a.q8mode, oct);
                     } else {
@@ -398,11 +474,11 @@ int rope_kv_paged_run(srhpm_ctx * ctx, const uint8_t * qkv, int64_t ldb, int n, 
         std::copy(ctx->rope_freq, ctx->rope_freq + D / 2, a.freq);
     }
     const int         grid = std::min(n, 8 * ctx->num_sms);
-    const bool        qf = q_out->type == SRHPM_TYPE_F16, q8 = c.type == SRHPM_TYPE_Q8_0;
-    const cudaError_t e = qf ? (q8 ? launch_k_pdl(rope_kv_paged_kernel<true, true>, dim3(grid), dim3(kStoreThreads), 0, stream, a)
-                                   : launch_k_pdl(rope_kv_paged_kernel<true, false>, dim3(grid), dim3(kStoreThreads), 0, stream, a))
-                             : (q8 ? launch_k_pdl(rope_kv_paged_kernel<false, true>, dim3(grid), dim3(kStoreThreads), 0, stream, a)
-                                   : launch_k_pdl(rope_kv_paged_kernel<false, false>, dim3(grid), dim3(kStoreThreads), 0, stream, a));
+    const bool qf = q_out->type == SRHPM_TYPE_F16;
+    auto       kern = c.type == SRHPM_TYPE_Q4_0   ? (qf ? rope_kv_paged_kernel<true, SRHPM_TYPE_Q4_0> : rope_kv_paged_kernel<false, SRHPM_TYPE_Q4_0>)
+                      : c.type == SRHPM_TYPE_Q8_0 ? (qf ? rope_kv_paged_kernel<true, SRHPM_TYPE_Q8_0> : rope_kv_paged_kernel<false, SRHPM_TYPE_Q8_0>)
+                                                  : (qf ? rope_kv_paged_kernel<true, SRHPM_TYPE_F16> : rope_kv_paged_kernel<false, SRHPM_TYPE_F16>);
+    const cudaError_t e = launch_k_pdl(kern, dim3(grid), dim3(kStoreThreads), 0, stream, a);
     ctx->launches.fetch_add(1);
     return cuda_status(e);
 }

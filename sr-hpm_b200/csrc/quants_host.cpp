@@ -329,7 +329,7 @@ extern "C" size_t srhpm_quantize_chunk(int type, const float * src, void * dst, 
     (void) imatrix;  // uniform importance (the verify-GEMM sweep quantizes IQ4_XS with a uniform matrix)
     const int    qk = srhpm_blck_size(type);
     const size_t bs = srhpm_type_size(type);
-    if (qk <= 0 || n_per_row % qk || start % n_per_row || nrows < 0) {
+    if (qk <= 0 || type == SRHPM_TYPE_Q4_0 || n_per_row % qk || start % n_per_row || nrows < 0) {
         return 0;
     }
     const int64_t nblk  = nrows * (n_per_row / qk);

@@ -12,8 +12,8 @@ LIB_PATH = os.path.join(HERE, "libsrhpm_b200.so")
 HEADER_PATH = os.path.abspath(os.path.join(HERE, "..", "..", "include", "srhpm_b200.h"))
 
 # ggml_type numbering
-F32, F16, Q8_0, Q3_K, Q4_K, Q5_K, Q6_K, Q8_K, IQ4_XS, I32 = 0, 1, 8, 11, 12, 13, 14, 15, 23, 26
-TYPE_NAMES = {F32: "f32", F16: "f16", Q8_0: "q8_0", Q3_K: "q3_K", Q4_K: "q4_K", Q5_K: "q5_K", Q6_K: "q6_K",
+F32, F16, Q4_0, Q8_0, Q3_K, Q4_K, Q5_K, Q6_K, Q8_K, IQ4_XS, I32 = 0, 1, 2, 8, 11, 12, 13, 14, 15, 23, 26
+TYPE_NAMES = {F32: "f32", F16: "f16", Q4_0: "q4_0", Q8_0: "q8_0", Q3_K: "q3_K", Q4_K: "q4_K", Q5_K: "q5_K", Q6_K: "q6_K",
               Q8_K: "q8_K", IQ4_XS: "iq4_xs", I32: "i32"}
 TYPE_BY_NAME = {v.lower(): k for k, v in TYPE_NAMES.items()}
 
@@ -100,6 +100,13 @@ _SIGNATURES = {
     "srhpm_verify_sample_work_size": (ctypes.c_int, [_P, _P, ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
     "srhpm_verify_sample": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, _P,
                                            ctypes.c_size_t, _P]),
+    "srhpm_page_fork": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, ctypes.c_int, _P, _P, ctypes.c_int, _P, ctypes.c_int, _P,
+                                       _P, _P, _P, _P, _P]),
+    "srhpm_page_copy": (ctypes.c_int, [_P, _P, ctypes.c_int, _P, _P, ctypes.c_int, _P, _P]),
+    "srhpm_page_free": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, _P, _P, ctypes.c_int, _P, ctypes.c_int, _P, _P, _P]),
+    "srhpm_page_compact": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, _P, _P, _P, _P, _P, _P]),
+    "srhpm_adjust_logits": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, _P, _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_int, _P,
+                                           _P, _P, _P]),
     "srhpm_quantize_chunk": (ctypes.c_size_t, [ctypes.c_int, _P, _P, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                                 _P]),
 }

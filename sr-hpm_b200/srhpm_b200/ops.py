@@ -10,9 +10,14 @@
                                    patch/srhpm.patch:779-823, with devices as the chunks)
     Context.sample_and_accept_n()  greedy longest-prefix acceptance (reference: common_sampler_sample_and_accept_n,
                                    patch/srhpm.patch:1-37)
-    Context.page_plan / rope_kv_paged / flash_attn_paged / verify_sample
-                                   a batch of sequences over a paged KV cache: the step's tables and slots, the store
-                                   into pages, attention over them, acceptance by sampling (no reference counterpart)
+    Context.page_plan / rope_kv_paged / flash_attn_paged / adjust_logits / verify_sample
+                                   a batch of sequences over a paged KV cache (f16, q8_0 or q4_0): the step's tables and
+                                   slots, the store into pages, attention over them, penalties, biases and token masks
+                                   on the logits, acceptance by sampling (no reference counterpart)
+    Context.page_fork / page_copy / page_free / page_compact
+                                   pages between steps: sequences that go on from others', whole-page copies in all
+                                   layers, finished sequences' pages given back, pages in use moved together (no
+                                   reference counterpart)
 
 Tensors are torch tensors in device memory; torch only provides allocation and streams. Every compute call goes to
 libsrhpm_b200.so through its C ABI; a missing library raises.
@@ -56,6 +61,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 PagePlan = collections.namedtuple("PagePlan", "q_start kv_len pos slots status n_taken")
+PageFork = collections.namedtuple("PageFork", "src dst status n_taken")
+PageMoves = collections.namedtuple("PageMoves", "src dst n_moves n_used")
 
 # The calls of a serving step are short on the GPU, so their host side is kept short too: a view is the bytes of an
 # srhpm_tensor (type, ne[4], nb[4], data), packed in one go.
@@ -87,13 +94,16 @@ def _head_rows(x, heads_first):
     return _pack(t, D, T, H, 1, e, a, b, a * T, x.data_ptr())
 
 
+_BLOCK = {L.Q8_0: (34, 32), L.Q4_0: (18, 32)}  # bytes and values of a block
+
+
 def _paged(c, kv_type):
     """View of a paged cache uint8 [pages, page_size, Hkv, row bytes]: ne = [D, page_size, Hkv, pages]."""
     if c.dtype is not torch.uint8 or c.dim() != 4 or c.stride(3) != 1:
         raise ValueError("a paged cache is uint8 [pages, page_size, Hkv, row bytes] with contiguous rows")
     n, P, Hkv, rowb = c.shape
     n3, n1, n2, _ = c.stride()
-    size, blk = (34, 32) if kv_type == L.Q8_0 else (2, 1)
+    size, blk = _BLOCK.get(kv_type, (2, 1))
     if rowb % size:
         raise ValueError("row bytes do not hold whole blocks of the cache type")
     return _pack(kv_type, rowb // size * blk, P, Hkv, n, size, n1, n2, n3, c.data_ptr())
@@ -573,6 +583,101 @@ class Context:
                    _rows_2d(block_table, torch.int32, L.I32, "block_table"), _ints(q_start, torch.int32, S + 1, "q_start"),
                    _ints(kv_len, torch.int32, S, "kv_len"), sv, scale, softcap, window, _head_rows(out, True),
                    work.data_ptr(), work.numel())
+        return out
+
+    def page_fork(self, parent, child, n_keep, block_table, page_refs, free_pages, page_size, free_head=None, out=None,
+                  stream=None):
+        """New sequences that begin with the first n_keep[i] tokens of others (srhpm_page_fork): table row child[i] gets
+        the pages of row parent[i], whole ones shared (counted in page_refs int32 [pages]: holders beyond the first), a
+        partly filled one replaced by a page from free_pages (as in page_plan). parent, child, n_keep int32 [n].
+        Returns a PageFork: src, dst int32 [n] (the copies still to be made with page_copy; -1: none), status int32 [n],
+        n_taken int32 [1] (`out`: one to write into)."""
+        n, i32 = parent.numel(), torch.int32
+        self._on_device(parent, child, n_keep, block_table, page_refs, free_pages, free_head)
+        if out is None:
+            out = PageFork(*self._new(3 * n + 1, i32, stream).split_with_sizes((n, n, n, 1)))
+        else:
+            self._on_device(*out)
+        self._call(self.lib.srhpm_page_fork, "srhpm_page_fork", stream, _ints(parent, i32, n, "parent"),
+                   _ints(child, i32, n, "child"), _ints(n_keep, i32, n, "n_keep"), n, page_size,
+                   _rows_2d(block_table, i32, L.I32, "block_table"), _ints(page_refs, i32, 1, "page_refs"),
+                   page_refs.numel(), _ints(free_pages, i32, 0, "free_pages"), free_pages.numel(),
+                   None if free_head is None else _ints(free_head, i32, 1, "free_head"), _ints(out.src, i32, n, "src"),
+                   _ints(out.dst, i32, n, "dst"), _ints(out.status, i32, n, "status"),
+                   _ints(out.n_taken, i32, 1, "n_taken"))
+        return out
+
+    def page_copy(self, caches, kv_type, src, dst, n_moves=None, stream=None):
+        """Pages src[i] copied to dst[i] (int32 [n]; no page: nothing) in every pool of `caches`, a list of uint8 [pages,
+        page_size, Hkv, row bytes] of one shape and layout, in one launch (srhpm_page_copy). n_moves int32 [1]: only that many."""
+        self._on_device(src, dst, n_moves, *caches)
+        n = src.numel()
+        self._call(self.lib.srhpm_page_copy, "srhpm_page_copy", stream, b"".join([_paged(c, kv_type) for c in caches]),
+                   len(caches), _ints(src, torch.int32, n, "src"), _ints(dst, torch.int32, n, "dst"), n,
+                   None if n_moves is None else _ints(n_moves, torch.int32, 1, "n_moves"))
+
+    def page_free(self, rows, begin, end, block_table, page_refs, free_pages, free_head, out=None, stream=None):
+        """Entries begin[i] .. end[i] - 1 of table rows rows[i] given up (int32 [n]; begin None: 0): they become -1, and pages that no
+        sequence holds any more go onto the free list in front of free_head, in the order of their numbers
+        (srhpm_page_free). Returns n_freed int32 [1] (`out`: one to write into): the next head is free_head - n_freed."""
+        n, i32 = rows.numel(), torch.int32
+        self._on_device(rows, begin, end, block_table, page_refs, free_pages, free_head, out)
+        if out is None:
+            out = self._new(1, i32, stream)
+        self._call(self.lib.srhpm_page_free, "srhpm_page_free", stream, _ints(rows, i32, n, "rows"),
+                   None if begin is None else _ints(begin, i32, n, "begin"), _ints(end, i32, n, "end"), n,
+                   _rows_2d(block_table, i32, L.I32, "block_table"), _ints(page_refs, i32, 1, "page_refs"),
+                   page_refs.numel(), _ints(free_pages, i32, 0, "free_pages"), free_pages.numel(),
+                   _ints(free_head, i32, 1, "free_head"), _ints(out, i32, 1, "n_freed"))
+        return out
+
+    def page_compact(self, block_table, n_held, page_refs, free_pages, out=None, stream=None):
+        """The pages that the first n_held[s] entries of the table's rows name get the lowest numbers (srhpm_page_compact):
+        table, page_refs int32 [pages] and free_pages int32 [pages] are rewritten, and page_copy has still to move the bytes. Returns a
+        PageMoves: src, dst int32 [pages // 2], n_moves, n_used int32 [1]; the free list's head is n_used from here on
+        (`out`: (src, dst) to write into; entries behind n_moves stay as they are)."""
+        n, i32 = page_refs.numel(), torch.int32
+        self._on_device(block_table, n_held, page_refs, free_pages)
+        if out is None:
+            src, dst, count = self._new(2 * (n // 2) + 2, i32, stream).split_with_sizes((n // 2, n // 2, 2))
+        else:
+            self._on_device(*out)
+            (src, dst), count = out, self._new(2, i32, stream)
+        moves = PageMoves(src, dst, count[:1], count[1:])
+        self._call(self.lib.srhpm_page_compact, "srhpm_page_compact", stream,
+                   _rows_2d(block_table, i32, L.I32, "block_table"), _ints(n_held, i32, block_table.shape[0], "n_held"),
+                   _ints(page_refs, i32, n, "page_refs"), n, _ints(free_pages, i32, n, "free_pages"),
+                   _ints(src, i32, n // 2, "src"), _ints(dst, i32, n // 2, "dst"), count.data_ptr(), count.data_ptr() + 4)
+        return moves
+
+    def adjust_logits(self, logits, ids, q_start, history=None, n_history=None, last_n=None, repeat=None, frequency=None,
+                      presence=None, bias=None, mask=None, mask_row=None, out=None, stream=None):
+        """Rules on the logits f32 [T, V] of a step's rows before verify_sample (srhpm_adjust_logits): biases of tokens (bias:
+        (starts int32 [S + 1], tokens int32, values f32)), penalties for the tokens in each row's window, the last
+        last_n[s] (int32 [S]; negative or None: all) of history int32 [S, capacity] (n_history int32 [S] of them) and the sequence's rows up to this one in ids int32 [T]: repeat,
+        frequency, presence f32 [S] or None; and masks int32 [n, >= ceil(V / 32)] with a bit per allowed token, row r's
+        being mask_row[r] (int32 [T]; negative: none; None: r). Returns out (`out`: logits itself, or a tensor that
+        shares nothing with them; None: a new one). Padding rows stay as they are."""
+        T, S, i32, f32 = logits.shape[0], q_start.numel() - 1, torch.int32, torch.float32
+        if out is None:
+            out = self._new(logits.shape, f32, stream)
+        if mask_row is not None and mask is None:
+            raise ValueError("mask_row without a mask")
+        starts, tokens, values = (None, None, None) if bias is None else bias
+        self._on_device(logits, ids, q_start, history, n_history, last_n, repeat, frequency, presence, starts, tokens, values,
+                        mask, mask_row, out)
+
+        def vec(t, dtype, n, what):
+            return None if t is None else _ints(t, dtype, n, what)
+
+        nb = 0 if bias is None else tokens.numel()
+        self._call(self.lib.srhpm_adjust_logits, "srhpm_adjust_logits", stream, _rows_2d(logits, f32, L.F32, "logits"),
+                   _ints(ids, i32, T, "ids"), _ints(q_start, i32, S + 1, "q_start"), S,
+                   None if history is None else _rows_2d(history, i32, L.I32, "history"), vec(n_history, i32, S, "n_history"),
+                   vec(last_n, i32, S, "last_n"), vec(repeat, f32, S, "repeat"), vec(frequency, f32, S, "frequency"),
+                   vec(presence, f32, S, "presence"), vec(starts, i32, S + 1, "bias starts"), vec(tokens, i32, nb, "bias tokens"),
+                   vec(values, f32, nb, "bias values"), nb, None if mask is None else _rows_2d(mask, i32, L.I32, "mask"),
+                   vec(mask_row, i32, T, "mask_row"), _rows_2d(out, f32, L.F32, "out"))
         return out
 
     def verify_sample(self, logits, ids, q_start, u_accept, u_sample, draft_probs=None, temperature=None, out=None,
