@@ -1278,7 +1278,7 @@ struct Tile {
     int nt, br;
 };
 Tile tile_of(int T, int S, int G, int D, int kv_type, bool f32) {
-    if (kv_type == SRHPM_TYPE_Q4_0) return { 1, q4_few_rows(D) };
+    if (kv_type == SRHPM_TYPE_Q4_0) return { 1, q4_rows(T, S, G, f32) };
     if ((kv_type == SRHPM_TYPE_Q8_0 && f32) || (int64_t) T * G <= (int64_t) S * kFew) return { 1, kFew };
     return { D <= 128 ? 2 : 1, 128 };
 }
@@ -1310,6 +1310,16 @@ int launch_tile(srhpm_ctx * ctx, Tile t, const PArgs & a, const CUtensorMap & mk
 int record_rows(int T, int G, Tile t) { return (int) std::min<int64_t>((int64_t) t.br * t.nt, (int64_t) T * G); }
 
 }  // namespace
+
+bool fap::encode_rows(void * map, const void * p, uint64_t width, int tokens, int64_t pages, int64_t nb1, int64_t nb3, int box, int tokens_box) {
+    EncodeTiled enc = encode_fn();
+    if (!enc) return false;
+    const cuuint64_t dims[3] = { width, (cuuint64_t) tokens, (cuuint64_t) pages }, st[2] = { (cuuint64_t) nb1, (cuuint64_t) nb3 };
+    const cuuint32_t bx[3] = { (cuuint32_t) box, (cuuint32_t) tokens_box, 1 }, es[3] = { 1, 1, 1 };
+    return enc(static_cast<CUtensorMap *>(map), CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(p), dims, st, bx, es,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 int fap::merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int rows_y, cudaStream_t stream) {
     auto kern = D == 64 ? (f32 ? fa_paged_merge_kernel<64, true> : fa_paged_merge_kernel<64, false>)
@@ -1368,7 +1378,7 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     a.desc     = reinterpret_cast<int4 *>(wb + recs * D * sizeof(float) + align16(recs * sizeof(float2)));
     a.status   = ctx->d_status;
 
-    if (v.c.type == SRHPM_TYPE_Q4_0) return q4_few_run(ctx, a, v.c, v.f32, stream);
+    if (v.c.type == SRHPM_TYPE_Q4_0) return q4_run(ctx, a, v.c, tl.br, v.f32, stream);
     const bool q8 = v.c.type == SRHPM_TYPE_Q8_0;
     a.box = q8 ? kRawTok : 64;
     while (a.page % a.box) a.box >>= 1;  // the page is a multiple of 16

@@ -210,9 +210,13 @@ __device__ __forceinline__ void plan_part(const PArgs & a, int * tot, int * nbg,
     }
 }
 
-// fa_paged_q4.cu: few rows per KV head over q4_0 pages; rows of its tile
-int q4_few_rows(int D);
-int q4_few_run(srhpm_ctx * ctx, const PArgs & a, const PagedCache & c, bool f32, cudaStream_t stream);
+// over q4_0 pages: rows of a tile (fa_paged_q4.cu)
+int q4_rows(int T, int S, int G, bool f32);
+int q4_few_run(srhpm_ctx * ctx, const PArgs & a, const void * maps, const PagedCache & c, bool f32, cudaStream_t stream);  // fa_paged_q4_few.cu
+int q4_run(srhpm_ctx * ctx, PArgs & a, const PagedCache & c, int rows, bool f32, cudaStream_t stream);
+
+// tensor map of bytes [pages][tokens][width], boxes of `tokens_box` rows of `box` bytes (fa_paged.cu); false: not encoded
+bool encode_rows(void * map, const void * p, uint64_t width, int tokens, int64_t pages, int64_t nb1, int64_t nb3, int box, int tokens_box);
 
 // the records' join behind a kernel that cut items (fa_paged.cu)
 int merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int rows_y, cudaStream_t stream);

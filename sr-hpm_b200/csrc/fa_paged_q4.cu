@@ -1,521 +1,860 @@
-// Attention of a batch's new tokens over a paged cache of q4_0 rows, for the few rows per KV head of decoding steps
-// (srhpm_flash_attn_paged).
+// Attention of a batch's new tokens over a paged cache of q4_0 rows (srhpm_flash_attn_paged), on the 5th-generation tensor
+// cores, with the cached tokens along the products' long side:
+//   S^T = K Q^T        M = 128 tokens, N rows; K as f16 in tensor memory (a lane per token), Q in shared memory
+//   softmax            a thread has one token's scores; a row's maximum is raised only when a score exceeds it by 2^8, which all
+//                      threads of the row learn through one barrier with a vote; p = 2^(s - m + 7) as f16 into shared memory
+//   O^T += V^T P^T     M = 128 dims, N rows, K = 128 tokens: V as it lies, a row of f16 per token
+// The rows of a sequence and KV head (query heads of its group x new tokens) are the narrow side, so 4 rows of a decoding step
+// cost a product of N = 16, not one of 64 or 128 rows that mostly are none, and 4-bit numbers are unpacked once for all rows of
+// a tile. Unpacking goes where it costs least: K's into tensor memory, whose writes take no shared memory bandwidth, V's into
+// the 128-byte swizzled rows that the product reads.
 //
-// A row tile (8 NT rows of a sequence and KV head, packed token by token) fills an eighth or less of a 5th-generation tensor
-// product, and 4-bit values would have to go through shared memory as f16 to reach one: four times the cache's bytes in
-// writes and as much again in reads. Here the numbers become f16 in registers and stay there: a warp multiplies 16 tokens x
-// 16 dims by 8 rows (mma.sync m16n8k16, f32 sums), with K as the left operand of S^T = K Q^T and V as that of O^T = V^T P^T.
-//   operand order  A product's inner index may run in any order that both sides share, so no value moves between lanes: lane
-//                  4 g + t takes, of the 36 bytes of a pair of blocks, word t of either block (K: token g; V: token 4 t + i,
-//                  word g), and Q is laid out once per item in the order in which K's lanes hold their dims
-//   numbers        (w & 0x000f000f) | 0x64006400 is the f16 pair 1024 + q; minus 1032 it is q - 8, exactly; the high halves
-//                  of the bytes come as 1024 + 16 q and go through x / 16 - 72, exactly. Then one product with d, rounded: the
-//                  cache's value
-//   P^T            comes out of S^T with the rows along the columns; two 8 x 8 transpositions (movmatrix) per 16 tokens make
-//                  it the right operand of the second product
-//   softmax        the running maximum is raised only when a score exceeds it by 2^8, sums in f32; p is kept times 2^7 as f16
-//
-// Work: the line of all items' units is cut into equal parts, one per CTA (plan_part). The CTA's warps share an item's steps
-// of TS tokens out, every W-th each, with rings of their own that cp.async fills (no barrier in the loop): 9 pieces of D / 16
-// bytes make a row, whatever its strides are. At an item's end the warps' sums are joined in shared memory.
+// Work: as in fa_paged.cu, all items' units of 128 tokens stand in one line that is cut into equal parts, one per CTA.
+// Roles: 8 softmax warps (two groups, half of the rows each), 1 MMA warp, 3 warps that bring Q, 4 that unpack K and 4 that
+// unpack V. An unpacking warp has 32 tokens of each tile and brings their bytes itself, by cp.async into a ring of its own,
+// several tiles ahead and across items: 9 pieces make a row of 64 or 128 values, whatever the strides are.
+// f32 rows (PREC): Q and P as sums of two f16 parts, and as the tensor cores' sums are truncated (a shrink of 2^-25 per product
+// step, measured: 2e-5 after 400), O is taken out every kFlush tiles and summed up in f32 in the item's record.
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "fa_paged.cuh"
 #include "fastdiv.cuh"
 #include "internal.h"
 #include "launch.cuh"
 #include "ptx.cuh"
+#include "q4.cuh"
+#include "tc.cuh"
 
 namespace srhpm {
 using namespace fap;
 namespace {
 
-constexpr int kUnit = 128;  // tokens of a unit of work
+constexpr int      kTile   = 128;  // tokens of a tile and of a unit of work
+constexpr int      kSm     = 8;    // softmax warps
+constexpr int      kQW     = 3;    // warps that bring Q
+constexpr int      kThr    = (kSm + 1 + kQW + 8) * 32;
+constexpr int      kFlush  = 4;    // tiles
+constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s
+constexpr float    kUnset  = -3e38f;    // a row's reference before its first score
 
 struct Pool4 {
     const uint8_t * p;
     int64_t         nb1, nb2, nb3;
 };
 
-template <int D, int NT, bool PREC> struct LayF {
-    static constexpr int BM    = 8 * NT;               // rows of a tile
-    static constexpr int TS    = D == 256 ? 16 : 32;   // tokens of a step
-    static constexpr int W     = D * NT > 128 ? 8 : 16;  // warps: O takes D NT / 4 registers of a lane
-    static constexpr int rowb  = D / 16 * 9;
-    static constexpr int CB    = D / 16;               // bytes of a copy
-    static constexpr int stage = 2 * TS * rowb;        // K rows, V rows
+// a stage's rows: HD values of a token in RS bytes, of which TMA fills all (its boxes start on 16 bytes, a row up to 12 later)
+constexpr int row_values(int D) { return D < 128 ? D : 128; }
+constexpr int row_stride(int D) { return D < 128 ? 48 : 80; }
+
+template <int D, int N, bool PREC> struct LayT {
     static constexpr int parts = PREC ? 2 : 1;
-    static constexpr int pad   = D + 4;
-    static constexpr int q     = 0;                                   // [2][parts][D / 32][NT][32] uint4
-    static constexpr int qset  = parts * (D / 32) * NT * 512;
-    static constexpr int part  = q + 2 * qset;                        // f32 [W][BM][pad]
-    static constexpr int ms    = part + W * BM * pad * 4;             // float2 [W][BM]
-    static constexpr int misc  = ms + W * BM * 8;
-    static constexpr int ring  = misc + 64;
-    static constexpr int room  = 232448 - ring;
-    static constexpr int ST    = room / (W * stage) < 4 ? room / (W * stage) : 4;
-    static constexpr int total = ring + ST * W * stage;
-    static_assert(ST >= 2 && ring % 16 == 0 && ST * W * stage >= kMaxSeqs * 8, "shared memory");
+    static constexpr int MT    = D == 256 ? 2 : 1;             // products along the dims
+    static constexpr int MM    = D == 64 ? 64 : 128;           // dims of a product
+    static constexpr int NP    = N < 32 ? 32 : N;              // tensor-memory columns of N
+    static constexpr int CH    = D == 256 ? 2 : 1;             // chunks of a V tile, 32 KB at most
+    static constexpr int vtok  = kTile / CH;
+    static constexpr int chunk = vtok * D * 2;
+    static constexpr int VS    = 2;                            // chunks in the ring
+    static constexpr int KB    = D / 2 * 2 + MT * NP + 2 * NP <= 512 ? 2 : 1;   // K tiles in tensor memory
+    static constexpr int SB    = KB * D / 2 + MT * NP + 2 * NP <= 512 ? 2 : 1;  // score buffers
+    static constexpr int qtile = N * D * 2;
+    static constexpr int planes = (N + 63) / 64;
+    static constexpr int ptile = planes * kTile * 128;         // one part of P
+    static constexpr int q     = 0;
+    static constexpr int ring  = q + parts * qtile;
+    static constexpr int p     = ring + VS * chunk;
+    // P buffers: two where shared memory has room for them beside three stages of raw rows
+    static constexpr int HD    = row_values(D);
+    static constexpr int SPT   = D / HD;                       // stages of a tile
+    static constexpr int rowb  = HD / 16 * 9;
+    static constexpr int CB    = HD / 16;
+    static constexpr int RS    = row_stride(D);
+    static constexpr int stage = 32 * RS;                      // of one warp
+    static constexpr int tail  = 2560 + 24 * N;                // barriers, rows' numbers
+    static constexpr int PB    = 232448 - tail - p - 2 * parts * ptile >= 4 * 8 * stage ? 2 : 1;
+    static constexpr int raw   = p + PB * parts * ptile;
+    static constexpr int room  = (232448 - tail - raw) / (8 * stage);
+    static constexpr int ST    = room < 6 * SPT ? room : 6 * SPT;
+    static constexpr int rows  = raw + ST * 8 * stage;         // off, m, fac, frec: f32 [N]; lo, hi: int [N]
+    static constexpr int red   = rows + 24 * N;                // f32 [2][4][32]
+    static constexpr int bar   = red + 1024;
+    static constexpr int nbar  = 2 * KB + 2 * VS + 2 * SB + PB + 2 + 2 + 8 * ST;
+    static constexpr int misc  = bar + nbar * 8;
+    static constexpr int total = misc + 80;
+    static constexpr int CW    = N / 2 < 32 ? N / 2 : 32;      // columns that a softmax thread takes at a time
+    static constexpr int NC    = N / 2 / CW;
+    static constexpr uint32_t tO = 0, tS = MT * NP, tK = tS + SB * NP;
+    static_assert(total <= 232448 && ST >= 2 && raw % 16 == 0 && rows >= kMaxSeqs * 8, "shared memory");
+    static_assert(tK + KB * D / 2 <= 512, "tensor memory");
+    // registers of the softmax warps, of the MMA's and Q's, of the unpacking ones: the launch's 96 a thread, shared out anew
+    static constexpr int rs = N == 128 ? 144 : 120, rm = N == 128 ? 72 : 56, ru = N == 128 ? 56 : 88;
+    static_assert(256 * rs + 128 * rm + 256 * ru <= kThr * 96, "registers");
 };
 
-template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const uint8_t * src, uint32_t size) {
-    if constexpr (N == 16) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(size) : "memory");
-    } else {
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(size) : "memory");
-    }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
-
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-    uint32_t r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-    return r;
-}
-template <uint32_t MASK> __device__ __forceinline__ uint32_t magic(uint32_t x) {  // (x & MASK) | 0x64006400
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "n"(MASK), "r"(0x64006400u));
-    return r;
-}
-__device__ __forceinline__ uint32_t low4(uint32_t x, uint32_t dd) {  // bits 0..3 of either half -> d (q - 8)
-    const uint32_t m = magic<0x000f000fu>(x);
-    __half2        h = __hsub2(*reinterpret_cast<const __half2 *>(&m), __floats2half2_rn(1032.0f, 1032.0f));
-    h                = __hmul2(h, *reinterpret_cast<const __half2 *>(&dd));
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t high4(uint32_t x, uint32_t dd) {  // bits 4..7
-    const uint32_t m = magic<0x00f000f0u>(x);
-    __half2        h = __hfma2(*reinterpret_cast<const __half2 *>(&m), __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.0f, -72.0f));
-    h                = __hmul2(h, *reinterpret_cast<const __half2 *>(&dd));
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
-    uint32_t r;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-    return r;
+// A from tensor memory (K-major f16 pairs, lane = row)
+__device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u)
+        : "memory");
 }
 __device__ __forceinline__ float exp2a(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-
-// byte of a block's 16 that byte b of word w is: word 3 of an even block is made of the bytes around its others (the first
-// block of a pair starts 2 bytes off the words)
-__device__ __forceinline__ int byte_of(bool odd, int w, int b) { return odd ? 4 * w + b : w < 3 ? 2 + 4 * w + b : b < 2 ? b : 12 + b; }
-
-// an item's tokens in this CTA
-struct Run {
-    int t0, n;  // first token (a multiple of TS), steps
-};
-template <int TS> __device__ __forceinline__ Run run_of(const Walk & w) {
-    Run r{ 0, 0 };
-    if (w.sp.nkv) {
-        const int b = (w.sp.kt0 + w.off) * kUnit;
-        const int e = min(b + w.take * kUnit, w.sp.hi);
-        r.t0        = max(b, w.sp.lo) & ~(TS - 1);
-        r.n         = (e - r.t0 + TS - 1) / TS;
+__device__ __forceinline__ void wait_bar(uint64_t * bar, uint32_t parity, int32_t * status, bool & bad) {
+    if (bad) return;
+    for (uint32_t i = 0; i < kProbes; i++) {
+        if (mbar_try_wait(bar, parity)) return;
     }
-    return r;
+    bad = true;  // this thread waits for nothing more: its results are void, its accesses stay in bounds
+    atomicExch(status, kErrWaitFull);
+}
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap * m, int x, int y, int z, uint64_t * bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+// true for all `count` threads of barrier `id` if one of them says so
+__device__ __forceinline__ bool bar_any(int id, int count, bool v) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %3, 0;\n\tbar.red.or.pred q, %1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r)
+                 : "r"(id), "r"(count), "r"((uint32_t) v)
+                 : "memory");
+    return r != 0;
 }
 
-template <int D, int NT, bool PREC>
-__global__ void __launch_bounds__(LayF<D, NT, PREC>::W * 32, 1)
-    fa_paged_q4_few_kernel(const __grid_constant__ PArgs a, const __grid_constant__ Pool4 kp, const __grid_constant__ Pool4 vp) {
-    using Ly           = LayF<D, NT, PREC>;
-    constexpr int BM   = Ly::BM;
-    constexpr int TS   = Ly::TS;
-    constexpr int W    = Ly::W;
-    constexpr int ST   = Ly::ST;
-    constexpr int MT   = TS / 16;
-    constexpr int NG   = D / 64;
-    constexpr int CB   = Ly::CB;
-    constexpr int NI   = (TS * 9 + 31) / 32;
-    constexpr int rowb = Ly::rowb;
-    extern __shared__ __align__(16) uint8_t sm[];
-    float *   part  = reinterpret_cast<float *>(sm + Ly::part);
-    float2 *  ms    = reinterpret_cast<float2 *>(sm + Ly::ms);
-    int *     first = reinterpret_cast<int *>(sm + Ly::misc);
-    int64_t * range = reinterpret_cast<int64_t *>(sm + Ly::misc + 16);
+template <int W> __device__ __forceinline__ void ld_t(uint32_t t, uint32_t (&r)[W]) {
+    if constexpr (W == 32) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+            "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+              "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+              "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+            : "r"(t));
+    } else {
+        tc::ld8(t, r);
+    }
+}
+template <int W> __device__ __forceinline__ void st_t(uint32_t t, const uint32_t (&r)[W]) {
+    if constexpr (W == 32) {
+        tc::st16(t, *reinterpret_cast<const uint32_t(*)[16]>(&r[0]));
+        tc::st16(t + 16, *reinterpret_cast<const uint32_t(*)[16]>(&r[16]));
+    } else {
+        tc::st8(t, r);
+    }
+}
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    if (tid == 0) first[0] = -1;
+// o += what the record holds of it, times the factors that its rows were rescaled by since; all loads in flight at once
+template <int W> __device__ __forceinline__ void add_record(uint32_t (&o)[W], const float * rec, int stride, int n, const float * f) {
+    float x[W];
+#pragma unroll
+    for (int e = 0; e < W; e++) x[e] = e < n ? rec[e * stride] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < W; e++) o[e] = __float_as_uint(fmaf(x[e], f[e], __uint_as_float(o[e])));
+}
+
+// W columns over the warp's 32 lanes: afterwards lane l has the result of column l % W in x[0]
+template <int W, class T, class F> __device__ __forceinline__ float fold(T (&x)[W], F f) {
+    const int lane = threadIdx.x & 31;
+    int       n = W;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        if (o >= W) {
+#pragma unroll
+            for (int k = 0; k < W; k++) x[k] = f(x[k], __shfl_xor_sync(0xffffffffu, x[k], o));
+        } else {
+            n = o;
+#pragma unroll
+            for (int k = 0; k < W / 2; k++) {
+                if (k < n) {
+                    const T keep = (lane & o) ? x[k + n] : x[k], give = (lane & o) ? x[k] : x[k + n];
+                    x[k]             = f(keep, __shfl_xor_sync(0xffffffffu, give, o));
+                }
+            }
+        }
+    }
+    if constexpr (sizeof(T) == 4 && !std::is_same<T, float>::value) {
+        return __uint_as_float(x[0]);
+    } else {
+        return x[0];
+    }
+}
+
+template <int D, int N, bool PREC>
+__global__ void __launch_bounds__(kThr, 1)
+    fa_paged_q4_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ PArgs a,
+                       const __grid_constant__ Pool4 kp, const __grid_constant__ Pool4 vp) {
+    using Ly           = LayT<D, N, PREC>;
+    constexpr int KB = Ly::KB, SB = Ly::SB, PB = Ly::PB, VS = Ly::VS, CH = Ly::CH, ST = Ly::ST, CW = Ly::CW, NC = Ly::NC;
+    extern __shared__ __align__(1024) uint8_t sm[];
+    uint64_t * kfull  = reinterpret_cast<uint64_t *>(sm + Ly::bar);
+    uint64_t * kempty = kfull + KB;
+    uint64_t * vfull  = kempty + KB;
+    uint64_t * vempty = vfull + VS;
+    uint64_t * sfull  = vempty + VS;
+    uint64_t * sfree  = sfull + SB;
+    uint64_t * pfull  = sfree + SB;
+    uint64_t * pvdone = pfull + PB;  // [2] in turn
+    uint64_t * qfull  = pvdone + 2;
+    uint64_t * qempty = qfull + 1;
+    uint64_t * rawfull = qempty + 1;  // [8][ST]
+    uint32_t * tptr   = reinterpret_cast<uint32_t *>(sm + Ly::misc);
+    int *      first  = reinterpret_cast<int *>(sm + Ly::misc + 16);
+    int64_t *  range  = reinterpret_cast<int64_t *>(sm + Ly::misc + 32);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    bool      bad = false;
+    if (smem_u32(sm) & 1023u) {  // the swizzled operands need it; the linker places the only shared array so
+        if (tid == 0) atomicExch(a.status, kErrWaitFull);
+        pdl_wait();
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < KB; i++) {
+            mbar_init(&kfull[i], 4);
+            mbar_init(&kempty[i], 1);
+        }
+        for (int i = 0; i < VS; i++) {
+            mbar_init(&vfull[i], 4 / CH);
+            mbar_init(&vempty[i], 1);
+        }
+        for (int i = 0; i < SB; i++) {
+            mbar_init(&sfull[i], 1);
+            mbar_init(&sfree[i], kSm);
+        }
+        for (int i = 0; i < PB; i++) mbar_init(&pfull[i], kSm);
+        for (int i = 0; i < 2; i++) mbar_init(&pvdone[i], 1);
+        mbar_init(qfull, kQW);
+        mbar_init(qempty, 1);
+        for (int i = 0; i < 8 * ST; i++) mbar_init(&rawfull[i], a.box ? 1 : 32);
+        fence_mbar_init();
+        first[0] = -1;
+    }
+    if (warp == kSm) tc::tmem_alloc(tptr, 512);
     pdl_launch_dependents();
     pdl_wait();
-    plan_part<BM, kUnit>(a, reinterpret_cast<int *>(sm + Ly::ring), reinterpret_cast<int *>(sm + Ly::ms), first, range);
+    plan_part<N, kTile>(a, reinterpret_cast<int *>(sm), reinterpret_cast<int *>(sm + Ly::red), first, range);
+    tc::fence_before();
     __syncthreads();
+    tc::fence_after();
+    const uint32_t tb = *tptr;
     if (tid == 0) a.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
     Walk w;
-    w.s = first[0];
-    if (w.s < 0) return;
-    w.h   = first[1];
-    w.rt  = first[2];
-    w.off = first[3];
-    w.rem = w.part = range[1] - range[0];
-    walk_load<BM>(a, w);
-    walk_item<BM, kUnit>(a, w);
+    w.s         = first[0];
+    bool active = w.s >= 0;
+    if (active) {
+        w.h   = first[1];
+        w.rt  = first[2];
+        w.off = first[3];
+        w.rem = w.part = range[1] - range[0];
+        walk_load<N>(a, w);
+        walk_item<N, kTile>(a, w);
+    }
 
-    // ---- this warp's copies, up to ST steps ahead of its products, across items ----
-    Walk      pw   = w;
-    Run       prun = run_of<TS>(pw);
-    int       pst  = warp;
-    bool      pact = true;
-    int       pg = -1, pin = 0;  // lane = token of the step to come: its page (-1: nobody sees it) and place
-    const uint32_t ring0 = smem_u32(sm + Ly::ring + warp * (ST * Ly::stage));
-    auto           look  = [&]() {
-        while (pact && pst >= prun.n) {
-            pact = walk_next<BM, kUnit>(a, pw);
-            if (pact) {
-                prun = run_of<TS>(pw);
-                pst  = warp;
+    if (warp < kSm) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Ly::rs));
+        // ---------------- softmax ----------------
+        const int wg = warp >> 2, wq = warp & 3, tg = tid & 127, bid = 1 + wg;
+        float *   off = reinterpret_cast<float *>(sm + Ly::rows), *mrow = off + N, *fac = mrow + N, *frec = fac + N;
+        int *     rlo = reinterpret_cast<int *>(frec + N), *rhi = rlo + N;
+        float *   red = reinterpret_cast<float *>(sm + Ly::red) + wg * 128;
+        const int g0  = wg * (N / 2);  // this group's rows
+        // dim of this lane's row of O^T, of each product along the dims
+        const int  od   = D == 64 ? q4::value_at(16 * wq + (lane & 15)) : 64 * (wq >> 1) + q4::value_at(32 * (wq & 1) + lane);
+        const bool mine = D != 64 || lane < 16;
+        uint32_t   gi = 0, pvw = 0;
+        auto       pv_wait = [&](uint32_t upto) {
+            for (; pvw < upto; pvw++) wait_bar(&pvdone[pvw & 1], (pvw >> 1) & 1, a.status, bad);
+        };
+        for (; active; active = walk_next<N, kTile>(a, w)) {
+            const int  n = w.sp.nkv ? w.take : 0, rb = w.rt * N, rows = min(N, w.n * a.G - rb);
+            const int  slot = 2 * blockIdx.x + (w.off == 0 ? 1 : 0);
+            const bool whole = w.off == 0 && w.take == w.sp.units;
+            if (tg < N / 2) {
+                const int  r = g0 + tg;
+                const bool is = r < rows;
+                const int  pos = w.kv - w.n + a.byG.div(rb + (is ? r : 0));
+                rhi[r]  = is ? min(pos + 1, w.sp.hi) : 0;
+                rlo[r]  = a.window > 0 ? max(w.sp.lo, (int) max((int64_t) INT32_MIN, (int64_t) pos - a.window + 1)) : w.sp.lo;
+                off[r]  = is ? kUnset : INFINITY;  // rows that are none: p = 0
+                mrow[r] = is ? -INFINITY : INFINITY;
+                frec[r] = 1.0f;
             }
-        }
-        pg = -1;
-        if (pact && lane < TS) {
-            const int tok = prun.t0 + pst * TS + lane;
-            if (tok >= pw.sp.lo && tok < pw.sp.hi) {
-                const int pi = a.byPage.div(tok);
-                pin          = tok - pi * a.page;
-                pg           = reinterpret_cast<const int32_t *>(a.table + (int64_t) pw.s * a.tstride)[pi];
-                if (pg < 0 || pg >= a.n_pages) {  // no page: reads as zeros
-                    atomicExch(a.status, kErrPage);
-                    pg = -1;
+            named_bar_sync(bid, 128);
+            // tokens that every row sees
+            const int pmin = w.kv - w.n + a.byG.div(rb), pmax = w.kv - w.n + a.byG.div(rb + rows - 1);
+            const int ahi = min(pmin + 1, w.sp.hi), alo = a.window > 0 ? (int) max((int64_t) 0, (int64_t) pmax - a.window + 1) : w.sp.lo;
+            float     l[NC][CW];
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+#pragma unroll
+                for (int e = 0; e < CW; e++) l[c][e] = 0.0f;
+            }
+            const float qs = a.softcap_l2 != 0.0f ? 1.0f : a.qscale;
+            // O's part of one chunk of columns: f(values, product along the dims)
+            auto each_o = [&](int c0, auto f) {
+#pragma unroll 1
+                for (int mt = 0; mt < Ly::MT; mt++) {
+                    uint32_t       o[CW];
+                    const uint32_t at = tc::taddr(tb + Ly::tO + mt * Ly::NP + c0, wq, 0);
+                    ld_t<CW>(at, o);
+                    tc::wait_ld();
+                    f(o, mt, at);
                 }
-            }
-        }
-    };
-    auto issue = [&](int stage) {
-        if (pact) {
-            const int64_t ko = pg < 0 ? -1 : pg * kp.nb3 + pin * kp.nb1 + pw.h * kp.nb2;
-            const int64_t vo = pg < 0 ? -1 : pg * vp.nb3 + pin * vp.nb1 + pw.h * vp.nb2;
-            const uint32_t to = ring0 + stage * Ly::stage;
+            };
+            for (int i = 0; i < n; i++, gi++) {
+                const uint32_t sb = gi % SB, pb = gi % PB;
+                const int      t0 = w.tile(i) * kTile, pos = t0 + 32 * wq + lane;
+                const bool     mask = t0 < alo || t0 + kTile > ahi;
+                wait_bar(&sfull[sb], (gi / SB) & 1, a.status, bad);
+                tc::fence_after();
+                if constexpr (PREC) {
+                    if (i > 0 && i % kFlush == 0) {  // O so far to the record
+                        pv_wait(gi);
+                        tc::fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < NC; c++) {
+                            each_o(g0 + c * CW, [&](uint32_t (&o)[CW], int mt, uint32_t) {
+                                float *   rec = a.part_acc + ((int64_t) slot * a.prow + g0 + c * CW) * D + 128 * mt + od;
+                                const int nr  = mine ? rows - (g0 + c * CW) : 0;
+                                if (i > kFlush) add_record(o, rec, D, nr, frec + g0 + c * CW);
 #pragma unroll
-            for (int i = 0; i < NI; i++) {
-                const int     idx = i * 32 + lane, tk = idx / 9, ch = idx - 9 * tk;
-                const int64_t ks = __shfl_sync(0xffffffffu, ko, tk & (TS - 1)), vs = __shfl_sync(0xffffffffu, vo, tk & (TS - 1));
-                if (idx < TS * 9) {
-                    copy_async<CB>(to + idx * CB, kp.p + (ks < 0 ? 0 : ks + ch * CB), ks < 0 ? 0 : CB);
-                    copy_async<CB>(to + TS * rowb + idx * CB, vp.p + (vs < 0 ? 0 : vs + ch * CB), vs < 0 ? 0 : CB);
-                }
-            }
-            pst += W;
-            look();
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    look();
-    for (int s = 0; s < ST; s++) issue(s);
-
-    const uint32_t selv = g == 3 ? 0x1076u : 0x3210u, selk = t == 3 ? 0x1076u : 0x3210u, seld = g < 4 ? 0x5410u : 0x7632u;
-    const uint32_t tmask = 4 * (g >> 1) + (g & 1);  // token of this lane's first score of 16; the second is 2 behind it
-    int            stage = 0, par = 0;
-    for (bool active = true; active; par ^= 1) {
-        const int n  = w.n * a.G, rb = w.rt * BM, rows = min(BM, n - rb);
-        const Run run = run_of<TS>(w);
-        // ---- Q, in the order of K's lanes; rows that are none as zeros ----
-        uint4 * qb = reinterpret_cast<uint4 *>(sm + Ly::q + par * Ly::qset);
-        for (int u = tid; u < (D / 32) * NT * 32; u += W * 32) {
-            const int ln = u & 31, nt = (u >> 5) % NT, blk = (u >> 5) / NT, row = 8 * nt + (ln >> 2), tt = ln & 3;
-            float     x[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = 0.0f;
-            if (row < rows) {
-                const int       tok = a.byG.div(rb + row), h = w.h * a.G + (rb + row - tok * a.G);
-                const uint8_t * src = a.q + (int64_t) (w.r0 + tok) * a.qnb1 + (int64_t) h * a.qnb2;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {  // pairs (0, 2), (1, 3) of the low, then of the high halves
-                    const int b = (e & 1) * 2 + ((e >> 1) & 1), d = 32 * blk + byte_of(blk & 1, tt, b) + 16 * (e >> 2);
-                    x[e] = PREC ? reinterpret_cast<const float *>(src)[d] : __half2float(reinterpret_cast<const __half *>(src)[d]);
-                }
-            }
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const __half2 h2 = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
-                const __half2 l2 = __floats2half2_rn(x[2 * e] - __low2float(h2), x[2 * e + 1] - __high2float(h2));
-                hi[e] = *reinterpret_cast<const uint32_t *>(&h2);
-                lo[e] = *reinterpret_cast<const uint32_t *>(&l2);
-            }
-            qb[u] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if constexpr (PREC) qb[(D / 32) * NT * 32 + u] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        // ---- what this lane's rows see ----
-        int   vlo[NT][2], vhi[NT][2];
-        float m[NT][2], l[NT][2];
-        float o[NG][4][NT][4];
-        int   alo = 0, ahi = INT32_MAX;  // seen by every row
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const int  row = 8 * nt + 2 * t + k;
-                const bool is  = row < rows;
-                const int  pos = w.kv - w.n + a.byG.div(rb + (is ? row : 0));
-                vhi[nt][k]     = is ? min(pos + 1, w.sp.hi) : 0;
-                vlo[nt][k]     = a.window > 0 ? max(w.sp.lo, (int) max((int64_t) INT32_MIN, (int64_t) pos - a.window + 1)) : w.sp.lo;
-                if (is) {
-                    alo = max(alo, vlo[nt][k]);
-                    ahi = min(ahi, vhi[nt][k]);
-                }
-                m[nt][k]       = -INFINITY;
-                l[nt][k]       = 0.0f;
-            }
-        }
-        alo = __reduce_max_sync(0xffffffffu, alo);
-        ahi = __reduce_min_sync(0xffffffffu, ahi);
-#pragma unroll
-        for (int i = 0; i < NG; i++) {
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[i][b][nt][e] = 0.0f;
-                }
-            }
-        }
-        __syncthreads();
-        const uint4 * ql = qb + lane;
-        for (int st = warp; st < run.n; st += W) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(ST - 1) : "memory");
-            __syncwarp();
-            const uint8_t * kr = sm + Ly::ring + warp * (ST * Ly::stage) + stage * Ly::stage;
-            const uint8_t * vr = kr + TS * rowb;
-            float           s[MT][NT][4];
-#pragma unroll
-            for (int i = 0; i < MT; i++) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[i][nt][e] = 0.0f;
-                }
-            }
-#pragma unroll
-            for (int bp = 0; bp < NG; bp++) {
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    uint32_t p[2][2][4];  // token, block, pairs
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const uint32_t * row = reinterpret_cast<const uint32_t *>(kr + (16 * i + tmask + 2 * k) * rowb + 36 * bp);
-                        const uint32_t   y0 = row[0], y1 = row[4], z = row[5 + t];
-                        const uint32_t   x = prmt(row[1 + t], y0, selk);
-                        const uint32_t   d0 = prmt(y0, y0, 0x1010u), d1 = prmt(y1, y1, 0x3232u);
-                        p[k][0][0] = low4(x, d0);
-                        p[k][0][1] = low4(x >> 8, d0);
-                        p[k][0][2] = high4(x, d0);
-                        p[k][0][3] = high4(x >> 8, d0);
-                        p[k][1][0] = low4(z, d1);
-                        p[k][1][1] = low4(z >> 8, d1);
-                        p[k][1][2] = high4(z, d1);
-                        p[k][1][3] = high4(z >> 8, d1);
+                                for (int e = 0; e < CW; e++) {
+                                    if (e < nr) rec[e * D] = __uint_as_float(o[e]);
+                                }
+                            });
+                        }
+                        named_bar_sync(bid, 128);
+                        if (tg < N / 2) frec[g0 + tg] = 1.0f;
                     }
+                }
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
+                for (int c = 0; c < NC; c++) {
+                    const int      c0 = g0 + c * CW;
+                    const uint32_t ts = tc::taddr(tb + Ly::tS + sb * Ly::NP + c0, wq, 0);
+                    uint32_t       s[CW];
+                    auto           scores = [&]() {
+                        ld_t<CW>(ts, s);
+                        tc::wait_ld();
+                        if (a.softcap_l2 != 0.0f) {
 #pragma unroll
-                        for (int b = 0; b < 2; b++) {
+                            for (int e = 0; e < CW; e++) s[e] = __float_as_uint(a.softcap_l2 * tanhf(__uint_as_float(s[e]) * a.qscale));
+                        }
+                        if (mask) {
 #pragma unroll
-                            for (int pr = 0; pr < Ly::parts; pr++) {
-                                const uint4 qv = ql[((pr * (D / 32) + 2 * bp + b) * NT + nt) * 32];
-                                mma16816(s[i][nt], p[0][b][0], p[1][b][0], p[0][b][1], p[1][b][1], qv.x, qv.y);
-                                mma16816(s[i][nt], p[0][b][2], p[1][b][2], p[0][b][3], p[1][b][3], qv.z, qv.w);
+                            for (int e = 0; e < CW; e++) {
+                                if (pos < rlo[c0 + e] || pos >= rhi[c0 + e]) s[e] = __float_as_uint(-INFINITY);
+                            }
+                        }
+                    };
+                    auto shifted = [&]() {
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int e = 0; e < CW; e += 4) {
+                            const float4 o = *reinterpret_cast<const float4 *>(off + c0 + e);
+                            float        x0, x1, x2, x3;
+                            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f2_pack(qs, qs), f2_pack(-o.x, -o.y)), x0, x1);
+                            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), f2_pack(qs, qs), f2_pack(-o.z, -o.w)), x2, x3);
+                            s[e] = __float_as_uint(x0); s[e + 1] = __float_as_uint(x1); s[e + 2] = __float_as_uint(x2); s[e + 3] = __float_as_uint(x3);
+                            top = fmaxf(fmaxf(top, fmaxf(x0, x1)), fmaxf(x2, x3));
+                        }
+                        return top;
+                    };
+                    scores();
+                    const float top = shifted();
+                    if (bar_any(bid, 128, top > kLazy + kShift)) {
+                        // raise the rows' references: largest scores over the tile's tokens
+                        scores();
+                        const float best = qs * fold(s, [](uint32_t u, uint32_t v) { return __float_as_uint(fmaxf(__uint_as_float(u), __uint_as_float(v))); });
+                        if (lane < CW) red[wq * 32 + lane] = best;
+                        named_bar_sync(bid, 128);
+                        if (tg < CW) {
+                            const float v = fmaxf(fmaxf(red[tg], red[32 + tg]), fmaxf(red[64 + tg], red[96 + tg])), mo = mrow[c0 + tg];
+                            float       f = 1.0f;
+                            if (v > mo + kLazy) {  // of -inf: any score
+                                f             = exp2a(mo - v);
+                                mrow[c0 + tg] = v;
+                                off[c0 + tg]  = v - kShift;
+                                frec[c0 + tg] *= f;
+                            }
+                            fac[c0 + tg] = f;
+                        }
+                        named_bar_sync(bid, 128);
+#pragma unroll
+                        for (int e = 0; e < CW; e++) l[c][e] *= fac[c0 + e];
+                        if (i > 0 && (!PREC || i % kFlush)) {
+                            pv_wait(gi);
+                            tc::fence_after();
+                            each_o(c0, [&](uint32_t (&o)[CW], int, uint32_t at) {
+#pragma unroll
+                                for (int e = 0; e < CW; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac[c0 + e]);
+                                st_t<CW>(at, o);
+                            });
+                            tc::wait_st();
+                        }
+                        scores();
+                        shifted();
+                    }
+                    if (c == NC - 1) {  // S is read
+                        tc::fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sfree[sb]);
+                    }
+                    if (c == 0) pv_wait(gi + 1 > PB ? gi + 1 - PB : 0);  // the product that read this P buffer
+                    uint8_t * pr = sm + Ly::p + pb * Ly::parts * Ly::ptile + (c0 >> 6) * (kTile * 128) + (32 * wq + lane) * 128;
+#pragma unroll
+                    for (int e = 0; e < CW; e += 8) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const float x0 = exp2a(__uint_as_float(s[e + 2 * k])), x1 = exp2a(__uint_as_float(s[e + 2 * k + 1]));
+                            f2_unpack(f2_add(f2_pack(l[c][e + 2 * k], l[c][e + 2 * k + 1]), f2_pack(x0, x1)), l[c][e + 2 * k], l[c][e + 2 * k + 1]);
+                            const __half2 h2 = __floats2half2_rn(x0, x1);
+                            hi[k]            = *reinterpret_cast<const uint32_t *>(&h2);
+                            if constexpr (PREC) {
+                                const __half2 r2 = __floats2half2_rn(x0 - __low2float(h2), x1 - __high2float(h2));
+                                lo[k]            = *reinterpret_cast<const uint32_t *>(&r2);
+                            }
+                        }
+                        uint8_t * to = pr + (((((c0 + e) >> 3) & 7) ^ (lane & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        if constexpr (PREC) *reinterpret_cast<uint4 *>(to + Ly::ptile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                }
+                fence_proxy_async_smem();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[pb]);
+            }
+            // ---------------- the item's end ----------------
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const int   c0 = g0 + c * CW;
+                const float sum = fold(l[c], [](float u, float v) { return u + v; });
+                if (lane < CW) red[wq * 32 + lane] = sum;
+                named_bar_sync(bid, 128);
+                if (tg < CW && c0 + tg < rows) {
+                    const int   r = c0 + tg, tok = a.byG.div(rb + r), h = w.h * a.G + (rb + r - tok * a.G);
+                    float       L = (red[tg] + red[32 + tg]) + (red[64 + tg] + red[96 + tg]);
+                    const float M = mrow[r];
+                    float       f = 1.0f;
+                    if (!whole) {
+                        a.part_ms[(int64_t) slot * a.prow + r] = make_float2(M, L);
+                    } else {
+                        if (a.sinks) {  // relative to the larger of the two
+                            const float sk = a.sinks[h] * kLog2e;
+                            if (sk > M) {
+                                f = M == -INFINITY ? 0.0f : exp2a(M - sk);
+                                L = L * f + exp2f(kShift);
+                            } else if (sk > -INFINITY) {
+                                L += exp2a(sk - M + kShift);
+                            }
+                        }
+                        f = L == 0.0f ? 0.0f : f / L;  // a NaN stays one
+                    }
+                    fac[r] = f;
+                }
+                named_bar_sync(bid, 128);
+            }
+            if (n > 0) {
+                pv_wait(gi);
+                tc::fence_after();
+            }
+#pragma unroll 1
+            for (int c = 0; c < NC; c++) {
+                const int c0 = g0 + c * CW;
+                if (c0 >= rows) break;
+                auto put = [&](uint32_t (&o)[CW], int mt, uint32_t) {
+                    float * rec = a.part_acc + ((int64_t) slot * a.prow + c0) * D + 128 * mt + od;
+                    if (PREC && n > kFlush) add_record(o, rec, D, mine ? rows - c0 : 0, frec + c0);
+#pragma unroll
+                    for (int e = 0; e < CW; e++) {
+                        const int r = c0 + e;
+                        if (!mine || r >= rows) continue;
+                        float x = __uint_as_float(o[e]);
+                        if (!whole) {
+                            rec[e * D] = x;
+                            continue;
+                        }
+                        const float f = fac[r];
+                        x             = f != 0.0f ? x * f : 0.0f;
+                        const int tok = a.byG.div(rb + r), h = w.h * a.G + (rb + r - tok * a.G);
+                        uint8_t * dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) (w.r0 + tok) * a.dnb2;
+                        if constexpr (PREC) {
+                            reinterpret_cast<float *>(dst)[128 * mt + od] = x;
+                        } else {
+                            reinterpret_cast<__half *>(dst)[128 * mt + od] = __float2half_rn(x);
+                        }
+                    }
+                };
+                if (n > 0) {
+                    each_o(c0, put);
+                } else {
+                    uint32_t o[CW];
+#pragma unroll
+                    for (int e = 0; e < CW; e++) o[e] = 0;
+                    for (int mt = 0; mt < Ly::MT; mt++) put(o, mt, 0);
+                }
+            }
+            tc::fence_before();  // O is read: the next item's products may write it
+            if (tid == 0 && !whole && w.off == 0) {
+                // this CTA opens an item that others go on with: parts of it, for the join
+                const int64_t end = range[0] + (range[1] - range[0] - w.rem) + w.sp.units;
+                int           e   = blockIdx.x;
+                while (range[2] * (e + 1) / range[3] < end) e++;
+                a.desc[2 * blockIdx.x + 1] = make_int4(rb, rows, 0, 0);
+                a.desc[2 * blockIdx.x]     = make_int4(e - (int) blockIdx.x + 1, w.h, w.r0, 0);
+            }
+            named_bar_sync(bid, 128);  // the rows' numbers are read
+        }
+    } else if (warp < kSm + 1 + kQW) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Ly::rm));
+        if (warp == kSm) {
+            // ---------------- MMA ----------------
+            constexpr uint32_t idqk = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kKMajor, tc::kKMajor, N, 128);
+            constexpr uint32_t idpv = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kMNMajor, tc::kMNMajor, N, Ly::MM);
+            constexpr uint64_t sw   = 2ull << 61;  // 128-byte swizzle
+            const uint64_t     qd0  = tc::sdesc(smem_u32(sm + Ly::q), 16, 1024) | sw;  // addresses step by bytes / 16
+            const uint64_t     vd0  = tc::sdesc(smem_u32(sm + Ly::ring), Ly::vtok * 128, 1024) | sw;
+            const uint64_t     pd0  = tc::sdesc(smem_u32(sm + Ly::p), kTile * 128, 1024) | sw;
+            uint32_t           gi = 0, items = 0;
+            for (; active; active = walk_next<N, kTile>(a, w)) {
+                const int n = __shfl_sync(0xffffffffu, w.sp.nkv ? w.take : 0, 0);
+                if (n == 0) continue;
+                wait_bar(qfull, items & 1, a.status, bad);
+                items++;
+                auto qk = [&](int i) {
+                    const uint32_t g = gi + i, kb = g % KB, sb = g % SB;
+                    wait_bar(&kfull[kb], (g / KB) & 1, a.status, bad);
+                    if (g >= SB) wait_bar(&sfree[sb], (g / SB - 1) & 1, a.status, bad);
+                    tc::fence_after();
+                    __syncwarp();
+                    if (elect_one()) {
+                        // a plane of 64 dims at a time: the descriptors of all products at once would not fit the registers
+                        uint64_t qd = qd0;
+                        uint32_t ka = tb + Ly::tK + kb * (D / 2);
+#pragma unroll 1
+                        for (int pl = 0; pl < Ly::parts * (D / 64); pl++) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                mma_f16_ta(tb + Ly::tS + sb * Ly::NP, ka + 8 * j, qd + 2 * j, idqk, (uint32_t) (pl > 0 || j > 0));
+                            }
+                            qd += N * 128 / 16;
+                            ka = pl + 1 == D / 64 ? ka + 32 - D / 2 : ka + 32;
+                        }
+                        tc::commit(&kempty[kb]);
+                        tc::commit(&sfull[sb]);
+                        if (i == n - 1) tc::commit(qempty);
+                    }
+                    __syncwarp();
+                };
+                qk(0);
+                for (int i = 0; i < n; i++) {
+                    if (i + 1 < n) qk(i + 1);
+                    const uint32_t g = gi + i, pb = g % PB;
+                    const bool     fresh = PREC ? i % kFlush == 0 : i == 0;
+#pragma unroll
+                    for (int ch = 0; ch < CH; ch++) wait_bar(&vfull[(g * CH + ch) % VS], ((g * CH + ch) / VS) & 1, a.status, bad);
+                    wait_bar(&pfull[pb], (g / PB) & 1, a.status, bad);
+                    tc::fence_after();
+                    __syncwarp();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ch = 0; ch < CH; ch++) {
+                            const uint32_t sl = (g * CH + ch) % VS;
+#pragma unroll 1
+                            for (int mt = 0; mt < Ly::MT; mt++) {
+                                uint64_t vd = vd0 + (sl * Ly::chunk + mt * 2 * (Ly::vtok * 128)) / 16;
+                                uint64_t pd = pd0 + (pb * Ly::parts * Ly::ptile + ch * (Ly::vtok / 16) * 2048) / 16;
+#pragma unroll 1
+                                for (int j = 0; j < Ly::vtok / 16; j += 2) {
+#pragma unroll
+                                    for (int k = 0; k < 2; k++) {
+#pragma unroll
+                                        for (int part = 0; part < Ly::parts; part++) {
+                                            tc::mma_f16(tb + Ly::tO + mt * Ly::NP, vd + k * 2048 / 16, pd + (part * Ly::ptile + k * 2048) / 16, idpv,
+                                                        (uint32_t) (!fresh || ch > 0 || j + k > 0 || part > 0));
+                                        }
+                                    }
+                                    vd += 4096 / 16;
+                                    pd += 4096 / 16;
+                                }
+                            }
+                            tc::commit(&vempty[sl]);
+                        }
+                        tc::commit(&pvdone[g & 1]);
+                    }
+                    __syncwarp();
+                }
+                gi += n;
+            }
+        } else {
+            // ---------------- Q: 16-byte pieces of 8 dims in K's order, 128-byte swizzle; rows that are none as zeros ----------------
+            constexpr int all = N * (D / 8), per = kQW * 32, UN = PREC ? 1 : 2;
+            const int     u0 = tid - (kSm + 1) * 32;
+            uint32_t      items = 0;
+            for (; active; active = walk_next<N, kTile>(a, w)) {
+                if (w.sp.nkv == 0) continue;
+                const int rb = w.rt * N, rows = min(N, w.n * a.G - rb);
+#pragma unroll 1
+                for (int u = u0; u < all; u += UN * per) {
+                    uint2 x[UN][4];
+#pragma unroll
+                    for (int k = 0; k < UN; k++) {
+                        const int v = u + k * per, row = v / (D / 8), pc = v % (D / 8), odd = (pc >> 2) & 1, word = pc & 3;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[k][e] = make_uint2(0u, 0u);
+                        if (v < all && row < rows) {
+                            const int       tok = a.byG.div(rb + row), h = w.h * a.G + (rb + row - tok * a.G);
+                            const uint8_t * src = a.q + (int64_t) (w.r0 + tok) * a.qnb1 + (int64_t) h * a.qnb2;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {  // pairs of neighbouring dims: bytes 0, 1 and 2, 3, low and high halves
+                                const int d = (pc >> 2) * 32 + q4::byte_of(odd, word, 2 * (e & 1)) + 16 * (e >> 1);
+                                if constexpr (PREC) {
+                                    x[k][e] = *reinterpret_cast<const uint2 *>(src + 4 * d);
+                                } else {
+                                    x[k][e].x = *reinterpret_cast<const uint32_t *>(src + 2 * d);
+                                }
                             }
                         }
                     }
-                }
-            }
-            // ---- softmax: this lane has tokens tmask, tmask + 2 of every 16 and rows 2 t, 2 t + 1 of every 8 ----
-            const int  tb   = run.t0 + st * TS;
-            const bool mask = tb < alo || tb + TS > ahi;
-            const float qs  = a.qscale;
-            float      mx[NT][2];
-            bool       up = false;
+                    if (u == u0 && items > 0) wait_bar(qempty, (items - 1) & 1, a.status, bad);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                mx[nt][0] = mx[nt][1] = -INFINITY;
+                    for (int k = 0; k < UN; k++) {
+                        const int v = u + k * per, row = v / (D / 8), pc = v % (D / 8);
+                        if (v >= all) break;
+                        uint8_t * to = sm + Ly::q + (pc >> 3) * (N * 128) + row * 128 + (((pc & 7) ^ (row & 7)) << 4);
+                        uint32_t  hw[4], lw[4];
 #pragma unroll
-                for (int i = 0; i < MT; i++) {
+                        for (int e = 0; e < 2; e++) {  // low halves, high halves
+                            const uint2 A = x[k][2 * e], B = x[k][2 * e + 1];
+                            if constexpr (PREC) {
+                                const float f[4] = { __uint_as_float(A.x), __uint_as_float(B.x), __uint_as_float(A.y), __uint_as_float(B.y) };
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        float x = s[i][nt][e] * qs;
-                        if (a.softcap_l2 != 0.0f) x = a.softcap_l2 * tanhf(x);
-                        if (mask) {
-                            const int pos = tb + 16 * i + (int) tmask + (e >> 1) * 2;
-                            x             = pos >= vlo[nt][e & 1] && pos < vhi[nt][e & 1] ? x : -INFINITY;
+                                for (int m = 0; m < 2; m++) {
+                                    const __half2 h2 = __floats2half2_rn(f[2 * m], f[2 * m + 1]);
+                                    const __half2 l2 = __floats2half2_rn(f[2 * m] - __low2float(h2), f[2 * m + 1] - __high2float(h2));
+                                    hw[2 * e + m] = *reinterpret_cast<const uint32_t *>(&h2);
+                                    lw[2 * e + m] = *reinterpret_cast<const uint32_t *>(&l2);
+                                }
+                            } else {
+                                hw[2 * e]     = q4::prmt(A.x, B.x, 0x5410u);
+                                hw[2 * e + 1] = q4::prmt(A.x, B.x, 0x7632u);
+                            }
                         }
-                        s[i][nt][e]   = x;
-                        mx[nt][e & 1] = fmaxf(mx[nt][e & 1], x);
-                    }
-                }
-                up |= mx[nt][0] > m[nt][0] + kLazy || mx[nt][1] > m[nt][1] + kLazy;
-            }
-            if (__any_sync(0xffffffffu, up)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float f[2];
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        float x = mx[nt][k];
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        f[k] = 1.0f;
-                        if (x > m[nt][k] + kLazy) {
-                            f[k]     = exp2a(m[nt][k] - x);
-                            m[nt][k] = x;
-                        }
-                        l[nt][k] *= f[k];
-                    }
-#pragma unroll
-                    for (int i = 0; i < NG; i++) {
-#pragma unroll
-                        for (int b = 0; b < 4; b++) {
-#pragma unroll
-                            for (int e = 0; e < 4; e++) o[i][b][nt][e] *= f[e & 1];
-                        }
+                        *reinterpret_cast<uint4 *>(to) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                        if constexpr (PREC) *reinterpret_cast<uint4 *>(to + Ly::qtile) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
                     }
                 }
-            }
-            uint32_t ph[MT][NT][2];
-            [[maybe_unused]] uint32_t pl[MT][NT][2];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const float o0 = (m[nt][0] == -INFINITY ? 0.0f : m[nt][0]) - kShift, o1 = (m[nt][1] == -INFINITY ? 0.0f : m[nt][1]) - kShift;
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const float x0 = exp2a(s[i][nt][2 * k] - o0), x1 = exp2a(s[i][nt][2 * k + 1] - o1);
-                        l[nt][0] += x0;
-                        l[nt][1] += x1;
-                        const __half2 h2 = __floats2half2_rn(x0, x1);
-                        ph[i][nt][k]     = transpose8(*reinterpret_cast<const uint32_t *>(&h2));
-                        if constexpr (PREC) {
-                            const __half2 r2 = __floats2half2_rn(x0 - __low2float(h2), x1 - __high2float(h2));
-                            pl[i][nt][k]     = transpose8(*reinterpret_cast<const uint32_t *>(&r2));
-                        }
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MT; i++) {
-#pragma unroll
-                for (int gq = 0; gq < NG; gq++) {
-                    uint32_t v[4], y[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t * row = reinterpret_cast<const uint32_t *>(vr + (16 * i + 4 * t + k) * rowb + 36 * gq);
-                        y[k]                 = row[g < 4 ? 0 : 4];
-                        v[k]                 = prmt(row[1 + g], y[k], selv);
-                    }
-                    const uint32_t d0 = prmt(y[0], y[1], seld), d1 = prmt(y[2], y[3], seld);
-#pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        const uint32_t sel = 0x4400u + 0x1111u * b, x0 = prmt(v[0], v[1], sel), x1 = prmt(v[2], v[3], sel);
-                        const uint32_t a0 = low4(x0, d0), a1 = high4(x0, d0), a2 = low4(x1, d1), a3 = high4(x1, d1);
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            mma16816(o[gq][b][nt], a0, a1, a2, a3, ph[i][nt][0], ph[i][nt][1]);
-                            if constexpr (PREC) mma16816(o[gq][b][nt], a0, a1, a2, a3, pl[i][nt][0], pl[i][nt][1]);
-                        }
-                    }
-                }
-            }
-            __syncwarp();
-            issue(stage);
-            stage = stage + 1 == ST ? 0 : stage + 1;
-        }
-        // ---- the item's end: the warps' sums side by side ----
-        const bool some = warp < run.n;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                float x = l[nt][k];
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-                if (g == 0) ms[warp * BM + 8 * nt + 2 * t + k] = make_float2(m[nt][k], x);
-                if (some) {
-                    float * to = part + (warp * BM + 8 * nt + 2 * t + k) * Ly::pad;
-#pragma unroll
-                    for (int gq = 0; gq < NG; gq++) {
-#pragma unroll
-                        for (int b = 0; b < 4; b++) {
-                            const int d = 64 * gq + 32 * (g >> 2) + byte_of(g >= 4, g & 3, b);
-                            to[d]       = o[gq][b][nt][k];
-                            to[d + 16]  = o[gq][b][nt][2 + k];
-                        }
-                    }
-                }
+                items++;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(qfull);
             }
         }
-        __syncthreads();
-        const bool whole = w.off == 0 && w.take == w.sp.units;
-        const int  slot  = 2 * blockIdx.x + (w.off == 0 ? 1 : 0);
-        for (int u = tid; u < rows * D; u += W * 32) {
-            const int row = u / D, d = u % D;
-            float     M = -INFINITY, L = 0.0f, x = 0.0f;
-#pragma unroll
-            for (int k = 0; k < W; k++) M = fmaxf(M, ms[k * BM + row].x);
-#pragma unroll
-            for (int k = 0; k < W; k++) {
-                const float2 r = ms[k * BM + row];
-                if (!(r.y == 0.0f)) {  // a warp without weight may have left anything; a NaN stays one
-                    const float wt = exp2a(r.x == -INFINITY && M == -INFINITY ? 0.0f : r.x - M);
-                    L += wt * r.y;
-                    x += wt * part[(k * BM + row) * Ly::pad + d];
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Ly::ru));
+        // ---------------- unpacking: K into tensor memory, V into swizzled rows ----------------
+        const int      wq = warp & 3;
+        const bool     isk = warp < kSm + 1 + kQW + 4;
+        const Pool4 &  pool = isk ? kp : vp;
+        uint8_t *      raw = sm + Ly::raw + (isk ? wq : 4 + wq) * (ST * Ly::stage);
+        const uint32_t raw0 = smem_u32(raw);
+        // copies: the tile and stage that come next
+        uint64_t * rf = rawfull + (isk ? wq : 4 + wq) * ST;
+        Walk       pw = w;
+        int        pn = w.sp.nkv ? w.take : 0, pi = 0, ph = 0;
+        bool       pact = active;
+        // lane j: page of the (j / 2)-th tile from i0 on, tokens 16 (j & 1) .. of this warp's 32. Sixteen tiles' at a time: a table
+        // entry asked for tile by tile held the warp up for its 700 cycles, half of the tile's time
+        int        ent = -1, i0 = 0;
+        auto       look = [&]() {
+            bool fresh = pi - i0 == 16;
+            while (pact && pi >= pn) {
+                pact = walk_next<N, kTile>(a, pw);
+                pn   = pact && pw.sp.nkv ? pw.take : 0;
+                pi   = 0;
+                fresh = true;
+            }
+            if (pact && fresh) {
+                i0            = pi;
+                const int ti  = pi + (lane >> 1);
+                ent           = -1;
+                if (ti < pn) {
+                    const int tok = pw.tile(ti) * kTile + 32 * wq + 16 * (lane & 1);
+                    if (tok < pw.sp.hi && tok + 16 > pw.sp.lo) {
+                        ent = reinterpret_cast<const int32_t *>(a.table + (int64_t) pw.s * a.tstride)[a.byPage.div(tok)];
+                        if (ent < 0 || ent >= a.n_pages) {  // no page: reads as zeros
+                            atomicExch(a.status, kErrPage);
+                            ent = a.n_pages;
+                        }
+                    }
                 }
             }
-            if (!whole) {
-                a.part_acc[((int64_t) slot * a.prow + row) * D + d] = x;
-                if (d == 0) a.part_ms[(int64_t) slot * a.prow + row] = make_float2(M, L);
-                continue;
-            }
-            const int tok = a.byG.div(rb + row), h = w.h * a.G + (rb + row - tok * a.G);
-            float     f = 1.0f;
-            if (a.sinks) {  // relative to the larger of the two maxima
-                const float sk = a.sinks[h] * kLog2e;
-                if (sk > M) {
-                    f = M == -INFINITY ? 0.0f : exp2a(M - sk);
-                    L = L * f + exp2f(kShift);
-                } else if (sk > -INFINITY) {
-                    L += exp2a(sk - M + kShift);
+        };
+        auto issue = [&](int st) {
+            if (!pact) return;
+            const uint32_t to = raw0 + st * Ly::stage;
+            const int      t0 = pw.tile(pi) * kTile + 32 * wq;
+            const int      p0 = __shfl_sync(0xffffffffu, ent, 2 * (pi - i0)), p1 = __shfl_sync(0xffffffffu, ent, 2 * (pi - i0) + 1);  // -1: not seen
+            const int      y0 = t0 - a.byPage.div(t0) * a.page, y1 = t0 + 16 - a.byPage.div(t0 + 16) * a.page;
+            if (a.box) {
+                // boxes of 16 tokens, or of 32 where pages hold them; one that no row sees is left out
+                const int  x = (pw.h * (D / 16 * 9) + ph * Ly::rowb) & ~15;
+                const bool one = a.box == 32, b0 = p0 >= 0 || (one && p1 >= 0), b1 = !one && p1 >= 0;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(&rf[st], (b0 + b1) * a.box * Ly::RS);
+                    if (b0) tma_rows(to, isk ? &mk : &mv, x, y0, one ? max(p0, p1) : p0, &rf[st]);
+                    if (b1) tma_rows(to + 16 * Ly::RS, isk ? &mk : &mv, x, y1, p1, &rf[st]);
                 }
-            }
-            f = L == 0.0f ? 0.0f : f / L;
-            x = f != 0.0f ? x * f : 0.0f;
-            uint8_t * dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) (w.r0 + tok) * a.dnb2;
-            if constexpr (PREC) {
-                reinterpret_cast<float *>(dst)[d] = x;
+                __syncwarp();
             } else {
-                reinterpret_cast<__half *>(dst)[d] = __float2half_rn(x);
+                const int64_t o0 = p0 < 0 || p0 >= a.n_pages ? -1 : p0 * pool.nb3 + y0 * pool.nb1 + pw.h * pool.nb2 + ph * Ly::rowb;
+                const int64_t o1 = p1 < 0 || p1 >= a.n_pages ? -1 : p1 * pool.nb3 + y1 * pool.nb1 + pw.h * pool.nb2 + ph * Ly::rowb;
+#pragma unroll 1
+                for (int k = 0; k < 9; k++) {
+                    const int     idx = 32 * k + lane, tk = idx / 9, pc = idx - 9 * tk;
+                    const int64_t s = tk < 16 ? o0 : o1;
+                    q4::copy_async<Ly::CB>(to + tk * Ly::RS + pc * Ly::CB, pool.p + (s < 0 ? 0 : s + (tk & 15) * pool.nb1 + pc * Ly::CB), s < 0 ? 0 : Ly::CB);
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&rf[st])) : "memory");
+            }
+            if (++ph == Ly::SPT) {
+                ph = 0;
+                pi++;
+                look();
+            }
+        };
+        i0 = -16;
+        look();
+        for (int s = 0; s < ST; s++) issue(s);
+        uint32_t gi = 0, use = 0;
+        int      st = 0;
+        for (; active; active = walk_next<N, kTile>(a, w)) {
+            const int n = w.sp.nkv ? w.take : 0;
+            for (int i = 0; i < n; i++, gi++) {
+                const uint32_t kb = gi % KB, c = gi * CH + (CH == 2 ? wq >> 1 : 0), sl = c % VS;
+                const int      tok = w.tile(i) * kTile + 32 * wq + lane;
+                const bool     none = tok < w.sp.lo || tok >= w.sp.hi;  // no row sees it: its V row is zeros, as 0 * NaN is NaN
+#pragma unroll 1
+                for (int h = 0; h < Ly::SPT; h++) {
+                    wait_bar(&rf[st], use & 1, a.status, bad);
+                    __syncwarp();
+                    const uint8_t * row  = raw + st * Ly::stage + lane * Ly::RS;
+                    const int       lead = a.box ? (w.h * (D / 16 * 9) + h * Ly::rowb) & 15 : 0;
+                    uint32_t        W[9];  // of a pair of blocks
+                    [[maybe_unused]] uint32_t X[20];
+                    if constexpr (Ly::HD == 128) {  // the whole row: rows of 80 bytes give 16-byte loads without bank conflicts
+#pragma unroll
+                        for (int e = 0; e < 5; e++) {
+                            const uint4 x = *reinterpret_cast<const uint4 *>(row + 16 * e);
+                            X[4 * e] = x.x; X[4 * e + 1] = x.y; X[4 * e + 2] = x.z; X[4 * e + 3] = x.w;
+                        }
+                    }
+                    auto words = [&](int k) {
+#pragma unroll
+                        for (int e = 0; e < 9; e++) {
+                            if constexpr (Ly::HD == 128) {
+                                W[e] = lead ? X[9 * k + e + 2] : X[9 * k + e];
+                            } else {
+                                W[e] = *reinterpret_cast<const uint32_t *>(row + lead + 4 * e);
+                            }
+                        }
+                    };
+                    if (isk) {
+                        if (h == 0 && gi >= KB) {
+                            wait_bar(&kempty[kb], (gi / KB - 1) & 1, a.status, bad);
+                            tc::fence_after();
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < Ly::HD / 64; k++) {
+                            words(k);
+                            uint32_t       v[16];
+                            const uint32_t at = tc::taddr(tb + Ly::tK + kb * (D / 2) + h * (Ly::HD / 2) + 32 * k, wq, 0);
+                            q4::unpack<false>(W, v);
+                            tc::st16(at, v);
+                            q4::unpack<true>(W, v);
+                            tc::st16(at + 16, v);
+                        }
+                    } else {
+                        if (h == 0 && c >= VS) wait_bar(&vempty[sl], (c / VS - 1) & 1, a.status, bad);
+                        uint8_t * to = sm + Ly::ring + sl * Ly::chunk + ((32 * wq) % Ly::vtok + lane) * 128;
+#pragma unroll
+                        for (int k = 0; k < Ly::HD / 64; k++) {
+                            words(k);
+                            if (none) {
+#pragma unroll
+                                for (int e = 0; e < 9; e++) W[e] = 0;
+                            }
+                            uint8_t * pl = to + (h * (Ly::HD / 64) + k) * (Ly::vtok * 128);
+                            uint32_t  v[16];
+                            auto      put = [&](int c0) {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    *reinterpret_cast<uint4 *>(pl + (((c0 + e) ^ (lane & 7)) << 4)) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                                }
+                            };
+                            q4::unpack<false>(W, v);
+                            put(0);
+                            q4::unpack<true>(W, v);
+                            put(4);
+                        }
+                    }
+                    __syncwarp();
+                    issue(st);
+                    if (++st == ST) {
+                        st = 0;
+                        use++;
+                    }
+                }
+                if (isk) {
+                    tc::wait_st();
+                    tc::fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&kfull[kb]);
+                } else {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&vfull[sl]);
+                }
             }
         }
-        if (tid == 0 && !whole && w.off == 0) {
-            // this CTA opens an item that others go on with: parts of it, for the join
-            const int64_t end = range[0] + (range[1] - range[0] - w.rem) + w.sp.units;
-            int           e   = blockIdx.x;
-            while (range[2] * (e + 1) / range[3] < end) e++;
-            a.desc[2 * blockIdx.x + 1] = make_int4(rb, rows, 0, 0);
-            a.desc[2 * blockIdx.x]     = make_int4(e - (int) blockIdx.x + 1, w.h, w.r0, 0);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        // a wait that gave up: the loads in flight land before this CTA's shared memory goes
+        if (bad && a.box) {
+            for (int s = 0; s < ST; s++) mbar_wait(&rf[s], (use + (s < st)) & 1);
         }
-        active = walk_next<BM, kUnit>(a, w);
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+    tc::fence_before();
+    __syncthreads();
+    if (warp == kSm) tc::tmem_free(tb, 512);
 }
 
-template <int D, int NT, bool PREC>
-int launch_few(srhpm_ctx * ctx, const PArgs & a, const Pool4 & k, const Pool4 & v, cudaStream_t stream) {
-    using Ly = LayF<D, NT, PREC>;
-    auto                         kern = fa_paged_q4_few_kernel<D, NT, PREC>;
+template <int D, int N, bool PREC>
+int launch_t(srhpm_ctx * ctx, const PArgs & a, const CUtensorMap & mk, const CUtensorMap & mv, const Pool4 & k, const Pool4 & v,
+             cudaStream_t stream) {
+    using Ly = LayT<D, N, PREC>;
+    auto                         kern = fa_paged_q4_kernel<D, N, PREC>;
     static std::atomic<unsigned> done{ 0 };
     const unsigned               bit = 1u << (ctx->device & 31);
     if (!(done.load() & bit)) {
@@ -523,21 +862,57 @@ int launch_few(srhpm_ctx * ctx, const PArgs & a, const Pool4 & k, const Pool4 & 
         if (st != SRHPM_OK) return st;
         done.fetch_or(bit);
     }
-    const int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms), dim3(Ly::W * 32), Ly::total, stream, a, k, v));
+    const int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms), dim3(kThr), Ly::total, stream, mk, mv, a, k, v));
     ctx->launches.fetch_add(1);
     if (st != SRHPM_OK) return st;
     return merge_launch(ctx, a, D, PREC, std::min(32, a.prow), stream);
 }
+template <int D>
+int launch_d(srhpm_ctx * ctx, int rows, bool f32, const PArgs & a, const CUtensorMap & mk, const CUtensorMap & mv, const Pool4 & k,
+             const Pool4 & v, cudaStream_t stream) {
+    if (f32) return rows == 16 ? launch_t<D, 16, true>(ctx, a, mk, mv, k, v, stream) : launch_t<D, 64, true>(ctx, a, mk, mv, k, v, stream);
+    return rows == 16   ? launch_t<D, 16, false>(ctx, a, mk, mv, k, v, stream)
+           : rows == 64 ? launch_t<D, 64, false>(ctx, a, mk, mv, k, v, stream)
+                        : launch_t<D, 128, false>(ctx, a, mk, mv, k, v, stream);
+}
 
 }  // namespace
 
-int fap::q4_few_rows(int) { return 8; }
+int fap::q4_rows(int T, int S, int G, bool f32) {
+    const int64_t R = (int64_t) T * G;
+    if (R <= (int64_t) S * 8) return 8;
+    if (R <= (int64_t) S * 16) return 16;
+    if (f32 || R <= (int64_t) S * 64) return 64;
+    return 128;
+}
 
-int fap::q4_few_run(srhpm_ctx * ctx, const PArgs & a, const PagedCache & c, bool f32, cudaStream_t stream) {
+int fap::q4_run(srhpm_ctx * ctx, PArgs & a, const PagedCache & c, int rows, bool f32, cudaStream_t stream) {
     const Pool4 k{ c.k, c.knb1, c.knb2, c.knb3 }, v{ c.v, c.vnb1, c.vnb2, c.vnb3 };
-    if (c.D == 64) return f32 ? launch_few<64, 1, true>(ctx, a, k, v, stream) : launch_few<64, 1, false>(ctx, a, k, v, stream);
-    if (c.D == 128) return f32 ? launch_few<128, 1, true>(ctx, a, k, v, stream) : launch_few<128, 1, false>(ctx, a, k, v, stream);
-    return f32 ? launch_few<256, 1, true>(ctx, a, k, v, stream) : launch_few<256, 1, false>(ctx, a, k, v, stream);
+    CUtensorMap maps[2] = {}, &mk = maps[0], &mv = maps[1];
+    // the few-row kernel takes whole rows of 256 values, this file's half a row at a time
+    const int box = rows == 8 && c.D == 256 ? 144 : row_stride(c.D);
+    // TMA takes the rows where a token's heads stand side by side and tokens and pages start on 16 bytes; other layouts come in
+    // pieces by cp.async
+    const int rowb = c.D / 16 * 9;
+    auto      fits = [&](const Pool4 & p) {
+        return (p.nb2 == rowb || c.Hkv == 1) && c.Hkv * rowb >= box && p.nb1 % 16 == 0 && p.nb3 % 16 == 0 &&
+               reinterpret_cast<uintptr_t>(p.p) % 16 == 0 && p.nb1 >= (int64_t) c.Hkv * rowb;
+    };
+    a.box = 0;
+    if (fits(k) && fits(v)) {
+        a.box = c.page % 32 || (rows == 8 && c.D == 256) ? 16 : 32;  // a step of the few-row kernel has 16 tokens of 256 values
+        for (const Pool4 * p : { &k, &v }) {
+            // a dimension of one element never steps: any valid stride
+            const int64_t s3 = c.n_pages > 1 ? p->nb3 : p->nb1 * c.page;
+            if (!encode_rows(p == &k ? &mk : &mv, p->p, (uint64_t) c.Hkv * rowb, c.page, c.n_pages, p->nb1, s3, box, a.box)) {
+                return SRHPM_ERR_INVALID;
+            }
+        }
+    }
+    if (rows == 8) return q4_few_run(ctx, a, maps, c, f32, stream);
+    if (c.D == 64) return launch_d<64>(ctx, rows, f32, a, mk, mv, k, v, stream);
+    if (c.D == 128) return launch_d<128>(ctx, rows, f32, a, mk, mv, k, v, stream);
+    return launch_d<256>(ctx, rows, f32, a, mk, mv, k, v, stream);
 }
 
 }  // namespace srhpm
