@@ -1118,7 +1118,8 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
 // 36.4 / 38.5 (24 / 4 heads of 256); 4 rows in 9 parts 22.6 / 22.0, 64 in 9 36.5 / 40.9 (32 / 8 heads of 128). Tiles of more
 // rows have 16 CTAs per item: 126 rows in 148 parts 58 / 66. Four records of a lane in flight: 16 took so many registers that the cut items of 18 prompts of 64
 // tokens were joined in 41 us instead of 17.
-template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_merge_kernel(const __grid_constant__ PArgs a) {
+// A CTA looks after the items that `per` parts of the line open (8 where every warp has a part of its own: few of those open one).
+template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_merge_kernel(const __grid_constant__ PArgs a, int per) {
     constexpr int V  = D / 32;  // values per lane, in pairs or fours side by side
     constexpr int VW = V >= 4 ? 4 : 2;
     constexpr int MO = 4;
@@ -1126,11 +1127,11 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
     __shared__ float l_s[8], m_s[8];
     pdl_launch_dependents();
     pdl_wait();
-    const int  c  = blockIdx.x;
-    const int4 d0 = a.desc[2 * c];
-    if (d0.x == 0) return;
-    const int4 d1 = a.desc[2 * c + 1];
-    const int  lane = threadIdx.x & 31, warp = threadIdx.x >> 5, parts = d0.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (uint32_t open = __ballot_sync(0xffffffffu, lane < per && a.desc[2 * (blockIdx.x * per + lane)].x != 0); open; open &= open - 1) {
+    const int  c  = blockIdx.x * per + __ffs(open) - 1;
+    const int4 d0 = a.desc[2 * c], d1 = a.desc[2 * c + 1];
+    const int  parts = d0.x;
     const bool many = 2 * d1.y <= 3 * parts && d1.y <= 64;
     for (int row = many ? blockIdx.y : blockIdx.y * 8 + warp; row < d1.y; row += many ? gridDim.y : gridDim.y * 8) {
         const int tok = a.byG.div(d1.x + row), h = d0.y * a.G + (d1.x + row - tok * a.G);
@@ -1241,6 +1242,7 @@ template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_me
             __syncthreads();
         }
     }
+    }
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -1307,6 +1309,9 @@ int launch_tile(srhpm_ctx * ctx, Tile t, const PArgs & a, const CUtensorMap & mk
     else return launch_paged<D, D <= 128 ? 2 : 1, 128, PREC, Q8>(ctx, a, mk, mv, stream);
 }
 
+// parts that the line of units is cut into on each SM
+int parts_of(int kv_type, Tile t, int D) { return kv_type == SRHPM_TYPE_Q4_0 ? q4_parts(t.br, D) : 1; }
+
 int record_rows(int T, int G, Tile t) { return (int) std::min<int64_t>((int64_t) t.br * t.nt, (int64_t) T * G); }
 
 }  // namespace
@@ -1321,18 +1326,20 @@ bool fap::encode_rows(void * map, const void * p, uint64_t width, int tokens, in
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int fap::merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int rows_y, cudaStream_t stream) {
+int fap::merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int rows_y, cudaStream_t stream, int parts) {
     auto kern = D == 64 ? (f32 ? fa_paged_merge_kernel<64, true> : fa_paged_merge_kernel<64, false>)
                 : D == 128 ? (f32 ? fa_paged_merge_kernel<128, true> : fa_paged_merge_kernel<128, false>)
                            : (f32 ? fa_paged_merge_kernel<256, true> : fa_paged_merge_kernel<256, false>);
-    const int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms, rows_y), dim3(256), 0, stream, a));
+    const int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms * parts / (parts > 1 ? 8 : 1), rows_y), dim3(256), 0, stream, a, parts > 1 ? 8 : 1));
     ctx->launches.fetch_add(1);
     return st;
 }
 
 size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S, int kv_type, bool f32) {
-    const size_t recs = (size_t) 2 * ctx->num_sms * record_rows(T, H / Hkv, tile_of(T, S, H / Hkv, D, kv_type, f32));
-    return recs * D * sizeof(float) + align16(recs * sizeof(float2)) + 2 * (size_t) ctx->num_sms * sizeof(int4) + 32;
+    const Tile   t     = tile_of(T, S, H / Hkv, D, kv_type, f32);
+    const size_t parts = (size_t) ctx->num_sms * parts_of(kv_type, t, D);
+    const size_t recs  = 2 * parts * record_rows(T, H / Hkv, t);
+    return recs * D * sizeof(float) + align16(recs * sizeof(float2)) + 2 * parts * sizeof(int4) + 32;
 }
 
 int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t wsize, cudaStream_t stream) {
@@ -1341,7 +1348,7 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     // a sequence's units per KV head are counted in 32 bits: tiles of 56 rows or more times tiles of 64 tokens or more
     const int64_t seen = std::min<int64_t>((int64_t) v.cols * v.c.page, INT32_MAX);
     if (v.c.type != SRHPM_TYPE_Q4_0 && ((int64_t) v.T * G / kFew + 1) * (seen / 64 + 1) > INT32_MAX) return SRHPM_UNSUPPORTED;
-    if (v.c.type == SRHPM_TYPE_Q4_0 && ((int64_t) v.T * G / 8 + 1) * (seen / 128 + 1) > INT32_MAX) return SRHPM_UNSUPPORTED;
+    if (v.c.type == SRHPM_TYPE_Q4_0 && ((int64_t) v.T * G / 8 + 1) * (seen / 16 + 1) > INT32_MAX) return SRHPM_UNSUPPORTED;
     if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.c.Hkv, D, v.S, v.c.type, v.f32)) return SRHPM_ERR_WORKSPACE;
     const Tile tl = tile_of(v.T, v.S, G, D, v.c.type, v.f32);
     PArgs      a;
@@ -1371,7 +1378,7 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     a.softcap_l2 = v.softcap * kLog2e;
     a.sinks      = v.sinks;
     a.prow       = record_rows(v.T, G, tl);
-    const size_t recs = (size_t) 2 * ctx->num_sms * a.prow;
+    const size_t recs = (size_t) 2 * ctx->num_sms * parts_of(v.c.type, tl, D) * a.prow;
     uint8_t *    wb   = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(wdata) + 31) & ~(uintptr_t) 31);
     a.part_acc = reinterpret_cast<float *>(wb);
     a.part_ms  = reinterpret_cast<float2 *>(wb + recs * D * sizeof(float));

@@ -118,11 +118,9 @@ template <int BMN, int BN> __device__ __forceinline__ bool walk_next(const PArgs
     return true;
 }
 
-// This CTA's part of the line of units, taken by all of its threads: first = {s, h, rt, off} of its first unit (s stays as it
-// was, -1, for an empty part), range = {start, end, units in all, parts}. tot: 2 a.S words of scratch, nbg one; all four in
-// shared memory. Ends without a barrier.
-template <int BMN, int BN>
-__device__ __forceinline__ void plan_part(const PArgs & a, int * tot, int * nbg, int * first, int64_t * range) {
+// Units per KV head of each sequence into tot, by all of the CTA's threads. tot: 2 a.S words of scratch, nbg one, both in shared
+// memory. Ends with a barrier.
+template <int BMN, int BN> __device__ __forceinline__ void plan_sums(const PArgs & a, int * tot, int * nbg) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int * big = tot + a.S;  // sequences whose tiles a warp sums up
     if (tid == 0) *nbg = 0;
@@ -147,71 +145,101 @@ __device__ __forceinline__ void plan_part(const PArgs & a, int * tot, int * nbg,
         if (lane == 0) tot[s] = u;
     }
     __syncthreads();
-    if (warp == 0) {
-        int64_t sum = 0;
-        for (int s = lane; s < a.S; s += 32) sum += tot[s];
+}
+
+// Part `part` of `parts` of the line of units, found by one warp: its first unit (s = -1: the part is empty), its place in the
+// line, the units and the parts in all
+struct Part {
+    int     s, h, rt, off;
+    int64_t b0, b1, all, parts;
+};
+template <int BMN, int BN> __device__ __forceinline__ Part plan_find(const PArgs & a, const int * tot, int part, int parts) {
+    const int lane = threadIdx.x & 31;
+    Part      p;
+    p.s = -1;
+    int64_t sum = 0;
+    for (int s = lane; s < a.S; s += 32) sum += tot[s];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        // fewer units than CTAs: one each for the first W, so that an item's parts stand in neighbouring CTAs
-        const int64_t W = sum * a.Hkv, np = max((int64_t) 1, min((int64_t) gridDim.x, W)), c = min((int64_t) blockIdx.x, np);
-        const int64_t b0 = W * c / np, b1 = W * min(c + 1, np) / np;
-        if (lane == 0) {
-            range[0] = b0;
-            range[1] = b1;
-            range[2] = W;
-            range[3] = np;
-        }
-        if (b1 > b0) {
-            int64_t before = 0;
-            for (int s0 = 0; s0 < a.S; s0 += 32) {
-                const int64_t v   = s0 + lane < a.S ? (int64_t) tot[s0 + lane] * a.Hkv : 0;
-                int64_t       inc = v;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    // fewer units than parts: one each for the first W, so that an item's parts stand side by side
+    const int64_t W = sum * a.Hkv, np = max((int64_t) 1, min((int64_t) parts, W)), c = min((int64_t) part, np);
+    const int64_t b0 = W * c / np, b1 = W * min(c + 1, np) / np;
+    p.b0    = b0;
+    p.b1    = b1;
+    p.all   = W;
+    p.parts = np;
+    if (b1 > b0) {
+        int64_t before = 0;
+        for (int s0 = 0; s0 < a.S; s0 += 32) {
+            const int64_t v   = s0 + lane < a.S ? (int64_t) tot[s0 + lane] * a.Hkv : 0;
+            int64_t       inc = v;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
-                    if (lane >= o) inc += x;
-                }
-                const int64_t  end = before + inc, beg = end - v;
-                const uint32_t hit = __ballot_sync(0xffffffffu, b0 >= beg && b0 < end);
-                if (hit) {
-                    const int     src = __ffs(hit) - 1, s = s0 + src;
-                    const int64_t in  = b0 - __shfl_sync(0xffffffffu, beg, src);
-                    const int     per = tot[s];
-                    const int     h   = (int) (in / per);
-                    int           off = (int) (in - (int64_t) h * per);
-                    const int     r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = max(a.kv_len[s], 0);
-                    for (int t0 = 0; t0 < nt; t0 += 32) {
-                        const int u  = t0 + lane < nt ? span_of<BMN, BN>(a, n, kv, t0 + lane).units : 0;
-                        int       ic = u;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t x = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += x;
+            }
+            const int64_t  end = before + inc, beg = end - v;
+            const uint32_t hit = __ballot_sync(0xffffffffu, b0 >= beg && b0 < end);
+            if (hit) {
+                const int     src = __ffs(hit) - 1, s = s0 + src;
+                const int64_t in  = b0 - __shfl_sync(0xffffffffu, beg, src);
+                const int     per = tot[s];
+                const int     h   = (int) (in / per);
+                int           off = (int) (in - (int64_t) h * per);
+                const int     r0 = row_at(a, s), n = row_at(a, s + 1) - r0, nt = tiles_of<BMN>(a, n), kv = max(a.kv_len[s], 0);
+                for (int t0 = 0; t0 < nt; t0 += 32) {
+                    const int u  = t0 + lane < nt ? span_of<BMN, BN>(a, n, kv, t0 + lane).units : 0;
+                    int       ic = u;
 #pragma unroll
-                        for (int o = 1; o < 32; o <<= 1) {
-                            const int x = __shfl_up_sync(0xffffffffu, ic, o);
-                            if (lane >= o) ic += x;
-                        }
-                        const uint32_t ht = __ballot_sync(0xffffffffu, off >= ic - u && off < ic);
-                        if (ht) {
-                            const int l = __ffs(ht) - 1;
-                            off -= __shfl_sync(0xffffffffu, ic - u, l);
-                            if (lane == 0) {
-                                first[0] = s;
-                                first[1] = h;
-                                first[2] = t0 + l;
-                                first[3] = off;
-                            }
-                            break;
-                        }
-                        off -= __shfl_sync(0xffffffffu, ic, 31);
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const int x = __shfl_up_sync(0xffffffffu, ic, o);
+                        if (lane >= o) ic += x;
                     }
-                    break;
+                    const uint32_t ht = __ballot_sync(0xffffffffu, off >= ic - u && off < ic);
+                    if (ht) {
+                        const int l = __ffs(ht) - 1;
+                        off -= __shfl_sync(0xffffffffu, ic - u, l);
+                        p.s   = s;
+                        p.h   = h;
+                        p.rt  = t0 + l;
+                        p.off = off;
+                        break;
+                    }
+                    off -= __shfl_sync(0xffffffffu, ic, 31);
                 }
-                before = __shfl_sync(0xffffffffu, end, 31);
+                break;
+            }
+            before = __shfl_sync(0xffffffffu, end, 31);
+        }
+    }
+    return p;
+}
+
+// This CTA's part of the line, as one of gridDim.x: first = {s, h, rt, off} (s stays as it was, -1, for an empty part), range =
+// {start, end, units in all, parts}, both in shared memory. Ends without a barrier.
+template <int BMN, int BN>
+__device__ __forceinline__ void plan_part(const PArgs & a, int * tot, int * nbg, int * first, int64_t * range) {
+    plan_sums<BMN, BN>(a, tot, nbg);
+    if (threadIdx.x < 32) {
+        const Part p = plan_find<BMN, BN>(a, tot, blockIdx.x, gridDim.x);
+        if (threadIdx.x == 0) {
+            range[0] = p.b0;
+            range[1] = p.b1;
+            range[2] = p.all;
+            range[3] = p.parts;
+            if (p.s >= 0) {
+                first[0] = p.s;
+                first[1] = p.h;
+                first[2] = p.rt;
+                first[3] = p.off;
             }
         }
     }
 }
 
-// over q4_0 pages: rows of a tile (fa_paged_q4.cu)
+// over q4_0 pages: rows of a tile, parts that the line is cut into on each SM (fa_paged_q4.cu)
 int q4_rows(int T, int S, int G, bool f32);
+int q4_parts(int rows, int D);
 int q4_few_run(srhpm_ctx * ctx, const PArgs & a, const void * maps, const PagedCache & c, bool f32, cudaStream_t stream);  // fa_paged_q4_few.cu
 int q4_run(srhpm_ctx * ctx, PArgs & a, const PagedCache & c, int rows, bool f32, cudaStream_t stream);
 
@@ -219,7 +247,7 @@ int q4_run(srhpm_ctx * ctx, PArgs & a, const PagedCache & c, int rows, bool f32,
 bool encode_rows(void * map, const void * p, uint64_t width, int tokens, int64_t pages, int64_t nb1, int64_t nb3, int box, int tokens_box);
 
 // the records' join behind a kernel that cut items (fa_paged.cu)
-int merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int rows_y, cudaStream_t stream);
+int merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int rows_y, cudaStream_t stream, int parts = 1);  // parts: of an SM
 
 inline size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 

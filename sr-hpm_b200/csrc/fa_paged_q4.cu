@@ -886,6 +886,8 @@ int fap::q4_rows(int T, int S, int G, bool f32) {
     return 128;
 }
 
+int fap::q4_parts(int rows, int D) { return rows == 8 ? (D == 256 ? 8 : 16) : 1; }
+
 int fap::q4_run(srhpm_ctx * ctx, PArgs & a, const PagedCache & c, int rows, bool f32, cudaStream_t stream) {
     const Pool4 k{ c.k, c.knb1, c.knb2, c.knb3 }, v{ c.v, c.vnb1, c.vnb2, c.vnb3 };
     CUtensorMap maps[2] = {}, &mk = maps[0], &mv = maps[1];

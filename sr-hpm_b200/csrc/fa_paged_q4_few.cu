@@ -14,11 +14,10 @@
 //                  f32 rows (PREC): Q and P as sums of two f16 parts; a step's part of O is summed up apart and then added, as
 //                  the tensor cores' sums are truncated (a shrink of 2^-25 per product, measured: 2e-5 after 400)
 //
-// Work: the line of all items' units is cut into equal parts, one per CTA (plan_part). The CTA's warps share an item's steps
-// of TS tokens out, every W-th each, with rings of their own that TMA fills (row boxes of 16-byte multiples, so that a row may
-// start up to 12 bytes into its place; layouts that TMA does not take come by cp.async, 9 pieces of D / 16 bytes a row). Rows
-// of 48, 80 and 144 bytes make every load from the ring free of bank conflicts. At an item's end the warps' sums are joined in
-// shared memory.
+// Work: the line of all items' units of TS tokens is cut into equal parts, one per warp: every warp is by itself from the plan on, with
+// a ring that TMA fills (row boxes of 16-byte multiples, so that a row may start up to 12 bytes into its place; layouts that TMA
+// does not take come by cp.async, 9 pieces of D / 16 bytes a row) and records of its own. Rows of 48, 80 and 144 bytes make
+// every load from the ring free of bank conflicts.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -37,8 +36,6 @@ namespace srhpm {
 using namespace fap;
 namespace {
 
-constexpr int kUnit = 128;  // tokens of a unit of work
-
 struct Pool4 {
     const uint8_t * p;
     int64_t         nb1, nb2, nb3;
@@ -51,24 +48,20 @@ template <int D, bool PREC> struct LayF {
     static constexpr int BM    = 8;                    // rows of a tile
     static constexpr int TS    = D == 256 ? 16 : 32;   // tokens of a step
     static constexpr int W     = D == 256 ? 8 : 16;    // warps: O takes D / 4 registers of a lane
-    static constexpr int JW    = 8;                    // warps whose sums are joined at once
     static constexpr int rowb  = D / 16 * 9;
     static constexpr int CB    = D / 16;               // bytes of a copy
     static constexpr int RS    = row_stride(D);
     static constexpr int stage = 2 * TS * RS;          // K rows, V rows
     static constexpr int parts = PREC ? 2 : 1;
-    static constexpr int pad   = D + 4;
-    static constexpr int q     = 0;                                   // [2][parts][D / 32][32] uint4
-    static constexpr int qset  = parts * (D / 32) * 512;
-    static constexpr int part  = q + 2 * qset;                        // f32 [JW][BM][pad]
-    static constexpr int ms    = part + JW * BM * pad * 4;            // float2 [JW][BM]
-    static constexpr int misc  = ms + JW * BM * 8;
-    static constexpr int bar   = misc + 64;
-    static constexpr int ring  = (bar + W * 4 * 8 + 127) / 128 * 128;
+    static constexpr int qset  = parts * (D / 32) * 512;              // of a warp: [parts][D / 32][32] uint4
+    static constexpr int bar   = 0;
+    static constexpr int misc  = W * 4 * 8;
+    static constexpr int q     = (misc + 16 + 127) / 128 * 128;
+    static constexpr int ring  = q + W * qset;
     static constexpr int room  = 232448 - ring;
     static constexpr int ST    = room / (W * stage) < 4 ? room / (W * stage) : 4;
     static constexpr int total = ring + ST * W * stage;
-    static_assert(ST >= 2 && ST * W * stage >= kMaxSeqs * 8, "shared memory");
+    static_assert(ST >= 2 && ring % 128 == 0 && ST * W * stage >= kMaxSeqs * 8, "shared memory");
 };
 
 __device__ __forceinline__ bool elect_one() {
@@ -98,17 +91,20 @@ __device__ __forceinline__ float exp2a(float x) {
     return r;
 }
 
-// an item's tokens in this CTA
+// an item's steps in this warp: steps t0 + TS u, u = rot, rot + 1 .. n - 1, 0 .. rot - 1
 struct Run {
-    int t0, n;  // first token (a multiple of TS), steps
+    int t0, n, rot;
 };
-template <int TS> __device__ __forceinline__ Run run_of(const Walk & w) {
-    Run r{ 0, 0 };
+// Heads of one sequence stand side by side in the cache, a row of 36 to 144 bytes each, and memory gives 64 bytes at least: what one head
+// leaves of them another should find in L2. So a warp begins its part where its step's number is a multiple of the parts'
+// length, and all heads come to a token at about the same time.
+template <int TS> __device__ __forceinline__ Run run_of(const Walk & w, int period) {
+    Run r{ 0, 0, 0 };
     if (w.sp.nkv) {
-        const int b = (w.sp.kt0 + w.off) * kUnit;
-        const int e = min(b + w.take * kUnit, w.sp.hi);
-        r.t0        = max(b, w.sp.lo) & ~(TS - 1);
-        r.n         = (e - r.t0 + TS - 1) / TS;
+        r.t0 = (w.sp.kt0 + w.off) * TS;
+        r.n  = w.take;
+        r.rot = (period - w.off % period) % period;
+        if (r.rot >= r.n) r.rot = 0;
     }
     return r;
 }
@@ -125,63 +121,65 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
     constexpr int MT   = TS / 16;
     constexpr int NG   = D / 64;
     constexpr int CB   = Ly::CB;
-    constexpr int JW   = Ly::JW;
     constexpr int RS   = Ly::RS;
     constexpr int GP   = TS / 16;  // 16-token groups of a step
     constexpr int rowb = Ly::rowb;
-    extern __shared__ __align__(16) uint8_t sm[];
-    float *   part  = reinterpret_cast<float *>(sm + Ly::part);
-    float2 *  ms    = reinterpret_cast<float2 *>(sm + Ly::ms);
-    int *     first = reinterpret_cast<int *>(sm + Ly::misc);
-    int64_t * range = reinterpret_cast<int64_t *>(sm + Ly::misc + 16);
+    extern __shared__ __align__(128) uint8_t sm[];
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    uint64_t * full = reinterpret_cast<uint64_t *>(sm + Ly::bar) + warp * ST;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, part = blockIdx.x * W + warp;
+    uint64_t * full = reinterpret_cast<uint64_t *>(sm + Ly::bar) + warp * 4;
     bool       bad  = false;
-    if (tid == 0) first[0] = -1;
     if (lane == 0) {
         for (int i = 0; i < ST; i++) mbar_init(&full[i], a.box ? 1 : 32);
         fence_mbar_init();
     }
+    if (tid == 0 && a.box) {
+        prefetch_tmap(&mk);
+        prefetch_tmap(&mv);
+    }
     pdl_launch_dependents();
     pdl_wait();
-    plan_part<BM, kUnit>(a, reinterpret_cast<int *>(sm + Ly::ring), reinterpret_cast<int *>(sm + Ly::ms), first, range);
-    __syncthreads();
-    if (tid == 0) a.desc[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+    int * tot = reinterpret_cast<int *>(sm + Ly::ring);
+    plan_sums<BM, TS>(a, tot, reinterpret_cast<int *>(sm + Ly::misc));
+    const Part pt = plan_find<BM, TS>(a, tot, part, gridDim.x * W);
+    __syncthreads();  // the ring is free; no warp waits for another from here on
+    if (lane == 0) a.desc[2 * part] = make_int4(0, 0, 0, 0);
+    if (pt.s < 0) return;
+    const int period = (int) min((pt.all + pt.parts - 1) / pt.parts, (int64_t) 1 << 30);
     Walk w;
-    w.s = first[0];
-    if (w.s < 0) return;
-    w.h   = first[1];
-    w.rt  = first[2];
-    w.off = first[3];
-    w.rem = w.part = range[1] - range[0];
+    w.s   = pt.s;
+    w.h   = pt.h;
+    w.rt  = pt.rt;
+    w.off = pt.off;
+    w.rem = w.part = pt.b1 - pt.b0;
     walk_load<BM>(a, w);
-    walk_item<BM, kUnit>(a, w);
+    walk_item<BM, TS>(a, w);
 
     // ---- this warp's copies, up to ST steps ahead of its products, across items ----
     Walk pw   = w;
-    Run  prun = run_of<TS>(pw);
-    int  pst  = warp;  // step of the item
+    Run  prun = run_of<TS>(pw, period);
+    int  pst  = 0;  // step of the item
     bool pact = true;
-    // lane j: page of the 16-token group j % GP of the (j / GP)-th of this warp's steps from step i0 on: asked for step by step, an entry's
-    // 700 cycles held the warp up each time
+    // lane j: page of the 16-token group j % GP of the (j / GP)-th step from i0 on: asked for step by step, an entry's 700 cycles held
+    // the warp up each time
+    auto step_at = [](const Run & r, int i) { return r.t0 + (i + r.rot < r.n ? i + r.rot : i + r.rot - r.n) * TS; };
     int            ent = -1, i0 = 0;
     const uint32_t ring0 = smem_u32(sm + Ly::ring + warp * (ST * Ly::stage));
     auto           look  = [&](bool fresh) {
-        fresh |= pst - i0 >= 32 / GP * W;
+        fresh |= pst - i0 >= 32 / GP;
         while (pact && pst >= prun.n) {
-            pact = walk_next<BM, kUnit>(a, pw);
+            pact = walk_next<BM, TS>(a, pw);
             if (pact) {
-                prun  = run_of<TS>(pw);
-                pst   = warp;
+                prun  = run_of<TS>(pw, period);
+                pst   = 0;
                 fresh = true;
             }
         }
         if (pact && fresh) {
             i0            = pst;
             ent           = -1;
-            const int tok = prun.t0 + (pst + lane / GP * W) * TS + 16 * (lane % GP);
-            if (tok < pw.sp.hi && tok + 16 > pw.sp.lo) {
+            const int tok = step_at(prun, pst + lane / GP) + 16 * (lane % GP);
+            if (pst + lane / GP < prun.n && tok < pw.sp.hi && tok + 16 > pw.sp.lo) {
                 ent = reinterpret_cast<const int32_t *>(a.table + (int64_t) pw.s * a.tstride)[a.byPage.div(tok)];
                 if (ent < 0 || ent >= a.n_pages) {  // no page: reads as zeros
                     atomicExch(a.status, kErrPage);
@@ -193,7 +191,7 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
     auto issue = [&](int stage) {
         if (!pact) return;
         const uint32_t to = ring0 + stage * Ly::stage;
-        const int      t0 = prun.t0 + pst * TS, at = (pst - i0) / W * GP;
+        const int      t0 = step_at(prun, pst), at = (pst - i0) * GP;
         int            p[GP], y[GP];  // page (-1: no row sees the group) and place
 #pragma unroll
         for (int k = 0; k < GP; k++) {
@@ -232,21 +230,22 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
             }
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[stage])) : "memory");
         }
-        pst += W;
+        pst++;
         look(false);
     };
     look(true);
     for (int s = 0; s < ST; s++) issue(s);
 
     const uint32_t selv = g == 3 ? 0x1076u : 0x3210u, selk = t == 3 ? 0x1076u : 0x3210u, seld = g < 4 ? 0x5410u : 0x7632u;
-    int            stage = 0, use = 0, par = 0;
-    for (bool active = true; active; par ^= 1) {
+    int            stage = 0, use = 0;
+    for (bool active = true; active;) {
         const int n  = w.n * a.G, rb = w.rt * BM, rows = min(BM, n - rb);
-        const Run run = run_of<TS>(w);
+        const Run run = run_of<TS>(w, period);
         // ---- Q, in the order of K's lanes; rows that are none as zeros ----
-        uint4 * qb = reinterpret_cast<uint4 *>(sm + Ly::q + par * Ly::qset);
-        for (int u = tid; u < (D / 32) * 32; u += W * 32) {
-            const int ln = u & 31, blk = u >> 5, row = ln >> 2, tt = ln & 3;
+        uint4 * qb = reinterpret_cast<uint4 *>(sm + Ly::q + warp * Ly::qset);
+#pragma unroll 2
+        for (int blk = 0; blk < D / 32; blk++) {
+            const int u = 32 * blk + lane, row = g, tt = t;
             float     x[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) x[e] = 0.0f;
@@ -299,10 +298,10 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
                 for (int e = 0; e < 4; e++) o[i][b][e] = 0.0f;
             }
         }
-        __syncthreads();
+        __syncwarp();
         const uint4 * ql   = qb + lane;
         const int     lead = a.box ? (w.h * rowb) & 15 : 0;
-        for (int st = warp; st < run.n; st += W) {
+        for (int st = 0; st < run.n; st++) {
             if (!bad) {
                 uint32_t i = 0;
                 while (i < kProbes && !mbar_try_wait(&full[stage], use & 1)) i++;
@@ -314,7 +313,7 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
             __syncwarp();
             const uint8_t * kr = sm + Ly::ring + warp * (ST * Ly::stage) + stage * Ly::stage + lead;
             const uint8_t * vr = kr + TS * RS;
-            const int       tb   = run.t0 + st * TS;
+            const int       tb   = step_at(run, st);
             const bool      mask = tb < alo || tb + TS > ahi;
             float           s[MT][4];
 #pragma unroll
@@ -428,7 +427,13 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
                         const uint32_t * row = reinterpret_cast<const uint32_t *>(vr + tk * RS + 36 * gq);
                         y[k]                 = row[g < 4 ? 0 : 4];
                         v[k]                 = q4::prmt(row[1 + g], y[k], selv);
-                        if (edge && (tb + tk < w.sp.lo || tb + tk >= w.sp.hi)) y[k] = v[k] = 0;
+                    }
+                    if (edge) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const int tok = tb + 16 * i + 2 * t + (k & 1) + 8 * (k >> 1);
+                            if (tok < w.sp.lo || tok >= w.sp.hi) y[k] = v[k] = 0;
+                        }
                     }
                     const uint32_t d0 = q4::prmt(y[0], y[1], seld), d1 = q4::prmt(y[2], y[3], seld);
 #pragma unroll
@@ -458,106 +463,66 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
                 use++;
             }
         }
-        // ---- the item's end: the warps' sums side by side; of 16 warps the upper half's go to the lower half first ----
+        // ---- the item's end: a lane has rows 2 t, 2 t + 1, of each pair of blocks the numbers of its word ----
+        const bool whole = w.off == 0 && w.take == w.sp.units;
+        const int  slot  = 2 * part + (w.off == 0 ? 1 : 0);
 #pragma unroll
         for (int k = 0; k < 2; k++) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l[k] += __shfl_xor_sync(0xffffffffu, l[k], d);
-        }
-        float2 *   mw = ms + (warp & (JW - 1)) * BM;
-        float *    pw_o = part + (warp & (JW - 1)) * BM * Ly::pad;
-        const bool some = warp < run.n;
-        auto       each = [&](auto f) {  // f(row's value in the area, own value, its row's place in m and l)
+            const int row = 2 * t + k;
+            if (row >= rows) continue;
+            const int tok = a.byG.div(rb + row), h = w.h * a.G + (rb + row - tok * a.G);
+            float     f   = 1.0f;
+            if (whole) {
+                float L = l[k];
+                if (a.sinks) {  // relative to the larger of the two maxima
+                    const float sk = a.sinks[h] * kLog2e;
+                    if (sk > m[k]) {
+                        f = m[k] == -INFINITY ? 0.0f : exp2a(m[k] - sk);
+                        L = L * f + exp2f(kShift);
+                    } else if (sk > -INFINITY) {
+                        L += exp2a(sk - m[k] + kShift);
+                    }
+                }
+                f = L == 0.0f ? 0.0f : f / L;  // a NaN stays one
+            } else if (g == 0) {
+                a.part_ms[(int64_t) slot * a.prow + row] = make_float2(m[k], l[k]);
+            }
+            uint8_t * dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) (w.r0 + tok) * a.dnb2;
+            float *   acc = a.part_acc + ((int64_t) slot * a.prow + row) * D;
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
+            for (int gq = 0; gq < NG; gq++) {
 #pragma unroll
-                for (int gq = 0; gq < NG; gq++) {
+                for (int b = 0; b < 4; b += 2) {
 #pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        float * to = pw_o + (2 * t + k) * Ly::pad + 64 * gq + 32 * (g >> 2) + q4::byte_of(g >= 4, g & 3, b);
-                        f(to[0], o[gq][b][k], k);
-                        f(to[16], o[gq][b][2 + k], k);
+                    for (int hi = 0; hi < 2; hi++) {
+                        const int d = 64 * gq + 32 * (g >> 2) + q4::byte_of(g >= 4, g & 3, b) + 16 * hi;
+                        float2    x = make_float2(o[gq][b][2 * hi + k], o[gq][b + 1][2 * hi + k]);
+                        if (!whole) {
+                            *reinterpret_cast<float2 *>(acc + d) = x;
+                            continue;
+                        }
+                        x = f != 0.0f ? make_float2(x.x * f, x.y * f) : make_float2(0.0f, 0.0f);
+                        if constexpr (PREC) {
+                            *reinterpret_cast<float2 *>(dst + 4 * d) = x;
+                        } else {
+                            *reinterpret_cast<__half2 *>(dst + 2 * d) = __floats2half2_rn(x.x, x.y);
+                        }
                     }
                 }
             }
-        };
-        auto leave = [&]() {
-            if (g == 0) {
-                mw[2 * t]     = make_float2(m[0], l[0]);
-                mw[2 * t + 1] = make_float2(m[1], l[1]);
-            }
-            if (some) each([](float & to, float & x, int) { to = x; });
-        };
-        if constexpr (W > JW) {
-            if (warp >= JW) leave();
-            __syncthreads();
-            if (warp < JW && warp + JW < run.n) {
-                float fo[2], ft[2];
-#pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const float2 r = mw[2 * t + k];
-                    const float  M = fmaxf(m[k], r.x);
-                    fo[k]          = m[k] == -INFINITY ? (l[k] == 0.0f ? 0.0f : 1.0f) : exp2a(m[k] - M);  // NaN weights stay
-                    ft[k]          = r.x == -INFINITY ? (r.y == 0.0f ? 0.0f : 1.0f) : exp2a(r.x - M);
-                    l[k]           = l[k] * fo[k] + r.y * ft[k];
-                    m[k]           = M;
-                }
-                each([&](float & to, float & x, int k) { x = x * fo[k] + to * ft[k]; });
-            }
-            __syncwarp();
         }
-        if (warp < JW) leave();
-        __syncthreads();
-        const bool whole = w.off == 0 && w.take == w.sp.units;
-        const int  slot  = 2 * blockIdx.x + (w.off == 0 ? 1 : 0);
-        for (int u = tid; u < rows * D; u += W * 32) {
-            const int row = u / D, d = u % D;
-            float     M = -INFINITY, L = 0.0f, x = 0.0f;
-#pragma unroll
-            for (int k = 0; k < JW; k++) M = fmaxf(M, ms[k * BM + row].x);
-#pragma unroll
-            for (int k = 0; k < JW; k++) {
-                const float2 r = ms[k * BM + row];
-                if (!(r.y == 0.0f)) {  // a warp without weight may have left anything; a NaN stays one
-                    const float wt = exp2a(r.x == -INFINITY && M == -INFINITY ? 0.0f : r.x - M);
-                    L += wt * r.y;
-                    x += wt * part[(k * BM + row) * Ly::pad + d];
-                }
-            }
-            if (!whole) {
-                a.part_acc[((int64_t) slot * a.prow + row) * D + d] = x;
-                if (d == 0) a.part_ms[(int64_t) slot * a.prow + row] = make_float2(M, L);
-                continue;
-            }
-            const int tok = a.byG.div(rb + row), h = w.h * a.G + (rb + row - tok * a.G);
-            float     f = 1.0f;
-            if (a.sinks) {  // relative to the larger of the two maxima
-                const float sk = a.sinks[h] * kLog2e;
-                if (sk > M) {
-                    f = M == -INFINITY ? 0.0f : exp2a(M - sk);
-                    L = L * f + exp2f(kShift);
-                } else if (sk > -INFINITY) {
-                    L += exp2a(sk - M + kShift);
-                }
-            }
-            f = L == 0.0f ? 0.0f : f / L;
-            x = f != 0.0f ? x * f : 0.0f;
-            uint8_t * dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) (w.r0 + tok) * a.dnb2;
-            if constexpr (PREC) {
-                reinterpret_cast<float *>(dst)[d] = x;
-            } else {
-                reinterpret_cast<__half *>(dst)[d] = __float2half_rn(x);
-            }
+        if (lane == 0 && !whole && w.off == 0) {
+            // this warp opens an item that others go on with: parts of it, for the join
+            const int64_t end = pt.b0 + (pt.b1 - pt.b0 - w.rem) + w.sp.units;
+            int           e   = part;
+            while (pt.all * (e + 1) / pt.parts < end) e++;
+            a.desc[2 * part + 1] = make_int4(rb, rows, 0, 0);
+            a.desc[2 * part]     = make_int4(e - part + 1, w.h, w.r0, 0);
         }
-        if (tid == 0 && !whole && w.off == 0) {
-            // this CTA opens an item that others go on with: parts of it, for the join
-            const int64_t end = range[0] + (range[1] - range[0] - w.rem) + w.sp.units;
-            int           e   = blockIdx.x;
-            while (range[2] * (e + 1) / range[3] < end) e++;
-            a.desc[2 * blockIdx.x + 1] = make_int4(rb, rows, 0, 0);
-            a.desc[2 * blockIdx.x]     = make_int4(e - (int) blockIdx.x + 1, w.h, w.r0, 0);
-        }
-        active = walk_next<BM, kUnit>(a, w);
+        __syncwarp();  // Q is read
+        active = walk_next<BM, TS>(a, w);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     // a wait that gave up: the loads in flight land before this CTA's shared memory goes
@@ -581,7 +546,7 @@ int launch_few(srhpm_ctx * ctx, const PArgs & a, const CUtensorMap & mk, const C
     const int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms), dim3(Ly::W * 32), Ly::total, stream, mk, mv, a, k, v));
     ctx->launches.fetch_add(1);
     if (st != SRHPM_OK) return st;
-    return merge_launch(ctx, a, D, PREC, std::min(32, a.prow), stream);
+    return merge_launch(ctx, a, D, PREC, std::min(4, a.prow), stream, Ly::W);
 }
 
 }  // namespace
