@@ -1,11 +1,15 @@
 // Rules on the logits of the rows that a step scores (srhpm_adjust_logits): biases of single tokens, penalties for tokens
 // that the sequence has said already, and token masks.
 //
-// A row is a copy with a few changed places, so the copy is what costs: 8 bytes per logit (with out = logits only what a mask
-// takes away is written). A CTA has one row's slice of kSlice tokens: it loads the slice into registers, counts the window's
-// tokens that fall into the slice in shared memory meanwhile, writes the slice with the mask applied, and then goes through
-// the window and the biases once more: the first visitor of a token takes its count and writes its value. No sort, no hash, and the same
-// result whatever the order of the atomics: counts are whole numbers, and a token that is biased twice takes the later value.
+// A row is a copy with a few changed places, so the copy is what costs: 8 bytes per logit (with out = logits a row without a mask is
+// touched only where a rule changes it). A CTA has a slice of kSlice tokens, of all rows of a sequence one after another where there are sequences enough,
+// else of one row. The window's tokens that fall into the slice are counted in shared memory once per CTA; a warp has the same 512
+// tokens of every row, lists those with a rule once, and from then on waits for no other: a row comes in, goes through the warp's
+// shared memory, where 32 listed tokens at a time take their values, and out with the mask applied. From one row to the next the window
+// moves by a token. (64 sequences: each row's window counted anew in each of its slices 201 us; listed tokens fetched and written behind the
+// copy 154; barriers of the CTA around the listed tokens 142; rules applied by the lane that holds the token 180.)
+// The result does not hang on the order of the atomics: counts are whole numbers, and a token that is biased twice takes the
+// later value.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -17,42 +21,59 @@
 namespace srhpm {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kSlice   = 8192;
+constexpr int kThreads = 256;
+constexpr int kSlice   = 4096;
 constexpr int kVec     = kSlice / kThreads / 4;  // groups of four of a thread
+constexpr int kWarpTok = 128 * kVec;             // tokens of a warp
+constexpr uint32_t kListed = 1u << 31;           // beside a token's count
+constexpr int kSmem = kSlice * 14;
 
 struct Args {
     LogitView v;
-    int       slices;
+    int       slices, by_seq;
 };
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads) adjust_logits_kernel(const __grid_constant__ Args a) {
-    extern __shared__ uint32_t sh[];
-    uint32_t * cnt = sh;           // [kSlice] times in the window
-    uint32_t * bix = sh + kSlice;  // [kSlice] 1 + index of the token's bias
+__global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(const __grid_constant__ Args a) {
+    static_assert(kVec == 4, "a thread's 16 tokens");
+    extern __shared__ __align__(16) uint32_t cnt[];               // [kSlice] times in the window, kListed
+    uint32_t * bix  = cnt + kSlice;                               // [kSlice] 1 + index of the token's bias, then its value
+    float *    xs   = reinterpret_cast<float *>(bix + kSlice);    // [kSlice] the row
+    uint16_t * list = reinterpret_cast<uint16_t *>(xs + kSlice) + (threadIdx.x >> 5) * kWarpTok;
     const LogitView & v = a.v;
-    const int         tid = threadIdx.x;
-    const int         row = blockIdx.x / a.slices, x0 = (blockIdx.x - row * a.slices) * kSlice, nx = min(kSlice, v.V - x0);
+    const int         tid = threadIdx.x, lane = tid & 31, w0 = (tid >> 5) * kWarpTok;
+    const int         unit = blockIdx.x / a.slices, x0 = (blockIdx.x - unit * a.slices) * kSlice, nx = min(kSlice, v.V - x0);
     pdl_launch_dependents();
     pdl_wait();
-    const int rows = v.q_start[v.S];
-    if (row >= rows) return;  // padding
-    const float * in  = reinterpret_cast<const float *>(v.logits + (int64_t) row * v.ldb) + x0;
-    float *       out = reinterpret_cast<float *>(v.out + (int64_t) row * v.ldo) + x0;
-    const bool    same = in == out;
-    const uint32_t * mask = nullptr;
-    if (v.mask) {
-        const int mr = v.mask_row ? v.mask_row[row] : row;
-        if (mr >= 0 && mr < v.n_masks) mask = reinterpret_cast<const uint32_t *>(v.mask + (int64_t) mr * v.ldm) + x0 / 32;
+    int s, r0, r1, first;
+    if (a.by_seq) {
+        s     = unit;
+        first = max(v.q_start[s], 0);
+        r0    = first;
+        r1    = min(v.q_start[s + 1], v.T);
+    } else {
+        r0 = unit;
+        r1 = r0 + 1;
+        if (r0 >= v.q_start[v.S]) return;  // padding
+        s = -1;
+        for (int i0 = 0; i0 < v.S; i0 += kThreads) s += __syncthreads_count(i0 + tid < v.S && v.q_start[i0 + tid] <= r0);
+        if (s < 0) return;
+        first = max(v.q_start[s], 0);
     }
-    // the slice: group i of a thread has tokens 4 (i kThreads + tid) ..
-    float4     x[kVec];
-    const bool pass = !same || mask;
-    if (pass) {
+    if (r0 >= r1) return;
+    const bool same = v.logits == v.out;
+    float4     x[kVec];  // group i of a lane has tokens w0 + 4 (32 i + lane) ..
+    auto       in_row  = [&](int r) { return reinterpret_cast<const float *>(v.logits + (int64_t) r * v.ldb) + x0; };
+    uint32_t   mw[kVec];  // their words of the mask
+    auto       mask_row = [&](int r) { return v.mask && r < r1 ? v.mask_row ? v.mask_row[r] : r : -1; };
+    auto       mask_of  = [&](int m) -> const uint32_t * {
+        return m >= 0 && m < v.n_masks ? reinterpret_cast<const uint32_t *>(v.mask + (int64_t) m * v.ldm) + x0 / 32 : nullptr;
+    };
+    auto load = [&](const float * in, const uint32_t * mk) {
 #pragma unroll
         for (int i = 0; i < kVec; i++) {
-            const int at = 4 * (i * kThreads + tid);
+            const int at = w0 + 4 * (32 * i + lane);
+            mw[i]        = mk && at < nx ? mk[at >> 5] : ~0u;
             if constexpr (VEC) {
                 if (at + 4 <= nx) {
                     x[i] = __ldcs(reinterpret_cast<const float4 *>(in + at));
@@ -64,90 +85,163 @@ __global__ void __launch_bounds__(kThreads) adjust_logits_kernel(const __grid_co
             x[i].z = at + 2 < nx ? in[at + 2] : 0.0f;
             x[i].w = at + 3 < nx ? in[at + 3] : 0.0f;
         }
-    }
-    // the row's sequence: starts at or before it
-    int s = 0;
-    for (int i0 = 0; i0 < v.S; i0 += kThreads) s += __syncthreads_count(i0 + tid < v.S && v.q_start[i0 + tid] <= row);
-    s -= 1;
-    const int first = s >= 0 ? max(v.q_start[s], 0) : 0;
-    const int nh    = v.history && s >= 0 ? min(max(v.n_history[s], 0), v.cap) : 0;
-    const int total = nh + row - first + 1;
-    const int last  = v.last_n && s >= 0 ? v.last_n[s] : -1;
-    const int begin = last < 0 ? 0 : max(total - last, 0);
-    const bool pen  = s >= 0 && (v.repeat || v.frequency || v.presence) && begin < total;
+    };
+    const uint32_t * mask = mask_of(mask_row(r0));
+    if (!same || mask) load(in_row(r0), mask);
+    int m_next = mask_row(r0 + 1);
+    const int nh    = v.history ? min(max(v.n_history[s], 0), v.cap) : 0;
+    const int last  = v.last_n ? v.last_n[s] : -1;
+    int       total = nh + r0 - first + 1;
+    int       begin = last < 0 ? 0 : max(total - last, 0);
+    const bool pen  = (v.repeat || v.frequency || v.presence) && last != 0;
     int b0 = 0, b1 = 0;
-    if (v.n_bias && s >= 0) {
+    if (v.n_bias) {
         b0 = min(max(v.bias_start[s], 0), v.n_bias);
         b1 = min(max(v.bias_start[s + 1], b0), v.n_bias);
     }
-    const int32_t * said = v.history ? reinterpret_cast<const int32_t *>(v.history + (int64_t) max(s, 0) * v.ldh) : nullptr;
-    auto token = [&](int j) { return j < nh ? said[j] : v.ids[first + j - nh]; };
-    if (pen || b1 > b0) {
-        uint4 * z = reinterpret_cast<uint4 *>(sh);
-        for (int i = tid; i < 2 * kSlice / 4; i += kThreads) z[i] = make_uint4(0, 0, 0, 0);
+    const int32_t * said = v.history ? reinterpret_cast<const int32_t *>(v.history + (int64_t) s * v.ldh) : nullptr;
+    // place in the slice of the j-th token ahead of a row; those elsewhere are not below nx
+    auto token = [&](int j) { return (uint32_t) *(j < nh ? said + j : v.ids + first + (j - nh)) - (uint32_t) x0; };
+    const bool rules = pen || b1 > b0;
+    int        n_list = 0;  // of the warp's tokens: those with a rule
+    float      rep = 1.0f, fr = 0.0f, pr = 0.0f;
+    if (rules) {
+        uint4 * z = reinterpret_cast<uint4 *>(cnt);
+        for (int i = tid; i < kSlice / 4; i += kThreads) z[i] = make_uint4(0, 0, 0, 0);
+        z = reinterpret_cast<uint4 *>(bix);
+        for (int i = tid; b1 > b0 && i < kSlice / 4; i += kThreads) z[i] = make_uint4(0, 0, 0, 0);
+        if (v.repeat) rep = v.repeat[s];
+        if (v.frequency) fr = v.frequency[s];
+        if (v.presence) pr = v.presence[s];
         __syncthreads();
         if (pen) {
-            for (int j = begin + tid; j < total; j += kThreads) {
-                const uint32_t k = (uint32_t) token(j) - (uint32_t) x0;
-                if (k < (uint32_t) nx) atomicAdd(cnt + k, 1u);
+            constexpr int U = 8;  // tokens of a thread in flight
+            for (int j0 = begin; j0 < total; j0 += U * kThreads) {
+                uint32_t k[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {  // one load each, whichever list it is from, so that all are on their way at once
+                    const int j = min(j0 + u * kThreads + tid, total - 1);
+                    k[u]        = token(j);
+                }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (k[u] < (uint32_t) nx && j0 + u * kThreads + tid < total) atomicAdd(cnt + k[u], 1u);
+                }
             }
         }
         for (int j = b0 + tid; j < b1; j += kThreads) {
             const uint32_t k = (uint32_t) v.bias_ids[j] - (uint32_t) x0;
             if (k < (uint32_t) nx) atomicMax(bix + k, (uint32_t) j + 1u);
         }
-    }
-    if (pass) {
+        __syncthreads();
+        uint32_t hit = 0;  // of this lane's 16 tokens
 #pragma unroll
         for (int i = 0; i < kVec; i++) {
-            const int at = 4 * (i * kThreads + tid);
-            if (at >= nx) break;
-            const uint32_t ok = mask ? mask[at >> 5] >> (at & 31) & 15u : 15u;
-            if (same && ok == 15u) continue;
-            if (!(ok & 1u)) x[i].x = -INFINITY;
-            if (!(ok & 2u)) x[i].y = -INFINITY;
-            if (!(ok & 4u)) x[i].z = -INFINITY;
-            if (!(ok & 8u)) x[i].w = -INFINITY;
-            if constexpr (VEC) {
-                if (at + 4 <= nx) {
-                    __stcs(reinterpret_cast<float4 *>(out + at), x[i]);
-                    continue;
-                }
+            const int   at = w0 + 4 * (32 * i + lane);
+            const uint4 c = *reinterpret_cast<const uint4 *>(cnt + at), b = b1 > b0 ? *reinterpret_cast<const uint4 *>(bix + at) : make_uint4(0, 0, 0, 0);
+            hit |= ((c.x | b.x) != 0) << (4 * i) | ((c.y | b.y) != 0) << (4 * i + 1) | ((c.z | b.z) != 0) << (4 * i + 2) | ((c.w | b.w) != 0) << (4 * i + 3);
+        }
+        int to = __popc(hit);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, to, o);
+            if (lane >= o) to += u;
+        }
+        n_list = __shfl_sync(0xffffffffu, to, 31);
+        to -= __popc(hit);
+        for (; hit; hit &= hit - 1) {
+            const int e = __ffs(hit) - 1, k = w0 + 4 * (32 * (e >> 2) + lane) + (e & 3);
+            cnt[k] |= kListed;
+            list[to++] = (uint16_t) k;
+        }
+        __syncwarp();
+        if (b1 > b0) {
+            for (int i = lane; i < n_list; i += 32) {
+                const uint32_t k = list[i], bi = bix[k];
+                bix[k] = bi ? __float_as_uint(v.bias[bi - 1]) : 0u;
             }
-            out[at] = x[i].x;
-            if (at + 1 < nx) out[at + 1] = x[i].y;
-            if (at + 2 < nx) out[at + 2] = x[i].z;
-            if (at + 3 < nx) out[at + 3] = x[i].w;
         }
     }
-    if (!pen && b1 <= b0) return;
-    __syncthreads();  // the slice is written, the counts are there
-    const float rep = v.repeat ? v.repeat[s] : 1.0f, fr = v.frequency ? v.frequency[s] : 0.0f, pr = v.presence ? v.presence[s] : 0.0f;
-    auto put = [&](uint32_t k, uint32_t times, uint32_t bi) {
-        if (mask && !(mask[k >> 5] >> (k & 31) & 1u)) return;
-        float l = in[k];
-        if (bi) l += v.bias[bi - 1];
+    auto rule = [&](float l, uint32_t k) {
+        if (b1 > b0) l += __uint_as_float(bix[k]);
+        const uint32_t times = cnt[k] & ~kListed;
         if (times) {
             l = l > 0.0f ? __fdiv_rn(l, rep) : l * rep;
             l -= (float) times * fr + pr;
         }
-        out[k] = l;
+        return l;
     };
-    if (pen) {
-        for (int j = begin + tid; j < total; j += kThreads) {
-            const uint32_t k = (uint32_t) token(j) - (uint32_t) x0;
-            if (k < (uint32_t) nx && cnt[k]) {
-                const uint32_t times = atomicExch(cnt + k, 0u);
-                if (times) put(k, times, atomicExch(bix + k, 0u));
+    for (int r = r0; r < r1; r++) {
+        const float * in   = in_row(r);
+        float *       out  = reinterpret_cast<float *>(v.out + (int64_t) r * v.ldo) + x0;
+        const bool    pass = !same || mask;  // the whole row goes through; else only the listed tokens
+        uint32_t      add = ~0u, drop = ~0u;
+        if (pen && r + 1 < r1) {
+            add = token(total);
+            if (last >= 0 && total + 1 - last > begin) drop = token(begin);
+        }
+        uint32_t ok = 0;
+        if (pass) {
+#pragma unroll
+            for (int i = 0; i < kVec; i++) {
+                const int at = w0 + 4 * (32 * i + lane);
+                ok |= (mw[i] >> (at & 31) & 15u) << (4 * i);
+                *reinterpret_cast<float4 *>(xs + at) = x[i];
             }
         }
-        __syncthreads();  // biases of tokens in the window are done
-    }
-    for (int j = b0 + tid; j < b1; j += kThreads) {
-        const uint32_t k = (uint32_t) v.bias_ids[j] - (uint32_t) x0;
-        if (k < (uint32_t) nx) {
-            const uint32_t bi = atomicExch(bix + k, 0u);
-            if (bi) put(k, 0u, bi);
+        if (r + 1 < r1) {
+            mask = mask_of(m_next);
+            if (!same || mask) load(in_row(r + 1), mask);
+            m_next = mask_row(r + 2);
+        }
+        __syncwarp();
+        for (int i = lane; i < n_list; i += 32) {
+            const uint32_t k = list[i];
+            if (pass) {
+                xs[k] = rule(xs[k], k);
+            } else {
+                out[k] = rule(in[k], k);
+            }
+        }
+        __syncwarp();
+        if (pass) {
+#pragma unroll
+            for (int i = 0; i < kVec; i++) {
+                const int at = w0 + 4 * (32 * i + lane);
+                if (at >= nx) break;
+                float4         y = *reinterpret_cast<const float4 *>(xs + at);
+                const uint32_t o = ok >> (4 * i);
+                if (!(o & 1u)) y.x = -INFINITY;
+                if (!(o & 2u)) y.y = -INFINITY;
+                if (!(o & 4u)) y.z = -INFINITY;
+                if (!(o & 8u)) y.w = -INFINITY;
+                if constexpr (VEC) {
+                    if (at + 4 <= nx) {
+                        __stcs(reinterpret_cast<float4 *>(out + at), y);
+                        continue;
+                    }
+                }
+                out[at] = y.x;
+                if (at + 1 < nx) out[at + 1] = y.y;
+                if (at + 2 < nx) out[at + 2] = y.z;
+                if (at + 3 < nx) out[at + 3] = y.w;
+            }
+        }
+        if (r + 1 < r1 && pen) {  // the window of the next row: a token's count is its warp's own by now
+            total++;
+            if (last >= 0) begin = max(total - last, 0);
+            if (add - (uint32_t) w0 < (uint32_t) kWarpTok && add < (uint32_t) nx) {
+                const uint32_t old = cnt[add];
+                __syncwarp();
+                if (lane == 0) {
+                    cnt[add] = (old | kListed) + 1;
+                    if (!(old & kListed)) list[n_list] = (uint16_t) add;
+                }
+                if (!(old & kListed)) n_list++;
+                __syncwarp();
+            }
+            if (drop - (uint32_t) w0 < (uint32_t) kWarpTok && drop < (uint32_t) nx && lane == 0) cnt[drop]--;
+            __syncwarp();
         }
     }
 }
@@ -158,14 +252,15 @@ int adjust_logits_run(srhpm_ctx * ctx, const LogitView & v, cudaStream_t stream)
     Args a;
     a.v      = v;
     a.slices = (v.V + kSlice - 1) / kSlice;
-    const int64_t grid = (int64_t) a.slices * v.T;
-    if (grid > INT32_MAX) return SRHPM_UNSUPPORTED;
+    // all rows of a sequence in one CTA where that leaves some CTAs for each SM
+    a.by_seq           = (int64_t) v.S * a.slices >= 4 * (int64_t) ctx->num_sms;
+    if ((int64_t) a.slices * std::max(v.S, v.T) > INT32_MAX) return SRHPM_UNSUPPORTED;
+    const int64_t grid = (int64_t) a.slices * (a.by_seq ? v.S : v.T);
     const bool vec = ((reinterpret_cast<uintptr_t>(v.logits) | reinterpret_cast<uintptr_t>(v.out) | v.ldb | v.ldo) & 15) == 0;
     auto       kern = vec ? adjust_logits_kernel<true> : adjust_logits_kernel<false>;
-    constexpr int smem = 2 * kSlice * 4;
-    int st = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    int        st   = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     if (st != SRHPM_OK) return st;
-    st = cuda_status(launch_k_pdl(kern, dim3((unsigned) grid), dim3(kThreads), smem, stream, a));
+    st = cuda_status(launch_k_pdl(kern, dim3((unsigned) grid), dim3(kThreads), kSmem, stream, a));
     ctx->launches.fetch_add(1);
     return st;
 }
