@@ -10,9 +10,10 @@
 // the 128-byte swizzled rows that the product reads.
 //
 // Work: as in fa_paged.cu, all items' units of 128 tokens stand in one line that is cut into equal parts, one per CTA.
-// Roles: 8 softmax warps (two groups, half of the rows each), 1 MMA warp, 3 warps that bring Q, 4 that unpack K and 4 that
-// unpack V. An unpacking warp has 32 tokens of each tile and brings their bytes itself, by cp.async into a ring of its own,
-// several tiles ahead and across items: 9 pieces make a row of 64 or 128 values, whatever the strides are.
+// Roles: 16 softmax warps (four groups, a quarter of the rows each: with half of them a thread's scores and sums did not fit its
+// registers, and the chain from scores to P took 6000 cycles of a tile), 1 MMA warp, 2 producer warps (K's and V's raw rows by TMA, 64
+// tokens at a time, row boxes of 16-byte multiples; layouts that TMA does not take come by cp.async, 9 pieces a row), and 8 warps
+// that unpack, K's and V's, 32 tokens of a tile each.
 // f32 rows (PREC): Q and P as sums of two f16 parts, and as the tensor cores' sums are truncated (a shrink of 2^-25 per product
 // step, measured: 2e-5 after 400), O is taken out every kFlush tiles and summed up in f32 in the item's record.
 #include <cuda.h>
@@ -36,10 +37,11 @@ using namespace fap;
 namespace {
 
 constexpr int      kTile   = 128;  // tokens of a tile and of a unit of work
-constexpr int      kSm     = 8;    // softmax warps
-constexpr int      kQW     = 3;    // warps that bring Q
-constexpr int      kThr    = (kSm + 1 + kQW + 8) * 32;
-constexpr int      kFlush  = 4;    // tiles
+constexpr int      kSm     = 16;   // softmax warps, in groups of four
+constexpr int      kConv   = 8;    // unpacking warps: K's four, V's four
+constexpr int      kThr    = (kSm + 4 + kConv) * 32;
+constexpr int      kRawTok = 64;   // tokens of a raw stage
+constexpr int      kFlush  = 8;    // tiles
 constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s
 constexpr float    kUnset  = -3e38f;    // a row's reference before its first score
 
@@ -48,19 +50,16 @@ struct Pool4 {
     int64_t         nb1, nb2, nb3;
 };
 
-// a stage's rows: HD values of a token in RS bytes, of which TMA fills all (its boxes start on 16 bytes, a row up to 12 later)
-constexpr int row_values(int D) { return D < 128 ? D : 128; }
-constexpr int row_stride(int D) { return D < 128 ? 48 : 80; }
+// bytes of a raw row's place: TMA's boxes start on 16 bytes, the row up to 12 later
+constexpr int row_stride(int D) { return D == 64 ? 48 : D == 128 ? 80 : 144; }
 
 template <int D, int N, bool PREC> struct LayT {
     static constexpr int parts = PREC ? 2 : 1;
     static constexpr int MT    = D == 256 ? 2 : 1;             // products along the dims
     static constexpr int MM    = D == 64 ? 64 : 128;           // dims of a product
     static constexpr int NP    = N < 32 ? 32 : N;              // tensor-memory columns of N
-    static constexpr int CH    = D == 256 ? 2 : 1;             // chunks of a V tile, 32 KB at most
-    static constexpr int vtok  = kTile / CH;
-    static constexpr int chunk = vtok * D * 2;
-    static constexpr int VS    = 2;                            // chunks in the ring
+    static constexpr int chunk = 32 * D * 2;                   // a warp's tokens of V
+    static constexpr int VT    = D == 256 ? 1 : 2;             // V tiles in the ring
     static constexpr int KB    = D / 2 * 2 + MT * NP + 2 * NP <= 512 ? 2 : 1;   // K tiles in tensor memory
     static constexpr int SB    = KB * D / 2 + MT * NP + 2 * NP <= 512 ? 2 : 1;  // score buffers
     static constexpr int qtile = N * D * 2;
@@ -68,33 +67,31 @@ template <int D, int N, bool PREC> struct LayT {
     static constexpr int ptile = planes * kTile * 128;         // one part of P
     static constexpr int q     = 0;
     static constexpr int ring  = q + parts * qtile;
-    static constexpr int p     = ring + VS * chunk;
-    // P buffers: two where shared memory has room for them beside three stages of raw rows
-    static constexpr int HD    = row_values(D);
-    static constexpr int SPT   = D / HD;                       // stages of a tile
-    static constexpr int rowb  = HD / 16 * 9;
-    static constexpr int CB    = HD / 16;
+    static constexpr int p     = ring + VT * 4 * chunk;
+    static constexpr int rowb  = D / 16 * 9;
+    static constexpr int CB    = D / 16;
     static constexpr int RS    = row_stride(D);
-    static constexpr int stage = 32 * RS;                      // of one warp
-    static constexpr int tail  = 2560 + 24 * N;                // barriers, rows' numbers
-    static constexpr int PB    = 232448 - tail - p - 2 * parts * ptile >= 4 * 8 * stage ? 2 : 1;
+    static constexpr int stage = kRawTok * RS;
+    static constexpr int tail  = 3072 + 24 * N;                // barriers, rows' numbers
+    // P buffers: two where shared memory has room for them beside the raw rows of two tiles
+    static constexpr int PB    = 232448 - tail - p - 2 * parts * ptile >= 8 * stage ? 2 : 1;
     static constexpr int raw   = p + PB * parts * ptile;
-    static constexpr int room  = (232448 - tail - raw) / (8 * stage);
-    static constexpr int ST    = room < 6 * SPT ? room : 6 * SPT;
-    static constexpr int rows  = raw + ST * 8 * stage;         // off, m, fac, frec: f32 [N]; lo, hi: int [N]
-    static constexpr int red   = rows + 24 * N;                // f32 [2][4][32]
-    static constexpr int bar   = red + 1024;
-    static constexpr int nbar  = 2 * KB + 2 * VS + 2 * SB + PB + 2 + 2 + 8 * ST;
+    static constexpr int room  = (232448 - tail - raw) / stage;
+    static constexpr int NK    = room >= 12 ? 6 : room >= 6 ? 4 : 2;  // raw stages of K and of V (even: a slot is one half's of the tiles)
+    static constexpr int NV    = room >= 12 ? 6 : room >= 8 ? 4 : 2;
+    static constexpr int rows  = raw + (NK + NV) * stage;         // off, m, fac, frec: f32 [N]; lo, hi: int [N]
+    static constexpr int red   = rows + 24 * N;                // f32 [4][4][32]
+    static constexpr int bar   = red + 2048;
+    static constexpr int nbar  = 2 * KB + 8 * VT + 2 * SB + PB + 2 + 2 + 2 * (NK + NV);
     static constexpr int misc  = bar + nbar * 8;
     static constexpr int total = misc + 80;
-    static constexpr int CW    = N / 2 < 32 ? N / 2 : 32;      // columns that a softmax thread takes at a time
-    static constexpr int NC    = N / 2 / CW;
+    static constexpr int CW    = N / 4;                        // columns (rows of Q) of a softmax thread
     static constexpr uint32_t tO = 0, tS = MT * NP, tK = tS + SB * NP;
-    static_assert(total <= 232448 && ST >= 2 && raw % 16 == 0 && rows >= kMaxSeqs * 8, "shared memory");
+    static_assert(total <= 232448 && raw % 128 == 0 && rows >= kMaxSeqs * 8, "shared memory");
     static_assert(tK + KB * D / 2 <= 512, "tensor memory");
-    // registers of the softmax warps, of the MMA's and Q's, of the unpacking ones: the launch's 96 a thread, shared out anew
-    static constexpr int rs = N == 128 ? 144 : 120, rm = N == 128 ? 72 : 56, ru = N == 128 ? 56 : 88;
-    static_assert(256 * rs + 128 * rm + 256 * ru <= kThr * 96, "registers");
+    // registers of the softmax warps, of the MMA's and the producers', of the unpacking ones: the launch's 72 a thread, shared out anew
+    static constexpr int rs = N == 128 ? 88 : 72, rm = N == 128 ? 40 : 56, ru = N == 128 ? 56 : 80;
+    static_assert(kSm * 32 * rs + 128 * rm + kConv * 32 * ru <= kThr * 72, "registers");
 };
 
 __device__ __forceinline__ bool elect_one() {
@@ -149,17 +146,26 @@ template <int W> __device__ __forceinline__ void ld_t(uint32_t t, uint32_t (&r)[
               "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
               "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
             : "r"(t));
+    } else if constexpr (W == 16) {
+        tc::ld16(t, r);
     } else {
-        tc::ld8(t, r);
+        tc::ld4(t, r);
     }
 }
 template <int W> __device__ __forceinline__ void st_t(uint32_t t, const uint32_t (&r)[W]) {
     if constexpr (W == 32) {
         tc::st16(t, *reinterpret_cast<const uint32_t(*)[16]>(&r[0]));
         tc::st16(t + 16, *reinterpret_cast<const uint32_t(*)[16]>(&r[16]));
+    } else if constexpr (W == 16) {
+        tc::st16(t, r);
     } else {
-        tc::st8(t, r);
+        tc::st4(t, r);
     }
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 // o += what the record holds of it, times the factors that its rows were rescaled by since; all loads in flight at once
@@ -203,19 +209,20 @@ __global__ void __launch_bounds__(kThr, 1)
     fa_paged_q4_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ PArgs a,
                        const __grid_constant__ Pool4 kp, const __grid_constant__ Pool4 vp) {
     using Ly           = LayT<D, N, PREC>;
-    constexpr int KB = Ly::KB, SB = Ly::SB, PB = Ly::PB, VS = Ly::VS, CH = Ly::CH, ST = Ly::ST, CW = Ly::CW, NC = Ly::NC;
+    constexpr int KB = Ly::KB, SB = Ly::SB, PB = Ly::PB, VT = Ly::VT, NK = Ly::NK, NV = Ly::NV, CW = Ly::CW;
     extern __shared__ __align__(1024) uint8_t sm[];
     uint64_t * kfull  = reinterpret_cast<uint64_t *>(sm + Ly::bar);
     uint64_t * kempty = kfull + KB;
     uint64_t * vfull  = kempty + KB;
-    uint64_t * vempty = vfull + VS;
-    uint64_t * sfull  = vempty + VS;
+    uint64_t * vempty = vfull + 4 * VT;
+    uint64_t * sfull  = vempty + 4 * VT;
     uint64_t * sfree  = sfull + SB;
     uint64_t * pfull  = sfree + SB;
     uint64_t * pvdone = pfull + PB;  // [2] in turn
     uint64_t * qfull  = pvdone + 2;
     uint64_t * qempty = qfull + 1;
-    uint64_t * rawfull = qempty + 1;  // [8][ST]
+    uint64_t * rfull  = qempty + 1;         // K's NK, V's NV
+    uint64_t * rempty = rfull + NK + NV;
     uint32_t * tptr   = reinterpret_cast<uint32_t *>(sm + Ly::misc);
     int *      first  = reinterpret_cast<int *>(sm + Ly::misc + 16);
     int64_t *  range  = reinterpret_cast<int64_t *>(sm + Ly::misc + 32);
@@ -229,11 +236,11 @@ __global__ void __launch_bounds__(kThr, 1)
     }
     if (tid == 0) {
         for (int i = 0; i < KB; i++) {
-            mbar_init(&kfull[i], 4);
+            mbar_init(&kfull[i], kConv / 2);
             mbar_init(&kempty[i], 1);
         }
-        for (int i = 0; i < VS; i++) {
-            mbar_init(&vfull[i], 4 / CH);
+        for (int i = 0; i < 4 * VT; i++) {
+            mbar_init(&vfull[i], 1);
             mbar_init(&vempty[i], 1);
         }
         for (int i = 0; i < SB; i++) {
@@ -242,9 +249,12 @@ __global__ void __launch_bounds__(kThr, 1)
         }
         for (int i = 0; i < PB; i++) mbar_init(&pfull[i], kSm);
         for (int i = 0; i < 2; i++) mbar_init(&pvdone[i], 1);
-        mbar_init(qfull, kQW);
+        mbar_init(qfull, kSm);
         mbar_init(qempty, 1);
-        for (int i = 0; i < 8 * ST; i++) mbar_init(&rawfull[i], a.box ? 1 : 32);
+        for (int i = 0; i < NK + NV; i++) {
+            mbar_init(&rfull[i], a.box ? 1 : 32);
+            mbar_init(&rempty[i], 2);
+        }
         fence_mbar_init();
         first[0] = -1;
     }
@@ -270,56 +280,104 @@ __global__ void __launch_bounds__(kThr, 1)
     }
 
     if (warp < kSm) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Ly::rs));
+        if constexpr (Ly::rs > 72) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Ly::rs));
         // ---------------- softmax ----------------
-        const int wg = warp >> 2, wq = warp & 3, tg = tid & 127, bid = 1 + wg;
-        float *   off = reinterpret_cast<float *>(sm + Ly::rows), *mrow = off + N, *fac = mrow + N, *frec = fac + N;
+        const int wg = warp >> 2, wq = warp & 3, tg = tid & 127, bid = 1 + wg, g0 = wg * CW;  // rows g0 .. g0 + CW - 1
+        float *   off = reinterpret_cast<float *>(sm + Ly::rows) + g0, *mrow = off + N, *fac = mrow + N, *frec = fac + N;
         int *     rlo = reinterpret_cast<int *>(frec + N), *rhi = rlo + N;
         float *   red = reinterpret_cast<float *>(sm + Ly::red) + wg * 128;
-        const int g0  = wg * (N / 2);  // this group's rows
         // dim of this lane's row of O^T, of each product along the dims
         const int  od   = D == 64 ? q4::value_at(16 * wq + (lane & 15)) : 64 * (wq >> 1) + q4::value_at(32 * (wq & 1) + lane);
         const bool mine = D != 64 || lane < 16;
-        uint32_t   gi = 0, pvw = 0;
+        uint32_t   gi = 0, pvw = 0, items = 0;
         auto       pv_wait = [&](uint32_t upto) {
             for (; pvw < upto; pvw++) wait_bar(&pvdone[pvw & 1], (pvw >> 1) & 1, a.status, bad);
         };
-        for (; active; active = walk_next<N, kTile>(a, w)) {
+        // Q of an item: 16-byte pieces of 8 dims in K's order, 128-byte swizzle; rows that are none as zeros
+        auto bring_q = [&](const Walk & w) {
+            if (w.sp.nkv == 0) return;
+            const int rb = w.rt * N, rows = min(N, w.n * a.G - rb);
+            if (items > 0) wait_bar(qempty, (items - 1) & 1, a.status, bad);
+            items++;
+#pragma unroll 1
+            for (int v = tid; v < N * (D / 8); v += kSm * 32) {
+                const int row = v / (D / 8), pc = v % (D / 8), odd = (pc >> 2) & 1, word = pc & 3;
+                uint2     x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = make_uint2(0u, 0u);
+                if (row < rows) {
+                    const int       tok = a.byG.div(rb + row), h = w.h * a.G + (rb + row - tok * a.G);
+                    const uint8_t * src = a.q + (int64_t) (w.r0 + tok) * a.qnb1 + (int64_t) h * a.qnb2;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {  // pairs of neighbouring dims: bytes 0, 1 and 2, 3, low and high halves
+                        const int d = (pc >> 2) * 32 + q4::byte_of(odd, word, 2 * (e & 1)) + 16 * (e >> 1);
+                        if constexpr (PREC) {
+                            x[e] = *reinterpret_cast<const uint2 *>(src + 4 * d);
+                        } else {
+                            x[e].x = *reinterpret_cast<const uint32_t *>(src + 2 * d);
+                        }
+                    }
+                }
+                uint8_t * to = sm + Ly::q + (pc >> 3) * (N * 128) + row * 128 + (((pc & 7) ^ (row & 7)) << 4);
+                uint32_t  hw[4], lw[4];
+#pragma unroll
+                for (int e = 0; e < 2; e++) {  // low halves, high halves
+                    const uint2 A = x[2 * e], B = x[2 * e + 1];
+                    if constexpr (PREC) {
+                        const float f[4] = { __uint_as_float(A.x), __uint_as_float(B.x), __uint_as_float(A.y), __uint_as_float(B.y) };
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            const __half2 h2 = __floats2half2_rn(f[2 * m], f[2 * m + 1]);
+                            const __half2 l2 = __floats2half2_rn(f[2 * m] - __low2float(h2), f[2 * m + 1] - __high2float(h2));
+                            hw[2 * e + m] = *reinterpret_cast<const uint32_t *>(&h2);
+                            lw[2 * e + m] = *reinterpret_cast<const uint32_t *>(&l2);
+                        }
+                    } else {
+                        hw[2 * e]     = q4::prmt(A.x, B.x, 0x5410u);
+                        hw[2 * e + 1] = q4::prmt(A.x, B.x, 0x7632u);
+                    }
+                }
+                *reinterpret_cast<uint4 *>(to) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+                if constexpr (PREC) *reinterpret_cast<uint4 *>(to + Ly::qtile) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(qfull);
+        };
+        // O's part of this group: f(values, product along the dims, place)
+        auto each_o = [&](auto f) {
+#pragma unroll 1
+            for (int mt = 0; mt < Ly::MT; mt++) {
+                uint32_t       o[CW];
+                const uint32_t at = tc::taddr(tb + Ly::tO + mt * Ly::NP + g0, wq, 0);
+                ld_t<CW>(at, o);
+                tc::wait_ld();
+                f(o, mt, at);
+            }
+        };
+        const float qs = a.softcap_l2 != 0.0f ? 1.0f : a.qscale;
+        if (active) bring_q(w);
+        while (active) {
             const int  n = w.sp.nkv ? w.take : 0, rb = w.rt * N, rows = min(N, w.n * a.G - rb);
             const int  slot = 2 * blockIdx.x + (w.off == 0 ? 1 : 0);
             const bool whole = w.off == 0 && w.take == w.sp.units;
-            if (tg < N / 2) {
-                const int  r = g0 + tg;
-                const bool is = r < rows;
-                const int  pos = w.kv - w.n + a.byG.div(rb + (is ? r : 0));
-                rhi[r]  = is ? min(pos + 1, w.sp.hi) : 0;
-                rlo[r]  = a.window > 0 ? max(w.sp.lo, (int) max((int64_t) INT32_MIN, (int64_t) pos - a.window + 1)) : w.sp.lo;
-                off[r]  = is ? kUnset : INFINITY;  // rows that are none: p = 0
-                mrow[r] = is ? -INFINITY : INFINITY;
-                frec[r] = 1.0f;
+            if (tg < CW) {
+                const bool is = g0 + tg < rows;
+                const int  pos = w.kv - w.n + a.byG.div(rb + (is ? g0 + tg : 0));
+                rhi[tg]  = is ? min(pos + 1, w.sp.hi) : 0;
+                rlo[tg]  = a.window > 0 ? max(w.sp.lo, (int) max((int64_t) INT32_MIN, (int64_t) pos - a.window + 1)) : w.sp.lo;
+                off[tg]  = is ? kUnset : INFINITY;  // rows that are none: p = 0
+                mrow[tg] = is ? -INFINITY : INFINITY;
+                frec[tg] = 1.0f;
             }
             named_bar_sync(bid, 128);
             // tokens that every row sees
             const int pmin = w.kv - w.n + a.byG.div(rb), pmax = w.kv - w.n + a.byG.div(rb + rows - 1);
             const int ahi = min(pmin + 1, w.sp.hi), alo = a.window > 0 ? (int) max((int64_t) 0, (int64_t) pmax - a.window + 1) : w.sp.lo;
-            float     l[NC][CW];
+            float     l[CW];
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-#pragma unroll
-                for (int e = 0; e < CW; e++) l[c][e] = 0.0f;
-            }
-            const float qs = a.softcap_l2 != 0.0f ? 1.0f : a.qscale;
-            // O's part of one chunk of columns: f(values, product along the dims)
-            auto each_o = [&](int c0, auto f) {
+            for (int e = 0; e < CW; e++) l[e] = 0.0f;
 #pragma unroll 1
-                for (int mt = 0; mt < Ly::MT; mt++) {
-                    uint32_t       o[CW];
-                    const uint32_t at = tc::taddr(tb + Ly::tO + mt * Ly::NP + c0, wq, 0);
-                    ld_t<CW>(at, o);
-                    tc::wait_ld();
-                    f(o, mt, at);
-                }
-            };
             for (int i = 0; i < n; i++, gi++) {
                 const uint32_t sb = gi % SB, pb = gi % PB;
                 const int      t0 = w.tile(i) * kTile, pos = t0 + 32 * wq + lane;
@@ -330,171 +388,165 @@ __global__ void __launch_bounds__(kThr, 1)
                     if (i > 0 && i % kFlush == 0) {  // O so far to the record
                         pv_wait(gi);
                         tc::fence_after();
-#pragma unroll 1
-                        for (int c = 0; c < NC; c++) {
-                            each_o(g0 + c * CW, [&](uint32_t (&o)[CW], int mt, uint32_t) {
-                                float *   rec = a.part_acc + ((int64_t) slot * a.prow + g0 + c * CW) * D + 128 * mt + od;
-                                const int nr  = mine ? rows - (g0 + c * CW) : 0;
-                                if (i > kFlush) add_record(o, rec, D, nr, frec + g0 + c * CW);
-#pragma unroll
-                                for (int e = 0; e < CW; e++) {
-                                    if (e < nr) rec[e * D] = __uint_as_float(o[e]);
-                                }
-                            });
-                        }
-                        named_bar_sync(bid, 128);
-                        if (tg < N / 2) frec[g0 + tg] = 1.0f;
-                    }
-                }
-#pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    const int      c0 = g0 + c * CW;
-                    const uint32_t ts = tc::taddr(tb + Ly::tS + sb * Ly::NP + c0, wq, 0);
-                    uint32_t       s[CW];
-                    auto           scores = [&]() {
-                        ld_t<CW>(ts, s);
-                        tc::wait_ld();
-                        if (a.softcap_l2 != 0.0f) {
-#pragma unroll
-                            for (int e = 0; e < CW; e++) s[e] = __float_as_uint(a.softcap_l2 * tanhf(__uint_as_float(s[e]) * a.qscale));
-                        }
-                        if (mask) {
+                        each_o([&](uint32_t (&o)[CW], int mt, uint32_t) {
+                            float *   rec = a.part_acc + ((int64_t) slot * a.prow + g0) * D + 128 * mt + od;
+                            const int nr  = mine ? rows - g0 : 0;
+                            if (i > kFlush) add_record(o, rec, D, nr, frec);
 #pragma unroll
                             for (int e = 0; e < CW; e++) {
-                                if (pos < rlo[c0 + e] || pos >= rhi[c0 + e]) s[e] = __float_as_uint(-INFINITY);
+                                if (e < nr) rec[e * D] = __uint_as_float(o[e]);
                             }
-                        }
-                    };
-                    auto shifted = [&]() {
-                        float top = -INFINITY;
+                        });
+                        named_bar_sync(bid, 128);
+                        if (tg < CW) frec[tg] = 1.0f;
+                    }
+                }
+                const uint32_t ts = tc::taddr(tb + Ly::tS + sb * Ly::NP + g0, wq, 0);
+                uint32_t       s[CW];
+                auto           scores = [&]() {
+                    ld_t<CW>(ts, s);
+                    tc::wait_ld();
+                    if (a.softcap_l2 != 0.0f) {
 #pragma unroll
-                        for (int e = 0; e < CW; e += 4) {
-                            const float4 o = *reinterpret_cast<const float4 *>(off + c0 + e);
-                            float        x0, x1, x2, x3;
-                            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f2_pack(qs, qs), f2_pack(-o.x, -o.y)), x0, x1);
-                            f2_unpack(f2_fma(f2_pack(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), f2_pack(qs, qs), f2_pack(-o.z, -o.w)), x2, x3);
-                            s[e] = __float_as_uint(x0); s[e + 1] = __float_as_uint(x1); s[e + 2] = __float_as_uint(x2); s[e + 3] = __float_as_uint(x3);
-                            top = fmaxf(fmaxf(top, fmaxf(x0, x1)), fmaxf(x2, x3));
+                        for (int e = 0; e < CW; e++) s[e] = __float_as_uint(a.softcap_l2 * tanhf(__uint_as_float(s[e]) * a.qscale));
+                    }
+                    if (mask) {
+#pragma unroll
+                        for (int e = 0; e < CW; e++) {
+                            if (pos < rlo[e] || pos >= rhi[e]) s[e] = __float_as_uint(-INFINITY);
                         }
-                        return top;
-                    };
+                    }
+                };
+                auto shifted = [&]() {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < CW; e += 4) {
+                        const float4 o = *reinterpret_cast<const float4 *>(off + e);
+                        float        x0, x1, x2, x3;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), f2_pack(qs, qs), f2_pack(-o.x, -o.y)), x0, x1);
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3])), f2_pack(qs, qs), f2_pack(-o.z, -o.w)), x2, x3);
+                        s[e] = __float_as_uint(x0); s[e + 1] = __float_as_uint(x1); s[e + 2] = __float_as_uint(x2); s[e + 3] = __float_as_uint(x3);
+                        top = max3(max3(top, x0, x1), x2, x3);
+                    }
+                    return top;
+                };
+                scores();
+                const float top = shifted();
+                if (bar_any(bid, 128, top > kLazy + kShift)) {
+                    // raise the rows' references: largest scores over the tile's tokens
                     scores();
-                    const float top = shifted();
-                    if (bar_any(bid, 128, top > kLazy + kShift)) {
-                        // raise the rows' references: largest scores over the tile's tokens
-                        scores();
-                        const float best = qs * fold(s, [](uint32_t u, uint32_t v) { return __float_as_uint(fmaxf(__uint_as_float(u), __uint_as_float(v))); });
-                        if (lane < CW) red[wq * 32 + lane] = best;
-                        named_bar_sync(bid, 128);
-                        if (tg < CW) {
-                            const float v = fmaxf(fmaxf(red[tg], red[32 + tg]), fmaxf(red[64 + tg], red[96 + tg])), mo = mrow[c0 + tg];
-                            float       f = 1.0f;
-                            if (v > mo + kLazy) {  // of -inf: any score
-                                f             = exp2a(mo - v);
-                                mrow[c0 + tg] = v;
-                                off[c0 + tg]  = v - kShift;
-                                frec[c0 + tg] *= f;
-                            }
-                            fac[c0 + tg] = f;
+                    const float best = qs * fold(s, [](uint32_t u, uint32_t v) { return __float_as_uint(fmaxf(__uint_as_float(u), __uint_as_float(v))); });
+                    if (lane < CW) red[wq * 32 + lane] = best;
+                    named_bar_sync(bid, 128);
+                    if (tg < CW) {
+                        const float v = fmaxf(fmaxf(red[tg], red[32 + tg]), fmaxf(red[64 + tg], red[96 + tg])), mo = mrow[tg];
+                        float       f = 1.0f;
+                        if (v > mo + kLazy) {  // of -inf: any score
+                            f        = exp2a(mo - v);
+                            mrow[tg] = v;
+                            off[tg]  = v - kShift;
+                            frec[tg] *= f;
                         }
-                        named_bar_sync(bid, 128);
-#pragma unroll
-                        for (int e = 0; e < CW; e++) l[c][e] *= fac[c0 + e];
-                        if (i > 0 && (!PREC || i % kFlush)) {
-                            pv_wait(gi);
-                            tc::fence_after();
-                            each_o(c0, [&](uint32_t (&o)[CW], int, uint32_t at) {
-#pragma unroll
-                                for (int e = 0; e < CW; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac[c0 + e]);
-                                st_t<CW>(at, o);
-                            });
-                            tc::wait_st();
-                        }
-                        scores();
-                        shifted();
+                        fac[tg] = f;
                     }
-                    if (c == NC - 1) {  // S is read
-                        tc::fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sfree[sb]);
-                    }
-                    if (c == 0) pv_wait(gi + 1 > PB ? gi + 1 - PB : 0);  // the product that read this P buffer
-                    uint8_t * pr = sm + Ly::p + pb * Ly::parts * Ly::ptile + (c0 >> 6) * (kTile * 128) + (32 * wq + lane) * 128;
+                    named_bar_sync(bid, 128);
 #pragma unroll
-                    for (int e = 0; e < CW; e += 8) {
-                        uint32_t hi[4], lo[4];
+                    for (int e = 0; e < CW; e++) l[e] *= fac[e];
+                    if (i > 0 && (!PREC || i % kFlush)) {
+                        pv_wait(gi);
+                        tc::fence_after();
+                        each_o([&](uint32_t (&o)[CW], int, uint32_t at) {
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const float x0 = exp2a(__uint_as_float(s[e + 2 * k])), x1 = exp2a(__uint_as_float(s[e + 2 * k + 1]));
-                            f2_unpack(f2_add(f2_pack(l[c][e + 2 * k], l[c][e + 2 * k + 1]), f2_pack(x0, x1)), l[c][e + 2 * k], l[c][e + 2 * k + 1]);
-                            const __half2 h2 = __floats2half2_rn(x0, x1);
-                            hi[k]            = *reinterpret_cast<const uint32_t *>(&h2);
-                            if constexpr (PREC) {
-                                const __half2 r2 = __floats2half2_rn(x0 - __low2float(h2), x1 - __high2float(h2));
-                                lo[k]            = *reinterpret_cast<const uint32_t *>(&r2);
-                            }
-                        }
-                        uint8_t * to = pr + (((((c0 + e) >> 3) & 7) ^ (lane & 7)) << 4);
-                        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        if constexpr (PREC) *reinterpret_cast<uint4 *>(to + Ly::ptile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            for (int e = 0; e < CW; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac[e]);
+                            st_t<CW>(at, o);
+                        });
+                        tc::wait_st();
                     }
+                    scores();
+                    shifted();
+                }
+                tc::fence_before();  // S is read
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sfree[sb]);
+                uint8_t * pr = sm + Ly::p + pb * Ly::parts * Ly::ptile + (g0 >> 6) * (kTile * 128) + (32 * wq + lane) * 128;
+                uint32_t  hi[CW / 2];
+                [[maybe_unused]] uint32_t lo[CW / 2];
+#pragma unroll
+                for (int k = 0; k < CW / 2; k++) {
+                    const float x0 = exp2a(__uint_as_float(s[2 * k])), x1 = exp2a(__uint_as_float(s[2 * k + 1]));
+                    f2_unpack(f2_add(f2_pack(l[2 * k], l[2 * k + 1]), f2_pack(x0, x1)), l[2 * k], l[2 * k + 1]);
+                    const __half2 h2 = __floats2half2_rn(x0, x1);
+                    hi[k]            = *reinterpret_cast<const uint32_t *>(&h2);
+                    if constexpr (PREC) {
+                        const __half2 r2 = __floats2half2_rn(x0 - __low2float(h2), x1 - __high2float(h2));
+                        lo[k]            = *reinterpret_cast<const uint32_t *>(&r2);
+                    }
+                }
+                pv_wait(gi + 1 > PB ? gi + 1 - PB : 0);  // the product that read this P buffer
+                if constexpr (CW >= 8) {
+#pragma unroll
+                    for (int k = 0; k < CW / 2; k += 4) {
+                        uint8_t * to = pr + (((((g0 + 2 * k) >> 3) & 7) ^ (lane & 7)) << 4);
+                        *reinterpret_cast<uint4 *>(to) = make_uint4(hi[k], hi[k + 1], hi[k + 2], hi[k + 3]);
+                        if constexpr (PREC) *reinterpret_cast<uint4 *>(to + Ly::ptile) = make_uint4(lo[k], lo[k + 1], lo[k + 2], lo[k + 3]);
+                    }
+                } else {  // four rows: half a piece
+                    uint8_t * to = pr + (((g0 >> 3) ^ (lane & 7)) << 4) + 2 * (g0 & 7);
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(hi[0], hi[1]);
+                    if constexpr (PREC) *reinterpret_cast<uint2 *>(to + Ly::ptile) = make_uint2(lo[0], lo[1]);
                 }
                 fence_proxy_async_smem();
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&pfull[pb]);
             }
-            // ---------------- the item's end ----------------
-#pragma unroll
-            for (int c = 0; c < NC; c++) {
-                const int   c0 = g0 + c * CW;
-                const float sum = fold(l[c], [](float u, float v) { return u + v; });
-                if (lane < CW) red[wq * 32 + lane] = sum;
-                named_bar_sync(bid, 128);
-                if (tg < CW && c0 + tg < rows) {
-                    const int   r = c0 + tg, tok = a.byG.div(rb + r), h = w.h * a.G + (rb + r - tok * a.G);
-                    float       L = (red[tg] + red[32 + tg]) + (red[64 + tg] + red[96 + tg]);
-                    const float M = mrow[r];
-                    float       f = 1.0f;
-                    if (!whole) {
-                        a.part_ms[(int64_t) slot * a.prow + r] = make_float2(M, L);
-                    } else {
-                        if (a.sinks) {  // relative to the larger of the two
-                            const float sk = a.sinks[h] * kLog2e;
-                            if (sk > M) {
-                                f = M == -INFINITY ? 0.0f : exp2a(M - sk);
-                                L = L * f + exp2f(kShift);
-                            } else if (sk > -INFINITY) {
-                                L += exp2a(sk - M + kShift);
-                            }
+            // ---------------- the item's end; the next one's Q before it, so that its products start meanwhile ----------------
+            Walk       nw   = w;
+            const bool more = walk_next<N, kTile>(a, nw);
+            if (more) bring_q(nw);
+            const float sum = fold(l, [](float u, float v) { return u + v; });
+            if (lane < CW) red[wq * 32 + lane] = sum;
+            named_bar_sync(bid, 128);
+            if (tg < CW && g0 + tg < rows) {
+                const int   r = g0 + tg, tok = a.byG.div(rb + r), h = w.h * a.G + (rb + r - tok * a.G);
+                float       L = (red[tg] + red[32 + tg]) + (red[64 + tg] + red[96 + tg]);
+                const float M = mrow[tg];
+                float       f = 1.0f;
+                if (!whole) {
+                    a.part_ms[(int64_t) slot * a.prow + r] = make_float2(M, L);
+                } else {
+                    if (a.sinks) {  // relative to the larger of the two
+                        const float sk = a.sinks[h] * kLog2e;
+                        if (sk > M) {
+                            f = M == -INFINITY ? 0.0f : exp2a(M - sk);
+                            L = L * f + exp2f(kShift);
+                        } else if (sk > -INFINITY) {
+                            L += exp2a(sk - M + kShift);
                         }
-                        f = L == 0.0f ? 0.0f : f / L;  // a NaN stays one
                     }
-                    fac[r] = f;
+                    f = L == 0.0f ? 0.0f : f / L;  // a NaN stays one
                 }
-                named_bar_sync(bid, 128);
+                fac[tg] = f;
             }
+            named_bar_sync(bid, 128);
             if (n > 0) {
                 pv_wait(gi);
                 tc::fence_after();
             }
-#pragma unroll 1
-            for (int c = 0; c < NC; c++) {
-                const int c0 = g0 + c * CW;
-                if (c0 >= rows) break;
+            if (g0 < rows) {
                 auto put = [&](uint32_t (&o)[CW], int mt, uint32_t) {
-                    float * rec = a.part_acc + ((int64_t) slot * a.prow + c0) * D + 128 * mt + od;
-                    if (PREC && n > kFlush) add_record(o, rec, D, mine ? rows - c0 : 0, frec + c0);
+                    float * rec = a.part_acc + ((int64_t) slot * a.prow + g0) * D + 128 * mt + od;
+                    if (PREC && n > kFlush) add_record(o, rec, D, mine ? rows - g0 : 0, frec);
 #pragma unroll
                     for (int e = 0; e < CW; e++) {
-                        const int r = c0 + e;
+                        const int r = g0 + e;
                         if (!mine || r >= rows) continue;
                         float x = __uint_as_float(o[e]);
                         if (!whole) {
                             rec[e * D] = x;
                             continue;
                         }
-                        const float f = fac[r];
+                        const float f = fac[e];
                         x             = f != 0.0f ? x * f : 0.0f;
                         const int tok = a.byG.div(rb + r), h = w.h * a.G + (rb + r - tok * a.G);
                         uint8_t * dst = a.dst + (int64_t) h * a.dnb1 + (int64_t) (w.r0 + tok) * a.dnb2;
@@ -506,7 +558,7 @@ __global__ void __launch_bounds__(kThr, 1)
                     }
                 };
                 if (n > 0) {
-                    each_o(c0, put);
+                    each_o(put);
                 } else {
                     uint32_t o[CW];
 #pragma unroll
@@ -524,8 +576,10 @@ __global__ void __launch_bounds__(kThr, 1)
                 a.desc[2 * blockIdx.x]     = make_int4(e - (int) blockIdx.x + 1, w.h, w.r0, 0);
             }
             named_bar_sync(bid, 128);  // the rows' numbers are read
+            w      = nw;
+            active = more;
         }
-    } else if (warp < kSm + 1 + kQW) {
+    } else if (warp < kSm + 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Ly::rm));
         if (warp == kSm) {
             // ---------------- MMA ----------------
@@ -533,7 +587,7 @@ __global__ void __launch_bounds__(kThr, 1)
             constexpr uint32_t idpv = tc::idesc(tc::kD_F32, tc::kAB_F16, tc::kAB_F16, tc::kMNMajor, tc::kMNMajor, N, Ly::MM);
             constexpr uint64_t sw   = 2ull << 61;  // 128-byte swizzle
             const uint64_t     qd0  = tc::sdesc(smem_u32(sm + Ly::q), 16, 1024) | sw;  // addresses step by bytes / 16
-            const uint64_t     vd0  = tc::sdesc(smem_u32(sm + Ly::ring), Ly::vtok * 128, 1024) | sw;
+            const uint64_t     vd0  = tc::sdesc(smem_u32(sm + Ly::ring), 32 * 128, 1024) | sw;
             const uint64_t     pd0  = tc::sdesc(smem_u32(sm + Ly::p), kTile * 128, 1024) | sw;
             uint32_t           gi = 0, items = 0;
             for (; active; active = walk_next<N, kTile>(a, w)) {
@@ -571,277 +625,221 @@ __global__ void __launch_bounds__(kThr, 1)
                     if (i + 1 < n) qk(i + 1);
                     const uint32_t g = gi + i, pb = g % PB;
                     const bool     fresh = PREC ? i % kFlush == 0 : i == 0;
-#pragma unroll
-                    for (int ch = 0; ch < CH; ch++) wait_bar(&vfull[(g * CH + ch) % VS], ((g * CH + ch) / VS) & 1, a.status, bad);
                     wait_bar(&pfull[pb], (g / PB) & 1, a.status, bad);
-                    tc::fence_after();
-                    __syncwarp();
-                    if (elect_one()) {
-#pragma unroll
-                        for (int ch = 0; ch < CH; ch++) {
-                            const uint32_t sl = (g * CH + ch) % VS;
 #pragma unroll 1
+                    for (int ch = 0; ch < 4; ch++) {
+                        const uint32_t sl = g % VT * 4 + ch;
+                        wait_bar(&vfull[sl], (g / VT) & 1, a.status, bad);
+                        tc::fence_after();
+                        __syncwarp();
+                        if (elect_one()) {
+#pragma unroll
                             for (int mt = 0; mt < Ly::MT; mt++) {
-                                uint64_t vd = vd0 + (sl * Ly::chunk + mt * 2 * (Ly::vtok * 128)) / 16;
-                                uint64_t pd = pd0 + (pb * Ly::parts * Ly::ptile + ch * (Ly::vtok / 16) * 2048) / 16;
-#pragma unroll 1
-                                for (int j = 0; j < Ly::vtok / 16; j += 2) {
+                                const uint64_t vd = vd0 + (sl * Ly::chunk + mt * 2 * (32 * 128)) / 16;
+                                const uint64_t pd = pd0 + (pb * Ly::parts * Ly::ptile + ch * 4096) / 16;
 #pragma unroll
-                                    for (int k = 0; k < 2; k++) {
+                                for (int k = 0; k < 2; k++) {
 #pragma unroll
-                                        for (int part = 0; part < Ly::parts; part++) {
-                                            tc::mma_f16(tb + Ly::tO + mt * Ly::NP, vd + k * 2048 / 16, pd + (part * Ly::ptile + k * 2048) / 16, idpv,
-                                                        (uint32_t) (!fresh || ch > 0 || j + k > 0 || part > 0));
-                                        }
+                                    for (int part = 0; part < Ly::parts; part++) {
+                                        tc::mma_f16(tb + Ly::tO + mt * Ly::NP, vd + k * 2048 / 16, pd + (part * Ly::ptile + k * 2048) / 16, idpv,
+                                                    (uint32_t) (!fresh || ch > 0 || k > 0 || part > 0));
                                     }
-                                    vd += 4096 / 16;
-                                    pd += 4096 / 16;
                                 }
                             }
                             tc::commit(&vempty[sl]);
+                            if (ch == 3) tc::commit(&pvdone[g & 1]);
                         }
-                        tc::commit(&pvdone[g & 1]);
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
                 gi += n;
             }
-        } else {
-            // ---------------- Q: 16-byte pieces of 8 dims in K's order, 128-byte swizzle; rows that are none as zeros ----------------
-            constexpr int all = N * (D / 8), per = kQW * 32, UN = PREC ? 1 : 2;
-            const int     u0 = tid - (kSm + 1) * 32;
-            uint32_t      items = 0;
+        } else if (warp < kSm + 3) {
+            // ---------------- producers: raw rows, 64 tokens at a time ----------------
+            const bool isk = warp == kSm + 1;
+            const int  NR = isk ? NK : NV;
+            uint64_t * rf = rfull + (isk ? 0 : NK), *re = rempty + (isk ? 0 : NK);
+            const uint32_t raw0 = smem_u32(sm + Ly::raw + (isk ? 0 : NK * Ly::stage));
+            const Pool4 &  pool = isk ? kp : vp;
+            uint32_t       c = 0;  // stages so far
             for (; active; active = walk_next<N, kTile>(a, w)) {
-                if (w.sp.nkv == 0) continue;
-                const int rb = w.rt * N, rows = min(N, w.n * a.G - rb);
+                const int n = w.sp.nkv ? w.take : 0;
+                for (int i0 = 0; i0 < n; i0 += 4) {
+                    // lane j: page of tokens 16 (j % 8) .. of tile i0 + j / 8: four tiles' at a time, as an entry takes 700 cycles
+                    int       ent = -1, y = 0;  // -1: no row sees them
+                    const int ti  = i0 + (lane >> 3);
+                    if (ti < n) {
+                        const int tok = w.tile(ti) * kTile + 16 * (lane & 7);
+                        if (tok < w.sp.hi && tok + 16 > w.sp.lo) {
+                            const int e = a.byPage.div(tok);
+                            y           = tok - e * a.page;
+                            ent         = reinterpret_cast<const int32_t *>(a.table + (int64_t) w.s * a.tstride)[e];
+                            if (ent < 0 || ent >= a.n_pages) {  // no page: reads as zeros
+                                atomicExch(a.status, kErrPage);
+                                ent = a.n_pages;
+                            }
+                        }
+                    }
+                    for (int st = 0; st < 2 * min(4, n - i0); st++, c++) {
+                        const uint32_t sl = c % NR;
+                        if (c >= (uint32_t) NR) wait_bar(&re[sl], (c / NR - 1) & 1, a.status, bad);
+                        if (bad) break;
+                        const uint32_t to = raw0 + sl * Ly::stage;
+                        int            pg[4], yy[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            pg[k] = __shfl_sync(0xffffffffu, ent, 4 * st + k);
+                            yy[k] = __shfl_sync(0xffffffffu, y, 4 * st + k);
+                        }
+                        if (a.box) {
+                            // boxes of 16, 32 or 64 tokens, as pages hold them; one that no row sees is left out
+                            const int bs = a.box >> 4, x = (w.h * Ly::rowb) & ~15;
+                            int       nb = 0;
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                // a box's entry and place stand with its first 16 tokens; where those are not seen, with a later 16
+                                if (k % bs == 0) {
+                                    for (int e = 1; e < bs; e++) {
+                                        if (pg[k] < 0 && pg[(k + e) & 3] >= 0) {
+                                            pg[k] = pg[(k + e) & 3];
+                                            yy[k] = yy[(k + e) & 3] - 16 * e;
+                                        }
+                                    }
+                                    nb += pg[k] >= 0;
+                                }
+                            }
+                            if (elect_one()) {
+                                mbar_arrive_expect_tx(&rf[sl], nb * a.box * Ly::RS);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) {
+                                    if (k % bs == 0 && pg[k] >= 0) tma_rows(to + 16 * k * Ly::RS, isk ? &mk : &mv, x, yy[k], pg[k], &rf[sl]);
+                                }
+                            }
+                            __syncwarp();
+                        } else {
+                            const int64_t hb = w.h * pool.nb2;
 #pragma unroll 1
-                for (int u = u0; u < all; u += UN * per) {
-                    uint2 x[UN][4];
-#pragma unroll
-                    for (int k = 0; k < UN; k++) {
-                        const int v = u + k * per, row = v / (D / 8), pc = v % (D / 8), odd = (pc >> 2) & 1, word = pc & 3;
-#pragma unroll
-                        for (int e = 0; e < 4; e++) x[k][e] = make_uint2(0u, 0u);
-                        if (v < all && row < rows) {
-                            const int       tok = a.byG.div(rb + row), h = w.h * a.G + (rb + row - tok * a.G);
-                            const uint8_t * src = a.q + (int64_t) (w.r0 + tok) * a.qnb1 + (int64_t) h * a.qnb2;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {  // pairs of neighbouring dims: bytes 0, 1 and 2, 3, low and high halves
-                                const int d = (pc >> 2) * 32 + q4::byte_of(odd, word, 2 * (e & 1)) + 16 * (e >> 1);
-                                if constexpr (PREC) {
-                                    x[k][e] = *reinterpret_cast<const uint2 *>(src + 4 * d);
-                                } else {
-                                    x[k][e].x = *reinterpret_cast<const uint32_t *>(src + 2 * d);
-                                }
+                            for (int k = 0; k < kRawTok * 9; k += 32) {
+                                const int     idx = k + lane, tk = idx / 9, pc = idx - 9 * tk, q = tk >> 4;
+                                const int     p = q < 2 ? (q ? pg[1] : pg[0]) : q == 2 ? pg[2] : pg[3], yq = (q < 2 ? (q ? yy[1] : yy[0]) : q == 2 ? yy[2] : yy[3]) + (tk & 15);
+                                const bool    ok = p >= 0 && p < a.n_pages;
+                                const int64_t o = ok ? p * pool.nb3 + yq * pool.nb1 + hb + pc * Ly::CB : 0;
+                                q4::copy_async<Ly::CB>(to + tk * Ly::RS + pc * Ly::CB, pool.p + o, ok ? Ly::CB : 0);
                             }
+                            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&rf[sl])) : "memory");
                         }
                     }
-                    if (u == u0 && items > 0) wait_bar(qempty, (items - 1) & 1, a.status, bad);
-#pragma unroll
-                    for (int k = 0; k < UN; k++) {
-                        const int v = u + k * per, row = v / (D / 8), pc = v % (D / 8);
-                        if (v >= all) break;
-                        uint8_t * to = sm + Ly::q + (pc >> 3) * (N * 128) + row * 128 + (((pc & 7) ^ (row & 7)) << 4);
-                        uint32_t  hw[4], lw[4];
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {  // low halves, high halves
-                            const uint2 A = x[k][2 * e], B = x[k][2 * e + 1];
-                            if constexpr (PREC) {
-                                const float f[4] = { __uint_as_float(A.x), __uint_as_float(B.x), __uint_as_float(A.y), __uint_as_float(B.y) };
-#pragma unroll
-                                for (int m = 0; m < 2; m++) {
-                                    const __half2 h2 = __floats2half2_rn(f[2 * m], f[2 * m + 1]);
-                                    const __half2 l2 = __floats2half2_rn(f[2 * m] - __low2float(h2), f[2 * m + 1] - __high2float(h2));
-                                    hw[2 * e + m] = *reinterpret_cast<const uint32_t *>(&h2);
-                                    lw[2 * e + m] = *reinterpret_cast<const uint32_t *>(&l2);
-                                }
-                            } else {
-                                hw[2 * e]     = q4::prmt(A.x, B.x, 0x5410u);
-                                hw[2 * e + 1] = q4::prmt(A.x, B.x, 0x7632u);
-                            }
-                        }
-                        *reinterpret_cast<uint4 *>(to) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                        if constexpr (PREC) *reinterpret_cast<uint4 *>(to + Ly::qtile) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
-                    }
+                    if (bad) break;
                 }
-                items++;
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(qfull);
+                if (bad) break;
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (bad && a.box) {  // a wait that gave up: the loads in flight land before this CTA's shared memory goes
+                for (uint32_t k = c > (uint32_t) NR ? c - NR : 0; k < c; k++) mbar_wait(&rf[k % NR], (k / NR) & 1);
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Ly::ru));
+        if constexpr (Ly::ru < 72) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Ly::ru));
+        } else {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Ly::ru));
+        }
         // ---------------- unpacking: K into tensor memory, V into swizzled rows ----------------
-        const int      wq = warp & 3;
-        const bool     isk = warp < kSm + 1 + kQW + 4;
-        const Pool4 &  pool = isk ? kp : vp;
-        uint8_t *      raw = sm + Ly::raw + (isk ? wq : 4 + wq) * (ST * Ly::stage);
-        const uint32_t raw0 = smem_u32(raw);
-        // copies: the tile and stage that come next
-        uint64_t * rf = rawfull + (isk ? wq : 4 + wq) * ST;
-        Walk       pw = w;
-        int        pn = w.sp.nkv ? w.take : 0, pi = 0, ph = 0;
-        bool       pact = active;
-        // lane j: page of the (j / 2)-th tile from i0 on, tokens 16 (j & 1) .. of this warp's 32. Sixteen tiles' at a time: a table
-        // entry asked for tile by tile held the warp up for its 700 cycles, half of the tile's time
-        int        ent = -1, i0 = 0;
-        auto       look = [&]() {
-            bool fresh = pi - i0 == 16;
-            while (pact && pi >= pn) {
-                pact = walk_next<N, kTile>(a, pw);
-                pn   = pact && pw.sp.nkv ? pw.take : 0;
-                pi   = 0;
-                fresh = true;
-            }
-            if (pact && fresh) {
-                i0            = pi;
-                const int ti  = pi + (lane >> 1);
-                ent           = -1;
-                if (ti < pn) {
-                    const int tok = pw.tile(ti) * kTile + 32 * wq + 16 * (lane & 1);
-                    if (tok < pw.sp.hi && tok + 16 > pw.sp.lo) {
-                        ent = reinterpret_cast<const int32_t *>(a.table + (int64_t) pw.s * a.tstride)[a.byPage.div(tok)];
-                        if (ent < 0 || ent >= a.n_pages) {  // no page: reads as zeros
-                            atomicExch(a.status, kErrPage);
-                            ent = a.n_pages;
-                        }
-                    }
-                }
-            }
-        };
-        auto issue = [&](int st) {
-            if (!pact) return;
-            const uint32_t to = raw0 + st * Ly::stage;
-            const int      t0 = pw.tile(pi) * kTile + 32 * wq;
-            const int      p0 = __shfl_sync(0xffffffffu, ent, 2 * (pi - i0)), p1 = __shfl_sync(0xffffffffu, ent, 2 * (pi - i0) + 1);  // -1: not seen
-            const int      y0 = t0 - a.byPage.div(t0) * a.page, y1 = t0 + 16 - a.byPage.div(t0 + 16) * a.page;
-            if (a.box) {
-                // boxes of 16 tokens, or of 32 where pages hold them; one that no row sees is left out
-                const int  x = (pw.h * (D / 16 * 9) + ph * Ly::rowb) & ~15;
-                const bool one = a.box == 32, b0 = p0 >= 0 || (one && p1 >= 0), b1 = !one && p1 >= 0;
-                if (elect_one()) {
-                    mbar_arrive_expect_tx(&rf[st], (b0 + b1) * a.box * Ly::RS);
-                    if (b0) tma_rows(to, isk ? &mk : &mv, x, y0, one ? max(p0, p1) : p0, &rf[st]);
-                    if (b1) tma_rows(to + 16 * Ly::RS, isk ? &mk : &mv, x, y1, p1, &rf[st]);
-                }
-                __syncwarp();
-            } else {
-                const int64_t o0 = p0 < 0 || p0 >= a.n_pages ? -1 : p0 * pool.nb3 + y0 * pool.nb1 + pw.h * pool.nb2 + ph * Ly::rowb;
-                const int64_t o1 = p1 < 0 || p1 >= a.n_pages ? -1 : p1 * pool.nb3 + y1 * pool.nb1 + pw.h * pool.nb2 + ph * Ly::rowb;
-#pragma unroll 1
-                for (int k = 0; k < 9; k++) {
-                    const int     idx = 32 * k + lane, tk = idx / 9, pc = idx - 9 * tk;
-                    const int64_t s = tk < 16 ? o0 : o1;
-                    q4::copy_async<Ly::CB>(to + tk * Ly::RS + pc * Ly::CB, pool.p + (s < 0 ? 0 : s + (tk & 15) * pool.nb1 + pc * Ly::CB), s < 0 ? 0 : Ly::CB);
-                }
-                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&rf[st])) : "memory");
-            }
-            if (++ph == Ly::SPT) {
-                ph = 0;
-                pi++;
-                look();
-            }
-        };
-        i0 = -16;
-        look();
-        for (int s = 0; s < ST; s++) issue(s);
-        uint32_t gi = 0, use = 0;
-        int      st = 0;
+        const int  wq = warp & 3, th = wq >> 1;  // 32 tokens of the tile
+        const bool isk = warp < kSm + 4 + kConv / 2;
+        const int  NR = isk ? NK : NV;
+        uint64_t * rf = rfull + (isk ? 0 : NK), *re = rempty + (isk ? 0 : NK);
+        const uint8_t * raw = sm + Ly::raw + (isk ? 0 : NK * Ly::stage) + (32 * (wq & 1) + lane) * Ly::RS;
+        uint32_t        gi = 0;
         for (; active; active = walk_next<N, kTile>(a, w)) {
             const int n = w.sp.nkv ? w.take : 0;
+            const int lead = a.box ? (w.h * Ly::rowb) & 15 : 0;
             for (int i = 0; i < n; i++, gi++) {
-                const uint32_t kb = gi % KB, c = gi * CH + (CH == 2 ? wq >> 1 : 0), sl = c % VS;
-                const int      tok = w.tile(i) * kTile + 32 * wq + lane;
-                const bool     none = tok < w.sp.lo || tok >= w.sp.hi;  // no row sees it: its V row is zeros, as 0 * NaN is NaN
-#pragma unroll 1
-                for (int h = 0; h < Ly::SPT; h++) {
-                    wait_bar(&rf[st], use & 1, a.status, bad);
-                    __syncwarp();
-                    const uint8_t * row  = raw + st * Ly::stage + lane * Ly::RS;
-                    const int       lead = a.box ? (w.h * (D / 16 * 9) + h * Ly::rowb) & 15 : 0;
-                    uint32_t        W[9];  // of a pair of blocks
-                    [[maybe_unused]] uint32_t X[20];
-                    if constexpr (Ly::HD == 128) {  // the whole row: rows of 80 bytes give 16-byte loads without bank conflicts
+                const uint32_t c = 2 * gi + th, sl = c % NR, kb = gi % KB, vs = gi % VT * 4 + wq;
+                wait_bar(&rf[sl], (c / NR) & 1, a.status, bad);
+                __syncwarp();
+                const uint8_t * row = raw + sl * Ly::stage + lead;
+                uint32_t        W[9];  // of a pair of blocks
+                auto            words = [&](int k) {
+                    const uint8_t * r = row + 36 * k;
+                    if constexpr (D == 64) {
 #pragma unroll
-                        for (int e = 0; e < 5; e++) {
-                            const uint4 x = *reinterpret_cast<const uint4 *>(row + 16 * e);
-                            X[4 * e] = x.x; X[4 * e + 1] = x.y; X[4 * e + 2] = x.z; X[4 * e + 3] = x.w;
-                        }
-                    }
-                    auto words = [&](int k) {
+                        for (int e = 0; e < 9; e++) W[e] = *reinterpret_cast<const uint32_t *>(r + 4 * e);
+                    } else if ((k & 1) == 0) {  // 8-byte loads where they stand on 8 bytes
 #pragma unroll
-                        for (int e = 0; e < 9; e++) {
-                            if constexpr (Ly::HD == 128) {
-                                W[e] = lead ? X[9 * k + e + 2] : X[9 * k + e];
-                            } else {
-                                W[e] = *reinterpret_cast<const uint32_t *>(row + lead + 4 * e);
-                            }
+                        for (int e = 0; e < 8; e += 2) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(r + 4 * e);
+                            W[e] = x.x; W[e + 1] = x.y;
                         }
-                    };
-                    if (isk) {
-                        if (h == 0 && gi >= KB) {
-                            wait_bar(&kempty[kb], (gi / KB - 1) & 1, a.status, bad);
-                            tc::fence_after();
-                        }
-                        __syncwarp();
-#pragma unroll
-                        for (int k = 0; k < Ly::HD / 64; k++) {
-                            words(k);
-                            uint32_t       v[16];
-                            const uint32_t at = tc::taddr(tb + Ly::tK + kb * (D / 2) + h * (Ly::HD / 2) + 32 * k, wq, 0);
-                            q4::unpack<false>(W, v);
-                            tc::st16(at, v);
-                            q4::unpack<true>(W, v);
-                            tc::st16(at + 16, v);
-                        }
+                        W[8] = *reinterpret_cast<const uint32_t *>(r + 32);
                     } else {
-                        if (h == 0 && c >= VS) wait_bar(&vempty[sl], (c / VS - 1) & 1, a.status, bad);
-                        uint8_t * to = sm + Ly::ring + sl * Ly::chunk + ((32 * wq) % Ly::vtok + lane) * 128;
+                        W[0] = *reinterpret_cast<const uint32_t *>(r);
 #pragma unroll
-                        for (int k = 0; k < Ly::HD / 64; k++) {
-                            words(k);
-                            if (none) {
-#pragma unroll
-                                for (int e = 0; e < 9; e++) W[e] = 0;
-                            }
-                            uint8_t * pl = to + (h * (Ly::HD / 64) + k) * (Ly::vtok * 128);
-                            uint32_t  v[16];
-                            auto      put = [&](int c0) {
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    *reinterpret_cast<uint4 *>(pl + (((c0 + e) ^ (lane & 7)) << 4)) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-                                }
-                            };
-                            q4::unpack<false>(W, v);
-                            put(0);
-                            q4::unpack<true>(W, v);
-                            put(4);
+                        for (int e = 1; e < 9; e += 2) {
+                            const uint2 x = *reinterpret_cast<const uint2 *>(r + 4 * e);
+                            W[e] = x.x; W[e + 1] = x.y;
                         }
                     }
+                };
+                auto release = [&]() {
                     __syncwarp();
-                    issue(st);
-                    if (++st == ST) {
-                        st = 0;
-                        use++;
-                    }
-                }
+                    if (lane == 0) mbar_arrive(&re[sl]);
+                };
+                constexpr int NP2 = D / 64;  // pairs
+                uint32_t      v[16];
                 if (isk) {
+                    const uint32_t at = tc::taddr(tb + Ly::tK + kb * (D / 2), wq, 0);
+#pragma unroll
+                    for (int k = 0; k < NP2; k++) {
+                        words(k);
+                        if (k == NP2 - 1) release();
+                        q4::unpack<false>(W, v);
+                        if (k == 0) {
+                            if (gi >= KB) wait_bar(&kempty[kb], (gi / KB - 1) & 1, a.status, bad);
+                            tc::fence_after();
+                            __syncwarp();
+                        }
+                        tc::st16(at + 32 * k, v);
+                        q4::unpack<true>(W, v);
+                        tc::st16(at + 32 * k + 16, v);
+                    }
                     tc::wait_st();
                     tc::fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&kfull[kb]);
                 } else {
+                    const int  tok  = w.tile(i) * kTile + 32 * wq + lane;
+                    const bool none = tok < w.sp.lo || tok >= w.sp.hi;  // no row sees it: zeros, as 0 * NaN is NaN
+                    uint8_t *  to   = sm + Ly::ring + vs * Ly::chunk + lane * 128;
+                    auto       put  = [&](int plane, int c0) {
+                        uint8_t * pl = to + plane * (32 * 128);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            *reinterpret_cast<uint4 *>(pl + (((c0 + e) ^ (lane & 7)) << 4)) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                        }
+                    };
+#pragma unroll
+                    for (int k = 0; k < NP2; k++) {
+                        words(k);
+                        if (k == NP2 - 1) release();
+                        if (none) {
+#pragma unroll
+                            for (int e = 0; e < 9; e++) W[e] = 0;
+                        }
+                        q4::unpack<false>(W, v);
+                        if (k == 0 && gi >= VT) {
+                            wait_bar(&vempty[vs], (gi / VT - 1) & 1, a.status, bad);
+                            __syncwarp();
+                        }
+                        put(k, 0);
+                        q4::unpack<true>(W, v);
+                        put(k, 4);
+                    }
                     fence_proxy_async_smem();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&vfull[sl]);
+                    if (lane == 0) mbar_arrive(&vfull[vs]);
                 }
             }
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        // a wait that gave up: the loads in flight land before this CTA's shared memory goes
-        if (bad && a.box) {
-            for (int s = 0; s < ST; s++) mbar_wait(&rf[s], (use + (s < st)) & 1);
         }
     }
     __syncwarp();
@@ -891,8 +889,7 @@ int fap::q4_parts(int rows, int D) { return rows == 8 ? (D == 256 ? 8 : 16) : 1;
 int fap::q4_run(srhpm_ctx * ctx, PArgs & a, const PagedCache & c, int rows, bool f32, cudaStream_t stream) {
     const Pool4 k{ c.k, c.knb1, c.knb2, c.knb3 }, v{ c.v, c.vnb1, c.vnb2, c.vnb3 };
     CUtensorMap maps[2] = {}, &mk = maps[0], &mv = maps[1];
-    // the few-row kernel takes whole rows of 256 values, this file's half a row at a time
-    const int box = rows == 8 && c.D == 256 ? 144 : row_stride(c.D);
+    const int   box = row_stride(c.D);
     // TMA takes the rows where a token's heads stand side by side and tokens and pages start on 16 bytes; other layouts come in
     // pieces by cp.async
     const int rowb = c.D / 16 * 9;
@@ -902,7 +899,8 @@ int fap::q4_run(srhpm_ctx * ctx, PArgs & a, const PagedCache & c, int rows, bool
     };
     a.box = 0;
     if (fits(k) && fits(v)) {
-        a.box = c.page % 32 || (rows == 8 && c.D == 256) ? 16 : 32;  // a step of the few-row kernel has 16 tokens of 256 values
+        // within a page, and within a stage: of the few-row kernel's steps 32 tokens, 16 of 256 values
+        a.box = c.page % 32 || (rows == 8 && c.D == 256) ? 16 : c.page % 64 || rows == 8 ? 32 : 64;
         for (const Pool4 * p : { &k, &v }) {
             // a dimension of one element never steps: any valid stride
             const int64_t s3 = c.n_pages > 1 ? p->nb3 : p->nb1 * c.page;
