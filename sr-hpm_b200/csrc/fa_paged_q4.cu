@@ -90,7 +90,7 @@ template <int D, int N, bool PREC> struct LayT {
     static_assert(total <= 232448 && raw % 128 == 0 && rows >= kMaxSeqs * 8, "shared memory");
     static_assert(tK + KB * D / 2 <= 512, "tensor memory");
     // registers of the softmax warps, of the MMA's and the producers', of the unpacking ones: the launch's 72 a thread, shared out anew
-    static constexpr int rs = N == 128 ? 88 : 72, rm = N == 128 ? 40 : 56, ru = N == 128 ? 56 : 80;
+    static constexpr int rs = N == 96 ? 88 : N == 64 ? 80 : 72, rm = N == 96 ? 40 : 56, ru = N == 96 ? 56 : N == 64 ? 64 : 80;
     static_assert(kSm * 32 * rs + 128 * rm + kConv * 32 * ru <= kThr * 72, "registers");
 };
 
@@ -146,20 +146,16 @@ template <int W> __device__ __forceinline__ void ld_t(uint32_t t, uint32_t (&r)[
               "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
               "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
             : "r"(t));
-    } else if constexpr (W == 16) {
-        tc::ld16(t, r);
     } else {
-        tc::ld4(t, r);
+        tc::ld_cols<W>(t, r);
     }
 }
 template <int W> __device__ __forceinline__ void st_t(uint32_t t, const uint32_t (&r)[W]) {
     if constexpr (W == 32) {
         tc::st16(t, *reinterpret_cast<const uint32_t(*)[16]>(&r[0]));
         tc::st16(t + 16, *reinterpret_cast<const uint32_t(*)[16]>(&r[16]));
-    } else if constexpr (W == 16) {
-        tc::st16(t, r);
     } else {
-        tc::st4(t, r);
+        tc::st_cols<W>(t, r);
     }
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -177,8 +173,14 @@ template <int W> __device__ __forceinline__ void add_record(uint32_t (&o)[W], co
     for (int e = 0; e < W; e++) o[e] = __float_as_uint(fmaf(x[e], f[e], __uint_as_float(o[e])));
 }
 
-// W columns over the warp's 32 lanes: afterwards lane l has the result of column l % W in x[0]
+// W columns (a power of two, or 24) over the warp's 32 lanes: afterwards lane l has the result of column l % W in x[0]
 template <int W, class T, class F> __device__ __forceinline__ float fold(T (&x)[W], F f) {
+    if constexpr (W == 24) {
+        T y[32];
+#pragma unroll
+        for (int k = 0; k < 32; k++) y[k] = k < 24 ? x[k < 24 ? k : 0] : x[0];
+        return fold(y, f);
+    }
     const int lane = threadIdx.x & 31;
     int       n = W;
 #pragma unroll
@@ -468,7 +470,7 @@ __global__ void __launch_bounds__(kThr, 1)
                 tc::fence_before();  // S is read
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sfree[sb]);
-                uint8_t * pr = sm + Ly::p + pb * Ly::parts * Ly::ptile + (g0 >> 6) * (kTile * 128) + (32 * wq + lane) * 128;
+                uint8_t * pr = sm + Ly::p + pb * Ly::parts * Ly::ptile + (32 * wq + lane) * 128;
                 uint32_t  hi[CW / 2];
                 [[maybe_unused]] uint32_t lo[CW / 2];
 #pragma unroll
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(kThr, 1)
                 if constexpr (CW >= 8) {
 #pragma unroll
                     for (int k = 0; k < CW / 2; k += 4) {
-                        uint8_t * to = pr + (((((g0 + 2 * k) >> 3) & 7) ^ (lane & 7)) << 4);
+                        uint8_t * to = pr + ((g0 + 2 * k) >> 6) * (kTile * 128) + (((((g0 + 2 * k) >> 3) & 7) ^ (lane & 7)) << 4);
                         *reinterpret_cast<uint4 *>(to) = make_uint4(hi[k], hi[k + 1], hi[k + 2], hi[k + 3]);
                         if constexpr (PREC) *reinterpret_cast<uint4 *>(to + Ly::ptile) = make_uint4(lo[k], lo[k + 1], lo[k + 2], lo[k + 3]);
                     }
@@ -760,12 +762,12 @@ __global__ void __launch_bounds__(kThr, 1)
                 __syncwarp();
                 const uint8_t * row = raw + sl * Ly::stage + lead;
                 uint32_t        W[9];  // of a pair of blocks
-                auto            words = [&](int k) {
+                auto            words = [&](int k, int odd) {
                     const uint8_t * r = row + 36 * k;
                     if constexpr (D == 64) {
 #pragma unroll
                         for (int e = 0; e < 9; e++) W[e] = *reinterpret_cast<const uint32_t *>(r + 4 * e);
-                    } else if ((k & 1) == 0) {  // 8-byte loads where they stand on 8 bytes
+                    } else if (odd == 0) {  // 8-byte loads where they stand on 8 bytes
 #pragma unroll
                         for (int e = 0; e < 8; e += 2) {
                             const uint2 x = *reinterpret_cast<const uint2 *>(r + 4 * e);
@@ -785,23 +787,24 @@ __global__ void __launch_bounds__(kThr, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&re[sl]);
                 };
-                constexpr int NP2 = D / 64;  // pairs
+                constexpr int NP2 = D / 64, U2 = NP2 < 2 ? NP2 : 2;  // pairs
                 uint32_t      v[16];
                 if (isk) {
                     const uint32_t at = tc::taddr(tb + Ly::tK + kb * (D / 2), wq, 0);
+                    if (gi >= KB) wait_bar(&kempty[kb], (gi / KB - 1) & 1, a.status, bad);
+                    tc::fence_after();
+                    __syncwarp();
+#pragma unroll 1
+                    for (int k0 = 0; k0 < NP2; k0 += U2) {  // not unrolled: the roles' loops share the instruction cache
 #pragma unroll
-                    for (int k = 0; k < NP2; k++) {
-                        words(k);
-                        if (k == NP2 - 1) release();
-                        q4::unpack<false>(W, v);
-                        if (k == 0) {
-                            if (gi >= KB) wait_bar(&kempty[kb], (gi / KB - 1) & 1, a.status, bad);
-                            tc::fence_after();
-                            __syncwarp();
+                        for (int e = 0; e < U2; e++) {
+                            words(k0 + e, e);
+                            if (k0 + e == NP2 - 1) release();
+                            q4::unpack<false>(W, v);
+                            tc::st16(at + 32 * (k0 + e), v);
+                            q4::unpack<true>(W, v);
+                            tc::st16(at + 32 * (k0 + e) + 16, v);
                         }
-                        tc::st16(at + 32 * k, v);
-                        q4::unpack<true>(W, v);
-                        tc::st16(at + 32 * k + 16, v);
                     }
                     tc::wait_st();
                     tc::fence_before();
@@ -818,22 +821,23 @@ __global__ void __launch_bounds__(kThr, 1)
                             *reinterpret_cast<uint4 *>(pl + (((c0 + e) ^ (lane & 7)) << 4)) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                         }
                     };
+                    if (gi >= VT) wait_bar(&vempty[vs], (gi / VT - 1) & 1, a.status, bad);
+                    __syncwarp();
+#pragma unroll 1
+                    for (int k0 = 0; k0 < NP2; k0 += U2) {
 #pragma unroll
-                    for (int k = 0; k < NP2; k++) {
-                        words(k);
-                        if (k == NP2 - 1) release();
-                        if (none) {
+                        for (int e = 0; e < U2; e++) {
+                            words(k0 + e, e);
+                            if (k0 + e == NP2 - 1) release();
+                            if (none) {
 #pragma unroll
-                            for (int e = 0; e < 9; e++) W[e] = 0;
+                                for (int x = 0; x < 9; x++) W[x] = 0;
+                            }
+                            q4::unpack<false>(W, v);
+                            put(k0 + e, 0);
+                            q4::unpack<true>(W, v);
+                            put(k0 + e, 4);
                         }
-                        q4::unpack<false>(W, v);
-                        if (k == 0 && gi >= VT) {
-                            wait_bar(&vempty[vs], (gi / VT - 1) & 1, a.status, bad);
-                            __syncwarp();
-                        }
-                        put(k, 0);
-                        q4::unpack<true>(W, v);
-                        put(k, 4);
                     }
                     fence_proxy_async_smem();
                     __syncwarp();
@@ -871,7 +875,7 @@ int launch_d(srhpm_ctx * ctx, int rows, bool f32, const PArgs & a, const CUtenso
     if (f32) return rows == 16 ? launch_t<D, 16, true>(ctx, a, mk, mv, k, v, stream) : launch_t<D, 64, true>(ctx, a, mk, mv, k, v, stream);
     return rows == 16   ? launch_t<D, 16, false>(ctx, a, mk, mv, k, v, stream)
            : rows == 64 ? launch_t<D, 64, false>(ctx, a, mk, mv, k, v, stream)
-                        : launch_t<D, 128, false>(ctx, a, mk, mv, k, v, stream);
+                        : launch_t<D, 96, false>(ctx, a, mk, mv, k, v, stream);
 }
 
 }  // namespace
@@ -881,7 +885,7 @@ int fap::q4_rows(int T, int S, int G, bool f32) {
     if (R <= (int64_t) S * 8) return 8;
     if (R <= (int64_t) S * 16) return 16;
     if (f32 || R <= (int64_t) S * 64) return 64;
-    return 128;
+    return 96;
 }
 
 int fap::q4_parts(int rows, int D) { return rows == 8 ? (D == 256 ? 8 : 16) : 1; }
