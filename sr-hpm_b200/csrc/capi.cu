@@ -752,7 +752,7 @@ int srhpm_flash_attn_paged_work_size(const srhpm_ctx * ctx, const srhpm_tensor *
     PagedCache c;
     const int  st = check_fa_paged(q, k_cache, k_cache, &c);
     if (st != SRHPM_OK) return st;
-    *size = fa_paged_work_size(ctx, (int) q->ne[1], (int) q->ne[2], c.Hkv, c.D, n_seqs, c.type, q->type == SRHPM_TYPE_F32);
+    *size = fa_paged_work_size(ctx, (int) q->ne[1], (int) q->ne[2], n_seqs, c, q->type == SRHPM_TYPE_F32);
     return SRHPM_OK;
 }
 

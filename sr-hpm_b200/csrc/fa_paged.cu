@@ -1309,6 +1309,18 @@ int launch_tile(srhpm_ctx * ctx, Tile t, const PArgs & a, const CUtensorMap & mk
     else return launch_paged<D, D <= 128 ? 2 : 1, 128, PREC, Q8>(ctx, a, mk, mv, stream);
 }
 
+// Bytes of K's (and of V's) pages as f16 where a q4_0 cache is unpacked once (unpack_q4.cu) and the f16 form attends: f16 rows, more
+// than 1.5 head_dim of them per sequence and KV head. Against tiles unpacked as they come, over 30000 tokens: head_dim 256, 384 rows
+// 134 us (tiles 125), 600 rows 160 (183); 128, 128 rows 106 (95), 256 rows 117 (127); 64, 64 rows 106 (74), 100 rows 111 (135). Not
+// f32 rows, whose sums the f16 form keeps in the tensor cores (off by 2e-5 to 5e-5 over 20000 tokens; fa_paged_q4.cu 6e-6), nor pools
+// beyond kMostUnpacked, which were made q4_0 so that they fit.
+constexpr size_t kMostUnpacked = (size_t) 512 << 20;
+size_t unpacked_bytes(int T, int S, int G, const PagedCache & c, bool f32) {
+    if (c.type != SRHPM_TYPE_Q4_0 || f32 || (int64_t) T * G * 2 <= (int64_t) S * c.D * 3) return 0;
+    const size_t n = (size_t) c.n_pages * c.page * c.Hkv * c.D * 2;
+    return n <= kMostUnpacked ? n : 0;
+}
+
 // parts that the line of units is cut into on each SM
 int parts_of(int kv_type, Tile t, int D) { return kv_type == SRHPM_TYPE_Q4_0 ? q4_parts(t.br, D) : 1; }
 
@@ -1335,10 +1347,16 @@ int fap::merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int row
     return st;
 }
 
-size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int Hkv, int D, int S, int kv_type, bool f32) {
-    const Tile   t     = tile_of(T, S, H / Hkv, D, kv_type, f32);
-    const size_t parts = (size_t) ctx->num_sms * parts_of(kv_type, t, D);
-    const size_t recs  = 2 * parts * record_rows(T, H / Hkv, t);
+size_t fa_paged_work_size(const srhpm_ctx * ctx, int T, int H, int S, const PagedCache & c, bool f32) {
+    const int D = c.D, G = H / c.Hkv;
+    if (size_t n = unpacked_bytes(T, S, G, c, f32)) {
+        PagedCache f = c;
+        f.type       = SRHPM_TYPE_F16;
+        return 2 * n + 128 + fa_paged_work_size(ctx, T, H, S, f, f32);
+    }
+    const Tile   t     = tile_of(T, S, G, D, c.type, f32);
+    const size_t parts = (size_t) ctx->num_sms * parts_of(c.type, t, D);
+    const size_t recs  = 2 * parts * record_rows(T, G, t);
     return recs * D * sizeof(float) + align16(recs * sizeof(float2)) + 2 * parts * sizeof(int4) + 32;
 }
 
@@ -1349,7 +1367,20 @@ int fa_paged_run(srhpm_ctx * ctx, const FaPagedView & v, void * wdata, size_t ws
     const int64_t seen = std::min<int64_t>((int64_t) v.cols * v.c.page, INT32_MAX);
     if (v.c.type != SRHPM_TYPE_Q4_0 && ((int64_t) v.T * G / kFew + 1) * (seen / 64 + 1) > INT32_MAX) return SRHPM_UNSUPPORTED;
     if (v.c.type == SRHPM_TYPE_Q4_0 && ((int64_t) v.T * G / 8 + 1) * (seen / 16 + 1) > INT32_MAX) return SRHPM_UNSUPPORTED;
-    if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.c.Hkv, D, v.S, v.c.type, v.f32)) return SRHPM_ERR_WORKSPACE;
+    if (wdata == nullptr || wsize < fa_paged_work_size(ctx, v.T, v.H, v.S, v.c, v.f32)) return SRHPM_ERR_WORKSPACE;
+    if (const size_t n = unpacked_bytes(v.T, v.S, G, v.c, v.f32)) {
+        uint8_t *   base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(wdata) + 127) & ~(uintptr_t) 127);
+        FaPagedView f    = v;
+        const int   st   = unpack_q4_run(ctx, v, base, base + n, stream);
+        if (st != SRHPM_OK) return st;
+        f.c.type = SRHPM_TYPE_F16;
+        f.c.k    = base;
+        f.c.v    = base + n;
+        f.c.knb2 = f.c.vnb2 = (int64_t) D * 2;
+        f.c.knb1 = f.c.vnb1 = f.c.knb2 * v.c.Hkv;
+        f.c.knb3 = f.c.vnb3 = f.c.knb1 * v.c.page;
+        return fa_paged_run(ctx, f, base + 2 * n, wsize - (size_t) (base + 2 * n - static_cast<uint8_t *>(wdata)), stream);
+    }
     const Tile tl = tile_of(v.T, v.S, G, D, v.c.type, v.f32);
     PArgs      a;
     a.q       = v.q;

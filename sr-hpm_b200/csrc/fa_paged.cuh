@@ -243,6 +243,9 @@ int q4_parts(int rows, int D);
 int q4_few_run(srhpm_ctx * ctx, const PArgs & a, const void * maps, const PagedCache & c, bool f32, cudaStream_t stream);  // fa_paged_q4_few.cu
 int q4_run(srhpm_ctx * ctx, PArgs & a, const PagedCache & c, int rows, bool f32, cudaStream_t stream);
 
+// every page that a row sees, as f16 [pages][page][Hkv][D] under its own number (unpack_q4.cu); cols * page < 2^31 + 16
+int unpack_q4_run(srhpm_ctx * ctx, const FaPagedView & v, void * ko, void * vo, cudaStream_t stream);
+
 // tensor map of bytes [pages][tokens][width], boxes of `tokens_box` rows of `box` bytes (fa_paged.cu); false: not encoded
 bool encode_rows(void * map, const void * p, uint64_t width, int tokens, int64_t pages, int64_t nb1, int64_t nb3, int box, int tokens_box);
 

@@ -332,3 +332,29 @@ def test_attention_large_steps(ctx):
         vals = [X.q4_values(c) for c in caches]
         attn_run(ctx, (q, caches, vals, table, q_start, kv_len), Q4, 0.05)
     ctx.check()
+
+
+@pytest.mark.parametrize("D,H,Hkv", [(256, 6, 1), (256, 6, 3), (128, 14, 2), (64, 4, 4), (64, 1, 1)])
+@pytest.mark.parametrize("window", [0, 1, 100, 600])
+def test_attention_prompts(ctx, D, H, Hkv, window):
+    """Sequences that share the pages of a common beginning and bring rows by the hundred; one brings none, one has fewer cached tokens
+    than rows; released entries before a window; pages of [head][token] and K/V in one pool."""
+    rng = np.random.default_rng(16)
+    P, new = 48, [500, 0, 410, 390]
+    q, caches, vals, table, q_start, kv_len = case4(rng, [700, 5, 301, 0], new, H, Hkv, D, P, torch.float16, pad_rows=3)
+    table[2, :4] = table[0, :4]
+    kv_len[3] = 333
+    if window == 100:
+        table[0, :(700 - window + 1) // P] = [-1, 2 ** 30, -7, vals[0].shape[0]] * 3
+    heads = [cu(c).transpose(1, 2).contiguous().transpose(1, 2) for c in caches]
+    both = torch.stack([cu(c) for c in caches], 2)
+    first = None
+    for k, v in ((cu(caches[0]), cu(caches[1])), heads, (both[:, :, 0], both[:, :, 1])):
+        out = torch.full(q.shape, 7.0, device="cuda", dtype=torch.float16)
+        ctx.flash_attn_paged(cu(q), k, v, Q4, cu(table), cu(q_start), cu(kv_len), scale=D ** -0.5, window=window, out=out)
+        assert (out[-3:] == 7.0).all()  # rows behind the last sequence
+        if first is None:
+            first = out
+            attn_check(out.cpu().numpy(), q, vals, table, q_start, kv_len, D ** -0.5, window=window)
+        assert torch.equal(out, first)
+    ctx.check()
