@@ -222,19 +222,28 @@ struct SetArgs {
 };
 
 // visits the table entries of this cluster's rows, kForkChunk at a time per warp: f(pointer to the entry)
-template <class F> __device__ __forceinline__ void each_entry(const SetArgs & a, int rank, int ctas, F f) {
+// For each entry in range: p = take(entry), then r = look(p) for those that are pages, then use(entry, p, r). Each of the three
+// goes over a warp's 256 entries before the next, so that a round trip is waited for once and not eight times (48 of
+// 1024 sequences freed, 12000 pages: 19 us, now 15.6).
+template <class Take, class Look, class Use>
+__device__ __forceinline__ void each_entry(const SetArgs & a, int rank, int ctas, Take take, Look look, Use use) {
+    constexpr int K    = kForkChunk / 32;
     const int     lane = threadIdx.x & 31;
     const int64_t jobs = (int64_t) a.n * a.chunks, nwarp = (int64_t) ctas * (blockDim.x / 32);
     for (int64_t j = (int64_t) rank * (blockDim.x / 32) + (threadIdx.x >> 5); j < jobs; j += nwarp) {
-        const int i = (int) (j / a.chunks), c0 = (int) (j - (int64_t) i * a.chunks) * kForkChunk;
+        const int i = (int) (j / a.chunks), c0 = (int) (j - (int64_t) i * a.chunks) * kForkChunk + lane;
         const int row = a.rows ? a.rows[i] : i;
-        if (row < 0 || row >= a.trows) continue;
         const int lo = max(a.begin ? a.begin[i] : 0, 0), hi = min(a.end[i], a.cols);
-        int32_t * e  = reinterpret_cast<int32_t *>(a.table + (int64_t) row * a.tstride);
+        if (row < 0 || row >= a.trows) continue;
+        int32_t * e = reinterpret_cast<int32_t *>(a.table + (int64_t) row * a.tstride) + c0;
+        int       p[K], r[K];
 #pragma unroll
-        for (int k = 0; k < kForkChunk / 32; k++) {
-            const int c = c0 + 32 * k + lane;
-            if (c >= lo && c < hi) f(e + c);
+        for (int k = 0; k < K; k++) p[k] = c0 + 32 * k >= lo && c0 + 32 * k < hi ? take(e + 32 * k) : -1;
+#pragma unroll
+        for (int k = 0; k < K; k++) r[k] = p[k] >= 0 && p[k] < a.n_pages ? look(p[k]) : 0;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (p[k] >= 0 && p[k] < a.n_pages) use(e + 32 * k, p[k], r[k]);
         }
     }
 }
@@ -250,13 +259,12 @@ __global__ void __launch_bounds__(kSetThreads) page_free_kernel(const SetArgs a)
     for (int i = threadIdx.x; i < words; i += blockDim.x) bits[i] = 0;
     pdl_wait();
     cl.sync();
-    each_entry(a, rank, ctas, [&](int32_t * e) {
-        const int p = atomicExch(e, -1);  // an entry that is listed twice is freed once
-        if (p < 0 || p >= a.n_pages) return;
-        if (atomicSub(a.refs + p, 1) <= 0) {  // no holder left
-            const int q = p & ((1 << a.shift) - 1);
-            atomicOr(cl.map_shared_rank(bits, p >> a.shift) + (q >> 5), 1u << (q & 31));
-        }
+    auto take = [](int32_t * e) { return atomicExch(e, -1); };  // an entry that is listed twice is freed once
+    auto drop = [&](int p) { return atomicSub(a.refs + p, 1); };
+    each_entry(a, rank, ctas, take, drop, [&](int32_t *, int p, int others) {
+        if (others > 0) return;
+        const int q = p & ((1 << a.shift) - 1);
+        atomicOr(cl.map_shared_rank(bits, p >> a.shift) + (q >> 5), 1u << (q & 31));
     });
     cl.sync();
     // words of a thread stand side by side
@@ -299,12 +307,10 @@ __global__ void __launch_bounds__(kSetThreads) page_compact_kernel(const SetArgs
     for (int i = threadIdx.x; i < words; i += blockDim.x) bits[i] = 0;
     pdl_wait();
     cl.sync();
-    each_entry(a, rank, ctas, [&](int32_t * e) {
-        const int p = *e;
-        if (p < 0 || p >= a.n_pages) return;
-        const int  q = p & ((1 << a.shift) - 1);
-        uint32_t * w = cl.map_shared_rank(bits, p >> a.shift) + (q >> 5);
-        atomicOr(w, 1u << (q & 31));
+    auto read = [](int32_t * e) { return *e; };
+    each_entry(a, rank, ctas, read, [](int) { return 0; }, [&](int32_t *, int p, int) {
+        const int q = p & ((1 << a.shift) - 1);
+        atomicOr(cl.map_shared_rank(bits, p >> a.shift) + (q >> 5), 1u << (q & 31));
     });
     cl.sync();
     const int per = (words + blockDim.x - 1) / blockDim.x, w0 = min((int) threadIdx.x * per, words), w1 = min(w0 + per, words);
@@ -364,11 +370,12 @@ __global__ void __launch_bounds__(kSetThreads) page_compact_kernel(const SetArgs
             a.refs[d] = a.refs[s];
             a.refs[s] = 0;
         }
-        each_entry(a, rank, ctas, [&](int32_t * e) {
-            const int p = *e;
-            if (p < used || p >= a.n_pages) return;
+        auto place = [&](int p) {
             const int o = p >> a.shift;
-            *e = __ldcg(a.dst + before(cl.map_shared_rank(bits, o), cl.map_shared_rank(pre, o), p) - low);
+            return p < used ? p : __ldcg(a.dst + before(cl.map_shared_rank(bits, o), cl.map_shared_rank(pre, o), p) - low);
+        };
+        each_entry(a, rank, ctas, read, place, [](int32_t * e, int p, int to) {
+            if (to != p) *e = to;
         });
     }
     cl.sync();

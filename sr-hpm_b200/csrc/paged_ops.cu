@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
 // the first threads into shared memory while the row's loads are in flight. Bandwidth bound: a row is read once and
 // every output written once. A thread holds 4 pairs (two 16-byte loads); a row's loads go out before its angles. 8192 rows
 // of 32 + 2 * 8 heads of 128 into f16 pages: 49 us, 0.94 of the copy rate; 4001 rows of 24 + 2 * 4 of 256 into q8_0: 32.5,
-// 0.89; 9 rows 4.2 (the launch).
+// 0.89; 9 rows 4.2 (the launch). q4_0 pages: 67 us, and 2048 rows of 24 + 2 * 4 of 256 31: the numbers take a third of the
+// instructions, and the rare rotation in 64 bits has registers of its own (in the loop 75 us, capped at 3 CTAs per SM by them).
 constexpr int kStoreThreads = 256;
 constexpr int kMaxHalf      = 128;
 
@@ -195,7 +196,7 @@ struct StoreArgs {
     const uint8_t * qkv;
     int64_t         ldb;
     int             n, H, Hkv, D;
-    FastDiv         by_units;
+    FastDiv         by_units, by_page;
     const int32_t * pos;
     const int64_t * slots;
     uint8_t *       q;  // token stride qnb1, head stride qnb2
@@ -245,46 +246,44 @@ __device__ __forceinline__ void put4_q8(uint8_t * dst, int j, float4 v, int mode
     w[1]         = (uint16_t) ((q[2] & 0xff) | (q[3] & 0xff) << 8);
 }
 
-// what the 8 lanes of a q4_0 block need: -1/8 of its value of largest size (the first of equals) and the reciprocal
+// what the 8 lanes of a q4_0 block need: -1/8 of its value of largest size (the first of equals; a NaN is never it) and the
+// reciprocal
 struct Step4 {
     float d, id;
 };
-__device__ __forceinline__ Step4 step_q4(int j, float4 v, uint32_t mask) {
+__device__ __forceinline__ Step4 step_q4(float4 v, uint32_t mask) {
     const float x[4] = { v.x, v.y, v.z, v.w };
-    float       amax = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+    float       m = 0.0f;
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
-    int at = 64;  // 2 * place + sign
+    for (int e = 0; e < 4; e++) m = fabsf(x[e]) > fabsf(m) ? x[e] : m;
 #pragma unroll
-    for (int e = 3; e >= 0; e--) {
-        if (fabsf(x[e]) == amax) at = 2 * ((j & 31) + e) + (x[e] < 0.0f);
+    for (int o = 1; o <= 4; o <<= 1) {
+        const float w = __shfl_xor_sync(mask, m, o);
+        if (fabsf(w) > fabsf(m) || (fabsf(w) == fabsf(m) && (threadIdx.x & o))) m = w;
     }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) at = min(at, __shfl_xor_sync(mask, at, o));
-    const float d = ((at & 1) ? amax : -amax) * 0.125f;
-    return { d, d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f };
+    const float d = m * -0.125f;
+    return { d, d != 0.0f ? __frcp_rn(d) : 0.0f };
 }
-__device__ __forceinline__ float level_q4(float x, float id) { return __fadd_rn(__fmul_rn(x, id), 8.5f); }
-// a value stands so near to the border of two numbers that the rounding of its rotation may decide
-__device__ __forceinline__ bool near_q4(float4 v, float id) {
+// The numbers of 4 values, a byte each: x / d + 8.5 rounded down, 0 to 15 (NaN: 0). Added to 256 rounding down, the sum's bits hold
+// the number above 15 places of the fraction: the conversion instruction has an eighth of that rate. near: a value stands within
+// 2^-15 of the border of two numbers, where the rounding of its rotation may decide.
+__device__ __forceinline__ uint32_t numbers_q4(float4 v, float id, bool & near) {
     const float x[4] = { v.x, v.y, v.z, v.w };
-    bool        r = false;
+    uint32_t    n[4], low = 0x7fff;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        const float y = level_q4(x[e], id);
-        r |= fabsf(y - rintf(y)) < 0x1p-15f;
+        const float y = fminf(fmaxf(__fadd_rn(__fmul_rn(x[e], id), 8.5f), 0.0f), 15.75f);
+        n[e] = __float_as_uint(__fadd_rd(y, 256.0f));
+        low  = min(low, (n[e] + 1) & 0x7fffu);
     }
-    return r;
+    near |= low < 2;
+    return (n[0] >> 15 & 0xfu) | (n[1] >> 7 & 0xf00u) | (n[2] << 1 & 0xf0000u) | (n[3] << 9 & 0xf000000u);
 }
 // 4 of the 32 values of a q4_0 block: byte j holds number j in its low and number j + 16 in its high half
-__device__ __forceinline__ void put4_q4(uint8_t * dst, int j, float4 v, Step4 s, uint32_t mask) {
-    const float x[4] = { v.x, v.y, v.z, v.w };
-    uint32_t    q = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) q |= (uint32_t) min(max(__float2int_rz(level_q4(x[e], s.id)), 0), 15) << (8 * e);
+__device__ __forceinline__ void put4_q4(uint8_t * dst, int j, uint32_t q, float d, uint32_t mask) {
     const uint32_t up = __shfl_xor_sync(mask, q, 4);
     uint8_t *      b  = dst + (j >> 5) * 18;
-    if ((j & 31) == 0) *reinterpret_cast<__half *>(b) = __float2half_rn(s.d);
+    if ((j & 31) == 0) *reinterpret_cast<__half *>(b) = __float2half_rn(d);
     if ((j & 16) == 0) {
         const uint32_t w = q | up << 4;
         uint16_t *     p = reinterpret_cast<uint16_t *>(b + 2 + (j & 15));
@@ -293,22 +292,32 @@ __device__ __forceinline__ void put4_q4(uint8_t * dst, int j, float4 v, Step4 s,
     }
 }
 
-// 4 pairs turned in 64 bits
-__device__ __noinline__ void turn64(float4 & l, float4 & h, double pos, const double * freq) {
-    float * x = reinterpret_cast<float *>(&l);
-    float * y = reinterpret_cast<float *>(&h);
+// 4 pairs of a key's block and the one half a head further, turned in 64 bits (8 lanes, 32 pairs). Not inlined and from the row
+// itself: the registers that it needs would cost the kernel a third of its warps.
+__device__ __noinline__ void redo_q4(const float * x, int half, double pos, const double * freq, uint8_t * dst, int j, uint32_t mask) {
+    float l[4] = {}, h[4] = {};
+#pragma unroll 1
     for (int e = 0; e < 4; e++) {
-        double turns = pos * freq[e], s, c;
+        double turns = pos * freq[j + e], s, c;
         turns -= rint(turns);
         sincospi(2.0 * turns, &s, &c);
-        const double a = x[e], b = y[e];
-        x[e] = (float) (a * c - b * s);
-        y[e] = (float) (a * s + b * c);
+        const double a = x[j + e], b = x[half + j + e];
+        const float  nl = (float) (a * c - b * s), nh = (float) (a * s + b * c);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            l[i] = i == e ? nl : l[i];
+            h[i] = i == e ? nh : h[i];
+        }
     }
+    const float4 lo = make_float4(l[0], l[1], l[2], l[3]), hi = make_float4(h[0], h[1], h[2], h[3]);
+    const Step4  sl = step_q4(lo, mask), sh = step_q4(hi, mask);
+    bool         near = false;
+    put4_q4(dst, j, numbers_q4(lo, sl.id, near), sl.d, mask);
+    put4_q4(dst, half + j, numbers_q4(hi, sh.id, near), sh.d, mask);
 }
 
 template <bool QF16, int KV>
-__global__ void __launch_bounds__(kStoreThreads) rope_kv_paged_kernel(const __grid_constant__ StoreArgs a) {
+__global__ void __launch_bounds__(kStoreThreads, 4) rope_kv_paged_kernel(const __grid_constant__ StoreArgs a) {
     __shared__ __align__(16) float cs[2][kMaxHalf], sn[2][kMaxHalf];
     constexpr int NU = 3;  // units of a thread in flight: 48 heads of 128 or 32 of 256 in one turn
     pdl_launch_dependents();
@@ -343,7 +352,7 @@ __global__ void __launch_bounds__(kStoreThreads) rope_kv_paged_kernel(const __gr
             cs[par][threadIdx.x] = c;
             sn[par][threadIdx.x] = s;
         }
-        const int64_t pg = keep ? slot / a.page : 0, off = keep ? slot - pg * a.page : 0;
+        const int64_t pg = !keep ? 0 : a.n_slots <= INT32_MAX ? a.by_page.div((int) slot) : slot / a.page, off = keep ? slot - pg * a.page : 0;
         uint8_t *     kd = a.kc + pg * a.knb3 + off * a.knb1;
         uint8_t *     vd = a.vc + pg * a.vnb3 + off * a.vnb1;
         uint8_t *     qd = a.q + (int64_t) t * a.qnb1;
@@ -355,7 +364,6 @@ __global__ void __launch_bounds__(kStoreThreads) rope_kv_paged_kernel(const __gr
                 const int u = u0 + k * kStoreThreads;
                 if (u >= total) break;
                 const int hh = a.by_units.div(u), j = (u - hh * units) * 4;
-                [[maybe_unused]] const float4 l0 = lo[k], h0 = hi[k];
                 if (hh < a.H + a.Hkv) {
                     const float4 c = *reinterpret_cast<const float4 *>(cs[par] + j), s = *reinterpret_cast<const float4 *>(sn[par] + j);
                     const float4 l = lo[k], h = hi[k];
@@ -372,18 +380,17 @@ __global__ void __launch_bounds__(kStoreThreads) rope_kv_paged_kernel(const __gr
                     uint8_t *  d   = isk ? kd + (int64_t) g * a.knb2 : vd + (int64_t) g * a.vnb2;
                     [[maybe_unused]] const uint32_t oct = 0xffu << (threadIdx.x & 24);
                     if constexpr (KV == SRHPM_TYPE_Q4_0) {
-                        Step4 sl = step_q4(j, lo[k], oct), sh = step_q4(half + j, hi[k], oct);
+                        const Step4 sl = step_q4(lo[k], oct), sh = step_q4(hi[k], oct);
+                        bool           near = false;
+                        const uint32_t ql = numbers_q4(lo[k], sl.id, near), qh = numbers_q4(hi[k], sh.id, near);
                         // a number hangs on the 32-bit rotation only where a value is next to a border: there the whole
                         // block's are taken in 64 bits (one block in 500)
-                        if (isk && (__ballot_sync(oct, near_q4(lo[k], sl.id) || near_q4(hi[k], sh.id)) & oct)) {
-                            lo[k] = l0;
-                            hi[k] = h0;
-                            turn64(lo[k], hi[k], (double) a.pos[t], a.freq + j);
-                            sl = step_q4(j, lo[k], oct);
-                            sh = step_q4(half + j, hi[k], oct);
+                        if (isk && (__ballot_sync(oct, near) & oct)) {
+                            redo_q4(reinterpret_cast<const float *>(row) + hh * a.D, half, (double) a.pos[t], a.freq, d, j, oct);
+                        } else {
+                            put4_q4(d, j, ql, sl.d, oct);
+                            put4_q4(d, half + j, qh, sh.d, oct);
                         }
-                        put4_q4(d, j, lo[k], sl, oct);
-                        put4_q4(d, half + j, hi[k], sh, oct);
                     } else if constexpr (KV == SRHPM_TYPE_Q8_0) {
                         put4_q8(d, j, lo[k], a.q8mode, oct);
                         put4_q8(d, half + j, hi[k], a.q8mode, oct);
@@ -461,6 +468,7 @@ int rope_kv_paged_run(srhpm_ctx * ctx, const uint8_t * qkv, int64_t ldb, int n, 
     a.vnb3    = c.vnb3;
     a.page    = c.page;
     a.n_slots = c.n_pages * c.page;
+    a.by_page = FastDiv::of((uint32_t) c.page);
     a.q8mode  = ctx->q8_0_act_mode;
     // the frequencies of a model stay the same from call to call: 128 powers took the host 5 us of a 9-row step
     {

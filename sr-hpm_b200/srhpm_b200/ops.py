@@ -67,6 +67,7 @@ PageMoves = collections.namedtuple("PageMoves", "src dst n_moves n_used")
 # The calls of a serving step are short on the GPU, so their host side is kept short too: a view is the bytes of an
 # srhpm_tensor (type, ne[4], nb[4], data), packed in one go.
 _pack = struct.Struct("@iqqqqNNNNP").pack
+_address = struct.Struct("@P")  # the last of them
 assert struct.calcsize("@iqqqqNNNNP") == ctypes.sizeof(L.SrhpmTensor)
 
 
@@ -107,6 +108,16 @@ def _paged(c, kv_type):
     if rowb % size:
         raise ValueError("row bytes do not hold whole blocks of the cache type")
     return _pack(kv_type, rowb // size * blk, P, Hkv, n, size, n1, n2, n3, c.data_ptr())
+
+
+def _pools(caches, kv_type):
+    """Views of paged caches; those laid out like the first one differ from its view in the address alone."""
+    if not caches:
+        raise ValueError("no cache")
+    first = caches[0]
+    head, u8, shape, stride = _paged(first, kv_type)[:-_address.size], torch.uint8, first.shape, first.stride()
+    return b"".join([head + _address.pack(c.data_ptr()) if c.shape == shape and c.stride() == stride and c.dtype is u8
+                     else _paged(c, kv_type) for c in caches])
 
 
 def _ints(t, dtype, n, what):
@@ -612,7 +623,7 @@ class Context:
         page_size, Hkv, row bytes] of one shape and layout, in one launch (srhpm_page_copy). n_moves int32 [1]: only that many."""
         self._on_device(src, dst, n_moves, *caches)
         n = src.numel()
-        self._call(self.lib.srhpm_page_copy, "srhpm_page_copy", stream, b"".join([_paged(c, kv_type) for c in caches]),
+        self._call(self.lib.srhpm_page_copy, "srhpm_page_copy", stream, _pools(caches, kv_type),
                    len(caches), _ints(src, torch.int32, n, "src"), _ints(dst, torch.int32, n, "dst"), n,
                    None if n_moves is None else _ints(n_moves, torch.int32, 1, "n_moves"))
 
