@@ -6,8 +6,10 @@
 // else of one row. The window's tokens that fall into the slice are counted in shared memory once per CTA; a warp has the same 512
 // tokens of every row, lists those with a rule once, and from then on waits for no other: a row comes in, goes through the warp's
 // shared memory, where 32 listed tokens at a time take their values, and out with the mask applied. From one row to the next the window
-// moves by a token. (64 sequences: each row's window counted anew in each of its slices 201 us; listed tokens fetched and written behind the
-// copy 154; barriers of the CTA around the listed tokens 142; rules applied by the lane that holds the token 180.)
+// moves by a token. 64 sequences of 2 to 8 rows of 151936, windows of 4096: 100 us, 4.6 TB/s of what has to move. (Four CTAs per SM,
+// whose 64 registers spill, 121; sequences one after another in the grid 109, the last ones alone at its end; each row's window
+// counted anew in each of its slices 201; listed tokens fetched and written behind the copy 154; barriers of the CTA around the
+// listed tokens 142; rules applied by the lane that holds the token 180.)
 // The result does not hang on the order of the atomics: counts are whole numbers, and a token that is biased twice takes the
 // later value.
 #include <cuda_runtime.h>
@@ -34,7 +36,7 @@ struct Args {
 };
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 3) adjust_logits_kernel(const __grid_constant__ Args a) {
     static_assert(kVec == 4, "a thread's 16 tokens");
     extern __shared__ __align__(16) uint32_t cnt[];               // [kSlice] times in the window, kListed
     uint32_t * bix  = cnt + kSlice;                               // [kSlice] 1 + index of the token's bias, then its value
@@ -42,7 +44,9 @@ __global__ void __launch_bounds__(kThreads, 4) adjust_logits_kernel(const __grid
     uint16_t * list = reinterpret_cast<uint16_t *>(xs + kSlice) + (threadIdx.x >> 5) * kWarpTok;
     const LogitView & v = a.v;
     const int         tid = threadIdx.x, lane = tid & 31, w0 = (tid >> 5) * kWarpTok;
-    const int         unit = blockIdx.x / a.slices, x0 = (blockIdx.x - unit * a.slices) * kSlice, nx = min(kSlice, v.V - x0);
+    // slice by slice with all sequences of each, so that those with many rows are spread over the grid; row by row otherwise
+    const int unit = a.by_seq ? blockIdx.x % v.S : blockIdx.x / a.slices;
+    const int x0 = (a.by_seq ? blockIdx.x / v.S : blockIdx.x - unit * a.slices) * kSlice, nx = min(kSlice, v.V - x0);
     pdl_launch_dependents();
     pdl_wait();
     int s, r0, r1, first;
