@@ -354,15 +354,17 @@ int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, i
  * f32. f32 rows: q and the probabilities are taken as sums of two f16 parts: off by at most 2^-22 of themselves, or
  * 2^-25 (q) and 2^-32 of the row's largest (probabilities) where that is more, beside f32 sums. A q8_0 or q4_0
  * cache is read as d * q or d * (q - 8) rounded to f16 (2^-11 of each value), with f32 rows too. head_dim 64, 128 or 256
- * (q8_0: 256); page_size a multiple of 16; cache data aligned to 16 bytes and its strides multiples of 16 (q4_0: of head_dim
- * / 16 bytes); q and dst 16-byte aligned with strides
+ * (q8_0: 256); page_size a multiple of 16; cache data aligned to 16 bytes and its strides multiples of 16 (q4_0: both of
+ * head_dim / 16 bytes, which rows side by side always have); q and dst 16-byte aligned with strides
  * multiples of 16. Cache slots behind a sequence's kv_len and before its window may hold anything, and pages wholly
  * before the window may be given away (their entries are not read). A table entry that is not a page of the cache
  * reads as zeros and raises the context's device status; positions behind the table's entries are not seen. Where the
  * scores of a row hold a NaN, its result is NaN; a value of the cache that is infinite or NaN reaches every row of
  * its sequence if one of them sees it. f32 q: finite in f16's range. dst overlaps neither q nor the caches. n_seqs <=
- * 8192, and (T * n_head / n_head_kv / 56 + 1) * (entries * page_size / 64 + 1) < 2^31 (else SRHPM_UNSUPPORTED).
- * wdata: srhpm_flash_attn_paged_work_size bytes, of the call alone until it is done. */
+ * 8192, and (T * n_head / n_head_kv / 56 + 1) * (entries * page_size / 64 + 1) < 2^31, over q4_0 with 8 and 16 in place of 56
+ * and 64 (else SRHPM_UNSUPPORTED).
+ * wdata: srhpm_flash_attn_paged_work_size bytes, of the call alone until it is done; for f16 rows of prompts over a q4_0 cache (more
+ * than 1.5 head_dim rows per sequence and KV head, padding included) the pools as f16 are among them, up to 1 GiB. */
 int srhpm_flash_attn_paged_work_size(const srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_tensor * k_cache,
                                      int n_seqs, size_t * size);
 int srhpm_flash_attn_paged(srhpm_ctx * ctx, const srhpm_tensor * q, const srhpm_tensor * k_cache,
@@ -403,7 +405,9 @@ int srhpm_verify_sample(srhpm_ctx * ctx, const srhpm_tensor * logits, const int3
  * [n_forks], of srhpm_page_status: a refused fork writes no entry and takes nothing; SRHPM_PAGES_BAD_LENGTH also for a row
  * that the table lacks and for parent = child. An entry that is no page is handed on uncounted; if it is the partly filled
  * one's, a page is taken and nothing copied. No two forks have one child, and no child is a parent of the same call (the rows
- * then hold either's entries). Nothing else of the table is written. n_forks <= 8192. No output shares memory with an input
+ * then hold either's entries). The child's row names no page before that is not given up elsewhere. Nothing else of the table
+ * is written. Shared pages are not written to as long as neither sequence's n_past falls below n_keep[i] (below it, it
+ * would write into what the other reads). n_forks <= 8192. No output shares memory with an input
  * or another output (SRHPM_ERR_INVALID). Not before n_keep[i] tokens of the parent are stored: calls are ordered on the
  * stream. */
 int srhpm_page_fork(srhpm_ctx * ctx, const int32_t * parent, const int32_t * child, const int32_t * n_keep, int n_forks,
@@ -413,8 +417,8 @@ int srhpm_page_fork(srhpm_ctx * ctx, const int32_t * parent, const int32_t * chi
 
 /* srhpm_page_copy: page src[i] copied to page dst[i], i < n (i32 [n]; where either is not a page, nothing), in each of
  * n_caches pools (an array of views in HOST memory: K and V of every layer, say), in one launch per 256 of them. The pools
- * have one type (f16, q8_0 or q4_0), shape and strides (any multiples of 2). n_moves i32 [1] or NULL: only the first *n_moves. No dst stands
- * twice or is a src of the same call (its page then holds either's bytes). */
+ * have one type (f16, q8_0 or q4_0), shape and strides (any multiples of 2). n_moves i32 [1] or NULL: only the first
+ * *n_moves. No dst stands twice or is a src of the same call (its page then holds either's bytes). */
 int srhpm_page_copy(srhpm_ctx * ctx, const srhpm_tensor * caches, int n_caches, const int32_t * src, const int32_t * dst, int n,
                     const int32_t * n_moves, void * stream);
 
@@ -432,8 +436,9 @@ int srhpm_page_free(srhpm_ctx * ctx, const int32_t * rows, const int32_t * begin
 /* srhpm_page_compact: the pages in use (named by the first n_held[s] entries of the block table's rows; i32 [n_seqs]) get the
  * lowest numbers, so that the pool's end can be given away: with n_used of them, the k-th page in use from n_used on goes to
  * the k-th number below n_used that is not. The table's entries and page_refs follow, free_pages (i32 [n_pages]) becomes the
- * number i at place i for n_used <= i < n_pages (its head is n_used from here on; the places before it stay), and src, dst (i32 [n_pages / 2]),
- * n_moves, n_used (i32 [1]) say what srhpm_page_copy has to move; entries behind n_moves stay as they are. n_pages <= 2^22.
+ * number i at place i for n_used <= i < n_pages (its head is n_used from here on; the places before it stay), and src, dst
+ * (i32 [n_pages / 2]), n_moves, n_used (i32 [1]) say what srhpm_page_copy has to move; entries behind n_moves stay as they
+ * are. n_pages <= 2^22.
  * No output shares memory with an input or another output (SRHPM_ERR_INVALID). */
 int srhpm_page_compact(srhpm_ctx * ctx, const srhpm_tensor * block_table, const int32_t * n_held, int32_t * page_refs, int n_pages,
                        int32_t * free_pages, int32_t * src, int32_t * dst, int32_t * n_moves, int32_t * n_used, void * stream);
@@ -450,9 +455,9 @@ int srhpm_page_compact(srhpm_ctx * ctx, const srhpm_tensor * block_table, const 
  *   mask        l = -inf where bit x % 32 of word x / 32 is 0 in the row's mask (mask i32, ne = [>= ceil(n_vocab / 32),
  *               masks], or NULL): mask_row[r] (i32 [T]; outside the masks: none), or r where mask_row is NULL
  * each step rounded to f32. out f32 [n_vocab, T]: the logits themselves (rows without a mask are then touched only where a
- * rule changes them), or memory that shares nothing with them; padding rows of out stay as they are. Tokens outside the vocabulary are passed
- * over. A row whose mask leaves nothing is all -inf (srhpm_verify_sample then emits token 0). T and n_seqs <= 2^24, n_vocab <= 2^29, max(T,
- * n_seqs) * ceil(n_vocab / 4096) < 2^31 (else SRHPM_UNSUPPORTED). */
+ * rule changes them), or memory that shares nothing with them; padding rows of out stay as they are. Tokens outside the
+ * vocabulary are passed over. A row whose mask leaves nothing is all -inf (srhpm_verify_sample then emits token 0). T and
+ * n_seqs <= 2^24, n_vocab <= 2^29, max(T, n_seqs) * ceil(n_vocab / 4096) < 2^31 (else SRHPM_UNSUPPORTED). */
 int srhpm_adjust_logits(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start, int n_seqs,
                         const srhpm_tensor * history, const int32_t * n_history, const int32_t * last_n, const float * repeat,
                         const float * frequency, const float * presence, const int32_t * bias_start, const int32_t * bias_ids,

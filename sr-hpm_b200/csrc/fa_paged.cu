@@ -787,8 +787,7 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
             if (tid == 0 && !whole && w.off == 0) {
                 // this CTA opens an item that others go on with: parts of it, for the merge
                 const int64_t end = range[0] + (range[1] - range[0] - w.rem) + w.sp.units;
-                int           e   = blockIdx.x;
-                while (range[2] * (e + 1) / range[3] < end) e++;
+                const int     e   = part_of_end(range[2], range[3], end, blockIdx.x);
                 a.desc[2 * blockIdx.x + 1] = make_int4(w.rt * BMN, min(BMN, R - w.rt * BMN), 0, 0);
                 a.desc[2 * blockIdx.x]     = make_int4(e - (int) blockIdx.x + 1, w.h, w.r0, 0);
             }
@@ -1119,129 +1118,128 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
 // rows have 16 CTAs per item: 126 rows in 148 parts 58 / 66. Four records of a lane in flight: 16 took so many registers that the cut items of 18 prompts of 64
 // tokens were joined in 41 us instead of 17.
 // A CTA looks after the items that `per` parts of the line open (8 where every warp has a part of its own: few of those open one).
-template <int D, bool F32> __global__ void __launch_bounds__(256, 4) fa_paged_merge_kernel(const __grid_constant__ PArgs a, int per) {
+template <int D, bool F32, int MO> __global__ void __launch_bounds__(256, MO == 4 ? 4 : 2) fa_paged_merge_kernel(const __grid_constant__ PArgs a, int per) {
     constexpr int V  = D / 32;  // values per lane, in pairs or fours side by side
     constexpr int VW = V >= 4 ? 4 : 2;
-    constexpr int MO = 4;
     __shared__ float part_s[8][D];
     __shared__ float l_s[8], m_s[8];
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (uint32_t open = __ballot_sync(0xffffffffu, lane < per && a.desc[2 * (blockIdx.x * per + lane)].x != 0); open; open &= open - 1) {
-    const int  c  = blockIdx.x * per + __ffs(open) - 1;
-    const int4 d0 = a.desc[2 * c], d1 = a.desc[2 * c + 1];
-    const int  parts = d0.x;
-    const bool many = 2 * d1.y <= 3 * parts && d1.y <= 64;
-    for (int row = many ? blockIdx.y : blockIdx.y * 8 + warp; row < d1.y; row += many ? gridDim.y : gridDim.y * 8) {
-        const int tok = a.byG.div(d1.x + row), h = d0.y * a.G + (d1.x + row - tok * a.G);
-        auto      rec = [&](int p) { return (int64_t) (2 * (c + p) + (p == 0 ? 1 : 0)) * a.prow + row; };
-        float     M = -INFINITY, L = 0.0f, acc[V];  // of this warp's parts
+        const int  c  = blockIdx.x * per + __ffs(open) - 1;
+        const int4 d0 = a.desc[2 * c], d1 = a.desc[2 * c + 1];
+        const int  parts = d0.x;
+        const bool many = 2 * d1.y <= 3 * parts && d1.y <= 64;
+        for (int row = many ? blockIdx.y : blockIdx.y * 8 + warp; row < d1.y; row += many ? gridDim.y : gridDim.y * 8) {
+            const int tok = a.byG.div(d1.x + row), h = d0.y * a.G + (d1.x + row - tok * a.G);
+            auto      rec = [&](int p) { return (int64_t) (2 * (c + p) + (p == 0 ? 1 : 0)) * a.prow + row; };
+            float     M = -INFINITY, L = 0.0f, acc[V];  // of this warp's parts
 #pragma unroll
-        for (int e = 0; e < V; e++) acc[e] = 0.0f;
-        const int first = many ? warp : 0, step = many ? 8 : 1;
-        for (int p0 = first; p0 < parts; p0 += MO * step) {
-            float  x[MO][V];
-            float2 ms[MO];
+            for (int e = 0; e < V; e++) acc[e] = 0.0f;
+            const int first = many ? warp : 0, step = many ? 8 : 1;
+            for (int p0 = first; p0 < parts; p0 += MO * step) {
+                float  x[MO][V];
+                float2 ms[MO];
 #pragma unroll
-            for (int k = 0; k < MO; k++) {
-                const int p = p0 + k * step;
-                ms[k]       = make_float2(0.0f, 0.0f);
-                if (p < parts) {
-                    ms[k]             = __ldcg(a.part_ms + rec(p));
-                    const float * src = a.part_acc + rec(p) * D + lane * VW;
+                for (int k = 0; k < MO; k++) {
+                    const int p = p0 + k * step;
+                    ms[k]       = make_float2(0.0f, 0.0f);
+                    if (p < parts) {
+                        ms[k]             = __ldcg(a.part_ms + rec(p));
+                        const float * src = a.part_acc + rec(p) * D + lane * VW;
 #pragma unroll
-                    for (int e = 0; e < V; e += VW) {
-                        if constexpr (VW == 4) {
-                            const float4 f = __ldcg(reinterpret_cast<const float4 *>(src + 32 * e));
-                            x[k][e] = f.x; x[k][e + 1] = f.y; x[k][e + 2] = f.z; x[k][e + 3] = f.w;
-                        } else {
-                            const float2 f = __ldcg(reinterpret_cast<const float2 *>(src + 32 * e));
-                            x[k][e] = f.x; x[k][e + 1] = f.y;
+                        for (int e = 0; e < V; e += VW) {
+                            if constexpr (VW == 4) {
+                                const float4 f = __ldcg(reinterpret_cast<const float4 *>(src + 32 * e));
+                                x[k][e] = f.x; x[k][e + 1] = f.y; x[k][e + 2] = f.z; x[k][e + 3] = f.w;
+                            } else {
+                                const float2 f = __ldcg(reinterpret_cast<const float2 *>(src + 32 * e));
+                                x[k][e] = f.x; x[k][e + 1] = f.y;
+                            }
                         }
                     }
                 }
-            }
-            float mn = M;
+                float mn = M;
 #pragma unroll
-            for (int k = 0; k < MO; k++) mn = ms[k].y == 0.0f ? mn : fmaxf(mn, ms[k].x);
-            if (mn > M) {
-                const float f = ex2(M - mn);  // 0 the first time
-                L *= f;
+                for (int k = 0; k < MO; k++) mn = ms[k].y == 0.0f ? mn : fmaxf(mn, ms[k].x);
+                if (mn > M) {
+                    const float f = ex2(M - mn);  // 0 the first time
+                    L *= f;
 #pragma unroll
-                for (int e = 0; e < V; e++) acc[e] *= f;
-                M = mn;
-            }
-#pragma unroll
-            for (int k = 0; k < MO; k++) {
-                if (!(ms[k].y == 0.0f)) {  // a record without weight may hold anything; a NaN stays one
-                    const float w = ex2(ms[k].x - M);
-                    L             = fmaf(w, ms[k].y, L);
-#pragma unroll
-                    for (int e = 0; e < V; e++) acc[e] = fmaf(w, x[k][e], acc[e]);
+                    for (int e = 0; e < V; e++) acc[e] *= f;
+                    M = mn;
                 }
-            }
-        }
-        const float sk = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-        // weights relative to the larger of the maximum and the sink: of the sums so far, of the sink
-        auto with_sink = [&](float m, float & ws) {
-            const float top = fmaxf(m, sk);
-            ws              = sk > -INFINITY ? ex2(sk - top + kShift) : 0.0f;
-            return m > -INFINITY ? ex2(m - top) : 0.0f;
-        };
-        uint8_t *   dst  = a.dst + (int64_t) h * a.dnb1 + (int64_t) (d0.z + tok) * a.dnb2;
-        if (!many) {
-            float       ws;
-            const float wm = with_sink(M, ws);
-            L              = L * wm + ws;
-            const float f  = L == 0.0f ? 0.0f : wm / L;
 #pragma unroll
-            for (int e = 0; e < V; e += VW) {
+                for (int k = 0; k < MO; k++) {
+                    if (!(ms[k].y == 0.0f)) {  // a record without weight may hold anything; a NaN stays one
+                        const float w = ex2(ms[k].x - M);
+                        L             = fmaf(w, ms[k].y, L);
 #pragma unroll
-                for (int k = 0; k < VW; k += 2) {
-                    const int at = 32 * e + lane * VW + k;
-                    if constexpr (F32) {
-                        *reinterpret_cast<float2 *>(dst + 4 * at) = make_float2(acc[e + k] * f, acc[e + k + 1] * f);
-                    } else {
-                        *reinterpret_cast<__half2 *>(dst + 2 * at) = __floats2half2_rn(acc[e + k] * f, acc[e + k + 1] * f);
+                        for (int e = 0; e < V; e++) acc[e] = fmaf(w, x[k][e], acc[e]);
                     }
                 }
             }
-        } else {
+            const float sk = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
+            // weights relative to the larger of the maximum and the sink: of the sums so far, of the sink
+            auto with_sink = [&](float m, float & ws) {
+                const float top = fmaxf(m, sk);
+                ws              = sk > -INFINITY ? ex2(sk - top + kShift) : 0.0f;
+                return m > -INFINITY ? ex2(m - top) : 0.0f;
+            };
+            uint8_t *   dst  = a.dst + (int64_t) h * a.dnb1 + (int64_t) (d0.z + tok) * a.dnb2;
+            if (!many) {
+                float       ws;
+                const float wm = with_sink(M, ws);
+                L              = L * wm + ws;
+                const float f  = L == 0.0f ? 0.0f : wm / L;
 #pragma unroll
-            for (int e = 0; e < V; e += VW) {
+                for (int e = 0; e < V; e += VW) {
 #pragma unroll
-                for (int k = 0; k < VW; k++) part_s[warp][32 * e + lane * VW + k] = acc[e + k];
-            }
-            if (lane == 0) {
-                l_s[warp] = L;
-                m_s[warp] = M;
-            }
-            __syncthreads();
-            float m = -INFINITY, wt[8], ws;
-#pragma unroll
-            for (int w = 0; w < 8; w++) m = fmaxf(m, m_s[w]);
-            const float wm = with_sink(m, ws);
-            L              = ws;
-#pragma unroll
-            for (int w = 0; w < 8; w++) {
-                wt[w] = m_s[w] > -INFINITY ? ex2(m_s[w] - m) * wm : 0.0f;
-                L     = fmaf(wt[w], l_s[w], L);
-            }
-            const float f = L == 0.0f ? 0.0f : 1.0f / L;
-            for (int at = threadIdx.x; at < D; at += 256) {
-                float o = 0.0f;
-#pragma unroll
-                for (int w = 0; w < 8; w++) o = fmaf(wt[w], part_s[w][at], o);
-                if constexpr (F32) {
-                    reinterpret_cast<float *>(dst)[at] = o * f;
-                } else {
-                    reinterpret_cast<__half *>(dst)[at] = __float2half_rn(o * f);
+                    for (int k = 0; k < VW; k += 2) {
+                        const int at = 32 * e + lane * VW + k;
+                        if constexpr (F32) {
+                            *reinterpret_cast<float2 *>(dst + 4 * at) = make_float2(acc[e + k] * f, acc[e + k + 1] * f);
+                        } else {
+                            *reinterpret_cast<__half2 *>(dst + 2 * at) = __floats2half2_rn(acc[e + k] * f, acc[e + k + 1] * f);
+                        }
+                    }
                 }
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e += VW) {
+#pragma unroll
+                    for (int k = 0; k < VW; k++) part_s[warp][32 * e + lane * VW + k] = acc[e + k];
+                }
+                if (lane == 0) {
+                    l_s[warp] = L;
+                    m_s[warp] = M;
+                }
+                __syncthreads();
+                float m = -INFINITY, wt[8], ws;
+#pragma unroll
+                for (int w = 0; w < 8; w++) m = fmaxf(m, m_s[w]);
+                const float wm = with_sink(m, ws);
+                L              = ws;
+#pragma unroll
+                for (int w = 0; w < 8; w++) {
+                    wt[w] = m_s[w] > -INFINITY ? ex2(m_s[w] - m) * wm : 0.0f;
+                    L     = fmaf(wt[w], l_s[w], L);
+                }
+                const float f = L == 0.0f ? 0.0f : 1.0f / L;
+                for (int at = threadIdx.x; at < D; at += 256) {
+                    float o = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < 8; w++) o = fmaf(wt[w], part_s[w][at], o);
+                    if constexpr (F32) {
+                        reinterpret_cast<float *>(dst)[at] = o * f;
+                    } else {
+                        reinterpret_cast<__half *>(dst)[at] = __float2half_rn(o * f);
+                    }
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
-    }
     }
 }
 
@@ -1339,9 +1337,12 @@ bool fap::encode_rows(void * map, const void * p, uint64_t width, int tokens, in
 }
 
 int fap::merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int rows_y, cudaStream_t stream, int parts) {
-    auto kern = D == 64 ? (f32 ? fa_paged_merge_kernel<64, true> : fa_paged_merge_kernel<64, false>)
-                : D == 128 ? (f32 ? fa_paged_merge_kernel<128, true> : fa_paged_merge_kernel<128, false>)
-                           : (f32 ? fa_paged_merge_kernel<256, true> : fa_paged_merge_kernel<256, false>);
+    // eight records of a row at a time where an item has hundreds (one row over 30000 q4_0 tokens, 24 / 4 heads of 256: 30 us, four
+    // at a time 38; 32 / 8 heads of 128 the same, 16 sequences of 4000 tokens 41 and 38)
+    auto kern = D == 64    ? (f32 ? fa_paged_merge_kernel<64, true, 4> : fa_paged_merge_kernel<64, false, 4>)
+                : D == 128 ? (f32 ? fa_paged_merge_kernel<128, true, 4> : fa_paged_merge_kernel<128, false, 4>)
+                : parts == 1 ? (f32 ? fa_paged_merge_kernel<256, true, 4> : fa_paged_merge_kernel<256, false, 4>)
+                             : (f32 ? fa_paged_merge_kernel<256, true, 8> : fa_paged_merge_kernel<256, false, 8>);
     const int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms * parts / (parts > 1 ? 8 : 1), rows_y), dim3(256), 0, stream, a, parts > 1 ? 8 : 1));
     ctx->launches.fetch_add(1);
     return st;

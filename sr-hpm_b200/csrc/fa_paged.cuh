@@ -147,6 +147,11 @@ template <int BMN, int BN> __device__ __forceinline__ void plan_sums(const PArgs
     __syncthreads();
 }
 
+// the part, from `part` on, in which unit `end` - 1 of all stands (a search part by part took 30 us of one sequence's 80, cut into 1184)
+__device__ __forceinline__ int part_of_end(int64_t all, int64_t parts, int64_t end, int part) {
+    return max(part, (int) ((end * parts + all - 1) / all) - 1);
+}
+
 // Part `part` of `parts` of the line of units, found by one warp: its first unit (s = -1: the part is empty), its place in the
 // line, the units and the parts in all
 struct Part {
@@ -243,7 +248,7 @@ int q4_parts(int rows, int D);
 int q4_few_run(srhpm_ctx * ctx, const PArgs & a, const void * maps, const PagedCache & c, bool f32, cudaStream_t stream);  // fa_paged_q4_few.cu
 int q4_run(srhpm_ctx * ctx, PArgs & a, const PagedCache & c, int rows, bool f32, cudaStream_t stream);
 
-// every page that a row sees, as f16 [pages][page][Hkv][D] under its own number (unpack_q4.cu); cols * page < 2^31 + 16
+// every page that a row sees, as f16 [pages][page][Hkv][D] under its own number (unpack_q4.cu)
 int unpack_q4_run(srhpm_ctx * ctx, const FaPagedView & v, void * ko, void * vo, cudaStream_t stream);
 
 // tensor map of bytes [pages][tokens][width], boxes of `tokens_box` rows of `box` bytes (fa_paged.cu); false: not encoded

@@ -9,6 +9,11 @@
 // a tile. Unpacking goes where it costs least: K's into tensor memory, whose writes take no shared memory bandwidth, V's into
 // the 128-byte swizzled rows that the product reads.
 //
+// Measured: 9 f32 rows over 131072 tokens, 24 / 4 heads of 256: 127 us, 54 of 64 rows used; a tile of 128 tokens takes 7300 cycles on
+// its SM: two products of two parts each (3300, V's tiles waited for meanwhile: shared memory holds one of them), the softmax beside
+// them, and a seventh of it O's way out. Tiles of 96 rows, 2048 rows over 32768 tokens: 6500 cycles, unpacking 2700 of them, its raw
+// rows late by 1500 (2.69 ms; with 8 softmax warps 2.96; with 128 rows a tile 2.75).
+//
 // Work: as in fa_paged.cu, all items' units of 128 tokens stand in one line that is cut into equal parts, one per CTA.
 // Roles: 16 softmax warps (four groups, a quarter of the rows each: with half of them a thread's scores and sums did not fit its
 // registers, and the chain from scores to P took 6000 cycles of a tile), 1 MMA warp, 2 producer warps (K's and V's raw rows by TMA, 64
@@ -572,8 +577,7 @@ __global__ void __launch_bounds__(kThr, 1)
             if (tid == 0 && !whole && w.off == 0) {
                 // this CTA opens an item that others go on with: parts of it, for the join
                 const int64_t end = range[0] + (range[1] - range[0] - w.rem) + w.sp.units;
-                int           e   = blockIdx.x;
-                while (range[2] * (e + 1) / range[3] < end) e++;
+                const int     e   = part_of_end(range[2], range[3], end, blockIdx.x);
                 a.desc[2 * blockIdx.x + 1] = make_int4(rb, rows, 0, 0);
                 a.desc[2 * blockIdx.x]     = make_int4(e - (int) blockIdx.x + 1, w.h, w.r0, 0);
             }
@@ -880,12 +884,22 @@ int launch_d(srhpm_ctx * ctx, int rows, bool f32, const PArgs & a, const CUtenso
 
 }  // namespace
 
+// Rows of a tile, from the average of rows per sequence and KV head, padding included. 16 sequences of 4000 tokens, us by tile:
+//   rows per sequence          8     16     64     96
+//   24 / 4 heads of 256   6    44     54     70     85    (32 / 8 heads of 128, 8 rows: 38, 77, 87, 106)
+//                        12    72     54     71     85    (16 rows: 66, 76, 88, 108; one sequence of 30000 tokens 57, 43, 50, 60)
+//                        24   100     88     72     86
+//                        60   212    156     77     92
+//                        96          224    121     95
+//                       126                 122    145
+//                       192                 176    150
+// A tile of 96 takes 1.2 times one of 64, so the fewer tiles win above that. f32 rows have two parts of each operand, for which shared
+// memory holds 64 rows.
 int fap::q4_rows(int T, int S, int G, bool f32) {
-    const int64_t R = (int64_t) T * G;
-    if (R <= (int64_t) S * 8) return 8;
-    if (R <= (int64_t) S * 16) return 16;
-    if (f32 || R <= (int64_t) S * 64) return 64;
-    return 96;
+    const int64_t R = ((int64_t) T * G + S - 1) / S;
+    if (R <= 8) return 8;
+    if (R <= 16) return 16;
+    return f32 || (R + 63) / 64 * 5 <= (R + 95) / 96 * 6 ? 64 : 96;
 }
 
 int fap::q4_parts(int rows, int D) { return rows == 8 ? (D == 256 ? 8 : 16) : 1; }

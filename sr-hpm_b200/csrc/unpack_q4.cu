@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kThreads) unpack_q4_kernel(const __grid_consta
 }  // namespace
 
 int fap::unpack_q4_run(srhpm_ctx * ctx, const FaPagedView & v, void * ko, void * vo, cudaStream_t stream) {
-    const int64_t turns = ((int64_t) v.cols * v.c.page + kTokens - 1) / kTokens;
+    const int64_t turns = (std::min<int64_t>((int64_t) v.cols * v.c.page, INT32_MAX) + kTokens - 1) / kTokens;  // as far as kv_len counts
     Args a{ v.c.k, v.c.knb1, v.c.knb2, v.c.knb3, v.c.v, v.c.vnb1, v.c.vnb2, v.c.vnb3, v.table, v.tstride, v.cols, v.c.page, (int) v.c.n_pages,
             v.q_start, v.kv_len, v.S, v.T, v.c.Hkv, v.c.D, v.window, (int) turns, FastDiv::of((uint32_t) (v.c.Hkv * (v.c.D / 8))),
             FastDiv::of((uint32_t) v.c.page), static_cast<__half *>(ko), static_cast<__half *>(vo) };
