@@ -1118,7 +1118,14 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
 // rows have 16 CTAs per item: 126 rows in 148 parts 58 / 66. Four records of a lane in flight: 16 took so many registers that the cut items of 18 prompts of 64
 // tokens were joined in 41 us instead of 17.
 // A CTA looks after the items that `per` parts of the line open (8 where every warp has a part of its own: few of those open one).
-template <int D, bool F32, int MO> __global__ void __launch_bounds__(256, MO == 4 ? 4 : 2) fa_paged_merge_kernel(const __grid_constant__ PArgs a, int per) {
+// records of a row at a time: eight where an item has hundreds (one row over 30000 q4_0 tokens, 24 / 4 heads of 256: 30 us, four at a
+// time 38; 32 / 8 heads of 128 the same, 16 sequences of 4000 tokens 41 and 38)
+template <int D, int PER> constexpr int kMergeStep = PER > 1 && D == 256 ? 8 : 4;
+
+// PER: parts that a CTA looks after
+template <int D, bool F32, int PER>
+__global__ void __launch_bounds__(256, kMergeStep<D, PER> == 4 ? 4 : 2) fa_paged_merge_kernel(const __grid_constant__ PArgs a) {
+    constexpr int MO = kMergeStep<D, PER>;
     constexpr int V  = D / 32;  // values per lane, in pairs or fours side by side
     constexpr int VW = V >= 4 ? 4 : 2;
     __shared__ float part_s[8][D];
@@ -1126,10 +1133,13 @@ template <int D, bool F32, int MO> __global__ void __launch_bounds__(256, MO == 
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (uint32_t open = __ballot_sync(0xffffffffu, lane < per && a.desc[2 * (blockIdx.x * per + lane)].x != 0); open; open &= open - 1) {
-        const int  c  = blockIdx.x * per + __ffs(open) - 1;
+    uint32_t  open = 1;
+    if constexpr (PER > 1) open = __ballot_sync(0xffffffffu, lane < PER && a.desc[2 * (blockIdx.x * PER + lane)].x != 0);
+    for (; open; open = PER > 1 ? open & (open - 1) : 0) {
+        const int  c  = blockIdx.x * PER + (PER > 1 ? __ffs(open) - 1 : 0);
         const int4 d0 = a.desc[2 * c], d1 = a.desc[2 * c + 1];
         const int  parts = d0.x;
+        if (parts == 0) return;
         const bool many = 2 * d1.y <= 3 * parts && d1.y <= 64;
         for (int row = many ? blockIdx.y : blockIdx.y * 8 + warp; row < d1.y; row += many ? gridDim.y : gridDim.y * 8) {
             const int tok = a.byG.div(d1.x + row), h = d0.y * a.G + (d1.x + row - tok * a.G);
@@ -1337,13 +1347,14 @@ bool fap::encode_rows(void * map, const void * p, uint64_t width, int tokens, in
 }
 
 int fap::merge_launch(srhpm_ctx * ctx, const PArgs & a, int D, bool f32, int rows_y, cudaStream_t stream, int parts) {
-    // eight records of a row at a time where an item has hundreds (one row over 30000 q4_0 tokens, 24 / 4 heads of 256: 30 us, four
-    // at a time 38; 32 / 8 heads of 128 the same, 16 sequences of 4000 tokens 41 and 38)
-    auto kern = D == 64    ? (f32 ? fa_paged_merge_kernel<64, true, 4> : fa_paged_merge_kernel<64, false, 4>)
-                : D == 128 ? (f32 ? fa_paged_merge_kernel<128, true, 4> : fa_paged_merge_kernel<128, false, 4>)
-                : parts == 1 ? (f32 ? fa_paged_merge_kernel<256, true, 4> : fa_paged_merge_kernel<256, false, 4>)
-                             : (f32 ? fa_paged_merge_kernel<256, true, 8> : fa_paged_merge_kernel<256, false, 8>);
-    const int st = cuda_status(launch_k_pdl(kern, dim3(ctx->num_sms * parts / (parts > 1 ? 8 : 1), rows_y), dim3(256), 0, stream, a, parts > 1 ? 8 : 1));
+    auto one  = D == 64    ? (f32 ? fa_paged_merge_kernel<64, true, 1> : fa_paged_merge_kernel<64, false, 1>)
+                : D == 128 ? (f32 ? fa_paged_merge_kernel<128, true, 1> : fa_paged_merge_kernel<128, false, 1>)
+                           : (f32 ? fa_paged_merge_kernel<256, true, 1> : fa_paged_merge_kernel<256, false, 1>);
+    auto eight = D == 64    ? (f32 ? fa_paged_merge_kernel<64, true, 8> : fa_paged_merge_kernel<64, false, 8>)
+                 : D == 128 ? (f32 ? fa_paged_merge_kernel<128, true, 8> : fa_paged_merge_kernel<128, false, 8>)
+                            : (f32 ? fa_paged_merge_kernel<256, true, 8> : fa_paged_merge_kernel<256, false, 8>);
+    const int per = parts > 1 ? 8 : 1;
+    const int st  = cuda_status(launch_k_pdl(per > 1 ? eight : one, dim3(ctx->num_sms * parts / per, rows_y), dim3(256), 0, stream, a));
     ctx->launches.fetch_add(1);
     return st;
 }
