@@ -77,7 +77,7 @@ template <int D, int N, bool PREC> struct LayT {
     static constexpr int CB    = D / 16;
     static constexpr int RS    = row_stride(D);
     static constexpr int stage = kRawTok * RS;
-    static constexpr int tail  = 3072 + 24 * N;                // barriers, rows' numbers
+    static constexpr int tail  = 3 * 1024 + 24 * N;            // barriers, rows' numbers
     // P buffers: two where shared memory has room for them beside the raw rows of two tiles
     static constexpr int PB    = 232448 - tail - p - 2 * parts * ptile >= 8 * stage ? 2 : 1;
     static constexpr int raw   = p + PB * parts * ptile;
