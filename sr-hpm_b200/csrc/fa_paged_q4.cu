@@ -10,9 +10,9 @@
 // the 128-byte swizzled rows that the product reads.
 //
 // Measured: 9 f32 rows over 131072 tokens, 24 / 4 heads of 256: 127 us, 54 of 64 rows used; a tile of 128 tokens takes 7300 cycles on
-// its SM: two products of two parts each (3300, V's tiles waited for meanwhile: shared memory holds one of them), the softmax beside
-// them, and a seventh of it O's way out. Tiles of 96 rows, 2048 rows over 32768 tokens: 6500 cycles, unpacking 2700 of them, its raw
-// rows late by 1500 (2.69 ms; with 8 softmax warps 2.96; with 128 rows a tile 2.75).
+// its SM: the MMA warp waits for V 1400 (shared memory holds one tile of it) and issues P V for 2300, the softmax warps wait for
+// that 1900 and spend 1800 on O's way out and the rest. Tiles of 96 rows, 2048 rows over 32768 tokens: 6500 cycles, unpacking 2700 of
+// them, raw rows late by 1300 to 1900 (2.69 ms; with 128 rows a tile 2.75, with 8 softmax warps besides 2.96).
 //
 // Work: as in fa_paged.cu, all items' units of 128 tokens stand in one line that is cut into equal parts, one per CTA.
 // Roles: 16 softmax warps (four groups, a quarter of the rows each: with half of them a thread's scores and sums did not fit its
