@@ -9,6 +9,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "fastdiv.cuh"
 #include "internal.h"
@@ -381,7 +382,17 @@ __global__ void __launch_bounds__(kSetThreads) page_compact_kernel(const SetArgs
     cl.sync();
 }
 
-int set_launch(srhpm_ctx * ctx, void (*kern)(SetArgs), SetArgs & a, int bytes_per_word, cudaStream_t stream) {
+// WORD: bytes of shared memory per 32 pages of a CTA
+template <void (*KERN)(SetArgs), int WORD> int set_launch(srhpm_ctx * ctx, SetArgs & a, cudaStream_t stream) {
+    // The limit belongs to the kernel, not to the call: always that of the largest pool, as another thread's call over a smaller
+    // one may come between this one's limit and its launch.
+    static std::atomic<unsigned> done{ 0 };
+    const unsigned               bit = 1u << (ctx->device & 31);
+    if (!(done.load() & bit)) {
+        const int st = cuda_status(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxPages / kSetCtas / 32 * WORD));
+        if (st != SRHPM_OK) return st;
+        done.fetch_or(bit);
+    }
     // pages of a CTA: all 8 share them out, 1024 at least
     a.shift = 10;
     while (((int64_t) kSetCtas << a.shift) < a.n_pages) a.shift++;
@@ -389,13 +400,10 @@ int set_launch(srhpm_ctx * ctx, void (*kern)(SetArgs), SetArgs & a, int bytes_pe
     const int64_t jobs = (int64_t) a.n * a.chunks;
     int           ctas = 1;
     while (ctas < kSetCtas && (((int64_t) ctas << a.shift) < a.n_pages || ctas * 32 < jobs)) ctas *= 2;
-    const size_t smem = (size_t) bytes_per_word << (a.shift - 5);
-    int          st   = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) std::max<size_t>(smem, 1024)));
-    if (st != SRHPM_OK) return st;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim            = dim3(ctas);
     cfg.blockDim           = dim3(kSetThreads);
-    cfg.dynamicSmemBytes   = smem;
+    cfg.dynamicSmemBytes   = (size_t) WORD << (a.shift - 5);
     cfg.stream             = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -406,7 +414,7 @@ int set_launch(srhpm_ctx * ctx, void (*kern)(SetArgs), SetArgs & a, int bytes_pe
     attr[1].val.clusterDim.z                           = 1;
     cfg.attrs    = attr;
     cfg.numAttrs = 2;
-    st           = cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
+    const int st = cuda_status(cudaLaunchKernelEx(&cfg, KERN, a));
     ctx->launches.fetch_add(1);
     return st;
 }
@@ -438,14 +446,14 @@ int page_free_run(srhpm_ctx * ctx, const PageTable & t, const int32_t * rows, co
                   cudaStream_t stream) {
     SetArgs a{ rows, begin, end, n, (t.cols + kForkChunk - 1) / kForkChunk, t.data, t.stride, t.cols, t.rows, refs, n_pages, 0,
                free_pages, n_free, free_head, nullptr, nullptr, n_freed, nullptr, ctx->d_status };
-    return set_launch(ctx, page_free_kernel, a, 4, stream);
+    return set_launch<page_free_kernel, 4>(ctx, a, stream);
 }
 
 int page_compact_run(srhpm_ctx * ctx, const PageTable & t, const int32_t * held, int32_t * refs, int n_pages, int32_t * free_pages,
                      int32_t * src, int32_t * dst, int32_t * n_moves, int32_t * n_used, cudaStream_t stream) {
     SetArgs a{ nullptr, nullptr, held, t.rows, (t.cols + kForkChunk - 1) / kForkChunk, t.data, t.stride, t.cols, t.rows, refs, n_pages, 0,
                free_pages, n_pages, nullptr, src, dst, n_moves, n_used, ctx->d_status };
-    return set_launch(ctx, page_compact_kernel, a, 8, stream);
+    return set_launch<page_compact_kernel, 8>(ctx, a, stream);
 }
 
 int page_copy_run(srhpm_ctx * ctx, const srhpm_tensor * caches, int n_caches, const int32_t * src, const int32_t * dst, int n,
