@@ -36,6 +36,7 @@
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "q4.cuh"
+#include "ring.h"
 
 namespace srhpm {
 using namespace fap;
@@ -133,7 +134,6 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3, part = blockIdx.x * W + warp;
     uint64_t * full = reinterpret_cast<uint64_t *>(sm + Ly::bar) + warp * 4;
-    bool       bad  = false;
     if (lane == 0) {
         for (int i = 0; i < ST; i++) mbar_init(&full[i], a.box ? 1 : 32);
         fence_mbar_init();
@@ -163,8 +163,8 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
     // ---- this warp's copies, up to ST steps ahead of its products, across items ----
     Walk pw   = w;
     Run  prun = run_of<TS>(pw, period);
-    int  pst  = 0;  // step of the item
-    bool pact = true;
+    int  pst  = 0;   // step of the item
+    int  idle = -1;  // how often a load was asked for since there were no more (negative: there are more)
     // lane j: page of the 16-token group j % GP of the (j / GP)-th step from i0 on: asked for step by step, an entry's 700 cycles held
     // the warp up each time
     auto step_at = [](const Run & r, int i) { return r.t0 + (i + r.rot < r.n ? i + r.rot : i + r.rot - r.n) * TS; };
@@ -172,15 +172,16 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
     const uint32_t ring0 = smem_u32(sm + Ly::ring + warp * (ST * Ly::stage));
     auto           look  = [&](bool fresh) {
         fresh |= pst - i0 >= 32 / GP;
-        while (pact && pst >= prun.n) {
-            pact = walk_next<BM, TS>(a, pw);
-            if (pact) {
+        while (idle < 0 && pst >= prun.n) {
+            if (walk_next<BM, TS>(a, pw)) {
                 prun  = run_of<TS>(pw, period);
                 pst   = 0;
                 fresh = true;
+            } else {
+                idle = 0;
             }
         }
-        if (pact && fresh) {
+        if (idle < 0 && fresh) {
             i0            = pst;
             ent           = -1;
             const int tok = step_at(prun, pst + lane / GP) + 16 * (lane % GP);
@@ -194,7 +195,10 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
         }
     };
     auto issue = [&](int stage) {
-        if (!pact) return;
+        if (idle >= 0) {
+            idle++;
+            return;
+        }
         const uint32_t to = ring0 + stage * Ly::stage;
         const int      t0 = step_at(prun, pst), at = (pst - i0) * GP;
         int            p[GP], y[GP];  // page (-1: no row sees the group) and place
@@ -307,15 +311,16 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
         const uint4 * ql   = qb + lane;
         const int     lead = a.box ? (w.h * rowb) & 15 : 0;
         for (int st = 0; st < run.n; st++) {
-            if (!bad) {
-                uint32_t i = 0;
-                while (i < kProbes && !mbar_try_wait(&full[stage], use & 1)) i++;
-                if (i == kProbes) {  // this thread waits for nothing more: its results are void, its accesses stay in bounds
-                    bad = true;
-                    atomicExch(a.status, kErrWaitFull);
-                }
+            uint32_t i = 0;
+            while (i < kProbes && !mbar_try_wait(&full[stage], use & 1)) i++;
+            if (__any_sync(0xffffffffu, i == kProbes)) {
+                // The warp gives up as one and asks for nothing more; its results are void. Its loads in flight land before the
+                // CTA's shared memory goes.
+                if (lane == 0) atomicExch(a.status, kErrWaitFull);
+                const uint32_t done = use * ST + stage, issued = ring_issued(done, ST, idle);
+                for (uint32_t c = done; c < issued; c++) mbar_wait(&full[ring_slot(c, ST)], ring_parity(c, ST));
+                return;
             }
-            __syncwarp();
             const uint8_t * kr = sm + Ly::ring + warp * (ST * Ly::stage) + stage * Ly::stage + lead;
             const uint8_t * vr = kr + TS * RS;
             const int       tb   = step_at(run, st);
@@ -527,11 +532,6 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
         }
         __syncwarp();  // Q is read
         active = walk_next<BM, TS>(a, w);
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    // a wait that gave up: the loads in flight land before this CTA's shared memory goes
-    if (bad && a.box) {
-        for (int i = 0; i < ST; i++) mbar_wait(&full[i], (use + (i < stage)) & 1);
     }
 }
 
