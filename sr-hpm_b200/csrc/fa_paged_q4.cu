@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(kThr, 1)
     pdl_launch_dependents();
     pdl_wait();
     plan_part<N, kTile>(a, reinterpret_cast<int *>(sm), reinterpret_cast<int *>(sm + Ly::red), first, range);
+    fence_proxy_async_smem();  // the plan's sums stood where TMA writes next
     tc::fence_before();
     __syncthreads();
     tc::fence_after();

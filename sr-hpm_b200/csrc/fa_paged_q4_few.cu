@@ -147,6 +147,7 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
     int * tot = reinterpret_cast<int *>(sm + Ly::ring);
     plan_sums<BM, TS>(a, tot, reinterpret_cast<int *>(sm + Ly::misc));
     const Part pt = plan_find<BM, TS>(a, tot, part, gridDim.x * W);
+    fence_proxy_async_smem();  // the plan's sums stood where TMA writes next
     __syncthreads();  // the ring is free; no warp waits for another from here on
     if (lane == 0) a.desc[2 * part] = make_int4(0, 0, 0, 0);
     if (pt.s < 0) return;
