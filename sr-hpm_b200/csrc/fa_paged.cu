@@ -305,8 +305,8 @@ __global__ void __launch_bounds__(Lay<D, NT, BR, PREC, Q8>::threads, 1)
     pdl_wait();
 
     // ---------------- plan: this CTA's part of the line of units ----------------
-    plan_part<BMN, BN>(a, reinterpret_cast<int *>(sm + Ly::ring), reinterpret_cast<int *>(sm + Ly::red), first, range);
-    fence_proxy_async_smem();  // the plan's sums stood where TMA writes next
+    // (q8_0: its sums end within the ring, and TMA writes behind it)
+    plan_part<BMN, BN, !Q8>(a, reinterpret_cast<int *>(sm + Ly::ring), reinterpret_cast<int *>(sm + Ly::red), first, range);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();

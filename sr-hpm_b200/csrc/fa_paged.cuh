@@ -7,6 +7,7 @@
 
 #include "fastdiv.cuh"
 #include "internal.h"
+#include "ptx.cuh"
 
 namespace srhpm {
 namespace fap {
@@ -119,8 +120,8 @@ template <int BMN, int BN> __device__ __forceinline__ bool walk_next(const PArgs
 }
 
 // Units per KV head of each sequence into tot, by all of the CTA's threads. tot: 2 a.S words of scratch, nbg one, both in shared
-// memory. Ends with a barrier.
-template <int BMN, int BN> __device__ __forceinline__ void plan_sums(const PArgs & a, int * tot, int * nbg) {
+// memory. Ends with a barrier. TMA: loads of it come to the place of the sums next.
+template <int BMN, int BN, bool TMA> __device__ __forceinline__ void plan_sums(const PArgs & a, int * tot, int * nbg) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int * big = tot + a.S;  // sequences whose tiles a warp sums up
     if (tid == 0) *nbg = 0;
@@ -144,6 +145,7 @@ template <int BMN, int BN> __device__ __forceinline__ void plan_sums(const PArgs
         u = __reduce_add_sync(0xffffffffu, u);
         if (lane == 0) tot[s] = u;
     }
+    if constexpr (TMA) fence_proxy_async_smem();
     __syncthreads();
 }
 
@@ -222,9 +224,9 @@ template <int BMN, int BN> __device__ __forceinline__ Part plan_find(const PArgs
 
 // This CTA's part of the line, as one of gridDim.x: first = {s, h, rt, off} (s stays as it was, -1, for an empty part), range =
 // {start, end, units in all, parts}, both in shared memory. Ends without a barrier.
-template <int BMN, int BN>
+template <int BMN, int BN, bool TMA>
 __device__ __forceinline__ void plan_part(const PArgs & a, int * tot, int * nbg, int * first, int64_t * range) {
-    plan_sums<BMN, BN>(a, tot, nbg);
+    plan_sums<BMN, BN, TMA>(a, tot, nbg);
     if (threadIdx.x < 32) {
         const Part p = plan_find<BMN, BN>(a, tot, blockIdx.x, gridDim.x);
         if (threadIdx.x == 0) {

@@ -268,8 +268,7 @@ __global__ void __launch_bounds__(kThr, 1)
     if (warp == kSm) tc::tmem_alloc(tptr, 512);
     pdl_launch_dependents();
     pdl_wait();
-    plan_part<N, kTile>(a, reinterpret_cast<int *>(sm), reinterpret_cast<int *>(sm + Ly::red), first, range);
-    fence_proxy_async_smem();  // the plan's sums stood where TMA writes next
+    plan_part<N, kTile, true>(a, reinterpret_cast<int *>(sm), reinterpret_cast<int *>(sm + Ly::red), first, range);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();

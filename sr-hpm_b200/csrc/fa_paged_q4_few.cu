@@ -145,9 +145,8 @@ __global__ void __launch_bounds__(LayF<D, PREC>::W * 32, 1)
     pdl_launch_dependents();
     pdl_wait();
     int * tot = reinterpret_cast<int *>(sm + Ly::ring);
-    plan_sums<BM, TS>(a, tot, reinterpret_cast<int *>(sm + Ly::misc));
+    plan_sums<BM, TS, true>(a, tot, reinterpret_cast<int *>(sm + Ly::misc));
     const Part pt = plan_find<BM, TS>(a, tot, part, gridDim.x * W);
-    fence_proxy_async_smem();  // the plan's sums stood where TMA writes next
     __syncthreads();  // the ring is free; no warp waits for another from here on
     if (lane == 0) a.desc[2 * part] = make_int4(0, 0, 0, 0);
     if (pt.s < 0) return;
