@@ -233,6 +233,7 @@ __global__ void __launch_bounds__(kThr, 1)
     uint32_t * tptr   = reinterpret_cast<uint32_t *>(sm + Ly::misc);
     int *      first  = reinterpret_cast<int *>(sm + Ly::misc + 16);
     int64_t *  range  = reinterpret_cast<int64_t *>(sm + Ly::misc + 32);
+    uint64_t * mdone  = reinterpret_cast<uint64_t *>(sm + Ly::misc + 64);  // all products
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     bool      bad = false;
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(kThr, 1)
         for (int i = 0; i < 2; i++) mbar_init(&pvdone[i], 1);
         mbar_init(qfull, kSm);
         mbar_init(qempty, 1);
+        mbar_init(mdone, 1);
         for (int i = 0; i < NK + NV; i++) {
             mbar_init(&rfull[i], a.box ? 1 : 32);
             mbar_init(&rempty[i], 2);
@@ -660,6 +662,7 @@ __global__ void __launch_bounds__(kThr, 1)
                 }
                 gi += n;
             }
+            if (elect_one()) tc::commit(mdone);
         } else if (warp < kSm + 3) {
             // ---------------- producers: raw rows, 64 tokens at a time ----------------
             const bool isk = warp == kSm + 1;
@@ -689,6 +692,7 @@ __global__ void __launch_bounds__(kThr, 1)
                     for (int st = 0; st < 2 * min(4, n - i0); st++, c++) {
                         const uint32_t sl = c % NR;
                         if (c >= (uint32_t) NR) wait_bar(&re[sl], (c / NR - 1) & 1, a.status, bad);
+                        bad = __any_sync(0xffffffffu, bad);  // the warp gives up as one: the lanes shuffle below
                         if (bad) break;
                         const uint32_t to = raw0 + sl * Ly::stage;
                         int            pg[4], yy[4];
@@ -740,9 +744,9 @@ __global__ void __launch_bounds__(kThr, 1)
                 if (bad) break;
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
-            if (bad && a.box) {  // a wait that gave up: the loads in flight land before this CTA's shared memory goes
-                for (uint32_t k = c > (uint32_t) NR ? c - NR : 0; k < c; k++) mbar_wait(&rf[k % NR], (k / NR) & 1);
-            }
+            // The loads land before this CTA's shared memory goes, those too that a warp whose wait ran out does not take. Nobody else
+            // fills this warp's ring, so each slot's last phase is the one waited for.
+            for (uint32_t k = c > (uint32_t) NR ? c - NR : 0; a.box && k < c; k++) mbar_wait(&rf[k % NR], (k / NR) & 1);
         }
     } else {
         if constexpr (Ly::ru < 72) {
@@ -853,7 +857,11 @@ __global__ void __launch_bounds__(kThr, 1)
     __syncwarp();
     tc::fence_before();
     __syncthreads();
-    if (warp == kSm) tc::tmem_free(tb, 512);
+    if (warp == kSm) {
+        // the softmax warps wait for the last products, unless a wait of theirs ran out
+        mbar_wait(mdone, 0);
+        tc::tmem_free(tb, 512);
+    }
 }
 
 template <int D, int N, bool PREC>
