@@ -454,10 +454,11 @@ int srhpm_page_compact(srhpm_ctx * ctx, const srhpm_tensor * block_table, const 
  *               ids[r], so a drafted token counts in the rows behind it
  *   mask        l = -inf where bit x % 32 of word x / 32 is 0 in the row's mask (mask i32, ne = [>= ceil(n_vocab / 32),
  *               masks], or NULL): mask_row[r] (i32 [T]; outside the masks: none), or r where mask_row is NULL
- * each step rounded to f32. out f32 [n_vocab, T]: the logits themselves (rows without a mask are then touched only where a
- * rule changes them), or memory that shares nothing with them; padding rows of out stay as they are. Tokens outside the
- * vocabulary are passed over. A row whose mask leaves nothing is all -inf (srhpm_verify_sample then emits token 0). T and
- * n_seqs <= 2^24, n_vocab <= 2^29, max(T, n_seqs) * ceil(n_vocab / 4096) < 2^31 (else SRHPM_UNSUPPORTED). */
+ * each operation rounded to f32 by itself (c * frequency, then + presence, then l minus that). out f32 [n_vocab, T]:
+ * the logits themselves (rows without a mask are then touched only where a rule changes them), or memory that shares
+ * nothing with them; padding rows of out stay as they are. Tokens outside the vocabulary are passed over. A row whose
+ * mask leaves nothing is all -inf (srhpm_verify_sample then emits token 0). T and n_seqs <= 2^24, n_vocab <= 2^29,
+ * max(T, n_seqs) * ceil(n_vocab / 4096) < 2^31 (else SRHPM_UNSUPPORTED). */
 int srhpm_adjust_logits(srhpm_ctx * ctx, const srhpm_tensor * logits, const int32_t * ids, const int32_t * q_start, int n_seqs,
                         const srhpm_tensor * history, const int32_t * n_history, const int32_t * last_n, const float * repeat,
                         const float * frequency, const float * presence, const int32_t * bias_start, const int32_t * bias_ids,

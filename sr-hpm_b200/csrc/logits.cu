@@ -170,8 +170,8 @@ __global__ void __launch_bounds__(kThreads, 3) adjust_logits_kernel(const __grid
         if (b1 > b0) l += __uint_as_float(bix[k]);
         const uint32_t times = cnt[k] & ~kListed;
         if (times) {
-            l = l > 0.0f ? __fdiv_rn(l, rep) : l * rep;
-            l -= (float) times * fr + pr;
+            l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);  // each operation rounded by itself: no fused one
+            l = __fsub_rn(l, __fadd_rn(__fmul_rn((float) times, fr), pr));
         }
         return l;
     };
