@@ -28,6 +28,7 @@ constexpr int kSlice   = 4096;
 constexpr int kVec     = kSlice / kThreads / 4;  // groups of four of a thread
 constexpr int kWarpTok = 128 * kVec;             // tokens of a warp
 constexpr uint32_t kListed = 1u << 31;           // beside a token's count
+constexpr uint32_t kNoBias = 1u << 31;           // -0, which no sum shows: x + 0 would make +0 of -0
 constexpr int kSmem = kSlice * 14;
 
 struct Args {
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 3) adjust_logits_kernel(const __grid
         if (b1 > b0) {
             for (int i = lane; i < n_list; i += 32) {
                 const uint32_t k = list[i], bi = bix[k];
-                bix[k] = bi ? __float_as_uint(v.bias[bi - 1]) : 0u;
+                bix[k] = bi ? __float_as_uint(v.bias[bi - 1]) : kNoBias;
             }
         }
     }
@@ -239,7 +240,10 @@ __global__ void __launch_bounds__(kThreads, 3) adjust_logits_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) {
                     cnt[add] = (old | kListed) + 1;
-                    if (!(old & kListed)) list[n_list] = (uint16_t) add;
+                    if (!(old & kListed)) {
+                        list[n_list] = (uint16_t) add;
+                        bix[add]     = kNoBias;
+                    }
                 }
                 if (!(old & kListed)) n_list++;
                 __syncwarp();
