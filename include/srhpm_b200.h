@@ -337,10 +337,10 @@ int srhpm_page_plan(srhpm_ctx * ctx, const int32_t * n_past, const int32_t * n_n
  * srhpm_flash_attn_paged), the turned keys and the values into the cache rows of slots[t] (i64; a slot outside the
  * cache, -1 of a padding row among them, stores nothing; two rows with one slot leave either's values there). f16
  * values round to nearest, q8_0 uses the context's q8_0 mode, q4_0 ggml's reference rounding (d = -m / 8 for the value m of
- * largest size, the first of equals; number = min(15, trunc(x * (1 / d) + 8.5)) in f32; a turned key next to the border of
- * two numbers is turned in 64 bits). q_out shares no memory with qkv or the caches. head_dim
- * 64, 128 or 256; qkv and q_out 16-byte aligned with row strides multiples of 16; cache strides multiples of 16 (f16)
- * or 2 (q8_0, q4_0). */
+ * largest size, the first of equals; number = min(15, trunc(x * (1 / d) + 8.5)) in f32; a key's block is
+ * turned in 64 bits where a value is next to the border of two numbers, or where two values of unlike signs are nearly of
+ * the largest size). q_out shares no memory with qkv or the caches. head_dim 64, 128 or 256; qkv and q_out 16-byte
+ * aligned with row strides multiples of 16; cache strides multiples of 16 (f16) or 2 (q8_0, q4_0). */
 int srhpm_rope_kv_paged(srhpm_ctx * ctx, const srhpm_tensor * qkv, int n_head, int n_head_kv, const int32_t * pos,
                         const int64_t * slots, float theta_base, const srhpm_tensor * q_out,
                         const srhpm_tensor * k_cache, const srhpm_tensor * v_cache, void * stream);

@@ -265,18 +265,21 @@ __device__ __forceinline__ Step4 step_q4(float4 v, uint32_t mask) {
     return { d, d != 0.0f ? __frcp_rn(d) : 0.0f };
 }
 // The numbers of 4 values, a byte each: x / d + 8.5 rounded down, 0 to 15 (NaN: 0). Added to 256 rounding down, the sum's bits hold
-// the number above 15 places of the fraction: the conversion instruction has an eighth of that rate. near: a value stands within
-// 2^-15 of the border of two numbers, where the rounding of its rotation may decide.
+// the number above 15 places of the fraction: the conversion instruction has an eighth of that rate. near: the rounding of a
+// rotation may decide, as a value stands within 2^-15 of the border of two numbers, or within 2^-14 of the step's size at its other
+// end (16.5), where it and not the step's might be the largest.
 __device__ __forceinline__ uint32_t numbers_q4(float4 v, float id, bool & near) {
     const float x[4] = { v.x, v.y, v.z, v.w };
+    float       top = 0.0f;
     uint32_t    n[4], low = 0x7fff;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        const float y = fminf(fmaxf(__fadd_rn(__fmul_rn(x[e], id), 8.5f), 0.0f), 15.75f);
-        n[e] = __float_as_uint(__fadd_rd(y, 256.0f));
+        const float y = __fadd_rn(__fmul_rn(x[e], id), 8.5f);
+        top  = fmaxf(top, y);
+        n[e] = __float_as_uint(__fadd_rd(fminf(fmaxf(y, 0.0f), 15.75f), 256.0f));
         low  = min(low, (n[e] + 1) & 0x7fffu);
     }
-    near |= low < 2;
+    near |= low < 2 || top > 16.5f - 0x1p-14f;
     return (n[0] >> 15 & 0xfu) | (n[1] >> 7 & 0xf00u) | (n[2] << 1 & 0xf0000u) | (n[3] << 9 & 0xf000000u);
 }
 // 4 of the 32 values of a q4_0 block: byte j holds number j in its low and number j + 16 in its high half
