@@ -39,6 +39,7 @@
 
 namespace srhpm {
 using namespace fap;
+using namespace q4;
 namespace {
 
 constexpr int      kTile   = 128;  // tokens of a tile and of a unit of work
@@ -47,16 +48,7 @@ constexpr int      kConv   = 8;    // unpacking warps: K's four, V's four
 constexpr int      kThr    = (kSm + 4 + kConv) * 32;
 constexpr int      kRawTok = 64;   // tokens of a raw stage
 constexpr int      kFlush  = 8;    // tiles
-constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s
 constexpr float    kUnset  = -3e38f;    // a row's reference before its first score
-
-struct Pool4 {
-    const uint8_t * p;
-    int64_t         nb1, nb2, nb3;
-};
-
-// bytes of a raw row's place: TMA's boxes start on 16 bytes, the row up to 12 later
-constexpr int row_stride(int D) { return D == 64 ? 48 : D == 128 ? 80 : 144; }
 
 template <int D, int N, bool PREC> struct LayT {
     static constexpr int parts = PREC ? 2 : 1;
@@ -99,11 +91,6 @@ template <int D, int N, bool PREC> struct LayT {
     static_assert(kSm * 32 * rs + 128 * rm + kConv * 32 * ru <= kThr * 72, "registers");
 };
 
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p != 0;
-}
 // A from tensor memory (K-major f16 pairs, lane = row)
 __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
     asm volatile(
@@ -112,11 +99,6 @@ __device__ __forceinline__ void mma_f16_ta(uint32_t d, uint32_t a, uint64_t b, u
         "r"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u)
         : "memory");
 }
-__device__ __forceinline__ float exp2a(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
 __device__ __forceinline__ void wait_bar(uint64_t * bar, uint32_t parity, int32_t * status, bool & bad) {
     if (bad) return;
     for (uint32_t i = 0; i < kProbes; i++) {
@@ -124,12 +106,6 @@ __device__ __forceinline__ void wait_bar(uint64_t * bar, uint32_t parity, int32_
     }
     bad = true;  // this thread waits for nothing more: its results are void, its accesses stay in bounds
     atomicExch(status, kErrWaitFull);
-}
-__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap * m, int x, int y, int z, uint64_t * bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
 }
 // true for all `count` threads of barrier `id` if one of them says so
 __device__ __forceinline__ bool bar_any(int id, int count, bool v) {
@@ -141,28 +117,6 @@ __device__ __forceinline__ bool bar_any(int id, int count, bool v) {
     return r != 0;
 }
 
-template <int W> __device__ __forceinline__ void ld_t(uint32_t t, uint32_t (&r)[W]) {
-    if constexpr (W == 32) {
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-            "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-              "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-              "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-            : "r"(t));
-    } else {
-        tc::ld_cols<W>(t, r);
-    }
-}
-template <int W> __device__ __forceinline__ void st_t(uint32_t t, const uint32_t (&r)[W]) {
-    if constexpr (W == 32) {
-        tc::st16(t, *reinterpret_cast<const uint32_t(*)[16]>(&r[0]));
-        tc::st16(t + 16, *reinterpret_cast<const uint32_t(*)[16]>(&r[16]));
-    } else {
-        tc::st_cols<W>(t, r);
-    }
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -359,7 +313,7 @@ __global__ void __launch_bounds__(kThr, 1)
             for (int mt = 0; mt < Ly::MT; mt++) {
                 uint32_t       o[CW];
                 const uint32_t at = tc::taddr(tb + Ly::tO + mt * Ly::NP + g0, wq, 0);
-                ld_t<CW>(at, o);
+                tc::ld_cols<CW>(at, o);
                 tc::wait_ld();
                 f(o, mt, at);
             }
@@ -413,7 +367,7 @@ __global__ void __launch_bounds__(kThr, 1)
                 const uint32_t ts = tc::taddr(tb + Ly::tS + sb * Ly::NP + g0, wq, 0);
                 uint32_t       s[CW];
                 auto           scores = [&]() {
-                    ld_t<CW>(ts, s);
+                    tc::ld_cols<CW>(ts, s);
                     tc::wait_ld();
                     if (a.softcap_l2 != 0.0f) {
 #pragma unroll
@@ -467,7 +421,7 @@ __global__ void __launch_bounds__(kThr, 1)
                         each_o([&](uint32_t (&o)[CW], int, uint32_t at) {
 #pragma unroll
                             for (int e = 0; e < CW; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac[e]);
-                            st_t<CW>(at, o);
+                            tc::st_cols<CW>(at, o);
                         });
                         tc::wait_st();
                     }

@@ -40,15 +40,8 @@
 
 namespace srhpm {
 using namespace fap;
+using namespace q4;
 namespace {
-
-struct Pool4 {
-    const uint8_t * p;
-    int64_t         nb1, nb2, nb3;
-};
-constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s
-
-constexpr int row_stride(int D) { return D == 64 ? 48 : D == 128 ? 80 : 144; }
 
 template <int D, bool PREC> struct LayF {
     static constexpr int BM    = 8;                    // rows of a tile
@@ -70,17 +63,6 @@ template <int D, bool PREC> struct LayF {
     static_assert(ST >= 2 && ring % 128 == 0 && ST * W * stage >= kMaxSeqs * 8, "shared memory");
 };
 
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p != 0;
-}
-__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap * m, int x, int y, int z, uint64_t * bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -89,11 +71,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-    return r;
-}
-__device__ __forceinline__ float exp2a(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 

@@ -222,10 +222,9 @@ struct SetArgs {
     int32_t *       status;
 };
 
-// visits the table entries of this cluster's rows, kForkChunk at a time per warp: f(pointer to the entry)
-// For each entry in range: p = take(entry), then r = look(p) for those that are pages, then use(entry, p, r). Each of the three
-// goes over a warp's 256 entries before the next, so that a round trip is waited for once and not eight times (48 of
-// 1024 sequences freed, 12000 pages: 19 us, now 15.6).
+// For each entry in range of this cluster's rows, kForkChunk at a time per warp: p = take(entry), then r = look(p) for those that
+// are pages, then use(entry, p, r). Each of the three goes over a warp's 256 entries before the next, so that a round trip is waited
+// for once and not eight times (48 of 1024 sequences freed, 12000 pages: 19 us, now 15.6).
 template <class Take, class Look, class Use>
 __device__ __forceinline__ void each_entry(const SetArgs & a, int rank, int ctas, Take take, Look look, Use use) {
     constexpr int K    = kForkChunk / 32;

@@ -4,9 +4,12 @@
 // values come as f16 pairs of bytes (0, 2) and (1, 3), low halves before high ones; whoever multiplies with them takes the other
 // operand in the same order.
 #pragma once
+#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include <cstdint>
+
+#include "ptx.cuh"
 
 namespace srhpm {
 namespace q4 {
@@ -65,6 +68,34 @@ template <int N> __device__ __forceinline__ void copy_async(uint32_t dst, const 
     } else {
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(size) : "memory");
     }
+}
+
+
+// ---- what both kernels of attention over q4_0 pages use ----
+struct Pool4 {
+    const uint8_t * p;
+    int64_t         nb1, nb2, nb3;  // token, KV head, page
+};
+constexpr uint32_t kProbes = 1u << 19;  // of a wait before it gives up: about 2 s
+
+// bytes of a raw row's place: TMA's boxes start on 16 bytes, the row up to 12 later
+constexpr int row_stride(int D) { return D == 64 ? 48 : D == 128 ? 80 : 144; }
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap * m, int x, int y, int z, uint64_t * bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ float exp2a(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 }  // namespace q4
