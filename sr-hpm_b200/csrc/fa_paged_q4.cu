@@ -9,7 +9,7 @@
 // a tile. Unpacking goes where it costs least: K's into tensor memory, whose writes take no shared memory bandwidth, V's into
 // the 128-byte swizzled rows that the product reads.
 //
-// Measured: 9 f32 rows over 131072 tokens, 24 / 4 heads of 256: 127 us, 54 of 64 rows used; a tile of 128 tokens takes 7300 cycles on
+// Measured: 9 f32 rows over 131072 tokens, 24 / 4 heads of 256: 123 us, 54 of 64 rows used; a tile of 128 tokens takes 7300 cycles on
 // its SM: the MMA warp waits for V 1400 (shared memory holds one tile of it) and issues P V for 2300, the softmax warps wait for
 // that 1900 and spend 1800 on O's way out and the rest. Tiles of 96 rows, 2048 rows over 32768 tokens: 6500 cycles, unpacking 2700 of
 // them, raw rows late by 1300 to 1900 (2.69 ms; with 128 rows a tile 2.75, with 8 softmax warps besides 2.96).

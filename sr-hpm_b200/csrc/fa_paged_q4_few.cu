@@ -14,7 +14,7 @@
 //                  f32 rows (PREC): Q and P as sums of two f16 parts; a step's part of O is summed up apart and then added, as
 //                  the tensor cores' sums are truncated (a shrink of 2^-25 per product, measured: 2e-5 after 400)
 //
-// Measured: 32 sequences of 500 to 8192 tokens decoding, 32 / 8 heads of 128: 70 us with the join, 2.5 TB/s: the schedulers issue in 63 %
+// Measured: 32 sequences of 500 to 8192 tokens decoding, 32 / 8 heads of 128: 69 us with the join, 2.6 TB/s: the schedulers issue in 63 %
 // of their cycles, 1150 instructions per step of 32 tokens, 560 of them unpacking. One row over 30000 tokens, 24 / 4 heads of 256: 30 us,
 // over 131000 68. One warp per 16 rows and whole CTAs on a part (tiles unpacked in shared memory) 91 us; heads that come to a token at
 // different times 91.

@@ -187,8 +187,9 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanArgs 
 // the first threads into shared memory while the row's loads are in flight. Bandwidth bound: a row is read once and
 // every output written once. A thread holds 4 pairs (two 16-byte loads); a row's loads go out before its angles. 8192 rows
 // of 32 + 2 * 8 heads of 128 into f16 pages: 49 us, 0.94 of the copy rate; 4001 rows of 24 + 2 * 4 of 256 into q8_0: 32.5,
-// 0.89; 9 rows 4.2 (the launch). q4_0 pages: 67 us, and 2048 rows of 24 + 2 * 4 of 256 31: the numbers take a third of the
-// instructions, and the rare rotation in 64 bits has registers of its own (in the loop 75 us, capped at 3 CTAs per SM by them).
+// 0.89; 9 rows 4.2 (the launch). q4_0 pages: 62 us, and 4001 rows of 24 + 2 * 4 of 256 41 (q8_0 34): the numbers take a third of the
+// instructions, 66 % of the issue slots are used, and half of the SM's threads wait at 64 registers with 52 bytes spilled. The rare
+// rotation in 64 bits has registers of its own (in the loop 8 us more, capped at 3 CTAs per SM by them).
 constexpr int kStoreThreads = 256;
 constexpr int kMaxHalf      = 128;
 

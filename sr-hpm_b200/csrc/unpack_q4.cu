@@ -1,7 +1,7 @@
 // The visible pages of prompts' sequences as f16, for attention over a q4_0 cache by the kernel of f16 caches (fa_paged.cu): the
 // rows of a long prompt fill so many tiles that each cached token would be unpacked tens of times over, while once takes the time of
 // the bytes (0.56 read and 2 written per value). 2048 rows over 32768 tokens, 24 / 4 heads of 256: 42 us (4.1 TB/s)
-// and 1.69 ms in all, unpacked tile by tile 2.69.
+// and 1.67 ms in all, unpacked tile by tile 2.69.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
